@@ -1,0 +1,676 @@
+// Attention of few query rows (single tokens, drafts) over a paged cache, for sm_100a.
+//
+// What bounds it: reading K and V once. A tile of 64 keys is 32 KB (head_dim 128) and needs 256 m16n8k16 products for
+// 16 query rows, a fifth of the time that the tile's bytes take at an SM's share of HBM, so the products run on
+// mma.sync from registers and the design is about keeping bytes in flight: one producer warp streams K and V tiles with
+// TMA (one box per page and 64 channels, 128-byte swizzle) through a ring of stages, two CTAs per SM.
+//
+// Rows: the heads of a group share K and V, so a row is (query, head of the group), query-major; 16 * kM rows a CTA.
+// The four consumer warps split rows by 16 and, where there are fewer than four such groups, split each tile's keys:
+// every warp runs its own online softmax (maximum, sum and output in FP32 registers) and meets the others only when a
+// sequence and head is finished.
+//
+// Work: all tiles of all (sequence, KV head, row tile) in one line, cut into equal shares, one per CTA, so ragged
+// batches and a single long sequence fill all SMs alike, and the host needs no lengths. A CTA whose share holds only a
+// part of an item leaves (output, maximum, sum) in FP32 in the workspace; a second kernel joins the parts in order of
+// the CTAs (no atomics: results do not depend on timing). It is launched as a programmatic dependent, so its launch
+// overlaps the first kernel.
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+
+#include <algorithm>
+#include <string>
+
+#include "attend.cuh"
+
+namespace rc {
+namespace paged {
+
+constexpr int kShortTile = 64;       // keys of a tile
+constexpr int kShortThreads = 160;   // four consumer warps, one producer warp
+constexpr int kShortCtasPerSm = 2;
+
+template <int D>
+struct ShortShape {
+  static constexpr int boxes = D / 64;
+  static constexpr int box_bytes = kShortTile * 128;            // 64 keys x 64 channels
+  static constexpr int tile_bytes = boxes * box_bytes;          // one of K, V
+  static constexpr int stages = D == 128 ? 3 : 6;
+  static constexpr int join_off = stages * 2 * tile_bytes;      // 16 rows x D of FP32: warps joining their keys
+  static constexpr int join_bytes = 16 * D * 4;
+  static constexpr int bar_off = join_off + join_bytes;
+  static constexpr int bytes = bar_off + 1024 + 1024;           // + alignment slack
+  static_assert((bytes + 1024) * kShortCtasPerSm <= 228 * 1024, "two CTAs per SM");
+};
+
+// The workspace's line of work, written by CTA 0 of the first kernel for the second.
+struct Line {
+  int* share;   // [1]
+  int* first;   // [seqs]: first place of each sequence's items in the line
+  int* tiles;   // [seqs]: tiles of each of its items
+};
+
+struct Short {
+  Args a;
+  Line line;
+  float* part_o;   // [2 * CTAs, 16 kM, D]
+  float* part_ml;  // [2 * CTAs, 16 kM, 2]
+  int rows;        // rows of a row tile: 16 kM
+  int row_tiles;   // row tiles of a sequence and KV head, at most
+};
+
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+// Items and tiles of one sequence.
+struct SeqWork {
+  int q_first, q_len, kv_len, row_tiles, tiles;
+  // most: row tiles that the caller's bound on the new tokens allows
+  __device__ __forceinline__ SeqWork(const Args& a, int rows, int most, int s) {
+    q_first = __ldg(a.cu_q + s);
+    q_len = min(__ldg(a.cu_q + s + 1), a.tokens) - q_first;
+    if (q_first < 0 || q_len < 0) q_len = 0;
+    kv_len = static_cast<int>(min(static_cast<int64_t>(max(0, __ldg(a.kv_lens + s))),
+                                  static_cast<int64_t>(a.width) * a.tiling.page));
+    row_tiles = static_cast<int>(min(static_cast<int64_t>(most), (static_cast<int64_t>(q_len) * a.group + rows - 1) / rows));
+    tiles = 0;
+    if (q_len > 0) tiles = max(1, TileRange(a.tiling, Sight(a, kv_len, q_len), 0, q_len).count());
+  }
+  __device__ __forceinline__ int items(const Args& a) const { return row_tiles * a.kv_heads; }
+};
+
+template <typename T, int D, int kM>
+__global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
+    short_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                 const __grid_constant__ Short p) {
+  using Shape = ShortShape<D>;
+  constexpr int kGroups = 4 / kM;               // warps that split a tile's keys
+  constexpr int kKeys = kShortTile / kGroups;   // keys of a warp
+  constexpr int kN = kKeys / 8;                 // its n-tiles of S
+  constexpr int kRows = 16 * kM;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + Shape::bar_off);
+  uint64_t* empty = full + Shape::stages;
+  float* join_ml = reinterpret_cast<float*>(empty + Shape::stages);  // [key groups][rows][maximum, sum]: 64 rows in all
+  int* work = reinterpret_cast<int*>(join_ml + 128);                 // begin, end, sequence, its first place
+  const Args& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < Shape::stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 4);
+    }
+    fence_barrier_init();
+  }
+  // The line of work: total, this CTA's share, and where it begins.
+  if (warp == 4) {
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  if (warp == 0) {
+    int total = 0;
+    for (int s0 = 0; s0 < a.seqs; s0 += 32) {
+      int n = 0;
+      if (s0 + lane < a.seqs) {
+        const SeqWork w(a, kRows, p.row_tiles, s0 + lane);
+        n = w.tiles * w.items(a);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+      total += n;
+    }
+    const int share = max(1, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
+    const int begin = min(total, static_cast<int>(blockIdx.x) * share), end = min(total, begin + share);
+    int base = 0;
+    for (int s0 = 0; s0 < a.seqs; s0 += 32) {
+      int n = 0, t = 0;
+      if (s0 + lane < a.seqs) {
+        const SeqWork w(a, kRows, p.row_tiles, s0 + lane);
+        t = w.tiles;
+        n = w.tiles * w.items(a);
+      }
+      int x = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      const int mine = base + x - n;
+      if (begin < end && begin >= mine && begin < mine + n) {
+        work[2] = s0 + lane;
+        work[3] = mine;
+      }
+      if (blockIdx.x == 0 && s0 + lane < a.seqs) {
+        p.line.first[s0 + lane] = mine;
+        p.line.tiles[s0 + lane] = t;
+      }
+      base += __shfl_sync(0xffffffffu, x, 31);
+    }
+    if (lane == 0) {
+      work[0] = begin;
+      work[1] = end;
+      if (blockIdx.x == 0) *p.line.share = share;
+    }
+  }
+  __syncthreads();
+  const int begin = work[0], end = work[1];
+  if (begin >= end) return;
+  int s = work[2], base = work[3];
+
+  int stage = 0;
+  uint32_t phase = 0;
+  if (warp == 4) {
+    // ---------------- producer ----------------
+    for (int at = begin; at < end;) {
+      const SeqWork w(a, kRows, p.row_tiles, s);
+      const int n = w.tiles * w.items(a);
+      if (at >= base + n) {
+        base += n;
+        ++s;
+        continue;
+      }
+      const int item = (at - base) / w.tiles, t0 = (at - base) - item * w.tiles;
+      const int t1 = min(w.tiles, t0 + end - at);
+      const int head = item / w.row_tiles;
+      const TileRange range(a.tiling, Sight(a, w.kv_len, w.q_len), 0, w.q_len);
+      for (int t = t0; t < t1; ++t) {
+        int block, row;
+        const int first = a.tiling.first(range.tile(t), &block, &row);
+        const int rest = w.kv_len - first;  // pages that hold a key of this tile
+        const int pages = rest <= 0 ? 0 : a.tiling.per_page > 1 ? 1 : min(a.tiling.per_tile, (rest + a.tiling.page - 1) / a.tiling.page);
+        if (!mbar_wait(&empty[stage], phase ^ 1, a.status, kTimeoutProducer)) return;
+        if (lane == 0) {
+          if (pages > 0) mbar_arrive_expect_tx(&full[stage], pages * a.tiling.box * 128 * Shape::boxes * 2);
+          else mbar_arrive(&full[stage]);
+        }
+        __syncwarp();
+        if (lane < pages) {
+          int page = __ldg(a.table + static_cast<int64_t>(s) * a.width + block + lane);
+          if (page < 0 || page >= a.pages) {
+            page = -1;
+            if (a.status != nullptr) atomicCAS(a.status + kPagedWord, 0, kPageRange);
+          }
+          uint8_t* k = smem + stage * 2 * Shape::tile_bytes + lane * a.tiling.page * 128;
+          uint8_t* v = k + Shape::tile_bytes;
+#pragma unroll
+          for (int b = 0; b < Shape::boxes; ++b)
+            load_page_box(k + b * Shape::box_bytes, &tmK, &full[stage], b * 64, row, head, page);
+#pragma unroll
+          for (int b = 0; b < Shape::boxes; ++b)
+            load_page_box(v + b * Shape::box_bytes, &tmV, &full[stage], b * 64, row, head, page);
+        }
+        if (++stage == Shape::stages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+      at += t1 - t0;
+    }
+    return;
+  }
+
+  // ---------------- consumers ----------------
+  const int mt = warp % kM, kg = warp / kM;  // row group, key group
+  const int r0 = lane >> 2, c0 = (lane & 3) * 2;
+  bool ok = true;
+  for (int at = begin; at < end;) {
+    const SeqWork w(a, kRows, p.row_tiles, s);
+    const int n = w.tiles * w.items(a);
+    if (at >= base + n) {
+      base += n;
+      ++s;
+      continue;
+    }
+    const int item = (at - base) / w.tiles, t0 = (at - base) - item * w.tiles;
+    const int t1 = min(w.tiles, t0 + end - at);
+    const int head = item / w.row_tiles, row_tile = item - head * w.row_tiles;
+    const Sight sight(a, w.kv_len, w.q_len);
+    const TileRange range(a.tiling, sight, 0, w.q_len);
+
+    // this thread's two rows
+    int row_q[2], row_h[2], last[2], low[2];
+    bool valid[2];
+    uint32_t q[D / 16][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = row_tile * kRows + mt * 16 + r0 + i * 8;
+      row_q[i] = row / a.group;
+      row_h[i] = head * a.group + row - row_q[i] * a.group;
+      valid[i] = row_q[i] < w.q_len;
+      last[i] = sight.last(min(row_q[i], w.q_len - 1));
+      low[i] = sight.low(last[i]);
+      const T* src = static_cast<const T*>(a.q) + static_cast<int64_t>(w.q_first + row_q[i]) * a.q_token + row_h[i] * a.q_head + c0;
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        q[k][i] = valid[i] ? __ldg(reinterpret_cast<const uint32_t*>(src + k * 16)) : 0u;
+        q[k][i + 2] = valid[i] ? __ldg(reinterpret_cast<const uint32_t*>(src + k * 16 + 8)) : 0u;
+      }
+    }
+    // bounds over the row tile's queries, for tiles that need no mask
+    const int q_first = row_tile * kRows / a.group;
+    const int q_last = min(w.q_len - 1, (row_tile * kRows + kRows - 1) / a.group);
+    const int all_last = sight.last(q_first), all_low = sight.low(sight.last(q_last));
+    const int any_low = sight.low(all_last);
+
+    float o[D / 8][4];
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+
+    for (int t = t0; t < t1; ++t) {
+      int block, page_row;
+      const int first = a.tiling.first(range.tile(t), &block, &page_row);
+      const int count = a.tiling.count(page_row);
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, a.status, kTimeoutEpilogue));
+      if (ok) {
+        const uint32_t kb = smem_u32(smem + stage * 2 * Shape::tile_bytes);
+        const uint32_t vb = kb + Shape::tile_bytes;
+        float sc[kN][4];
+#pragma unroll
+        for (int j = 0; j < kN; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[j][e] = 0.0f;
+        // S = Q K^T: matrices (keys 0-7, d 0-7), (keys 0-7, d 8-15), (keys 8-15, d 0-7), (keys 8-15, d 8-15)
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+#pragma unroll
+          for (int j = 0; j < kN / 2; ++j) {
+            const int key = kg * kKeys + j * 16 + (lane & 7) + ((lane >> 4) << 3);
+            const int chunk = (k & 3) * 2 + ((lane >> 3) & 1);
+            uint32_t b[4];
+            ldmatrix_x4(b, kb + (k >> 2) * Shape::box_bytes + key * 128 + ((chunk ^ (key & 7)) << 4));
+            mma_16816(sc[2 * j], q[k], b[0], b[1], T());
+            mma_16816(sc[2 * j + 1], q[k], b[2], b[3], T());
+          }
+        }
+        const bool whole = count == kShortTile && first + kShortTile - 1 <= all_last &&
+                           (first >= all_low || first + kShortTile <= a.sinks);
+        if (!whole) {
+#pragma unroll
+          for (int j = 0; j < kN; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int r = kg * kKeys + j * 8 + c0 + (e & 1);
+              const int at_key = first + r;
+              const int i = e >> 1;
+              if (!(r < count && at_key <= last[i] && at_key < w.kv_len && (at_key >= low[i] || at_key < a.sinks)))
+                sc[j][e] = -INFINITY;
+            }
+        }
+        float alpha[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float mx = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < kN; ++j) mx = fmaxf(mx, fmaxf(sc[j][2 * i], sc[j][2 * i + 1]));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          const float top = fmaxf(m[i], mx * a.scale_log2);
+          const float use = top == -INFINITY ? 0.0f : top;  // a row that has seen no key yet
+          alpha[i] = exp2_approx(m[i] - use);
+          m[i] = top;
+          float sum = 0.0f;
+#pragma unroll
+          for (int j = 0; j < kN; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float x = exp2_approx(fmaf(sc[j][2 * i + e], a.scale_log2, -use));
+              sc[j][2 * i + e] = x;
+              sum += x;
+            }
+          l[i] = l[i] * alpha[i] + sum;
+        }
+        if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            o[i][0] *= alpha[0];
+            o[i][1] *= alpha[0];
+            o[i][2] *= alpha[1];
+            o[i][3] *= alpha[1];
+          }
+        }
+        // O += P V: matrices (keys 0-7, d 0-7), (keys 8-15, d 0-7), (keys 0-7, d 8-15), (keys 8-15, d 8-15). Rows of V
+        // that no query sees (past the sequence, before the window, never loaded) are taken as zeros whatever they
+        // hold: 0 * NaN is NaN.
+#pragma unroll
+        for (int k = 0; k < kKeys / 16; ++k) {
+          const uint32_t pa[4] = {pack2<T>(sc[2 * k][0], sc[2 * k][1]), pack2<T>(sc[2 * k][2], sc[2 * k][3]),
+                                  pack2<T>(sc[2 * k + 1][0], sc[2 * k + 1][1]), pack2<T>(sc[2 * k + 1][2], sc[2 * k + 1][3])};
+          uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+          if (!whole) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              keep[h] = 0;
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int r = kg * kKeys + k * 16 + h * 8 + c0 + e;
+                if (r < count && first + r < w.kv_len && (first + r >= any_low || first + r < a.sinks)) keep[h] |= 0xffffu << (16 * e);
+              }
+            }
+          }
+#pragma unroll
+          for (int d = 0; d < D / 16; ++d) {
+            const int key = kg * kKeys + k * 16 + (lane & 7) + (((lane >> 3) & 1) << 3);
+            const int chunk = (d & 3) * 2 + (lane >> 4);
+            uint32_t b[4];
+            ldmatrix_x4_trans(b, vb + (d >> 2) * Shape::box_bytes + key * 128 + ((chunk ^ (key & 7)) << 4));
+            mma_16816(o[2 * d], pa, b[0] & keep[0], b[1] & keep[1], T());
+            mma_16816(o[2 * d + 1], pa, b[2] & keep[0], b[3] & keep[1], T());
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[stage]);
+      }
+      if (++stage == Shape::stages) {
+        stage = 0;
+        phase ^= 1;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+    }
+    // Warps that split the keys join theirs into key group 0, one after the other through shared memory. The same lane
+    // of every warp holds the same rows and columns, so the buffer is laid out by lane.
+    if (kGroups > 1) {
+      if ((lane & 3) == 0) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          join_ml[(kg * kRows + mt * 16 + r0 + 8 * i) * 2] = m[i];
+          join_ml[(kg * kRows + mt * 16 + r0 + 8 * i) * 2 + 1] = l[i];
+        }
+      }
+      consumers_sync();
+      float w_o[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float top = -INFINITY, total = 0.0f;
+        float gm[kGroups];
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+          gm[g] = join_ml[(g * kRows + mt * 16 + r0 + 8 * i) * 2];
+          top = fmaxf(top, gm[g]);
+        }
+        const float use = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g)
+          total = fmaf(join_ml[(g * kRows + mt * 16 + r0 + 8 * i) * 2 + 1], exp2_approx(gm[g] - use), total);
+        w_o[i] = exp2_approx(m[i] - use);
+        m[i] = top;
+        l[i] = total;
+      }
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        o[i][0] *= w_o[0];
+        o[i][1] *= w_o[0];
+        o[i][2] *= w_o[1];
+        o[i][3] *= w_o[1];
+      }
+      constexpr int kBlock = D / 8 / kM;  // n-tiles that fit at a time
+      float4* buf = reinterpret_cast<float4*>(smem + Shape::join_off) + mt * kBlock * 32 + lane;
+#pragma unroll
+      for (int g = 1; g < kGroups; ++g) {
+#pragma unroll
+        for (int c = 0; c < kM; ++c) {
+          if (kg == g) {
+#pragma unroll
+            for (int i = 0; i < kBlock; ++i) {
+              const float(&x)[4] = o[c * kBlock + i];
+              buf[i * 32] = make_float4(x[0], x[1], x[2], x[3]);
+            }
+          }
+          consumers_sync();
+          if (kg == 0) {
+#pragma unroll
+            for (int i = 0; i < kBlock; ++i) {
+              const float4 x = buf[i * 32];
+              float(&y)[4] = o[c * kBlock + i];
+              y[0] += x.x;
+              y[1] += x.y;
+              y[2] += x.z;
+              y[3] += x.w;
+            }
+          }
+          consumers_sync();
+        }
+      }
+    }
+    if (kg == 0 && ok) {
+      const int item_first = base + item * w.tiles;
+      const bool starts = item_first >= begin, ends = item_first + w.tiles <= end;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (!valid[i]) continue;
+        const int64_t token = w.q_first + row_q[i];
+        if (starts && ends) {
+          const float inv = l[i] > 0.0f ? 1.0f / l[i] : 0.0f;
+          T* dst = static_cast<T*>(a.out) + token * a.out_token + row_h[i] * a.out_head + c0;
+#pragma unroll
+          for (int d = 0; d < D / 8; ++d)
+            *reinterpret_cast<uint32_t*>(dst + d * 8) = pack2<T>(o[d][2 * i] * inv, o[d][2 * i + 1] * inv);
+          if (a.lse != nullptr && (lane & 3) == 0)
+            a.lse[token * a.heads + row_h[i]] = l[i] > 0.0f ? (m[i] + log2f(l[i])) * kLn2 : -INFINITY;
+        } else {
+          const int64_t slot = (2 * static_cast<int64_t>(blockIdx.x) + (starts ? 1 : 0)) * kRows + mt * 16 + r0 + 8 * i;
+          float* dst = p.part_o + slot * D + c0;
+#pragma unroll
+          for (int d = 0; d < D / 8; ++d) *reinterpret_cast<float2*>(dst + d * 8) = make_float2(o[d][2 * i], o[d][2 * i + 1]);
+          if ((lane & 3) == 0) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(m[i], l[i]);
+        }
+      }
+    }
+    at += t1 - t0;
+  }
+}
+
+// Joins the parts of items that more than one CTA worked on. One warp per row; the parts are those of the CTAs whose
+// shares the item's tiles lie in, in order.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) short_join_kernel(const __grid_constant__ Short p) {
+  constexpr int kPer = D / 32;
+  const Args& a = p.a;
+  const int lane = threadIdx.x & 31;
+  const int quads = p.rows / 4;
+  const int row = (blockIdx.x % quads) * 4 + (threadIdx.x >> 5);
+  int item = blockIdx.x / quads;
+  const int s = item / (gridDim.x / quads / a.seqs);
+  item -= s * (gridDim.x / quads / a.seqs);
+  const SeqWork w(a, p.rows, p.row_tiles, s);  // the call's inputs: they do not wait for the first kernel
+  // every block waits, so that this kernel never ends before the first one does
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (item >= w.items(a)) return;
+  const int head = item / w.row_tiles, row_tile = item - head * w.row_tiles;
+  const int packed = row_tile * p.rows + row;
+  const int query = packed / a.group;
+  if (query >= w.q_len) return;
+  const int share = *p.line.share;
+  const int begin = p.line.first[s] + item * w.tiles, end = begin + w.tiles;
+  const int c0 = begin / share, c1 = (end - 1) / share;
+  if (c0 == c1) return;
+  float top = -INFINITY;
+  for (int c = c0; c <= c1; ++c) top = fmaxf(top, p.part_ml[((2 * static_cast<int64_t>(c) + (c == c0)) * p.rows + row) * 2]);
+  const float use = top == -INFINITY ? 0.0f : top;
+  float acc[kPer], sum = 0.0f;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) acc[e] = 0.0f;
+#pragma unroll 4
+  for (int c = c0; c <= c1; ++c) {
+    const int64_t slot = (2 * static_cast<int64_t>(c) + (c == c0)) * p.rows + row;
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot * 2);
+    const float wt = exp2_approx(ml.x - use);
+    sum = fmaf(wt, ml.y, sum);
+#pragma unroll
+    for (int e = 0; e < kPer; e += 2) {
+      const float2 x = *reinterpret_cast<const float2*>(p.part_o + slot * D + lane * kPer + e);
+      acc[e] = fmaf(wt, x.x, acc[e]);
+      acc[e + 1] = fmaf(wt, x.y, acc[e + 1]);
+    }
+  }
+  const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+  const int64_t token = w.q_first + query;
+  const int h = head * a.group + packed - query * a.group;
+  T* dst = static_cast<T*>(a.out) + token * a.out_token + h * a.out_head + lane * kPer;
+#pragma unroll
+  for (int e = 0; e < kPer; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack2<T>(acc[e] * inv, acc[e + 1] * inv);
+  if (a.lse != nullptr && lane == 0) a.lse[token * a.heads + h] = sum > 0.0f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+}
+
+template <typename T, int D, int kM>
+void short_launch(Args a, const at::Tensor& k_pages, const at::Tensor& v_pages, int max_q_len, const at::Tensor& like,
+                  cudaStream_t stream, int device) {
+  using Shape = ShortShape<D>;
+  static bool configured = false;
+  if (!configured) {
+    RC_CUDA(cudaFuncSetAttribute(short_kernel<T, D, kM>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::bytes));
+    configured = true;
+  }
+  constexpr int kRows = 16 * kM;
+  Short p{};
+  p.a = a;
+  p.rows = kRows;
+  p.a.tiling = Tiling::of(a.tiling.page, kShortTile);
+  const int64_t row_tiles = (static_cast<int64_t>(max_q_len) * a.group + kRows - 1) / kRows;
+  p.row_tiles = static_cast<int>(row_tiles);
+  const int64_t items = row_tiles * a.kv_heads;  // of one sequence, at most
+  const int64_t most_tiles = static_cast<int64_t>(a.seqs) * items * ((static_cast<int64_t>(a.width) * a.tiling.page + 7) / 8 + 2);
+  const int ctas = static_cast<int>(std::min<int64_t>(sm_count(device) * kShortCtasPerSm, most_tiles));
+  RC_CHECK(a.seqs * items * (kRows / 4) < (1ll << 31), "too many sequences and rows for one launch");
+  const int64_t floats = 2ll * ctas * kRows * (D + 2), ints = 1 + 2ll * a.seqs;
+  at::Tensor workspace = at::empty({floats + ints}, like.options().dtype(at::kFloat));
+  p.part_o = workspace.data_ptr<float>();
+  p.part_ml = p.part_o + 2ll * ctas * kRows * D;
+  int* line = reinterpret_cast<int*>(p.part_o + floats);
+  p.line = {line, line + 1, line + 1 + a.seqs};
+  const CUtensorMap tmK = page_map(k_pages, p.a.tiling.box), tmV = page_map(v_pages, p.a.tiling.box);
+  short_kernel<T, D, kM><<<ctas, kShortThreads, Shape::bytes, stream>>>(tmK, tmV, p);
+  RC_CUDA(cudaGetLastError());
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(a.seqs * items * (kRows / 4)));
+  config.blockDim = dim3(128);
+  config.stream = stream;
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  RC_CUDA(cudaLaunchKernelEx(&config, short_join_kernel<T, D>, p));
+}
+
+template <typename T, int D>
+void short_rows(const Args& a, const at::Tensor& k_pages, const at::Tensor& v_pages, int max_q_len, const at::Tensor& like,
+                cudaStream_t stream, int device) {
+  const int64_t rows = static_cast<int64_t>(max_q_len) * a.group;
+  if (rows <= 16) short_launch<T, D, 1>(a, k_pages, v_pages, max_q_len, like, stream, device);
+  else if (rows <= 32) short_launch<T, D, 2>(a, k_pages, v_pages, max_q_len, like, stream, device);
+  else short_launch<T, D, 4>(a, k_pages, v_pages, max_q_len, like, stream, device);
+}
+
+void attend_short(const Args& a, int head_dim, bool half, const at::Tensor& k_pages, const at::Tensor& v_pages,
+                  int max_q_len, const at::Tensor& like, cudaStream_t stream, int device) {
+  if (head_dim == 128)
+    half ? short_rows<__half, 128>(a, k_pages, v_pages, max_q_len, like, stream, device)
+         : short_rows<__nv_bfloat16, 128>(a, k_pages, v_pages, max_q_len, like, stream, device);
+  else
+    half ? short_rows<__half, 64>(a, k_pages, v_pages, max_q_len, like, stream, device)
+         : short_rows<__nv_bfloat16, 64>(a, k_pages, v_pages, max_q_len, like, stream, device);
+}
+
+}  // namespace paged
+
+// out = softmax over the visible keys of scale * q k^T, times v, for the new tokens of every sequence; lse its natural
+// log-sum-exp. max_q_len bounds every sequence's new tokens; tokens past a sequence's bound are left alone.
+void paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
+                     const at::Tensor& kv_lens, const at::Tensor& cu_q, at::Tensor& out,
+                     const c10::optional<at::Tensor>& lse, int64_t max_q_len, bool causal, int64_t window, int64_t sinks,
+                     double scale, const c10::optional<at::Tensor>& status) {
+  check_cuda_tensor(q, "q");
+  const at::ScalarType type = q.scalar_type();
+  RC_CHECK(type == at::kBFloat16 || type == at::kHalf, "paged attention takes bf16 or fp16");
+  RC_CHECK(q.dim() == 3 && (q.size(2) == 64 || q.size(2) == 128), "q must be [tokens, heads, head_dim] with head_dim 64 or 128");
+  RC_CHECK(q.size(0) < (1ll << 31), "too many tokens for one launch");
+  RC_CHECK(out.sizes() == q.sizes() && out.scalar_type() == type && out.device() == q.device(), "out must match q");
+  const at::Tensor* rows[2] = {&q, &out};
+  for (const at::Tensor* t : rows)
+    RC_CHECK(t->numel() == 0 || (t->stride(2) == 1 && t->stride(0) % 8 == 0 && t->stride(1) % 8 == 0 &&
+                                 reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0),
+             "rows must have unit inner stride and 16-byte aligned strides and base");
+  RC_CHECK(k_pages.device() == q.device() && v_pages.device() == q.device() && k_pages.scalar_type() == type &&
+               v_pages.scalar_type() == type && k_pages.dim() == 4,
+           "the pages must have the type and device of q");
+  const int64_t kv_heads = k_pages.size(2);
+  RC_CHECK(kv_heads >= 1 && q.size(1) % kv_heads == 0 && q.size(1) >= kv_heads, "heads must be a multiple of the KV heads");
+  const paged::Pages kp = paged::check_pages(k_pages, kv_heads, q.size(2), "k_pages");
+  const paged::Pages vp = paged::check_pages(v_pages, kv_heads, q.size(2), "v_pages");
+  RC_CHECK(kp.count == vp.count && kp.size == vp.size, "k_pages and v_pages must have the same pages");
+  const paged::Table t = paged::check_table(table, kv_lens, cu_q, q.device());
+  RC_CHECK(window >= 0 && sinks >= 0 && window < (1ll << 31) && sinks < (1ll << 31), "window and sinks must not be negative");
+  RC_CHECK(max_q_len >= 1 && max_q_len < (1ll << 24), "max_q_len must be positive");
+  paged::Args a{};
+  a.q = q.data_ptr();
+  a.q_token = q.stride(0);
+  a.q_head = q.stride(1);
+  a.out = out.data_ptr();
+  a.out_token = out.stride(0);
+  a.out_head = out.stride(1);
+  if (lse.has_value()) {
+    RC_CHECK(lse->scalar_type() == at::kFloat && lse->is_contiguous() && lse->device() == q.device() && lse->dim() == 2 &&
+                 lse->size(0) == q.size(0) && lse->size(1) == q.size(1),
+             "lse must be a contiguous float32 [tokens, heads]");
+    a.lse = lse->data_ptr<float>();
+  }
+  a.table = t.table;
+  a.kv_lens = t.kv_lens;
+  a.cu_q = t.cu_q;
+  a.seqs = t.seqs;
+  a.width = t.width;
+  a.pages = kp.count;
+  a.heads = static_cast<int>(q.size(1));
+  a.kv_heads = static_cast<int>(kv_heads);
+  a.group = a.heads / a.kv_heads;
+  a.causal = causal;
+  a.window = static_cast<int>(window);
+  a.sinks = window > 0 ? static_cast<int>(sinks) : 0;
+  a.tokens = static_cast<int>(q.size(0));
+  a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+  a.tiling.page = kp.size;
+  a.status = status_ptr(status);
+  if (a.tokens == 0 || a.seqs == 0) return;
+  c10::cuda::CUDAGuard guard(q.device());
+  const int device = q.get_device();
+  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device).stream();
+  paged::attend_short(a, static_cast<int>(q.size(2)), type == at::kHalf, k_pages, v_pages,
+                      static_cast<int>(std::min<int64_t>(max_q_len, a.tokens)), q, stream, device);
+}
+
+}  // namespace rc

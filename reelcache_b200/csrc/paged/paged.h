@@ -1,0 +1,59 @@
+// What the paged-cache kernels share: the checked views of pages and block tables, and their status codes.
+#pragma once
+
+#include <ATen/ATen.h>
+
+#include "../common/host.h"
+
+namespace rc {
+
+// The paged kernels report into the second word of the device's status words: a table entry that is out of range, or a
+// page-table call that was refused, leaves everything in bounds and consistent, so it must not stop the waits of later
+// kernels, which watch the first word.
+constexpr int kPagedWord = 1;
+constexpr int kPageExhausted = 0x401;
+constexpr int kPageRefused = 0x402;
+constexpr int kPageRange = 0x403;
+
+namespace paged {
+
+struct Pages {  // [pages, page_size, kv_heads, head_dim], strides in elements
+  int count, size;
+  int64_t page_stride, token_stride, head_stride;
+};
+
+struct Table {
+  const int* table;    // [seqs, width]
+  const int* kv_lens;  // [seqs]
+  const int* cu_q;     // [seqs + 1]
+  int seqs, width;
+};
+
+inline Pages check_pages(const at::Tensor& t, int64_t heads, int64_t head_dim, const char* name) {
+  const std::string who(name);
+  RC_CHECK(t.dim() == 4 && t.size(2) == heads && t.size(3) == head_dim && t.stride(3) == 1,
+           who + " must be [pages, page_size, kv_heads, head_dim] with unit inner stride");
+  RC_CHECK(t.size(0) >= 1 && t.size(0) < (1ll << 31) && t.size(1) >= 8 && t.size(1) % 8 == 0 && t.size(1) <= 65536,
+           who + ": the page size must be a multiple of 8 tokens, at most 65536");
+  RC_CHECK(t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && t.stride(2) % 8 == 0 &&
+               reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
+           who + " must have 16-byte aligned strides and base");
+  return {static_cast<int>(t.size(0)), static_cast<int>(t.size(1)), t.stride(0), t.stride(1), t.stride(2)};
+}
+
+inline Table check_table(const at::Tensor& table, const at::Tensor& kv_lens, const at::Tensor& cu_q,
+                         const at::Device& device) {
+  const at::Tensor* all[3] = {&table, &kv_lens, &cu_q};
+  for (const at::Tensor* t : all)
+    RC_CHECK(t->device() == device && t->scalar_type() == at::kInt && t->is_contiguous(),
+             "block_table, kv_lens and cu_q must be contiguous int32 tensors on the device of q");
+  RC_CHECK(table.dim() == 2 && kv_lens.dim() == 1 && cu_q.dim() == 1 && kv_lens.size(0) == table.size(0) &&
+               cu_q.size(0) == table.size(0) + 1,
+           "block_table is [seqs, width], kv_lens [seqs], cu_q [seqs + 1]");
+  RC_CHECK(table.size(0) < (1 << 20) && table.size(1) < (1ll << 31), "too many sequences or pages per sequence");
+  return {table.data_ptr<int>(), kv_lens.data_ptr<int>(), cu_q.data_ptr<int>(), static_cast<int>(table.size(0)),
+          static_cast<int>(table.size(1))};
+}
+
+}  // namespace paged
+}  // namespace rc

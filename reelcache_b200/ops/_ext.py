@@ -26,6 +26,9 @@ STATUS_NAMES = {
     0x105: "drain wait timed out",
     0x201: "peer flag wait timed out",
     0x301: "bad kernel argument",
+    0x401: "too few free pages: the page-table call was refused and changed nothing",
+    0x402: "a sequence or length of a page-table call is invalid: the call was refused and changed nothing",
+    0x403: "a page number lies outside the pool: its keys read as zeros, writes to it were dropped",
 }
 
 
@@ -60,7 +63,8 @@ def status_word(device) -> torch.Tensor:
 def check_status(device) -> None:
     """Raise DeviceStatusError if any kernel on ``device`` recorded a failure (synchronizes)."""
     word = status_word(device)
-    code = int(word[0].item())
+    first, paged = word[:2].tolist()  # the second word is the paged-cache operators'
+    code = first or paged
     if code:
         word.zero_()
         raise DeviceStatusError(f"kernel status 0x{code:x}: {STATUS_NAMES.get(code, 'unknown failure')}")
