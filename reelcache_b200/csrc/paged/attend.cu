@@ -1,0 +1,92 @@
+// Entry point of attention over a paged KV cache: checks, and the choice between the two kernels.
+//
+// Few query rows (new tokens x heads of a group) cannot fill the 128-row products of tcgen05, and reading K and V bounds
+// them anyway: they take the streaming kernel of attend_short.cu. More rows take attend_chunk.cu.
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+
+#include <algorithm>
+
+#include "attend.cuh"
+
+namespace rc {
+namespace paged {
+
+constexpr int kShortRows = 64;
+
+void attend_short(const Args& a, int head_dim, bool half, const at::Tensor& k_pages, const at::Tensor& v_pages,
+                  int max_q_len, const at::Tensor& like, cudaStream_t stream, int device);
+void attend_chunk(const Args& a, int head_dim, bool half, const at::Tensor& k_pages, const at::Tensor& v_pages,
+                  int max_q_len, const at::Tensor& like, cudaStream_t stream, int device);
+
+}  // namespace paged
+
+// out = softmax over the visible keys of scale * q k^T, times v, for the new tokens of every sequence; lse its natural
+// log-sum-exp. max_q_len bounds every sequence's new tokens; tokens past a sequence's bound are left alone.
+void paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
+                     const at::Tensor& kv_lens, const at::Tensor& cu_q, at::Tensor& out,
+                     const c10::optional<at::Tensor>& lse, int64_t max_q_len, bool causal, int64_t window, int64_t sinks,
+                     double scale, const c10::optional<at::Tensor>& status) {
+  check_cuda_tensor(q, "q");
+  const at::ScalarType type = q.scalar_type();
+  RC_CHECK(type == at::kBFloat16 || type == at::kHalf, "paged attention takes bf16 or fp16");
+  RC_CHECK(q.dim() == 3 && (q.size(2) == 64 || q.size(2) == 128), "q must be [tokens, heads, head_dim] with head_dim 64 or 128");
+  RC_CHECK(q.size(0) < (1ll << 31), "too many tokens for one launch");
+  RC_CHECK(out.sizes() == q.sizes() && out.scalar_type() == type && out.device() == q.device(), "out must match q");
+  const at::Tensor* rows[2] = {&q, &out};
+  for (const at::Tensor* t : rows)
+    RC_CHECK(t->numel() == 0 || (t->stride(2) == 1 && t->stride(0) % 8 == 0 && t->stride(1) % 8 == 0 &&
+                                 reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0),
+             "rows must have unit inner stride and 16-byte aligned strides and base");
+  RC_CHECK(k_pages.device() == q.device() && v_pages.device() == q.device() && k_pages.scalar_type() == type &&
+               v_pages.scalar_type() == type && k_pages.dim() == 4,
+           "the pages must have the type and device of q");
+  const int64_t kv_heads = k_pages.size(2);
+  RC_CHECK(kv_heads >= 1 && q.size(1) % kv_heads == 0 && q.size(1) >= kv_heads, "heads must be a multiple of the KV heads");
+  const paged::Pages kp = paged::check_pages(k_pages, kv_heads, q.size(2), "k_pages");
+  const paged::Pages vp = paged::check_pages(v_pages, kv_heads, q.size(2), "v_pages");
+  RC_CHECK(kp.count == vp.count && kp.size == vp.size, "k_pages and v_pages must have the same pages");
+  const paged::Table t = paged::check_table(table, kv_lens, cu_q, q.device());
+  RC_CHECK(window >= 0 && sinks >= 0 && window < (1ll << 31) && sinks < (1ll << 31), "window and sinks must not be negative");
+  RC_CHECK(scale > 0.0, "scale must be positive");
+  RC_CHECK(max_q_len >= 1 && max_q_len < (1ll << 24), "max_q_len must be positive");
+  paged::Args a{};
+  a.q = q.data_ptr();
+  a.q_token = q.stride(0);
+  a.q_head = q.stride(1);
+  a.out = out.data_ptr();
+  a.out_token = out.stride(0);
+  a.out_head = out.stride(1);
+  if (lse.has_value()) {
+    RC_CHECK(lse->scalar_type() == at::kFloat && lse->is_contiguous() && lse->device() == q.device() && lse->dim() == 2 &&
+                 lse->size(0) == q.size(0) && lse->size(1) == q.size(1),
+             "lse must be a contiguous float32 [tokens, heads]");
+    a.lse = lse->data_ptr<float>();
+  }
+  a.table = t.table;
+  a.kv_lens = t.kv_lens;
+  a.cu_q = t.cu_q;
+  a.seqs = t.seqs;
+  a.width = t.width;
+  a.pages = kp.count;
+  a.heads = static_cast<int>(q.size(1));
+  a.kv_heads = static_cast<int>(kv_heads);
+  a.group = a.heads / a.kv_heads;
+  a.causal = causal;
+  a.window = static_cast<int>(window);
+  a.sinks = window > 0 ? static_cast<int>(sinks) : 0;
+  a.tokens = static_cast<int>(q.size(0));
+  a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+  a.tiling.page = kp.size;
+  a.status = status_ptr(status);
+  if (a.tokens == 0 || a.seqs == 0) return;
+  c10::cuda::CUDAGuard guard(q.device());
+  const int device = q.get_device();
+  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device).stream();
+  const int most = static_cast<int>(std::min<int64_t>(max_q_len, a.tokens));
+  const auto attend = static_cast<int64_t>(most) * a.group <= paged::kShortRows ? paged::attend_short : paged::attend_chunk;
+  attend(a, static_cast<int>(q.size(2)), type == at::kHalf, k_pages, v_pages, most, q, stream, device);
+}
+
+}  // namespace rc

@@ -13,51 +13,17 @@ namespace paged {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// A tile holds consecutive positions of one sequence, at most `rows` of them, in at most one TMA box per page. Pages
-// smaller than a tile: `per_tile` whole pages (page size a multiple of 8, so each lands on a swizzle atom). Larger
-// pages: `per_page` boxes of `box` rows each; the last box of a page may reach past its end, where TMA fills zeros.
+// Tile t holds the positions [t * rows, (t + 1) * rows) of a sequence. Where they lie in one page, one TMA box of `rows`
+// token rows (and 64 channels) fetches them; else boxes of `step` rows do, the largest power of two that divides the page
+// size (a multiple of 8, so each box starts on a swizzle atom), which never cross a page's end.
 struct Tiling {
-  int page;      // page size
-  int box;       // rows of one TMA box
-  int per_page;  // tiles of one page (1 where pages are smaller than a tile)
-  int per_tile;  // pages of one tile (1 where tiles are smaller than a page)
+  int page;  // page size
+  int step;  // rows of a narrow box
 
   static Tiling of(int page, int rows) {
-    Tiling t{page, page, 1, 1};
-    if (page > rows) {
-      t.per_page = (page + rows - 1) / rows;
-      t.box = ((page + t.per_page - 1) / t.per_page + 7) / 8 * 8;
-      t.per_page = (page + t.box - 1) / t.box;
-    } else {
-      t.per_tile = rows / page;
-    }
-    return t;
+    const int two = page & -page;
+    return {page, two < rows ? two : rows};
   }
-
-  __device__ __forceinline__ int tile_of(int position) const {
-    if (per_page > 1) {
-      const int p = position / page;
-      return p * per_page + (position - p * page) / box;
-    }
-    return position / (page * per_tile);
-  }
-  // first position of a tile, its first page's block in the table, its first row in that page
-  __device__ __forceinline__ int first(int tile, int* block, int* row) const {
-    if (per_page > 1) {
-      *block = tile / per_page;
-      *row = (tile - *block * per_page) * box;
-      return *block * page + *row;
-    }
-    *block = tile * per_tile;
-    *row = 0;
-    return *block * page;
-  }
-  __device__ __forceinline__ int first(int tile) const {
-    int block, row;
-    return first(tile, &block, &row);
-  }
-  // positions of a tile that exist in its pages
-  __device__ __forceinline__ int count(int row) const { return per_page > 1 ? min(box, page - row) : page * per_tile; }
 };
 
 struct Args {
@@ -92,21 +58,52 @@ struct Sight {
 };
 
 // The tiles that the queries [first, end) of a sequence visit: [0, sink_end) and [window_begin, window_end).
+template <int kTile>
 struct TileRange {
   int sink_end, window_begin, window_end;
-  __device__ __forceinline__ TileRange(const Tiling& t, const Sight& s, int first, int end) {
+  __device__ __forceinline__ TileRange(const Sight& s, int first, int end) {
     const int top = s.last(end - 1);
     if (top < 0) {  // no query sees a key
       sink_end = window_begin = window_end = 0;
       return;
     }
     const int low = min(s.low(s.last(first)), top);
-    window_begin = t.tile_of(low);
-    window_end = t.tile_of(top) + 1;
-    sink_end = s.sinks > 0 ? min(window_begin, t.tile_of(min(s.sinks - 1, top)) + 1) : 0;
+    window_begin = low / kTile;
+    window_end = top / kTile + 1;
+    sink_end = s.sinks > 0 ? min(window_begin, min(s.sinks - 1, top) / kTile + 1) : 0;
   }
   __device__ __forceinline__ int count() const { return sink_end + window_end - window_begin; }
   __device__ __forceinline__ int tile(int i) const { return i < sink_end ? i : window_begin + i - sink_end; }
+};
+
+// The boxes that fetch one tile's rows of K or V: `count` of them (one per lane), `rows` rows each. Positions past the
+// sequence's end are not fetched (but for the rest of a box).
+template <int kTile>
+struct Boxes {
+  int count, rows;
+  __device__ __forceinline__ Boxes(const Tiling& t, int first, int kv_len) {
+    const int there = min(kTile, kv_len - first);
+    if (there <= 0) {
+      count = rows = 0;
+    } else if (t.step == kTile || first % t.page + kTile <= t.page) {
+      count = 1;
+      rows = kTile;
+    } else {
+      rows = t.step;
+      count = (there + rows - 1) / rows;
+    }
+  }
+  // page and row in it of the box that `lane` fetches; a page outside the pool comes out as -1 (it reads as zeros)
+  __device__ __forceinline__ int page(const int* table, int pages, const Tiling& t, int first, int lane, int* row, int* status) const {
+    const int at = first + lane * rows, block = at / t.page;
+    *row = at - block * t.page;
+    int page = __ldg(table + block);
+    if (page < 0 || page >= pages) {
+      page = -1;
+      if (status != nullptr) atomicCAS(status + kPagedWord, 0, kPageRange);
+    }
+    return page;
+  }
 };
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -148,6 +145,33 @@ inline CUtensorMap page_map(const at::Tensor& t, int box) {
       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   RC_CHECK(res == CUDA_SUCCESS, "cuTensorMapEncodeTiled (pages) failed (code " + std::to_string(static_cast<int>(res)) + ")");
   return map;
+}
+
+struct PageMaps {
+  CUtensorMap k_wide, v_wide, k_step, v_step;
+};
+
+inline PageMaps page_maps(const at::Tensor& k, const at::Tensor& v, const Tiling& t, int rows) {
+  PageMaps maps;
+  // a box may not be larger than the page it is cut from: without whole tiles in a page the wide maps are not used
+  const bool wide = t.page >= rows, step = t.step < rows;
+  if (wide) {
+    maps.k_wide = page_map(k, rows);
+    maps.v_wide = page_map(v, rows);
+  }
+  if (step) {
+    maps.k_step = page_map(k, t.step);
+    maps.v_step = page_map(v, t.step);
+  }
+  if (!wide) {
+    maps.k_wide = maps.k_step;
+    maps.v_wide = maps.v_step;
+  }
+  if (!step) {
+    maps.k_step = maps.k_wide;
+    maps.v_step = maps.v_wide;
+  }
+  return maps;
 }
 
 }  // namespace paged

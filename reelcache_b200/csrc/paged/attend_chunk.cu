@@ -1,0 +1,831 @@
+// Attention of many query rows (chunks, prompts) over a paged cache on tcgen05, for sm_100a: out = softmax(scale Q K^T) V
+// with Q, K, V in bf16 or fp16, head_dim 64 or 128, scores, statistics and outputs accumulated in FP32.
+//
+// What bounds it: the tensor core and the exponentials. A tile of 128 rows x 128 keys (head_dim 128) is 8.4 MFLOP, 1,024
+// cycles of an SM's tcgen05 rate, and 16,384 exponentials, 1,024 cycles of its 16 a cycle. So the two have to run at the
+// same time, and a part of the exponentials goes to the FMA pipe.
+//
+// A CTA works on 256 rows as two tiles of 128 that share every K and V block. Rows are (query, head of the group),
+// query-major, so grouped heads share the loads of their KV head. 384 threads:
+//   warps 0-3, 4-7  softmax of tile 0, 1: a thread owns a row (TMEM lane). S comes from TMEM, the running maximum moves
+//                   only when it grows by more than 8 (log2; then the row of O is rescaled in TMEM), P goes back to TMEM
+//                   over S, where the P V product reads it as its A operand. The tiles take turns on the exponentials.
+//   warps 8, 9      TMA: K blocks into a ring of 3, V blocks into a ring of 2. One box per page (or part of it).
+//   warp 10         issues the products, in the order O_0 += P_0 V', S_0 = Q_0 K, O_1 += P_1 V', S_1 = Q_1 K (V' of the
+//                   block before), without a break between one item and the next.
+//   warp 11         gathers the rows of Q with cp.async into the swizzled layout (any group size and strides).
+// V is read as it lies in the pages (keys x channels: an MN-major B operand), no transposed copy exists.
+// TMEM: S_g at column 128 g (P_g in its first 64), O_g at 256 + 128 g.
+//
+// Work: an item is 256 rows of one sequence and KV head with the tiles that they see. A plan kernel lists the items on the
+// device (the lengths never leave it) and deals them out: whole rounds of one item per SM as long as no SM gets more than
+// its share of all tiles, so that neighbours read the same keys at the same time; then the rest, cut like one line so that
+// every SM ends with its share. An item that is cut leaves FP32 parts, which a third kernel joins in order.
+//
+// Every wait is bounded (2 s): on expiry a status is recorded, the roles stop, the products in flight are drained and TMEM
+// is freed.
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+
+#include <algorithm>
+#include <string>
+#include <type_traits>
+
+#include "attend.cuh"
+
+namespace rc {
+namespace paged {
+
+constexpr int kTile = 128;      // keys of a block, rows of a tile
+constexpr int kItemRows = 256;  // rows of an item: two tiles
+constexpr int kChunkThreads = 384;
+constexpr int kPlanThreads = 1024;
+constexpr int kKStages = 3;
+constexpr int kVStages = 2;
+// Register split (setmaxnreg): the launch holds kLaunchRegs a thread (checked on the host); the third warpgroup gives up
+// registers for the softmax warpgroups, which hold a row of 128 scores.
+constexpr int kLaunchRegs = 168;
+constexpr int kSoftmaxRegs = 208;
+constexpr int kRoleRegs = 88;
+static_assert(2 * kSoftmaxRegs + kRoleRegs == 3 * kLaunchRegs, "register split must equal the launch's registers");
+constexpr float kRescale = 8.0f;  // log2 units
+constexpr int kPolyEvery = 4;     // one of so many pairs of exponentials is taken from the FMA pipe
+constexpr int kTurnBarrier = 1;   // named barriers 1 and 2
+
+template <int D>
+struct ChunkShape {
+  static constexpr int boxes = D / 64;
+  static constexpr int box_bytes = kTile * 128;
+  static constexpr int tile_bytes = boxes * box_bytes;
+  static constexpr int q_off = 0;
+  static constexpr int k_off = q_off + 2 * tile_bytes;
+  static constexpr int v_off = k_off + kKStages * tile_bytes;
+  static constexpr int bar_off = v_off + kVStages * tile_bytes;
+  static constexpr int bytes = bar_off + 256 + 1024;  // + barriers, alignment slack
+  static_assert(bytes <= 227 * 1024, "shared memory of one CTA");
+};
+
+struct Item {  // 32 bytes
+  int seq, head, row_tile, tiles;
+  int q_first, q_len, kv_len, start;  // start: its place in the line (items that are not dealt out whole)
+};
+
+struct Plan {
+  int* head;   // [0] items, [1] whole rounds
+  int* cut;    // [ctas + 1]: the line's cuts
+  int* first;  // [ctas]: the item in which each CTA's part of the line begins
+  int* base;   // [seqs]: first item of each sequence
+  Item* items;
+};
+
+struct Chunk {
+  Args a;
+  Plan plan;
+  float* part_o;   // [2 * ctas, 256, D]
+  float* part_ml;  // [2 * ctas, 256, 2]
+  int ctas;
+  int row_tiles;   // of a sequence and KV head, at most
+  int most_items;  // room for items
+};
+
+__device__ __forceinline__ int plan_scan(int value, int* warp_sums, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = value;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 31) warp_sums[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    int w = warp_sums[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += y;
+    }
+    warp_sums[lane] = w;
+  }
+  __syncthreads();
+  *total = warp_sums[31];
+  return x - value + (warp > 0 ? warp_sums[warp - 1] : 0);
+}
+
+// Queries of a row tile of a sequence: [first, end).
+struct RowQueries {
+  int first, end;
+  __device__ __forceinline__ RowQueries(const Args& a, int row_tile, int q_len) {
+    first = row_tile * kItemRows / a.group;
+    end = min(q_len, (row_tile * kItemRows + kItemRows - 1) / a.group + 1);
+  }
+};
+
+__global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const __grid_constant__ Chunk p) {
+  __shared__ int warp_sums[32];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const Args& a = p.a;
+  const Plan& plan = p.plan;
+  auto length = [&](int s, int* q_first, int* kv_len) {
+    *q_first = __ldg(a.cu_q + s);
+    int q_len = min(__ldg(a.cu_q + s + 1), a.tokens) - *q_first;
+    if (*q_first < 0 || q_len < 0) q_len = 0;
+    *kv_len = static_cast<int>(min(static_cast<int64_t>(max(0, __ldg(a.kv_lens + s))), static_cast<int64_t>(a.width) * a.tiling.page));
+    return q_len;
+  };
+  auto row_tiles = [&](int q_len) {
+    return static_cast<int>(min(static_cast<int64_t>(p.row_tiles), (static_cast<int64_t>(q_len) * a.group + kItemRows - 1) / kItemRows));
+  };
+  int items = 0;
+  for (int s0 = 0; s0 < a.seqs; s0 += kPlanThreads) {
+    const int s = s0 + threadIdx.x;
+    int n = 0, q_first, kv_len;
+    if (s < a.seqs) n = row_tiles(length(s, &q_first, &kv_len)) * a.kv_heads;
+    int total;
+    const int before = plan_scan(n, warp_sums, &total);
+    if (s < a.seqs) plan.base[s] = items + before;
+    items += total;
+  }
+  items = min(items, p.most_items);  // cu_q that runs backwards could name rows more than once
+  __syncthreads();
+  int sum = 0;
+  for (int i = threadIdx.x; i < items; i += kPlanThreads) {
+    int lo = 0, hi = a.seqs - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (plan.base[mid] <= i) lo = mid;
+      else hi = mid - 1;
+    }
+    Item item;
+    item.seq = lo;
+    item.q_len = length(lo, &item.q_first, &item.kv_len);
+    const int n = row_tiles(item.q_len), local = i - plan.base[lo];
+    item.head = local / n;
+    item.row_tile = n - 1 - (local - item.head * n);  // the rows that see most come first
+    const RowQueries rows(a, item.row_tile, item.q_len);
+    item.tiles = max(1, TileRange<kTile>(Sight(a, item.kv_len, item.q_len), rows.first, rows.end).count());
+    item.start = 0;
+    plan.items[i] = item;
+    sum += item.tiles;
+  }
+  int all;
+  plan_scan(sum, warp_sums, &all);
+  const int share = (all + p.ctas - 1) / p.ctas;
+  // whole rounds: 3 % above the share is less than cutting the last items costs
+  const int limit = share + share / 32;
+  const int c = threadIdx.x;
+  int whole = 0, rounds = 0;
+  for (;;) {
+    const int at = rounds * p.ctas;
+    if (at + p.ctas > items) break;
+    const int next = c < p.ctas ? whole + plan.items[at + c].tiles : 0;
+    if (!__syncthreads_and(next <= limit)) break;
+    whole = next;
+    ++rounds;
+  }
+  const int from = rounds * p.ctas;
+  int line = 0;
+  for (int i0 = from; i0 < items; i0 += kPlanThreads) {
+    const int i = i0 + threadIdx.x;
+    const int n = i < items ? plan.items[i].tiles : 0;
+    int total;
+    const int before = plan_scan(n, warp_sums, &total);
+    if (i < items) plan.items[i].start = line + before;
+    line += total;
+  }
+  __syncthreads();
+  int wanted_all;
+  const int before = plan_scan(c < p.ctas ? max(0, share - whole) : 0, warp_sums, &wanted_all);
+  // if whole rounds went over the share, the last CTA takes what is left
+  if (c <= p.ctas) {
+    const int cut = c == p.ctas ? line : min(line, before);
+    plan.cut[c] = cut;
+    if (c < p.ctas) {
+      int lo = from, hi = items - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (plan.items[mid].start <= cut) lo = mid;
+        else hi = mid - 1;
+      }
+      plan.first[c] = lo;
+    }
+  }
+  if (c == 0) {
+    plan.head[0] = items;
+    plan.head[1] = rounds;
+  }
+}
+
+// A CTA's n-th piece of work.
+struct Segment {
+  Item item;
+  int t0, t1;
+  bool starts, ends;  // holds the item's first, last tile
+
+  __device__ __forceinline__ bool load(const Chunk& p, int cta, int n) {
+    const int rounds = p.plan.head[1], items = p.plan.head[0];
+    int i, begin = 0, end = 1 << 30;
+    if (n < rounds) {
+      i = n * p.ctas + cta;
+    } else {
+      i = p.plan.first[cta] + n - rounds;
+      begin = p.plan.cut[cta];
+      end = p.plan.cut[cta + 1];
+      if (begin >= end || i >= items) return false;
+    }
+    const int4* src = reinterpret_cast<const int4*>(p.plan.items + i);
+    const int4 x = src[0], y = src[1];
+    item = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+    if (n < rounds) {
+      t0 = 0;
+      t1 = item.tiles;
+    } else {
+      if (item.start >= end) return false;
+      t0 = max(0, begin - item.start);
+      t1 = min(item.tiles, end - item.start);
+    }
+    starts = t0 == 0;
+    ends = t1 == item.tiles;
+    return t0 < t1;
+  }
+};
+
+// -- two FP32 numbers at a time ---------------------------------------------------------------------------------------
+
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 2^x for two x <= kRescale on the FMA and integer pipes: n = rint(x) through the low bits of x + 1.5 * 2^23, f = x - n
+// in [-1/2, 1/2], 2^f by the polynomial of degree 4 with p(0) = 1 that has the least relative error there (2.9e-6, a
+// thousandth of what rounding P to 16 bits loses), and n added to the exponent. Below 2^-125 it stays there (not masked
+// scores: those take the exponential unit, which gives 0).
+__device__ __forceinline__ void exp2_pair(uint64_t x, float& p0, float& p1) {
+  float x0, x1;
+  unpair(x, x0, x1);
+  x = pair(fmaxf(x0, -125.0f), fmaxf(x1, -125.0f));
+  const uint64_t magic = pair(12582912.0f, 12582912.0f), minus = pair(-12582912.0f, -12582912.0f);
+  const uint64_t t = add2(x, magic);
+  const uint64_t n = add2(t, minus);
+  const uint64_t f = fma2(n, pair(-1.0f, -1.0f), x);
+  uint64_t p = fma2(pair(0.009582853f, 0.009582853f), f, pair(0.055906426f, 0.055906426f));
+  p = fma2(p, f, pair(0.24024099f, 0.24024099f));
+  p = fma2(p, f, pair(0.69312418f, 0.69312418f));
+  p = fma2(p, f, pair(1.0f, 1.0f));
+  float t0, t1;
+  unpair(t, t0, t1);
+  unpair(p, p0, p1);
+  p0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
+  p1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
+}
+
+// One row's exponentials: r holds 128 raw scores, comes back as 64 pairs of P in r[.][0 .. 31]; returns their sum.
+template <typename T, int kPoly>
+__device__ __forceinline__ float softmax_row(uint32_t (&r)[2][64], float scale_log2, float neg_m, uint32_t (&pk)[2][32]) {
+  const uint64_t scale2 = pair(scale_log2, scale_log2), m2 = pair(neg_m, neg_m);
+  uint64_t sums[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int c = 0; c < 64; ++c) {
+    const int h = c >> 5, e = (c & 31) * 2;
+    const uint64_t x = fma2(pair(__uint_as_float(r[h][e]), __uint_as_float(r[h][e + 1])), scale2, m2);
+    float p0, p1;
+    if (kPoly > 0 && c % (kPoly > 0 ? kPoly : 1) == 1) {
+      exp2_pair(x, p0, p1);
+    } else {
+      unpair(x, p0, p1);
+      p0 = exp2_approx(p0);
+      p1 = exp2_approx(p1);
+    }
+    sums[c & 3] = add2(sums[c & 3], pair(p0, p1));
+    pk[h][c & 31] = pack2<T>(p0, p1);
+  }
+  float a, b;
+  unpair(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])), a, b);
+  return a + b;
+}
+
+__device__ __forceinline__ void named_sync(int id) { asm volatile("bar.sync %0, 256;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ void named_arrive(int id) { asm volatile("bar.arrive %0, 256;" ::"r"(id) : "memory"); }
+
+// Shared-memory descriptor of an MN-major operand in the 128-byte swizzle: blocks of 64 channels x 8 keys (1,024 bytes),
+// `block_bytes` between the blocks of 64 channels (leading offset), 1,024 bytes between groups of 8 keys (stride offset).
+__device__ __forceinline__ uint64_t sw128_mnmajor_desc(uint32_t smem_addr, uint32_t block_bytes) {
+  uint64_t desc = 0;
+  desc |= static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu);
+  desc |= static_cast<uint64_t>((block_bytes >> 4) & 0x3FFFu) << 16;
+  desc |= static_cast<uint64_t>(1024u >> 4) << 32;
+  desc |= static_cast<uint64_t>(1u) << 46;
+  desc |= static_cast<uint64_t>(2u) << 61;
+  return desc;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kChunkThreads, 1)
+    chunk_kernel(const __grid_constant__ PageMaps maps, const __grid_constant__ Chunk p) {
+  using Shape = ChunkShape<D>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + Shape::bar_off);
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* k_full = q_empty + 1;         // [kKStages]
+  uint64_t* k_empty = k_full + kKStages;  // [kKStages]
+  uint64_t* v_full = k_empty + kKStages;  // [kVStages]
+  uint64_t* v_empty = v_full + kVStages;  // [kVStages]
+  uint64_t* s_full = v_empty + kVStages;  // [2] per tile
+  uint64_t* p_full = s_full + 2;          // [2]
+  uint64_t* o_done = p_full + 2;          // [2]
+  uint64_t* drained = o_done + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
+  const Args& a = p.a;
+  int* status = a.status;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int cta = blockIdx.x;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 32);
+    mbar_init(q_empty, 1);
+    for (int b = 0; b < kKStages; ++b) {
+      mbar_init(&k_full[b], 1);
+      mbar_init(&k_empty[b], 1);
+    }
+    for (int b = 0; b < kVStages; ++b) {
+      mbar_init(&v_full[b], 1);
+      mbar_init(&v_empty[b], 1);
+    }
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(&s_full[g], 1);
+      mbar_init(&p_full[g], 4);
+      mbar_init(&o_done[g], 1);
+    }
+    mbar_init(drained, 1);
+    fence_barrier_init();
+  }
+  if (warp == 8 && lane == 0) {
+    tma_prefetch_desc(&maps.k_wide);
+    tma_prefetch_desc(&maps.v_wide);
+  }
+  if (warp == 10) tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the plan
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  Segment seg;
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRoleRegs));
+    if (warp < 10) {
+      // ---------------- TMA: warp 8 streams K, warp 9 streams V ----------------
+      const bool is_k = warp == 8;
+      const int stages = is_k ? kKStages : kVStages;
+      uint64_t* full = is_k ? k_full : v_full;
+      uint64_t* empty = is_k ? k_empty : v_empty;
+      uint8_t* ring = smem + (is_k ? Shape::k_off : Shape::v_off);
+      const CUtensorMap* wide = is_k ? &maps.k_wide : &maps.v_wide;
+      const CUtensorMap* step = is_k ? &maps.k_step : &maps.v_step;
+      int stage = 0;
+      uint32_t phase = 1;
+      bool ok = true;
+      for (int n = 0; ok && seg.load(p, cta, n); ++n) {
+        const RowQueries rows(a, seg.item.row_tile, seg.item.q_len);
+        const TileRange<kTile> range(Sight(a, seg.item.kv_len, seg.item.q_len), rows.first, rows.end);
+        const int* table = a.table + static_cast<int64_t>(seg.item.seq) * a.width;
+        for (int t = seg.t0; t < seg.t1; ++t) {
+          const int first = range.tile(t) * kTile;
+          const Boxes<kTile> boxes(a.tiling, first, seg.item.kv_len);
+          int row = 0, page = -1;
+          if (lane < boxes.count) page = boxes.page(table, a.pages, a.tiling, first, lane, &row, status);
+          ok = __all_sync(0xffffffffu, mbar_wait_park(&empty[stage], phase, status, kTimeoutProducer));
+          if (!ok) break;
+          if (lane == 0) {
+            if (boxes.count > 0) mbar_arrive_expect_tx(&full[stage], boxes.count * boxes.rows * 128 * Shape::boxes);
+            else mbar_arrive(&full[stage]);
+          }
+          __syncwarp();
+          if (lane < boxes.count) {
+            uint8_t* dst = ring + stage * Shape::tile_bytes + lane * boxes.rows * 128;
+            const CUtensorMap* map = boxes.rows == kTile ? wide : step;
+#pragma unroll
+            for (int b = 0; b < Shape::boxes; ++b)
+              load_page_box(dst + b * Shape::box_bytes, map, &full[stage], b * 64, row, seg.item.head, page);
+          }
+          if (++stage == stages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+    } else if (warp == 11) {
+      // ---------------- Q rows: 16-byte chunks, D / 8 lanes to a row ----------------
+      constexpr int kLanes = D / 8;          // lanes of a row
+      constexpr int kRowsPer = 32 / kLanes;  // rows of one pass
+      const int chunk = lane % kLanes, sub = lane / kLanes;
+      bool ok = true;
+      for (int n = 0; ok && seg.load(p, cta, n); ++n) {
+        if (n > 0) ok = __all_sync(0xffffffffu, mbar_wait_park(q_empty, (n - 1) & 1, status, kTimeoutGather));
+        if (!ok) break;
+        const int packed0 = seg.item.row_tile * kItemRows;
+#pragma unroll 4
+        for (int r0 = 0; r0 < kItemRows; r0 += kRowsPer) {
+          const int r = r0 + sub;
+          const int query = (packed0 + r) / a.group;
+          const bool valid = query < seg.item.q_len;
+          const int h = seg.item.head * a.group + packed0 + r - query * a.group;
+          const T* src = static_cast<const T*>(a.q);
+          if (valid) src += static_cast<int64_t>(seg.item.q_first + query) * a.q_token + h * a.q_head + chunk * 8;
+          const uint32_t dst = smem_u32(smem + Shape::q_off + (r >> 7) * Shape::tile_bytes + (chunk >> 3) * Shape::box_bytes) +
+                               (r & 127) * 128 + (((chunk & 7) ^ (r & 7)) << 4);
+          const int bytes = valid ? 16 : 0;  // rows past the sequence are zeros
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        fence_proxy_async_smem();
+        mbar_arrive(q_full);
+      }
+    } else {
+      // ---------------- products: the whole warp keeps step, lane 0 issues ----------------
+      constexpr uint32_t kFormat = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+      constexpr uint32_t idesc_s = make_idesc_f16(kTile, kTile, kFormat);
+      constexpr uint32_t idesc_o = make_idesc_f16(kTile, D, kFormat) | (1u << 16);  // B is MN-major
+      const uint32_t qa = smem_u32(smem + Shape::q_off);
+      bool ok = true;
+      int it = 0;  // blocks so far
+      int k_stage = 0, v_stage = 0;
+      uint32_t k_phase = 0, v_phase = 0;
+      // of the block before: whether it begins, ends its segment; V rows that no row sees: those outside [v_low, v_high)
+      // but for the first v_sink
+      bool was_first = false, was_last = false;
+      int v_low = 0, v_high = kTile, v_sink = 0;
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait_park(bar, parity, status, kTimeoutMma));
+      };
+      auto issue_s = [&](int g) {
+        if (!ok || lane != 0) return;
+        const uint32_t ka = smem_u32(smem + Shape::k_off + k_stage * Shape::tile_bytes);
+        const uint32_t qg = qa + g * Shape::tile_bytes;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t box = (kk >> 2) * Shape::box_bytes;
+          mma_f16(tmem_base + g * kTile, sw128_kmajor_desc(qg + box) + 2 * (kk & 3), sw128_kmajor_desc(ka + box) + 2 * (kk & 3),
+                  idesc_s, kk > 0 ? 1u : 0u);
+        }
+        mma_commit(&s_full[g]);
+      };
+      auto issue_pv = [&](int g) {  // the block before
+        wait(&p_full[g], (it - 1) & 1);
+        if (!ok) return;
+        tc_fence_after();
+        if (lane != 0) return;
+        const uint32_t va = smem_u32(smem + Shape::v_off + v_stage * Shape::tile_bytes);
+#pragma unroll
+        for (int kk = 0; kk < kTile / 16; ++kk)
+          mma_f16_ts(tmem_base + 256 + g * kTile, tmem_base + g * kTile + kk * 8,
+                     sw128_mnmajor_desc(va + kk * 16 * 128, Shape::box_bytes), idesc_o, (!was_first || kk > 0) ? 1u : 0u);
+        if (was_last) mma_commit(&o_done[g]);
+      };
+      auto take_v = [&]() {  // V of the block before has come; what no row sees of it becomes zeros (0 * NaN is NaN)
+        wait(&v_full[v_stage], v_phase);
+        if (ok && (v_low > 0 || v_high < kTile)) {
+          uint8_t* v = smem + Shape::v_off + v_stage * Shape::tile_bytes;
+          for (int r = 0; r < kTile; ++r) {
+            if ((r >= v_low || r < v_sink) && r < v_high) continue;
+            for (int c = lane; c < Shape::boxes * 8; c += 32)
+              *reinterpret_cast<uint4*>(v + (c >> 3) * Shape::box_bytes + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+      };
+      auto done_v = [&]() {
+        if (ok && lane == 0) mma_commit(&v_empty[v_stage]);
+        if (++v_stage == kVStages) {
+          v_stage = 0;
+          v_phase ^= 1;
+        }
+      };
+      for (int n = 0; ok && seg.load(p, cta, n); ++n) {
+        const RowQueries rows(a, seg.item.row_tile, seg.item.q_len);
+        const Sight sight(a, seg.item.kv_len, seg.item.q_len);
+        const TileRange<kTile> range(sight, rows.first, rows.end);
+        const int low = sight.low(sight.last(rows.first)), top = min(sight.last(rows.end - 1), seg.item.kv_len - 1);
+        for (int t = seg.t0; t < seg.t1 && ok; ++t) {
+          if (it > 0) {
+            take_v();
+            issue_pv(0);
+          }
+          if (t == seg.t0) wait(q_full, n & 1);
+          wait(&k_full[k_stage], k_phase);
+          tc_fence_after();
+          issue_s(0);
+          if (it > 0) {
+            issue_pv(1);
+            done_v();
+          }
+          issue_s(1);
+          if (ok && lane == 0) {
+            mma_commit(&k_empty[k_stage]);
+            if (t + 1 == seg.t1) mma_commit(q_empty);
+          }
+          if (++k_stage == kKStages) {
+            k_stage = 0;
+            k_phase ^= 1;
+          }
+          ++it;
+          was_first = t == seg.t0;
+          was_last = t + 1 == seg.t1;
+          const int first = range.tile(t) * kTile;
+          v_low = low - first;
+          v_high = min(kTile, top + 1 - first);
+          v_sink = a.sinks - first;
+          if (v_sink >= kTile) v_low = 0;
+        }
+      }
+      if (it > 0) {
+        take_v();
+        issue_pv(0);
+        issue_pv(1);
+        done_v();
+      }
+      __syncwarp();
+      if (lane == 0) {
+        mma_commit(drained);
+        (void)mbar_wait_park(drained, 0, nullptr, 0);
+      }
+      __syncwarp();
+    }
+  } else {
+    // ---------------- softmax: warpgroup g owns tile g ----------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    const int g = warp >> 2, quarter = warp & 3;
+    const int row = quarter * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t s_col = tmem_base + g * kTile + lanes;
+    const uint32_t o_col = tmem_base + 256 + g * kTile + lanes;
+    // Turns: warpgroup g runs the exponentials of a block after the other has run those of its last one. Every warp takes
+    // every turn, also after a failed wait, so none is left waiting.
+    if (g == 1) named_arrive(kTurnBarrier);
+    bool ok = true;
+    int it = 0;
+    for (int n = 0; seg.load(p, cta, n); ++n) {
+      const int packed = seg.item.row_tile * kItemRows + g * kTile + row;
+      const int query = packed / a.group;
+      const Sight sight(a, seg.item.kv_len, seg.item.q_len);
+      const RowQueries rows(a, seg.item.row_tile, seg.item.q_len);
+      const TileRange<kTile> range(sight, rows.first, rows.end);
+      const int last = min(sight.last(min(query, seg.item.q_len - 1)), seg.item.kv_len - 1);
+      const int low = sight.low(last);
+      float m_run = -INFINITY, l_run = 0.0f;  // of scale * log2(e) * s
+      for (int t = seg.t0; t < seg.t1; ++t, ++it) {
+        uint32_t r[2][64];
+        float mx = -INFINITY;
+        bool whole = true;
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait_park(&s_full[g], it & 1, status, kTimeoutEpilogue));
+        if (ok) {
+          tc_fence_after();
+          tmem_ld_32x32b_x64(s_col, r[0]);
+          tmem_ld_32x32b_x64(s_col + 64, r[1]);
+          tmem_wait_ld();
+          const int first = range.tile(t) * kTile;
+          const int high = last + 1 - first, from = low - first, sink = a.sinks - first;  // sees [from, high), [0, sink)
+          whole = __all_sync(0xffffffffu, high >= kTile && (from <= 0 || sink >= kTile));
+          if (!whole) {
+#pragma unroll
+            for (int b = 0; b < 8; ++b) {
+              if (__all_sync(0xffffffffu, high >= 16 * b + 16 && (from <= 16 * b || sink >= 16 * b + 16))) continue;
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const int c = 16 * b + e;
+                if (c >= high || (c < from && c >= sink)) r[c >> 6][c & 63] = __float_as_uint(-INFINITY);
+              }
+            }
+          }
+          float pm[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) pm[k] = __uint_as_float(r[0][k]);
+#pragma unroll
+          for (int c = 8; c < kTile - 8; c += 16)
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              pm[k] = max3(pm[k], __uint_as_float(r[(c + k) >> 6][(c + k) & 63]), __uint_as_float(r[(c + 8 + k) >> 6][(c + 8 + k) & 63]));
+#pragma unroll
+          for (int k = 0; k < 8; ++k) pm[k] = fmaxf(pm[k], __uint_as_float(r[1][56 + k]));
+          mx = max3(max3(pm[0], pm[1], pm[2]), max3(pm[3], pm[4], pm[5]), fmaxf(pm[6], pm[7])) * a.scale_log2;
+        }
+        named_sync(kTurnBarrier + g);
+        if (ok) {
+          if (t == seg.t0) {
+            m_run = mx;
+          } else {
+            // O_g holds the blocks before this one: their products were issued before this block's S
+            const bool need = mx > m_run + kRescale;
+            if (__any_sync(0xffffffffu, need)) {
+              const float alpha = need ? exp2_approx(m_run - mx) : 1.0f;
+#pragma unroll
+              for (int c = 0; c < D; c += 16) {
+                uint32_t o[16];
+                tmem_ld_32x32b_x16(o_col + c, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                tmem_st_32x32b_x16(o_col + c, o);
+              }
+              l_run *= alpha;
+              if (need) m_run = mx;
+            }
+          }
+          const float neg_m = m_run == -INFINITY ? 0.0f : -m_run;  // a row that has seen no key yet
+          uint32_t pk[2][32];
+          l_run += whole ? softmax_row<T, kPolyEvery>(r, a.scale_log2, neg_m, pk) : softmax_row<T, 0>(r, a.scale_log2, neg_m, pk);
+          tmem_st_32x32b_x32(s_col, pk[0]);
+          tmem_st_32x32b_x32(s_col + 32, pk[1]);
+        }
+        named_arrive(kTurnBarrier + 1 - g);
+        if (ok) {
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[g]);
+        }
+      }
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait_park(&o_done[g], n & 1, status, kTimeoutEpilogue));
+      if (ok) {
+        tc_fence_after();
+        const bool valid = query < seg.item.q_len, whole = seg.starts && seg.ends;
+        const float inv = whole ? (l_run > 0.0f ? 1.0f / l_run : 0.0f) : 1.0f;
+        const int64_t token = seg.item.q_first + query;
+        const int h = seg.item.head * a.group + packed - query * a.group;
+        const int64_t slot = (2 * static_cast<int64_t>(cta) + (seg.starts ? 1 : 0)) * kItemRows + g * kTile + row;
+#pragma unroll
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          uint32_t o[32];
+          tmem_ld_32x32b_x32(o_col + c0, o);
+          tmem_wait_ld();
+          if (valid && whole) {
+            T* dst = static_cast<T*>(a.out) + token * a.out_token + h * a.out_head + c0;
+#pragma unroll
+            for (int c = 0; c < 32; c += 8) {
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                w[e] = pack2<T>(__uint_as_float(o[c + 2 * e]) * inv, __uint_as_float(o[c + 2 * e + 1]) * inv);
+              *reinterpret_cast<uint4*>(dst + c) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          } else if (valid) {
+            float* dst = p.part_o + slot * D + c0;
+#pragma unroll
+            for (int c = 0; c < 32; c += 4)
+              *reinterpret_cast<uint4*>(dst + c) = make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+          }
+          __syncwarp();
+        }
+        tc_fence_before();  // the next item's products overwrite O after this warp's next arrival
+        if (valid && whole && a.lse != nullptr)
+          a.lse[token * a.heads + h] = l_run > 0.0f ? (m_run + log2f(l_run)) * kLn2 : -INFINITY;
+        if (valid && !whole) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(m_run, l_run);
+      }
+    }
+    if (g == 0) named_sync(kTurnBarrier);  // the other warpgroup's last turn
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 10) tmem_dealloc(tmem_base, 512);
+}
+
+// Joins the parts of items that were cut. Block (x, c): rows 8 x .. of the item that begins in CTA c's part of the line
+// and goes on in the next one's. One warp per row.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) chunk_join_kernel(const __grid_constant__ Chunk p) {
+  constexpr int kPer = D / 32;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const Args& a = p.a;
+  const int c0 = blockIdx.y;
+  const int cut = p.plan.cut[c0 + 1];
+  if (cut >= p.plan.cut[p.ctas]) return;
+  const Item item = p.plan.items[p.plan.first[c0 + 1]];
+  if (item.start >= cut || item.start < p.plan.cut[c0]) return;
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int packed = item.row_tile * kItemRows + row, query = packed / a.group;
+  if (query >= item.q_len) return;
+  const int end = item.start + item.tiles;
+  auto slot_of = [&](int c) { return (2 * static_cast<int64_t>(c) + (c == c0)) * kItemRows + row; };
+  // parts: c0 and every CTA after it whose part of the line is not empty and begins before the item's end
+  float top = p.part_ml[slot_of(c0) * 2];
+  for (int c = c0 + 1; c < p.ctas && p.plan.cut[c] < end; ++c)
+    if (p.plan.cut[c] < p.plan.cut[c + 1]) top = fmaxf(top, p.part_ml[slot_of(c) * 2]);
+  const float use = top == -INFINITY ? 0.0f : top;
+  float acc[kPer], sum = 0.0f;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) acc[e] = 0.0f;
+  for (int c = c0; c < p.ctas && (c == c0 || p.plan.cut[c] < end); ++c) {
+    if (p.plan.cut[c] >= p.plan.cut[c + 1]) continue;
+    const int64_t slot = slot_of(c);
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot * 2);
+    const float w = exp2_approx(ml.x - use);
+    sum = fmaf(w, ml.y, sum);
+#pragma unroll
+    for (int e = 0; e < kPer; e += 2) {
+      const float2 x = *reinterpret_cast<const float2*>(p.part_o + slot * D + lane * kPer + e);
+      acc[e] = fmaf(w, x.x, acc[e]);
+      acc[e + 1] = fmaf(w, x.y, acc[e + 1]);
+    }
+  }
+  const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+  const int64_t token = item.q_first + query;
+  const int h = item.head * a.group + packed - query * a.group;
+  T* dst = static_cast<T*>(a.out) + token * a.out_token + h * a.out_head + lane * kPer;
+#pragma unroll
+  for (int e = 0; e < kPer; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack2<T>(acc[e] * inv, acc[e + 1] * inv);
+  if (a.lse != nullptr && lane == 0) a.lse[token * a.heads + h] = sum > 0.0f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+}
+
+template <typename T, int D>
+void chunk_launch(const Args& args, const at::Tensor& k_pages, const at::Tensor& v_pages, int max_q_len,
+                  const at::Tensor& like, cudaStream_t stream, int device) {
+  using Shape = ChunkShape<D>;
+  static bool configured = false;
+  if (!configured) {
+    RC_CUDA(cudaFuncSetAttribute(chunk_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::bytes));
+    cudaFuncAttributes attr;  // the register split assumes exactly kLaunchRegs a thread
+    RC_CUDA(cudaFuncGetAttributes(&attr, chunk_kernel<T, D>));
+    RC_CHECK(attr.numRegs == kLaunchRegs, "paged attention compiled to " + std::to_string(attr.numRegs) +
+                                              " registers a thread; its register split needs " + std::to_string(kLaunchRegs));
+    configured = true;
+  }
+  Chunk p{};
+  p.a = args;
+  p.a.tiling = Tiling::of(args.tiling.page, kTile);
+  const int64_t row_tiles = (static_cast<int64_t>(max_q_len) * args.group + kItemRows - 1) / kItemRows;
+  const int64_t most_items = std::min<int64_t>(static_cast<int64_t>(args.seqs) * row_tiles,
+                                               static_cast<int64_t>(args.tokens) * args.group / kItemRows + args.seqs) * args.kv_heads;
+  RC_CHECK(most_items < (1ll << 26), "too many rows for one launch");
+  p.row_tiles = static_cast<int>(row_tiles);
+  p.most_items = static_cast<int>(most_items);
+  p.ctas = sm_count(device);
+  RC_CHECK(p.ctas < kPlanThreads, "more SMs than the plan's threads");
+  const int64_t o_floats = 2ll * p.ctas * kItemRows * D, ml_floats = 2ll * p.ctas * kItemRows * 2;
+  const int64_t ints = most_items * 8 + 4 + 2ll * (p.ctas + 1) + args.seqs;
+  at::Tensor workspace = at::empty({o_floats + ml_floats + ints}, like.options().dtype(at::kFloat));
+  p.part_o = workspace.data_ptr<float>();
+  p.part_ml = p.part_o + o_floats;
+  p.plan.items = reinterpret_cast<Item*>(p.part_ml + ml_floats);
+  p.plan.head = reinterpret_cast<int*>(p.plan.items + most_items);
+  p.plan.cut = p.plan.head + 4;
+  p.plan.first = p.plan.cut + p.ctas + 1;
+  p.plan.base = p.plan.first + p.ctas + 1;
+  const PageMaps maps = page_maps(k_pages, v_pages, p.a.tiling, kTile);
+  chunk_plan_kernel<<<1, kPlanThreads, 0, stream>>>(p);
+  RC_CUDA(cudaGetLastError());
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(p.ctas);
+  config.blockDim = dim3(kChunkThreads);
+  config.dynamicSmemBytes = Shape::bytes;
+  config.stream = stream;
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  RC_CUDA(cudaLaunchKernelEx(&config, chunk_kernel<T, D>, maps, p));
+  config.gridDim = dim3(kItemRows / 8, p.ctas - 1);
+  config.blockDim = dim3(256);
+  config.dynamicSmemBytes = 0;
+  RC_CUDA(cudaLaunchKernelEx(&config, chunk_join_kernel<T, D>, p));
+}
+
+void attend_chunk(const Args& a, int head_dim, bool half, const at::Tensor& k_pages, const at::Tensor& v_pages,
+                  int max_q_len, const at::Tensor& like, cudaStream_t stream, int device) {
+  if (head_dim == 128)
+    half ? chunk_launch<__half, 128>(a, k_pages, v_pages, max_q_len, like, stream, device)
+         : chunk_launch<__nv_bfloat16, 128>(a, k_pages, v_pages, max_q_len, like, stream, device);
+  else
+    half ? chunk_launch<__half, 64>(a, k_pages, v_pages, max_q_len, like, stream, device)
+         : chunk_launch<__nv_bfloat16, 64>(a, k_pages, v_pages, max_q_len, like, stream, device);
+}
+
+}  // namespace paged
+}  // namespace rc

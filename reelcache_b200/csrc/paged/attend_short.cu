@@ -99,15 +99,14 @@ struct SeqWork {
                                   static_cast<int64_t>(a.width) * a.tiling.page));
     row_tiles = static_cast<int>(min(static_cast<int64_t>(most), (static_cast<int64_t>(q_len) * a.group + rows - 1) / rows));
     tiles = 0;
-    if (q_len > 0) tiles = max(1, TileRange(a.tiling, Sight(a, kv_len, q_len), 0, q_len).count());
+    if (q_len > 0) tiles = max(1, TileRange<kShortTile>(Sight(a, kv_len, q_len), 0, q_len).count());
   }
   __device__ __forceinline__ int items(const Args& a) const { return row_tiles * a.kv_heads; }
 };
 
 template <typename T, int D, int kM>
 __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
-    short_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                 const __grid_constant__ Short p) {
+    short_kernel(const __grid_constant__ PageMaps maps, const __grid_constant__ Short p) {
   using Shape = ShortShape<D>;
   constexpr int kGroups = 4 / kM;               // warps that split a tile's keys
   constexpr int kKeys = kShortTile / kGroups;   // keys of a warp
@@ -132,8 +131,8 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
   }
   // The line of work: total, this CTA's share, and where it begins.
   if (warp == 4) {
-    tma_prefetch_desc(&tmK);
-    tma_prefetch_desc(&tmV);
+    tma_prefetch_desc(&maps.k_wide);
+    tma_prefetch_desc(&maps.v_wide);
   }
   if (warp == 0) {
     int total = 0;
@@ -200,32 +199,28 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
       const int item = (at - base) / w.tiles, t0 = (at - base) - item * w.tiles;
       const int t1 = min(w.tiles, t0 + end - at);
       const int head = item / w.row_tiles;
-      const TileRange range(a.tiling, Sight(a, w.kv_len, w.q_len), 0, w.q_len);
+      const TileRange<kShortTile> range(Sight(a, w.kv_len, w.q_len), 0, w.q_len);
       for (int t = t0; t < t1; ++t) {
-        int block, row;
-        const int first = a.tiling.first(range.tile(t), &block, &row);
-        const int rest = w.kv_len - first;  // pages that hold a key of this tile
-        const int pages = rest <= 0 ? 0 : a.tiling.per_page > 1 ? 1 : min(a.tiling.per_tile, (rest + a.tiling.page - 1) / a.tiling.page);
+        const int first = range.tile(t) * kShortTile;
+        const Boxes<kShortTile> boxes(a.tiling, first, w.kv_len);
         if (!mbar_wait(&empty[stage], phase ^ 1, a.status, kTimeoutProducer)) return;
         if (lane == 0) {
-          if (pages > 0) mbar_arrive_expect_tx(&full[stage], pages * a.tiling.box * 128 * Shape::boxes * 2);
+          if (boxes.count > 0) mbar_arrive_expect_tx(&full[stage], boxes.count * boxes.rows * 128 * Shape::boxes * 2);
           else mbar_arrive(&full[stage]);
         }
         __syncwarp();
-        if (lane < pages) {
-          int page = __ldg(a.table + static_cast<int64_t>(s) * a.width + block + lane);
-          if (page < 0 || page >= a.pages) {
-            page = -1;
-            if (a.status != nullptr) atomicCAS(a.status + kPagedWord, 0, kPageRange);
-          }
-          uint8_t* k = smem + stage * 2 * Shape::tile_bytes + lane * a.tiling.page * 128;
+        if (lane < boxes.count) {
+          int row;
+          const int page = boxes.page(a.table + static_cast<int64_t>(s) * a.width, a.pages, a.tiling, first, lane, &row, a.status);
+          const bool wide = boxes.rows == kShortTile;
+          const CUtensorMap* km = wide ? &maps.k_wide : &maps.k_step;
+          const CUtensorMap* vm = wide ? &maps.v_wide : &maps.v_step;
+          uint8_t* k = smem + stage * 2 * Shape::tile_bytes + lane * boxes.rows * 128;
           uint8_t* v = k + Shape::tile_bytes;
 #pragma unroll
-          for (int b = 0; b < Shape::boxes; ++b)
-            load_page_box(k + b * Shape::box_bytes, &tmK, &full[stage], b * 64, row, head, page);
+          for (int b = 0; b < Shape::boxes; ++b) load_page_box(k + b * Shape::box_bytes, km, &full[stage], b * 64, row, head, page);
 #pragma unroll
-          for (int b = 0; b < Shape::boxes; ++b)
-            load_page_box(v + b * Shape::box_bytes, &tmV, &full[stage], b * 64, row, head, page);
+          for (int b = 0; b < Shape::boxes; ++b) load_page_box(v + b * Shape::box_bytes, vm, &full[stage], b * 64, row, head, page);
         }
         if (++stage == Shape::stages) {
           stage = 0;
@@ -253,7 +248,7 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
     const int t1 = min(w.tiles, t0 + end - at);
     const int head = item / w.row_tiles, row_tile = item - head * w.row_tiles;
     const Sight sight(a, w.kv_len, w.q_len);
-    const TileRange range(a.tiling, sight, 0, w.q_len);
+    const TileRange<kShortTile> range(sight, 0, w.q_len);
 
     // this thread's two rows
     int row_q[2], row_h[2], last[2], low[2];
@@ -288,9 +283,7 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 
     for (int t = t0; t < t1; ++t) {
-      int block, page_row;
-      const int first = a.tiling.first(range.tile(t), &block, &page_row);
-      const int count = a.tiling.count(page_row);
+      const int first = range.tile(t) * kShortTile;
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, a.status, kTimeoutEpilogue));
       if (ok) {
         const uint32_t kb = smem_u32(smem + stage * 2 * Shape::tile_bytes);
@@ -313,7 +306,7 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
             mma_16816(sc[2 * j + 1], q[k], b[2], b[3], T());
           }
         }
-        const bool whole = count == kShortTile && first + kShortTile - 1 <= all_last &&
+        const bool whole = first + kShortTile - 1 <= all_last &&
                            (first >= all_low || first + kShortTile <= a.sinks);
         if (!whole) {
 #pragma unroll
@@ -323,7 +316,7 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
               const int r = kg * kKeys + j * 8 + c0 + (e & 1);
               const int at_key = first + r;
               const int i = e >> 1;
-              if (!(r < count && at_key <= last[i] && at_key < w.kv_len && (at_key >= low[i] || at_key < a.sinks)))
+              if (!(at_key <= last[i] && at_key < w.kv_len && (at_key >= low[i] || at_key < a.sinks)))
                 sc[j][e] = -INFINITY;
             }
         }
@@ -374,7 +367,7 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
                 const int r = kg * kKeys + k * 16 + h * 8 + c0 + e;
-                if (r < count && first + r < w.kv_len && (first + r >= any_low || first + r < a.sinks)) keep[h] |= 0xffffu << (16 * e);
+                if (first + r < w.kv_len && (first + r >= any_low || first + r < a.sinks)) keep[h] |= 0xffffu << (16 * e);
               }
             }
           }
@@ -563,7 +556,7 @@ void short_launch(Args a, const at::Tensor& k_pages, const at::Tensor& v_pages, 
   const int64_t row_tiles = (static_cast<int64_t>(max_q_len) * a.group + kRows - 1) / kRows;
   p.row_tiles = static_cast<int>(row_tiles);
   const int64_t items = row_tiles * a.kv_heads;  // of one sequence, at most
-  const int64_t most_tiles = static_cast<int64_t>(a.seqs) * items * ((static_cast<int64_t>(a.width) * a.tiling.page + 7) / 8 + 2);
+  const int64_t most_tiles = static_cast<int64_t>(a.seqs) * items * (static_cast<int64_t>(a.width) * a.tiling.page / kShortTile + 2);
   const int ctas = static_cast<int>(std::min<int64_t>(sm_count(device) * kShortCtasPerSm, most_tiles));
   RC_CHECK(a.seqs * items * (kRows / 4) < (1ll << 31), "too many sequences and rows for one launch");
   const int64_t floats = 2ll * ctas * kRows * (D + 2), ints = 1 + 2ll * a.seqs;
@@ -572,8 +565,8 @@ void short_launch(Args a, const at::Tensor& k_pages, const at::Tensor& v_pages, 
   p.part_ml = p.part_o + 2ll * ctas * kRows * D;
   int* line = reinterpret_cast<int*>(p.part_o + floats);
   p.line = {line, line + 1, line + 1 + a.seqs};
-  const CUtensorMap tmK = page_map(k_pages, p.a.tiling.box), tmV = page_map(v_pages, p.a.tiling.box);
-  short_kernel<T, D, kM><<<ctas, kShortThreads, Shape::bytes, stream>>>(tmK, tmV, p);
+  const PageMaps maps = page_maps(k_pages, v_pages, p.a.tiling, kShortTile);
+  short_kernel<T, D, kM><<<ctas, kShortThreads, Shape::bytes, stream>>>(maps, p);
   RC_CUDA(cudaGetLastError());
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(static_cast<unsigned>(a.seqs * items * (kRows / 4)));
@@ -607,70 +600,4 @@ void attend_short(const Args& a, int head_dim, bool half, const at::Tensor& k_pa
 }
 
 }  // namespace paged
-
-// out = softmax over the visible keys of scale * q k^T, times v, for the new tokens of every sequence; lse its natural
-// log-sum-exp. max_q_len bounds every sequence's new tokens; tokens past a sequence's bound are left alone.
-void paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
-                     const at::Tensor& kv_lens, const at::Tensor& cu_q, at::Tensor& out,
-                     const c10::optional<at::Tensor>& lse, int64_t max_q_len, bool causal, int64_t window, int64_t sinks,
-                     double scale, const c10::optional<at::Tensor>& status) {
-  check_cuda_tensor(q, "q");
-  const at::ScalarType type = q.scalar_type();
-  RC_CHECK(type == at::kBFloat16 || type == at::kHalf, "paged attention takes bf16 or fp16");
-  RC_CHECK(q.dim() == 3 && (q.size(2) == 64 || q.size(2) == 128), "q must be [tokens, heads, head_dim] with head_dim 64 or 128");
-  RC_CHECK(q.size(0) < (1ll << 31), "too many tokens for one launch");
-  RC_CHECK(out.sizes() == q.sizes() && out.scalar_type() == type && out.device() == q.device(), "out must match q");
-  const at::Tensor* rows[2] = {&q, &out};
-  for (const at::Tensor* t : rows)
-    RC_CHECK(t->numel() == 0 || (t->stride(2) == 1 && t->stride(0) % 8 == 0 && t->stride(1) % 8 == 0 &&
-                                 reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0),
-             "rows must have unit inner stride and 16-byte aligned strides and base");
-  RC_CHECK(k_pages.device() == q.device() && v_pages.device() == q.device() && k_pages.scalar_type() == type &&
-               v_pages.scalar_type() == type && k_pages.dim() == 4,
-           "the pages must have the type and device of q");
-  const int64_t kv_heads = k_pages.size(2);
-  RC_CHECK(kv_heads >= 1 && q.size(1) % kv_heads == 0 && q.size(1) >= kv_heads, "heads must be a multiple of the KV heads");
-  const paged::Pages kp = paged::check_pages(k_pages, kv_heads, q.size(2), "k_pages");
-  const paged::Pages vp = paged::check_pages(v_pages, kv_heads, q.size(2), "v_pages");
-  RC_CHECK(kp.count == vp.count && kp.size == vp.size, "k_pages and v_pages must have the same pages");
-  const paged::Table t = paged::check_table(table, kv_lens, cu_q, q.device());
-  RC_CHECK(window >= 0 && sinks >= 0 && window < (1ll << 31) && sinks < (1ll << 31), "window and sinks must not be negative");
-  RC_CHECK(max_q_len >= 1 && max_q_len < (1ll << 24), "max_q_len must be positive");
-  paged::Args a{};
-  a.q = q.data_ptr();
-  a.q_token = q.stride(0);
-  a.q_head = q.stride(1);
-  a.out = out.data_ptr();
-  a.out_token = out.stride(0);
-  a.out_head = out.stride(1);
-  if (lse.has_value()) {
-    RC_CHECK(lse->scalar_type() == at::kFloat && lse->is_contiguous() && lse->device() == q.device() && lse->dim() == 2 &&
-                 lse->size(0) == q.size(0) && lse->size(1) == q.size(1),
-             "lse must be a contiguous float32 [tokens, heads]");
-    a.lse = lse->data_ptr<float>();
-  }
-  a.table = t.table;
-  a.kv_lens = t.kv_lens;
-  a.cu_q = t.cu_q;
-  a.seqs = t.seqs;
-  a.width = t.width;
-  a.pages = kp.count;
-  a.heads = static_cast<int>(q.size(1));
-  a.kv_heads = static_cast<int>(kv_heads);
-  a.group = a.heads / a.kv_heads;
-  a.causal = causal;
-  a.window = static_cast<int>(window);
-  a.sinks = window > 0 ? static_cast<int>(sinks) : 0;
-  a.tokens = static_cast<int>(q.size(0));
-  a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
-  a.tiling.page = kp.size;
-  a.status = status_ptr(status);
-  if (a.tokens == 0 || a.seqs == 0) return;
-  c10::cuda::CUDAGuard guard(q.device());
-  const int device = q.get_device();
-  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device).stream();
-  paged::attend_short(a, static_cast<int>(q.size(2)), type == at::kHalf, k_pages, v_pages,
-                      static_cast<int>(std::min<int64_t>(max_q_len, a.tokens)), q, stream, device);
-}
-
 }  // namespace rc

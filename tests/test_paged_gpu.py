@@ -289,6 +289,15 @@ def test_chunks(new, totals, heads, kv_heads, d, page, dtype, causal):
 
 
 @pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("new,totals,heads,kv_heads,d,page", [
+    ([1100], [2000], 40, 40, 64, 64), ([900, 10, 333, 700], [3000, 2100, 333, 800], 20, 4, 128, 16),
+    ([2900], [2900], 24, 8, 64, 32), ([70] * 30, [200 + 90 * i for i in range(30)], 8, 4, 128, 128)])
+def test_more_items_than_sms(new, totals, heads, kv_heads, d, page, causal):
+    """Whole rounds of items and items cut between SMs, with group sizes that do not divide a tile."""
+    _check_attention(new, totals, heads, kv_heads, d, page, BF16, causal=causal)
+
+
+@pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("window,sinks", [(1, 0), (7, 0), (64, 3), (100, 64), (100, 130), (333, 5), (5000, 10)])
 @pytest.mark.parametrize("new,totals,heads,kv_heads,d,page", [
     ([1, 1], [700, 90], 8, 2, 128, 16), ([9], [400], 4, 4, 64, 24), ([150, 33], [900, 33], 4, 2, 128, 32), ([260], [3200], 2, 2, 128, 1560)])
@@ -460,7 +469,7 @@ def test_attention_refusals():
     nine = torch.randn(5, 9, 2, 64, device="cuda").bfloat16()
     for wrong in (dict(q=q.half()), dict(q=q.float()), dict(q=q[:, :3]), dict(k=k_pages[:, :, :1]), dict(k=nine, v=nine),
                   dict(v=v_pages[1:]), dict(t=table.long()), dict(n=kv_lens[:0]), dict(c=cu_q[:1]), dict(t=table.cpu()),
-                  dict(max_q_len=0), dict(sinks=-1, window=5), dict(q=torch.randn(1, 4, 96, device="cuda").bfloat16()),
+                  dict(max_q_len=0), dict(sinks=-1, window=5), dict(scale=0.0), dict(scale=-1.0), dict(q=torch.randn(1, 4, 96, device="cuda").bfloat16()),
                   dict(out=torch.empty(2, 4, 64, device="cuda", dtype=BF16)), dict(k=k_pages[..., ::2])):
         with pytest.raises(RuntimeError):
             call(**wrong)
