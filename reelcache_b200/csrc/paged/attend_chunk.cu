@@ -9,7 +9,8 @@
 // query-major, so grouped heads share the loads of their KV head. 384 threads:
 //   warps 0-3, 4-7  softmax of tile 0, 1: a thread owns a row (TMEM lane). S comes from TMEM, the running maximum moves
 //                   only when it grows by more than 8 (log2; then the row of O is rescaled in TMEM), P goes back to TMEM
-//                   over S, where the P V product reads it as its A operand. The tiles take turns on the exponentials.
+//                   over S, where the P V product reads it as its A operand, in two halves of 64 keys: the
+//                   product over the first runs during the exponentials of the second.
 //   warps 8, 9      TMA: K blocks into a ring of 3, V blocks into a ring of 2. One box per page (or part of it).
 //   warp 10         issues the products, in the order O_0 += P_0 V', S_0 = Q_0 K, O_1 += P_1 V', S_1 = Q_1 K (V' of the
 //                   block before), without a break between one item and the next.
@@ -50,8 +51,7 @@ constexpr int kSoftmaxRegs = 208;
 constexpr int kRoleRegs = 88;
 static_assert(2 * kSoftmaxRegs + kRoleRegs == 3 * kLaunchRegs, "register split must equal the launch's registers");
 constexpr float kRescale = 8.0f;  // log2 units
-constexpr int kPolyEvery = 4;     // one of so many pairs of exponentials is taken from the FMA pipe
-constexpr int kTurnBarrier = 1;   // named barriers 1 and 2
+constexpr int kPolyEvery = 8;     // one of so many pairs of exponentials is taken from the FMA pipe
 
 template <int D>
 struct ChunkShape {
@@ -301,15 +301,17 @@ __device__ __forceinline__ void exp2_pair(uint64_t x, float& p0, float& p1) {
   p1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
 }
 
-// One row's exponentials: r holds 128 raw scores, comes back as 64 pairs of P in r[.][0 .. 31]; returns their sum.
-template <typename T, int kPoly>
-__device__ __forceinline__ float softmax_row(uint32_t (&r)[2][64], float scale_log2, float neg_m, uint32_t (&pk)[2][32]) {
+// Exponentials of half a row: 64 raw scores become 32 pairs of P; their sum is added to `sum`. kMax: the maximum of the
+// whole row (this half and `other`) is found on the way, two steps of it after every pair.
+template <typename T, int kPoly, bool kMax>
+__device__ __forceinline__ void softmax_half(const uint32_t (&r)[64], const uint32_t (&other)[64], float scale_log2, float neg_m,
+                                             uint32_t (&pk)[32], float& sum, float& top) {
   const uint64_t scale2 = pair(scale_log2, scale_log2), m2 = pair(neg_m, neg_m);
-  uint64_t sums[4] = {0, 0, 0, 0};
+  uint64_t sums[2] = {0, 0};
+  float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-  for (int c = 0; c < 64; ++c) {
-    const int h = c >> 5, e = (c & 31) * 2;
-    const uint64_t x = fma2(pair(__uint_as_float(r[h][e]), __uint_as_float(r[h][e + 1])), scale2, m2);
+  for (int c = 0; c < 32; ++c) {
+    const uint64_t x = fma2(pair(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1])), scale2, m2);
     float p0, p1;
     if (kPoly > 0 && c % (kPoly > 0 ? kPoly : 1) == 1) {
       exp2_pair(x, p0, p1);
@@ -318,16 +320,55 @@ __device__ __forceinline__ float softmax_row(uint32_t (&r)[2][64], float scale_l
       p0 = exp2_approx(p0);
       p1 = exp2_approx(p1);
     }
-    sums[c & 3] = add2(sums[c & 3], pair(p0, p1));
-    pk[h][c & 31] = pack2<T>(p0, p1);
+    if (kMax) {
+      m[c & 1] = max3(m[c & 1], __uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]));
+      m[2 + (c & 1)] = max3(m[2 + (c & 1)], __uint_as_float(other[2 * c]), __uint_as_float(other[2 * c + 1]));
+    }
+    sums[c & 1] = add2(sums[c & 1], pair(p0, p1));
+    pk[c] = pack2<T>(p0, p1);
   }
   float a, b;
-  unpair(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])), a, b);
-  return a + b;
+  unpair(add2(sums[0], sums[1]), a, b);
+  sum += a + b;
+  if (kMax) top = fmaxf(max3(m[0], m[1], m[2]), m[3]);
 }
 
-__device__ __forceinline__ void named_sync(int id) { asm volatile("bar.sync %0, 256;" ::"r"(id) : "memory"); }
-__device__ __forceinline__ void named_arrive(int id) { asm volatile("bar.arrive %0, 256;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ float row_max(const uint32_t (&r)[2][64]) {
+  float m[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) m[k] = fmaxf(__uint_as_float(r[0][k]), __uint_as_float(r[1][k]));
+#pragma unroll
+  for (int c = 8; c < 64; c += 8)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) m[k] = max3(m[k], __uint_as_float(r[0][c + k]), __uint_as_float(r[1][c + k]));
+  return max3(max3(m[0], m[1], m[2]), max3(m[3], m[4], m[5]), fmaxf(m[6], m[7]));
+}
+
+// Scores outside [from, high) and [0, sink) of the tile become minus infinity; 16 columns at a time are left alone where
+// no row of the warp has one. kHalf: 0 or 1.
+template <int kHalf>
+__device__ __forceinline__ void mask_half(uint32_t (&r)[64], int from, int high, int sink) {
+#pragma unroll
+  for (int b = 4 * kHalf; b < 4 * kHalf + 4; ++b) {
+    if (__all_sync(0xffffffffu, high >= 16 * b + 16 && (from <= 16 * b || sink >= 16 * b + 16))) continue;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int c = 16 * b + e;
+      if (c >= high || (c < from && c >= sink)) r[c & 63] = __float_as_uint(-INFINITY);
+    }
+  }
+}
+
+// One thread of a converged warp (elect.sync: the compiler then knows that what it issues is uniform).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
 
 // Shared-memory descriptor of an MN-major operand in the 128-byte swizzle: blocks of 64 channels x 8 keys (1,024 bytes),
 // `block_bytes` between the blocks of 64 channels (leading offset), 1,024 bytes between groups of 8 keys (stride offset).
@@ -354,13 +395,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   uint64_t* v_full = k_empty + kKStages;  // [kVStages]
   uint64_t* v_empty = v_full + kVStages;  // [kVStages]
   uint64_t* s_full = v_empty + kVStages;  // [2] per tile
-  uint64_t* p_full = s_full + 2;          // [2]
-  uint64_t* o_done = p_full + 2;          // [2]
-  uint64_t* drained = o_done + 2;
+  uint64_t* p_full = s_full + 2;          // [4] per tile and half of the keys
+  uint64_t* o_done = p_full + 4;          // [2]
+  uint64_t* v_raw = o_done + 2;
+  uint64_t* drained = v_raw + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
   const Args& a = p.a;
   int* status = a.status;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int cta = blockIdx.x;
 
   if (threadIdx.x == 0) {
@@ -376,9 +418,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     }
     for (int g = 0; g < 2; ++g) {
       mbar_init(&s_full[g], 1);
-      mbar_init(&p_full[g], 4);
+      mbar_init(&p_full[2 * g], 4);
+      mbar_init(&p_full[2 * g + 1], 4);
       mbar_init(&o_done[g], 1);
     }
+    mbar_init(v_raw, 1);
     mbar_init(drained, 1);
     fence_barrier_init();
   }
@@ -407,30 +451,50 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       const CUtensorMap* wide = is_k ? &maps.k_wide : &maps.v_wide;
       const CUtensorMap* step = is_k ? &maps.k_step : &maps.v_step;
       int stage = 0;
-      uint32_t phase = 1;
+      uint32_t phase = 1, raw_phase = 0;
       bool ok = true;
       for (int n = 0; ok && seg.load(p, cta, n); ++n) {
         const RowQueries rows(a, seg.item.row_tile, seg.item.q_len);
-        const TileRange<kTile> range(Sight(a, seg.item.kv_len, seg.item.q_len), rows.first, rows.end);
+        const Sight sight(a, seg.item.kv_len, seg.item.q_len);
+        const TileRange<kTile> range(sight, rows.first, rows.end);
+        const int low = sight.low(sight.last(rows.first)), top = min(sight.last(rows.end - 1), seg.item.kv_len - 1);
         const int* table = a.table + static_cast<int64_t>(seg.item.seq) * a.width;
         for (int t = seg.t0; t < seg.t1; ++t) {
           const int first = range.tile(t) * kTile;
           const Boxes<kTile> boxes(a.tiling, first, seg.item.kv_len);
           int row = 0, page = -1;
           if (lane < boxes.count) page = boxes.page(table, a.pages, a.tiling, first, lane, &row, status);
+          // rows of V that no query of the item sees become zeros (0 * NaN is NaN): this warp does it between the copy
+          // and the products, so the block's bytes are counted on a barrier of its own
+          const int from = low - first, high = top + 1 - first, sink = a.sinks - first;
+          const bool clean = !is_k && (high < kTile || (from > 0 && sink < kTile));
+          uint64_t* bar = clean ? v_raw : &full[stage];
           ok = __all_sync(0xffffffffu, mbar_wait_park(&empty[stage], phase, status, kTimeoutProducer));
           if (!ok) break;
           if (lane == 0) {
-            if (boxes.count > 0) mbar_arrive_expect_tx(&full[stage], boxes.count * boxes.rows * 128 * Shape::boxes);
-            else mbar_arrive(&full[stage]);
+            if (boxes.count > 0) mbar_arrive_expect_tx(bar, boxes.count * boxes.rows * 128 * Shape::boxes);
+            else mbar_arrive(bar);
           }
           __syncwarp();
+          uint8_t* tile = ring + stage * Shape::tile_bytes;
           if (lane < boxes.count) {
-            uint8_t* dst = ring + stage * Shape::tile_bytes + lane * boxes.rows * 128;
             const CUtensorMap* map = boxes.rows == kTile ? wide : step;
 #pragma unroll
             for (int b = 0; b < Shape::boxes; ++b)
-              load_page_box(dst + b * Shape::box_bytes, map, &full[stage], b * 64, row, seg.item.head, page);
+              load_page_box(tile + lane * boxes.rows * 128 + b * Shape::box_bytes, map, bar, b * 64, row, seg.item.head, page);
+          }
+          if (clean) {
+            ok = __all_sync(0xffffffffu, mbar_wait_park(v_raw, raw_phase, status, kTimeoutProducer));
+            if (!ok) break;
+            raw_phase ^= 1;
+            for (int i = lane; i < kTile * Shape::boxes * 8; i += 32) {
+              const int r = i / (Shape::boxes * 8), c = i % (Shape::boxes * 8);
+              if (r >= high || (r < from && r >= sink))
+                *reinterpret_cast<uint4*>(tile + (c >> 3) * Shape::box_bytes + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[stage]);
           }
           if (++stage == stages) {
             stage = 0;
@@ -466,111 +530,88 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         mbar_arrive(q_full);
       }
     } else {
-      // ---------------- products: the whole warp keeps step, lane 0 issues ----------------
-      constexpr uint32_t kFormat = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-      constexpr uint32_t idesc_s = make_idesc_f16(kTile, kTile, kFormat);
-      constexpr uint32_t idesc_o = make_idesc_f16(kTile, D, kFormat) | (1u << 16);  // B is MN-major
-      const uint32_t qa = smem_u32(smem + Shape::q_off);
-      bool ok = true;
-      int it = 0;  // blocks so far
-      int k_stage = 0, v_stage = 0;
-      uint32_t k_phase = 0, v_phase = 0;
-      // of the block before: whether it begins, ends its segment; V rows that no row sees: those outside [v_low, v_high)
-      // but for the first v_sink
-      bool was_first = false, was_last = false;
-      int v_low = 0, v_high = kTile, v_sink = 0;
-      auto wait = [&](uint64_t* bar, uint32_t parity) {
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait_park(bar, parity, status, kTimeoutMma));
-      };
-      auto issue_s = [&](int g) {
-        if (!ok || lane != 0) return;
-        const uint32_t ka = smem_u32(smem + Shape::k_off + k_stage * Shape::tile_bytes);
-        const uint32_t qg = qa + g * Shape::tile_bytes;
+      // ---------------- products ----------------
+      // One thread issues everything; per block it has 32 instructions to get out, so descriptors are built once per
+      // operand tile and stepped by constants (the start address is in units of 16 bytes and never carries).
+      if (elect_one()) {
+        constexpr uint32_t kFormat = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+        constexpr uint32_t idesc_s = make_idesc_f16(kTile, kTile, kFormat);
+        constexpr uint32_t idesc_o = make_idesc_f16(kTile, D, kFormat) | (1u << 16);  // B is MN-major
+        const uint64_t q_desc = sw128_kmajor_desc(smem_u32(smem + Shape::q_off));
+        const uint64_t k_desc = sw128_kmajor_desc(smem_u32(smem + Shape::k_off));
+        const uint64_t v_desc = sw128_mnmajor_desc(smem_u32(smem + Shape::v_off), Shape::box_bytes);
+        bool ok = true;
+        int it = 0;  // blocks so far
+        int k_stage = 0, v_stage = 0;
+        uint32_t k_phase = 0, v_phase = 0;
+        bool was_first = false, was_last = false;  // the block before: whether it begins, ends its segment
+        auto issue_s = [&](int g) {
+          if (!ok) return;
+          const uint64_t ka = k_desc + k_stage * (Shape::tile_bytes >> 4), qg = q_desc + g * (Shape::tile_bytes >> 4);
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t box = (kk >> 2) * Shape::box_bytes;
-          mma_f16(tmem_base + g * kTile, sw128_kmajor_desc(qg + box) + 2 * (kk & 3), sw128_kmajor_desc(ka + box) + 2 * (kk & 3),
-                  idesc_s, kk > 0 ? 1u : 0u);
-        }
-        mma_commit(&s_full[g]);
-      };
-      auto issue_pv = [&](int g) {  // the block before
-        wait(&p_full[g], (it - 1) & 1);
-        if (!ok) return;
-        tc_fence_after();
-        if (lane != 0) return;
-        const uint32_t va = smem_u32(smem + Shape::v_off + v_stage * Shape::tile_bytes);
+          for (int kk = 0; kk < D / 16; ++kk) {
+            constexpr uint32_t kBox = Shape::box_bytes >> 4;
+            mma_f16(tmem_base + g * kTile, qg + (kk >> 2) * kBox + 2 * (kk & 3), ka + (kk >> 2) * kBox + 2 * (kk & 3), idesc_s,
+                    kk > 0 ? 1u : 0u);
+          }
+          mma_commit(&s_full[g]);
+        };
+        auto issue_pv = [&](int g) {  // the block before, each half of its keys as soon as its P is there
+          const uint64_t va = v_desc + v_stage * (Shape::tile_bytes >> 4);
 #pragma unroll
-        for (int kk = 0; kk < kTile / 16; ++kk)
-          mma_f16_ts(tmem_base + 256 + g * kTile, tmem_base + g * kTile + kk * 8,
-                     sw128_mnmajor_desc(va + kk * 16 * 128, Shape::box_bytes), idesc_o, (!was_first || kk > 0) ? 1u : 0u);
-        if (was_last) mma_commit(&o_done[g]);
-      };
-      auto take_v = [&]() {  // V of the block before has come; what no row sees of it becomes zeros (0 * NaN is NaN)
-        wait(&v_full[v_stage], v_phase);
-        if (ok && (v_low > 0 || v_high < kTile)) {
-          uint8_t* v = smem + Shape::v_off + v_stage * Shape::tile_bytes;
-          for (int r = 0; r < kTile; ++r) {
-            if ((r >= v_low || r < v_sink) && r < v_high) continue;
-            for (int c = lane; c < Shape::boxes * 8; c += 32)
-              *reinterpret_cast<uint4*>(v + (c >> 3) * Shape::box_bytes + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+          for (int half = 0; half < 2; ++half) {
+            if (ok) ok = mbar_wait_park(&p_full[2 * g + half], (it - 1) & 1, status, kTimeoutMma);
+            if (!ok) return;
+            tc_fence_after();
+#pragma unroll
+            for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
+              mma_f16_ts(tmem_base + 256 + g * kTile, tmem_base + g * kTile + kk * 8, va + kk * (16 * 128 >> 4), idesc_o,
+                         kk > 0 || !was_first ? 1u : 0u);
           }
-          fence_proxy_async_smem();
-          __syncwarp();
+          if (was_last) mma_commit(&o_done[g]);
+        };
+        auto done_v = [&]() {
+          if (ok) mma_commit(&v_empty[v_stage]);
+          if (++v_stage == kVStages) {
+            v_stage = 0;
+            v_phase ^= 1;
+          }
+        };
+        for (int n = 0; ok && seg.load(p, cta, n); ++n) {
+          for (int t = seg.t0; t < seg.t1 && ok; ++t) {
+            // everything that can be waited for ahead of P is
+            ok = mbar_wait_park(&k_full[k_stage], k_phase, status, kTimeoutMma);
+            if (it > 0) {
+              if (ok) ok = mbar_wait_park(&v_full[v_stage], v_phase, status, kTimeoutMma);
+              issue_pv(0);
+            }
+            if (ok && t == seg.t0) ok = mbar_wait_park(q_full, n & 1, status, kTimeoutMma);
+            tc_fence_after();
+            issue_s(0);
+            if (it > 0) {
+              issue_pv(1);
+              done_v();
+            }
+            issue_s(1);
+            if (ok) {
+              mma_commit(&k_empty[k_stage]);
+              if (t + 1 == seg.t1) mma_commit(q_empty);
+            }
+            if (++k_stage == kKStages) {
+              k_stage = 0;
+              k_phase ^= 1;
+            }
+            ++it;
+            was_first = t == seg.t0;
+            was_last = t + 1 == seg.t1;
+          }
         }
-      };
-      auto done_v = [&]() {
-        if (ok && lane == 0) mma_commit(&v_empty[v_stage]);
-        if (++v_stage == kVStages) {
-          v_stage = 0;
-          v_phase ^= 1;
+        if (it > 0) {
+          if (ok) ok = mbar_wait_park(&v_full[v_stage], v_phase, status, kTimeoutMma);
+          issue_pv(0);
+          issue_pv(1);
+          done_v();
         }
-      };
-      for (int n = 0; ok && seg.load(p, cta, n); ++n) {
-        const RowQueries rows(a, seg.item.row_tile, seg.item.q_len);
-        const Sight sight(a, seg.item.kv_len, seg.item.q_len);
-        const TileRange<kTile> range(sight, rows.first, rows.end);
-        const int low = sight.low(sight.last(rows.first)), top = min(sight.last(rows.end - 1), seg.item.kv_len - 1);
-        for (int t = seg.t0; t < seg.t1 && ok; ++t) {
-          if (it > 0) {
-            take_v();
-            issue_pv(0);
-          }
-          if (t == seg.t0) wait(q_full, n & 1);
-          wait(&k_full[k_stage], k_phase);
-          tc_fence_after();
-          issue_s(0);
-          if (it > 0) {
-            issue_pv(1);
-            done_v();
-          }
-          issue_s(1);
-          if (ok && lane == 0) {
-            mma_commit(&k_empty[k_stage]);
-            if (t + 1 == seg.t1) mma_commit(q_empty);
-          }
-          if (++k_stage == kKStages) {
-            k_stage = 0;
-            k_phase ^= 1;
-          }
-          ++it;
-          was_first = t == seg.t0;
-          was_last = t + 1 == seg.t1;
-          const int first = range.tile(t) * kTile;
-          v_low = low - first;
-          v_high = min(kTile, top + 1 - first);
-          v_sink = a.sinks - first;
-          if (v_sink >= kTile) v_low = 0;
-        }
-      }
-      if (it > 0) {
-        take_v();
-        issue_pv(0);
-        issue_pv(1);
-        done_v();
-      }
-      __syncwarp();
-      if (lane == 0) {
         mma_commit(drained);
         (void)mbar_wait_park(drained, 0, nullptr, 0);
       }
@@ -584,12 +625,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t s_col = tmem_base + g * kTile + lanes;
     const uint32_t o_col = tmem_base + 256 + g * kTile + lanes;
-    // Turns: warpgroup g runs the exponentials of a block after the other has run those of its last one. Every warp takes
-    // every turn, also after a failed wait, so none is left waiting.
-    if (g == 1) named_arrive(kTurnBarrier);
     bool ok = true;
     int it = 0;
-    for (int n = 0; seg.load(p, cta, n); ++n) {
+    for (int n = 0; ok && seg.load(p, cta, n); ++n) {
       const int packed = seg.item.row_tile * kItemRows + g * kTile + row;
       const int query = packed / a.group;
       const Sight sight(a, seg.item.kv_len, seg.item.q_len);
@@ -598,77 +636,64 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       const int last = min(sight.last(min(query, seg.item.q_len - 1)), seg.item.kv_len - 1);
       const int low = sight.low(last);
       float m_run = -INFINITY, l_run = 0.0f;  // of scale * log2(e) * s
-      for (int t = seg.t0; t < seg.t1; ++t, ++it) {
-        uint32_t r[2][64];
-        float mx = -INFINITY;
-        bool whole = true;
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait_park(&s_full[g], it & 1, status, kTimeoutEpilogue));
-        if (ok) {
-          tc_fence_after();
+      for (int t = seg.t0; t < seg.t1 && ok; ++t, ++it) {
+        uint32_t r[2][64], pk[32];
+        ok = __all_sync(0xffffffffu, mbar_wait_park(&s_full[g], it & 1, status, kTimeoutEpilogue));
+        if (!ok) break;
+        tc_fence_after();
+        tmem_ld_32x32b_x64(s_col, r[0]);
+        tmem_ld_32x32b_x64(s_col + 64, r[1]);
+        tmem_wait_ld();
+        const int first = range.tile(t) * kTile;
+        const int high = last + 1 - first, from = low - first, sink = a.sinks - first;  // sees [from, high), [0, sink)
+        const bool whole = __all_sync(0xffffffffu, high >= kTile && (from <= 0 || sink >= kTile));
+        if (!whole) {
+          mask_half<0>(r[0], from, high, sink);
+          mask_half<1>(r[1], from, high, sink);
+        }
+        // The exponentials start with the maximum so far, and this block's is found next to them (they leave issue slots
+        // for it). Only where it has grown by more than kRescale are they done again.
+        if (t == seg.t0) m_run = row_max(r) * a.scale_log2;
+        float neg_m = m_run == -INFINITY ? 0.0f : -m_run;  // a row that has seen no key yet
+        float sum = 0.0f, mx;
+        if (whole) softmax_half<T, kPolyEvery, true>(r[0], r[1], a.scale_log2, neg_m, pk, sum, mx);
+        else softmax_half<T, 0, true>(r[0], r[1], a.scale_log2, neg_m, pk, sum, mx);
+        mx *= a.scale_log2;
+        const bool need = mx > m_run + kRescale;
+        if (__any_sync(0xffffffffu, need)) {
+          // O_g holds the blocks before this one: their products were issued before this block's S
+          const float alpha = need ? exp2_approx(m_run - mx) : 1.0f;
+#pragma unroll
+          for (int c = 0; c < D; c += 16) {
+            uint32_t o[16];
+            tmem_ld_32x32b_x16(o_col + c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st_32x32b_x16(o_col + c, o);
+          }
+          l_run *= alpha;
+          if (need) m_run = mx;
+          neg_m = m_run == -INFINITY ? 0.0f : -m_run;
           tmem_ld_32x32b_x64(s_col, r[0]);
-          tmem_ld_32x32b_x64(s_col + 64, r[1]);
           tmem_wait_ld();
-          const int first = range.tile(t) * kTile;
-          const int high = last + 1 - first, from = low - first, sink = a.sinks - first;  // sees [from, high), [0, sink)
-          whole = __all_sync(0xffffffffu, high >= kTile && (from <= 0 || sink >= kTile));
-          if (!whole) {
-#pragma unroll
-            for (int b = 0; b < 8; ++b) {
-              if (__all_sync(0xffffffffu, high >= 16 * b + 16 && (from <= 16 * b || sink >= 16 * b + 16))) continue;
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                const int c = 16 * b + e;
-                if (c >= high || (c < from && c >= sink)) r[c >> 6][c & 63] = __float_as_uint(-INFINITY);
-              }
-            }
-          }
-          float pm[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) pm[k] = __uint_as_float(r[0][k]);
-#pragma unroll
-          for (int c = 8; c < kTile - 8; c += 16)
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              pm[k] = max3(pm[k], __uint_as_float(r[(c + k) >> 6][(c + k) & 63]), __uint_as_float(r[(c + 8 + k) >> 6][(c + 8 + k) & 63]));
-#pragma unroll
-          for (int k = 0; k < 8; ++k) pm[k] = fmaxf(pm[k], __uint_as_float(r[1][56 + k]));
-          mx = max3(max3(pm[0], pm[1], pm[2]), max3(pm[3], pm[4], pm[5]), fmaxf(pm[6], pm[7])) * a.scale_log2;
+          if (!whole) mask_half<0>(r[0], from, high, sink);
+          sum = 0.0f;
+          softmax_half<T, 0, false>(r[0], r[1], a.scale_log2, neg_m, pk, sum, mx);
         }
-        named_sync(kTurnBarrier + g);
-        if (ok) {
-          if (t == seg.t0) {
-            m_run = mx;
-          } else {
-            // O_g holds the blocks before this one: their products were issued before this block's S
-            const bool need = mx > m_run + kRescale;
-            if (__any_sync(0xffffffffu, need)) {
-              const float alpha = need ? exp2_approx(m_run - mx) : 1.0f;
-#pragma unroll
-              for (int c = 0; c < D; c += 16) {
-                uint32_t o[16];
-                tmem_ld_32x32b_x16(o_col + c, o);
-                tmem_wait_ld();
-#pragma unroll
-                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-                tmem_st_32x32b_x16(o_col + c, o);
-              }
-              l_run *= alpha;
-              if (need) m_run = mx;
-            }
-          }
-          const float neg_m = m_run == -INFINITY ? 0.0f : -m_run;  // a row that has seen no key yet
-          uint32_t pk[2][32];
-          l_run += whole ? softmax_row<T, kPolyEvery>(r, a.scale_log2, neg_m, pk) : softmax_row<T, 0>(r, a.scale_log2, neg_m, pk);
-          tmem_st_32x32b_x32(s_col, pk[0]);
-          tmem_st_32x32b_x32(s_col + 32, pk[1]);
-        }
-        named_arrive(kTurnBarrier + 1 - g);
-        if (ok) {
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[g]);
-        }
+        tmem_st_32x32b_x32(s_col, pk);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[2 * g]);
+        if (whole) softmax_half<T, kPolyEvery, false>(r[1], r[0], a.scale_log2, neg_m, pk, sum, mx);
+        else softmax_half<T, 0, false>(r[1], r[0], a.scale_log2, neg_m, pk, sum, mx);
+        l_run += sum;
+        tmem_st_32x32b_x32(s_col + 32, pk);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[2 * g + 1]);
       }
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait_park(&o_done[g], n & 1, status, kTimeoutEpilogue));
       if (ok) {
@@ -707,7 +732,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         if (valid && !whole) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(m_run, l_run);
       }
     }
-    if (g == 0) named_sync(kTurnBarrier);  // the other warpgroup's last turn
   }
 
   tc_fence_before();
