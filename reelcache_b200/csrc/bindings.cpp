@@ -2,7 +2,11 @@
 // host fast paths).
 #include <torch/extension.h>
 
+#include <memory>
+#include <utility>
 #include <vector>
+
+#include "paged/rope_plan.h"
 
 namespace rc {
 int64_t pread_many(const std::vector<std::string>& paths, const std::vector<int64_t>& offsets,
@@ -56,17 +60,17 @@ void nvls_reduce_upper(int64_t mc_ptr, int64_t buffer_elems, const at::Tensor& o
 void gram_reduce_scatter(const at::Tensor& xt, int64_t matrices, const std::vector<at::Tensor>& partials,
                          const at::Tensor& owners, const at::Tensor& slots, int64_t rank,
                          const c10::optional<at::Tensor>& status, bool to_local);
-std::vector<at::Tensor> rotate(const at::Tensor& q, const c10::optional<at::Tensor>& k, const at::Tensor& positions,
-                               const at::Tensor& turns, const std::vector<int64_t>& sections, bool halves);
-void paged_append(const at::Tensor& q, at::Tensor& q_out, const at::Tensor& k, const at::Tensor& v,
-                  const c10::optional<at::Tensor>& positions, const c10::optional<at::Tensor>& turns,
-                  const std::vector<int64_t>& sections, bool halves, at::Tensor& k_pages, at::Tensor& v_pages,
-                  const at::Tensor& table, const at::Tensor& kv_lens, const at::Tensor& cu_q,
-                  const c10::optional<at::Tensor>& status);
-void paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
-                     const at::Tensor& kv_lens, const at::Tensor& cu_q, at::Tensor& out,
-                     const c10::optional<at::Tensor>& lse, int64_t max_q_len, bool causal, int64_t window, int64_t sinks,
-                     double scale, const c10::optional<at::Tensor>& status);
+std::pair<at::Tensor, c10::optional<at::Tensor>> rotate(const at::Tensor& q, const c10::optional<at::Tensor>& k,
+                                                        const at::Tensor& positions, std::shared_ptr<RopePlan> plan);
+at::Tensor paged_append(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& positions,
+                        const RopePlan& plan, at::Tensor& k_pages, at::Tensor& v_pages, const at::Tensor& table,
+                        const at::Tensor& kv_lens, const at::Tensor& cu_q, const c10::optional<at::Tensor>& out,
+                        const c10::optional<at::Tensor>& status);
+std::pair<at::Tensor, c10::optional<at::Tensor>> paged_attention(
+    const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
+    const at::Tensor& kv_lens, const at::Tensor& cu_q, int64_t max_q_len, bool causal, int64_t window, int64_t sinks,
+    c10::optional<double> scale, bool want_lse, const c10::optional<at::Tensor>& out_given,
+    const c10::optional<at::Tensor>& status);
 void pages_allocate(at::Tensor& refcount, at::Tensor& lens, at::Tensor& table, int64_t page_size, const at::Tensor& seqs,
                     const at::Tensor& new_lens, const c10::optional<at::Tensor>& status);
 void pages_fork(at::Tensor& refcount, at::Tensor& lens, at::Tensor& table, int64_t page_size, const at::Tensor& parents,
@@ -153,16 +157,19 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("canvas"), py::arg("geometry"));
   m.def("dot2_gemm", &rc::dot2_gemm, "compensated FP32 GEMM out = x @ rows^T", py::arg("x"), py::arg("rows"),
         py::arg("out"));
+  py::class_<rc::RopePlan, std::shared_ptr<rc::RopePlan>>(m, "RopePlan", "a multi-axis rotation's table on one device")
+      .def(py::init<const at::Tensor&, const std::vector<int64_t>&, bool>(), py::arg("turns"), py::arg("sections"),
+           py::arg("halves"))
+      .def_readonly("turns", &rc::RopePlan::turns);
   m.def("rotate", &rc::rotate, "multi-axis rotary positions of q and k (differentiable)", py::arg("q"), py::arg("k"),
-        py::arg("positions"), py::arg("turns"), py::arg("sections"), py::arg("halves"));
-  m.def("paged_append", &rc::paged_append, "rotate q, write rotated k and v into their pages", py::arg("q"),
-        py::arg("q_out"), py::arg("k"), py::arg("v"), py::arg("positions"), py::arg("turns"), py::arg("sections"),
-        py::arg("halves"), py::arg("k_pages"), py::arg("v_pages"), py::arg("table"), py::arg("kv_lens"), py::arg("cu_q"),
-        py::arg("status") = py::none());
+        py::arg("positions"), py::arg("plan"));
+  m.def("paged_append", &rc::paged_append, "rotate q, write rotated k and v into their pages", py::arg("q"), py::arg("k"),
+        py::arg("v"), py::arg("positions"), py::arg("plan"), py::arg("k_pages"), py::arg("v_pages"), py::arg("table"),
+        py::arg("kv_lens"), py::arg("cu_q"), py::arg("out"), py::arg("status"));
   m.def("paged_attention", &rc::paged_attention, "attention of new tokens over a paged KV cache", py::arg("q"),
-        py::arg("k_pages"), py::arg("v_pages"), py::arg("table"), py::arg("kv_lens"), py::arg("cu_q"), py::arg("out"),
-        py::arg("lse"), py::arg("max_q_len"), py::arg("causal"), py::arg("window"), py::arg("sinks"), py::arg("scale"),
-        py::arg("status") = py::none());
+        py::arg("k_pages"), py::arg("v_pages"), py::arg("table"), py::arg("kv_lens"), py::arg("cu_q"),
+        py::arg("max_q_len"), py::arg("causal"), py::arg("window"), py::arg("sinks"), py::arg("scale"),
+        py::arg("want_lse"), py::arg("out"), py::arg("status"));
   m.def("pages_allocate", &rc::pages_allocate, "grow sequences of a page table", py::arg("refcount"), py::arg("lens"),
         py::arg("table"), py::arg("page_size"), py::arg("seqs"), py::arg("new_lens"), py::arg("status") = py::none());
   m.def("pages_fork", &rc::pages_fork, "share pages with forked sequences, copy partial tails", py::arg("refcount"),

@@ -3,10 +3,13 @@
 // Few query rows (new tokens x heads of a group) cannot fill the 128-row products of tcgen05, and reading K and V bounds
 // them anyway: they take the streaming kernel of attend_short.cu. More rows take attend_chunk.cu.
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
 #include <algorithm>
+#include <cmath>
+#include <utility>
 
 #include "attend.cuh"
 
@@ -24,15 +27,21 @@ void attend_chunk(const Args& a, int head_dim, bool half, const at::Tensor& k_pa
 
 // out = softmax over the visible keys of scale * q k^T, times v, for the new tokens of every sequence; lse its natural
 // log-sum-exp. max_q_len bounds every sequence's new tokens; tokens past a sequence's bound are left alone.
-void paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
-                     const at::Tensor& kv_lens, const at::Tensor& cu_q, at::Tensor& out,
-                     const c10::optional<at::Tensor>& lse, int64_t max_q_len, bool causal, int64_t window, int64_t sinks,
-                     double scale, const c10::optional<at::Tensor>& status) {
+std::pair<at::Tensor, c10::optional<at::Tensor>> paged_attention(
+    const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
+    const at::Tensor& kv_lens, const at::Tensor& cu_q, int64_t max_q_len, bool causal, int64_t window, int64_t sinks,
+    c10::optional<double> scale_given, bool want_lse, const c10::optional<at::Tensor>& out_given,
+    const c10::optional<at::Tensor>& status) {
   check_cuda_tensor(q, "q");
+  RC_CHECK(!c10::GradMode::is_enabled() || !(q.requires_grad() || k_pages.requires_grad() || v_pages.requires_grad()),
+           "attention over pages has no gradient: call it without grad");
   const at::ScalarType type = q.scalar_type();
   RC_CHECK(type == at::kBFloat16 || type == at::kHalf, "paged attention takes bf16 or fp16");
   RC_CHECK(q.dim() == 3 && (q.size(2) == 64 || q.size(2) == 128), "q must be [tokens, heads, head_dim] with head_dim 64 or 128");
   RC_CHECK(q.size(0) < (1ll << 31), "too many tokens for one launch");
+  c10::cuda::CUDAGuard guard(q.device());
+  const double scale = scale_given.has_value() ? *scale_given : 1.0 / std::sqrt(static_cast<double>(q.size(2)));
+  const at::Tensor out = out_given.has_value() ? *out_given : at::empty(q.sizes(), q.options());
   RC_CHECK(out.sizes() == q.sizes() && out.scalar_type() == type && out.device() == q.device(), "out must match q");
   const at::Tensor* rows[2] = {&q, &out};
   for (const at::Tensor* t : rows)
@@ -58,10 +67,9 @@ void paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::T
   a.out = out.data_ptr();
   a.out_token = out.stride(0);
   a.out_head = out.stride(1);
-  if (lse.has_value()) {
-    RC_CHECK(lse->scalar_type() == at::kFloat && lse->is_contiguous() && lse->device() == q.device() && lse->dim() == 2 &&
-                 lse->size(0) == q.size(0) && lse->size(1) == q.size(1),
-             "lse must be a contiguous float32 [tokens, heads]");
+  c10::optional<at::Tensor> lse;
+  if (want_lse) {
+    lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
     a.lse = lse->data_ptr<float>();
   }
   a.table = t.table;
@@ -80,13 +88,13 @@ void paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::T
   a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
   a.tiling.page = kp.size;
   a.status = status_ptr(status);
-  if (a.tokens == 0 || a.seqs == 0) return;
-  c10::cuda::CUDAGuard guard(q.device());
+  if (a.tokens == 0 || a.seqs == 0) return {out, lse};
   const int device = q.get_device();
   cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device).stream();
   const int most = static_cast<int>(std::min<int64_t>(max_q_len, a.tokens));
   const auto attend = static_cast<int64_t>(most) * a.group <= paged::kShortRows ? paged::attend_short : paged::attend_chunk;
   attend(a, static_cast<int>(q.size(2)), type == at::kHalf, k_pages, v_pages, most, q, stream, device);
+  return {out, lse};
 }
 
 }  // namespace rc

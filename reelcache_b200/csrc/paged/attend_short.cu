@@ -30,6 +30,7 @@ namespace paged {
 constexpr int kShortTile = 64;       // keys of a tile
 constexpr int kShortThreads = 160;   // four consumer warps, one producer warp
 constexpr int kShortCtasPerSm = 2;
+constexpr int kShortLeast = 2;       // tiles of a share, at least: every part costs a pass through the workspace
 
 template <int D>
 struct ShortShape {
@@ -37,8 +38,8 @@ struct ShortShape {
   static constexpr int box_bytes = kShortTile * 128;            // 64 keys x 64 channels
   static constexpr int tile_bytes = boxes * box_bytes;          // one of K, V
   static constexpr int stages = D == 128 ? 3 : 6;
-  static constexpr int join_off = stages * 2 * tile_bytes;      // 16 rows x D of FP32: warps joining their keys
-  static constexpr int join_bytes = 16 * D * 4;
+  static constexpr int join_off = stages * 2 * tile_bytes;      // FP32 rows: warps joining their keys
+  static constexpr int join_bytes = 24 * D * 4;                 // three warps' lower 8 rows, or one warp's 16
   static constexpr int bar_off = join_off + join_bytes;
   static constexpr int bytes = bar_off + 1024 + 1024;           // + alignment slack
   static_assert((bytes + 1024) * kShortCtasPerSm <= 228 * 1024, "two CTAs per SM");
@@ -117,7 +118,7 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + Shape::bar_off);
   uint64_t* empty = full + Shape::stages;
   float* join_ml = reinterpret_cast<float*>(empty + Shape::stages);  // [key groups][rows][maximum, sum]: 64 rows in all
-  int* work = reinterpret_cast<int*>(join_ml + 128);                 // begin, end, sequence, its first place
+  int* work = reinterpret_cast<int*>(join_ml + 128);                 // begin, end, sequence, its first place; warps' sums
   const Args& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -134,49 +135,55 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
     tma_prefetch_desc(&maps.k_wide);
     tma_prefetch_desc(&maps.v_wide);
   }
-  if (warp == 0) {
-    int total = 0;
-    for (int s0 = 0; s0 < a.seqs; s0 += 32) {
-      int n = 0;
-      if (s0 + lane < a.seqs) {
-        const SeqWork w(a, kRows, p.row_tiles, s0 + lane);
-        n = w.tiles * w.items(a);
+  if (warp < 4) {
+    // Thread i counts the tiles of sequences [i per, i per + per); their prefix sums place the share.
+    const int per = (a.seqs + 127) / 128, s0 = static_cast<int>(threadIdx.x) * per;
+    int mine = 0;
+#pragma unroll 4
+    for (int i = 0; i < per; ++i) {
+      if (s0 + i < a.seqs) {
+        const SeqWork w(a, kRows, p.row_tiles, s0 + i);
+        mine += w.tiles * w.items(a);
       }
+    }
+    int x = mine;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) work[4 + warp] = x;
+    consumers_sync();
+    int before = x - mine, total = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int n = work[4 + i];
+      if (i < warp) before += n;
       total += n;
     }
-    const int share = max(1, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
+    const int ctas = static_cast<int>(gridDim.x);
+    const int share = max(min(kShortLeast, total), (total + ctas - 1) / ctas);
     const int begin = min(total, static_cast<int>(blockIdx.x) * share), end = min(total, begin + share);
-    int base = 0;
-    for (int s0 = 0; s0 < a.seqs; s0 += 32) {
-      int n = 0, t = 0;
-      if (s0 + lane < a.seqs) {
-        const SeqWork w(a, kRows, p.row_tiles, s0 + lane);
-        t = w.tiles;
-        n = w.tiles * w.items(a);
-      }
-      int x = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      const int mine = base + x - n;
-      if (begin < end && begin >= mine && begin < mine + n) {
-        work[2] = s0 + lane;
-        work[3] = mine;
-      }
-      if (blockIdx.x == 0 && s0 + lane < a.seqs) {
-        p.line.first[s0 + lane] = mine;
-        p.line.tiles[s0 + lane] = t;
-      }
-      base += __shfl_sync(0xffffffffu, x, 31);
-    }
-    if (lane == 0) {
+    if (threadIdx.x == 0) {
       work[0] = begin;
       work[1] = end;
       if (blockIdx.x == 0) *p.line.share = share;
+    }
+    const bool here = begin < end && begin >= before && begin < before + mine;
+    if (here || blockIdx.x == 0) {
+      for (int i = 0; i < per && s0 + i < a.seqs; ++i) {
+        const SeqWork w(a, kRows, p.row_tiles, s0 + i);
+        const int n = w.tiles * w.items(a);
+        if (here && begin >= before && begin < before + n) {
+          work[2] = s0 + i;
+          work[3] = before;
+        }
+        if (blockIdx.x == 0) {
+          p.line.first[s0 + i] = before;
+          p.line.tiles[s0 + i] = w.tiles;
+        }
+        before += n;
+      }
     }
   }
   __syncthreads();
@@ -269,6 +276,7 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
         q[k][i + 2] = valid[i] ? __ldg(reinterpret_cast<const uint32_t*>(src + k * 16 + 8)) : 0u;
       }
     }
+    const int rows_here = w.q_len * a.group - row_tile * kRows;  // of the row tile (or more)
     // bounds over the row tile's queries, for tiles that need no mask
     const int q_first = row_tile * kRows / a.group;
     const int q_last = min(w.q_len - 1, (row_tile * kRows + kRows - 1) / a.group);
@@ -430,32 +438,53 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
         o[i][2] *= w_o[1];
         o[i][3] *= w_o[1];
       }
-      constexpr int kBlock = D / 8 / kM;  // n-tiles that fit at a time
-      float4* buf = reinterpret_cast<float4*>(smem + Shape::join_off) + mt * kBlock * 32 + lane;
+      if (kM == 1 && rows_here <= 8) {
+        // only the first 8 rows hold anything: all warps at once
+        float2* buf = reinterpret_cast<float2*>(smem + Shape::join_off) + lane;
+        if (kg > 0) {
 #pragma unroll
-      for (int g = 1; g < kGroups; ++g) {
+          for (int i = 0; i < D / 8; ++i) buf[((kg - 1) * (D / 8) + i) * 32] = make_float2(o[i][0], o[i][1]);
+        }
+        consumers_sync();
+        if (kg == 0) {
 #pragma unroll
-        for (int c = 0; c < kM; ++c) {
-          if (kg == g) {
+          for (int g = 0; g < kGroups - 1; ++g)
 #pragma unroll
-            for (int i = 0; i < kBlock; ++i) {
-              const float(&x)[4] = o[c * kBlock + i];
-              buf[i * 32] = make_float4(x[0], x[1], x[2], x[3]);
+            for (int i = 0; i < D / 8; ++i) {
+              const float2 x = buf[(g * (D / 8) + i) * 32];
+              o[i][0] += x.x;
+              o[i][1] += x.y;
             }
-          }
-          consumers_sync();
-          if (kg == 0) {
+        }
+        consumers_sync();
+      } else {
+        constexpr int kBlock = D / 8 / kM;  // n-tiles that fit at a time
+        float4* buf = reinterpret_cast<float4*>(smem + Shape::join_off) + mt * kBlock * 32 + lane;
 #pragma unroll
-            for (int i = 0; i < kBlock; ++i) {
-              const float4 x = buf[i * 32];
-              float(&y)[4] = o[c * kBlock + i];
-              y[0] += x.x;
-              y[1] += x.y;
-              y[2] += x.z;
-              y[3] += x.w;
+        for (int g = 1; g < kGroups; ++g) {
+#pragma unroll
+          for (int c = 0; c < kM; ++c) {
+            if (kg == g) {
+#pragma unroll
+              for (int i = 0; i < kBlock; ++i) {
+                const float(&x)[4] = o[c * kBlock + i];
+                buf[i * 32] = make_float4(x[0], x[1], x[2], x[3]);
+              }
             }
+            consumers_sync();
+            if (kg == 0) {
+#pragma unroll
+              for (int i = 0; i < kBlock; ++i) {
+                const float4 x = buf[i * 32];
+                float(&y)[4] = o[c * kBlock + i];
+                y[0] += x.x;
+                y[1] += x.y;
+                y[2] += x.z;
+                y[3] += x.w;
+              }
+            }
+            consumers_sync();
           }
-          consumers_sync();
         }
       }
     }
@@ -511,23 +540,39 @@ __global__ void __launch_bounds__(128) short_join_kernel(const __grid_constant__
   const int begin = p.line.first[s] + item * w.tiles, end = begin + w.tiles;
   const int c0 = begin / share, c1 = (end - 1) / share;
   if (c0 == c1) return;
-  float top = -INFINITY;
-  for (int c = c0; c <= c1; ++c) top = fmaxf(top, p.part_ml[((2 * static_cast<int64_t>(c) + (c == c0)) * p.rows + row) * 2]);
-  const float use = top == -INFINITY ? 0.0f : top;
-  float acc[kPer], sum = 0.0f;
+  // 32 parts at a time, a lane to each one's maximum and sum
+  float top = -INFINITY, acc[kPer], sum = 0.0f;
 #pragma unroll
   for (int e = 0; e < kPer; ++e) acc[e] = 0.0f;
-#pragma unroll 4
-  for (int c = c0; c <= c1; ++c) {
-    const int64_t slot = (2 * static_cast<int64_t>(c) + (c == c0)) * p.rows + row;
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot * 2);
-    const float wt = exp2_approx(ml.x - use);
-    sum = fmaf(wt, ml.y, sum);
+  for (int cb = c0; cb <= c1; cb += 32) {
+    const int n = min(32, c1 - cb + 1);
+    const int64_t first_slot = (2 * static_cast<int64_t>(cb) + (cb == c0)) * p.rows + row;
+    const int64_t slot = (2 * static_cast<int64_t>(cb + lane) + (cb + lane == c0)) * p.rows + row;
+    float2 ml = make_float2(-INFINITY, 0.0f);
+    if (lane < n) ml = *reinterpret_cast<const float2*>(p.part_ml + slot * 2);
+    float mx = ml.x;
 #pragma unroll
-    for (int e = 0; e < kPer; e += 2) {
-      const float2 x = *reinterpret_cast<const float2*>(p.part_o + slot * D + lane * kPer + e);
-      acc[e] = fmaf(wt, x.x, acc[e]);
-      acc[e + 1] = fmaf(wt, x.y, acc[e + 1]);
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    mx = fmaxf(mx, top);
+    const float use = mx == -INFINITY ? 0.0f : mx;
+    const float old = exp2_approx(top - use), wt = exp2_approx(ml.x - use);
+    top = mx;
+    float part = wt * ml.y;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+    sum = fmaf(sum, old, part);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) acc[e] *= old;
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) {
+      const float weight = __shfl_sync(0xffffffffu, wt, i);
+      const int64_t at = i == 0 ? first_slot : 2 * static_cast<int64_t>(cb + i) * p.rows + row;
+#pragma unroll
+      for (int e = 0; e < kPer; e += 2) {
+        const float2 x = *reinterpret_cast<const float2*>(p.part_o + at * D + lane * kPer + e);
+        acc[e] = fmaf(weight, x.x, acc[e]);
+        acc[e + 1] = fmaf(weight, x.y, acc[e + 1]);
+      }
     }
   }
   const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;

@@ -15,6 +15,7 @@
 // covers whole 256-byte head rows. The fused form writes k and v through the block table, so the rotated keys never
 // exist outside the cache.
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda_bf16.h>
@@ -22,6 +23,7 @@
 
 #include "../common/host.h"
 #include "paged.h"
+#include "rope_plan.h"
 
 namespace rc {
 namespace rotary {
@@ -284,31 +286,27 @@ void dispatch(const Args& a, at::ScalarType type, bool halves, cudaStream_t stre
   }
 }
 
-// The rotation's part of the arguments, checked: positions [tokens, axes], turns [2, pairs], sections.
-void set_rotation(Args& a, const at::Tensor& positions, const at::Tensor& turns, const std::vector<int64_t>& sections,
-                  int tokens, int head_dim, const at::Device& device) {
-  const int axes = static_cast<int>(sections.size());
-  RC_CHECK(axes >= 1 && axes <= 4, "rotary positions have one to four axes");
-  RC_CHECK(head_dim % 16 == 0 && head_dim <= 256, "head_dim must be a multiple of 16, at most 256");
-  a.pairs = head_dim / 2;
+// The rotation's part of the arguments, checked: positions [tokens, axes].
+void set_rotation(Args& a, const at::Tensor& positions, const RopePlan& plan, int64_t tokens, int64_t head_dim,
+                  const at::Device& device) {
+  const int axes = static_cast<int>(plan.sections.size());
+  RC_CHECK(head_dim == 2 * plan.pairs, "the rotation is for another head_dim");
+  RC_CHECK(plan.turns.device() == device, "the rotation's table is on another device");
+  a.pairs = static_cast<int>(plan.pairs);
   int end = 0;
   for (int i = 0; i < 4; ++i) {
-    if (i < axes) end += static_cast<int>(sections[i]);
+    if (i < axes) end += static_cast<int>(plan.sections[i]);
     a.ends[i] = end;
   }
-  RC_CHECK(end == a.pairs, "the axes' sections must add up to head_dim / 2");
   RC_CHECK(positions.device() == device && positions.dim() == 2 && positions.size(0) == tokens &&
                positions.size(1) == axes && positions.is_contiguous() &&
                (positions.scalar_type() == at::kInt || positions.scalar_type() == at::kFloat),
            "positions must be a contiguous int32 or float32 [tokens, axes] tensor on the same device");
-  RC_CHECK(turns.device() == device && turns.scalar_type() == at::kFloat && turns.is_contiguous() &&
-               turns.numel() == 2 * a.pairs,
-           "the rotation's table must be float32 [2, head_dim / 2] on the same device");
   a.positions = positions.data_ptr();
   a.position_float = positions.scalar_type() == at::kFloat;
   a.axes = axes;
-  a.turns = turns.data_ptr<float>();
-  a.tokens = tokens;
+  a.turns = plan.turns.data_ptr<float>();
+  a.tokens = static_cast<int>(tokens);
 }
 
 bool vector_rows(const at::Tensor& t) {
@@ -324,17 +322,16 @@ bool rotary_rows_ok(const at::Tensor& t) { return t.numel() == 0 || rotary::vect
 // out = rotation of x by sign * phi, for up to two tensors [tokens, heads, head_dim] in one launch (either may be
 // undefined, not both).
 void rotate_launch(const at::Tensor& q, at::Tensor& q_out, const at::Tensor& k, at::Tensor& k_out,
-                   const at::Tensor& positions, const at::Tensor& turns, const std::vector<int64_t>& sections,
-                   bool halves, double sign) {
+                   const at::Tensor& positions, const RopePlan& plan, double sign) {
   const at::Tensor& any = q.defined() ? q : k;
   RC_CHECK(any.defined() && any.is_cuda() && any.dim() == 3, "rotate takes CUDA tensors [tokens, heads, head_dim]");
   rotary::Args a{};
-  const int head_dim = static_cast<int>(any.size(2));
+  const int64_t head_dim = any.size(2);
   RC_CHECK(any.size(0) < (1ll << 31), "too many tokens for one launch");
   const int tokens = static_cast<int>(any.size(0));
   const at::ScalarType type = any.scalar_type();
   RC_CHECK(type == at::kBFloat16 || type == at::kHalf || type == at::kFloat, "rotate takes bf16, fp16 or fp32");
-  rotary::set_rotation(a, positions, turns, sections, tokens, head_dim, any.device());
+  rotary::set_rotation(a, positions, plan, tokens, head_dim, any.device());
   const at::Tensor* in[2] = {&q, &k};
   at::Tensor* out[2] = {&q_out, &k_out};
   rotary::Rows* rows[2] = {&a.q, &a.k};
@@ -355,20 +352,23 @@ void rotate_launch(const at::Tensor& q, at::Tensor& q_out, const at::Tensor& k, 
   a.sign = static_cast<float>(sign);
   if (tokens == 0 || a.q.heads + a.k.heads == 0) return;
   c10::cuda::CUDAGuard guard(any.device());
-  rotary::dispatch<false>(a, type, halves, c10::cuda::getCurrentCUDAStream(any.get_device()).stream(),
+  rotary::dispatch<false>(a, type, plan.halves, c10::cuda::getCurrentCUDAStream(any.get_device()).stream(),
                           sm_count(any.get_device()));
 }
 
-// q_out = rotation of q; k rotated and v as it is into their pages: token i of sequence s goes to position
-// kv_lens[s] - (cu_q[s + 1] - cu_q[s]) + i of the sequence.
-void paged_append(const at::Tensor& q, at::Tensor& q_out, const at::Tensor& k, const at::Tensor& v,
-                  const c10::optional<at::Tensor>& positions, const c10::optional<at::Tensor>& turns,
-                  const std::vector<int64_t>& sections, bool halves, at::Tensor& k_pages, at::Tensor& v_pages,
-                  const at::Tensor& table, const at::Tensor& kv_lens, const at::Tensor& cu_q,
-                  const c10::optional<at::Tensor>& status) {
+// Rotation of q (returned; into `out` if it is given); k rotated and v as it is into their pages: token i of sequence s
+// goes to position kv_lens[s] - (cu_q[s + 1] - cu_q[s]) + i of the sequence.
+at::Tensor paged_append(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& positions,
+                        const RopePlan& plan, at::Tensor& k_pages, at::Tensor& v_pages, const at::Tensor& table,
+                        const at::Tensor& kv_lens, const at::Tensor& cu_q, const c10::optional<at::Tensor>& out,
+                        const c10::optional<at::Tensor>& status) {
   check_cuda_tensor(q, "q");
+  RC_CHECK(!c10::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || v.requires_grad()),
+           "append has no gradient: call it without grad");
   const at::ScalarType type = q.scalar_type();
   RC_CHECK(type == at::kBFloat16 || type == at::kHalf, "a paged cache holds bf16 or fp16");
+  c10::cuda::CUDAGuard guard(q.device());
+  at::Tensor q_out = out.has_value() ? *out : at::empty(q.sizes(), q.options());
   RC_CHECK(q.dim() == 3 && k.dim() == 3 && v.sizes() == k.sizes() && k.size(0) == q.size(0) && k.size(2) == q.size(2) &&
                q_out.sizes() == q.sizes(),
            "q is [tokens, heads, head_dim], k and v [tokens, kv_heads, head_dim]");
@@ -384,8 +384,7 @@ void paged_append(const at::Tensor& q, at::Tensor& q_out, const at::Tensor& k, c
   RC_CHECK(kp.count == vp.count && kp.size == vp.size, "k_pages and v_pages must have the same pages");
   rotary::Args a{};
   const int tokens = static_cast<int>(q.size(0));
-  RC_CHECK(turns.has_value() && positions.has_value(), "append needs positions and a rotation");
-  rotary::set_rotation(a, *positions, *turns, sections, tokens, static_cast<int>(q.size(2)), q.device());
+  rotary::set_rotation(a, positions, plan, tokens, q.size(2), q.device());
   a.sign = 1.0f;
   a.q = {static_cast<const char*>(q.data_ptr()), static_cast<char*>(q_out.data_ptr()), q.stride(0) * 2, q.stride(1) * 2,
          q_out.stride(0) * 2, q_out.stride(1) * 2, static_cast<int>(q.size(1))};
@@ -403,9 +402,9 @@ void paged_append(const at::Tensor& q, at::Tensor& q_out, const at::Tensor& k, c
   a.page_k = kp.page_stride * 2;
   a.page_v = vp.page_stride * 2;
   a.status = status_ptr(status);
-  if (tokens == 0 || t.seqs == 0) return;
-  c10::cuda::CUDAGuard guard(q.device());
-  rotary::dispatch<true>(a, type, halves, c10::cuda::getCurrentCUDAStream(q.get_device()).stream(), sm_count(q.get_device()));
+  if (tokens > 0 && t.seqs > 0)
+    rotary::dispatch<true>(a, type, plan.halves, c10::cuda::getCurrentCUDAStream(q.get_device()).stream(), sm_count(q.get_device()));
+  return q_out;
 }
 
 }  // namespace rc

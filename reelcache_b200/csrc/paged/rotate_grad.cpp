@@ -1,70 +1,82 @@
 // The multi-axis rotation as a differentiable function. It is linear and orthogonal, so its gradient is the same
-// rotation turned back, which is again this function (gradients of any order). The node lives in C++ because a training
-// step calls it once per layer on tensors that take a few microseconds: a Python node costs several times that.
+// rotation turned back, which is again this function (gradients of any order). The node is written out in C++ because a
+// training step calls it once per layer on tensors that take a few microseconds: a Python function costs several times
+// that, and a generic C++ one a dictionary per call.
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/extension.h>
 
+#include <memory>
 #include <vector>
+
+#include "rope_plan.h"
 
 namespace rc {
 
 bool rotary_rows_ok(const at::Tensor& t);
 void rotate_launch(const at::Tensor& q, at::Tensor& q_out, const at::Tensor& k, at::Tensor& k_out,
-                   const at::Tensor& positions, const at::Tensor& turns, const std::vector<int64_t>& sections,
-                   bool halves, double sign);
+                   const at::Tensor& positions, const RopePlan& plan, double sign);
 
 namespace {
 
+using torch::autograd::Variable;
+using torch::autograd::variable_list;
+
 at::Tensor dense_rows(const at::Tensor& t) { return !t.defined() || rotary_rows_ok(t) ? t : t.contiguous(); }
 
-// The rotation of one or two tensors (the second may be undefined; then one comes back).
-std::vector<at::Tensor> rotated(const at::Tensor& first, const at::Tensor& second, const at::Tensor& positions,
-                                const at::Tensor& turns, const std::vector<int64_t>& sections, bool halves, double sign) {
-  const at::Tensor x = dense_rows(first), y = dense_rows(second);
-  std::vector<at::Tensor> out = {at::empty(x.sizes(), x.options())};
-  at::Tensor none;
-  if (y.defined()) out.push_back(at::empty(y.sizes(), y.options()));
-  rotate_launch(x, out[0], y, y.defined() ? out[1] : none, positions, turns, sections, halves, sign);
+variable_list turned(const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions,
+                     const std::shared_ptr<RopePlan>& plan, double sign);
+
+struct RotateBackward : public torch::autograd::Node {
+  std::shared_ptr<RopePlan> plan;
+  torch::autograd::SavedVariable positions;
+  double sign = 1.0;
+
+  variable_list apply(variable_list&& grads) override {
+    // an output that was not used has no gradient; an input that needs none gets none
+    at::Tensor q = grads[0], k = grads.size() > 1 ? grads[1] : at::Tensor();
+    if (!task_should_compute_output(0)) q = at::Tensor();
+    if (!task_should_compute_output(1)) k = at::Tensor();
+    if (!q.defined() && !k.defined()) return variable_list(2);
+    const at::Tensor at = positions.unpack();
+    return turned(q, k, at, plan, -sign);
+  }
+  void release_variables() override { positions.reset_data(); }
+  std::string name() const override { return "RotateBackward"; }
+};
+
+variable_list turned(const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions,
+                     const std::shared_ptr<RopePlan>& plan, double sign) {
+  std::shared_ptr<RotateBackward> node;
+  if (torch::autograd::compute_requires_grad(q, k)) {
+    node = std::shared_ptr<RotateBackward>(new RotateBackward(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(q, k));
+    node->plan = plan;
+    node->positions = torch::autograd::SavedVariable(positions, false);
+    node->sign = sign;
+  }
+  variable_list out(2);
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const at::Tensor x = dense_rows(q), y = dense_rows(k);
+    if (x.defined()) out[0] = at::empty(x.sizes(), x.options());
+    if (y.defined()) out[1] = at::empty(y.sizes(), y.options());
+    rotate_launch(x, out[0], y, out[1], positions, *plan, sign);
+  }
+  if (node) {
+    for (at::Tensor& t : out) {
+      if (t.defined()) torch::autograd::set_history(t, node);
+      else node->add_input_metadata(torch::autograd::Node::undefined_input());
+    }
+  }
   return out;
 }
 
-struct Rotate : public torch::autograd::Function<Rotate> {
-  static std::vector<at::Tensor> forward(torch::autograd::AutogradContext* ctx, const at::Tensor& first,
-                                         const c10::optional<at::Tensor>& second, const at::Tensor& positions,
-                                         const at::Tensor& turns, std::vector<int64_t> sections, bool halves,
-                                         double sign) {
-    ctx->set_materialize_grads(false);
-    ctx->save_for_backward({positions, turns});
-    ctx->saved_data["sections"] = sections;
-    ctx->saved_data["halves"] = halves;
-    ctx->saved_data["sign"] = sign;
-    return rotated(first, second.value_or(at::Tensor()), positions, turns, sections, halves, sign);
-  }
-
-  static std::vector<at::Tensor> backward(torch::autograd::AutogradContext* ctx, std::vector<at::Tensor> grads) {
-    const auto saved = ctx->get_saved_variables();
-    const std::vector<int64_t> sections = ctx->saved_data["sections"].toIntVector();
-    const bool halves = ctx->saved_data["halves"].toBool();
-    const double sign = -ctx->saved_data["sign"].toDouble();
-    std::vector<at::Tensor> out(7);  // one per input; only the rotated tensors have a gradient
-    std::vector<int> with;           // outputs that were used
-    for (int i = 0; i < static_cast<int>(grads.size()); ++i)
-      if (grads[i].defined()) with.push_back(i);
-    if (with.empty()) return out;
-    c10::optional<at::Tensor> second;
-    if (with.size() > 1) second = grads[with[1]];
-    const std::vector<at::Tensor> back = apply(grads[with[0]], second, saved[0], saved[1], sections, halves, sign);
-    for (size_t i = 0; i < with.size(); ++i) out[with[i]] = back[i];
-    return out;
-  }
-};
-
 }  // namespace
 
-std::vector<at::Tensor> rotate(const at::Tensor& q, const c10::optional<at::Tensor>& k, const at::Tensor& positions,
-                               const at::Tensor& turns, const std::vector<int64_t>& sections, bool halves) {
-  if (at::GradMode::is_enabled() && (q.requires_grad() || (k.has_value() && k->requires_grad())))
-    return Rotate::apply(q, k, positions, turns, sections, halves, 1.0);
-  return rotated(q, k.value_or(at::Tensor()), positions, turns, sections, halves, 1.0);
+std::pair<at::Tensor, c10::optional<at::Tensor>> rotate(const at::Tensor& q, const c10::optional<at::Tensor>& k,
+                                                        const at::Tensor& positions, std::shared_ptr<RopePlan> plan) {
+  variable_list out = turned(q, k.value_or(at::Tensor()), positions, plan, 1.0);
+  return {out[0], out[1].defined() ? c10::optional<at::Tensor>(out[1]) : c10::nullopt};
 }
 
 }  // namespace rc

@@ -50,6 +50,9 @@ def available() -> bool:
 
 def status_word(device) -> torch.Tensor:
     device = torch.device(device)
+    word = _status.get(device.index)
+    if word is not None:
+        return word
     if device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())
     with _lock:

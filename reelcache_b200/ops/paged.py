@@ -13,8 +13,6 @@ reported by :func:`reelcache_b200.ops._ext.check_status`.
 
 from __future__ import annotations
 
-import math
-
 import torch
 
 from ..errors import ConfigurationError, UnsupportedError
@@ -25,15 +23,13 @@ from .rope import AxisRope
 def append(q, k, v, positions, rope: AxisRope, k_pages, v_pages, block_table, kv_lens, cu_q, *, out=None):
     """Rotate ``q[T, heads, D]`` and ``k[T, kv_heads, D]`` at ``positions[T, axes]`` and write ``k`` and ``v`` into
     their sequences' pages, in one launch. Returns the rotated ``q`` (``out`` if given). bf16 or fp16."""
-    if q.device.type != "cuda":
+    if not q.is_cuda:
         raise UnsupportedError("append needs CUDA tensors")
     if q.shape[-1] != rope.head_dim:
         raise ConfigurationError(f"the rotation is for head_dim {rope.head_dim}, q has {q.shape[-1]}")
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ext().paged_append(q, out, k, v, positions, rope.turns(q.device), rope.sections, rope.halves, k_pages, v_pages,
-                       block_table, kv_lens, cu_q, status_word(q.device))
-    return out
+    device = q.device
+    return ext().paged_append(q, k, v, positions, rope.plan(device), k_pages, v_pages, block_table, kv_lens, cu_q, out,
+                              status_word(device))
 
 
 def attention(q, k_pages, v_pages, block_table, kv_lens, cu_q, *, max_q_len: int, causal: bool = False,
@@ -45,15 +41,12 @@ def attention(q, k_pages, v_pages, block_table, kv_lens, cu_q, *, max_q_len: int
     bidirectional in itself). ``window`` keeps the last ``window`` of the positions it would see, and the first
     ``sinks`` of the sequence. A token that sees nothing gets zeros (and ``lse`` of minus infinity).
     ``max_q_len`` bounds the new tokens of every sequence. ``return_lse`` adds the natural log-sum-exp ``[T, heads]``."""
-    if q.device.type != "cuda":
+    if not q.is_cuda:
         raise UnsupportedError("paged attention needs CUDA tensors")
     if window is not None and window < 1:
         raise ConfigurationError(f"window {window} must be positive")
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
-    ext().paged_attention(q, k_pages, v_pages, block_table, kv_lens, cu_q, out, lse, max_q_len, causal, window or 0, sinks,
-                          1.0 / math.sqrt(q.shape[-1]) if scale is None else scale, status_word(q.device))
+    out, lse = ext().paged_attention(q, k_pages, v_pages, block_table, kv_lens, cu_q, max_q_len, causal, window or 0, sinks,
+                                     scale, return_lse, out, status_word(q.device))
     return (out, lse) if return_lse else out
 
 
@@ -61,7 +54,7 @@ def copy_pages(storage, source, target, rows=None):
     """Copy pages ``source[i]`` to ``target[i]`` (int32 vectors) in every plane of ``storage [planes, pages, page_size,
     ...]``: whole pages, or their first ``rows[i]`` tokens. Pairs of -1 are skipped. Targets must differ from one another
     and from every source (the copies run at the same time)."""
-    if storage.device.type != "cuda":
+    if not storage.is_cuda:
         raise UnsupportedError("copy_pages needs CUDA tensors")
     ext().pages_copy(storage, source, target, rows, status_word(storage.device))
     return storage

@@ -22,7 +22,7 @@ class AxisRope:
     """A rotation: ``sections`` channel pairs per axis (they add up to ``head_dim // 2``), base ``theta`` and the
     pairs' layout: ``"interleaved"`` neighbours ``(2j, 2j + 1)`` or ``"halves"`` ``(j, j + head_dim / 2)``.
 
-    Keep one per model: :meth:`turns` builds its small device table at its first use on a device (with a copy from the
+    Keep one per model: :meth:`plan` builds its small device table at its first use on a device (with a copy from the
     host, so outside of graph capture)."""
 
     def __init__(self, head_dim: int, sections: Sequence[int], *, theta: float = 10000.0, layout: str = "interleaved"):
@@ -36,8 +36,7 @@ class AxisRope:
             raise ConfigurationError(f"rotary theta {theta} must be positive")
         if layout not in LAYOUTS:
             raise ConfigurationError(f"rotary layout {layout!r} must be one of {LAYOUTS}")
-        self.halves = layout == "halves"
-        self._tables = {}
+        self._plans = {}
 
     @classmethod
     def wan(cls, head_dim: int, *, theta: float = 10000.0, layout: str = "interleaved") -> "AxisRope":
@@ -45,25 +44,24 @@ class AxisRope:
         third = head_dim // 2 // 3
         return cls(head_dim, (head_dim // 2 - 2 * third, third, third), theta=theta, layout=layout)
 
-    def turns(self, device) -> torch.Tensor:
-        """``float32 [2, head_dim / 2]``: turns per position of every pair, high and low part."""
-        table = self._tables.get(device)
-        if table is None:
+    def plan(self, device):
+        """The rotation on ``device``, as the kernels take it: turns per position of every pair, in two float32 parts."""
+        plan = self._plans.get(device)
+        if plan is None:
             exponents = [torch.arange(n, dtype=torch.float64) / max(n, 1) for n in self.sections]
             turns = self.theta ** -torch.cat(exponents) / (2.0 * math.pi)
             high = turns.float()
             table = torch.stack([high, (turns - high.double()).float()]).to(device)
-            self._tables[device] = table
-        return table
+            plan = self._plans[device] = ext().RopePlan(table, self.sections, self.layout == "halves")
+        return plan
 
 
 def rotate(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, rope: AxisRope):
     """``q[T, heads, head_dim]`` and ``k[T, kv_heads, head_dim]`` (or ``None``) at ``positions[T, axes]`` (int32 or
     float32), rotated in one launch; bf16, fp16 or fp32, FP32 math. Rows may be strided (views of a fused projection).
     Differentiable in ``q`` and ``k``. Returns ``(q', k')``, new contiguous tensors of the same type."""
-    if q.device.type != "cuda":
+    if not q.is_cuda:
         raise UnsupportedError("rotate needs CUDA tensors")
     if q.shape[-1] != rope.head_dim:
         raise ConfigurationError(f"the rotation is for head_dim {rope.head_dim}, q has {q.shape[-1]}")
-    out = ext().rotate(q, k, positions, rope.turns(q.device), rope.sections, rope.halves)
-    return (out[0], out[1]) if k is not None else (out[0], None)
+    return ext().rotate(q, k, positions, rope.plan(q.device))

@@ -219,6 +219,30 @@ def test_append_writes_only_the_new_tokens(new, totals, heads, kv_heads, d, page
     assert torch.equal(k_pages, want_k)  # nothing else moved
 
 
+def test_append_refusals():
+    from reelcache_b200.errors import ConfigurationError, UnsupportedError
+    from reelcache_b200.ops import paged
+    from reelcache_b200.ops.rope import AxisRope
+    g = _gen(20)
+    rope = AxisRope.wan(64)
+    k_pages, v_pages, table, kv_lens, cu_q = paged_batch(g, [2], [10], 2, 64, 8, BF16)
+    q, k = (torch.randn(2, n, 64, generator=g, device="cuda").bfloat16() for n in (4, 2))
+    positions = _positions(g, 2, 3)
+    call = lambda q=q, k=k, v=k, p=positions, kp=k_pages, vp=v_pages, t=table, n=kv_lens, c=cu_q, **kw: paged.append(  # noqa: E731
+        q, k, v, p, rope, kp, vp, t, n, c, **kw)
+    call()
+    with pytest.raises(UnsupportedError):
+        call(q=q.cpu())
+    with pytest.raises(ConfigurationError):
+        call(q=torch.randn(2, 4, 128, device="cuda").bfloat16())
+    nine = torch.randn(5, 9, 2, 64, device="cuda").bfloat16()
+    for wrong in (dict(q=q.float(), k=k.float(), v=k.float()), dict(k=k.half()), dict(k=k[:1]), dict(v=k[:, :1]), dict(p=positions.float()[:1]),
+                  dict(p=positions[:, :2]), dict(kp=nine, vp=nine), dict(kp=k_pages[:, :, :1]), dict(vp=v_pages[1:]), dict(t=table.long()),
+                  dict(n=kv_lens.cpu()), dict(c=cu_q[:1]), dict(q=q[..., 1:]), dict(out=q[:1].clone()), dict(q=q.clone().requires_grad_())):
+        with pytest.raises((RuntimeError, ConfigurationError)):
+            call(**wrong)
+
+
 def test_append_out_of_range_is_reported_and_dropped(cuda_device):
     from reelcache_b200.errors import DeviceStatusError
     from reelcache_b200.ops import _ext, paged
@@ -469,7 +493,7 @@ def test_attention_refusals():
     nine = torch.randn(5, 9, 2, 64, device="cuda").bfloat16()
     for wrong in (dict(q=q.half()), dict(q=q.float()), dict(q=q[:, :3]), dict(k=k_pages[:, :, :1]), dict(k=nine, v=nine),
                   dict(v=v_pages[1:]), dict(t=table.long()), dict(n=kv_lens[:0]), dict(c=cu_q[:1]), dict(t=table.cpu()),
-                  dict(max_q_len=0), dict(sinks=-1, window=5), dict(scale=0.0), dict(scale=-1.0), dict(q=torch.randn(1, 4, 96, device="cuda").bfloat16()),
+                  dict(max_q_len=0), dict(sinks=-1, window=5), dict(scale=0.0), dict(scale=-1.0), dict(q=q.clone().requires_grad_()), dict(q=torch.randn(1, 4, 96, device="cuda").bfloat16()),
                   dict(out=torch.empty(2, 4, 64, device="cuda", dtype=BF16)), dict(k=k_pages[..., ::2])):
         with pytest.raises(RuntimeError):
             call(**wrong)
