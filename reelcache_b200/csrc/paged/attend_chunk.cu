@@ -218,34 +218,29 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const __grid_c
   }
 }
 
+// What the plan deals to a CTA: its whole rounds, then its part [begin, end) of the line.
+struct Share {
+  int rounds, items, first, begin, end;
+  __device__ __forceinline__ Share(const Chunk& p, int cta)
+      : rounds(p.plan.head[1]), items(p.plan.head[0]), first(p.plan.first[cta]), begin(p.plan.cut[cta]), end(p.plan.cut[cta + 1]) {}
+};
+
 // A CTA's n-th piece of work.
 struct Segment {
   Item item;
   int t0, t1;
   bool starts, ends;  // holds the item's first, last tile
 
-  __device__ __forceinline__ bool load(const Chunk& p, int cta, int n) {
-    const int rounds = p.plan.head[1], items = p.plan.head[0];
-    int i, begin = 0, end = 1 << 30;
-    if (n < rounds) {
-      i = n * p.ctas + cta;
-    } else {
-      i = p.plan.first[cta] + n - rounds;
-      begin = p.plan.cut[cta];
-      end = p.plan.cut[cta + 1];
-      if (begin >= end || i >= items) return false;
-    }
+  __device__ __forceinline__ bool load(const Chunk& p, const Share& share, int cta, int n) {
+    const bool whole = n < share.rounds;
+    const int i = whole ? n * p.ctas + cta : share.first + n - share.rounds;
+    if (!whole && (share.begin >= share.end || i >= share.items)) return false;
     const int4* src = reinterpret_cast<const int4*>(p.plan.items + i);
     const int4 x = src[0], y = src[1];
     item = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-    if (n < rounds) {
-      t0 = 0;
-      t1 = item.tiles;
-    } else {
-      if (item.start >= end) return false;
-      t0 = max(0, begin - item.start);
-      t1 = min(item.tiles, end - item.start);
-    }
+    if (!whole && item.start >= share.end) return false;
+    t0 = whole ? 0 : max(0, share.begin - item.start);
+    t1 = whole ? item.tiles : min(item.tiles, share.end - item.start);
     starts = t0 == 0;
     ends = t1 == item.tiles;
     return t0 < t1;
@@ -359,6 +354,13 @@ __device__ __forceinline__ void mask_half(uint32_t (&r)[64], int from, int high,
   }
 }
 
+// A whole sector in one store: a thread writes its own row, so narrower stores would each touch a sector of their own.
+__device__ __forceinline__ void store_32_bytes(float* dst, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
 // One thread of a converged warp (elect.sync: the compiler then knows that what it issues is uniform).
 __device__ __forceinline__ bool elect_one() {
   uint32_t one;
@@ -438,6 +440,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the plan
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
+  const Share share(p, cta);
   Segment seg;
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRoleRegs));
@@ -453,7 +456,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       int stage = 0;
       uint32_t phase = 1, raw_phase = 0;
       bool ok = true;
-      for (int n = 0; ok && seg.load(p, cta, n); ++n) {
+      for (int n = 0; ok && seg.load(p, share, cta, n); ++n) {
         const RowQueries rows(a, seg.item.row_tile, seg.item.q_len);
         const Sight sight(a, seg.item.kv_len, seg.item.q_len);
         const TileRange<kTile> range(sight, rows.first, rows.end);
@@ -503,27 +506,38 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         }
       }
     } else if (warp == 11) {
-      // ---------------- Q rows: 16-byte chunks, D / 8 lanes to a row ----------------
-      constexpr int kLanes = D / 8;          // lanes of a row
-      constexpr int kRowsPer = 32 / kLanes;  // rows of one pass
-      const int chunk = lane % kLanes, sub = lane / kLanes;
+      // ---------------- Q rows: each lane finds where 8 rows lie, then four lanes fetch a row 64 bytes at a time ------
+      const int quarter = lane & 3, sub = lane >> 2;
       bool ok = true;
-      for (int n = 0; ok && seg.load(p, cta, n); ++n) {
+      for (int n = 0; ok && seg.load(p, share, cta, n); ++n) {
+        const int packed0 = seg.item.row_tile * kItemRows;
+        const T* place[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int packed = packed0 + 32 * i + lane, query = packed / a.group;
+          const int h = seg.item.head * a.group + packed - query * a.group;
+          place[i] = query < seg.item.q_len
+                         ? static_cast<const T*>(a.q) + static_cast<int64_t>(seg.item.q_first + query) * a.q_token + h * a.q_head
+                         : nullptr;
+        }
         if (n > 0) ok = __all_sync(0xffffffffu, mbar_wait_park(q_empty, (n - 1) & 1, status, kTimeoutGather));
         if (!ok) break;
-        const int packed0 = seg.item.row_tile * kItemRows;
-#pragma unroll 4
-        for (int r0 = 0; r0 < kItemRows; r0 += kRowsPer) {
-          const int r = r0 + sub;
-          const int query = (packed0 + r) / a.group;
-          const bool valid = query < seg.item.q_len;
-          const int h = seg.item.head * a.group + packed0 + r - query * a.group;
-          const T* src = static_cast<const T*>(a.q);
-          if (valid) src += static_cast<int64_t>(seg.item.q_first + query) * a.q_token + h * a.q_head + chunk * 8;
-          const uint32_t dst = smem_u32(smem + Shape::q_off + (r >> 7) * Shape::tile_bytes + (chunk >> 3) * Shape::box_bytes) +
-                               (r & 127) * 128 + (((chunk & 7) ^ (r & 7)) << 4);
-          const int bytes = valid ? 16 : 0;  // rows past the sequence are zeros
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int r = 32 * i + 8 * j + sub;
+            const uint64_t src = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(place[i]), 8 * j + sub);
+            const int bytes = src != 0 ? 16 : 0;  // rows past the sequence are zeros
+            const uint64_t from = src != 0 ? src + quarter * 16 : reinterpret_cast<uint64_t>(a.q);
+            const uint32_t row = smem_u32(smem + Shape::q_off + (r >> 7) * Shape::tile_bytes) + (r & 127) * 128;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              const uint32_t dst = row + (c >> 1) * Shape::box_bytes + ((((c & 1) * 4 + quarter) ^ (r & 7)) << 4);
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(bytes ? from + c * 64 : from), "r"(bytes)
+                           : "memory");
+            }
+          }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
         fence_proxy_async_smem();
@@ -577,7 +591,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             v_phase ^= 1;
           }
         };
-        for (int n = 0; ok && seg.load(p, cta, n); ++n) {
+        for (int n = 0; ok && seg.load(p, share, cta, n); ++n) {
           for (int t = seg.t0; t < seg.t1 && ok; ++t) {
             // everything that can be waited for ahead of P is
             ok = mbar_wait_park(&k_full[k_stage], k_phase, status, kTimeoutMma);
@@ -627,7 +641,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     const uint32_t o_col = tmem_base + 256 + g * kTile + lanes;
     bool ok = true;
     int it = 0;
-    for (int n = 0; ok && seg.load(p, cta, n); ++n) {
+    for (int n = 0; ok && seg.load(p, share, cta, n); ++n) {
       const int packed = seg.item.row_tile * kItemRows + g * kTile + row;
       const int query = packed / a.group;
       const Sight sight(a, seg.item.kv_len, seg.item.q_len);
@@ -710,19 +724,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           tmem_wait_ld();
           if (valid && whole) {
             T* dst = static_cast<T*>(a.out) + token * a.out_token + h * a.out_head + c0;
+            uint32_t w[16];
 #pragma unroll
-            for (int c = 0; c < 32; c += 8) {
-              uint32_t w[4];
+            for (int e = 0; e < 16; ++e) w[e] = pack2<T>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                w[e] = pack2<T>(__uint_as_float(o[c + 2 * e]) * inv, __uint_as_float(o[c + 2 * e + 1]) * inv);
-              *reinterpret_cast<uint4*>(dst + c) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
+            for (int c = 0; c < 16; c += 4)
+              *reinterpret_cast<uint4*>(dst + 2 * c) = make_uint4(w[c], w[c + 1], w[c + 2], w[c + 3]);
           } else if (valid) {
             float* dst = p.part_o + slot * D + c0;
 #pragma unroll
-            for (int c = 0; c < 32; c += 4)
-              *reinterpret_cast<uint4*>(dst + c) = make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+            for (int c = 0; c < 32; c += 8) store_32_bytes(dst + c, o + c);
           }
           __syncwarp();
         }
@@ -757,26 +768,45 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const __grid_constant__
   if (query >= item.q_len) return;
   const int end = item.start + item.tiles;
   auto slot_of = [&](int c) { return (2 * static_cast<int64_t>(c) + (c == c0)) * kItemRows + row; };
-  // parts: c0 and every CTA after it whose part of the line is not empty and begins before the item's end
-  float top = p.part_ml[slot_of(c0) * 2];
-  for (int c = c0 + 1; c < p.ctas && p.plan.cut[c] < end; ++c)
-    if (p.plan.cut[c] < p.plan.cut[c + 1]) top = fmaxf(top, p.part_ml[slot_of(c) * 2]);
-  const float use = top == -INFINITY ? 0.0f : top;
-  float acc[kPer], sum = 0.0f;
+  // parts: c0's and those of the CTAs after it whose part of the line is not empty and begins before the item's end; 32
+  // CTAs at a time, a lane to each one's maximum and sum
+  float top = -INFINITY, acc[kPer], sum = 0.0f;
 #pragma unroll
   for (int e = 0; e < kPer; ++e) acc[e] = 0.0f;
-  for (int c = c0; c < p.ctas && (c == c0 || p.plan.cut[c] < end); ++c) {
-    if (p.plan.cut[c] >= p.plan.cut[c + 1]) continue;
-    const int64_t slot = slot_of(c);
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot * 2);
-    const float w = exp2_approx(ml.x - use);
-    sum = fmaf(w, ml.y, sum);
+  for (int cb = c0; cb < p.ctas; cb += 32) {
+    const int c = cb + lane;
+    const int from = c < p.ctas ? p.plan.cut[c] : end, to = c < p.ctas ? p.plan.cut[c + 1] : end;
+    const bool part = c == c0 || (from < to && from < end);
+    float2 ml = make_float2(-INFINITY, 0.0f);
+    if (part) ml = *reinterpret_cast<const float2*>(p.part_ml + slot_of(c) * 2);
+    float mx = ml.x;
 #pragma unroll
-    for (int e = 0; e < kPer; e += 2) {
-      const float2 x = *reinterpret_cast<const float2*>(p.part_o + slot * D + lane * kPer + e);
-      acc[e] = fmaf(w, x.x, acc[e]);
-      acc[e + 1] = fmaf(w, x.y, acc[e + 1]);
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    mx = fmaxf(mx, top);
+    const float use = mx == -INFINITY ? 0.0f : mx;
+    const float old = exp2_approx(top - use), wt = exp2_approx(ml.x - use);
+    top = mx;
+    float add = wt * ml.y;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) add += __shfl_xor_sync(0xffffffffu, add, o);
+    sum = fmaf(sum, old, add);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) acc[e] *= old;
+    uint32_t parts = __ballot_sync(0xffffffffu, part);
+#pragma unroll 4
+    while (parts != 0) {
+      const int i = __ffs(parts) - 1;
+      parts &= parts - 1;
+      const float w = __shfl_sync(0xffffffffu, wt, i);
+      const float* src = p.part_o + slot_of(cb + i) * D + lane * kPer;
+#pragma unroll
+      for (int e = 0; e < kPer; e += 2) {
+        const float2 x = *reinterpret_cast<const float2*>(src + e);
+        acc[e] = fmaf(w, x.x, acc[e]);
+        acc[e + 1] = fmaf(w, x.y, acc[e + 1]);
+      }
     }
+    if (__shfl_sync(0xffffffffu, to, 31) >= end) break;
   }
   const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
   const int64_t token = item.q_first + query;
