@@ -57,8 +57,8 @@ struct Short {
   Line line;
   float* part_o;   // [2 * CTAs, 16 kM, D]
   float* part_ml;  // [2 * CTAs, 16 kM, 2]
-  int rows;        // rows of a row tile: 16 kM
-  int row_tiles;   // row tiles of a sequence and KV head, at most
+  int rows;        // 16 kM
+  int cluster;     // CTAs of a cluster (the clustered form)
 };
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
@@ -86,26 +86,37 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t add
                : "memory");
 }
 
+__device__ __forceinline__ float2 load_cluster_2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 load_cluster_4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
 __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
-// Items and tiles of one sequence.
+// New tokens and tiles of one sequence (of each of its KV heads).
 struct SeqWork {
-  int q_first, q_len, kv_len, row_tiles, tiles;
-  // most: row tiles that the caller's bound on the new tokens allows
-  __device__ __forceinline__ SeqWork(const Args& a, int rows, int most, int s) {
+  int q_first, q_len, kv_len, tiles;
+  __device__ __forceinline__ SeqWork(const Args& a, int s) {
     q_first = __ldg(a.cu_q + s);
     q_len = min(__ldg(a.cu_q + s + 1), a.tokens) - q_first;
     if (q_first < 0 || q_len < 0) q_len = 0;
     kv_len = static_cast<int>(min(static_cast<int64_t>(max(0, __ldg(a.kv_lens + s))),
                                   static_cast<int64_t>(a.width) * a.tiling.page));
-    row_tiles = static_cast<int>(min(static_cast<int64_t>(most), (static_cast<int64_t>(q_len) * a.group + rows - 1) / rows));
     tiles = 0;
     if (q_len > 0) tiles = max(1, TileRange<kShortTile>(Sight(a, kv_len, q_len), 0, q_len).count());
   }
-  __device__ __forceinline__ int items(const Args& a) const { return row_tiles * a.kv_heads; }
 };
 
-template <typename T, int D, int kM>
+template <typename T, int D, int kM, bool kCluster>
 __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
     short_kernel(const __grid_constant__ PageMaps maps, const __grid_constant__ Short p) {
   using Shape = ShortShape<D>;
@@ -130,20 +141,23 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
     }
     fence_barrier_init();
   }
-  // The line of work: total, this CTA's share, and where it begins.
   if (warp == 4) {
     tma_prefetch_desc(&maps.k_wide);
     tma_prefetch_desc(&maps.v_wide);
   }
-  if (warp < 4) {
+  if (kCluster) {
+    // A cluster per sequence and KV head: this CTA's tiles are its rank's part of the item's, and the line is the item.
+    __syncthreads();
+  } else if (warp < 4) {
+    // The line of work: total, this CTA's share, and where it begins.
     // Thread i counts the tiles of sequences [i per, i per + per); their prefix sums place the share.
     const int per = (a.seqs + 127) / 128, s0 = static_cast<int>(threadIdx.x) * per;
     int mine = 0;
 #pragma unroll 4
     for (int i = 0; i < per; ++i) {
       if (s0 + i < a.seqs) {
-        const SeqWork w(a, kRows, p.row_tiles, s0 + i);
-        mine += w.tiles * w.items(a);
+        const SeqWork w(a, s0 + i);
+        mine += w.tiles * a.kv_heads;
       }
     }
     int x = mine;
@@ -172,8 +186,8 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
     const bool here = begin < end && begin >= before && begin < before + mine;
     if (here || blockIdx.x == 0) {
       for (int i = 0; i < per && s0 + i < a.seqs; ++i) {
-        const SeqWork w(a, kRows, p.row_tiles, s0 + i);
-        const int n = w.tiles * w.items(a);
+        const SeqWork w(a, s0 + i);
+        const int n = w.tiles * a.kv_heads;
         if (here && begin >= before && begin < before + n) {
           work[2] = s0 + i;
           work[3] = before;
@@ -186,31 +200,45 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
       }
     }
   }
-  __syncthreads();
-  const int begin = work[0], end = work[1];
-  if (begin >= end) return;
-  int s = work[2], base = work[3];
+  int s, base, begin, end;
+  if (kCluster) {
+    const int item = static_cast<int>(blockIdx.x) / p.cluster, rank = static_cast<int>(blockIdx.x) - item * p.cluster;
+    s = item / a.kv_heads;
+    const SeqWork w(a, s);
+    if (w.tiles == 0) return;  // no new tokens: the whole cluster
+    base = (s * a.kv_heads - item) * w.tiles;  // the item's tiles are places 0 ..
+    begin = w.tiles * rank / p.cluster;
+    end = w.tiles * (rank + 1) / p.cluster;
+  } else {
+    __syncthreads();
+    begin = work[0];
+    end = work[1];
+    if (begin >= end) return;
+    s = work[2];
+    base = work[3];
+  }
 
   int stage = 0;
   uint32_t phase = 0;
   if (warp == 4) {
     // ---------------- producer ----------------
-    for (int at = begin; at < end;) {
-      const SeqWork w(a, kRows, p.row_tiles, s);
-      const int n = w.tiles * w.items(a);
+    bool ok = true;
+    for (int at = begin; ok && at < end;) {
+      const SeqWork w(a, s);
+      const int n = w.tiles * a.kv_heads;
       if (at >= base + n) {
         base += n;
         ++s;
         continue;
       }
-      const int item = (at - base) / w.tiles, t0 = (at - base) - item * w.tiles;
+      const int head = (at - base) / w.tiles, t0 = (at - base) - head * w.tiles;
       const int t1 = min(w.tiles, t0 + end - at);
-      const int head = item / w.row_tiles;
       const TileRange<kShortTile> range(Sight(a, w.kv_len, w.q_len), 0, w.q_len);
       for (int t = t0; t < t1; ++t) {
         const int first = range.tile(t) * kShortTile;
         const Boxes<kShortTile> boxes(a.tiling, first, w.kv_len);
-        if (!mbar_wait(&empty[stage], phase ^ 1, a.status, kTimeoutProducer)) return;
+        ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1, a.status, kTimeoutProducer));
+        if (!ok) break;
         if (lane == 0) {
           if (boxes.count > 0) mbar_arrive_expect_tx(&full[stage], boxes.count * boxes.rows * 128 * Shape::boxes * 2);
           else mbar_arrive(&full[stage]);
@@ -236,6 +264,10 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
       }
       at += t1 - t0;
     }
+    if (kCluster) {
+      cluster_sync_all();
+      cluster_sync_all();
+    }
     return;
   }
 
@@ -243,17 +275,17 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
   const int mt = warp % kM, kg = warp / kM;  // row group, key group
   const int r0 = lane >> 2, c0 = (lane & 3) * 2;
   bool ok = true;
-  for (int at = begin; at < end;) {
-    const SeqWork w(a, kRows, p.row_tiles, s);
-    const int n = w.tiles * w.items(a);
-    if (at >= base + n) {
+  for (int at = begin; kCluster || at < end;) {  // a cluster's CTA goes round once, also without tiles
+    const SeqWork w(a, s);
+    const int n = w.tiles * a.kv_heads;
+    if (!kCluster && at >= base + n) {
       base += n;
       ++s;
       continue;
     }
-    const int item = (at - base) / w.tiles, t0 = (at - base) - item * w.tiles;
-    const int t1 = min(w.tiles, t0 + end - at);
-    const int head = item / w.row_tiles, row_tile = item - head * w.row_tiles;
+    const int head = kCluster ? static_cast<int>(blockIdx.x) / p.cluster - s * a.kv_heads : (at - base) / w.tiles;
+    const int t0 = kCluster ? begin : (at - base) - head * w.tiles;
+    const int t1 = kCluster ? end : min(w.tiles, t0 + end - at);
     const Sight sight(a, w.kv_len, w.q_len);
     const TileRange<kShortTile> range(sight, 0, w.q_len);
 
@@ -263,7 +295,7 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
     uint32_t q[D / 16][4];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int row = row_tile * kRows + mt * 16 + r0 + i * 8;
+      const int row = mt * 16 + r0 + i * 8;
       row_q[i] = row / a.group;
       row_h[i] = head * a.group + row - row_q[i] * a.group;
       valid[i] = row_q[i] < w.q_len;
@@ -276,11 +308,9 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
         q[k][i + 2] = valid[i] ? __ldg(reinterpret_cast<const uint32_t*>(src + k * 16 + 8)) : 0u;
       }
     }
-    const int rows_here = w.q_len * a.group - row_tile * kRows;  // of the row tile (or more)
-    // bounds over the row tile's queries, for tiles that need no mask
-    const int q_first = row_tile * kRows / a.group;
-    const int q_last = min(w.q_len - 1, (row_tile * kRows + kRows - 1) / a.group);
-    const int all_last = sight.last(q_first), all_low = sight.low(sight.last(q_last));
+    const int rows_here = w.q_len * a.group;  // or fewer: kRows
+    // bounds over the queries, for tiles that need no mask
+    const int all_last = sight.last(0), all_low = sight.low(sight.last(w.q_len - 1));
     const int any_low = sight.low(all_last);
 
     float o[D / 8][4];
@@ -488,8 +518,67 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
         }
       }
     }
+    if (kCluster) {
+      // The CTAs of the cluster put rows, maxima and sums into their stages (every tile has been consumed), then each
+      // joins a part of the channels over all of them, in order, through distributed shared memory.
+      float* res = reinterpret_cast<float*>(smem);  // [kRows][D]
+      float* res_ml = res + kRows * D;              // [kRows][2]
+      consumers_sync();
+      if (kg == 0) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int row = mt * 16 + r0 + 8 * i;
+#pragma unroll
+          for (int d = 0; d < D / 8; ++d) *reinterpret_cast<float2*>(res + row * D + d * 8 + c0) = make_float2(o[d][2 * i], o[d][2 * i + 1]);
+          if ((lane & 3) == 0) *reinterpret_cast<float2*>(res_ml + row * 2) = make_float2(m[i], l[i]);
+        }
+      }
+      cluster_sync_all();
+      const int rank = static_cast<int>(blockIdx.x) % p.cluster;
+      const int vecs = D / 4 / p.cluster;  // float4 of a row that this CTA joins
+      const int rows = min(kRows, rows_here);
+      for (int v = static_cast<int>(threadIdx.x); v < rows * vecs; v += 128) {
+        const int row = v / vecs, col = (rank * vecs + v - row * vecs) * 4;
+        float top = -INFINITY, sum = 0.0f;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int c0 = 0; c0 < p.cluster; c0 += 8) {  // eight CTAs' values at a time
+          float2 ml[8];
+          float4 x[8];
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            ml[c] = load_cluster_2(cluster_addr(res_ml + row * 2, c0 + c));
+            x[c] = load_cluster_4(cluster_addr(res + row * D + col, c0 + c));
+          }
+          float mx = top;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) mx = fmaxf(mx, ml[c].x);
+          const float use = mx == -INFINITY ? 0.0f : mx;
+          const float old = exp2_approx(top - use);
+          top = mx;
+          sum *= old;
+          acc.x *= old, acc.y *= old, acc.z *= old, acc.w *= old;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const float wt = exp2_approx(ml[c].x - use);
+            sum = fmaf(wt, ml[c].y, sum);
+            acc.x = fmaf(wt, x[c].x, acc.x);
+            acc.y = fmaf(wt, x[c].y, acc.y);
+            acc.z = fmaf(wt, x[c].z, acc.z);
+            acc.w = fmaf(wt, x[c].w, acc.w);
+          }
+        }
+        const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+        const int query = row / a.group, h = head * a.group + row - query * a.group;
+        const int64_t token = w.q_first + query;
+        T* dst = static_cast<T*>(a.out) + token * a.out_token + h * a.out_head + col;
+        if (ok) *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+        if (ok && a.lse != nullptr && col == 0) a.lse[token * a.heads + h] = sum > 0.0f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+      }
+      cluster_sync_all();  // the others have read this CTA's rows
+      return;
+    }
     if (kg == 0 && ok) {
-      const int item_first = base + item * w.tiles;
+      const int item_first = base + head * w.tiles;
       const bool starts = item_first >= begin, ends = item_first + w.tiles <= end;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -525,19 +614,14 @@ __global__ void __launch_bounds__(128) short_join_kernel(const __grid_constant__
   const int lane = threadIdx.x & 31;
   const int quads = p.rows / 4;
   const int row = (blockIdx.x % quads) * 4 + (threadIdx.x >> 5);
-  int item = blockIdx.x / quads;
-  const int s = item / (gridDim.x / quads / a.seqs);
-  item -= s * (gridDim.x / quads / a.seqs);
-  const SeqWork w(a, p.rows, p.row_tiles, s);  // the call's inputs: they do not wait for the first kernel
+  const int item = blockIdx.x / quads, s = item / a.kv_heads, head = item - s * a.kv_heads;
+  const SeqWork w(a, s);  // the call's inputs: they do not wait for the first kernel
   // every block waits, so that this kernel never ends before the first one does
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (item >= w.items(a)) return;
-  const int head = item / w.row_tiles, row_tile = item - head * w.row_tiles;
-  const int packed = row_tile * p.rows + row;
-  const int query = packed / a.group;
+  const int query = row / a.group;
   if (query >= w.q_len) return;
   const int share = *p.line.share;
-  const int begin = p.line.first[s] + item * w.tiles, end = begin + w.tiles;
+  const int begin = p.line.first[s] + head * w.tiles, end = begin + w.tiles;
   const int c0 = begin / share, c1 = (end - 1) / share;
   if (c0 == c1) return;
   // 32 parts at a time, a lane to each one's maximum and sum
@@ -577,7 +661,7 @@ __global__ void __launch_bounds__(128) short_join_kernel(const __grid_constant__
   }
   const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
   const int64_t token = w.q_first + query;
-  const int h = head * a.group + packed - query * a.group;
+  const int h = head * a.group + row - query * a.group;
   T* dst = static_cast<T*>(a.out) + token * a.out_token + h * a.out_head + lane * kPer;
 #pragma unroll
   for (int e = 0; e < kPer; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack2<T>(acc[e] * inv, acc[e + 1] * inv);
@@ -585,42 +669,57 @@ __global__ void __launch_bounds__(128) short_join_kernel(const __grid_constant__
 }
 
 template <typename T, int D, int kM>
-void short_launch(Args a, const at::Tensor& k_pages, const at::Tensor& v_pages, int max_q_len, const at::Tensor& like,
-                  cudaStream_t stream, int device) {
+void short_launch(Args a, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& like, cudaStream_t stream,
+                  int device) {
   using Shape = ShortShape<D>;
   static bool configured = false;
   if (!configured) {
-    RC_CUDA(cudaFuncSetAttribute(short_kernel<T, D, kM>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::bytes));
+    RC_CUDA(cudaFuncSetAttribute(short_kernel<T, D, kM, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::bytes));
+    RC_CUDA(cudaFuncSetAttribute(short_kernel<T, D, kM, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::bytes));
+    RC_CUDA(cudaFuncSetAttribute(short_kernel<T, D, kM, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     configured = true;
   }
   constexpr int kRows = 16 * kM;
+  static_assert(kRows * (D + 2) * 4 <= Shape::stages * 2 * Shape::tile_bytes, "a CTA's rows fit its stages");
   Short p{};
   p.a = a;
   p.rows = kRows;
   p.a.tiling = Tiling::of(a.tiling.page, kShortTile);
-  const int64_t row_tiles = (static_cast<int64_t>(max_q_len) * a.group + kRows - 1) / kRows;
-  p.row_tiles = static_cast<int>(row_tiles);
-  const int64_t items = row_tiles * a.kv_heads;  // of one sequence, at most
-  const int64_t most_tiles = static_cast<int64_t>(a.seqs) * items * (static_cast<int64_t>(a.width) * a.tiling.page / kShortTile + 2);
-  const int ctas = static_cast<int>(std::min<int64_t>(sm_count(device) * kShortCtasPerSm, most_tiles));
-  RC_CHECK(a.seqs * items * (kRows / 4) < (1ll << 31), "too many sequences and rows for one launch");
+  const PageMaps maps = page_maps(k_pages, v_pages, p.a.tiling, kShortTile);
+  const int64_t items = static_cast<int64_t>(a.seqs) * a.kv_heads, slots = sm_count(device) * kShortCtasPerSm;
+  cudaLaunchConfig_t config{};
+  config.blockDim = dim3(kShortThreads);
+  config.dynamicSmemBytes = Shape::bytes;
+  config.stream = stream;
+  cudaLaunchAttribute attribute{};
+  config.attrs = &attribute;
+  if (items * 8 <= slots) {
+    p.cluster = items * 16 <= slots ? 16 : 8;
+    config.gridDim = dim3(static_cast<unsigned>(items * p.cluster));
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = p.cluster;
+    attribute.val.clusterDim.y = 1;
+    attribute.val.clusterDim.z = 1;
+    config.numAttrs = 1;
+    RC_CUDA(cudaLaunchKernelEx(&config, short_kernel<T, D, kM, true>, maps, p));
+    return;
+  }
+  const int64_t most_tiles = items * (static_cast<int64_t>(a.width) * a.tiling.page / kShortTile + 2);
+  const int ctas = static_cast<int>(std::min<int64_t>(slots, most_tiles));
+  RC_CHECK(items * (kRows / 4) < (1ll << 31), "too many sequences and rows for one launch");
   const int64_t floats = 2ll * ctas * kRows * (D + 2), ints = 1 + 2ll * a.seqs;
   at::Tensor workspace = at::empty({floats + ints}, like.options().dtype(at::kFloat));
   p.part_o = workspace.data_ptr<float>();
   p.part_ml = p.part_o + 2ll * ctas * kRows * D;
   int* line = reinterpret_cast<int*>(p.part_o + floats);
   p.line = {line, line + 1, line + 1 + a.seqs};
-  const PageMaps maps = page_maps(k_pages, v_pages, p.a.tiling, kShortTile);
-  short_kernel<T, D, kM><<<ctas, kShortThreads, Shape::bytes, stream>>>(maps, p);
-  RC_CUDA(cudaGetLastError());
-  cudaLaunchConfig_t config{};
-  config.gridDim = dim3(static_cast<unsigned>(a.seqs * items * (kRows / 4)));
+  config.gridDim = dim3(ctas);
+  RC_CUDA(cudaLaunchKernelEx(&config, short_kernel<T, D, kM, false>, maps, p));
+  config.gridDim = dim3(static_cast<unsigned>(items * (kRows / 4)));
   config.blockDim = dim3(128);
-  config.stream = stream;
-  cudaLaunchAttribute attribute{};
+  config.dynamicSmemBytes = 0;
   attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attribute.val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = &attribute;
   config.numAttrs = 1;
   RC_CUDA(cudaLaunchKernelEx(&config, short_join_kernel<T, D>, p));
 }
@@ -629,9 +728,9 @@ template <typename T, int D>
 void short_rows(const Args& a, const at::Tensor& k_pages, const at::Tensor& v_pages, int max_q_len, const at::Tensor& like,
                 cudaStream_t stream, int device) {
   const int64_t rows = static_cast<int64_t>(max_q_len) * a.group;
-  if (rows <= 16) short_launch<T, D, 1>(a, k_pages, v_pages, max_q_len, like, stream, device);
-  else if (rows <= 32) short_launch<T, D, 2>(a, k_pages, v_pages, max_q_len, like, stream, device);
-  else short_launch<T, D, 4>(a, k_pages, v_pages, max_q_len, like, stream, device);
+  if (rows <= 16) short_launch<T, D, 1>(a, k_pages, v_pages, like, stream, device);
+  else if (rows <= 32) short_launch<T, D, 2>(a, k_pages, v_pages, like, stream, device);
+  else short_launch<T, D, 4>(a, k_pages, v_pages, like, stream, device);
 }
 
 void attend_short(const Args& a, int head_dim, bool half, const at::Tensor& k_pages, const at::Tensor& v_pages,
