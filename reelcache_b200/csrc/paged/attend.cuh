@@ -123,6 +123,21 @@ __device__ __forceinline__ void load_page_box(void* dst, const CUtensorMap* map,
       : "memory");
 }
 
+// Distributed shared memory: values of another CTA of the cluster (addresses from cluster_addr).
+__device__ __forceinline__ float2 load_cluster_2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 load_cluster_4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <>

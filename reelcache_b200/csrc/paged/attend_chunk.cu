@@ -63,6 +63,8 @@ struct ChunkShape {
   static constexpr int v_off = k_off + kKStages * tile_bytes;
   static constexpr int bar_off = v_off + kVStages * tile_bytes;
   static constexpr int bytes = bar_off + 256 + 1024;  // + barriers, alignment slack
+  static constexpr int ml_off = kItemRows * D * 4;    // at the end, clustered: rows of FP32 from 0, then maxima and sums
+  static_assert(ml_off + kItemRows * 8 <= bar_off, "the rows fit where the operands were");
   static_assert(bytes <= 227 * 1024, "shared memory of one CTA");
 };
 
@@ -85,6 +87,7 @@ struct Chunk {
   float* part_o;   // [2 * ctas, 256, D]
   float* part_ml;  // [2 * ctas, 256, 2]
   int ctas;
+  int cluster;     // CTAs of an item (the direct form)
   int row_tiles;   // of a sequence and KV head, at most
   int most_items;  // room for items
 };
@@ -114,6 +117,15 @@ __device__ __forceinline__ int plan_scan(int value, int* warp_sums, int* total) 
   return x - value + (warp > 0 ? warp_sums[warp - 1] : 0);
 }
 
+// New tokens of a sequence (returned), where they begin and how many keys it has.
+__device__ __forceinline__ int sequence(const Args& a, int s, int* q_first, int* kv_len) {
+  *q_first = __ldg(a.cu_q + s);
+  int q_len = min(__ldg(a.cu_q + s + 1), a.tokens) - *q_first;
+  if (*q_first < 0 || q_len < 0) q_len = 0;
+  *kv_len = static_cast<int>(min(static_cast<int64_t>(max(0, __ldg(a.kv_lens + s))), static_cast<int64_t>(a.width) * a.tiling.page));
+  return q_len;
+}
+
 // Queries of a row tile of a sequence: [first, end).
 struct RowQueries {
   int first, end;
@@ -123,18 +135,15 @@ struct RowQueries {
   }
 };
 
+__device__ __forceinline__ int tiles_of(const Args& a, const Item& item, const RowQueries& rows) {
+  return max(1, TileRange<kTile>(Sight(a, item.kv_len, item.q_len), rows.first, rows.end).count());
+}
+
 __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const __grid_constant__ Chunk p) {
   __shared__ int warp_sums[32];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const Args& a = p.a;
   const Plan& plan = p.plan;
-  auto length = [&](int s, int* q_first, int* kv_len) {
-    *q_first = __ldg(a.cu_q + s);
-    int q_len = min(__ldg(a.cu_q + s + 1), a.tokens) - *q_first;
-    if (*q_first < 0 || q_len < 0) q_len = 0;
-    *kv_len = static_cast<int>(min(static_cast<int64_t>(max(0, __ldg(a.kv_lens + s))), static_cast<int64_t>(a.width) * a.tiling.page));
-    return q_len;
-  };
   auto row_tiles = [&](int q_len) {
     return static_cast<int>(min(static_cast<int64_t>(p.row_tiles), (static_cast<int64_t>(q_len) * a.group + kItemRows - 1) / kItemRows));
   };
@@ -142,7 +151,7 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const __grid_c
   for (int s0 = 0; s0 < a.seqs; s0 += kPlanThreads) {
     const int s = s0 + threadIdx.x;
     int n = 0, q_first, kv_len;
-    if (s < a.seqs) n = row_tiles(length(s, &q_first, &kv_len)) * a.kv_heads;
+    if (s < a.seqs) n = row_tiles(sequence(a, s, &q_first, &kv_len)) * a.kv_heads;
     int total;
     const int before = plan_scan(n, warp_sums, &total);
     if (s < a.seqs) plan.base[s] = items + before;
@@ -160,12 +169,12 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const __grid_c
     }
     Item item;
     item.seq = lo;
-    item.q_len = length(lo, &item.q_first, &item.kv_len);
+    item.q_len = sequence(a, lo, &item.q_first, &item.kv_len);
     const int n = row_tiles(item.q_len), local = i - plan.base[lo];
     item.head = local / n;
     item.row_tile = n - 1 - (local - item.head * n);  // the rows that see most come first
     const RowQueries rows(a, item.row_tile, item.q_len);
-    item.tiles = max(1, TileRange<kTile>(Sight(a, item.kv_len, item.q_len), rows.first, rows.end).count());
+    item.tiles = tiles_of(a, item, rows);
     item.start = 0;
     plan.items[i] = item;
     sum += item.tiles;
@@ -221,11 +230,12 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const __grid_c
 // What the plan deals to a CTA: its whole rounds, then its part [begin, end) of the line.
 struct Share {
   int rounds, items, first, begin, end;
+  Share() = default;
   __device__ __forceinline__ Share(const Chunk& p, int cta)
       : rounds(p.plan.head[1]), items(p.plan.head[0]), first(p.plan.first[cta]), begin(p.plan.cut[cta]), end(p.plan.cut[cta + 1]) {}
 };
 
-// A CTA's n-th piece of work.
+// A CTA's n-th piece of work. Direct form: the only one, rank `rank` of `cluster` of the item that the block index names.
 struct Segment {
   Item item;
   int t0, t1;
@@ -244,6 +254,22 @@ struct Segment {
     starts = t0 == 0;
     ends = t1 == item.tiles;
     return t0 < t1;
+  }
+
+  __device__ __forceinline__ bool direct(const Chunk& p, int block) {
+    const int index = block / p.cluster, rank = block - index * p.cluster, each = p.a.kv_heads * p.row_tiles;
+    item.seq = index / each;
+    item.head = (index - item.seq * each) / p.row_tiles;
+    item.row_tile = p.row_tiles - 1 - index % p.row_tiles;  // the rows that see most come first
+    item.q_len = sequence(p.a, item.seq, &item.q_first, &item.kv_len);
+    item.start = 0;
+    if (static_cast<int64_t>(item.row_tile) * kItemRows >= static_cast<int64_t>(item.q_len) * p.a.group) return false;
+    item.tiles = tiles_of(p.a, item, RowQueries(p.a, item.row_tile, item.q_len));
+    t0 = item.tiles * rank / p.cluster;
+    t1 = item.tiles * (rank + 1) / p.cluster;
+    starts = t0 == 0;
+    ends = t1 == item.tiles;
+    return true;
   }
 };
 
@@ -384,7 +410,7 @@ __device__ __forceinline__ uint64_t sw128_mnmajor_desc(uint32_t smem_addr, uint3
   return desc;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool kDirect>
 __global__ void __launch_bounds__(kChunkThreads, 1)
     chunk_kernel(const __grid_constant__ PageMaps maps, const __grid_constant__ Chunk p) {
   using Shape = ChunkShape<D>;
@@ -406,6 +432,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   int* status = a.status;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int cta = blockIdx.x;
+  Segment seg;
+  if (kDirect && !seg.direct(p, cta)) return;  // the whole cluster
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 32);
@@ -437,11 +465,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the plan
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-
-  const Share share(p, cta);
-  Segment seg;
+  Share share{};
+  if (!kDirect) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the plan
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    share = Share(p, cta);
+  }
+  auto next = [&](int n) { return kDirect ? n == 0 && seg.t0 < seg.t1 : seg.load(p, share, cta, n); };
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRoleRegs));
     if (warp < 10) {
@@ -456,7 +486,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       int stage = 0;
       uint32_t phase = 1, raw_phase = 0;
       bool ok = true;
-      for (int n = 0; ok && seg.load(p, share, cta, n); ++n) {
+      for (int n = 0; ok && next(n); ++n) {
         const RowQueries rows(a, seg.item.row_tile, seg.item.q_len);
         const Sight sight(a, seg.item.kv_len, seg.item.q_len);
         const TileRange<kTile> range(sight, rows.first, rows.end);
@@ -509,7 +539,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       // ---------------- Q rows: each lane finds where 8 rows lie, then four lanes fetch a row 64 bytes at a time ------
       const int quarter = lane & 3, sub = lane >> 2;
       bool ok = true;
-      for (int n = 0; ok && seg.load(p, share, cta, n); ++n) {
+      for (int n = 0; ok && next(n); ++n) {
         const int packed0 = seg.item.row_tile * kItemRows;
         const T* place[8];
 #pragma unroll
@@ -591,7 +621,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             v_phase ^= 1;
           }
         };
-        for (int n = 0; ok && seg.load(p, share, cta, n); ++n) {
+        for (int n = 0; ok && next(n); ++n) {
           for (int t = seg.t0; t < seg.t1 && ok; ++t) {
             // everything that can be waited for ahead of P is
             ok = mbar_wait_park(&k_full[k_stage], k_phase, status, kTimeoutMma);
@@ -641,7 +671,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     const uint32_t o_col = tmem_base + 256 + g * kTile + lanes;
     bool ok = true;
     int it = 0;
-    for (int n = 0; ok && seg.load(p, share, cta, n); ++n) {
+    for (int n = 0; ok && next(n); ++n) {
       const int packed = seg.item.row_tile * kItemRows + g * kTile + row;
       const int query = packed / a.group;
       const Sight sight(a, seg.item.kv_len, seg.item.q_len);
@@ -710,7 +740,24 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         if (lane == 0) mbar_arrive(&p_full[2 * g + 1]);
       }
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait_park(&o_done[g], n & 1, status, kTimeoutEpilogue));
-      if (ok) {
+      if (kDirect && p.cluster > 1) {
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait_park(&o_done[1 - g], 0, status, kTimeoutEpilogue));
+        if (ok) {  // every product is done: the operands' memory takes the rows, 16-byte chunks turned against bank conflicts
+          tc_fence_after();
+          float4* rows_at = reinterpret_cast<float4*>(smem) + (g * kTile + row) * (D / 4);
+#pragma unroll
+          for (int c0 = 0; c0 < D; c0 += 32) {
+            uint32_t o[32];
+            tmem_ld_32x32b_x32(o_col + c0, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 32; c += 4)
+              rows_at[((c0 + c) / 4) ^ (row & 15)] = make_float4(__uint_as_float(o[c]), __uint_as_float(o[c + 1]),
+                                                                  __uint_as_float(o[c + 2]), __uint_as_float(o[c + 3]));
+          }
+          reinterpret_cast<float2*>(smem + Shape::ml_off)[g * kTile + row] = make_float2(m_run, l_run);
+        }
+      } else if (ok) {
         tc_fence_after();
         const bool valid = query < seg.item.q_len, whole = seg.starts && seg.ends;
         const float inv = whole ? (l_run > 0.0f ? 1.0f / l_run : 0.0f) : 1.0f;
@@ -745,6 +792,43 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     }
   }
 
+  if (kDirect && p.cluster > 1) {
+    // CTAs without tiles have nothing to give; every CTA joins a part of the item's rows over all of them, in order.
+    if (seg.t0 == seg.t1 && threadIdx.x < kItemRows)
+      reinterpret_cast<float2*>(smem + Shape::ml_off)[threadIdx.x] = make_float2(-INFINITY, 0.0f);
+    cluster_sync_all();
+    if (threadIdx.x < kItemRows) {
+      const int packed0 = seg.item.row_tile * kItemRows;
+      const int rows = static_cast<int>(min(static_cast<int64_t>(kItemRows), static_cast<int64_t>(seg.item.q_len) * a.group - packed0));
+      const int rank = cta % p.cluster;
+      for (int v = rank * kItemRows + static_cast<int>(threadIdx.x); v < rows * (D / 4); v += p.cluster * kItemRows) {
+        const int row = v / (D / 4), chunk = v % (D / 4);
+        const float4* from = reinterpret_cast<const float4*>(smem) + row * (D / 4) + (chunk ^ (row & 15));
+        const float2* from_ml = reinterpret_cast<const float2*>(smem + Shape::ml_off) + row;
+        float top = -INFINITY, sum = 0.0f;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int c = 0; c < p.cluster; ++c) {
+          const float2 ml = load_cluster_2(cluster_addr(from_ml, c));
+          if (ml.x == -INFINITY) continue;  // no key seen there (nor, perhaps, anything written)
+          const float4 x = load_cluster_4(cluster_addr(from, c));
+          const float mx = fmaxf(top, ml.x), old = exp2_approx(top - mx), wt = exp2_approx(ml.x - mx);
+          top = mx;
+          sum = fmaf(sum, old, wt * ml.y);
+          acc.x = fmaf(acc.x, old, wt * x.x);
+          acc.y = fmaf(acc.y, old, wt * x.y);
+          acc.z = fmaf(acc.z, old, wt * x.z);
+          acc.w = fmaf(acc.w, old, wt * x.w);
+        }
+        const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+        const int query = (packed0 + row) / a.group, h = seg.item.head * a.group + packed0 + row - query * a.group;
+        const int64_t token = seg.item.q_first + query;
+        T* dst = static_cast<T*>(a.out) + token * a.out_token + h * a.out_head + chunk * 4;
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+        if (a.lse != nullptr && chunk == 0) a.lse[token * a.heads + h] = sum > 0.0f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+      }
+    }
+    cluster_sync_all();  // the others have read this CTA's rows
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -817,29 +901,104 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const __grid_constant__
   if (a.lse != nullptr && lane == 0) a.lse[token * a.heads + h] = sum > 0.0f ? (top + log2f(sum)) * kLn2 : -INFINITY;
 }
 
+template <typename T, int D, bool kDirect>
+void chunk_configure() {
+  static bool configured = false;
+  if (configured) return;
+  RC_CUDA(cudaFuncSetAttribute(chunk_kernel<T, D, kDirect>, cudaFuncAttributeMaxDynamicSharedMemorySize, ChunkShape<D>::bytes));
+  if (kDirect) RC_CUDA(cudaFuncSetAttribute(chunk_kernel<T, D, kDirect>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  cudaFuncAttributes attr;  // the register split assumes exactly kLaunchRegs a thread
+  RC_CUDA(cudaFuncGetAttributes(&attr, chunk_kernel<T, D, kDirect>));
+  RC_CHECK(attr.numRegs == kLaunchRegs, "paged attention compiled to " + std::to_string(attr.numRegs) +
+                                            " registers a thread; its register split needs " + std::to_string(kLaunchRegs));
+  configured = true;
+}
+
+// Clusters of `size` CTAs that the device holds at a time.
+template <typename T, int D>
+int clusters_at_once(int size, int device) {
+  static int known[64][5] = {};
+  int index = 0;
+  while ((1 << index) < size) ++index;
+  int& count = known[device & 63][index];
+  if (count == 0) {
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(size);
+    config.blockDim = dim3(kChunkThreads);
+    config.dynamicSmemBytes = ChunkShape<D>::bytes;
+    cudaLaunchAttribute attribute{};
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = size;
+    attribute.val.clusterDim.y = 1;
+    attribute.val.clusterDim.z = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, chunk_kernel<T, D, true>, &config) != cudaSuccess) {
+      (void)cudaGetLastError();
+      n = 0;
+    }
+    count = n > 0 ? n : -1;
+  }
+  return count;
+}
+
+// CTAs of an item in the direct form, or 0 for the planned form, by estimated time in tile pairs (about 1.8 us each):
+// direct, every item takes its tiles over its cluster, in as many rounds as its clusters need; planned, all SMs share all
+// tiles, but the plan, the join and the cut items cost about 8 tiles.
+template <typename T, int D>
+int direct_cluster(int64_t items, int64_t tiles, bool uneven, int device) {
+  double best = static_cast<double>(items) * tiles / sm_count(device) * (uneven ? 0.75 : 1.0) + 8.0;
+  int cluster = 0;
+  for (int c = 1; c <= 16; c *= 2) {
+    const int64_t slots = clusters_at_once<T, D>(c, device);
+    if (slots <= 0) continue;
+    const double t = static_cast<double>((items + slots - 1) / slots) * ((tiles + c - 1) / c) + (c > 1 ? 1.0 : 0.0);
+    if (t < best) {
+      best = t;
+      cluster = c;
+    }
+  }
+  return cluster;
+}
+
 template <typename T, int D>
 void chunk_launch(const Args& args, const at::Tensor& k_pages, const at::Tensor& v_pages, int max_q_len,
                   const at::Tensor& like, cudaStream_t stream, int device) {
   using Shape = ChunkShape<D>;
-  static bool configured = false;
-  if (!configured) {
-    RC_CUDA(cudaFuncSetAttribute(chunk_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::bytes));
-    cudaFuncAttributes attr;  // the register split assumes exactly kLaunchRegs a thread
-    RC_CUDA(cudaFuncGetAttributes(&attr, chunk_kernel<T, D>));
-    RC_CHECK(attr.numRegs == kLaunchRegs, "paged attention compiled to " + std::to_string(attr.numRegs) +
-                                              " registers a thread; its register split needs " + std::to_string(kLaunchRegs));
-    configured = true;
-  }
   Chunk p{};
   p.a = args;
   p.a.tiling = Tiling::of(args.tiling.page, kTile);
   const int64_t row_tiles = (static_cast<int64_t>(max_q_len) * args.group + kItemRows - 1) / kItemRows;
-  const int64_t most_items = std::min<int64_t>(static_cast<int64_t>(args.seqs) * row_tiles,
-                                               static_cast<int64_t>(args.tokens) * args.group / kItemRows + args.seqs) * args.kv_heads;
+  const int64_t grid_items = static_cast<int64_t>(args.seqs) * row_tiles * args.kv_heads;
+  const int64_t most_items = std::min<int64_t>(grid_items, (static_cast<int64_t>(args.tokens) * args.group / kItemRows + args.seqs) * args.kv_heads);
   RC_CHECK(most_items < (1ll << 26), "too many rows for one launch");
   p.row_tiles = static_cast<int>(row_tiles);
   p.most_items = static_cast<int>(most_items);
   p.ctas = sm_count(device);
+  const PageMaps maps = page_maps(k_pages, v_pages, p.a.tiling, kTile);
+  cudaLaunchConfig_t config{};
+  config.blockDim = dim3(kChunkThreads);
+  config.dynamicSmemBytes = Shape::bytes;
+  config.stream = stream;
+  cudaLaunchAttribute attribute{};
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  // tiles of an item, at most: the table's width, or what a window leaves of it
+  int64_t keys = static_cast<int64_t>(args.width) * args.tiling.page;
+  if (args.window > 0) keys = std::min<int64_t>(keys, static_cast<int64_t>(args.window) + args.sinks + kItemRows / args.group + 2 * kTile);
+  chunk_configure<T, D, true>();
+  p.cluster = direct_cluster<T, D>(most_items, (keys + kTile - 1) / kTile, args.causal && row_tiles > 1, device);
+  if (p.cluster > 0) {
+    config.gridDim = dim3(static_cast<unsigned>(grid_items * p.cluster));
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = p.cluster;
+    attribute.val.clusterDim.y = 1;
+    attribute.val.clusterDim.z = 1;
+    RC_CUDA(cudaLaunchKernelEx(&config, chunk_kernel<T, D, true>, maps, p));
+    return;
+  }
+  chunk_configure<T, D, false>();
   RC_CHECK(p.ctas < kPlanThreads, "more SMs than the plan's threads");
   const int64_t o_floats = 2ll * p.ctas * kItemRows * D, ml_floats = 2ll * p.ctas * kItemRows * 2;
   const int64_t ints = most_items * 8 + 4 + 2ll * (p.ctas + 1) + args.seqs;
@@ -851,20 +1010,12 @@ void chunk_launch(const Args& args, const at::Tensor& k_pages, const at::Tensor&
   p.plan.cut = p.plan.head + 4;
   p.plan.first = p.plan.cut + p.ctas + 1;
   p.plan.base = p.plan.first + p.ctas + 1;
-  const PageMaps maps = page_maps(k_pages, v_pages, p.a.tiling, kTile);
   chunk_plan_kernel<<<1, kPlanThreads, 0, stream>>>(p);
   RC_CUDA(cudaGetLastError());
-  cudaLaunchConfig_t config{};
   config.gridDim = dim3(p.ctas);
-  config.blockDim = dim3(kChunkThreads);
-  config.dynamicSmemBytes = Shape::bytes;
-  config.stream = stream;
-  cudaLaunchAttribute attribute{};
   attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attribute.val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = &attribute;
-  config.numAttrs = 1;
-  RC_CUDA(cudaLaunchKernelEx(&config, chunk_kernel<T, D>, maps, p));
+  RC_CUDA(cudaLaunchKernelEx(&config, chunk_kernel<T, D, false>, maps, p));
   config.gridDim = dim3(kItemRows / 8, p.ctas - 1);
   config.blockDim = dim3(256);
   config.dynamicSmemBytes = 0;

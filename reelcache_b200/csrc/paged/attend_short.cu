@@ -30,6 +30,8 @@ namespace paged {
 constexpr int kShortTile = 64;       // keys of a tile
 constexpr int kShortThreads = 160;   // four consumer warps, one producer warp
 constexpr int kShortCtasPerSm = 2;
+constexpr int kFewTiles = 8;         // tiles of a CTA that are done before an even share would have paid
+constexpr int kLongTiles = 64;       // the same where clusters are large and few
 constexpr int kShortLeast = 2;       // tiles of a share, at least: every part costs a pass through the workspace
 
 template <int D>
@@ -84,20 +86,6 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t add
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr)
                : "memory");
-}
-
-__device__ __forceinline__ float2 load_cluster_2(uint32_t addr) {
-  float2 v;
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
-  return v;
-}
-__device__ __forceinline__ float4 load_cluster_4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(addr)
-               : "memory");
-  return v;
 }
 
 __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
@@ -541,13 +529,18 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
         const int row = v / vecs, col = (rank * vecs + v - row * vecs) * 4;
         float top = -INFINITY, sum = 0.0f;
         float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int c0 = 0; c0 < p.cluster; c0 += 8) {  // eight CTAs' values at a time
+        for (int first = 0; first < p.cluster; first += 8) {  // eight CTAs' values at a time
           float2 ml[8];
           float4 x[8];
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
-            ml[c] = load_cluster_2(cluster_addr(res_ml + row * 2, c0 + c));
-            x[c] = load_cluster_4(cluster_addr(res + row * D + col, c0 + c));
+            if (first + c >= p.cluster) {
+              ml[c] = make_float2(-INFINITY, 0.0f);
+              x[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+              continue;
+            }
+            ml[c] = load_cluster_2(cluster_addr(res_ml + row * 2, first + c));
+            x[c] = load_cluster_4(cluster_addr(res + row * D + col, first + c));
           }
           float mx = top;
 #pragma unroll
@@ -693,8 +686,14 @@ void short_launch(Args a, const at::Tensor& k_pages, const at::Tensor& v_pages, 
   config.stream = stream;
   cudaLaunchAttribute attribute{};
   config.attrs = &attribute;
-  if (items * 8 <= slots) {
-    p.cluster = items * 16 <= slots ? 16 : 8;
+  // Clusters of the largest size that all find room at once, unless the table's width allows sequences so long that an
+  // even share of all tiles matters more than the second kernel that it costs (measured on one B200, 8 KV heads: one
+  // session of 2,048 keys 8.3 us clustered and 11.7 us shared out, 16 sessions of 512 keys 11 and 14 us, one session of
+  // 131,072 keys 104 and 95 us).
+  const int64_t most_tiles = (static_cast<int64_t>(a.width) * a.tiling.page + kShortTile - 1) / kShortTile;
+  for (int c = 16; c > 1 && p.cluster == 0; c /= 2)
+    if (items * c <= slots && most_tiles <= c * (c >= 8 ? kLongTiles : kFewTiles)) p.cluster = c;
+  if (p.cluster > 0) {
     config.gridDim = dim3(static_cast<unsigned>(items * p.cluster));
     attribute.id = cudaLaunchAttributeClusterDimension;
     attribute.val.clusterDim.x = p.cluster;
@@ -704,8 +703,7 @@ void short_launch(Args a, const at::Tensor& k_pages, const at::Tensor& v_pages, 
     RC_CUDA(cudaLaunchKernelEx(&config, short_kernel<T, D, kM, true>, maps, p));
     return;
   }
-  const int64_t most_tiles = items * (static_cast<int64_t>(a.width) * a.tiling.page / kShortTile + 2);
-  const int ctas = static_cast<int>(std::min<int64_t>(slots, most_tiles));
+  const int ctas = static_cast<int>(std::min<int64_t>(slots, items * (most_tiles + 1)));
   RC_CHECK(items * (kRows / 4) < (1ll << 31), "too many sequences and rows for one launch");
   const int64_t floats = 2ll * ctas * kRows * (D + 2), ints = 1 + 2ll * a.seqs;
   at::Tensor workspace = at::empty({floats + ints}, like.options().dtype(at::kFloat));
