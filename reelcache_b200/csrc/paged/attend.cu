@@ -77,6 +77,7 @@ std::pair<at::Tensor, c10::optional<at::Tensor>> paged_attention(
   a.cu_q = t.cu_q;
   a.seqs = t.seqs;
   a.width = t.width;
+  a.table_row = t.row;
   a.pages = kp.count;
   a.heads = static_cast<int>(q.size(1));
   a.kv_heads = static_cast<int>(kv_heads);

@@ -36,6 +36,7 @@ struct Args {
   const int* kv_lens;
   const int* cu_q;
   int seqs, width, pages;
+  int64_t table_row;  // elements from one sequence's row of the table to the next
   int heads, kv_heads, group;
   int causal, window, sinks;  // window 0: no window
   int tokens;

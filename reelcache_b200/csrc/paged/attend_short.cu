@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
         __syncwarp();
         if (lane < boxes.count) {
           int row;
-          const int page = boxes.page(a.table + static_cast<int64_t>(s) * a.width, a.pages, a.tiling, first, lane, &row, a.status);
+          const int page = boxes.page(a.table + s * a.table_row, a.pages, a.tiling, first, lane, &row, a.status);
           const bool wide = boxes.rows == kShortTile;
           const CUtensorMap* km = wide ? &maps.k_wide : &maps.k_step;
           const CUtensorMap* vm = wide ? &maps.v_wide : &maps.v_step;

@@ -23,10 +23,11 @@ struct Pages {  // [pages, page_size, kv_heads, head_dim], strides in elements
 };
 
 struct Table {
-  const int* table;    // [seqs, width]
+  const int* table;    // [seqs, width], `row` elements apart
   const int* kv_lens;  // [seqs]
   const int* cu_q;     // [seqs + 1]
   int seqs, width;
+  int64_t row;         // elements from one sequence's row to the next
 };
 
 inline Pages check_pages(const at::Tensor& t, int64_t heads, int64_t head_dim, const char* name) {
@@ -45,14 +46,15 @@ inline Table check_table(const at::Tensor& table, const at::Tensor& kv_lens, con
                          const at::Device& device) {
   const at::Tensor* all[3] = {&table, &kv_lens, &cu_q};
   for (const at::Tensor* t : all)
-    RC_CHECK(t->device() == device && t->scalar_type() == at::kInt && t->is_contiguous(),
-             "block_table, kv_lens and cu_q must be contiguous int32 tensors on the device of q");
-  RC_CHECK(table.dim() == 2 && kv_lens.dim() == 1 && cu_q.dim() == 1 && kv_lens.size(0) == table.size(0) &&
+    RC_CHECK(t->device() == device && t->scalar_type() == at::kInt && (t == &table || t->is_contiguous()),
+             "block_table, kv_lens and cu_q must be contiguous int32 tensors on the device of q (rows of the table may be "
+             "strided)");
+  RC_CHECK(table.dim() == 2 && (table.stride(1) == 1 || table.size(1) <= 1) && table.stride(0) >= 0 && kv_lens.dim() == 1 && cu_q.dim() == 1 && kv_lens.size(0) == table.size(0) &&
                cu_q.size(0) == table.size(0) + 1,
            "block_table is [seqs, width], kv_lens [seqs], cu_q [seqs + 1]");
   RC_CHECK(table.size(0) < (1 << 20) && table.size(1) < (1ll << 31), "too many sequences or pages per sequence");
   return {table.data_ptr<int>(), kv_lens.data_ptr<int>(), cu_q.data_ptr<int>(), static_cast<int>(table.size(0)),
-          static_cast<int>(table.size(1))};
+          static_cast<int>(table.size(1)), table.stride(0)};
 }
 
 }  // namespace paged

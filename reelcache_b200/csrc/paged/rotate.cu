@@ -114,6 +114,7 @@ struct Args {
   const int* kv_lens;
   const int* cu_q;
   int seqs, table_width, page, pages;
+  int64_t table_row;
   int64_t page_k, page_v;  // page strides in bytes (dst_token / dst_head are strides inside a page)
   int* status;
 };
@@ -170,7 +171,7 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant_
     if (stored) {
       const int slot = at >= 0 ? at / a.page : -1;
       row = at - slot * a.page;
-      page = slot >= 0 && slot < a.table_width ? __ldg(a.table + static_cast<int64_t>(lo) * a.table_width + slot) : -1;
+      page = slot >= 0 && slot < a.table_width ? __ldg(a.table + lo * a.table_row + slot) : -1;
       if (page < 0 || page >= a.pages) {
         stored = false;
         if (vec == 0 && group == 0 && a.status != nullptr) atomicCAS(a.status + kPagedWord, 0, kPageRange);
@@ -397,6 +398,7 @@ at::Tensor paged_append(const at::Tensor& q, const at::Tensor& k, const at::Tens
   a.cu_q = t.cu_q;
   a.seqs = t.seqs;
   a.table_width = t.width;
+  a.table_row = t.row;
   a.page = kp.size;
   a.pages = kp.count;
   a.page_k = kp.page_stride * 2;

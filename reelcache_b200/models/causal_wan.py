@@ -25,6 +25,7 @@ import torch
 
 from ..ops import attention as attn_ops
 from ..ops import gemm, norms
+from ..ops.rope import AxisRope
 from ..restore_kernels import RopeTable
 
 
@@ -170,6 +171,7 @@ class CausalWanDiT:
         pairs = cfg.head_dim // 2
         self.rope = RopeTable.wan(cfg.head_dim, 1024, theta=cfg.rope_theta, device=self.device)
         assert self.rope.pairs == pairs
+        self._axis_rope = None
 
     # -- conditioning ------------------------------------------------------------------------------------------
 
@@ -264,6 +266,69 @@ class CausalWanDiT:
         y = norms.ln_modulate(x, shift=shift, scale=scale, eps=cfg.eps)
         out = gemm.linear(y, self.head_w, self.head_b, out_dtype=torch.float32)
         return self.unpatchify(out)
+
+    @property
+    def axis_rope(self) -> AxisRope:
+        """The rotation of :attr:`rope` from per-token positions (the paged cache's form)."""
+        if self._axis_rope is None:
+            self._axis_rope = AxisRope.wan(self.cfg.head_dim, theta=self.cfg.rope_theta)
+        return self._axis_rope
+
+    def session_positions(self, chunk_indices) -> torch.Tensor:
+        """Frame, row and column ``int32 [len(chunk_indices) * chunk_tokens, 3]`` of the tokens of some chunks."""
+        cfg = self.cfg
+        at = torch.arange(cfg.chunk_tokens, device=self.device, dtype=torch.int32)
+        frame, rest = at // cfg.tokens_per_frame, at % cfg.tokens_per_frame
+        grid = torch.stack([frame, rest // cfg.grid_w, rest % cfg.grid_w], dim=1)
+        first = torch.tensor([[cfg.frames_per_chunk * c, 0, 0] for c in chunk_indices], dtype=torch.int32)
+        return (grid + first.to(self.device)[:, None]).flatten(0, 1)
+
+    def forward_sessions(self, latents: torch.Tensor, t: float, cache, batch, text_kv, *, capture=None) -> torch.Tensor:
+        """One forward of the newest chunk of several sessions of a :class:`~reelcache_b200.paged_cache.PagedKVCache`
+        (``batch`` from its ``extend`` or ``again``, a chunk for each): ``latents[sessions, in_dim, F, H, W]`` at timestep
+        ``t``, the weights read once for all of them, histories shared page by page between forks. Same block math as
+        :meth:`forward_chunk`. ``capture(layer, k_pre, v)`` receives the rows of all sessions, one after the other.
+        Returns the flow predictions ``[sessions, in_dim, F, H, W]`` (FP32)."""
+        cfg = self.cfg
+        tokens, sessions = cfg.chunk_tokens, len(batch.sessions)
+        if any(n != tokens for n in batch.counts) or latents.shape[0] != sessions:
+            raise ValueError("every session of the batch needs one chunk of new tokens and its latents")
+        if any(s.length % tokens for s in batch.sessions):
+            raise ValueError("the sessions' histories must be whole chunks")
+        rows = sessions * tokens
+        x = gemm.linear(torch.cat([self.patchify(one) for one in latents]).to(torch.bfloat16).contiguous(), self.patch_w,
+                        self.patch_b)
+        e, e0 = self.time_modulation(t)
+        positions = self.session_positions([s.length // tokens - 1 for s in batch.sessions])
+        heads = (rows, cfg.heads, cfg.head_dim)
+        for layer, blk in enumerate(self.blocks):
+            mod = blk["modulation"] + e0
+            y = norms.ln_modulate(x, shift=mod[0], scale=mod[1], eps=cfg.eps)
+            qkv = gemm.linear(y, blk["qkv_w"], blk["qkv_b"])
+            q = torch.empty((rows, cfg.dim), dtype=torch.bfloat16, device=self.device)
+            k = torch.empty_like(q)
+            norms.rms_norm(qkv[:, :cfg.dim], blk["norm_q"], eps=cfg.eps, out=q)
+            norms.rms_norm(qkv[:, cfg.dim:2 * cfg.dim], blk["norm_k"], eps=cfg.eps, out=k)
+            v = qkv[:, 2 * cfg.dim:]
+            if capture is not None:
+                capture(layer, k, v)
+            q = cache.append(layer, batch, q.view(heads), k.view(heads), v.unflatten(1, heads[1:]), positions, self.axis_rope)
+            o = cache.attend(layer, batch, q)
+            gemm.linear_gated_residual(o.view(rows, cfg.dim), blk["o_w"], blk["o_b"], mod[2].contiguous(), x)
+            y = norms.ln_modulate(x, weight=blk["norm3_w"], bias=blk["norm3_b"], eps=cfg.eps)
+            cq = norms.rms_norm(gemm.linear(y, blk["cq_w"], blk["cq_b"]), blk["cnorm_q"], eps=cfg.eps)
+            ck, cv = text_kv[layer]
+            co = attn_ops.attention(cq.view(heads), ck.view(-1, cfg.heads, cfg.head_dim),
+                                    cv.view(-1, cfg.heads, cfg.head_dim))
+            gemm.linear_gated_residual(co.view(rows, cfg.dim), blk["co_w"], blk["co_b"], None, x)
+            y = norms.ln_modulate(x, shift=mod[3], scale=mod[4], eps=cfg.eps)
+            h = gemm.linear_gelu(y, blk["ffn1_w"], blk["ffn1_b"])
+            gemm.linear_gated_residual(h, blk["ffn2_w"], blk["ffn2_b"], mod[5].contiguous(), x)
+        shift = (self.head_mod[0] + e).contiguous()
+        scale = (self.head_mod[1] + e).contiguous()
+        y = norms.ln_modulate(x, shift=shift, scale=scale, eps=cfg.eps)
+        out = gemm.linear(y, self.head_w, self.head_b, out_dtype=torch.float32)
+        return torch.stack([self.unpatchify(one) for one in out.view(sessions, tokens, -1)])
 
     def forward_chunk_sp(self, latents: torch.Tensor, t: float, chunk_index: int, cache: SPKVCache, text_kv, *,
                          group, capture=None, layer_wait=None, attention_backend: str = "auto") -> torch.Tensor:

@@ -4,8 +4,8 @@
 Pages: ``k_pages, v_pages [pages, page_size, kv_heads, head_dim]`` of one layer (any 16-byte aligned strides; the page
 size is a multiple of 8 tokens). A batch of sequences is described by ``block_table [seqs, width]`` (page of each block
 of ``page_size`` tokens, -1 for none), ``kv_lens [seqs]`` (tokens held, the new ones included) and ``cu_q [seqs + 1]``
-(where each sequence's new tokens begin in ``q``), all int32 on the device: nothing is read back, every call can be
-captured in a graph. Sequence ``s``'s new tokens are its last ``cu_q[s + 1] - cu_q[s]`` positions.
+(where each sequence's new tokens begin in ``q``), all int32 on the device (rows of the table may be strided: a slice
+``table[:, :n]`` will do): nothing is read back, every call can be captured in a graph. Sequence ``s``'s new tokens are its last ``cu_q[s + 1] - cu_q[s]`` positions.
 
 Calls with page numbers outside the pool, or page-table calls that cannot be served, do nothing out of bounds and are
 reported by :func:`reelcache_b200.ops._ext.check_status`.

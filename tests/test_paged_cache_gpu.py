@@ -1,0 +1,153 @@
+"""The paged KV cache as a user has it: sessions that fork, rewind and end, and the video DiT over it."""
+
+import importlib.util
+from pathlib import Path
+
+import pytest
+import torch
+
+from .paged_support import attend, spun
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _checked(cuda_device):
+    from reelcache_b200.ops import _ext
+    yield
+    _ext.check_status(cuda_device)
+
+
+def _cache(**kw):
+    from reelcache_b200.paged_cache import PagedKVCache
+    return PagedKVCache(2, 2, 64, **{"pages": 24, "page_size": 16, "max_sessions": 6, "max_tokens": 128, **kw})
+
+
+def test_sessions_follow_their_own_histories():
+    """Forks, rewinds, ends and compactions against histories kept as plain tensors."""
+    from reelcache_b200.ops.rope import AxisRope
+    g = torch.Generator(device="cuda").manual_seed(0)
+    rope = AxisRope.wan(64)
+    cache = _cache()
+    plain = {}  # slot -> per layer (k, v) [tokens, 2, 64]
+    empty = lambda: [(torch.zeros(0, 2, 64, device="cuda").bfloat16(),) * 2 for _ in range(2)]  # noqa: E731
+
+    def step(pairs, causal):
+        batch = cache.extend(pairs)
+        rows = batch.tokens
+        positions = torch.randint(0, 900, (rows, 3), generator=g, device="cuda", dtype=torch.int32)
+        for layer in range(2):
+            q, k, v = (torch.randn(rows, h, 64, generator=g, device="cuda").bfloat16() for h in (4, 2, 2))
+            turned = cache.append(layer, batch, q, k, v, positions, rope)
+            out = cache.attend(layer, batch, turned, causal=causal)
+            at = 0
+            for s, n in pairs:
+                want_k = spun(k[at:at + n], positions[at:at + n], rope.sections, 10000.0, "interleaved")[0]
+                have = plain[s.slot][layer]
+                plain[s.slot][layer] = (torch.cat([have[0], want_k.bfloat16()]), torch.cat([have[1], v[at:at + n]]))
+                kv = plain[s.slot][layer]
+                table = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+                want = attend(turned[at:at + n], kv[0][None], kv[1][None], table, [kv[0].shape[0]], [n], causal=causal)[0]
+                assert float((out[at:at + n].double() - want).norm() / want.norm().clamp(min=1e-9)) < 1e-2
+                at += n
+
+    a = cache.open()
+    plain[a.slot] = empty()
+    step([(a, 37)], False)
+    b, c = cache.fork(a, [37, 20])
+    for s, n in ((b, 37), (c, 20)):
+        plain[s.slot] = [(k[:n], v[:n]) for k, v in plain[a.slot]]
+    assert cache.pages - cache.free_pages == 3 + 1 + 1  # three pages, and a copied tail for each fork
+    step([(a, 1), (b, 1), (c, 1)], True)
+    step([(c, 30), (a, 16)], True)
+    cache.close(a)
+    assert cache.compact() == cache.pages - cache.free_pages
+    step([(b, 40), (c, 5)], False)
+    (d,) = cache.fork(b)
+    plain[d.slot] = [tuple(kv) for kv in plain[b.slot]]
+    step([(d, 3), (b, 11), (c, 2)], True)
+    cache.close(b, c, d)
+    assert cache.free_pages == cache.pages and int(cache.table.refcount.abs().sum()) == 0
+
+
+def test_refusals():
+    from reelcache_b200.errors import CapacityError, ConfigurationError, StateError, UnsupportedError
+    from reelcache_b200.paged_cache import PagedKVCache
+    for wrong in (dict(page_size=12), dict(pages=0), dict(max_sessions=0), dict(max_tokens=0)):
+        with pytest.raises(ConfigurationError):
+            _cache(**wrong)
+    with pytest.raises(UnsupportedError):
+        _cache(device="cpu")
+    with pytest.raises(ConfigurationError):
+        PagedKVCache(1, 1, 96, pages=1, page_size=8, max_sessions=1, max_tokens=8)
+    cache = _cache(pages=6, max_sessions=3)
+    a, b = cache.open(), cache.open()
+    cache.extend([(a, 40), (b, 16)])
+    with pytest.raises(CapacityError):
+        cache.extend([(a, 30), (b, 30)])
+    with pytest.raises(CapacityError):
+        cache.extend([(a, 100)])
+    with pytest.raises(StateError):
+        cache.extend([(a, 1), (a, 1)])
+    with pytest.raises(ConfigurationError):
+        cache.fork(a, [41])
+    with pytest.raises(CapacityError):
+        cache.fork(a, [40, 40])  # one slot left
+    (c,) = cache.fork(a, [32])
+    with pytest.raises(StateError):
+        cache.again([(c, 8)])  # those rows are a's too
+    with pytest.raises(CapacityError):
+        cache.open()
+    cache.close(a)
+    for call in (lambda: cache.close(a), lambda: cache.extend([(a, 1)]), lambda: cache.fork(a), lambda: cache.close(b, b)):
+        with pytest.raises(StateError):
+            call()
+    cache.again([(c, 8)])  # now its own
+    assert cache.free_pages == 3
+
+
+def test_dit_over_pages_equals_the_dense_cache():
+    """The newest chunk of forked sessions in one batched forward, against the contiguous cache session by session."""
+    from reelcache_b200.models.causal_wan import CAUSVID, CausalWanDiT, KVCache
+    from reelcache_b200.paged_cache import PagedKVCache
+    cfg = CAUSVID.scaled(layers=2, dim=256, heads=2, ffn=512, text_dim=128, text_len=16, latent_height=8, latent_width=16)
+    model = CausalWanDiT(cfg, "cuda", seed=3)
+    text_kv = model.encode_text(torch.randn(cfg.text_len, cfg.text_dim, device="cuda"))
+    torch.manual_seed(0)
+    draw = lambda: torch.randn(cfg.in_dim, cfg.frames_per_chunk, cfg.latent_height, cfg.latent_width, device="cuda")  # noqa: E731
+    first, second, left, right = (draw() for _ in range(4))
+    cache = PagedKVCache(cfg.layers, cfg.heads, cfg.head_dim, pages=40, page_size=cfg.tokens_per_frame, max_sessions=4,
+                         max_tokens=4 * cfg.chunk_tokens)
+    root = cache.open()
+    captured = {}
+    for x in (first, second):
+        batch = cache.extend([(root, cfg.chunk_tokens)])
+        model.forward_sessions(x[None], 500.0, cache, batch, text_kv, capture=lambda l, k, v: captured.__setitem__(l, (k.clone(), v.clone())))
+    a, b = cache.fork(root, [2 * cfg.chunk_tokens, cfg.chunk_tokens])
+    batch = cache.extend([(a, cfg.chunk_tokens), (b, cfg.chunk_tokens)])
+    got = model.forward_sessions(torch.stack([left, right]), 250.0, cache, batch, text_kv)
+    for latents, history, out in ((left, [first, second], got[0]), (right, [first], got[1])):
+        dense = KVCache(cfg, 4, "cuda")
+        kept = {}
+        for i, x in enumerate(history):
+            model.forward_chunk(x, 500.0, i, dense, text_kv, capture=lambda l, k, v: kept.__setitem__(l, (k.clone(), v.clone())))
+        if len(history) == 2:
+            for layer in range(cfg.layers):
+                for x, y in zip(captured[layer], kept[layer]):
+                    assert float((x.float() - y.float()).norm() / y.float().norm()) < 1e-2
+        want = model.forward_chunk(latents, 250.0, len(history), dense, text_kv)
+        assert float((out - want).norm() / want.norm()) < 2e-2
+    with pytest.raises(ValueError):
+        model.forward_sessions(left[None], 250.0, cache, cache.extend([(root, 5)]), text_kv)
+
+
+def test_example_runs():
+    path = Path(__file__).resolve().parents[1] / "examples" / "paged_sessions.py"
+    spec = importlib.util.spec_from_file_location("paged_sessions", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    from reelcache_b200.models.causal_wan import CAUSVID
+    report = module.run(CAUSVID.scaled(**module.SMALL), chunks=3, branches=4, steps=1)
+    assert report["history_pages"] == 9 and report["pages_after_forks"] == 9 and report["pages_if_copied"] == 30
+    assert report["batched_vs_separate_difference"] < 2e-2
+    assert report["pages_after_compaction"] == 9 + 2 * 3 and report["pages_used_at_the_end"] == 9 + 4 * 3
