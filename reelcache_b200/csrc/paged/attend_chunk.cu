@@ -141,7 +141,8 @@ __device__ __forceinline__ int tiles_of(const Args& a, const Item& item, const R
 
 __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const __grid_constant__ Chunk p) {
   __shared__ int warp_sums[32];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  let_later();
+  after_earlier();
   const Args& a = p.a;
   const Plan& plan = p.plan;
   auto row_tiles = [&](int q_len) {
@@ -433,8 +434,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int cta = blockIdx.x;
   Segment seg;
-  if (kDirect && !seg.direct(p, cta)) return;  // the whole cluster
 
+  let_later();
   if (threadIdx.x == 0) {
     mbar_init(q_full, 32);
     mbar_init(q_empty, 1);
@@ -460,17 +461,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     tma_prefetch_desc(&maps.k_wide);
     tma_prefetch_desc(&maps.v_wide);
   }
+  after_earlier();
+  if (kDirect && !seg.direct(p, cta)) return;  // the whole cluster
   if (warp == 10) tmem_alloc(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   Share share{};
-  if (!kDirect) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // the plan
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    share = Share(p, cta);
-  }
+  if (!kDirect) share = Share(p, cta);
   auto next = [&](int n) { return kDirect ? n == 0 && seg.t0 < seg.t1 : seg.load(p, share, cta, n); };
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRoleRegs));
@@ -840,7 +839,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 template <typename T, int D>
 __global__ void __launch_bounds__(256) chunk_join_kernel(const __grid_constant__ Chunk p) {
   constexpr int kPer = D / 32;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  let_later();
+  after_earlier();
   const Args& a = p.a;
   const int c0 = blockIdx.y;
   const int cut = p.plan.cut[c0 + 1];
@@ -977,25 +977,14 @@ void chunk_launch(const Args& args, const at::Tensor& k_pages, const at::Tensor&
   p.most_items = static_cast<int>(most_items);
   p.ctas = sm_count(device);
   const PageMaps maps = page_maps(k_pages, v_pages, p.a.tiling, kTile);
-  cudaLaunchConfig_t config{};
-  config.blockDim = dim3(kChunkThreads);
-  config.dynamicSmemBytes = Shape::bytes;
-  config.stream = stream;
-  cudaLaunchAttribute attribute{};
-  config.attrs = &attribute;
-  config.numAttrs = 1;
   // tiles of an item, at most: the table's width, or what a window leaves of it
   int64_t keys = static_cast<int64_t>(args.width) * args.tiling.page;
   if (args.window > 0) keys = std::min<int64_t>(keys, static_cast<int64_t>(args.window) + args.sinks + kItemRows / args.group + 2 * kTile);
   chunk_configure<T, D, true>();
   p.cluster = direct_cluster<T, D>(most_items, (keys + kTile - 1) / kTile, args.causal && row_tiles > 1, device);
   if (p.cluster > 0) {
-    config.gridDim = dim3(static_cast<unsigned>(grid_items * p.cluster));
-    attribute.id = cudaLaunchAttributeClusterDimension;
-    attribute.val.clusterDim.x = p.cluster;
-    attribute.val.clusterDim.y = 1;
-    attribute.val.clusterDim.z = 1;
-    RC_CUDA(cudaLaunchKernelEx(&config, chunk_kernel<T, D, true>, maps, p));
+    launch(chunk_kernel<T, D, true>, dim3(static_cast<unsigned>(grid_items * p.cluster)), kChunkThreads, Shape::bytes, p.cluster,
+           stream, maps, p);
     return;
   }
   chunk_configure<T, D, false>();
@@ -1010,16 +999,9 @@ void chunk_launch(const Args& args, const at::Tensor& k_pages, const at::Tensor&
   p.plan.cut = p.plan.head + 4;
   p.plan.first = p.plan.cut + p.ctas + 1;
   p.plan.base = p.plan.first + p.ctas + 1;
-  chunk_plan_kernel<<<1, kPlanThreads, 0, stream>>>(p);
-  RC_CUDA(cudaGetLastError());
-  config.gridDim = dim3(p.ctas);
-  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute.val.programmaticStreamSerializationAllowed = 1;
-  RC_CUDA(cudaLaunchKernelEx(&config, chunk_kernel<T, D, false>, maps, p));
-  config.gridDim = dim3(kItemRows / 8, p.ctas - 1);
-  config.blockDim = dim3(256);
-  config.dynamicSmemBytes = 0;
-  RC_CUDA(cudaLaunchKernelEx(&config, chunk_join_kernel<T, D>, p));
+  launch(chunk_plan_kernel, dim3(1), kPlanThreads, 0, 0, stream, p);
+  launch(chunk_kernel<T, D, false>, dim3(p.ctas), kChunkThreads, Shape::bytes, 0, stream, maps, p);
+  launch(chunk_join_kernel<T, D>, dim3(kItemRows / 8, p.ctas - 1), 256, 0, 0, stream, p);
 }
 
 void attend_chunk(const Args& a, int head_dim, bool half, const at::Tensor& k_pages, const at::Tensor& v_pages,

@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
   const Args& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  let_later();
   if (threadIdx.x == 0) {
     for (int s = 0; s < Shape::stages; ++s) {
       mbar_init(&full[s], 1);
@@ -133,6 +133,7 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
     tma_prefetch_desc(&maps.k_wide);
     tma_prefetch_desc(&maps.v_wide);
   }
+  after_earlier();
   if (kCluster) {
     // A cluster per sequence and KV head: this CTA's tiles are its rank's part of the item's, and the line is the item.
     __syncthreads();
@@ -608,9 +609,9 @@ __global__ void __launch_bounds__(128) short_join_kernel(const __grid_constant__
   const int quads = p.rows / 4;
   const int row = (blockIdx.x % quads) * 4 + (threadIdx.x >> 5);
   const int item = blockIdx.x / quads, s = item / a.kv_heads, head = item - s * a.kv_heads;
-  const SeqWork w(a, s);  // the call's inputs: they do not wait for the first kernel
-  // every block waits, so that this kernel never ends before the first one does
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  let_later();
+  after_earlier();
+  const SeqWork w(a, s);
   const int query = row / a.group;
   if (query >= w.q_len) return;
   const int share = *p.line.share;
@@ -680,12 +681,6 @@ void short_launch(Args a, const at::Tensor& k_pages, const at::Tensor& v_pages, 
   p.a.tiling = Tiling::of(a.tiling.page, kShortTile);
   const PageMaps maps = page_maps(k_pages, v_pages, p.a.tiling, kShortTile);
   const int64_t items = static_cast<int64_t>(a.seqs) * a.kv_heads, slots = sm_count(device) * kShortCtasPerSm;
-  cudaLaunchConfig_t config{};
-  config.blockDim = dim3(kShortThreads);
-  config.dynamicSmemBytes = Shape::bytes;
-  config.stream = stream;
-  cudaLaunchAttribute attribute{};
-  config.attrs = &attribute;
   // Clusters of the largest size that all find room at once, unless the table's width allows sequences so long that an
   // even share of all tiles matters more than the second kernel that it costs (measured on one B200, 8 KV heads: one
   // session of 2,048 keys 8.3 us clustered and 11.7 us shared out, 16 sessions of 512 keys 11 and 14 us, one session of
@@ -694,13 +689,8 @@ void short_launch(Args a, const at::Tensor& k_pages, const at::Tensor& v_pages, 
   for (int c = 16; c > 1 && p.cluster == 0; c /= 2)
     if (items * c <= slots && most_tiles <= c * (c >= 8 ? kLongTiles : kFewTiles)) p.cluster = c;
   if (p.cluster > 0) {
-    config.gridDim = dim3(static_cast<unsigned>(items * p.cluster));
-    attribute.id = cudaLaunchAttributeClusterDimension;
-    attribute.val.clusterDim.x = p.cluster;
-    attribute.val.clusterDim.y = 1;
-    attribute.val.clusterDim.z = 1;
-    config.numAttrs = 1;
-    RC_CUDA(cudaLaunchKernelEx(&config, short_kernel<T, D, kM, true>, maps, p));
+    launch(short_kernel<T, D, kM, true>, dim3(static_cast<unsigned>(items * p.cluster)), kShortThreads, Shape::bytes, p.cluster,
+           stream, maps, p);
     return;
   }
   const int ctas = static_cast<int>(std::min<int64_t>(slots, items * (most_tiles + 1)));
@@ -711,15 +701,8 @@ void short_launch(Args a, const at::Tensor& k_pages, const at::Tensor& v_pages, 
   p.part_ml = p.part_o + 2ll * ctas * kRows * D;
   int* line = reinterpret_cast<int*>(p.part_o + floats);
   p.line = {line, line + 1, line + 1 + a.seqs};
-  config.gridDim = dim3(ctas);
-  RC_CUDA(cudaLaunchKernelEx(&config, short_kernel<T, D, kM, false>, maps, p));
-  config.gridDim = dim3(static_cast<unsigned>(items * (kRows / 4)));
-  config.blockDim = dim3(128);
-  config.dynamicSmemBytes = 0;
-  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute.val.programmaticStreamSerializationAllowed = 1;
-  config.numAttrs = 1;
-  RC_CUDA(cudaLaunchKernelEx(&config, short_join_kernel<T, D>, p));
+  launch(short_kernel<T, D, kM, false>, dim3(ctas), kShortThreads, Shape::bytes, 0, stream, maps, p);
+  launch(short_join_kernel<T, D>, dim3(static_cast<unsigned>(items * (kRows / 4))), 128, 0, 0, stream, p);
 }
 
 template <typename T, int D>
@@ -727,8 +710,7 @@ void short_rows(const Args& a, const at::Tensor& k_pages, const at::Tensor& v_pa
                 cudaStream_t stream, int device) {
   const int64_t rows = static_cast<int64_t>(max_q_len) * a.group;
   if (rows <= 16) short_launch<T, D, 1>(a, k_pages, v_pages, like, stream, device);
-  else if (rows <= 32) short_launch<T, D, 2>(a, k_pages, v_pages, like, stream, device);
-  else short_launch<T, D, 4>(a, k_pages, v_pages, like, stream, device);
+  else short_launch<T, D, 2>(a, k_pages, v_pages, like, stream, device);
 }
 
 void attend_short(const Args& a, int head_dim, bool half, const at::Tensor& k_pages, const at::Tensor& v_pages,

@@ -17,6 +17,34 @@ constexpr int kPageRange = 0x403;
 
 namespace paged {
 
+// Every kernel here is launched as a programmatic dependent of what runs before it on the stream: its launch and its setup
+// overlap that kernel's end. after_earlier() comes before its first access to global memory and waits until everything
+// before it on the stream is complete and visible; let_later() allows the next such kernel to be set up.
+#ifdef __CUDACC__
+__device__ __forceinline__ void after_earlier() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_later() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// `cluster` CTAs to a cluster (0: no clusters).
+template <typename... Params, typename... Args>
+void launch(void (*kernel)(Params...), dim3 grid, int threads, int smem, int cluster, cudaStream_t stream, const Args&... args) {
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid;
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  cudaLaunchAttribute attributes[2] = {};
+  attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[0].val.programmaticStreamSerializationAllowed = 1;
+  attributes[1].id = cudaLaunchAttributeClusterDimension;
+  attributes[1].val.clusterDim.x = cluster;
+  attributes[1].val.clusterDim.y = 1;
+  attributes[1].val.clusterDim.z = 1;
+  config.attrs = attributes;
+  config.numAttrs = cluster > 0 ? 2 : 1;
+  RC_CUDA(cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...));
+}
+#endif
+
 struct Pages {  // [pages, page_size, kv_heads, head_dim], strides in elements
   int count, size;
   int64_t page_stride, token_stride, head_stride;

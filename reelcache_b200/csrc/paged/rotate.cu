@@ -9,17 +9,22 @@
 // fma(p, hi, -n) + p lo is the fraction of a turn, exact to an ULP of 0.5 however many turns p makes (p w in radians
 // would lose one bit for each doubling of p). sincospi takes it from there.
 //
-// What bounds it: memory, one read and one write of q, k (and v). So a thread owns one 16-byte vector position of a
-// token (4 or 8 pairs), computes their sines once and applies them to kHeads heads, whose loads are all issued before
-// the sines are computed. Neighbouring threads take neighbouring vectors, then neighbouring heads: every warp access
-// covers whole 256-byte head rows. The fused form writes k and v through the block table, so the rotated keys never
-// exist outside the cache.
+// What bounds it: memory, one read and one write of q, k (and v); next, the sines. So a thread owns one 16-byte vector
+// position of a token (4 or 8 pairs), computes their sines once and applies them to as many heads of one tensor as leave
+// every SM full; the loads of the first heads are issued before the sines are computed. A warp access covers whole heads
+// (256 bytes each). A block works on one tensor, so nothing of it branches: v takes no sines, q no pages. The fused form
+// writes k and v through the block table, so the rotated keys never exist outside the cache.
+//
+// 16-bit types take sin and cos from the special function unit (off by at most 2^-21, a thousandth of what rounding to
+// fp16 loses), fp32 takes sincospi.
 #include <ATen/ATen.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <algorithm>
 
 #include "../common/host.h"
 #include "paged.h"
@@ -97,6 +102,8 @@ struct Rows {  // one tensor [tokens, heads, head_dim]: byte strides
   char* dst;
   int64_t src_token, src_head, dst_token, dst_head;
   int heads;
+  int per;     // heads of a thread
+  int groups;  // threads that share a token and vector
 };
 
 struct Args {
@@ -108,7 +115,6 @@ struct Args {
   const float* turns;      // [2, pairs]: hi, lo
   float sign;              // -1 turns back
   int tokens, pairs;
-  int groups;              // head groups: thread group g takes heads g, g + groups, ...
   // the paged form: k and v rows go to page table[seq][at / page], row at % page
   const int* table;
   const int* kv_lens;
@@ -122,66 +128,61 @@ struct Args {
 // kHalves: pairs (j, j + pairs), a thread holds one vector of each half; else neighbours in one vector.
 template <typename T, bool kHalves, bool kPaged, int kHeads>
 __global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant__ Args a) {
+  paged::let_later();
+  paged::after_earlier();
   constexpr int kVec = Vec<T>::n;
   constexpr int kPairs = kHalves ? kVec : kVec / 2;  // pairs a thread turns
   constexpr int kParts = kHalves ? 2 : 1;            // vectors a thread holds per head
   const int per_row = a.pairs / kPairs;
   const int64_t index = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  const int64_t item = index / per_row;
-  const int vec = static_cast<int>(index - item * per_row);
-  const int token = static_cast<int>(item / a.groups);
-  const int group = static_cast<int>(item - static_cast<int64_t>(token) * a.groups);
+  const int token = static_cast<int>(index / per_row);
+  const int vec = static_cast<int>(index - static_cast<int64_t>(token) * per_row);
   if (token >= a.tokens) return;
-  const int heads = a.q.heads + a.k.heads + a.v.heads;
+  const int y = blockIdx.y;
+  const bool is_q = y < a.q.groups, is_k = !is_q && y < a.q.groups + a.k.groups;
+  const Rows& r = is_q ? a.q : is_k ? a.k : a.v;
+  const int first = (is_q ? y : is_k ? y - a.q.groups : y - a.q.groups - a.k.groups) * r.per;
+  const int count = min(r.heads - first, r.per);
   const int part_bytes = a.pairs * static_cast<int>(sizeof(T));  // from the first half of a head to the second
+  const char* src = r.src + token * r.src_token + first * r.src_head + vec * 16;
 
   uint4 raw[kHeads][kParts];
+  auto load = [&](int done) {
 #pragma unroll
-  for (int i = 0; i < kHeads; ++i) {
-    int h = group + i * a.groups;
-    if (h >= heads) continue;
-    const Rows* r = &a.q;
-    if (h >= a.q.heads) {
-      h -= a.q.heads;
-      r = &a.k;
-      if (h >= a.k.heads) {
-        h -= a.k.heads;
-        r = &a.v;
+    for (int i = 0; i < kHeads; ++i) {
+      if (done + i < count) {
+#pragma unroll
+        for (int s = 0; s < kParts; ++s) raw[i][s] = __ldg(reinterpret_cast<const uint4*>(src + i * r.src_head + s * part_bytes));
       }
     }
-    const char* p = r->src + token * r->src_token + h * r->src_head + vec * 16;
-#pragma unroll
-    for (int s = 0; s < kParts; ++s) raw[i][s] = __ldg(reinterpret_cast<const uint4*>(p + s * part_bytes));
-  }
+    src += kHeads * r.src_head;
+  };
+  load(0);
 
-  // the token's page (the paged form)
-  int64_t page = 0;
-  int row = 0;
-  bool stored = true;
-  if (kPaged) {
+  char* dst = r.dst + first * r.dst_head + vec * 16;
+  if (!kPaged || is_q) {
+    dst += token * r.dst_token;
+  } else {
     int lo = 0, hi = a.seqs - 1;  // the last sequence that starts at or before the token
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
       if (__ldg(a.cu_q + mid) <= token) lo = mid;
       else hi = mid - 1;
     }
-    const int first = __ldg(a.cu_q + lo), end = __ldg(a.cu_q + lo + 1);
+    const int begin = __ldg(a.cu_q + lo), end = __ldg(a.cu_q + lo + 1);
+    if (token < begin || token >= end) return;  // tokens past the last sequence belong to none
     const int at = __ldg(a.kv_lens + lo) - end + token;
-    stored = token >= first && token < end;  // tokens past the last sequence belong to none
-    if (stored) {
-      const int slot = at >= 0 ? at / a.page : -1;
-      row = at - slot * a.page;
-      page = slot >= 0 && slot < a.table_width ? __ldg(a.table + lo * a.table_row + slot) : -1;
-      if (page < 0 || page >= a.pages) {
-        stored = false;
-        if (vec == 0 && group == 0 && a.status != nullptr) atomicCAS(a.status + kPagedWord, 0, kPageRange);
-      }
+    const int slot = at >= 0 ? at / a.page : -1;
+    const int page = slot >= 0 && slot < a.table_width ? __ldg(a.table + lo * a.table_row + slot) : -1;
+    if (page < 0 || page >= a.pages) {
+      if (vec == 0 && a.status != nullptr) atomicCAS(a.status + kPagedWord, 0, kPageRange);
+      return;
     }
+    dst += page * (is_k ? a.page_k : a.page_v) + (at - slot * a.page) * r.dst_token;
   }
 
   float cs[kPairs], sn[kPairs];
-  {
-    const int j0 = vec * kPairs;
+  if (!kPaged || is_q || is_k) {
     float p[4];
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
@@ -193,87 +194,86 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant_
       }
     }
 #pragma unroll
-    for (int e = 0; e < kPairs; ++e) {
-      const int j = j0 + e;
-      const float pos = j < a.ends[0] ? p[0] : j < a.ends[1] ? p[1] : j < a.ends[2] ? p[2] : p[3];
-      const float hi = __ldg(a.turns + j), lo = __ldg(a.turns + a.pairs + j);
-      const float n = rintf(pos * hi);
-      const float part = fmaf(pos, lo, fmaf(pos, hi, -n));
-      sincospif(2.0f * part, &sn[e], &cs[e]);
-      sn[e] *= a.sign;
+    for (int e0 = 0; e0 < kPairs; e0 += 2) {
+      const int j0 = vec * kPairs + e0;
+      const float2 hi2 = __ldg(reinterpret_cast<const float2*>(a.turns + j0));
+      const float2 lo2 = __ldg(reinterpret_cast<const float2*>(a.turns + a.pairs + j0));
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int j = j0 + e;
+        const float pos = j < a.ends[0] ? p[0] : j < a.ends[1] ? p[1] : j < a.ends[2] ? p[2] : p[3];
+        const float hi = e ? hi2.y : hi2.x, lo = e ? lo2.y : lo2.x;
+        const float part = fmaf(pos, lo, fmaf(pos, hi, -rintf(pos * hi)));
+        if (sizeof(T) == 4) {
+          sincospif(2.0f * part, &sn[e0 + e], &cs[e0 + e]);
+        } else {
+          __sincosf(6.283185307179586f * part, &sn[e0 + e], &cs[e0 + e]);
+        }
+        sn[e0 + e] *= a.sign;
+      }
     }
   }
 
+  for (int done = 0;;) {
 #pragma unroll
-  for (int i = 0; i < kHeads; ++i) {
-    int h = group + i * a.groups;
-    if (h >= heads) continue;
-    const Rows* r = &a.q;
-    int64_t base = token * a.q.dst_token;
-    bool turn = true;
-    if (h >= a.q.heads) {
-      if (kPaged && !stored) continue;
-      h -= a.q.heads;
-      r = &a.k;
-      base = kPaged ? page * a.page_k + row * a.k.dst_token : token * a.k.dst_token;
-      if (h >= a.k.heads) {
-        h -= a.k.heads;
-        r = &a.v;
-        base = page * a.page_v + row * a.v.dst_token;
-        turn = false;
-      }
-    }
-    if (turn) {
-      if (kHalves) {
-        float x[kVec], y[kVec];
-        Vec<T>::unpack(raw[i][0], x);
-        Vec<T>::unpack(raw[i][kParts - 1], y);
+    for (int i = 0; i < kHeads; ++i) {
+      if (done + i >= count) continue;
+      if (!kPaged || is_q || is_k) {
+        if (kHalves) {
+          float x[kVec], y2[kVec];
+          Vec<T>::unpack(raw[i][0], x);
+          Vec<T>::unpack(raw[i][kParts - 1], y2);
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) {
-          const float u = x[e] * cs[e % kPairs] - y[e] * sn[e % kPairs];
-          y[e] = x[e] * sn[e % kPairs] + y[e] * cs[e % kPairs];
-          x[e] = u;
+          for (int e = 0; e < kVec; ++e) {
+            const float u = x[e] * cs[e % kPairs] - y2[e] * sn[e % kPairs];
+            y2[e] = x[e] * sn[e % kPairs] + y2[e] * cs[e % kPairs];
+            x[e] = u;
+          }
+          raw[i][0] = Vec<T>::pack(x);
+          raw[i][kParts - 1] = Vec<T>::pack(y2);
+        } else {
+          float x[kVec];
+          Vec<T>::unpack(raw[i][0], x);
+#pragma unroll
+          for (int e = 0; e < kVec / 2; ++e) {
+            const float u = x[2 * e] * cs[e] - x[2 * e + 1] * sn[e];
+            x[2 * e + 1] = x[2 * e] * sn[e] + x[2 * e + 1] * cs[e];
+            x[2 * e] = u;
+          }
+          raw[i][0] = Vec<T>::pack(x);
         }
-        raw[i][0] = Vec<T>::pack(x);
-        raw[i][kParts - 1] = Vec<T>::pack(y);
-      } else {
-        float x[kVec];
-        Vec<T>::unpack(raw[i][0], x);
-#pragma unroll
-        for (int e = 0; e < kVec / 2; ++e) {
-          const float u = x[2 * e] * cs[e] - x[2 * e + 1] * sn[e];
-          x[2 * e + 1] = x[2 * e] * sn[e] + x[2 * e + 1] * cs[e];
-          x[2 * e] = u;
-        }
-        raw[i][0] = Vec<T>::pack(x);
       }
-    }
-    char* p = r->dst + base + h * r->dst_head + vec * 16;
 #pragma unroll
-    for (int s = 0; s < kParts; ++s) *reinterpret_cast<uint4*>(p + s * part_bytes) = raw[i][s];
+      for (int s = 0; s < kParts; ++s) *reinterpret_cast<uint4*>(dst + i * r.dst_head + s * part_bytes) = raw[i][s];
+    }
+    done += kHeads;
+    if (done >= count) break;
+    dst += kHeads * r.dst_head;
+    load(done);
   }
 }
 
 template <typename T, bool kHalves, bool kPaged>
 void launch(Args a, cudaStream_t stream, int sms) {
-  const int heads = a.q.heads + a.k.heads + a.v.heads;
   const int per_row = a.pairs / (kHalves ? Vec<T>::n : Vec<T>::n / 2);
-  // Heads per thread: as many as leave every SM a full set of threads.
-  const int64_t wanted = static_cast<int64_t>(sms) * 2048;
-  int n = 8;
-  while (n > 1 && static_cast<int64_t>(a.tokens) * per_row * ((heads + n - 1) / n) < wanted) n /= 2;
-  a.groups = (heads + n - 1) / n;
-  const int64_t threads = static_cast<int64_t>(a.tokens) * per_row * a.groups;
-  const int64_t blocks = (threads + kThreads - 1) / kThreads;
-  RC_CHECK(blocks < (1ll << 31), "too many tokens for one launch");
-  const dim3 grid(static_cast<unsigned>(blocks));
-  switch (n) {
-    case 1: rotate_kernel<T, kHalves, kPaged, 1><<<grid, kThreads, 0, stream>>>(a); break;
-    case 2: rotate_kernel<T, kHalves, kPaged, 2><<<grid, kThreads, 0, stream>>>(a); break;
-    case 4: rotate_kernel<T, kHalves, kPaged, 4><<<grid, kThreads, 0, stream>>>(a); break;
-    default: rotate_kernel<T, kHalves, kPaged, 8><<<grid, kThreads, 0, stream>>>(a); break;
+  const int64_t rows = static_cast<int64_t>(a.tokens) * per_row;
+  const int heads = a.q.heads + a.k.heads + a.v.heads;
+  // Heads of a thread: as many as leave every SM a full set of threads, and then evenly spread over a tensor's threads.
+  const int most = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(64, rows * heads / (static_cast<int64_t>(sms) * 2048))));
+  int widest = 1;
+  for (Rows* r : {&a.q, &a.k, &a.v}) {
+    r->groups = (r->heads + most - 1) / most;
+    r->per = r->groups > 0 ? (r->heads + r->groups - 1) / r->groups : 1;
+    widest = std::max(widest, r->per);
   }
-  RC_CUDA(cudaGetLastError());
+  const int64_t blocks = (rows + kThreads - 1) / kThreads;
+  const int groups = a.q.groups + a.k.groups + a.v.groups;
+  RC_CHECK(blocks < (1ll << 31) && groups < 65536, "too many tokens or heads for one launch");
+  const dim3 grid(static_cast<unsigned>(blocks), groups);
+  // loads in flight: 4 heads at a time (halves hold two vectors of each)
+  if (widest == 1) paged::launch(rotate_kernel<T, kHalves, kPaged, 1>, grid, kThreads, 0, 0, stream, a);
+  else if (widest == 2) paged::launch(rotate_kernel<T, kHalves, kPaged, 2>, grid, kThreads, 0, 0, stream, a);
+  else paged::launch(rotate_kernel<T, kHalves, kPaged, kHalves ? 4 : 8>, grid, kThreads, 0, 0, stream, a);
 }
 
 template <bool kPaged>

@@ -113,6 +113,8 @@ __device__ __forceinline__ bool take(int* seen, int seq) { return atomicExch(see
 __global__ void __launch_bounds__(kPlanThreads) allocate_kernel(State s, const int* __restrict__ seqs,
                                                                 const int* __restrict__ lens, int n, int* list,
                                                                 int* offsets, int* seen, int* status) {
+  paged::let_later();
+  paged::after_earlier();
   __shared__ int warp_sums[32];
   __shared__ int bad;
   if (threadIdx.x == 0) bad = 0;
@@ -168,6 +170,8 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(State s, const 
                                                                  const int* __restrict__ children,
                                                                  const int* __restrict__ at, int n, int* list, int* seen,
                                                                  Plan plan, int* status) {
+  paged::let_later();
+  paged::after_earlier();
   __shared__ int warp_sums[32];
   __shared__ int bad;
   if (threadIdx.x == 0) bad = 0;
@@ -208,6 +212,8 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(State s, const 
 }
 
 __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(State s, int* place, Plan plan, int* in_use) {
+  paged::let_later();
+  paged::after_earlier();
   __shared__ int warp_sums[32];
   int live = 0;
   for (int base = 0; base < s.pages; base += kPlanThreads * 4) {
@@ -306,12 +312,16 @@ __device__ __forceinline__ void move_pages(const Storage& st, int moves, int pag
 __global__ void __launch_bounds__(kMoveThreads) copy_kernel(Storage st, int pages, const int* __restrict__ source,
                                                             const int* __restrict__ target, const int* __restrict__ rows,
                                                             int moves, int* status) {
+  paged::let_later();
+  paged::after_earlier();
   move_pages(st, moves, pages, source, target, rows, status);
 }
 
 __global__ void __launch_bounds__(kMoveThreads) fork_kernel(State s, Storage st, const int* __restrict__ parents,
                                                             const int* __restrict__ children, const int* __restrict__ at,
                                                             int n, Plan plan, int* status) {
+  paged::let_later();
+  paged::after_earlier();
   if (*plan.count < 0) return;
   const int64_t cells = static_cast<int64_t>(n) * s.width;
   for (int64_t c = static_cast<int64_t>(blockIdx.x) * kMoveThreads + threadIdx.x; c < cells;
@@ -334,6 +344,8 @@ __global__ void __launch_bounds__(kMoveThreads) fork_kernel(State s, Storage st,
 
 __global__ void __launch_bounds__(kMoveThreads) compact_kernel(State s, Storage st, const int* __restrict__ place,
                                                                const int* __restrict__ in_use, Plan plan, int* status) {
+  paged::let_later();
+  paged::after_earlier();
   const int moves = *plan.count, live = *in_use;
   const int64_t cells = static_cast<int64_t>(s.seqs) * s.width;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kMoveThreads;
@@ -350,6 +362,8 @@ __global__ void __launch_bounds__(kMoveThreads) compact_kernel(State s, Storage 
 }
 
 __global__ void __launch_bounds__(kMoveThreads) release_kernel(State s, const int* __restrict__ seqs, int n, int* status) {
+  paged::let_later();
+  paged::after_earlier();
   const int64_t cells = static_cast<int64_t>(n) * s.width;
   for (int64_t c = static_cast<int64_t>(blockIdx.x) * kMoveThreads + threadIdx.x; c < cells;
        c += static_cast<int64_t>(gridDim.x) * kMoveThreads) {
@@ -430,10 +444,9 @@ void pages_allocate(at::Tensor& refcount, at::Tensor& lens, at::Tensor& table, i
   cudaStream_t stream = c10::cuda::getCurrentCUDAStream(refcount.get_device()).stream();
   at::Tensor scratch = at::empty({s.pages + n + 1 + s.seqs}, refcount.options());
   int* list = scratch.data_ptr<int>();
-  pagetable::allocate_kernel<<<1, pagetable::kPlanThreads, 0, stream>>>(s, ids, to, static_cast<int>(n), list,
+  paged::launch(pagetable::allocate_kernel, dim3(1), pagetable::kPlanThreads, 0, 0, stream, s, ids, to, static_cast<int>(n), list,
                                                                        list + s.pages, list + s.pages + n + 1,
                                                                        status_ptr(status));
-  RC_CUDA(cudaGetLastError());
 }
 
 void pages_fork(at::Tensor& refcount, at::Tensor& lens, at::Tensor& table, int64_t page_size, const at::Tensor& parents,
@@ -452,12 +465,10 @@ void pages_fork(at::Tensor& refcount, at::Tensor& lens, at::Tensor& table, int64
   int* p = scratch.data_ptr<int>();
   const pagetable::Plan plan{p, p + 1, p + 1 + n, p + 1 + 2 * n};
   int* list = p + 1 + 3 * n;
-  pagetable::fork_plan_kernel<<<1, pagetable::kPlanThreads, 0, stream>>>(s, from, to, len, static_cast<int>(n), list,
+  paged::launch(pagetable::fork_plan_kernel, dim3(1), pagetable::kPlanThreads, 0, 0, stream, s, from, to, len, static_cast<int>(n), list,
                                                                         list + s.pages, plan, status_ptr(status));
-  RC_CUDA(cudaGetLastError());
-  pagetable::fork_kernel<<<pagetable::move_grid(refcount.get_device()), pagetable::kMoveThreads, 0, stream>>>(
+  paged::launch(pagetable::fork_kernel, dim3(pagetable::move_grid(refcount.get_device())), pagetable::kMoveThreads, 0, 0, stream,
       s, st, from, to, len, static_cast<int>(n), plan, status_ptr(status));
-  RC_CUDA(cudaGetLastError());
 }
 
 void pages_release(at::Tensor& refcount, at::Tensor& lens, at::Tensor& table, int64_t page_size, const at::Tensor& seqs,
@@ -470,8 +481,7 @@ void pages_release(at::Tensor& refcount, at::Tensor& lens, at::Tensor& table, in
   cudaStream_t stream = c10::cuda::getCurrentCUDAStream(refcount.get_device()).stream();
   const int64_t blocks = (n * s.width + pagetable::kMoveThreads - 1) / pagetable::kMoveThreads;
   const int grid = static_cast<int>(std::min<int64_t>(blocks, pagetable::move_grid(refcount.get_device())));
-  pagetable::release_kernel<<<grid, pagetable::kMoveThreads, 0, stream>>>(s, ids, static_cast<int>(n), status_ptr(status));
-  RC_CUDA(cudaGetLastError());
+  paged::launch(pagetable::release_kernel, dim3(grid), pagetable::kMoveThreads, 0, 0, stream, s, ids, static_cast<int>(n), status_ptr(status));
 }
 
 // Returns an int32 tensor of one entry: the pages in use, which after the call are pages 0 .. in_use.
@@ -486,11 +496,9 @@ at::Tensor pages_compact(at::Tensor& refcount, at::Tensor& lens, at::Tensor& tab
   int* p = scratch.data_ptr<int>();
   const pagetable::Plan plan{p, p + 1, p + 1 + s.pages, nullptr};
   int* place = p + 1 + 2 * static_cast<int64_t>(s.pages);
-  pagetable::compact_plan_kernel<<<1, pagetable::kPlanThreads, 0, stream>>>(s, place, plan, in_use.data_ptr<int>());
-  RC_CUDA(cudaGetLastError());
-  pagetable::compact_kernel<<<pagetable::move_grid(refcount.get_device()), pagetable::kMoveThreads, 0, stream>>>(
+  paged::launch(pagetable::compact_plan_kernel, dim3(1), pagetable::kPlanThreads, 0, 0, stream, s, place, plan, in_use.data_ptr<int>());
+  paged::launch(pagetable::compact_kernel, dim3(pagetable::move_grid(refcount.get_device())), pagetable::kMoveThreads, 0, 0, stream,
       s, st, place, in_use.data_ptr<int>(), plan, status_ptr(status));
-  RC_CUDA(cudaGetLastError());
   return in_use;
 }
 
@@ -507,9 +515,8 @@ void pages_copy(at::Tensor& storage, const at::Tensor& source, const at::Tensor&
   if (n == 0) return;
   c10::cuda::CUDAGuard guard(storage.device());
   cudaStream_t stream = c10::cuda::getCurrentCUDAStream(storage.get_device()).stream();
-  pagetable::copy_kernel<<<pagetable::move_grid(storage.get_device()), pagetable::kMoveThreads, 0, stream>>>(
+  paged::launch(pagetable::copy_kernel, dim3(pagetable::move_grid(storage.get_device())), pagetable::kMoveThreads, 0, 0, stream,
       st, static_cast<int>(storage.size(1)), from, to, part, static_cast<int>(n), status_ptr(status));
-  RC_CUDA(cudaGetLastError());
 }
 
 }  // namespace rc
