@@ -71,14 +71,14 @@ std::pair<at::Tensor, c10::optional<at::Tensor>> paged_attention(
     const at::Tensor& kv_lens, const at::Tensor& cu_q, int64_t max_q_len, bool causal, int64_t window, int64_t sinks,
     c10::optional<double> scale, bool want_lse, const c10::optional<at::Tensor>& out_given,
     const c10::optional<at::Tensor>& status);
-void pages_allocate(at::Tensor& refcount, at::Tensor& lens, at::Tensor& table, int64_t page_size, const at::Tensor& seqs,
+void pages_allocate(at::Tensor& state, int64_t pages, int64_t seqs_held, int64_t page_size, const at::Tensor& seqs,
                     const at::Tensor& new_lens, const c10::optional<at::Tensor>& status);
-void pages_fork(at::Tensor& refcount, at::Tensor& lens, at::Tensor& table, int64_t page_size, const at::Tensor& parents,
+void pages_fork(at::Tensor& state, int64_t pages, int64_t seqs_held, int64_t page_size, const at::Tensor& parents,
                 const at::Tensor& children, const at::Tensor& at_lens, at::Tensor& storage,
                 const c10::optional<at::Tensor>& status);
-void pages_release(at::Tensor& refcount, at::Tensor& lens, at::Tensor& table, int64_t page_size, const at::Tensor& seqs,
+void pages_release(at::Tensor& state, int64_t pages, int64_t seqs_held, int64_t page_size, const at::Tensor& seqs,
                    const c10::optional<at::Tensor>& status);
-at::Tensor pages_compact(at::Tensor& refcount, at::Tensor& lens, at::Tensor& table, int64_t page_size, at::Tensor& storage,
+at::Tensor pages_compact(at::Tensor& state, int64_t pages, int64_t seqs_held, int64_t page_size, at::Tensor& storage,
                          const c10::optional<at::Tensor>& status);
 void pages_copy(at::Tensor& storage, const at::Tensor& source, const at::Tensor& target,
                 const c10::optional<at::Tensor>& rows, const c10::optional<at::Tensor>& status);
@@ -170,15 +170,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("k_pages"), py::arg("v_pages"), py::arg("table"), py::arg("kv_lens"), py::arg("cu_q"),
         py::arg("max_q_len"), py::arg("causal"), py::arg("window"), py::arg("sinks"), py::arg("scale"),
         py::arg("want_lse"), py::arg("out"), py::arg("status"));
-  m.def("pages_allocate", &rc::pages_allocate, "grow sequences of a page table", py::arg("refcount"), py::arg("lens"),
-        py::arg("table"), py::arg("page_size"), py::arg("seqs"), py::arg("new_lens"), py::arg("status") = py::none());
-  m.def("pages_fork", &rc::pages_fork, "share pages with forked sequences, copy partial tails", py::arg("refcount"),
-        py::arg("lens"), py::arg("table"), py::arg("page_size"), py::arg("parents"), py::arg("children"),
+  m.def("pages_allocate", &rc::pages_allocate, "grow sequences of a page table", py::arg("state"), py::arg("pages"), py::arg("seqs_held"), py::arg("page_size"), py::arg("seqs"), py::arg("new_lens"), py::arg("status") = py::none());
+  m.def("pages_fork", &rc::pages_fork, "share pages with forked sequences, copy partial tails", py::arg("state"),
+        py::arg("pages"), py::arg("seqs_held"), py::arg("page_size"), py::arg("parents"), py::arg("children"),
         py::arg("at_lens"), py::arg("storage"), py::arg("status") = py::none());
-  m.def("pages_release", &rc::pages_release, "give the pages of sequences back", py::arg("refcount"), py::arg("lens"),
-        py::arg("table"), py::arg("page_size"), py::arg("seqs"), py::arg("status") = py::none());
+  m.def("pages_release", &rc::pages_release, "give the pages of sequences back", py::arg("state"), py::arg("pages"), py::arg("seqs_held"), py::arg("page_size"), py::arg("seqs"), py::arg("status") = py::none());
   m.def("pages_compact", &rc::pages_compact, "move the pages in use to the front; returns their number (on the device)",
-        py::arg("refcount"), py::arg("lens"), py::arg("table"), py::arg("page_size"), py::arg("storage"),
+        py::arg("state"), py::arg("pages"), py::arg("seqs_held"), py::arg("page_size"), py::arg("storage"),
         py::arg("status") = py::none());
   m.def("pages_copy", &rc::pages_copy, "copy pages (or their first rows) in every plane", py::arg("storage"),
         py::arg("source"), py::arg("target"), py::arg("rows") = py::none(), py::arg("status") = py::none());

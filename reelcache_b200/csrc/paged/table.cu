@@ -380,21 +380,19 @@ __global__ void __launch_bounds__(kMoveThreads) release_kernel(State s, const in
   }
 }
 
-State check_state(at::Tensor& refcount, at::Tensor& lens, at::Tensor& table, int64_t page_size) {
-  const at::Tensor* all[3] = {&refcount, &lens, &table};
-  for (const at::Tensor* t : all)
-    RC_CHECK(t->is_cuda() && t->device() == refcount.device() && t->scalar_type() == at::kInt && t->is_contiguous(),
-             "refcount, lens and block_table must be contiguous int32 tensors on one CUDA device");
-  RC_CHECK(refcount.dim() == 1 && lens.dim() == 1 && table.dim() == 2 && table.size(0) == lens.size(0),
-           "refcount is [pages], lens [seqs], block_table [seqs, width]");
+// state: refcount[pages] | lens[seqs] | table[seqs, width]
+State check_state(at::Tensor& state, int64_t pages, int64_t seqs, int64_t page_size) {
+  RC_CHECK(state.is_cuda() && state.scalar_type() == at::kInt && state.dim() == 1 && state.is_contiguous(),
+           "a page table's state must be a contiguous int32 CUDA vector");
   // (below 2^20 pages the 1,024 needs that one prefix sum adds up stay below 2^31)
-  RC_CHECK(refcount.numel() >= 1 && refcount.numel() < (1 << 20) && lens.numel() >= 1 && lens.numel() < (1 << 20) &&
-               table.size(1) >= 1 && table.size(1) < (1 << 28),
-           "the page table is empty or too large");
+  RC_CHECK(pages >= 1 && pages < (1 << 20) && seqs >= 1 && seqs < (1 << 20), "the page table is empty or too large");
+  const int64_t cells = state.numel() - pages - seqs, width = cells / seqs;
+  RC_CHECK(cells > 0 && cells % seqs == 0 && width < (1 << 28), "a page table's state is pages + seqs + seqs * width entries");
   RC_CHECK(page_size >= 8 && page_size % 8 == 0 && page_size <= 65536,
            "the page size must be a multiple of 8 tokens, at most 65536");
-  return {refcount.data_ptr<int>(), lens.data_ptr<int>(), table.data_ptr<int>(), static_cast<int>(refcount.size(0)),
-          static_cast<int>(lens.size(0)), static_cast<int>(table.size(1)), static_cast<int>(page_size)};
+  int* p = state.data_ptr<int>();
+  return {p, p + pages, p + pages + seqs, static_cast<int>(pages), static_cast<int>(seqs), static_cast<int>(width),
+          static_cast<int>(page_size)};
 }
 
 const int* check_list(const at::Tensor& t, const at::Device& device, int64_t n, const char* name) {
@@ -433,71 +431,71 @@ int move_grid(int device) { return sm_count(device) * 8; }
 
 using pagetable::State;
 
-void pages_allocate(at::Tensor& refcount, at::Tensor& lens, at::Tensor& table, int64_t page_size, const at::Tensor& seqs,
+void pages_allocate(at::Tensor& state, int64_t pages, int64_t seqs_held, int64_t page_size, const at::Tensor& seqs,
                     const at::Tensor& new_lens, const c10::optional<at::Tensor>& status) {
-  const State s = pagetable::check_state(refcount, lens, table, page_size);
+  const State s = pagetable::check_state(state, pages, seqs_held, page_size);
   const int64_t n = seqs.numel();
-  const int* ids = pagetable::check_list(seqs, refcount.device(), n, "seqs");
-  const int* to = pagetable::check_list(new_lens, refcount.device(), n, "lens");
+  const int* ids = pagetable::check_list(seqs, state.device(), n, "seqs");
+  const int* to = pagetable::check_list(new_lens, state.device(), n, "lens");
   if (n == 0) return;
-  c10::cuda::CUDAGuard guard(refcount.device());
-  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(refcount.get_device()).stream();
-  at::Tensor scratch = at::empty({s.pages + n + 1 + s.seqs}, refcount.options());
+  c10::cuda::CUDAGuard guard(state.device());
+  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(state.get_device()).stream();
+  at::Tensor scratch = at::empty({s.pages + n + 1 + s.seqs}, state.options());
   int* list = scratch.data_ptr<int>();
   paged::launch(pagetable::allocate_kernel, dim3(1), pagetable::kPlanThreads, 0, 0, stream, s, ids, to, static_cast<int>(n), list,
                                                                        list + s.pages, list + s.pages + n + 1,
                                                                        status_ptr(status));
 }
 
-void pages_fork(at::Tensor& refcount, at::Tensor& lens, at::Tensor& table, int64_t page_size, const at::Tensor& parents,
+void pages_fork(at::Tensor& state, int64_t pages, int64_t seqs_held, int64_t page_size, const at::Tensor& parents,
                 const at::Tensor& children, const at::Tensor& at_lens, at::Tensor& storage,
                 const c10::optional<at::Tensor>& status) {
-  const State s = pagetable::check_state(refcount, lens, table, page_size);
+  const State s = pagetable::check_state(state, pages, seqs_held, page_size);
   const int64_t n = parents.numel();
-  const int* from = pagetable::check_list(parents, refcount.device(), n, "parents");
-  const int* to = pagetable::check_list(children, refcount.device(), n, "children");
-  const int* len = pagetable::check_list(at_lens, refcount.device(), n, "lens");
-  const pagetable::Storage st = pagetable::check_storage(storage, s.pages, page_size, refcount.device());
+  const int* from = pagetable::check_list(parents, state.device(), n, "parents");
+  const int* to = pagetable::check_list(children, state.device(), n, "children");
+  const int* len = pagetable::check_list(at_lens, state.device(), n, "lens");
+  const pagetable::Storage st = pagetable::check_storage(storage, s.pages, page_size, state.device());
   if (n == 0) return;
-  c10::cuda::CUDAGuard guard(refcount.device());
-  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(refcount.get_device()).stream();
-  at::Tensor scratch = at::empty({1 + 3 * n + s.pages + s.seqs}, refcount.options());
+  c10::cuda::CUDAGuard guard(state.device());
+  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(state.get_device()).stream();
+  at::Tensor scratch = at::empty({1 + 3 * n + s.pages + s.seqs}, state.options());
   int* p = scratch.data_ptr<int>();
   const pagetable::Plan plan{p, p + 1, p + 1 + n, p + 1 + 2 * n};
   int* list = p + 1 + 3 * n;
   paged::launch(pagetable::fork_plan_kernel, dim3(1), pagetable::kPlanThreads, 0, 0, stream, s, from, to, len, static_cast<int>(n), list,
                                                                         list + s.pages, plan, status_ptr(status));
-  paged::launch(pagetable::fork_kernel, dim3(pagetable::move_grid(refcount.get_device())), pagetable::kMoveThreads, 0, 0, stream,
+  paged::launch(pagetable::fork_kernel, dim3(pagetable::move_grid(state.get_device())), pagetable::kMoveThreads, 0, 0, stream,
       s, st, from, to, len, static_cast<int>(n), plan, status_ptr(status));
 }
 
-void pages_release(at::Tensor& refcount, at::Tensor& lens, at::Tensor& table, int64_t page_size, const at::Tensor& seqs,
+void pages_release(at::Tensor& state, int64_t pages, int64_t seqs_held, int64_t page_size, const at::Tensor& seqs,
                    const c10::optional<at::Tensor>& status) {
-  const State s = pagetable::check_state(refcount, lens, table, page_size);
+  const State s = pagetable::check_state(state, pages, seqs_held, page_size);
   const int64_t n = seqs.numel();
-  const int* ids = pagetable::check_list(seqs, refcount.device(), n, "seqs");
+  const int* ids = pagetable::check_list(seqs, state.device(), n, "seqs");
   if (n == 0) return;
-  c10::cuda::CUDAGuard guard(refcount.device());
-  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(refcount.get_device()).stream();
+  c10::cuda::CUDAGuard guard(state.device());
+  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(state.get_device()).stream();
   const int64_t blocks = (n * s.width + pagetable::kMoveThreads - 1) / pagetable::kMoveThreads;
-  const int grid = static_cast<int>(std::min<int64_t>(blocks, pagetable::move_grid(refcount.get_device())));
+  const int grid = static_cast<int>(std::min<int64_t>(blocks, pagetable::move_grid(state.get_device())));
   paged::launch(pagetable::release_kernel, dim3(grid), pagetable::kMoveThreads, 0, 0, stream, s, ids, static_cast<int>(n), status_ptr(status));
 }
 
 // Returns an int32 tensor of one entry: the pages in use, which after the call are pages 0 .. in_use.
-at::Tensor pages_compact(at::Tensor& refcount, at::Tensor& lens, at::Tensor& table, int64_t page_size, at::Tensor& storage,
+at::Tensor pages_compact(at::Tensor& state, int64_t pages, int64_t seqs_held, int64_t page_size, at::Tensor& storage,
                          const c10::optional<at::Tensor>& status) {
-  const State s = pagetable::check_state(refcount, lens, table, page_size);
-  const pagetable::Storage st = pagetable::check_storage(storage, s.pages, page_size, refcount.device());
-  c10::cuda::CUDAGuard guard(refcount.device());
-  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(refcount.get_device()).stream();
-  at::Tensor scratch = at::empty({1 + 3 * s.pages}, refcount.options());
-  at::Tensor in_use = at::empty({1}, refcount.options());
+  const State s = pagetable::check_state(state, pages, seqs_held, page_size);
+  const pagetable::Storage st = pagetable::check_storage(storage, s.pages, page_size, state.device());
+  c10::cuda::CUDAGuard guard(state.device());
+  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(state.get_device()).stream();
+  at::Tensor scratch = at::empty({1 + 3 * s.pages}, state.options());
+  at::Tensor in_use = at::empty({1}, state.options());
   int* p = scratch.data_ptr<int>();
   const pagetable::Plan plan{p, p + 1, p + 1 + s.pages, nullptr};
   int* place = p + 1 + 2 * static_cast<int64_t>(s.pages);
   paged::launch(pagetable::compact_plan_kernel, dim3(1), pagetable::kPlanThreads, 0, 0, stream, s, place, plan, in_use.data_ptr<int>());
-  paged::launch(pagetable::compact_kernel, dim3(pagetable::move_grid(refcount.get_device())), pagetable::kMoveThreads, 0, 0, stream,
+  paged::launch(pagetable::compact_kernel, dim3(pagetable::move_grid(state.get_device())), pagetable::kMoveThreads, 0, 0, stream,
       s, st, place, in_use.data_ptr<int>(), plan, status_ptr(status));
   return in_use;
 }

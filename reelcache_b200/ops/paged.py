@@ -62,19 +62,32 @@ def copy_pages(storage, source, target, rows=None):
 
 class PageTable:
     """The page table of ``seqs`` sequence slots over ``pages`` pages, one int32 tensor ``state`` on the device:
-    ``refcount [pages]``, ``lens [seqs]`` and ``block_table [seqs, width]`` are its parts.
+    ``refcount [pages]``, ``lens [seqs]`` and ``block_table [seqs, width]`` are its parts (views).
 
     All operators run on the device in stream order and take int32 vectors on it. Free pages are taken lowest first, in
     the order of the call's sequences. A call that cannot be served changes nothing (see the module)."""
 
     def __init__(self, state: torch.Tensor, *, pages: int, seqs: int, page_size: int):
-        width, rest = divmod(state.numel() - pages - seqs, max(seqs, 1))
-        if state.dim() != 1 or state.dtype != torch.int32 or pages < 1 or seqs < 1 or width < 1 or rest:
+        cells = state.numel() - pages - seqs
+        if state.dim() != 1 or state.dtype is not torch.int32 or pages < 1 or seqs < 1 or cells < 1 or cells % seqs:
             raise ConfigurationError(f"a page table of {pages} pages and {seqs} sequences is an int32 vector of pages + "
                                      f"seqs + seqs * width entries, got {state.dtype} {tuple(state.shape)}")
-        self.state, self.page_size = state, page_size
-        self.refcount, self.lens, blocks = state.split((pages, seqs, seqs * width))
-        self.block_table = blocks.view(seqs, width)
+        self.state, self.pages, self.seqs, self.page_size = state, pages, seqs, page_size
+
+    @property
+    def refcount(self) -> torch.Tensor:
+        """``[pages]``: sequences that hold each page (0: it is free)."""
+        return self.state[:self.pages]
+
+    @property
+    def lens(self) -> torch.Tensor:
+        """``[seqs]``: tokens that each sequence holds."""
+        return self.state[self.pages:self.pages + self.seqs]
+
+    @property
+    def block_table(self) -> torch.Tensor:
+        """``[seqs, width]``: page of each block of each sequence, -1 for none."""
+        return self.state[self.pages + self.seqs:].view(self.seqs, -1)
 
     @classmethod
     def empty(cls, pages: int, seqs: int, width: int, page_size: int, device) -> "PageTable":
@@ -84,7 +97,7 @@ class PageTable:
         return cls(state, pages=pages, seqs=seqs, page_size=page_size)
 
     def _parts(self):
-        return self.refcount, self.lens, self.block_table, self.page_size
+        return self.state, self.pages, self.seqs, self.page_size
 
     def allocate(self, seqs, lens):
         """Sequences ``seqs[i]`` grow to ``lens[i]`` tokens (at least what they hold)."""
