@@ -43,7 +43,6 @@ constexpr int kItemRows = 256;  // rows of an item: two tiles
 constexpr int kChunkThreads = 384;
 constexpr int kPlanThreads = 1024;
 constexpr int kKStages = 3;
-constexpr int kVStages = 2;
 // Register split (setmaxnreg): the launch holds kLaunchRegs a thread (checked on the host); the third warpgroup gives up
 // registers for the softmax warpgroups, which hold a row of 128 scores.
 constexpr int kLaunchRegs = 168;
@@ -53,15 +52,18 @@ static_assert(2 * kSoftmaxRegs + kRoleRegs == 3 * kLaunchRegs, "register split m
 constexpr float kRescale = 8.0f;  // log2 units
 constexpr int kPolyEvery = 8;     // one of so many pairs of exponentials is taken from the FMA pipe
 
-template <int D>
+template <int D, bool kTwin>
 struct ChunkShape {
+  static constexpr int q_tiles = kTwin ? 1 : 2;
+  static constexpr int v_stages = kTwin ? 3 : 2;
+  static constexpr int rows = q_tiles * kTile;  // of an item
   static constexpr int boxes = D / 64;
   static constexpr int box_bytes = kTile * 128;
   static constexpr int tile_bytes = boxes * box_bytes;
   static constexpr int q_off = 0;
-  static constexpr int k_off = q_off + 2 * tile_bytes;
+  static constexpr int k_off = q_off + q_tiles * tile_bytes;
   static constexpr int v_off = k_off + kKStages * tile_bytes;
-  static constexpr int bar_off = v_off + kVStages * tile_bytes;
+  static constexpr int bar_off = v_off + v_stages * tile_bytes;
   static constexpr int bytes = bar_off + 256 + 1024;  // + barriers, alignment slack
   static constexpr int ml_off = kItemRows * D * 4;    // at the end, clustered: rows of FP32 from 0, then maxima and sums
   static_assert(ml_off + kItemRows * 8 <= bar_off, "the rows fit where the operands were");
@@ -129,9 +131,9 @@ __device__ __forceinline__ int sequence(const Args& a, int s, int* q_first, int*
 // Queries of a row tile of a sequence: [first, end).
 struct RowQueries {
   int first, end;
-  __device__ __forceinline__ RowQueries(const Args& a, int row_tile, int q_len) {
-    first = row_tile * kItemRows / a.group;
-    end = min(q_len, (row_tile * kItemRows + kItemRows - 1) / a.group + 1);
+  __device__ __forceinline__ RowQueries(const Args& a, int row_tile, int q_len, int item_rows = kItemRows) {
+    first = row_tile * item_rows / a.group;
+    end = min(q_len, (row_tile * item_rows + item_rows - 1) / a.group + 1);
   }
 };
 
@@ -257,15 +259,15 @@ struct Segment {
     return t0 < t1;
   }
 
-  __device__ __forceinline__ bool direct(const Chunk& p, int block) {
+  __device__ __forceinline__ bool direct(const Chunk& p, int block, int item_rows) {
     const int index = block / p.cluster, rank = block - index * p.cluster, each = p.a.kv_heads * p.row_tiles;
     item.seq = index / each;
     item.head = (index - item.seq * each) / p.row_tiles;
     item.row_tile = p.row_tiles - 1 - index % p.row_tiles;  // the rows that see most come first
     item.q_len = sequence(p.a, item.seq, &item.q_first, &item.kv_len);
     item.start = 0;
-    if (static_cast<int64_t>(item.row_tile) * kItemRows >= static_cast<int64_t>(item.q_len) * p.a.group) return false;
-    item.tiles = tiles_of(p.a, item, RowQueries(p.a, item.row_tile, item.q_len));
+    if (static_cast<int64_t>(item.row_tile) * item_rows >= static_cast<int64_t>(item.q_len) * p.a.group) return false;
+    item.tiles = tiles_of(p.a, item, RowQueries(p.a, item.row_tile, item.q_len, item_rows));
     t0 = item.tiles * rank / p.cluster;
     t1 = item.tiles * (rank + 1) / p.cluster;
     starts = t0 == 0;
@@ -411,19 +413,20 @@ __device__ __forceinline__ uint64_t sw128_mnmajor_desc(uint32_t smem_addr, uint3
   return desc;
 }
 
-template <typename T, int D, bool kDirect>
+template <typename T, int D, bool kDirect, bool kTwin>
 __global__ void __launch_bounds__(kChunkThreads, 1)
     chunk_kernel(const __grid_constant__ PageMaps maps, const __grid_constant__ Chunk p) {
-  using Shape = ChunkShape<D>;
+  using Shape = ChunkShape<D, kTwin>;
+  static_assert(kDirect || !kTwin, "twin items are dealt out whole");
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + Shape::bar_off);
   uint64_t* q_empty = q_full + 1;
   uint64_t* k_full = q_empty + 1;         // [kKStages]
   uint64_t* k_empty = k_full + kKStages;  // [kKStages]
-  uint64_t* v_full = k_empty + kKStages;  // [kVStages]
-  uint64_t* v_empty = v_full + kVStages;  // [kVStages]
-  uint64_t* s_full = v_empty + kVStages;  // [2] per tile
+  uint64_t* v_full = k_empty + kKStages;  // [v_stages]
+  uint64_t* v_empty = v_full + Shape::v_stages;
+  uint64_t* s_full = v_empty + Shape::v_stages;  // [2] per tile
   uint64_t* p_full = s_full + 2;          // [4] per tile and half of the keys
   uint64_t* o_done = p_full + 4;          // [2]
   uint64_t* v_raw = o_done + 2;
@@ -443,7 +446,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       mbar_init(&k_full[b], 1);
       mbar_init(&k_empty[b], 1);
     }
-    for (int b = 0; b < kVStages; ++b) {
+    for (int b = 0; b < Shape::v_stages; ++b) {
       mbar_init(&v_full[b], 1);
       mbar_init(&v_empty[b], 1);
     }
@@ -462,7 +465,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     tma_prefetch_desc(&maps.v_wide);
   }
   after_earlier();
-  if (kDirect && !seg.direct(p, cta)) return;  // the whole cluster
+  if (kDirect && !seg.direct(p, cta, Shape::rows)) return;  // the whole cluster
   if (warp == 10) tmem_alloc(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
@@ -476,7 +479,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     if (warp < 10) {
       // ---------------- TMA: warp 8 streams K, warp 9 streams V ----------------
       const bool is_k = warp == 8;
-      const int stages = is_k ? kKStages : kVStages;
+      const int stages = is_k ? kKStages : Shape::v_stages;
       uint64_t* full = is_k ? k_full : v_full;
       uint64_t* empty = is_k ? k_empty : v_empty;
       uint8_t* ring = smem + (is_k ? Shape::k_off : Shape::v_off);
@@ -486,7 +489,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       uint32_t phase = 1, raw_phase = 0;
       bool ok = true;
       for (int n = 0; ok && next(n); ++n) {
-        const RowQueries rows(a, seg.item.row_tile, seg.item.q_len);
+        const RowQueries rows(a, seg.item.row_tile, seg.item.q_len, Shape::rows);
         const Sight sight(a, seg.item.kv_len, seg.item.q_len);
         const TileRange<kTile> range(sight, rows.first, rows.end);
         const int low = sight.low(sight.last(rows.first)), top = min(sight.last(rows.end - 1), seg.item.kv_len - 1);
@@ -535,14 +538,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         }
       }
     } else if (warp == 11) {
-      // ---------------- Q rows: each lane finds where 8 rows lie, then four lanes fetch a row 64 bytes at a time ------
+      // ---------------- Q rows: each lane finds where a few rows lie, then four lanes fetch a row 64 bytes at a time ------
       const int quarter = lane & 3, sub = lane >> 2;
       bool ok = true;
       for (int n = 0; ok && next(n); ++n) {
-        const int packed0 = seg.item.row_tile * kItemRows;
-        const T* place[8];
+        constexpr int kPlaces = Shape::rows / 32;
+        const int packed0 = seg.item.row_tile * Shape::rows;
+        const T* place[kPlaces];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < kPlaces; ++i) {
           const int packed = packed0 + 32 * i + lane, query = packed / a.group;
           const int h = seg.item.head * a.group + packed - query * a.group;
           place[i] = query < seg.item.q_len
@@ -552,7 +556,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         if (n > 0) ok = __all_sync(0xffffffffu, mbar_wait_park(q_empty, (n - 1) & 1, status, kTimeoutGather));
         if (!ok) break;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < kPlaces; ++i) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int r = 32 * i + 8 * j + sub;
@@ -588,9 +592,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         int k_stage = 0, v_stage = 0;
         uint32_t k_phase = 0, v_phase = 0;
         bool was_first = false, was_last = false;  // the block before: whether it begins, ends its segment
+        int last_block[2] = {0, 0};                // twin: each tile's last block
         auto issue_s = [&](int g) {
           if (!ok) return;
-          const uint64_t ka = k_desc + k_stage * (Shape::tile_bytes >> 4), qg = q_desc + g * (Shape::tile_bytes >> 4);
+          const uint64_t ka = k_desc + k_stage * (Shape::tile_bytes >> 4), qg = q_desc + (kTwin ? 0 : g) * (Shape::tile_bytes >> 4);
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             constexpr uint32_t kBox = Shape::box_bytes >> 4;
@@ -611,21 +616,73 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
               mma_f16_ts(tmem_base + 256 + g * kTile, tmem_base + g * kTile + kk * 8, va + kk * (16 * 128 >> 4), idesc_o,
                          kk > 0 || !was_first ? 1u : 0u);
           }
-          if (was_last) mma_commit(&o_done[g]);
+          if (kTwin ? it - 1 == last_block[g] : was_last) mma_commit(&o_done[g]);
         };
         auto done_v = [&]() {
           if (ok) mma_commit(&v_empty[v_stage]);
-          if (++v_stage == kVStages) {
+          if (++v_stage == Shape::v_stages) {
             v_stage = 0;
             v_phase ^= 1;
           }
         };
-        for (int n = 0; ok && next(n); ++n) {
+        auto take_k = [&]() {
+          if (ok) ok = mbar_wait_park(&k_full[k_stage], k_phase, status, kTimeoutMma);
+          tc_fence_after();
+        };
+        auto done_k = [&]() {
+          if (ok) mma_commit(&k_empty[k_stage]);
+          if (++k_stage == kKStages) {
+            k_stage = 0;
+            k_phase ^= 1;
+          }
+        };
+        auto take_v = [&]() {
+          if (ok) ok = mbar_wait_park(&v_full[v_stage], v_phase, status, kTimeoutMma);
+        };
+        if (kTwin && next(0)) {
+          // tile 0 takes the even blocks, tile 1 the odd ones, with the same rows: twice the keys in flight for few rows
+          const int n = seg.t1 - seg.t0;
+          last_block[0] = (n + 1) / 2 - 1;
+          last_block[1] = n / 2 - 1;
+          ok = mbar_wait_park(q_full, 0, status, kTimeoutMma);
+          for (; it <= last_block[0] && ok; ++it) {
+            was_first = it == 1;
+            take_k();
+            if (it > 0) {
+              take_v();
+              issue_pv(0);
+              done_v();
+            }
+            issue_s(0);
+            done_k();
+            if (it > 0) {
+              take_v();
+              issue_pv(1);
+              done_v();
+            }
+            if (it <= last_block[1]) {
+              take_k();
+              issue_s(1);
+              done_k();
+            }
+          }
+          was_first = it == 1;
+          take_v();
+          issue_pv(0);
+          done_v();
+          if (it - 1 <= last_block[1]) {
+            take_v();
+            issue_pv(1);
+            done_v();
+          }
+          it = 0;  // nothing is left to do
+        }
+        for (int n = 0; !kTwin && ok && next(n); ++n) {
           for (int t = seg.t0; t < seg.t1 && ok; ++t) {
             // everything that can be waited for ahead of P is
-            ok = mbar_wait_park(&k_full[k_stage], k_phase, status, kTimeoutMma);
+            take_k();
             if (it > 0) {
-              if (ok) ok = mbar_wait_park(&v_full[v_stage], v_phase, status, kTimeoutMma);
+              take_v();
               issue_pv(0);
             }
             if (ok && t == seg.t0) ok = mbar_wait_park(q_full, n & 1, status, kTimeoutMma);
@@ -636,21 +693,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
               done_v();
             }
             issue_s(1);
-            if (ok) {
-              mma_commit(&k_empty[k_stage]);
-              if (t + 1 == seg.t1) mma_commit(q_empty);
-            }
-            if (++k_stage == kKStages) {
-              k_stage = 0;
-              k_phase ^= 1;
-            }
+            done_k();
+            if (ok && t + 1 == seg.t1) mma_commit(q_empty);
             ++it;
             was_first = t == seg.t0;
             was_last = t + 1 == seg.t1;
           }
         }
         if (it > 0) {
-          if (ok) ok = mbar_wait_park(&v_full[v_stage], v_phase, status, kTimeoutMma);
+          take_v();
           issue_pv(0);
           issue_pv(1);
           done_v();
@@ -671,15 +722,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     bool ok = true;
     int it = 0;
     for (int n = 0; ok && next(n); ++n) {
-      const int packed = seg.item.row_tile * kItemRows + g * kTile + row;
+      const int packed = seg.item.row_tile * Shape::rows + (kTwin ? 0 : g * kTile) + row;
       const int query = packed / a.group;
       const Sight sight(a, seg.item.kv_len, seg.item.q_len);
-      const RowQueries rows(a, seg.item.row_tile, seg.item.q_len);
+      const RowQueries rows(a, seg.item.row_tile, seg.item.q_len, Shape::rows);
       const TileRange<kTile> range(sight, rows.first, rows.end);
       const int last = min(sight.last(min(query, seg.item.q_len - 1)), seg.item.kv_len - 1);
       const int low = sight.low(last);
       float m_run = -INFINITY, l_run = 0.0f;  // of scale * log2(e) * s
-      for (int t = seg.t0; t < seg.t1 && ok; ++t, ++it) {
+      for (int t = seg.t0 + (kTwin ? g : 0); t < seg.t1 && ok; t += kTwin ? 2 : 1, ++it) {
         uint32_t r[2][64], pk[32];
         ok = __all_sync(0xffffffffu, mbar_wait_park(&s_full[g], it & 1, status, kTimeoutEpilogue));
         if (!ok) break;
@@ -696,7 +747,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         }
         // The exponentials start with the maximum so far, and this block's is found next to them (they leave issue slots
         // for it). Only where it has grown by more than kRescale are they done again.
-        if (t == seg.t0) m_run = row_max(r) * a.scale_log2;
+        if (t < seg.t0 + (kTwin ? 2 : 1)) m_run = row_max(r) * a.scale_log2;
         float neg_m = m_run == -INFINITY ? 0.0f : -m_run;  // a row that has seen no key yet
         float sum = 0.0f, mx;
         if (whole) softmax_half<T, kPolyEvery, true>(r[0], r[1], a.scale_log2, neg_m, pk, sum, mx);
@@ -738,9 +789,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[2 * g + 1]);
       }
-      if (ok) ok = __all_sync(0xffffffffu, mbar_wait_park(&o_done[g], n & 1, status, kTimeoutEpilogue));
-      if (kDirect && p.cluster > 1) {
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait_park(&o_done[1 - g], 0, status, kTimeoutEpilogue));
+      const bool none = kTwin && seg.t0 + g >= seg.t1;  // a twin without blocks
+      if (ok && !none) ok = __all_sync(0xffffffffu, mbar_wait_park(&o_done[g], n & 1, status, kTimeoutEpilogue));
+      if (kDirect && (kTwin || p.cluster > 1)) {
+        if (ok && (!kTwin || seg.t0 + 1 - g < seg.t1))
+          ok = __all_sync(0xffffffffu, mbar_wait_park(&o_done[1 - g], 0, status, kTimeoutEpilogue));
         if (ok) {  // every product is done: the operands' memory takes the rows, 16-byte chunks turned against bank conflicts
           tc_fence_after();
           float4* rows_at = reinterpret_cast<float4*>(smem) + (g * kTile + row) * (D / 4);
@@ -791,25 +844,25 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     }
   }
 
-  if (kDirect && p.cluster > 1) {
+  if (kDirect && (kTwin || p.cluster > 1)) {
     // CTAs without tiles have nothing to give; every CTA joins a part of the item's rows over all of them, in order.
     if (seg.t0 == seg.t1 && threadIdx.x < kItemRows)
       reinterpret_cast<float2*>(smem + Shape::ml_off)[threadIdx.x] = make_float2(-INFINITY, 0.0f);
     cluster_sync_all();
     if (threadIdx.x < kItemRows) {
-      const int packed0 = seg.item.row_tile * kItemRows;
-      const int rows = static_cast<int>(min(static_cast<int64_t>(kItemRows), static_cast<int64_t>(seg.item.q_len) * a.group - packed0));
+      const int packed0 = seg.item.row_tile * Shape::rows;
+      const int rows = static_cast<int>(min(static_cast<int64_t>(Shape::rows), static_cast<int64_t>(seg.item.q_len) * a.group - packed0));
       const int rank = cta % p.cluster;
       for (int v = rank * kItemRows + static_cast<int>(threadIdx.x); v < rows * (D / 4); v += p.cluster * kItemRows) {
         const int row = v / (D / 4), chunk = v % (D / 4);
-        const float4* from = reinterpret_cast<const float4*>(smem) + row * (D / 4) + (chunk ^ (row & 15));
-        const float2* from_ml = reinterpret_cast<const float2*>(smem + Shape::ml_off) + row;
         float top = -INFINITY, sum = 0.0f;
         float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int c = 0; c < p.cluster; ++c) {
-          const float2 ml = load_cluster_2(cluster_addr(from_ml, c));
+        for (int c = 0; c < (kTwin ? 2 : 1) * p.cluster; ++c) {
+          const int at = row + (kTwin ? (c & 1) * kTile : 0), cta_of = kTwin ? c >> 1 : c;
+          const float4* from = reinterpret_cast<const float4*>(smem) + at * (D / 4) + (chunk ^ (row & 15));
+          const float2 ml = load_cluster_2(cluster_addr(reinterpret_cast<const float2*>(smem + Shape::ml_off) + at, cta_of));
           if (ml.x == -INFINITY) continue;  // no key seen there (nor, perhaps, anything written)
-          const float4 x = load_cluster_4(cluster_addr(from, c));
+          const float4 x = load_cluster_4(cluster_addr(from, cta_of));
           const float mx = fmaxf(top, ml.x), old = exp2_approx(top - mx), wt = exp2_approx(ml.x - mx);
           top = mx;
           sum = fmaf(sum, old, wt * ml.y);
@@ -901,14 +954,14 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const __grid_constant__
   if (a.lse != nullptr && lane == 0) a.lse[token * a.heads + h] = sum > 0.0f ? (top + log2f(sum)) * kLn2 : -INFINITY;
 }
 
-template <typename T, int D, bool kDirect>
+template <typename T, int D, bool kDirect, bool kTwin>
 void chunk_configure() {
   static bool configured = false;
   if (configured) return;
-  RC_CUDA(cudaFuncSetAttribute(chunk_kernel<T, D, kDirect>, cudaFuncAttributeMaxDynamicSharedMemorySize, ChunkShape<D>::bytes));
-  if (kDirect) RC_CUDA(cudaFuncSetAttribute(chunk_kernel<T, D, kDirect>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  RC_CUDA(cudaFuncSetAttribute(chunk_kernel<T, D, kDirect, kTwin>, cudaFuncAttributeMaxDynamicSharedMemorySize, ChunkShape<D, kTwin>::bytes));
+  if (kDirect) RC_CUDA(cudaFuncSetAttribute(chunk_kernel<T, D, kDirect, kTwin>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   cudaFuncAttributes attr;  // the register split assumes exactly kLaunchRegs a thread
-  RC_CUDA(cudaFuncGetAttributes(&attr, chunk_kernel<T, D, kDirect>));
+  RC_CUDA(cudaFuncGetAttributes(&attr, chunk_kernel<T, D, kDirect, kTwin>));
   RC_CHECK(attr.numRegs == kLaunchRegs, "paged attention compiled to " + std::to_string(attr.numRegs) +
                                             " registers a thread; its register split needs " + std::to_string(kLaunchRegs));
   configured = true;
@@ -925,7 +978,7 @@ int clusters_at_once(int size, int device) {
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(size);
     config.blockDim = dim3(kChunkThreads);
-    config.dynamicSmemBytes = ChunkShape<D>::bytes;
+    config.dynamicSmemBytes = ChunkShape<D, false>::bytes;
     cudaLaunchAttribute attribute{};
     attribute.id = cudaLaunchAttributeClusterDimension;
     attribute.val.clusterDim.x = size;
@@ -934,7 +987,7 @@ int clusters_at_once(int size, int device) {
     config.attrs = &attribute;
     config.numAttrs = 1;
     int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, chunk_kernel<T, D, true>, &config) != cudaSuccess) {
+    if (cudaOccupancyMaxActiveClusters(&n, chunk_kernel<T, D, true, false>, &config) != cudaSuccess) {
       (void)cudaGetLastError();
       n = 0;
     }
@@ -965,7 +1018,7 @@ int direct_cluster(int64_t items, int64_t tiles, bool uneven, int device) {
 template <typename T, int D>
 void chunk_launch(const Args& args, const at::Tensor& k_pages, const at::Tensor& v_pages, int max_q_len,
                   const at::Tensor& like, cudaStream_t stream, int device) {
-  using Shape = ChunkShape<D>;
+  using Shape = ChunkShape<D, false>;
   Chunk p{};
   p.a = args;
   p.a.tiling = Tiling::of(args.tiling.page, kTile);
@@ -980,14 +1033,22 @@ void chunk_launch(const Args& args, const at::Tensor& k_pages, const at::Tensor&
   // tiles of an item, at most: the table's width, or what a window leaves of it
   int64_t keys = static_cast<int64_t>(args.width) * args.tiling.page;
   if (args.window > 0) keys = std::min<int64_t>(keys, static_cast<int64_t>(args.window) + args.sinks + kItemRows / args.group + 2 * kTile);
-  chunk_configure<T, D, true>();
-  p.cluster = direct_cluster<T, D>(most_items, (keys + kTile - 1) / kTile, args.causal && row_tiles > 1, device);
+  chunk_configure<T, D, true, false>();
+  const int64_t tiles = (keys + kTile - 1) / kTile;
+  const bool twin = static_cast<int64_t>(max_q_len) * args.group <= kTile;
+  p.cluster = direct_cluster<T, D>(most_items, twin ? (tiles + 1) / 2 : tiles, args.causal && row_tiles > 1, device);
+  if (p.cluster > 0 && twin) {
+    chunk_configure<T, D, true, true>();
+    launch(chunk_kernel<T, D, true, true>, dim3(static_cast<unsigned>(grid_items * p.cluster)), kChunkThreads,
+           ChunkShape<D, true>::bytes, p.cluster, stream, maps, p);
+    return;
+  }
   if (p.cluster > 0) {
-    launch(chunk_kernel<T, D, true>, dim3(static_cast<unsigned>(grid_items * p.cluster)), kChunkThreads, Shape::bytes, p.cluster,
+    launch(chunk_kernel<T, D, true, false>, dim3(static_cast<unsigned>(grid_items * p.cluster)), kChunkThreads, Shape::bytes, p.cluster,
            stream, maps, p);
     return;
   }
-  chunk_configure<T, D, false>();
+  chunk_configure<T, D, false, false>();
   RC_CHECK(p.ctas < kPlanThreads, "more SMs than the plan's threads");
   const int64_t o_floats = 2ll * p.ctas * kItemRows * D, ml_floats = 2ll * p.ctas * kItemRows * 2;
   const int64_t ints = most_items * 8 + 4 + 2ll * (p.ctas + 1) + args.seqs;
@@ -1000,7 +1061,7 @@ void chunk_launch(const Args& args, const at::Tensor& k_pages, const at::Tensor&
   p.plan.first = p.plan.cut + p.ctas + 1;
   p.plan.base = p.plan.first + p.ctas + 1;
   launch(chunk_plan_kernel, dim3(1), kPlanThreads, 0, 0, stream, p);
-  launch(chunk_kernel<T, D, false>, dim3(p.ctas), kChunkThreads, Shape::bytes, 0, stream, maps, p);
+  launch(chunk_kernel<T, D, false, false>, dim3(p.ctas), kChunkThreads, Shape::bytes, 0, stream, maps, p);
   launch(chunk_join_kernel<T, D>, dim3(kItemRows / 8, p.ctas - 1), 256, 0, 0, stream, p);
 }
 
