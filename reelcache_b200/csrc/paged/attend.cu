@@ -16,7 +16,7 @@
 namespace rc {
 namespace paged {
 
-constexpr int kShortRows = 32;
+constexpr int kShortRows = 16;
 
 void attend_short(const Args& a, int head_dim, bool half, const at::Tensor& k_pages, const at::Tensor& v_pages,
                   int max_q_len, const at::Tensor& like, cudaStream_t stream, int device);

@@ -5,12 +5,11 @@
 // mma.sync from registers and the design is about keeping bytes in flight: one producer warp streams K and V tiles with
 // TMA (one box per page and 64 channels, 128-byte swizzle) through a ring of stages, two CTAs per SM.
 //
-// Rows: the heads of a group share K and V, so a row is (query, head of the group), query-major; 16 * kM rows a CTA.
-// The four consumer warps split rows by 16 and, where there are fewer than four such groups, split each tile's keys:
-// every warp runs its own online softmax (maximum, sum and output in FP32 registers) and meets the others only when a
-// sequence and head is finished.
+// Rows: the heads of a group share K and V, so a row is (query, head of the group), query-major, 16 rows at most. The four
+// consumer warps take 16 keys of each tile: every warp runs its own online softmax (maximum, sum and output in FP32
+// registers) and meets the others only when a sequence and head is finished.
 //
-// Work: all tiles of all (sequence, KV head, row tile) in one line, cut into equal shares, one per CTA, so ragged
+// Work: all tiles of all (sequence, KV head) in one line, cut into equal shares, one per CTA, so ragged
 // batches and a single long sequence fill all SMs alike, and the host needs no lengths. A CTA whose share holds only a
 // part of an item leaves (output, maximum, sum) in FP32 in the workspace; a second kernel joins the parts in order of
 // the CTAs (no atomics: results do not depend on timing). It is launched as a programmatic dependent, so its launch
@@ -28,6 +27,8 @@ namespace rc {
 namespace paged {
 
 constexpr int kShortTile = 64;       // keys of a tile
+constexpr int kRows = 16;            // rows: new tokens x heads of a group, at most
+constexpr int kGroups = 4;           // consumer warps, each with 16 keys of a tile
 constexpr int kShortThreads = 160;   // four consumer warps, one producer warp
 constexpr int kShortCtasPerSm = 2;
 constexpr int kFewTiles = 8;         // tiles of a CTA that are done before an even share would have paid
@@ -57,9 +58,8 @@ struct Line {
 struct Short {
   Args a;
   Line line;
-  float* part_o;   // [2 * CTAs, 16 kM, D]
-  float* part_ml;  // [2 * CTAs, 16 kM, 2]
-  int rows;        // 16 kM
+  float* part_o;   // [2 * CTAs, 16, D]
+  float* part_ml;  // [2 * CTAs, 16, 2]
   int cluster;     // CTAs of a cluster (the clustered form)
 };
 
@@ -104,14 +104,12 @@ struct SeqWork {
   }
 };
 
-template <typename T, int D, int kM, bool kCluster>
+template <typename T, int D, bool kCluster>
 __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
     short_kernel(const __grid_constant__ PageMaps maps, const __grid_constant__ Short p) {
   using Shape = ShortShape<D>;
-  constexpr int kGroups = 4 / kM;               // warps that split a tile's keys
-  constexpr int kKeys = kShortTile / kGroups;   // keys of a warp
-  constexpr int kN = kKeys / 8;                 // its n-tiles of S
-  constexpr int kRows = 16 * kM;
+  constexpr int kKeys = kShortTile / kGroups;  // keys of a warp
+  constexpr int kN = kKeys / 8;                // its n-tiles of S
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + Shape::bar_off);
@@ -261,7 +259,7 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
   }
 
   // ---------------- consumers ----------------
-  const int mt = warp % kM, kg = warp / kM;  // row group, key group
+  const int kg = warp;  // its keys
   const int r0 = lane >> 2, c0 = (lane & 3) * 2;
   bool ok = true;
   for (int at = begin; kCluster || at < end;) {  // a cluster's CTA goes round once, also without tiles
@@ -284,7 +282,7 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
     uint32_t q[D / 16][4];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int row = mt * 16 + r0 + i * 8;
+      const int row = r0 + i * 8;
       row_q[i] = row / a.group;
       row_h[i] = head * a.group + row - row_q[i] * a.group;
       valid[i] = row_q[i] < w.q_len;
@@ -423,88 +421,78 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
     }
     // Warps that split the keys join theirs into key group 0, one after the other through shared memory. The same lane
     // of every warp holds the same rows and columns, so the buffer is laid out by lane.
-    if (kGroups > 1) {
-      if ((lane & 3) == 0) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          join_ml[(kg * kRows + mt * 16 + r0 + 8 * i) * 2] = m[i];
-          join_ml[(kg * kRows + mt * 16 + r0 + 8 * i) * 2 + 1] = l[i];
-        }
-      }
-      consumers_sync();
-      float w_o[2];
+    if ((lane & 3) == 0) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        float top = -INFINITY, total = 0.0f;
-        float gm[kGroups];
-#pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-          gm[g] = join_ml[(g * kRows + mt * 16 + r0 + 8 * i) * 2];
-          top = fmaxf(top, gm[g]);
-        }
-        const float use = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-        for (int g = 0; g < kGroups; ++g)
-          total = fmaf(join_ml[(g * kRows + mt * 16 + r0 + 8 * i) * 2 + 1], exp2_approx(gm[g] - use), total);
-        w_o[i] = exp2_approx(m[i] - use);
-        m[i] = top;
-        l[i] = total;
+        join_ml[(kg * kRows + r0 + 8 * i) * 2] = m[i];
+        join_ml[(kg * kRows + r0 + 8 * i) * 2 + 1] = l[i];
       }
+    }
+    consumers_sync();
+    float w_o[2];
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        o[i][0] *= w_o[0];
-        o[i][1] *= w_o[0];
-        o[i][2] *= w_o[1];
-        o[i][3] *= w_o[1];
+    for (int i = 0; i < 2; ++i) {
+      float top = -INFINITY, total = 0.0f;
+      float gm[kGroups];
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        gm[g] = join_ml[(g * kRows + r0 + 8 * i) * 2];
+        top = fmaxf(top, gm[g]);
       }
-      if (kM == 1 && rows_here <= 8) {
-        // only the first 8 rows hold anything: all warps at once
-        float2* buf = reinterpret_cast<float2*>(smem + Shape::join_off) + lane;
-        if (kg > 0) {
+      const float use = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-          for (int i = 0; i < D / 8; ++i) buf[((kg - 1) * (D / 8) + i) * 32] = make_float2(o[i][0], o[i][1]);
+      for (int g = 0; g < kGroups; ++g)
+        total = fmaf(join_ml[(g * kRows + r0 + 8 * i) * 2 + 1], exp2_approx(gm[g] - use), total);
+      w_o[i] = exp2_approx(m[i] - use);
+      m[i] = top;
+      l[i] = total;
+    }
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) {
+      o[i][0] *= w_o[0];
+      o[i][1] *= w_o[0];
+      o[i][2] *= w_o[1];
+      o[i][3] *= w_o[1];
+    }
+    if (rows_here <= 8) {
+      // only the first 8 rows hold anything: all warps at once
+      float2* buf = reinterpret_cast<float2*>(smem + Shape::join_off) + lane;
+      if (kg > 0) {
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) buf[((kg - 1) * (D / 8) + i) * 32] = make_float2(o[i][0], o[i][1]);
+      }
+      consumers_sync();
+      if (kg == 0) {
+#pragma unroll
+        for (int g = 0; g < kGroups - 1; ++g)
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            const float2 x = buf[(g * (D / 8) + i) * 32];
+            o[i][0] += x.x;
+            o[i][1] += x.y;
+          }
+      }
+      consumers_sync();
+    } else {
+      float4* buf = reinterpret_cast<float4*>(smem + Shape::join_off) + lane;
+#pragma unroll
+      for (int g = 1; g < kGroups; ++g) {
+        if (kg == g) {
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) buf[i * 32] = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
         }
         consumers_sync();
         if (kg == 0) {
 #pragma unroll
-          for (int g = 0; g < kGroups - 1; ++g)
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-              const float2 x = buf[(g * (D / 8) + i) * 32];
-              o[i][0] += x.x;
-              o[i][1] += x.y;
-            }
-        }
-        consumers_sync();
-      } else {
-        constexpr int kBlock = D / 8 / kM;  // n-tiles that fit at a time
-        float4* buf = reinterpret_cast<float4*>(smem + Shape::join_off) + mt * kBlock * 32 + lane;
-#pragma unroll
-        for (int g = 1; g < kGroups; ++g) {
-#pragma unroll
-          for (int c = 0; c < kM; ++c) {
-            if (kg == g) {
-#pragma unroll
-              for (int i = 0; i < kBlock; ++i) {
-                const float(&x)[4] = o[c * kBlock + i];
-                buf[i * 32] = make_float4(x[0], x[1], x[2], x[3]);
-              }
-            }
-            consumers_sync();
-            if (kg == 0) {
-#pragma unroll
-              for (int i = 0; i < kBlock; ++i) {
-                const float4 x = buf[i * 32];
-                float(&y)[4] = o[c * kBlock + i];
-                y[0] += x.x;
-                y[1] += x.y;
-                y[2] += x.z;
-                y[3] += x.w;
-              }
-            }
-            consumers_sync();
+          for (int i = 0; i < D / 8; ++i) {
+            const float4 x = buf[i * 32];
+            o[i][0] += x.x;
+            o[i][1] += x.y;
+            o[i][2] += x.z;
+            o[i][3] += x.w;
           }
         }
+        consumers_sync();
       }
     }
     if (kCluster) {
@@ -516,7 +504,7 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
       if (kg == 0) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int row = mt * 16 + r0 + 8 * i;
+          const int row = r0 + 8 * i;
 #pragma unroll
           for (int d = 0; d < D / 8; ++d) *reinterpret_cast<float2*>(res + row * D + d * 8 + c0) = make_float2(o[d][2 * i], o[d][2 * i + 1]);
           if ((lane & 3) == 0) *reinterpret_cast<float2*>(res_ml + row * 2) = make_float2(m[i], l[i]);
@@ -587,7 +575,7 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
           if (a.lse != nullptr && (lane & 3) == 0)
             a.lse[token * a.heads + row_h[i]] = l[i] > 0.0f ? (m[i] + log2f(l[i])) * kLn2 : -INFINITY;
         } else {
-          const int64_t slot = (2 * static_cast<int64_t>(blockIdx.x) + (starts ? 1 : 0)) * kRows + mt * 16 + r0 + 8 * i;
+          const int64_t slot = (2 * static_cast<int64_t>(blockIdx.x) + (starts ? 1 : 0)) * kRows + r0 + 8 * i;
           float* dst = p.part_o + slot * D + c0;
 #pragma unroll
           for (int d = 0; d < D / 8; ++d) *reinterpret_cast<float2*>(dst + d * 8) = make_float2(o[d][2 * i], o[d][2 * i + 1]);
@@ -606,7 +594,7 @@ __global__ void __launch_bounds__(128) short_join_kernel(const __grid_constant__
   constexpr int kPer = D / 32;
   const Args& a = p.a;
   const int lane = threadIdx.x & 31;
-  const int quads = p.rows / 4;
+  const int quads = kRows / 4;
   const int row = (blockIdx.x % quads) * 4 + (threadIdx.x >> 5);
   const int item = blockIdx.x / quads, s = item / a.kv_heads, head = item - s * a.kv_heads;
   let_later();
@@ -624,8 +612,8 @@ __global__ void __launch_bounds__(128) short_join_kernel(const __grid_constant__
   for (int e = 0; e < kPer; ++e) acc[e] = 0.0f;
   for (int cb = c0; cb <= c1; cb += 32) {
     const int n = min(32, c1 - cb + 1);
-    const int64_t first_slot = (2 * static_cast<int64_t>(cb) + (cb == c0)) * p.rows + row;
-    const int64_t slot = (2 * static_cast<int64_t>(cb + lane) + (cb + lane == c0)) * p.rows + row;
+    const int64_t first_slot = (2 * static_cast<int64_t>(cb) + (cb == c0)) * kRows + row;
+    const int64_t slot = (2 * static_cast<int64_t>(cb + lane) + (cb + lane == c0)) * kRows + row;
     float2 ml = make_float2(-INFINITY, 0.0f);
     if (lane < n) ml = *reinterpret_cast<const float2*>(p.part_ml + slot * 2);
     float mx = ml.x;
@@ -644,7 +632,7 @@ __global__ void __launch_bounds__(128) short_join_kernel(const __grid_constant__
 #pragma unroll 8
     for (int i = 0; i < n; ++i) {
       const float weight = __shfl_sync(0xffffffffu, wt, i);
-      const int64_t at = i == 0 ? first_slot : 2 * static_cast<int64_t>(cb + i) * p.rows + row;
+      const int64_t at = i == 0 ? first_slot : 2 * static_cast<int64_t>(cb + i) * kRows + row;
 #pragma unroll
       for (int e = 0; e < kPer; e += 2) {
         const float2 x = *reinterpret_cast<const float2*>(p.part_o + at * D + lane * kPer + e);
@@ -662,22 +650,20 @@ __global__ void __launch_bounds__(128) short_join_kernel(const __grid_constant__
   if (a.lse != nullptr && lane == 0) a.lse[token * a.heads + h] = sum > 0.0f ? (top + log2f(sum)) * kLn2 : -INFINITY;
 }
 
-template <typename T, int D, int kM>
+template <typename T, int D>
 void short_launch(Args a, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& like, cudaStream_t stream,
                   int device) {
   using Shape = ShortShape<D>;
   static bool configured = false;
   if (!configured) {
-    RC_CUDA(cudaFuncSetAttribute(short_kernel<T, D, kM, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::bytes));
-    RC_CUDA(cudaFuncSetAttribute(short_kernel<T, D, kM, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::bytes));
-    RC_CUDA(cudaFuncSetAttribute(short_kernel<T, D, kM, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    RC_CUDA(cudaFuncSetAttribute(short_kernel<T, D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::bytes));
+    RC_CUDA(cudaFuncSetAttribute(short_kernel<T, D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::bytes));
+    RC_CUDA(cudaFuncSetAttribute(short_kernel<T, D, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     configured = true;
   }
-  constexpr int kRows = 16 * kM;
   static_assert(kRows * (D + 2) * 4 <= Shape::stages * 2 * Shape::tile_bytes, "a CTA's rows fit its stages");
   Short p{};
   p.a = a;
-  p.rows = kRows;
   p.a.tiling = Tiling::of(a.tiling.page, kShortTile);
   const PageMaps maps = page_maps(k_pages, v_pages, p.a.tiling, kShortTile);
   const int64_t items = static_cast<int64_t>(a.seqs) * a.kv_heads, slots = sm_count(device) * kShortCtasPerSm;
@@ -689,7 +675,7 @@ void short_launch(Args a, const at::Tensor& k_pages, const at::Tensor& v_pages, 
   for (int c = 16; c > 1 && p.cluster == 0; c /= 2)
     if (items * c <= slots && most_tiles <= c * (c >= 8 ? kLongTiles : kFewTiles)) p.cluster = c;
   if (p.cluster > 0) {
-    launch(short_kernel<T, D, kM, true>, dim3(static_cast<unsigned>(items * p.cluster)), kShortThreads, Shape::bytes, p.cluster,
+    launch(short_kernel<T, D, true>, dim3(static_cast<unsigned>(items * p.cluster)), kShortThreads, Shape::bytes, p.cluster,
            stream, maps, p);
     return;
   }
@@ -701,26 +687,18 @@ void short_launch(Args a, const at::Tensor& k_pages, const at::Tensor& v_pages, 
   p.part_ml = p.part_o + 2ll * ctas * kRows * D;
   int* line = reinterpret_cast<int*>(p.part_o + floats);
   p.line = {line, line + 1, line + 1 + a.seqs};
-  launch(short_kernel<T, D, kM, false>, dim3(ctas), kShortThreads, Shape::bytes, 0, stream, maps, p);
+  launch(short_kernel<T, D, false>, dim3(ctas), kShortThreads, Shape::bytes, 0, stream, maps, p);
   launch(short_join_kernel<T, D>, dim3(static_cast<unsigned>(items * (kRows / 4))), 128, 0, 0, stream, p);
 }
 
-template <typename T, int D>
-void short_rows(const Args& a, const at::Tensor& k_pages, const at::Tensor& v_pages, int max_q_len, const at::Tensor& like,
-                cudaStream_t stream, int device) {
-  const int64_t rows = static_cast<int64_t>(max_q_len) * a.group;
-  if (rows <= 16) short_launch<T, D, 1>(a, k_pages, v_pages, like, stream, device);
-  else short_launch<T, D, 2>(a, k_pages, v_pages, like, stream, device);
-}
-
 void attend_short(const Args& a, int head_dim, bool half, const at::Tensor& k_pages, const at::Tensor& v_pages,
-                  int max_q_len, const at::Tensor& like, cudaStream_t stream, int device) {
+                  int, const at::Tensor& like, cudaStream_t stream, int device) {
   if (head_dim == 128)
-    half ? short_rows<__half, 128>(a, k_pages, v_pages, max_q_len, like, stream, device)
-         : short_rows<__nv_bfloat16, 128>(a, k_pages, v_pages, max_q_len, like, stream, device);
+    half ? short_launch<__half, 128>(a, k_pages, v_pages, like, stream, device)
+         : short_launch<__nv_bfloat16, 128>(a, k_pages, v_pages, like, stream, device);
   else
-    half ? short_rows<__half, 64>(a, k_pages, v_pages, max_q_len, like, stream, device)
-         : short_rows<__nv_bfloat16, 64>(a, k_pages, v_pages, max_q_len, like, stream, device);
+    half ? short_launch<__half, 64>(a, k_pages, v_pages, like, stream, device)
+         : short_launch<__nv_bfloat16, 64>(a, k_pages, v_pages, like, stream, device);
 }
 
 }  // namespace paged
