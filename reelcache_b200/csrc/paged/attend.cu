@@ -67,6 +67,7 @@ std::pair<at::Tensor, c10::optional<at::Tensor>> paged_attention(
   a.out = out.data_ptr();
   a.out_token = out.stride(0);
   a.out_head = out.stride(1);
+  a.out_sectors = out.stride(0) % 16 == 0 && out.stride(1) % 16 == 0 && reinterpret_cast<uintptr_t>(out.data_ptr()) % 32 == 0;
   c10::optional<at::Tensor> lse;
   if (want_lse) {
     lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));

@@ -31,6 +31,7 @@ struct Args {
   int64_t q_token, q_head;
   void* out;
   int64_t out_token, out_head;
+  int out_sectors;  // every row of out begins on 32 bytes
   float* lse;  // [tokens, heads] or null
   const int* table;
   const int* kv_lens;

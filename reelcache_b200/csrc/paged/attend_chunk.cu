@@ -2,8 +2,9 @@
 // with Q, K, V in bf16 or fp16, head_dim 64 or 128, scores, statistics and outputs accumulated in FP32.
 //
 // What bounds it: the tensor core and the exponentials. A tile of 128 rows x 128 keys (head_dim 128) is 8.4 MFLOP, 1,024
-// cycles of an SM's tcgen05 rate, and 16,384 exponentials, 1,024 cycles of its 16 a cycle. So the two have to run at the
-// same time, and a part of the exponentials goes to the FMA pipe.
+// cycles of an SM's tcgen05 rate, and 16,384 exponentials, 1,024 cycles of its 16 a cycle, so the two have to run at the
+// same time. In long runs the card's power limit binds before either (990 W, 1.3 to 1.7 GHz): what saves energy is what
+// helps then (exponentials by a polynomial on the FMA pipe cost 2 to 5 %; items out of step with each other 15 to 20 %).
 //
 // A CTA works on 256 rows as two tiles of 128 that share every K and V block. Rows are (query, head of the group),
 // query-major, so grouped heads share the loads of their KV head. 384 threads:
@@ -50,7 +51,6 @@ constexpr int kSoftmaxRegs = 208;
 constexpr int kRoleRegs = 88;
 static_assert(2 * kSoftmaxRegs + kRoleRegs == 3 * kLaunchRegs, "register split must equal the launch's registers");
 constexpr float kRescale = 8.0f;  // log2 units
-constexpr int kPolyEvery = 8;     // one of so many pairs of exponentials is taken from the FMA pipe
 
 template <int D, bool kTwin>
 struct ChunkShape {
@@ -302,32 +302,9 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-// 2^x for two x <= kRescale on the FMA and integer pipes: n = rint(x) through the low bits of x + 1.5 * 2^23, f = x - n
-// in [-1/2, 1/2], 2^f by the polynomial of degree 4 with p(0) = 1 that has the least relative error there (2.9e-6, a
-// thousandth of what rounding P to 16 bits loses), and n added to the exponent. Below 2^-125 it stays there (not masked
-// scores: those take the exponential unit, which gives 0).
-__device__ __forceinline__ void exp2_pair(uint64_t x, float& p0, float& p1) {
-  float x0, x1;
-  unpair(x, x0, x1);
-  x = pair(fmaxf(x0, -125.0f), fmaxf(x1, -125.0f));
-  const uint64_t magic = pair(12582912.0f, 12582912.0f), minus = pair(-12582912.0f, -12582912.0f);
-  const uint64_t t = add2(x, magic);
-  const uint64_t n = add2(t, minus);
-  const uint64_t f = fma2(n, pair(-1.0f, -1.0f), x);
-  uint64_t p = fma2(pair(0.009582853f, 0.009582853f), f, pair(0.055906426f, 0.055906426f));
-  p = fma2(p, f, pair(0.24024099f, 0.24024099f));
-  p = fma2(p, f, pair(0.69312418f, 0.69312418f));
-  p = fma2(p, f, pair(1.0f, 1.0f));
-  float t0, t1;
-  unpair(t, t0, t1);
-  unpair(p, p0, p1);
-  p0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
-  p1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
-}
-
 // Exponentials of half a row: 64 raw scores become 32 pairs of P; their sum is added to `sum`. kMax: the maximum of the
 // whole row (this half and `other`) is found on the way, two steps of it after every pair.
-template <typename T, int kPoly, bool kMax>
+template <typename T, bool kMax>
 __device__ __forceinline__ void softmax_half(const uint32_t (&r)[64], const uint32_t (&other)[64], float scale_log2, float neg_m,
                                              uint32_t (&pk)[32], float& sum, float& top) {
   const uint64_t scale2 = pair(scale_log2, scale_log2), m2 = pair(neg_m, neg_m);
@@ -335,15 +312,10 @@ __device__ __forceinline__ void softmax_half(const uint32_t (&r)[64], const uint
   float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
   for (int c = 0; c < 32; ++c) {
-    const uint64_t x = fma2(pair(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1])), scale2, m2);
     float p0, p1;
-    if (kPoly > 0 && c % (kPoly > 0 ? kPoly : 1) == 1) {
-      exp2_pair(x, p0, p1);
-    } else {
-      unpair(x, p0, p1);
-      p0 = exp2_approx(p0);
-      p1 = exp2_approx(p1);
-    }
+    unpair(fma2(pair(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1])), scale2, m2), p0, p1);
+    p0 = exp2_approx(p0);
+    p1 = exp2_approx(p1);
     if (kMax) {
       m[c & 1] = max3(m[c & 1], __uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]));
       m[2 + (c & 1)] = max3(m[2 + (c & 1)], __uint_as_float(other[2 * c]), __uint_as_float(other[2 * c + 1]));
@@ -368,23 +340,26 @@ __device__ __forceinline__ float row_max(const uint32_t (&r)[2][64]) {
   return max3(max3(m[0], m[1], m[2]), max3(m[3], m[4], m[5]), fmaxf(m[6], m[7]));
 }
 
-// Scores outside [from, high) and [0, sink) of the tile become minus infinity; 16 columns at a time are left alone where
-// no row of the warp has one. kHalf: 0 or 1.
+// Bits [0, n) of a word.
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+
+// Scores outside [from, high) and [0, sink) of the tile become minus infinity: 32 columns at a time as bits of a word, and
+// not at all where no row of the warp has one. kHalf: 0 or 1.
 template <int kHalf>
 __device__ __forceinline__ void mask_half(uint32_t (&r)[64], int from, int high, int sink) {
 #pragma unroll
-  for (int b = 4 * kHalf; b < 4 * kHalf + 4; ++b) {
-    if (__all_sync(0xffffffffu, high >= 16 * b + 16 && (from <= 16 * b || sink >= 16 * b + 16))) continue;
+  for (int w = 0; w < 2; ++w) {
+    const int first = 64 * kHalf + 32 * w;
+    const uint32_t seen = low_bits(high - first) & (~low_bits(from - first) | low_bits(sink - first));
+    if (__all_sync(0xffffffffu, seen == 0xffffffffu)) continue;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int c = 16 * b + e;
-      if (c >= high || (c < from && c >= sink)) r[c & 63] = __float_as_uint(-INFINITY);
-    }
+    for (int e = 0; e < 32; ++e)
+      if ((seen & (1u << e)) == 0) r[32 * w + e] = __float_as_uint(-INFINITY);
   }
 }
 
 // A whole sector in one store: a thread writes its own row, so narrower stores would each touch a sector of their own.
-__device__ __forceinline__ void store_32_bytes(float* dst, const uint32_t* v) {
+__device__ __forceinline__ void store_32_bytes(void* dst, const uint32_t* v) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]),
                "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                : "memory");
@@ -721,7 +696,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     const uint32_t o_col = tmem_base + 256 + g * kTile + lanes;
     bool ok = true;
     int it = 0;
-    for (int n = 0; ok && next(n); ++n) {
+    bool more = next(0);
+    for (int n = 0; ok && more; ++n) {
       const int packed = seg.item.row_tile * Shape::rows + (kTwin ? 0 : g * kTile) + row;
       const int query = packed / a.group;
       const Sight sight(a, seg.item.kv_len, seg.item.q_len);
@@ -750,8 +726,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         if (t < seg.t0 + (kTwin ? 2 : 1)) m_run = row_max(r) * a.scale_log2;
         float neg_m = m_run == -INFINITY ? 0.0f : -m_run;  // a row that has seen no key yet
         float sum = 0.0f, mx;
-        if (whole) softmax_half<T, kPolyEvery, true>(r[0], r[1], a.scale_log2, neg_m, pk, sum, mx);
-        else softmax_half<T, 0, true>(r[0], r[1], a.scale_log2, neg_m, pk, sum, mx);
+        softmax_half<T, true>(r[0], r[1], a.scale_log2, neg_m, pk, sum, mx);
         mx *= a.scale_log2;
         const bool need = mx > m_run + kRescale;
         if (__any_sync(0xffffffffu, need)) {
@@ -773,15 +748,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           tmem_wait_ld();
           if (!whole) mask_half<0>(r[0], from, high, sink);
           sum = 0.0f;
-          softmax_half<T, 0, false>(r[0], r[1], a.scale_log2, neg_m, pk, sum, mx);
+          softmax_half<T, false>(r[0], r[1], a.scale_log2, neg_m, pk, sum, mx);
         }
         tmem_st_32x32b_x32(s_col, pk);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[2 * g]);
-        if (whole) softmax_half<T, kPolyEvery, false>(r[1], r[0], a.scale_log2, neg_m, pk, sum, mx);
-        else softmax_half<T, 0, false>(r[1], r[0], a.scale_log2, neg_m, pk, sum, mx);
+        softmax_half<T, false>(r[1], r[0], a.scale_log2, neg_m, pk, sum, mx);
         l_run += sum;
         tmem_st_32x32b_x32(s_col + 32, pk);
         tmem_wait_st();
@@ -789,6 +763,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[2 * g + 1]);
       }
+      // the next piece of work is looked up before the stores of this one fill the memory pipe
+      Segment after = seg;
+      more = kDirect ? false : after.load(p, share, cta, n + 1);
       const bool none = kTwin && seg.t0 + g >= seg.t1;  // a twin without blocks
       if (ok && !none) ok = __all_sync(0xffffffffu, mbar_wait_park(&o_done[g], n & 1, status, kTimeoutEpilogue));
       if (kDirect && (kTwin || p.cluster > 1)) {
@@ -826,9 +803,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             uint32_t w[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) w[e] = pack2<T>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+            if (a.out_sectors) {
+              store_32_bytes(dst, w);
+              store_32_bytes(dst + 16, w + 8);
+            } else {
 #pragma unroll
-            for (int c = 0; c < 16; c += 4)
-              *reinterpret_cast<uint4*>(dst + 2 * c) = make_uint4(w[c], w[c + 1], w[c + 2], w[c + 3]);
+              for (int c = 0; c < 16; c += 4)
+                *reinterpret_cast<uint4*>(dst + 2 * c) = make_uint4(w[c], w[c + 1], w[c + 2], w[c + 3]);
+            }
           } else if (valid) {
             float* dst = p.part_o + slot * D + c0;
 #pragma unroll
@@ -841,6 +823,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           a.lse[token * a.heads + h] = l_run > 0.0f ? (m_run + log2f(l_run)) * kLn2 : -INFINITY;
         if (valid && !whole) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(m_run, l_run);
       }
+      seg = after;
     }
   }
 
@@ -929,18 +912,23 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const __grid_constant__
     sum = fmaf(sum, old, add);
 #pragma unroll
     for (int e = 0; e < kPer; ++e) acc[e] *= old;
-    uint32_t parts = __ballot_sync(0xffffffffu, part);
-#pragma unroll 4
-    while (parts != 0) {
-      const int i = __ffs(parts) - 1;
-      parts &= parts - 1;
-      const float w = __shfl_sync(0xffffffffu, wt, i);
-      const float* src = p.part_o + slot_of(cb + i) * D + lane * kPer;
+    const uint32_t parts = __ballot_sync(0xffffffffu, part);
+    for (int i0 = 0; i0 < 32 && (parts >> i0) != 0; i0 += 8) {
+      float2 x[8][kPer / 2];
 #pragma unroll
-      for (int e = 0; e < kPer; e += 2) {
-        const float2 x = *reinterpret_cast<const float2*>(src + e);
-        acc[e] = fmaf(w, x.x, acc[e]);
-        acc[e + 1] = fmaf(w, x.y, acc[e + 1]);
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int e = 0; e < kPer / 2; ++e)
+          x[i][e] = (parts >> (i0 + i)) & 1 ? *reinterpret_cast<const float2*>(p.part_o + slot_of(cb + i0 + i) * D + lane * kPer + 2 * e)
+                                            : make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float w = __shfl_sync(0xffffffffu, wt, i0 + i);
+#pragma unroll
+        for (int e = 0; e < kPer / 2; ++e) {
+          acc[2 * e] = fmaf(w, x[i][e].x, acc[2 * e]);
+          acc[2 * e + 1] = fmaf(w, x[i][e].y, acc[2 * e + 1]);
+        }
       }
     }
     if (__shfl_sync(0xffffffffu, to, 31) >= end) break;

@@ -389,6 +389,20 @@ def test_page_layouts_and_strided_queries(new):
     assert torch.equal(paged.attention(q, by_layer[1, 1], by_layer[1, 0], table, kv_lens, cu_q, max_q_len=new), want)
 
 
+@pytest.mark.parametrize("new", [1, 6, 150, 700])
+def test_outputs_given_with_strides(new):
+    """Outputs inside a larger buffer, on 16 but not on 32 bytes."""
+    from reelcache_b200.ops import paged
+    g = _gen(21)
+    k_pages, v_pages, table, kv_lens, cu_q = paged_batch(g, [new], [new + 900], 2, 64, 32, BF16)
+    q = torch.randn(new, 4, 64, generator=g, device="cuda").bfloat16()
+    want = paged.attention(q, k_pages, v_pages, table, kv_lens, cu_q, max_q_len=new)
+    buffer = torch.zeros(new, 5, 72, dtype=BF16, device="cuda")
+    paged.attention(q, k_pages, v_pages, table, kv_lens, cu_q, max_q_len=new, out=buffer[:, :4, 8:])
+    assert torch.equal(buffer[:, :4, 8:], want)
+    assert not bool(buffer[:, 4].any()) and not bool(buffer[:, :, :8].any())
+
+
 @pytest.mark.parametrize("new", [1, 200])
 def test_pages_beyond_32_bit_offsets(new):
     """A pool of more than 2^32 elements: its last pages are read where they are."""
