@@ -388,6 +388,70 @@ __device__ __forceinline__ uint64_t sw128_mnmajor_desc(uint32_t smem_addr, uint3
   return desc;
 }
 
+// The clustered end: the rows that the CTAs of a cluster hold in shared memory (row-major FP32, 16-byte chunks turned by
+// the row, maxima and sums at ml_off) become the item's output; rank r's threads take the r-th of every `cluster` blocks of
+// vectors. A thread has kBatch vectors of four channels and kParts CTAs' values of each in flight (remote shared memory
+// takes most of a microsecond).
+template <typename T, int D, int kBatch, int kParts>
+__device__ __forceinline__ void join_cluster(const Args& a, const Item& item, const uint8_t* smem, int ml_off, int item_rows,
+                                             int rank, int cluster) {
+  const int packed0 = item.row_tile * item_rows;
+  const int rows = static_cast<int>(min(static_cast<int64_t>(item_rows), static_cast<int64_t>(item.q_len) * a.group - packed0));
+  const int total = rows * (D / 4), step = cluster * kItemRows;
+  for (int v0 = rank * kItemRows + static_cast<int>(threadIdx.x); v0 < total; v0 += kBatch * step) {
+    float top[kBatch], sum[kBatch];
+    float4 acc[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      top[i] = -INFINITY;
+      sum[i] = 0.0f;
+      acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+    for (int c0 = 0; c0 < cluster; c0 += kParts) {
+      float2 ml[kBatch][kParts];
+      float4 x[kBatch][kParts];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int v = v0 + i * step, row = v / (D / 4), chunk = v % (D / 4);
+#pragma unroll
+        for (int j = 0; j < kParts; ++j) ml[i][j].x = -INFINITY;
+        if (v < total) {
+#pragma unroll
+          for (int j = 0; j < kParts; ++j) {
+            ml[i][j] = load_cluster_2(cluster_addr(reinterpret_cast<const float2*>(smem + ml_off) + row, c0 + j));
+            x[i][j] = load_cluster_4(cluster_addr(reinterpret_cast<const float4*>(smem) + row * (D / 4) + (chunk ^ (row & 15)), c0 + j));
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+#pragma unroll
+        for (int j = 0; j < kParts; ++j) {
+          if (ml[i][j].x == -INFINITY) continue;  // no key seen there (nor, perhaps, anything written)
+          const float mx = fmaxf(top[i], ml[i][j].x), old = exp2_approx(top[i] - mx), wt = exp2_approx(ml[i][j].x - mx);
+          top[i] = mx;
+          sum[i] = fmaf(sum[i], old, wt * ml[i][j].y);
+          acc[i].x = fmaf(acc[i].x, old, wt * x[i][j].x);
+          acc[i].y = fmaf(acc[i].y, old, wt * x[i][j].y);
+          acc[i].z = fmaf(acc[i].z, old, wt * x[i][j].z);
+          acc[i].w = fmaf(acc[i].w, old, wt * x[i][j].w);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int v = v0 + i * step, row = v / (D / 4), chunk = v % (D / 4);
+      if (v >= total) continue;
+      const float inv = sum[i] > 0.0f ? 1.0f / sum[i] : 0.0f;
+      const int query = (packed0 + row) / a.group, h = item.head * a.group + packed0 + row - query * a.group;
+      const int64_t token = item.q_first + query;
+      T* dst = static_cast<T*>(a.out) + token * a.out_token + h * a.out_head + chunk * 4;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(acc[i].x * inv, acc[i].y * inv), pack2<T>(acc[i].z * inv, acc[i].w * inv));
+      if (a.lse != nullptr && chunk == 0)
+        a.lse[token * a.heads + h] = sum[i] > 0.0f ? (top[i] + log2f(sum[i])) * kLn2 : -INFINITY;
+    }
+  }
+}
+
 template <typename T, int D, bool kDirect, bool kTwin>
 __global__ void __launch_bounds__(kChunkThreads, 1)
     chunk_kernel(const __grid_constant__ PageMaps maps, const __grid_constant__ Chunk p) {
@@ -771,9 +835,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       if (kDirect && (kTwin || p.cluster > 1)) {
         if (ok && (!kTwin || seg.t0 + 1 - g < seg.t1))
           ok = __all_sync(0xffffffffu, mbar_wait_park(&o_done[1 - g], 0, status, kTimeoutEpilogue));
-        if (ok) {  // every product is done: the operands' memory takes the rows, 16-byte chunks turned against bank conflicts
-          tc_fence_after();
-          float4* rows_at = reinterpret_cast<float4*>(smem) + (g * kTile + row) * (D / 4);
+        tc_fence_after();
+      }
+      // Every product is done in those forms, so the operands' memory takes rows: 16-byte chunks turned against bank
+      // conflicts, a row's maximum and sum behind them.
+      float4* rows_at = reinterpret_cast<float4*>(smem) + (g * kTile + row) * (D / 4);
+      float2* ml_at = reinterpret_cast<float2*>(smem + Shape::ml_off) + g * kTile + row;
+      float keep = 1.0f, add = 0.0f;  // twin: weights of this tile's row and the other's
+      if (kTwin) {
+        if (g == 1) {
 #pragma unroll
           for (int c0 = 0; c0 < D; c0 += 32) {
             uint32_t o[32];
@@ -784,8 +854,43 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
               rows_at[((c0 + c) / 4) ^ (row & 15)] = make_float4(__uint_as_float(o[c]), __uint_as_float(o[c + 1]),
                                                                   __uint_as_float(o[c + 2]), __uint_as_float(o[c + 3]));
           }
-          reinterpret_cast<float2*>(smem + Shape::ml_off)[g * kTile + row] = make_float2(m_run, l_run);
+          *ml_at = make_float2(m_run, l_run);
         }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (g == 1) break;
+        const float2 ml = ml_at[kTile];
+        const float top = fmaxf(m_run, ml.x), use = top == -INFINITY ? 0.0f : top;
+        keep = exp2_approx(m_run - use);
+        add = ml.x == -INFINITY ? 0.0f : exp2_approx(ml.x - use);
+        l_run = l_run * keep + add * ml.y;
+        m_run = top;
+      }
+      // (twin) the row's columns from c0 joined with the other tile's
+      auto join = [&](uint32_t (&o)[32], int c0) {
+        if (!kTwin || add == 0.0f) return;
+        const float4* other = rows_at + kTile * (D / 4);
+#pragma unroll
+        for (int c = 0; c < 32; c += 4) {
+          const float4 x = other[((c0 + c) / 4) ^ (row & 15)];
+          o[c] = __float_as_uint(fmaf(add, x.x, keep * __uint_as_float(o[c])));
+          o[c + 1] = __float_as_uint(fmaf(add, x.y, keep * __uint_as_float(o[c + 1])));
+          o[c + 2] = __float_as_uint(fmaf(add, x.z, keep * __uint_as_float(o[c + 2])));
+          o[c + 3] = __float_as_uint(fmaf(add, x.w, keep * __uint_as_float(o[c + 3])));
+        }
+      };
+      if (kDirect && p.cluster > 1) {
+#pragma unroll
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          uint32_t o[32];
+          tmem_ld_32x32b_x32(o_col + c0, o);
+          tmem_wait_ld();
+          join(o, c0);
+#pragma unroll
+          for (int c = 0; c < 32; c += 4)
+            rows_at[((c0 + c) / 4) ^ (row & 15)] = make_float4(__uint_as_float(o[c]), __uint_as_float(o[c + 1]),
+                                                                __uint_as_float(o[c + 2]), __uint_as_float(o[c + 3]));
+        }
+        *ml_at = make_float2(m_run, l_run);
       } else if (ok) {
         tc_fence_after();
         const bool valid = query < seg.item.q_len, whole = seg.starts && seg.ends;
@@ -798,6 +903,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           uint32_t o[32];
           tmem_ld_32x32b_x32(o_col + c0, o);
           tmem_wait_ld();
+          join(o, c0);
           if (valid && whole) {
             T* dst = static_cast<T*>(a.out) + token * a.out_token + h * a.out_head + c0;
             uint32_t w[16];
@@ -827,40 +933,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     }
   }
 
-  if (kDirect && (kTwin || p.cluster > 1)) {
+  if (kDirect && p.cluster > 1) {
     // CTAs without tiles have nothing to give; every CTA joins a part of the item's rows over all of them, in order.
     if (seg.t0 == seg.t1 && threadIdx.x < kItemRows)
       reinterpret_cast<float2*>(smem + Shape::ml_off)[threadIdx.x] = make_float2(-INFINITY, 0.0f);
     cluster_sync_all();
     if (threadIdx.x < kItemRows) {
-      const int packed0 = seg.item.row_tile * Shape::rows;
-      const int rows = static_cast<int>(min(static_cast<int64_t>(Shape::rows), static_cast<int64_t>(seg.item.q_len) * a.group - packed0));
-      const int rank = cta % p.cluster;
-      for (int v = rank * kItemRows + static_cast<int>(threadIdx.x); v < rows * (D / 4); v += p.cluster * kItemRows) {
-        const int row = v / (D / 4), chunk = v % (D / 4);
-        float top = -INFINITY, sum = 0.0f;
-        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int c = 0; c < (kTwin ? 2 : 1) * p.cluster; ++c) {
-          const int at = row + (kTwin ? (c & 1) * kTile : 0), cta_of = kTwin ? c >> 1 : c;
-          const float4* from = reinterpret_cast<const float4*>(smem) + at * (D / 4) + (chunk ^ (row & 15));
-          const float2 ml = load_cluster_2(cluster_addr(reinterpret_cast<const float2*>(smem + Shape::ml_off) + at, cta_of));
-          if (ml.x == -INFINITY) continue;  // no key seen there (nor, perhaps, anything written)
-          const float4 x = load_cluster_4(cluster_addr(from, cta_of));
-          const float mx = fmaxf(top, ml.x), old = exp2_approx(top - mx), wt = exp2_approx(ml.x - mx);
-          top = mx;
-          sum = fmaf(sum, old, wt * ml.y);
-          acc.x = fmaf(acc.x, old, wt * x.x);
-          acc.y = fmaf(acc.y, old, wt * x.y);
-          acc.z = fmaf(acc.z, old, wt * x.z);
-          acc.w = fmaf(acc.w, old, wt * x.w);
-        }
-        const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-        const int query = (packed0 + row) / a.group, h = seg.item.head * a.group + packed0 + row - query * a.group;
-        const int64_t token = seg.item.q_first + query;
-        T* dst = static_cast<T*>(a.out) + token * a.out_token + h * a.out_head + chunk * 4;
-        *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
-        if (a.lse != nullptr && chunk == 0) a.lse[token * a.heads + h] = sum > 0.0f ? (top + log2f(sum)) * kLn2 : -INFINITY;
-      }
+      if (p.cluster >= 8) join_cluster<T, D, 1, 8>(a, seg.item, smem, Shape::ml_off, Shape::rows, cta % p.cluster, p.cluster);
+      else if (p.cluster >= 4) join_cluster<T, D, 2, 4>(a, seg.item, smem, Shape::ml_off, Shape::rows, cta % p.cluster, p.cluster);
+      else join_cluster<T, D, 4, 2>(a, seg.item, smem, Shape::ml_off, Shape::rows, cta % p.cluster, p.cluster);
     }
     cluster_sync_all();  // the others have read this CTA's rows
   }
