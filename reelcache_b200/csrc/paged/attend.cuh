@@ -46,6 +46,15 @@ struct Args {
   int* status;
 };
 
+// Keys of a sequence: as many as kv_lens says and its row of the table can name (a longer length is reported).
+__device__ __forceinline__ int held_keys(const Args& a, int s) {
+  const int64_t most = static_cast<int64_t>(a.width) * a.tiling.page;
+  const int n = max(0, __ldg(a.kv_lens + s));
+  if (n <= most) return n;
+  if (a.status != nullptr) atomicCAS(a.status + kPagedWord, 0, kPageRange);
+  return static_cast<int>(most);
+}
+
 // The keys that queries see. A query whose last key is at `last` sees [max(0, last - window + 1), last] and the sinks
 // [0, sinks) below it; `last` is the query's own position (causal) or the sequence's end.
 struct Sight {

@@ -124,7 +124,7 @@ __device__ __forceinline__ int sequence(const Args& a, int s, int* q_first, int*
   *q_first = __ldg(a.cu_q + s);
   int q_len = min(__ldg(a.cu_q + s + 1), a.tokens) - *q_first;
   if (*q_first < 0 || q_len < 0) q_len = 0;
-  *kv_len = static_cast<int>(min(static_cast<int64_t>(max(0, __ldg(a.kv_lens + s))), static_cast<int64_t>(a.width) * a.tiling.page));
+  *kv_len = held_keys(a, s);
   return q_len;
 }
 
@@ -1024,8 +1024,9 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const __grid_constant__
 }
 
 template <typename T, int D, bool kDirect, bool kTwin>
-void chunk_configure() {
-  static bool configured = false;
+void chunk_configure(int device) {
+  static bool known[64] = {};
+  bool& configured = known[device & 63];
   if (configured) return;
   RC_CUDA(cudaFuncSetAttribute(chunk_kernel<T, D, kDirect, kTwin>, cudaFuncAttributeMaxDynamicSharedMemorySize, ChunkShape<D, kTwin>::bytes));
   if (kDirect) RC_CUDA(cudaFuncSetAttribute(chunk_kernel<T, D, kDirect, kTwin>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
@@ -1102,12 +1103,12 @@ void chunk_launch(const Args& args, const at::Tensor& k_pages, const at::Tensor&
   // tiles of an item, at most: the table's width, or what a window leaves of it
   int64_t keys = static_cast<int64_t>(args.width) * args.tiling.page;
   if (args.window > 0) keys = std::min<int64_t>(keys, static_cast<int64_t>(args.window) + args.sinks + kItemRows / args.group + 2 * kTile);
-  chunk_configure<T, D, true, false>();
+  chunk_configure<T, D, true, false>(device);
   const int64_t tiles = (keys + kTile - 1) / kTile;
   const bool twin = static_cast<int64_t>(max_q_len) * args.group <= kTile;
   p.cluster = direct_cluster<T, D>(most_items, twin ? (tiles + 1) / 2 : tiles, args.causal && row_tiles > 1, device);
   if (p.cluster > 0 && twin) {
-    chunk_configure<T, D, true, true>();
+    chunk_configure<T, D, true, true>(device);
     launch(chunk_kernel<T, D, true, true>, dim3(static_cast<unsigned>(grid_items * p.cluster)), kChunkThreads,
            ChunkShape<D, true>::bytes, p.cluster, stream, maps, p);
     return;
@@ -1117,7 +1118,7 @@ void chunk_launch(const Args& args, const at::Tensor& k_pages, const at::Tensor&
            stream, maps, p);
     return;
   }
-  chunk_configure<T, D, false, false>();
+  chunk_configure<T, D, false, false>(device);
   RC_CHECK(p.ctas < kPlanThreads, "more SMs than the plan's threads");
   const int64_t o_floats = 2ll * p.ctas * kItemRows * D, ml_floats = 2ll * p.ctas * kItemRows * 2;
   const int64_t ints = most_items * 8 + 4 + 2ll * (p.ctas + 1) + args.seqs;

@@ -97,8 +97,7 @@ struct SeqWork {
     q_first = __ldg(a.cu_q + s);
     q_len = min(__ldg(a.cu_q + s + 1), a.tokens) - q_first;
     if (q_first < 0 || q_len < 0) q_len = 0;
-    kv_len = static_cast<int>(min(static_cast<int64_t>(max(0, __ldg(a.kv_lens + s))),
-                                  static_cast<int64_t>(a.width) * a.tiling.page));
+    kv_len = held_keys(a, s);
     tiles = 0;
     if (q_len > 0) tiles = max(1, TileRange<kShortTile>(Sight(a, kv_len, q_len), 0, q_len).count());
   }
@@ -654,7 +653,8 @@ template <typename T, int D>
 void short_launch(Args a, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& like, cudaStream_t stream,
                   int device) {
   using Shape = ShortShape<D>;
-  static bool configured = false;
+  static bool known[64] = {};
+  bool& configured = known[device & 63];
   if (!configured) {
     RC_CUDA(cudaFuncSetAttribute(short_kernel<T, D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::bytes));
     RC_CUDA(cudaFuncSetAttribute(short_kernel<T, D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::bytes));

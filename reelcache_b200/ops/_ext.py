@@ -28,7 +28,8 @@ STATUS_NAMES = {
     0x301: "bad kernel argument",
     0x401: "too few free pages: the page-table call was refused and changed nothing",
     0x402: "a sequence or length of a page-table call is invalid: the call was refused and changed nothing",
-    0x403: "a page number lies outside the pool: its keys read as zeros, writes to it were dropped",
+    0x403: "a page number lies outside the pool, or a length outside the block table: such keys read as zeros or not at "
+           "all, writes to them were dropped",
 }
 
 

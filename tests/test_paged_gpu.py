@@ -489,6 +489,11 @@ def test_attention_page_out_of_range_is_reported(cuda_device):
                 assert bool(torch.isfinite(out.float()).all())
                 with pytest.raises(DeviceStatusError, match="page number"):
                     _ext.check_status(cuda_device)
+    for most in (1, 150):  # a length that the table's row cannot name
+        out = paged.attention(q[:most], k_pages, v_pages, table[:1], kv_lens[:1] + 10 ** 6, torch.tensor([0, most], dtype=torch.int32, device="cuda"),
+                              max_q_len=most)
+        with pytest.raises(DeviceStatusError, match="block table"):
+            _ext.check_status(cuda_device)
 
 
 def test_attention_refusals():
