@@ -3,26 +3,35 @@
 //
 // What bounds it: the tensor core and the exponentials. A tile of 128 rows x 128 keys (head_dim 128) is 8.4 MFLOP, 1,024
 // cycles of an SM's tcgen05 rate, and 16,384 exponentials, 1,024 cycles of its 16 a cycle, so the two have to run at the
-// same time. In long runs the card's power limit binds before either (990 W, 1.3 to 1.7 GHz): what saves energy is what
-// helps then (exponentials by a polynomial on the FMA pipe cost 2 to 5 %; items out of step with each other 15 to 20 %).
+// same time. Measured: 3,300 cycles for a pair of tiles (2,048 of them on the tensor core); 4,680 tokens over 23,400 keys
+// of 12 heads 556 us in a short run (1,210 TFLOP/s), 645 us in a long one, where the card's power limit binds before
+// either (990 W, 1.3 to 1.7 GHz): what saves energy is what helps then (exponentials by a polynomial on the FMA pipe cost
+// 2 to 5 %; items out of step with each other 15 to 20 %).
 //
 // A CTA works on 256 rows as two tiles of 128 that share every K and V block. Rows are (query, head of the group),
 // query-major, so grouped heads share the loads of their KV head. 384 threads:
 //   warps 0-3, 4-7  softmax of tile 0, 1: a thread owns a row (TMEM lane). S comes from TMEM, the running maximum moves
 //                   only when it grows by more than 8 (log2; then the row of O is rescaled in TMEM), P goes back to TMEM
-//                   over S, where the P V product reads it as its A operand, in two halves of 64 keys: the
-//                   product over the first runs during the exponentials of the second.
+//                   over S, where the P V product reads it as its A operand, in two halves of 64 keys: the product over
+//                   the first runs during the exponentials of the second.
 //   warps 8, 9      TMA: K blocks into a ring of 3, V blocks into a ring of 2. One box per page (or part of it).
-//   warp 10         issues the products, in the order O_0 += P_0 V', S_0 = Q_0 K, O_1 += P_1 V', S_1 = Q_1 K (V' of the
-//                   block before), without a break between one item and the next.
+//   warp 10         one thread issues the products, in the order O_0 += P_0 V', S_0 = Q_0 K, O_1 += P_1 V', S_1 = Q_1 K
+//                   (V' of the block before), without a break between one item and the next.
 //   warp 11         gathers the rows of Q with cp.async into the swizzled layout (any group size and strides).
 // V is read as it lies in the pages (keys x channels: an MN-major B operand), no transposed copy exists.
 // TMEM: S_g at column 128 g (P_g in its first 64), O_g at 256 + 128 g.
 //
-// Work: an item is 256 rows of one sequence and KV head with the tiles that they see. A plan kernel lists the items on the
-// device (the lengths never leave it) and deals them out: whole rounds of one item per SM as long as no SM gets more than
-// its share of all tiles, so that neighbours read the same keys at the same time; then the rest, cut like one line so that
-// every SM ends with its share. An item that is cut leaves FP32 parts, which a third kernel joins in order.
+// Twin form, up to 128 rows: both tiles hold the same rows, tile 0 takes the even blocks of keys and tile 1 the odd ones,
+// so that twice the keys are in flight; the tiles are joined at the end through shared memory. 16 sessions x 16 tokens over
+// 4,096 keys (32 / 8 heads): 49 us, 67.8 us with the second tile idle, 89.9 us on mma.sync.
+//
+// Work: an item is 256 (twin: 128) rows of one sequence and KV head with the tiles that they see.
+//   direct   a cluster of 1 to 16 CTAs per item, each with an even part of its tiles; they join through distributed shared
+//            memory. One launch, no workspace: for work that a wave or two holds.
+//   planned  a plan kernel lists the items on the device (the lengths never leave it) and deals them out: whole rounds of
+//            one item per SM as long as no SM gets more than its share of all tiles, so that neighbours read the same keys
+//            at the same time; then the rest, cut like one line so that every SM ends with its share. An item that is cut
+//            leaves FP32 parts, which a third kernel joins in order. Plan and join cost about 20 us.
 //
 // Every wait is bounded (2 s): on expiry a status is recorded, the roles stop, the products in flight are drained and TMEM
 // is freed.

@@ -9,11 +9,15 @@
 // consumer warps take 16 keys of each tile: every warp runs its own online softmax (maximum, sum and output in FP32
 // registers) and meets the others only when a sequence and head is finished.
 //
-// Work: all tiles of all (sequence, KV head) in one line, cut into equal shares, one per CTA, so ragged
-// batches and a single long sequence fill all SMs alike, and the host needs no lengths. A CTA whose share holds only a
-// part of an item leaves (output, maximum, sum) in FP32 in the workspace; a second kernel joins the parts in order of
-// the CTAs (no atomics: results do not depend on timing). It is launched as a programmatic dependent, so its launch
-// overlaps the first kernel.
+// Work, shared out: all tiles of all (sequence, KV head) in one line, cut into equal shares, one per CTA, so ragged batches
+// and a single long sequence fill all SMs alike, and the host needs no lengths. A CTA whose share holds only a part of an
+// item leaves (output, maximum, sum) in FP32 in the workspace; a second kernel joins the parts in order of the CTAs (no
+// atomics: results do not depend on timing).
+// Work, clustered (few sequences): a cluster of up to 16 CTAs per sequence and head, joined through distributed shared
+// memory; no scan of the lengths, no workspace, no second launch.
+//
+// Measured: 48 sessions of up to 16,384 keys (32 / 8 heads, 1.67 GB) 255 to 260 us, 6.5 TB/s; one session over 2,048 keys
+// 7.9 us clustered, 11.7 us shared out.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
