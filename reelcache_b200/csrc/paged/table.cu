@@ -14,7 +14,8 @@
 // allocate, fork and compact start with a plan by one block of 1,024 threads: prefix sums over the call's sequences and
 // over refcount, which it reads only as far as it finds what it needs. A call that cannot be served (too few free pages,
 // a sequence out of range or named twice, a table row too short, a child that still holds pages) is refused whole: the
-// plan writes nothing but the status word. Tables, counts and data are then moved by one launch over all SMs, which
+// plan writes nothing but the status word (a release skips sequences out of range, and gives back once what is named
+// twice). Tables, counts and data are then moved by one launch over all SMs, which
 // reads the plan from device memory. The plan is latency (4 to 6 us); the move is a copy, bound by HBM (measured: 0.5 GB of
 // pages moved together in 155 us, 6.3 TB/s read and written).
 #include <ATen/ATen.h>

@@ -27,7 +27,8 @@ STATUS_NAMES = {
     0x201: "peer flag wait timed out",
     0x301: "bad kernel argument",
     0x401: "too few free pages: the page-table call was refused and changed nothing",
-    0x402: "a sequence or length of a page-table call is invalid: the call was refused and changed nothing",
+    0x402: "a sequence or length of a page-table call is invalid: the call was refused and changed nothing (a release "
+           "skips such sequences)",
     0x403: "a page number lies outside the pool, or a length outside the block table: such keys read as zeros or not at "
            "all, writes to them were dropped",
 }
