@@ -135,6 +135,11 @@ __device__ __forceinline__ void load_page_box(void* dst, const CUtensorMap* map,
 }
 
 // Distributed shared memory: values of another CTA of the cluster (addresses from cluster_addr).
+__device__ __forceinline__ uint32_t cluster_addr_of(uint32_t addr, int rank) {
+  uint32_t out;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(addr), "r"(rank));
+  return out;
+}
 __device__ __forceinline__ float2 load_cluster_2(uint32_t addr) {
   float2 v;
   asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");

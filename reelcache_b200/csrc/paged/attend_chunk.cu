@@ -31,7 +31,7 @@
 //   planned  a plan kernel lists the items on the device (the lengths never leave it) and deals them out: whole rounds of
 //            one item per SM as long as no SM gets more than its share of all tiles, so that neighbours read the same keys
 //            at the same time; then the rest, cut like one line so that every SM ends with its share. An item that is cut
-//            leaves FP32 parts, which a third kernel joins in order. Plan and join cost about 20 us.
+//            leaves FP32 parts, which a third kernel joins in order. Plan, cut items and join cost about 25 us.
 //
 // Every wait is bounded (2 s): on expiry a status is recorded, the roles stop, the products in flight are drained and TMEM
 // is freed.
@@ -75,7 +75,8 @@ struct ChunkShape {
   static constexpr int bar_off = v_off + v_stages * tile_bytes;
   static constexpr int bytes = bar_off + 256 + 1024;  // + barriers, alignment slack
   static constexpr int ml_off = kItemRows * D * 4;    // at the end, clustered: rows of FP32 from 0, then maxima and sums
-  static_assert(ml_off + kItemRows * 8 <= bar_off, "the rows fit where the operands were");
+  static constexpr int scratch_off = ml_off + kItemRows * 8;  // weights of a share's rows and parts, places of its rows
+  static_assert(scratch_off + kItemRows * 4 + kItemRows * 8 <= bar_off, "the rows fit where the operands were");
   static_assert(bytes <= 227 * 1024, "shared memory of one CTA");
 };
 
@@ -398,66 +399,78 @@ __device__ __forceinline__ uint64_t sw128_mnmajor_desc(uint32_t smem_addr, uint3
 }
 
 // The clustered end: the rows that the CTAs of a cluster hold in shared memory (row-major FP32, 16-byte chunks turned by
-// the row, maxima and sums at ml_off) become the item's output; rank r's threads take the r-th of every `cluster` blocks of
-// vectors. A thread has kBatch vectors of four channels and kParts CTAs' values of each in flight (remote shared memory
-// takes most of a microsecond).
-template <typename T, int D, int kBatch, int kParts>
-__device__ __forceinline__ void join_cluster(const Args& a, const Item& item, const uint8_t* smem, int ml_off, int item_rows,
-                                             int rank, int cluster) {
+// the row, maxima and sums at ml_off) become the item's output, each CTA an even share of the rows. A thread per row and
+// part finds the part's weight and where the row goes (scratch_off: weights, then places); then a warp or half per row adds
+// the parts, a vector of four channels a lane, kRows rows and kParts parts of it in flight, the first of them asked for
+// before the weights are (remote shared memory takes most of a microsecond; more than eight vectors spill, and a spilled
+// load waits). 256 threads; `cluster` is a power of two up to 16. Weights found again for each vector took 10 us of a 45 us
+// call of clusters of two; so, 3 us.
+template <typename T, int D, int kRows, int kParts>
+__device__ __forceinline__ void join_cluster(const Args& a, const Item& item, uint8_t* smem, int ml_off, int scratch_off,
+                                             int item_rows, int rank, int cluster) {
+  constexpr int kLanes = D / 4, kStep = 8 * (32 / kLanes);
   const int packed0 = item.row_tile * item_rows;
   const int rows = static_cast<int>(min(static_cast<int64_t>(item_rows), static_cast<int64_t>(item.q_len) * a.group - packed0));
-  const int total = rows * (D / 4), step = cluster * kItemRows;
-  for (int v0 = rank * kItemRows + static_cast<int>(threadIdx.x); v0 < total; v0 += kBatch * step) {
-    float top[kBatch], sum[kBatch];
-    float4 acc[kBatch];
+  const int share = (rows + cluster - 1) / cluster, first = rank * share, count = min(share, rows - first), last = max(count, 1) - 1;
+  float* weights = reinterpret_cast<float*>(smem + scratch_off);                     // [share][cluster]
+  int64_t* places = reinterpret_cast<int64_t*>(smem + scratch_off + kItemRows * 4);  // [share]
+
+  const int chunk = threadIdx.x % kLanes;
+  float4 x[kRows][kParts];
+  const auto load = [&](int r0, int c0) {
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      top[i] = -INFINITY;
-      sum[i] = 0.0f;
-      acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int i = 0; i < kRows; ++i) {
+      const int row = first + min(r0 + i * kStep, last);
+      const uint32_t at = smem_u32(smem) + (row * kLanes + (chunk ^ (row & 15))) * 16;
+#pragma unroll
+      for (int j = 0; j < kParts; ++j) x[i][j] = load_cluster_4(cluster_addr_of(at, c0 + j));
     }
-    for (int c0 = 0; c0 < cluster; c0 += kParts) {
-      float2 ml[kBatch][kParts];
-      float4 x[kBatch][kParts];
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const int v = v0 + i * step, row = v / (D / 4), chunk = v % (D / 4);
-#pragma unroll
-        for (int j = 0; j < kParts; ++j) ml[i][j].x = -INFINITY;
-        if (v < total) {
-#pragma unroll
-          for (int j = 0; j < kParts; ++j) {
-            ml[i][j] = load_cluster_2(cluster_addr(reinterpret_cast<const float2*>(smem + ml_off) + row, c0 + j));
-            x[i][j] = load_cluster_4(cluster_addr(reinterpret_cast<const float4*>(smem) + row * (D / 4) + (chunk ^ (row & 15)), c0 + j));
-          }
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i)
-#pragma unroll
-        for (int j = 0; j < kParts; ++j) {
-          if (ml[i][j].x == -INFINITY) continue;  // no key seen there (nor, perhaps, anything written)
-          const float mx = fmaxf(top[i], ml[i][j].x), old = exp2_approx(top[i] - mx), wt = exp2_approx(ml[i][j].x - mx);
-          top[i] = mx;
-          sum[i] = fmaf(sum[i], old, wt * ml[i][j].y);
-          acc[i].x = fmaf(acc[i].x, old, wt * x[i][j].x);
-          acc[i].y = fmaf(acc[i].y, old, wt * x[i][j].y);
-          acc[i].z = fmaf(acc[i].z, old, wt * x[i][j].z);
-          acc[i].w = fmaf(acc[i].w, old, wt * x[i][j].w);
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const int v = v0 + i * step, row = v / (D / 4), chunk = v % (D / 4);
-      if (v >= total) continue;
-      const float inv = sum[i] > 0.0f ? 1.0f / sum[i] : 0.0f;
+  };
+  int r0 = threadIdx.x / kLanes, c0 = 0;
+  {
+    const int at = threadIdx.x / cluster, part = threadIdx.x % cluster, row = first + min(at, last);
+    const float2 ml = load_cluster_2(cluster_addr(reinterpret_cast<const float2*>(smem + ml_off) + row, part));
+    load(r0, c0);
+    float top = ml.x;
+    for (int i = cluster >> 1; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
+    const float weight = exp2_approx(ml.x - (top == -INFINITY ? 0.0f : top));
+    float sum = weight * ml.y;
+    for (int i = cluster >> 1; i > 0; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
+    weights[threadIdx.x] = ml.x == -INFINITY ? -1.0f : weight / sum;  // (-1: no key seen there, nor, perhaps, anything written)
+    if (part == 0 && at < count) {
       const int query = (packed0 + row) / a.group, h = item.head * a.group + packed0 + row - query * a.group;
       const int64_t token = item.q_first + query;
-      T* dst = static_cast<T*>(a.out) + token * a.out_token + h * a.out_head + chunk * 4;
-      *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(acc[i].x * inv, acc[i].y * inv), pack2<T>(acc[i].z * inv, acc[i].w * inv));
-      if (a.lse != nullptr && chunk == 0)
-        a.lse[token * a.heads + h] = sum[i] > 0.0f ? (top[i] + log2f(sum[i])) * kLn2 : -INFINITY;
+      places[at] = token * a.out_token + h * a.out_head;
+      if (a.lse != nullptr) a.lse[token * a.heads + h] = sum > 0.0f ? (top + log2f(sum)) * kLn2 : -INFINITY;
     }
+  }
+  asm volatile("bar.sync 3, 256;" ::: "memory");
+  float4 acc[kRows] = {};
+  while (r0 < count) {
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+#pragma unroll
+      for (int j = 0; j < kParts; ++j) {
+        const float w = weights[min(r0 + i * kStep, last) * cluster + c0 + j];
+        if (w < 0.0f) continue;
+        acc[i].x = fmaf(w, x[i][j].x, acc[i].x);
+        acc[i].y = fmaf(w, x[i][j].y, acc[i].y);
+        acc[i].z = fmaf(w, x[i][j].z, acc[i].z);
+        acc[i].w = fmaf(w, x[i][j].w, acc[i].w);
+      }
+    c0 += kParts;
+    if (c0 == cluster) {
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        if (r0 + i * kStep < count)
+          *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + places[r0 + i * kStep] + chunk * 4) =
+              make_uint2(pack2<T>(acc[i].x, acc[i].y), pack2<T>(acc[i].z, acc[i].w));
+        acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      }
+      c0 = 0;
+      r0 += kRows * kStep;
+    }
+    if (r0 < count) load(r0, c0);
   }
 }
 
@@ -948,9 +961,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       reinterpret_cast<float2*>(smem + Shape::ml_off)[threadIdx.x] = make_float2(-INFINITY, 0.0f);
     cluster_sync_all();
     if (threadIdx.x < kItemRows) {
-      if (p.cluster >= 8) join_cluster<T, D, 1, 8>(a, seg.item, smem, Shape::ml_off, Shape::rows, cta % p.cluster, p.cluster);
-      else if (p.cluster >= 4) join_cluster<T, D, 2, 4>(a, seg.item, smem, Shape::ml_off, Shape::rows, cta % p.cluster, p.cluster);
-      else join_cluster<T, D, 4, 2>(a, seg.item, smem, Shape::ml_off, Shape::rows, cta % p.cluster, p.cluster);
+      const int rank = cta % p.cluster;
+      if (p.cluster >= 8) join_cluster<T, D, 1, 8>(a, seg.item, smem, Shape::ml_off, Shape::scratch_off, Shape::rows, rank, p.cluster);
+      else if (p.cluster >= 4) join_cluster<T, D, 2, 4>(a, seg.item, smem, Shape::ml_off, Shape::scratch_off, Shape::rows, rank, p.cluster);
+      else join_cluster<T, D, 4, 2>(a, seg.item, smem, Shape::ml_off, Shape::scratch_off, Shape::rows, rank, p.cluster);
     }
     cluster_sync_all();  // the others have read this CTA's rows
   }
@@ -1076,16 +1090,19 @@ int clusters_at_once(int size, int device) {
 }
 
 // CTAs of an item in the direct form, or 0 for the planned form, by estimated time in tile pairs (about 1.8 us each):
-// direct, every item takes its tiles over its cluster, in as many rounds as its clusters need; planned, all SMs share all
-// tiles, but the plan, the join and the cut items cost about 8 tiles.
+// direct, every item takes its tiles over its cluster, in as many rounds as its clusters need, and each round has its start
+// and end to pay: about 3.5 tiles alone, 6 in a cluster, which joins. Planned, all SMs share all tiles, but the plan, the join
+// and the cut items cost about 16. Measured with 1, 2, 4 and 8 CTAs and planned (us): 16 items of 63 tiles
+// 117, 65, 40, 52 and 40; 54 of 27: 55, 38, 50, 80 and 52; 32 of 63: 118, 66, 42, 78 and 57; 84 of 49: 97, 108, 105, 150
+// and 87; 16 of 8: 21, 18, 15, 25 and 25.
 template <typename T, int D>
 int direct_cluster(int64_t items, int64_t tiles, bool uneven, int device) {
-  double best = static_cast<double>(items) * tiles / sm_count(device) * (uneven ? 0.75 : 1.0) + 8.0;
+  double best = static_cast<double>(items) * tiles / sm_count(device) * (uneven ? 0.75 : 1.0) + 16.0;
   int cluster = 0;
   for (int c = 1; c <= 16; c *= 2) {
     const int64_t slots = clusters_at_once<T, D>(c, device);
     if (slots <= 0) continue;
-    const double t = static_cast<double>((items + slots - 1) / slots) * ((tiles + c - 1) / c) + (c > 1 ? 1.0 : 0.0);
+    const double t = static_cast<double>((items + slots - 1) / slots) * (static_cast<double>((tiles + c - 1) / c) + (c > 1 ? 6.0 : 3.5));
     if (t < best) {
       best = t;
       cluster = c;
