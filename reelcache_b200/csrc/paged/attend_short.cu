@@ -35,8 +35,6 @@ constexpr int kRows = 16;            // rows: new tokens x heads of a group, at 
 constexpr int kGroups = 4;           // consumer warps, each with 16 keys of a tile
 constexpr int kShortThreads = 160;   // four consumer warps, one producer warp
 constexpr int kShortCtasPerSm = 2;
-constexpr int kFewTiles = 8;         // tiles of a CTA that are done before an even share would have paid
-constexpr int kLongTiles = 64;       // the same where clusters are large and few
 constexpr int kShortLeast = 2;       // tiles of a share, at least: every part costs a pass through the workspace
 
 template <int D>
@@ -653,6 +651,62 @@ __global__ void __launch_bounds__(128) short_join_kernel(const __grid_constant__
   if (a.lse != nullptr && lane == 0) a.lse[token * a.heads + h] = sum > 0.0f ? (top + log2f(sum)) * kLn2 : -INFINITY;
 }
 
+// Clusters of `size` CTAs that run at the same time, or -1 where none does.
+template <typename T, int D>
+int short_clusters_at_once(int size, int device) {
+  static int known[64][5] = {};
+  int slot = 0;
+  while ((1 << slot) < size) ++slot;
+  int& count = known[device & 63][slot];
+  if (count == 0) {
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<unsigned>(size));
+    config.blockDim = dim3(kShortThreads);
+    config.dynamicSmemBytes = ShortShape<D>::bytes;
+    cudaLaunchAttribute attribute{};
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = size;
+    attribute.val.clusterDim.y = 1;
+    attribute.val.clusterDim.z = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, short_kernel<T, D, true>, &config) != cudaSuccess) {
+      (void)cudaGetLastError();
+      n = 0;
+    }
+    count = n > 0 ? n : -1;
+  }
+  return count;
+}
+
+// CTAs of an item in the clustered form, or 0 for the line, by estimated time in us. Clusters run in rounds of about 5 and
+// the tiles of a CTA: 0.6 and 0.045 for every box that fetches one (pages of 16, 128 channels: 16 boxes, 1.3), or what HBM
+// takes for all CTAs' tiles where that is more. The line takes 10, 0.2 for every part of an item (they are joined one after
+// the other) and HBM's time for an even share of all tiles, of which a ragged batch may have fewer than its table has room
+// for (so 0.75 of them). Measured clustered and as a line (8 KV heads, pages of 16): 1 session of 2,048 keys 8.1 and 13.4,
+// of 65,536 keys 97 and 60; 2 of 2,048 keys 11.0 (clusters of 8; of 16, in two rounds, 15.3) and 13.8, of 16,384 keys 51
+// and 35; 16 of 512 keys 11.4 and 13.8.
+template <typename T, int D>
+int short_cluster(int64_t items, int64_t tiles, int step, bool several, int device) {
+  const double hbm = 2.0 * ShortShape<D>::tile_bytes / 6.5e6;  // us of a tile, for one CTA alone
+  const double box = 0.6 + 0.045 * (2 * ShortShape<D>::boxes * kShortTile / step);
+  const double slots = kShortCtasPerSm * sm_count(device), share = std::max<double>(kShortLeast, items * tiles / slots);
+  double best = 10.0 + 0.2 * std::min<double>(tiles / kShortLeast, slots / items) + hbm * slots * (several ? 0.75 : 1.0) * share;
+  int cluster = 0;
+  for (int c = 2; c <= 16; c *= 2) {
+    const int64_t at_once = short_clusters_at_once<T, D>(c, device);
+    if (at_once <= 0) continue;
+    const double tile = std::max(box, hbm * c * std::min<int64_t>(items, at_once));
+    const double t = static_cast<double>((items + at_once - 1) / at_once) * (5.0 + tile * static_cast<double>((tiles + c - 1) / c));
+    if (t < best - (cluster > 0 ? 0.5 : 0.0)) {  // (larger clusters find room less easily: only where they gain something)
+      best = t;
+      cluster = c;
+    }
+  }
+  return cluster;
+}
+
 template <typename T, int D>
 void short_launch(Args a, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& like, cudaStream_t stream,
                   int device) {
@@ -671,13 +725,8 @@ void short_launch(Args a, const at::Tensor& k_pages, const at::Tensor& v_pages, 
   p.a.tiling = Tiling::of(a.tiling.page, kShortTile);
   const PageMaps maps = page_maps(k_pages, v_pages, p.a.tiling, kShortTile);
   const int64_t items = static_cast<int64_t>(a.seqs) * a.kv_heads, slots = sm_count(device) * kShortCtasPerSm;
-  // Clusters of the largest size that all find room at once, unless the table's width allows sequences so long that an
-  // even share of all tiles matters more than the second kernel that it costs (measured on one B200, 8 KV heads: one
-  // session of 2,048 keys 8.3 us clustered and 11.7 us shared out, 16 sessions of 512 keys 11 and 14 us, one session of
-  // 131,072 keys 104 and 95 us).
   const int64_t most_tiles = (static_cast<int64_t>(a.width) * a.tiling.page + kShortTile - 1) / kShortTile;
-  for (int c = 16; c > 1 && p.cluster == 0; c /= 2)
-    if (items * c <= slots && most_tiles <= c * (c >= 8 ? kLongTiles : kFewTiles)) p.cluster = c;
+  p.cluster = short_cluster<T, D>(items, most_tiles, p.a.tiling.step, a.seqs > 1, device);
   if (p.cluster > 0) {
     launch(short_kernel<T, D, true>, dim3(static_cast<unsigned>(items * p.cluster)), kShortThreads, Shape::bytes, p.cluster,
            stream, maps, p);
