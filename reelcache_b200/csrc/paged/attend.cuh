@@ -49,7 +49,7 @@ struct Args {
 // Keys of a sequence: as many as kv_lens says and its row of the table can name (a longer length is reported).
 __device__ __forceinline__ int held_keys(const Args& a, int s) {
   const int64_t most = static_cast<int64_t>(a.width) * a.tiling.page;
-  const int n = max(0, __ldg(a.kv_lens + s));
+  const int n = max(0, a.kv_lens[s]);
   if (n <= most) return n;
   if (a.status != nullptr) atomicCAS(a.status + kPagedWord, 0, kPageRange);
   return static_cast<int>(most);
@@ -108,7 +108,7 @@ struct Boxes {
   __device__ __forceinline__ int page(const int* table, int pages, const Tiling& t, int first, int lane, int* row, int* status) const {
     const int at = first + lane * rows, block = at / t.page;
     *row = at - block * t.page;
-    int page = __ldg(table + block);
+    int page = table[block];
     if (page < 0 || page >= pages) {
       page = -1;
       if (status != nullptr) atomicCAS(status + kPagedWord, 0, kPageRange);

@@ -131,8 +131,8 @@ __device__ __forceinline__ int plan_scan(int value, int* warp_sums, int* total) 
 
 // New tokens of a sequence (returned), where they begin and how many keys it has.
 __device__ __forceinline__ int sequence(const Args& a, int s, int* q_first, int* kv_len) {
-  *q_first = __ldg(a.cu_q + s);
-  int q_len = min(__ldg(a.cu_q + s + 1), a.tokens) - *q_first;
+  *q_first = a.cu_q[s];
+  int q_len = min(a.cu_q[s + 1], a.tokens) - *q_first;
   if (*q_first < 0 || q_len < 0) q_len = 0;
   *kv_len = held_keys(a, s);
   return q_len;

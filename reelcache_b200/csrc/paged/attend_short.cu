@@ -96,8 +96,8 @@ __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 128
 struct SeqWork {
   int q_first, q_len, kv_len, tiles;
   __device__ __forceinline__ SeqWork(const Args& a, int s) {
-    q_first = __ldg(a.cu_q + s);
-    q_len = min(__ldg(a.cu_q + s + 1), a.tokens) - q_first;
+    q_first = a.cu_q[s];
+    q_len = min(a.cu_q[s + 1], a.tokens) - q_first;
     if (q_first < 0 || q_len < 0) q_len = 0;
     kv_len = held_keys(a, s);
     tiles = 0;
@@ -292,8 +292,8 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
       const T* src = static_cast<const T*>(a.q) + static_cast<int64_t>(w.q_first + row_q[i]) * a.q_token + row_h[i] * a.q_head + c0;
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
-        q[k][i] = valid[i] ? __ldg(reinterpret_cast<const uint32_t*>(src + k * 16)) : 0u;
-        q[k][i + 2] = valid[i] ? __ldg(reinterpret_cast<const uint32_t*>(src + k * 16 + 8)) : 0u;
+        q[k][i] = valid[i] ? *reinterpret_cast<const uint32_t*>(src + k * 16) : 0u;
+        q[k][i + 2] = valid[i] ? *reinterpret_cast<const uint32_t*>(src + k * 16 + 8) : 0u;
       }
     }
     const int rows_here = w.q_len * a.group;  // or fewer: kRows

@@ -20,6 +20,9 @@ namespace paged {
 // Every kernel here is launched as a programmatic dependent of what runs before it on the stream: its launch and its setup
 // overlap that kernel's end. after_earlier() comes before its first access to global memory and waits until everything
 // before it on the stream is complete and visible; let_later() allows the next such kernel to be set up.
+// A grid is thus alive while kernels before it still write, so its inputs must not go through the non-coherent path, which
+// is for what nobody writes in a grid's lifetime: no __ldg and no __restrict__ on anything that another kernel makes
+// (rows, positions, tables, lengths, plans).
 #ifdef __CUDACC__
 __device__ __forceinline__ void after_earlier() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_later() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }

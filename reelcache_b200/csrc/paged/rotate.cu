@@ -150,17 +150,14 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant_
   const char* src = r.src + token * r.src_token + first * r.src_head + vec * 16;
 
   uint4 raw[kHeads][kParts];
-  auto load = [&](int done) {
+  auto load = [&](int i, int head) {
+    if (head < count) {
 #pragma unroll
-    for (int i = 0; i < kHeads; ++i) {
-      if (done + i < count) {
-#pragma unroll
-        for (int s = 0; s < kParts; ++s) raw[i][s] = __ldg(reinterpret_cast<const uint4*>(src + i * r.src_head + s * part_bytes));
-      }
+      for (int s = 0; s < kParts; ++s) raw[i][s] = *reinterpret_cast<const uint4*>(src + head * r.src_head + s * part_bytes);
     }
-    src += kHeads * r.src_head;
   };
-  load(0);
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i) load(i, i);
 
   char* dst = r.dst + first * r.dst_head + vec * 16;
   if (!kPaged || is_q) {
@@ -169,14 +166,14 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant_
     int lo = 0, hi = a.seqs - 1;  // the last sequence that starts at or before the token
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (__ldg(a.cu_q + mid) <= token) lo = mid;
+      if (a.cu_q[mid] <= token) lo = mid;
       else hi = mid - 1;
     }
-    const int begin = __ldg(a.cu_q + lo), end = __ldg(a.cu_q + lo + 1);
+    const int begin = a.cu_q[lo], end = a.cu_q[lo + 1];
     if (token < begin || token >= end) return;  // tokens past the last sequence belong to none
-    const int at = __ldg(a.kv_lens + lo) - end + token;
+    const int at = a.kv_lens[lo] - end + token;
     const int slot = at >= 0 ? at / a.page : -1;
-    const int page = slot >= 0 && slot < a.table_width ? __ldg(a.table + lo * a.table_row + slot) : -1;
+    const int page = slot >= 0 && slot < a.table_width ? a.table[lo * a.table_row + slot] : -1;
     if (page < 0 || page >= a.pages) {
       if (vec == 0 && a.status != nullptr) atomicCAS(a.status + kPagedWord, 0, kPageRange);
       return;
@@ -192,13 +189,14 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant_
       p[x] = 0.0f;
       if (x < a.axes) {
         const int64_t at = static_cast<int64_t>(token) * a.axes + x;
-        p[x] = a.position_float ? __ldg(static_cast<const float*>(a.positions) + at)
-                                : static_cast<float>(__ldg(static_cast<const int*>(a.positions) + at));
+        p[x] = a.position_float ? static_cast<const float*>(a.positions)[at]
+                                : static_cast<float>(static_cast<const int*>(a.positions)[at]);
       }
     }
 #pragma unroll
     for (int e0 = 0; e0 < kPairs; e0 += 2) {
       const int j0 = vec * kPairs + e0;
+      // (the table is written once, long before: the one input that no kernel writes)
       const float2 hi2 = __ldg(reinterpret_cast<const float2*>(a.turns + j0));
       const float2 lo2 = __ldg(reinterpret_cast<const float2*>(a.turns + a.pairs + j0));
 #pragma unroll
@@ -217,42 +215,42 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant_
     }
   }
 
-  for (int done = 0;;) {
+  for (int done = 0; done < count; done += kHeads) {
 #pragma unroll
     for (int i = 0; i < kHeads; ++i) {
       if (done + i >= count) continue;
+      uint4 out[kParts];
+#pragma unroll
+      for (int s = 0; s < kParts; ++s) out[s] = raw[i][s];
       if (!kPaged || is_q || is_k) {
         if (kHalves) {
           float x[kVec], y2[kVec];
-          Vec<T>::unpack(raw[i][0], x);
-          Vec<T>::unpack(raw[i][kParts - 1], y2);
+          Vec<T>::unpack(out[0], x);
+          Vec<T>::unpack(out[kParts - 1], y2);
 #pragma unroll
           for (int e = 0; e < kVec; ++e) {
             const float u = x[e] * cs[e % kPairs] - y2[e] * sn[e % kPairs];
             y2[e] = x[e] * sn[e % kPairs] + y2[e] * cs[e % kPairs];
             x[e] = u;
           }
-          raw[i][0] = Vec<T>::pack(x);
-          raw[i][kParts - 1] = Vec<T>::pack(y2);
+          out[0] = Vec<T>::pack(x);
+          out[kParts - 1] = Vec<T>::pack(y2);
         } else {
           float x[kVec];
-          Vec<T>::unpack(raw[i][0], x);
+          Vec<T>::unpack(out[0], x);
 #pragma unroll
           for (int e = 0; e < kVec / 2; ++e) {
             const float u = x[2 * e] * cs[e] - x[2 * e + 1] * sn[e];
             x[2 * e + 1] = x[2 * e] * sn[e] + x[2 * e + 1] * cs[e];
             x[2 * e] = u;
           }
-          raw[i][0] = Vec<T>::pack(x);
+          out[0] = Vec<T>::pack(x);
         }
       }
+      load(i, done + kHeads + i);  // before the store, which the compiler must take for one to the same memory
 #pragma unroll
-      for (int s = 0; s < kParts; ++s) *reinterpret_cast<uint4*>(dst + i * r.dst_head + s * part_bytes) = raw[i][s];
+      for (int s = 0; s < kParts; ++s) *reinterpret_cast<uint4*>(dst + (done + i) * r.dst_head + s * part_bytes) = out[s];
     }
-    done += kHeads;
-    if (done >= count) break;
-    dst += kHeads * r.dst_head;
-    load(done);
   }
 }
 

@@ -112,9 +112,8 @@ __device__ int list_free(const State& s, int wanted, int* list, int* warp_sums) 
 __device__ __forceinline__ bool take(int* seen, int seq) { return atomicExch(seen + seq, 1) == 0; }
 
 // scratch: list[pages] | offsets[n + 1] | seen[seqs]
-__global__ void __launch_bounds__(kPlanThreads) allocate_kernel(State s, const int* __restrict__ seqs,
-                                                                const int* __restrict__ lens, int n, int* list,
-                                                                int* offsets, int* seen, int* status) {
+__global__ void __launch_bounds__(kPlanThreads) allocate_kernel(State s, const int* seqs, const int* lens, int n,
+                                                                int* list, int* offsets, int* seen, int* status) {
   paged::let_later();
   paged::after_earlier();
   __shared__ int warp_sums[32];
@@ -168,10 +167,9 @@ __global__ void __launch_bounds__(kPlanThreads) allocate_kernel(State s, const i
 }
 
 // Plans a fork: move i copies the partial tail of fork i (rows 0: there is none).
-__global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(State s, const int* __restrict__ parents,
-                                                                 const int* __restrict__ children,
-                                                                 const int* __restrict__ at, int n, int* list, int* seen,
-                                                                 Plan plan, int* status) {
+__global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(State s, const int* parents, const int* children,
+                                                                 const int* at, int n, int* list, int* seen, Plan plan,
+                                                                 int* status) {
   paged::let_later();
   paged::after_earlier();
   __shared__ int warp_sums[32];
@@ -277,51 +275,56 @@ struct Storage {  // planes x pages, each page `page_bytes` contiguous bytes of 
   int row_bytes;
 };
 
-// The copies of a plan: items of (move, plane, 32 KB part), spread over the grid. rows == nullptr: whole pages.
+// The copies of a plan: items of (move, plane, 32 KB part), spread over the grid. rows == nullptr: whole pages. The next
+// item's entries of the plan are asked for before this one's stores, which the compiler must take for stores to the plan.
 __device__ __forceinline__ void move_pages(const Storage& st, int moves, int pages, const int* source, const int* target,
                                            const int* rows, int* status) {
   const int parts = static_cast<int>((st.page_bytes + kMoveBytes - 1) / kMoveBytes);
   const int64_t items = static_cast<int64_t>(moves) * st.planes * parts;
+  int src = 0, dst = 0;
+  int64_t bytes = 0;
+  auto look_up = [&](int64_t item) {
+    if (item >= items) return;
+    const int move = static_cast<int>(item / parts / st.planes);
+    src = source[move];
+    dst = target[move];
+    bytes = rows == nullptr ? st.page_bytes : static_cast<int64_t>(rows[move]) * st.row_bytes;
+  };
+  look_up(blockIdx.x);
   for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const int part = static_cast<int>(item % parts);
-    const int64_t rest = item / parts;
-    const int plane = static_cast<int>(rest % st.planes);
-    const int move = static_cast<int>(rest / st.planes);
-    const int src = __ldg(source + move), dst = __ldg(target + move);
-    const int64_t bytes = rows == nullptr ? st.page_bytes : static_cast<int64_t>(__ldg(rows + move)) * st.row_bytes;
-    if (bytes <= 0) continue;
-    if (src < 0 || src >= pages || dst < 0 || dst >= pages || bytes > st.page_bytes) {
+    const int plane = static_cast<int>(item / parts % st.planes);
+    const int64_t at = item % parts * kMoveBytes + threadIdx.x * 16, there = bytes;
+    bool ok = there > 0;
+    if (ok && (src < 0 || src >= pages || dst < 0 || dst >= pages || there > st.page_bytes)) {
       if (threadIdx.x == 0 && !(src == -1 && dst == -1)) refuse(status, kPageRange);
-      continue;
+      ok = false;
     }
     const char* from = st.base + plane * st.plane_stride + src * st.page_stride;
     char* to = st.base + plane * st.plane_stride + dst * st.page_stride;
-    const int64_t at = static_cast<int64_t>(part) * kMoveBytes + threadIdx.x * 16;
     uint4 v[kMoveVecs];
 #pragma unroll
     for (int e = 0; e < kMoveVecs; ++e) {
       const int64_t o = at + e * (kMoveThreads * 16);
-      if (o < bytes) v[e] = *reinterpret_cast<const uint4*>(from + o);
+      if (ok && o < there) v[e] = *reinterpret_cast<const uint4*>(from + o);
     }
+    look_up(item + gridDim.x);
 #pragma unroll
     for (int e = 0; e < kMoveVecs; ++e) {
       const int64_t o = at + e * (kMoveThreads * 16);
-      if (o < bytes) *reinterpret_cast<uint4*>(to + o) = v[e];
+      if (ok && o < there) *reinterpret_cast<uint4*>(to + o) = v[e];
     }
   }
 }
 
-__global__ void __launch_bounds__(kMoveThreads) copy_kernel(Storage st, int pages, const int* __restrict__ source,
-                                                            const int* __restrict__ target, const int* __restrict__ rows,
-                                                            int moves, int* status) {
+__global__ void __launch_bounds__(kMoveThreads) copy_kernel(Storage st, int pages, const int* source, const int* target,
+                                                            const int* rows, int moves, int* status) {
   paged::let_later();
   paged::after_earlier();
   move_pages(st, moves, pages, source, target, rows, status);
 }
 
-__global__ void __launch_bounds__(kMoveThreads) fork_kernel(State s, Storage st, const int* __restrict__ parents,
-                                                            const int* __restrict__ children, const int* __restrict__ at,
-                                                            int n, Plan plan, int* status) {
+__global__ void __launch_bounds__(kMoveThreads) fork_kernel(State s, Storage st, const int* parents, const int* children,
+                                                            const int* at, int n, Plan plan, int* status) {
   paged::let_later();
   paged::after_earlier();
   if (*plan.count < 0) return;
@@ -329,10 +332,10 @@ __global__ void __launch_bounds__(kMoveThreads) fork_kernel(State s, Storage st,
   for (int64_t c = static_cast<int64_t>(blockIdx.x) * kMoveThreads + threadIdx.x; c < cells;
        c += static_cast<int64_t>(gridDim.x) * kMoveThreads) {
     const int i = static_cast<int>(c / s.width), block = static_cast<int>(c - static_cast<int64_t>(i) * s.width);
-    const int len = __ldg(at + i), full = len / s.page, child = __ldg(children + i);
+    const int len = at[i], full = len / s.page, child = children[i];
     int page = -1;
     if (block < full) {
-      page = s.table[static_cast<int64_t>(__ldg(parents + i)) * s.width + block];
+      page = s.table[static_cast<int64_t>(parents[i]) * s.width + block];
       if (page >= 0 && page < s.pages) atomicAdd(s.refcount + page, 1);
     } else if (block == full && plan.rows[i] > 0) {
       page = plan.target[i];
@@ -344,8 +347,8 @@ __global__ void __launch_bounds__(kMoveThreads) fork_kernel(State s, Storage st,
   move_pages(st, n, s.pages, plan.source, plan.target, plan.rows, status);
 }
 
-__global__ void __launch_bounds__(kMoveThreads) compact_kernel(State s, Storage st, const int* __restrict__ place,
-                                                               const int* __restrict__ in_use, Plan plan, int* status) {
+__global__ void __launch_bounds__(kMoveThreads) compact_kernel(State s, Storage st, const int* place, const int* in_use, Plan plan,
+                                                               int* status) {
   paged::let_later();
   paged::after_earlier();
   const int moves = *plan.count, live = *in_use;
@@ -363,14 +366,14 @@ __global__ void __launch_bounds__(kMoveThreads) compact_kernel(State s, Storage 
   move_pages(st, moves, s.pages, plan.source, plan.target, nullptr, status);
 }
 
-__global__ void __launch_bounds__(kMoveThreads) release_kernel(State s, const int* __restrict__ seqs, int n, int* status) {
+__global__ void __launch_bounds__(kMoveThreads) release_kernel(State s, const int* seqs, int n, int* status) {
   paged::let_later();
   paged::after_earlier();
   const int64_t cells = static_cast<int64_t>(n) * s.width;
   for (int64_t c = static_cast<int64_t>(blockIdx.x) * kMoveThreads + threadIdx.x; c < cells;
        c += static_cast<int64_t>(gridDim.x) * kMoveThreads) {
     const int i = static_cast<int>(c / s.width), block = static_cast<int>(c - static_cast<int64_t>(i) * s.width);
-    const int seq = __ldg(seqs + i);
+    const int seq = seqs[i];
     if (seq < 0 || seq >= s.seqs) {
       if (block == 0) refuse(status, kPageRefused);
       continue;
