@@ -123,6 +123,17 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+// A row's maximum `top` and its sum of exp2(x - base_of(top)), and what follows from them. No key seen: -inf and 0, which
+// give zeros and a log-sum-exp of -inf. A score of +inf leaves the sum at +inf (so base_of is 0 there too), one of NaN at
+// NaN: log_sum passes both on, and the output, whose P holds them, is NaN. fade is what a sum or output that was taken
+// relative to `before` is worth relative to `top` (infinite maxima that agree are worth 1, not exp2(inf - inf)).
+__device__ __forceinline__ float base_of(float top) { return fabsf(top) == INFINITY ? 0.0f : top; }
+__device__ __forceinline__ float fade(float before, float top) { return before == top ? 1.0f : exp2_approx(before - top); }
+__device__ __forceinline__ float inverse(float sum) { return sum == 0.0f ? 0.0f : 1.0f / sum; }
+__device__ __forceinline__ float log_sum(float top, float sum) {
+  return sum == 0.0f ? -INFINITY : (base_of(top) + log2f(sum)) * kLn2;
+}
+
 // 4-D tile load of one page's rows: channels from c, token rows from `row`, one head, one page. A page number outside
 // the map reads zeros.
 __device__ __forceinline__ void load_page_box(void* dst, const CUtensorMap* map, uint64_t* bar, int c, int row, int head,

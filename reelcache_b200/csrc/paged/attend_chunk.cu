@@ -433,15 +433,16 @@ __device__ __forceinline__ void join_cluster(const Args& a, const Item& item, ui
     load(r0, c0);
     float top = ml.x;
     for (int i = cluster >> 1; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
-    const float weight = exp2_approx(ml.x - (top == -INFINITY ? 0.0f : top));
+    const float weight = exp2_approx(ml.x - base_of(top));
     float sum = weight * ml.y;
     for (int i = cluster >> 1; i > 0; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
-    weights[threadIdx.x] = ml.x == -INFINITY ? -1.0f : weight / sum;  // (-1: no key seen there, nor, perhaps, anything written)
+    // (-1: no key seen there, nor, perhaps, anything written)
+    weights[threadIdx.x] = ml.x == -INFINITY && ml.y == 0.0f ? -1.0f : weight / sum;
     if (part == 0 && at < count) {
       const int query = (packed0 + row) / a.group, h = item.head * a.group + packed0 + row - query * a.group;
       const int64_t token = item.q_first + query;
       places[at] = token * a.out_token + h * a.out_head;
-      if (a.lse != nullptr) a.lse[token * a.heads + h] = sum > 0.0f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+      if (a.lse != nullptr) a.lse[token * a.heads + h] = log_sum(top, sum);
     }
   }
   asm volatile("bar.sync 3, 256;" ::: "memory");
@@ -810,7 +811,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         // The exponentials start with the maximum so far, and this block's is found next to them (they leave issue slots
         // for it). Only where it has grown by more than kRescale are they done again.
         if (t < seg.t0 + (kTwin ? 2 : 1)) m_run = row_max(r) * a.scale_log2;
-        float neg_m = m_run == -INFINITY ? 0.0f : -m_run;  // a row that has seen no key yet
+        float neg_m = -base_of(m_run);
         float sum = 0.0f, mx;
         softmax_half<T, true>(r[0], r[1], a.scale_log2, neg_m, pk, sum, mx);
         mx *= a.scale_log2;
@@ -829,7 +830,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           }
           l_run *= alpha;
           if (need) m_run = mx;
-          neg_m = m_run == -INFINITY ? 0.0f : -m_run;
+          neg_m = -base_of(m_run);
           tmem_ld_32x32b_x64(s_col, r[0]);
           tmem_wait_ld();
           if (!whole) mask_half<0>(r[0], from, high, sink);
@@ -881,7 +882,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         asm volatile("bar.sync 1, 256;" ::: "memory");
         if (g == 1) break;
         const float2 ml = ml_at[kTile];
-        const float top = fmaxf(m_run, ml.x), use = top == -INFINITY ? 0.0f : top;
+        const float top = fmaxf(m_run, ml.x), use = base_of(top);
         keep = exp2_approx(m_run - use);
         add = ml.x == -INFINITY ? 0.0f : exp2_approx(ml.x - use);
         l_run = l_run * keep + add * ml.y;
@@ -916,7 +917,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       } else if (ok) {
         tc_fence_after();
         const bool valid = query < seg.item.q_len, whole = seg.starts && seg.ends;
-        const float inv = whole ? (l_run > 0.0f ? 1.0f / l_run : 0.0f) : 1.0f;
+        const float inv = whole ? inverse(l_run) : 1.0f;
         const int64_t token = seg.item.q_first + query;
         const int h = seg.item.head * a.group + packed - query * a.group;
         const int64_t slot = (2 * static_cast<int64_t>(cta) + (seg.starts ? 1 : 0)) * kItemRows + g * kTile + row;
@@ -948,7 +949,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         }
         tc_fence_before();  // the next item's products overwrite O after this warp's next arrival
         if (valid && whole && a.lse != nullptr)
-          a.lse[token * a.heads + h] = l_run > 0.0f ? (m_run + log2f(l_run)) * kLn2 : -INFINITY;
+          a.lse[token * a.heads + h] = log_sum(m_run, l_run);
         if (valid && !whole) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(m_run, l_run);
       }
       seg = after;
@@ -1007,8 +1008,7 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const __grid_constant__
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     mx = fmaxf(mx, top);
-    const float use = mx == -INFINITY ? 0.0f : mx;
-    const float old = exp2_approx(top - use), wt = exp2_approx(ml.x - use);
+    const float old = fade(top, mx), wt = exp2_approx(ml.x - base_of(mx));
     top = mx;
     float add = wt * ml.y;
 #pragma unroll
@@ -1037,13 +1037,13 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const __grid_constant__
     }
     if (__shfl_sync(0xffffffffu, to, 31) >= end) break;
   }
-  const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+  const float inv = inverse(sum);
   const int64_t token = item.q_first + query;
   const int h = item.head * a.group + packed - query * a.group;
   T* dst = static_cast<T*>(a.out) + token * a.out_token + h * a.out_head + lane * kPer;
 #pragma unroll
   for (int e = 0; e < kPer; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack2<T>(acc[e] * inv, acc[e + 1] * inv);
-  if (a.lse != nullptr && lane == 0) a.lse[token * a.heads + h] = sum > 0.0f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+  if (a.lse != nullptr && lane == 0) a.lse[token * a.heads + h] = log_sum(top, sum);
 }
 
 template <typename T, int D, bool kDirect, bool kTwin>

@@ -355,8 +355,8 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
           const float top = fmaxf(m[i], mx * a.scale_log2);
-          const float use = top == -INFINITY ? 0.0f : top;  // a row that has seen no key yet
-          alpha[i] = exp2_approx(m[i] - use);
+          const float use = base_of(top);
+          alpha[i] = fade(m[i], top);
           m[i] = top;
           float sum = 0.0f;
 #pragma unroll
@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
         gm[g] = join_ml[(g * kRows + r0 + 8 * i) * 2];
         top = fmaxf(top, gm[g]);
       }
-      const float use = top == -INFINITY ? 0.0f : top;
+      const float use = base_of(top);
 #pragma unroll
       for (int g = 0; g < kGroups; ++g)
         total = fmaf(join_ml[(g * kRows + r0 + 8 * i) * 2 + 1], exp2_approx(gm[g] - use), total);
@@ -535,8 +535,7 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
           float mx = top;
 #pragma unroll
           for (int c = 0; c < 8; ++c) mx = fmaxf(mx, ml[c].x);
-          const float use = mx == -INFINITY ? 0.0f : mx;
-          const float old = exp2_approx(top - use);
+          const float use = base_of(mx), old = fade(top, mx);
           top = mx;
           sum *= old;
           acc.x *= old, acc.y *= old, acc.z *= old, acc.w *= old;
@@ -550,12 +549,12 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
             acc.w = fmaf(wt, x[c].w, acc.w);
           }
         }
-        const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+        const float inv = inverse(sum);
         const int query = row / a.group, h = head * a.group + row - query * a.group;
         const int64_t token = w.q_first + query;
         T* dst = static_cast<T*>(a.out) + token * a.out_token + h * a.out_head + col;
         if (ok) *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
-        if (ok && a.lse != nullptr && col == 0) a.lse[token * a.heads + h] = sum > 0.0f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+        if (ok && a.lse != nullptr && col == 0) a.lse[token * a.heads + h] = log_sum(top, sum);
       }
       cluster_sync_all();  // the others have read this CTA's rows
       return;
@@ -568,13 +567,13 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
         if (!valid[i]) continue;
         const int64_t token = w.q_first + row_q[i];
         if (starts && ends) {
-          const float inv = l[i] > 0.0f ? 1.0f / l[i] : 0.0f;
+          const float inv = inverse(l[i]);
           T* dst = static_cast<T*>(a.out) + token * a.out_token + row_h[i] * a.out_head + c0;
 #pragma unroll
           for (int d = 0; d < D / 8; ++d)
             *reinterpret_cast<uint32_t*>(dst + d * 8) = pack2<T>(o[d][2 * i] * inv, o[d][2 * i + 1] * inv);
           if (a.lse != nullptr && (lane & 3) == 0)
-            a.lse[token * a.heads + row_h[i]] = l[i] > 0.0f ? (m[i] + log2f(l[i])) * kLn2 : -INFINITY;
+            a.lse[token * a.heads + row_h[i]] = log_sum(m[i], l[i]);
         } else {
           const int64_t slot = (2 * static_cast<int64_t>(blockIdx.x) + (starts ? 1 : 0)) * kRows + r0 + 8 * i;
           float* dst = p.part_o + slot * D + c0;
@@ -621,8 +620,7 @@ __global__ void __launch_bounds__(128) short_join_kernel(const __grid_constant__
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     mx = fmaxf(mx, top);
-    const float use = mx == -INFINITY ? 0.0f : mx;
-    const float old = exp2_approx(top - use), wt = exp2_approx(ml.x - use);
+    const float old = fade(top, mx), wt = exp2_approx(ml.x - base_of(mx));
     top = mx;
     float part = wt * ml.y;
 #pragma unroll
@@ -642,13 +640,13 @@ __global__ void __launch_bounds__(128) short_join_kernel(const __grid_constant__
       }
     }
   }
-  const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+  const float inv = inverse(sum);
   const int64_t token = w.q_first + query;
   const int h = head * a.group + row - query * a.group;
   T* dst = static_cast<T*>(a.out) + token * a.out_token + h * a.out_head + lane * kPer;
 #pragma unroll
   for (int e = 0; e < kPer; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack2<T>(acc[e] * inv, acc[e + 1] * inv);
-  if (a.lse != nullptr && lane == 0) a.lse[token * a.heads + h] = sum > 0.0f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+  if (a.lse != nullptr && lane == 0) a.lse[token * a.heads + h] = log_sum(top, sum);
 }
 
 // Clusters of `size` CTAs that run at the same time, or -1 where none does.

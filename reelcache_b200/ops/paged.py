@@ -39,7 +39,8 @@ def attention(q, k_pages, v_pages, block_table, kv_lens, cu_q, *, max_q_len: int
 
     ``causal``: a token sees positions up to its own; else every new token sees the whole sequence (a chunk that is
     bidirectional in itself). ``window`` keeps the last ``window`` of the positions it would see, and the first
-    ``sinks`` of the sequence. A token that sees nothing gets zeros (and ``lse`` of minus infinity).
+    ``sinks`` of the sequence. A token that sees nothing gets zeros (and ``lse`` of minus infinity). A
+    score of NaN makes its token's output and ``lse`` NaN; one of plus infinity makes ``lse`` plus infinity, the output NaN.
     ``max_q_len`` bounds the new tokens of every sequence. ``return_lse`` adds the natural log-sum-exp ``[T, heads]``."""
     if not q.is_cuda:
         raise UnsupportedError("paged attention needs CUDA tensors")

@@ -84,3 +84,66 @@ def test_calls_back_to_back_see_what_was_written_before(new, steps):
 
     for got, want in zip(run(False), run(True)):
         assert torch.equal(got, want)
+
+
+# -- values at the edges ----------------------------------------------------------------------------------------------
+
+def _same(got, want, bound):
+    """Within the bound, or NaN on both sides."""
+    return within(torch.where(want.isnan(), 0.0, got.double()), want.nan_to_num(0.0, posinf=math.inf, neginf=-math.inf),
+                  bound.nan_to_num(0.0)) and torch.equal(got.isnan(), want.isnan())
+
+
+# few rows clustered and as a line; the twin form; direct with one and with several CTAs; planned
+EDGE_SHAPES = [([1], [700], 4, 2), ([1] * 90, [40 + 7 * i for i in range(90)], 8, 4), ([30], [400], 4, 4), ([150], [300], 4, 2),
+               ([300], [3000], 2, 2), ([1100], [1500], 32, 32)]
+
+
+@pytest.mark.parametrize("kind", ["nan", "inf", "-inf", "nan query"])
+@pytest.mark.parametrize("new,totals,heads,kv_heads", EDGE_SHAPES)
+def test_nan_and_infinite_scores(new, totals, heads, kv_heads, kind):
+    """A NaN score makes its rows' outputs and log-sum-exps NaN; a score of plus infinity makes the log-sum-exp that, and
+    the output NaN; one of minus infinity weighs nothing. Rows that do not see the key keep their results."""
+    from reelcache_b200.ops import paged
+    d, page = 64, 16
+    g = _gen(31)
+    k_pages, v_pages, table, kv_lens, cu_q = paged_batch(g, new, totals, kv_heads, d, page, BF16)
+    q = torch.randn(sum(new), heads, d, generator=g, device="cuda").bfloat16()
+    q[..., 0] = 1.0
+    if kind == "nan query":
+        q[sum(new) // 2, 1, 5] = math.nan
+    else:
+        for s, total in enumerate(totals):  # one key that the last new tokens see and the first do not, and one that all see
+            for at in (total - 1 - new[s] // 3, total // 5):
+                k_pages[int(table[s, at // page]), at % page, 0] = 0.0
+                k_pages[int(table[s, at // page]), at % page, 0, 0] = float(kind)
+    for causal, window in ((True, None), (True, 17), (False, None)):
+        out, lse = paged.attention(q, k_pages, v_pages, table, kv_lens, cu_q, max_q_len=max(new), causal=causal, window=window, return_lse=True)
+        want, want_lse, bound, lse_bound = attend(q, k_pages, v_pages, table, kv_lens, new, causal=causal, window=window)
+        if kind == "-inf":  # (the bounds take magnitudes of scores: without the infinite ones)
+            finite = k_pages.clone()
+            finite[finite == -math.inf] = 0.0
+            bound, lse_bound = attend(q, finite, v_pages, table, kv_lens, new, causal=causal, window=window)[2:]
+        assert _same(lse, want_lse, lse_bound)
+        assert _same(out, want, bound)
+        assert kind == "-inf" or not bool(torch.isfinite(want_lse).all())
+
+
+def test_rows_whose_only_score_is_nan_or_minus_infinity():
+    """The first new token of a sequence without history sees one key, alone in its tile."""
+    from reelcache_b200.ops import paged
+    for new, heads in ((1, 2), (9, 2), (100, 2), (400, 2)):
+        for value in (math.nan, -math.inf, math.inf):
+            g = _gen(32)
+            k_pages, v_pages, table, kv_lens, cu_q = paged_batch(g, [new], [new], 1, 64, 16, BF16)
+            q = torch.randn(new, heads, 64, generator=g, device="cuda").bfloat16()
+            q[..., 0] = 1.0
+            k_pages[int(table[0, 0]), 0] = 0.0
+            k_pages[int(table[0, 0]), 0, 0, 0] = value
+            out, lse = paged.attention(q, k_pages, v_pages, table, kv_lens, cu_q, max_q_len=new, causal=True, return_lse=True)
+            if value == -math.inf:
+                assert not bool(out[0].any()) and bool((lse[0] == -math.inf).all())
+                assert bool(torch.isfinite(out.float()).all())
+            else:
+                assert bool(out.isnan().all())
+                assert bool(lse.isnan().all() if math.isnan(value) else (lse == math.inf).all())
