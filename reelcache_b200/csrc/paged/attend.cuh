@@ -65,7 +65,8 @@ struct Sight {
   __device__ __forceinline__ Sight(const Args& a, int kv_len, int q_len)
       : length(kv_len), first_last(a.causal ? kv_len - q_len : kv_len - 1), window(a.window), sinks(a.sinks), causal(a.causal) {}
   __device__ __forceinline__ int last(int query) const { return causal ? first_last + query : first_last; }
-  __device__ __forceinline__ int low(int last) const { return window > 0 ? max(0, last - window + 1) : 0; }
+  // (`last` may be far below 0, where last - window would wrap)
+  __device__ __forceinline__ int low(int last) const { return window > 0 && last >= window ? last - window + 1 : 0; }
 };
 
 // The tiles that the queries [first, end) of a sequence visit: [0, sink_end) and [window_begin, window_end).

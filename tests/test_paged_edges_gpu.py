@@ -147,3 +147,18 @@ def test_rows_whose_only_score_is_nan_or_minus_infinity():
             else:
                 assert bool(out.isnan().all())
                 assert bool(lse.isnan().all() if math.isnan(value) else (lse == math.inf).all())
+
+
+@pytest.mark.parametrize("new,totals", [([5], [2]), ([200, 1], [60, 0]), ([200, 30], [190, 30]), ([400], [390])])
+def test_a_window_of_any_size(new, totals):
+    """Positions before the first (more new tokens than the session holds) and a window up to the largest integer."""
+    from reelcache_b200.ops import paged
+    g = _gen(33)
+    k_pages, v_pages, table, kv_lens, cu_q = paged_batch(g, new, totals, 2, 64, 16, BF16, fill=math.nan)
+    q = torch.randn(sum(new), 4, 64, generator=g, device="cuda").bfloat16()
+    call = lambda **kw: paged.attention(q, k_pages, v_pages, table, kv_lens, cu_q, max_q_len=max(new), causal=True,  # noqa: E731
+                                        return_lse=True, **kw)
+    want = call()
+    for window in (2 ** 31 - 1, 2 ** 31 - 100, 2 ** 30):
+        for got, x in zip(call(window=window), want):
+            assert torch.equal(got, x)
