@@ -3,10 +3,12 @@
 #pragma once
 
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <initializer_list>
 #include <mutex>
 #include <stdexcept>
 #include <string>
@@ -96,6 +98,13 @@ inline int sm_count(int device) {
 
 inline void check_cuda_tensor(const at::Tensor& t, const char* name) {
   RC_CHECK(t.is_cuda(), std::string(name) + " must be a CUDA tensor");
+}
+
+// A dual tensor's tangent would be dropped by a kernel that computes on its values alone.
+inline void refuse_tangents(std::initializer_list<const at::Tensor*> tensors, const char* what) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const at::Tensor* t : tensors)
+    RC_CHECK(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), std::string(what) + " has no forward-mode derivative");
 }
 
 inline int* status_ptr(const c10::optional<at::Tensor>& status) {

@@ -35,6 +35,7 @@ std::pair<at::Tensor, c10::optional<at::Tensor>> paged_attention(
   check_cuda_tensor(q, "q");
   RC_CHECK(!c10::GradMode::is_enabled() || !(q.requires_grad() || k_pages.requires_grad() || v_pages.requires_grad()),
            "attention over pages has no gradient: call it without grad");
+  refuse_tangents({&q, &k_pages, &v_pages}, "attention over pages");
   const at::ScalarType type = q.scalar_type();
   RC_CHECK(type == at::kBFloat16 || type == at::kHalf, "paged attention takes bf16 or fp16");
   RC_CHECK(q.dim() == 3 && (q.size(2) == 64 || q.size(2) == 128), "q must be [tokens, heads, head_dim] with head_dim 64 or 128");

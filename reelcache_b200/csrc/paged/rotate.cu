@@ -367,6 +367,7 @@ at::Tensor paged_append(const at::Tensor& q, const at::Tensor& k, const at::Tens
   check_cuda_tensor(q, "q");
   RC_CHECK(!c10::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || v.requires_grad()),
            "append has no gradient: call it without grad");
+  refuse_tangents({&q, &k, &v, &positions, &k_pages, &v_pages}, "append");
   const at::ScalarType type = q.scalar_type();
   RC_CHECK(type == at::kBFloat16 || type == at::kHalf, "a paged cache holds bf16 or fp16");
   c10::cuda::CUDAGuard guard(q.device());

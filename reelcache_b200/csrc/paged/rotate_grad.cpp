@@ -46,6 +46,7 @@ struct RotateBackward : public torch::autograd::Node {
 
 variable_list turned(const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions,
                      const std::shared_ptr<RopePlan>& plan, double sign) {
+  refuse_tangents({&q, &k, &positions}, "rotate");
   std::shared_ptr<RotateBackward> node;
   if (torch::autograd::compute_requires_grad(q, k)) {
     node = std::shared_ptr<RotateBackward>(new RotateBackward(), torch::autograd::deleteNode);

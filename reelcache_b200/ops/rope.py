@@ -59,7 +59,7 @@ class AxisRope:
 def rotate(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, rope: AxisRope):
     """``q[T, heads, head_dim]`` and ``k[T, kv_heads, head_dim]`` (or ``None``) at ``positions[T, axes]`` (int32 or
     float32), rotated in one launch; bf16, fp16 or fp32, FP32 math. Rows may be strided (views of a fused projection).
-    Differentiable in ``q`` and ``k``. Returns ``(q', k')``, new contiguous tensors of the same type."""
+    Differentiable in ``q`` and ``k`` (in reverse mode). Returns ``(q', k')``, new contiguous tensors of the same type."""
     if not q.is_cuda:
         raise UnsupportedError("rotate needs CUDA tensors")
     if q.shape[-1] != rope.head_dim:

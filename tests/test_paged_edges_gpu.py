@@ -162,3 +162,30 @@ def test_a_window_of_any_size(new, totals):
     for window in (2 ** 31 - 1, 2 ** 31 - 100, 2 ** 30):
         for got, x in zip(call(window=window), want):
             assert torch.equal(got, x)
+
+
+# -- derivatives that the operators do not have -----------------------------------------------------------------------
+
+def test_forward_mode_tangents_are_refused():
+    """A tangent would be lost without a word: the calls raise, as they do for gradients that they do not have."""
+    from torch.autograd import forward_ad
+    from reelcache_b200.ops import paged
+    from reelcache_b200.ops.rope import AxisRope, rotate
+    g = _gen(41)
+    rope = AxisRope.wan(64)
+    k_pages, v_pages, table, kv_lens, cu_q = paged_batch(g, [3], [20], 2, 64, 16, BF16)
+    (positions,) = _ints([[1, 2, 3]] * 3)
+    q, k = (torch.randn(3, n, 64, generator=g, device="cuda").bfloat16() for n in (4, 2))
+    append = lambda q, k, v, kp, vp: paged.append(q, k, v, positions, rope, kp, vp, table, kv_lens, cu_q)  # noqa: E731
+    attention = lambda q, kp, vp: paged.attention(q, kp, vp, table, kv_lens, cu_q, max_q_len=3)  # noqa: E731
+    with forward_ad.dual_level():
+        dual = lambda x: forward_ad.make_dual(x, torch.ones_like(x))  # noqa: E731
+        for call, args in ((lambda a, b: rotate(a, b, positions, rope), (q, k)), (append, (q, k, k, k_pages, v_pages)),
+                           (attention, (q, k_pages, v_pages))):
+            for i in range(len(args)):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call(*[dual(x) if j == i else x for j, x in enumerate(args)])
+            call(*args)
+    before = k_pages.clone()
+    attention(q, k_pages, v_pages)
+    assert torch.equal(before, k_pages)
