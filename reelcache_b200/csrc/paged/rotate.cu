@@ -365,7 +365,7 @@ at::Tensor paged_append(const at::Tensor& q, const at::Tensor& k, const at::Tens
                         const at::Tensor& kv_lens, const at::Tensor& cu_q, const c10::optional<at::Tensor>& out,
                         const c10::optional<at::Tensor>& status) {
   check_cuda_tensor(q, "q");
-  RC_CHECK(!c10::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || v.requires_grad()),
+  RC_CHECK(!c10::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || v.requires_grad() || positions.requires_grad()),
            "append has no gradient: call it without grad");
   refuse_tangents({&q, &k, &v, &positions, &k_pages, &v_pages}, "append");
   const at::ScalarType type = q.scalar_type();

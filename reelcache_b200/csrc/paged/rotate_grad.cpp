@@ -47,6 +47,7 @@ struct RotateBackward : public torch::autograd::Node {
 variable_list turned(const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions,
                      const std::shared_ptr<RopePlan>& plan, double sign) {
   refuse_tangents({&q, &k, &positions}, "rotate");
+  RC_CHECK(!torch::autograd::compute_requires_grad(positions), "rotate has no gradient with respect to positions");
   std::shared_ptr<RotateBackward> node;
   if (torch::autograd::compute_requires_grad(q, k)) {
     node = std::shared_ptr<RotateBackward>(new RotateBackward(), torch::autograd::deleteNode);

@@ -189,3 +189,16 @@ def test_forward_mode_tangents_are_refused():
     before = k_pages.clone()
     attention(q, k_pages, v_pages)
     assert torch.equal(before, k_pages)
+
+
+def test_gradients_with_respect_to_positions_are_refused():
+    from reelcache_b200.ops.rope import AxisRope, rotate
+    q = torch.randn(3, 4, 64, device="cuda", requires_grad=True)
+    positions = torch.rand(3, 3, device="cuda", requires_grad=True)
+    with pytest.raises(RuntimeError, match="positions"):
+        rotate(q, None, positions, AxisRope.wan(64))
+    with torch.no_grad():
+        rotate(q, None, positions, AxisRope.wan(64))
+    out, _ = rotate(q, None, positions.detach(), AxisRope.wan(64))
+    out.sum().backward()
+    assert q.grad is not None
