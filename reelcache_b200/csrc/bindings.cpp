@@ -158,8 +158,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("dot2_gemm", &rc::dot2_gemm, "compensated FP32 GEMM out = x @ rows^T", py::arg("x"), py::arg("rows"),
         py::arg("out"));
   py::class_<rc::RopePlan, std::shared_ptr<rc::RopePlan>>(m, "RopePlan", "a multi-axis rotation's table on one device")
-      .def(py::init<const at::Tensor&, const std::vector<int64_t>&, bool>(), py::arg("turns"), py::arg("sections"),
-           py::arg("halves"))
+      .def(py::init<const at::Tensor&, const at::Tensor&, const std::vector<int64_t>&, bool>(), py::arg("turns"),
+           py::arg("exact"), py::arg("sections"), py::arg("halves"))
       .def_readonly("turns", &rc::RopePlan::turns);
   m.def("rotate", &rc::rotate, "multi-axis rotary positions of q and k (differentiable)", py::arg("q"), py::arg("k"),
         py::arg("positions"), py::arg("plan"));

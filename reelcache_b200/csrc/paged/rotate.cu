@@ -7,7 +7,9 @@
 //
 // The angle is kept in turns: w_j / (2 pi) comes as the sum of two FP32 numbers hi + lo, n = rint(p hi), and
 // fma(p, hi, -n) + p lo is the fraction of a turn, exact to an ULP of 0.5 however many turns p makes (p w in radians
-// would lose one bit for each doubling of p). sincospi takes it from there.
+// would lose one bit for each doubling of p). sincospi takes it from there. That holds for |p| < 2^24, which FP32 counts
+// exactly; a token with a position beyond takes the fraction in FP64 (off by 2^-25 of a turn at 2^31) from w_j / (2 pi) in
+// FP64: a branch that other tokens pass by.
 //
 // What bounds it: memory, one read and one write of q, k (and v); next, the sines. So a thread owns one 16-byte vector
 // position of a token (4 or 8 pairs), computes their sines once and applies them to as many heads of one tensor as leave
@@ -116,6 +118,7 @@ struct Args {
   int axes;
   int ends[4];             // first pair after each axis's section
   const float* turns;      // [2, pairs]: hi, lo
+  const double* exact;     // [pairs]: the same in FP64
   float sign;              // -1 turns back
   int tokens, pairs;
   // the paged form: k and v rows go to page table[seq][at / page], row at % page
@@ -127,6 +130,18 @@ struct Args {
   int64_t page_k, page_v;  // page strides in bytes (dst_token / dst_head are strides inside a page)
   int* status;
 };
+
+constexpr float kFar = 16777216.0f;  // 2^24: from here on FP32 does not hold every whole number
+
+// The fraction of a turn of pair j at a far position.
+__device__ __forceinline__ float far_part(const Args& a, int token, int j) {
+  const int axis = j < a.ends[0] ? 0 : j < a.ends[1] ? 1 : j < a.ends[2] ? 2 : 3;
+  const int64_t at = static_cast<int64_t>(token) * a.axes + axis;
+  const double p = a.position_float ? static_cast<double>(static_cast<const float*>(a.positions)[at])
+                                    : static_cast<double>(static_cast<const int*>(a.positions)[at]);
+  const double t = __ldg(a.exact + j), n = p * t;
+  return static_cast<float>((n - rint(n)) + fma(p, t, -n));
+}
 
 // kHalves: pairs (j, j + pairs), a thread holds one vector of each half; else neighbours in one vector.
 template <typename T, bool kHalves, bool kPaged, int kHeads>
@@ -184,6 +199,7 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant_
   float cs[kPairs], sn[kPairs];
   if (!kPaged || is_q || is_k) {
     float p[4];
+    bool far = false;
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       p[x] = 0.0f;
@@ -191,6 +207,7 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant_
         const int64_t at = static_cast<int64_t>(token) * a.axes + x;
         p[x] = a.position_float ? static_cast<const float*>(a.positions)[at]
                                 : static_cast<float>(static_cast<const int*>(a.positions)[at]);
+        far = far || fabsf(p[x]) >= kFar;
       }
     }
 #pragma unroll
@@ -204,7 +221,8 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant_
         const int j = j0 + e;
         const float pos = j < a.ends[0] ? p[0] : j < a.ends[1] ? p[1] : j < a.ends[2] ? p[2] : p[3];
         const float hi = e ? hi2.y : hi2.x, lo = e ? lo2.y : lo2.x;
-        const float part = fmaf(pos, lo, fmaf(pos, hi, -rintf(pos * hi)));
+        float part = fmaf(pos, lo, fmaf(pos, hi, -rintf(pos * hi)));
+        if (far) part = far_part(a, token, j);
         if (sizeof(T) == 4) {
           sincospif(2.0f * part, &sn[e0 + e], &cs[e0 + e]);
         } else {
@@ -308,6 +326,7 @@ void set_rotation(Args& a, const at::Tensor& positions, const RopePlan& plan, in
   a.position_float = positions.scalar_type() == at::kFloat;
   a.axes = axes;
   a.turns = plan.turns.data_ptr<float>();
+  a.exact = plan.exact.data_ptr<double>();
   a.tokens = static_cast<int>(tokens);
 }
 

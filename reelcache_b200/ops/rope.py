@@ -2,7 +2,8 @@
 row, column, ...), every channel pair belongs to one axis.
 
 Pair ``j`` of axis ``a`` (the ``i``-th of its ``sections[a]`` pairs) turns by ``positions[:, a] * theta ** (-i /
-sections[a])``. The angle is formed in turns from a two-float frequency, so its error does not grow with the position.
+sections[a])``. The angle is formed in turns, from a two-float frequency below 2^24 and in FP64 beyond, so its error does
+not grow with the position.
 """
 
 from __future__ import annotations
@@ -52,7 +53,7 @@ class AxisRope:
             turns = self.theta ** -torch.cat(exponents) / (2.0 * math.pi)
             high = turns.float()
             table = torch.stack([high, (turns - high.double()).float()]).to(device)
-            plan = self._plans[device] = ext().RopePlan(table, self.sections, self.layout == "halves")
+            plan = self._plans[device] = ext().RopePlan(table, turns.to(device), self.sections, self.layout == "halves")
         return plan
 
 

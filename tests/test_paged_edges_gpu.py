@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from .paged_support import attend, paged_batch, within
+from .paged_support import attend, paged_batch, rotate_bound, within
 
 pytestmark = pytest.mark.gpu
 
@@ -202,3 +202,35 @@ def test_gradients_with_respect_to_positions_are_refused():
     out, _ = rotate(q, None, positions.detach(), AxisRope.wan(64))
     out.sum().backward()
     assert q.grad is not None
+
+
+# -- positions beyond what a float can count --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("layout", ["interleaved", "halves"])
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+def test_rotate_positions_of_any_size(dtype, layout):
+    """int32 positions up to the largest, and float32 ones beyond 2^24: the angles in 80-bit floats are off by less than
+    2^31 * 2^-63 of a radian."""
+    import numpy as np
+    from reelcache_b200.ops.rope import AxisRope, rotate
+    sections = (22, 21, 21)
+    rope = AxisRope(128, sections, layout=layout)
+    q = torch.randn(64, 2, 128, generator=_gen(51), device="cuda").to(dtype)
+    rng = np.random.default_rng(51)
+    some = rng.integers(-2 ** 31, 2 ** 31, (64, 3))
+    some[0], some[1], some[2] = 2 ** 31 - 1, -2 ** 31, (2 ** 24, 2 ** 24 + 1, 2 ** 24 - 1)
+    some[3:20] = rng.integers(2 ** 24, 2 ** 25, (17, 3)) | 1
+    assert np.finfo(np.longdouble).nmant >= 63
+    for kind in (torch.int32, FP32):
+        positions = torch.tensor(some).to(kind).cuda()
+        at = positions.cpu().numpy().astype(np.longdouble)
+        angle = np.concatenate([at[:, a:a + 1] * np.longdouble(10000) ** (-np.arange(n, dtype=np.longdouble) / n)
+                                for a, n in enumerate(sections)], axis=1)
+        cos, sin = (torch.tensor(f(angle).astype(np.float64), device="cuda")[:, None] for f in (np.cos, np.sin))
+        x = q.double()
+        a, b = (x[..., 0::2], x[..., 1::2]) if layout == "interleaved" else x.chunk(2, dim=-1)
+        u, v, size = a * cos - b * sin, a * sin + b * cos, a.abs() + b.abs()
+        pairs = [(u, v), (size, size)]
+        want, size = (torch.stack(p, dim=-1).flatten(-2) if layout == "interleaved" else torch.cat(p, dim=-1) for p in pairs)
+        got, _ = rotate(q, None, positions, rope)
+        assert within(got, want, rotate_bound(want, size, dtype)), float(((got.double() - want).abs()).max())
