@@ -10,7 +10,9 @@ A step over a batch of sessions::
     q = cache.append(layer, batch, q, k, v, positions, rope)
     o = cache.attend(layer, batch, q)
 
-A session is rewound by forking it at the earlier length and closing it.
+A session is rewound by forking it at the earlier length and closing it. A batch is good as long as its sessions are open
+and their pages where they were; it can be written as long as no fork has taken its new tokens. :meth:`PagedKVCache.again`
+gives a new one.
 """
 
 from __future__ import annotations
@@ -26,12 +28,19 @@ from .ops.rope import AxisRope
 
 
 class _Block:
-    """One page that sessions hold, as the host counts it."""
+    """One page that sessions hold, as the host counts it: its holders, and the forks that copied its first rows (when, and
+    how many; of several, those that no later one exceeds)."""
 
-    __slots__ = ("holders",)
+    __slots__ = ("holders", "copies")
 
     def __init__(self):
         self.holders = 1
+        self.copies = []
+
+    def copied(self, when: int, rows: int):
+        while self.copies and self.copies[-1][1] <= rows:
+            self.copies.pop()
+        self.copies.append((when, rows))
 
 
 @dataclass
@@ -47,13 +56,17 @@ class PagedSession:
 @dataclass(frozen=True)
 class PagedBatch:
     """Sessions with new tokens, as the device operators take them: rows of the block table, lengths with the new tokens,
-    where each session's new tokens begin."""
+    where each session's new tokens begin. Made by a cache, whose calls refuse it once it is out of date."""
 
     sessions: tuple
     counts: tuple
+    lengths: tuple
     table: torch.Tensor
     kv_lens: torch.Tensor
     cu_q: torch.Tensor
+    cache: "PagedKVCache" = field(repr=False, compare=False)
+    made: int = field(repr=False, compare=False)  # the cache's change before it
+    checked: list = field(repr=False, compare=False)  # [the change after which it was last found good to write]
 
     @property
     def tokens(self) -> int:
@@ -88,6 +101,7 @@ class PagedKVCache:
         self._planes = self.storage.flatten(0, 1)
         self._free_slots = list(range(max_sessions))[::-1]
         self._held = 0
+        self._changes = self._compacted = 0  # forks, ends and compactions so far; which of them was the last compaction
 
     # -- sessions --------------------------------------------------------------------------------------------------------
 
@@ -135,12 +149,14 @@ class PagedKVCache:
             return []
         self._admit(sum(n % self.page_size > 0 for n in lengths))
         slots = self._take_slots(len(lengths))
+        self._changes += 1
         children = []
         for slot, n in zip(slots, lengths):
             child = PagedSession(slot, n, True, session.blocks[:n // self.page_size])
             for block in child.blocks:
                 block.holders += 1
             if n % self.page_size:
+                session.blocks[n // self.page_size].copied(self._changes, n % self.page_size)
                 child.blocks.append(_Block())
                 self._held += 1
             children.append(child)
@@ -155,6 +171,7 @@ class PagedKVCache:
         if not sessions:
             return
         self.table.release(self._ints(s.slot for s in sessions))
+        self._changes += 1
         for s in sessions:
             for block in s.blocks:
                 block.holders -= 1
@@ -203,24 +220,50 @@ class PagedKVCache:
         for n in counts:
             starts.append(starts[-1] + n)
         table = self.table.block_table[:, :width].index_select(0, slots)
-        return PagedBatch(tuple(sessions), tuple(counts), table, lens, self._ints(starts))
+        return PagedBatch(tuple(sessions), tuple(counts), tuple(s.length for s in sessions), table, lens, self._ints(starts),
+                          self, self._changes, [self._changes])
+
+    def _check_batch(self, batch: PagedBatch, *, write: bool):
+        """Refuse a batch whose pages may hold something else by now, or (``write``) whose new tokens a fork has taken:
+        writing them would change the child's history, or leave what it copied behind."""
+        if batch.cache is not self:
+            raise StateError("the batch is another cache's")
+        if batch.checked[0] == self._changes:
+            return
+        self._check(batch.sessions)
+        if batch.made < self._compacted:
+            raise StateError("the batch is from before a compaction, which moved pages: make it again")
+        if not write:
+            return
+        for s, n, length in zip(batch.sessions, batch.counts, batch.lengths):
+            first = length - n
+            for i in range(first // self.page_size, -(-length // self.page_size) if n else 0):
+                block, row = s.blocks[i], max(first - i * self.page_size, 0)
+                if block.holders > 1 or any(when > batch.made and rows > row for when, rows in block.copies):
+                    raise StateError(f"the session in slot {s.slot} was forked after the batch, with its new tokens: fork before "
+                                     "them, or make the batch again")
+        batch.checked[0] = self._changes
 
     def compact(self) -> int:
         """Move the pages in use to the front of the pool (the rest of the storage is then free in one piece). Returns how
-        many there are. Batches made before are stale."""
+        many there are. Batches made before are refused from here on."""
         self.table.compact(self._planes)
+        self._changes += 1
+        self._compacted = self._changes
         return self._held
 
     # -- layers ----------------------------------------------------------------------------------------------------------
 
     def append(self, layer: int, batch: PagedBatch, q, k, v, positions, rope: AxisRope, *, out=None):
         """Write the new tokens of one layer (``k`` rotated at ``positions``, ``v`` as it is); returns ``q`` rotated."""
+        self._check_batch(batch, write=True)
         return paged.append(q, k, v, positions, rope, self.storage[layer, 0], self.storage[layer, 1], batch.table,
                             batch.kv_lens, batch.cu_q, out=out)
 
     def attend(self, layer: int, batch: PagedBatch, q, *, causal: bool = False, window: int | None = None, sinks: int = 0,
                scale: float | None = None, return_lse: bool = False, out=None):
         """Attention of the new tokens over their sessions (:func:`reelcache_b200.ops.paged.attention`)."""
+        self._check_batch(batch, write=False)
         return paged.attention(q, self.storage[layer, 0], self.storage[layer, 1], batch.table, batch.kv_lens, batch.cu_q,
                                max_q_len=max(max(batch.counts), 1), causal=causal, window=window, sinks=sinks, scale=scale,
                                return_lse=return_lse, out=out)

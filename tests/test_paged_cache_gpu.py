@@ -151,3 +151,111 @@ def test_example_runs():
     assert report["history_pages"] == 9 and report["pages_after_forks"] == 9 and report["pages_if_copied"] == 30
     assert report["batched_vs_separate_difference"] < 2e-2
     assert report["pages_after_compaction"] == 9 + 2 * 3 and report["pages_used_at_the_end"] == 9 + 4 * 3
+
+
+# -- batches that are out of date -------------------------------------------------------------------------------------
+
+def _rows(n, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    q, k, v = (torch.randn(n, h, 64, generator=g, device="cuda").bfloat16() for h in (4, 2, 2))
+    return q, k, v, torch.zeros(n, 3, dtype=torch.int32, device="cuda")
+
+
+def test_a_batch_of_a_closed_session_is_refused():
+    """Its pages may be another session's by now."""
+    from reelcache_b200.errors import StateError
+    from reelcache_b200.ops.rope import AxisRope
+    rope = AxisRope.wan(64)
+    cache = _cache()
+    a = cache.open()
+    old = cache.extend([(a, 20)])
+    cache.append(0, old, *_rows(20), rope)
+    cache.close(a)
+    b = cache.open()
+    batch = cache.extend([(b, 20)])
+    cache.append(0, batch, *_rows(20, 1), rope)
+    before = cache.storage.clone()
+    q = _rows(20)[0]
+    for call in (lambda: cache.append(0, old, *_rows(20, 2), rope), lambda: cache.attend(0, old, q)):
+        with pytest.raises(StateError):
+            call()
+    assert torch.equal(cache.storage, before)
+    cache.attend(0, batch, q)
+
+
+def test_a_batch_from_before_a_compaction_is_refused():
+    from reelcache_b200.errors import StateError
+    from reelcache_b200.ops.rope import AxisRope
+    rope = AxisRope.wan(64)
+    cache = _cache()
+    a, b = cache.open(), cache.open()
+    cache.extend([(a, 40)])
+    batch = cache.extend([(b, 20)])
+    cache.append(0, batch, *_rows(20), rope)
+    cache.close(a)
+    cache.compact()
+    before = cache.storage.clone()
+    for call in (lambda: cache.append(0, batch, *_rows(20, 2), rope), lambda: cache.attend(0, batch, _rows(20)[0])):
+        with pytest.raises(StateError):
+            call()
+    assert torch.equal(cache.storage, before)
+    batch = cache.again([(b, 20)])
+    cache.append(0, batch, *_rows(20, 2), rope)
+    cache.attend(0, batch, _rows(20)[0])
+
+
+@pytest.mark.parametrize("lengths,refused", [([48], True), ([45], True), ([33], True), ([32], False), ([31], False), ([17], False),
+                                             ([48, 17], True), ([17, 48], True), ([], False)])
+def test_a_batch_whose_tokens_were_forked_is_refused(lengths, refused):
+    """After a fork that took some of the batch's new tokens (16 of 48 here: a page of their own, or the copied rows of a
+    page), writing them would change the child's history or leave its copy behind."""
+    from reelcache_b200.errors import StateError
+    from reelcache_b200.ops.rope import AxisRope
+    rope = AxisRope.wan(64)
+    cache = _cache()
+    a = cache.open()
+    cache.append(0, cache.extend([(a, 32)]), *_rows(32), rope)
+    batch = cache.extend([(a, 16)])
+    children = cache.fork(a, lengths)
+    if not refused:
+        cache.append(0, batch, *_rows(16), rope)
+    else:
+        before = cache.storage.clone()
+        with pytest.raises(StateError):
+            cache.append(0, batch, *_rows(16), rope)
+        assert torch.equal(cache.storage, before)
+    cache.attend(0, batch, _rows(16)[0])  # reading is not writing
+    cache.close(*children)
+    cache.append(0, cache.again([(a, 16)]), *_rows(16), rope)
+
+
+def test_a_batch_inside_a_page_that_was_forked_before_it():
+    """Rows before the batch's tokens in the same page may have been copied, at any time."""
+    from reelcache_b200.errors import StateError
+    from reelcache_b200.ops.rope import AxisRope
+    rope = AxisRope.wan(64)
+    cache = _cache()
+    a = cache.open()
+    cache.append(0, cache.extend([(a, 20)]), *_rows(20), rope)
+    cache.fork(a, [20])
+    batch = cache.extend([(a, 6)])  # tokens 20 to 25
+    cache.append(0, batch, *_rows(6), rope)
+    cache.fork(a, [18])
+    cache.append(1, batch, *_rows(6), rope)
+    (c,) = cache.fork(a, [21])
+    with pytest.raises(StateError):
+        cache.append(0, batch, *_rows(6), rope)
+    cache.append(0, cache.again([(a, 6)]), *_rows(6), rope)  # once more, by intent
+    cache.append(0, cache.extend([(a, 3)]), *_rows(3), rope)
+    cache.append(0, cache.extend([(c, 3)]), *_rows(3), rope)
+
+
+def test_a_batch_of_another_cache_is_refused():
+    from reelcache_b200.errors import StateError
+    from reelcache_b200.ops.rope import AxisRope
+    rope = AxisRope.wan(64)
+    cache, other = _cache(), _cache()
+    batch = cache.extend([(cache.open(), 20)])
+    for call in (lambda: other.append(0, batch, *_rows(20), rope), lambda: other.attend(0, batch, _rows(20)[0])):
+        with pytest.raises(StateError):
+            call()
