@@ -293,13 +293,13 @@ class CausalWanDiT:
         tokens, sessions = cfg.chunk_tokens, len(batch.sessions)
         if any(n != tokens for n in batch.counts) or latents.shape[0] != sessions:
             raise ValueError("every session of the batch needs one chunk of new tokens and its latents")
-        if any(s.length % tokens for s in batch.sessions):
+        if any(n % tokens for n in batch.lengths):
             raise ValueError("the sessions' histories must be whole chunks")
         rows = sessions * tokens
         x = gemm.linear(torch.cat([self.patchify(one) for one in latents]).to(torch.bfloat16).contiguous(), self.patch_w,
                         self.patch_b)
         e, e0 = self.time_modulation(t)
-        positions = self.session_positions([s.length // tokens - 1 for s in batch.sessions])
+        positions = self.session_positions([n // tokens - 1 for n in batch.lengths])
         heads = (rows, cfg.heads, cfg.head_dim)
         for layer, blk in enumerate(self.blocks):
             mod = blk["modulation"] + e0

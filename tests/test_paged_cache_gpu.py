@@ -259,3 +259,23 @@ def test_a_batch_of_another_cache_is_refused():
     for call in (lambda: other.append(0, batch, *_rows(20), rope), lambda: other.attend(0, batch, _rows(20)[0])):
         with pytest.raises(StateError):
             call()
+
+
+def test_a_later_extension_leaves_a_batch_as_it_is():
+    """A batch from before its session's next extension names the same tokens, and the model rotates them at their place."""
+    from reelcache_b200.models.causal_wan import CAUSVID, CausalWanDiT
+    from reelcache_b200.paged_cache import PagedKVCache
+    cfg = CAUSVID.scaled(layers=2, dim=256, heads=2, ffn=512, text_dim=128, text_len=16, latent_height=8, latent_width=16)
+    model = CausalWanDiT(cfg, "cuda", seed=3)
+    text_kv = model.encode_text(torch.randn(cfg.text_len, cfg.text_dim, device="cuda"))
+    cache = PagedKVCache(cfg.layers, cfg.heads, cfg.head_dim, pages=40, page_size=cfg.tokens_per_frame, max_sessions=4,
+                         max_tokens=4 * cfg.chunk_tokens)
+    a = cache.open()
+    x = torch.randn(1, cfg.in_dim, cfg.frames_per_chunk, cfg.latent_height, cfg.latent_width, device="cuda")
+    model.forward_sessions(x, 500.0, cache, cache.extend([(a, cfg.chunk_tokens)]), text_kv)
+    batch = cache.extend([(a, cfg.chunk_tokens)])
+    want = model.forward_sessions(x, 500.0, cache, batch, text_kv)
+    kept = cache.storage.clone()
+    cache.extend([(a, cfg.chunk_tokens)])
+    assert torch.equal(model.forward_sessions(x, 500.0, cache, batch, text_kv), want)
+    assert torch.equal(cache.storage, kept)
