@@ -26,7 +26,8 @@ void attend_chunk(const Args& a, int head_dim, bool half, const at::Tensor& k_pa
 }  // namespace paged
 
 // out = softmax over the visible keys of scale * q k^T, times v, for the new tokens of every sequence; lse its natural
-// log-sum-exp. max_q_len bounds every sequence's new tokens; tokens past a sequence's bound are left alone.
+// log-sum-exp. max_q_len bounds every sequence's new tokens (more are reported); rows of q that no sequence names are left
+// alone.
 std::pair<at::Tensor, c10::optional<at::Tensor>> paged_attention(
     const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
     const at::Tensor& kv_lens, const at::Tensor& cu_q, int64_t max_q_len, bool causal, int64_t window, int64_t sinks,
@@ -88,6 +89,7 @@ std::pair<at::Tensor, c10::optional<at::Tensor>> paged_attention(
   a.window = static_cast<int>(window);
   a.sinks = window > 0 ? static_cast<int>(sinks) : 0;
   a.tokens = static_cast<int>(q.size(0));
+  a.max_q_len = static_cast<int>(max_q_len);
   a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
   a.tiling.page = kp.size;
   a.status = status_ptr(status);

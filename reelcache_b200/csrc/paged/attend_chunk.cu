@@ -131,11 +131,8 @@ __device__ __forceinline__ int plan_scan(int value, int* warp_sums, int* total) 
 
 // New tokens of a sequence (returned), where they begin and how many keys it has.
 __device__ __forceinline__ int sequence(const Args& a, int s, int* q_first, int* kv_len) {
-  *q_first = a.cu_q[s];
-  int q_len = min(a.cu_q[s + 1], a.tokens) - *q_first;
-  if (*q_first < 0 || q_len < 0) q_len = 0;
   *kv_len = held_keys(a, s);
-  return q_len;
+  return new_tokens(a, s, q_first);
 }
 
 // Queries of a row tile of a sequence: [first, end).
@@ -164,7 +161,10 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const __grid_c
   for (int s0 = 0; s0 < a.seqs; s0 += kPlanThreads) {
     const int s = s0 + threadIdx.x;
     int n = 0, q_first, kv_len;
-    if (s < a.seqs) n = row_tiles(sequence(a, s, &q_first, &kv_len)) * a.kv_heads;
+    if (s < a.seqs) {
+      n = row_tiles(sequence(a, s, &q_first, &kv_len)) * a.kv_heads;
+      report_rows(a, s);
+    }
     int total;
     const int before = plan_scan(n, warp_sums, &total);
     if (s < a.seqs) plan.base[s] = items + before;
@@ -527,7 +527,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     tma_prefetch_desc(&maps.v_wide);
   }
   after_earlier();
-  if (kDirect && !seg.direct(p, cta, Shape::rows)) return;  // the whole cluster
+  if (kDirect && !seg.direct(p, cta, Shape::rows)) {  // the whole cluster
+    if (threadIdx.x == 0 && seg.item.row_tile == 0) report_rows(a, seg.item.seq);
+    return;
+  }
   if (warp == 10) tmem_alloc(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
@@ -602,6 +605,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     } else if (warp == 11) {
       // ---------------- Q rows: each lane finds where a few rows lie, then four lanes fetch a row 64 bytes at a time ------
       const int quarter = lane & 3, sub = lane >> 2;
+      if (kDirect && lane == 0 && seg.item.row_tile == 0) report_rows(a, seg.item.seq);
       bool ok = true;
       for (int n = 0; ok && next(n); ++n) {
         constexpr int kPlaces = Shape::rows / 32;

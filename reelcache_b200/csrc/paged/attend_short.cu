@@ -96,9 +96,7 @@ __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 128
 struct SeqWork {
   int q_first, q_len, kv_len, tiles;
   __device__ __forceinline__ SeqWork(const Args& a, int s) {
-    q_first = a.cu_q[s];
-    q_len = min(a.cu_q[s + 1], a.tokens) - q_first;
-    if (q_first < 0 || q_len < 0) q_len = 0;
+    q_len = new_tokens(a, s, &q_first);
     kv_len = held_keys(a, s);
     tiles = 0;
     if (q_len > 0) tiles = max(1, TileRange<kShortTile>(Sight(a, kv_len, q_len), 0, q_len).count());
@@ -193,7 +191,10 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
     const int item = static_cast<int>(blockIdx.x) / p.cluster, rank = static_cast<int>(blockIdx.x) - item * p.cluster;
     s = item / a.kv_heads;
     const SeqWork w(a, s);
-    if (w.tiles == 0) return;  // no new tokens: the whole cluster
+    if (w.tiles == 0) {  // no new tokens: the whole cluster
+      if (threadIdx.x == 0) report_rows(a, s);
+      return;
+    }
     base = (s * a.kv_heads - item) * w.tiles;  // the item's tiles are places 0 ..
     begin = w.tiles * rank / p.cluster;
     end = w.tiles * (rank + 1) / p.cluster;
@@ -253,6 +254,7 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
       at += t1 - t0;
     }
     if (kCluster) {
+      if (lane == 0) report_rows(a, s);
       cluster_sync_all();
       cluster_sync_all();
     }
@@ -599,6 +601,7 @@ __global__ void __launch_bounds__(128) short_join_kernel(const __grid_constant__
   const int item = blockIdx.x / quads, s = item / a.kv_heads, head = item - s * a.kv_heads;
   let_later();
   after_earlier();
+  if (row == 0 && head == 0 && lane == 0) report_rows(a, s);
   const SeqWork w(a, s);
   const int query = row / a.group;
   if (query >= w.q_len) return;

@@ -14,6 +14,7 @@ constexpr int kPagedWord = 1;
 constexpr int kPageExhausted = 0x401;
 constexpr int kPageRefused = 0x402;
 constexpr int kPageRange = 0x403;
+constexpr int kPageRows = 0x404;
 
 namespace paged {
 

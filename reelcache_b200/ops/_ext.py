@@ -31,6 +31,8 @@ STATUS_NAMES = {
            "skips such sequences)",
     0x403: "a page number lies outside the pool, or a length outside the block table: such keys read as zeros or not at "
            "all, writes to them were dropped",
+    0x404: "a sequence has more new tokens than max_q_len, or cu_q runs backwards or past the rows of q: rows beyond have no "
+           "result",
 }
 
 

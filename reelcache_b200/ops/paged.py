@@ -5,10 +5,11 @@ Pages: ``k_pages, v_pages [pages, page_size, kv_heads, head_dim]`` of one layer 
 size is a multiple of 8 tokens). A batch of sequences is described by ``block_table [seqs, width]`` (page of each block
 of ``page_size`` tokens, -1 for none), ``kv_lens [seqs]`` (tokens held, the new ones included) and ``cu_q [seqs + 1]``
 (where each sequence's new tokens begin in ``q``), all int32 on the device (rows of the table may be strided: a slice
-``table[:, :n]`` will do): nothing is read back, every call can be captured in a graph. Sequence ``s``'s new tokens are its last ``cu_q[s + 1] - cu_q[s]`` positions.
+``table[:, :n]`` will do): nothing is read back, every call can be captured in a graph. Sequence ``s``'s new tokens are
+its last ``cu_q[s + 1] - cu_q[s]`` positions.
 
-Calls with page numbers outside the pool, or page-table calls that cannot be served, do nothing out of bounds and are
-reported by :func:`reelcache_b200.ops._ext.check_status`.
+Calls with page numbers outside the pool, lengths that do not fit their tensors or bounds, or page-table calls that cannot
+be served, do nothing out of bounds and are reported by :func:`reelcache_b200.ops._ext.check_status`.
 """
 
 from __future__ import annotations
@@ -41,7 +42,8 @@ def attention(q, k_pages, v_pages, block_table, kv_lens, cu_q, *, max_q_len: int
     bidirectional in itself). ``window`` keeps the last ``window`` of the positions it would see, and the first
     ``sinks`` of the sequence. A token that sees nothing gets zeros (and ``lse`` of minus infinity). A
     score of NaN makes its token's output and ``lse`` NaN; one of plus infinity makes ``lse`` plus infinity, the output NaN.
-    ``max_q_len`` bounds the new tokens of every sequence. ``return_lse`` adds the natural log-sum-exp ``[T, heads]``."""
+    ``max_q_len`` bounds the new tokens of every sequence (more are reported, see the module). Rows of ``q`` outside of
+    ``cu_q`` belong to no sequence: they have no result (a new output holds anything there). ``return_lse`` adds the natural log-sum-exp ``[T, heads]``."""
     if not q.is_cuda:
         raise UnsupportedError("paged attention needs CUDA tensors")
     if window is not None and window < 1:

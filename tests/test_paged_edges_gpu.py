@@ -234,3 +234,26 @@ def test_rotate_positions_of_any_size(dtype, layout):
         want, size = (torch.stack(p, dim=-1).flatten(-2) if layout == "interleaved" else torch.cat(p, dim=-1) for p in pairs)
         got, _ = rotate(q, None, positions, rope)
         assert within(got, want, rotate_bound(want, size, dtype)), float(((got.double() - want).abs()).max())
+
+
+# -- tokens that the lengths do not cover -----------------------------------------------------------------------------
+
+@pytest.mark.parametrize("new,bound", [([1, 5], 2), ([1, 20], 4), ([300, 1], 200), ([200] * 40, 150), ([700, 9], 100)])
+def test_more_new_tokens_than_the_bound_are_reported(cuda_device, new, bound):
+    """max_q_len below a sequence's new tokens leaves rows without a result: the status says so."""
+    from reelcache_b200.errors import DeviceStatusError
+    from reelcache_b200.ops import _ext, paged
+    g = _gen(61)
+    k_pages, v_pages, table, kv_lens, cu_q = paged_batch(g, new, [n + 50 for n in new], 2, 64, 16, BF16)
+    q = torch.randn(sum(new), 4, 64, generator=g, device="cuda").bfloat16()
+    call = lambda q=q, **kw: paged.attention(q, k_pages, v_pages, table, kv_lens, cu_q, **{"max_q_len": max(new), **kw})  # noqa: E731
+    want = call()
+    _ext.check_status(cuda_device)
+    assert torch.equal(call(max_q_len=10 ** 6), want)
+    _ext.check_status(cuda_device)
+    call(max_q_len=bound)
+    with pytest.raises(DeviceStatusError, match="max_q_len"):
+        _ext.check_status(cuda_device)
+    call(q=q[:-1])  # fewer rows than cu_q names
+    with pytest.raises(DeviceStatusError, match="max_q_len"):
+        _ext.check_status(cuda_device)
