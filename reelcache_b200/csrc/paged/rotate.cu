@@ -425,7 +425,8 @@ at::Tensor paged_append(const at::Tensor& q, const at::Tensor& k, const at::Tens
   a.page_k = kp.page_stride * 2;
   a.page_v = vp.page_stride * 2;
   a.status = status_ptr(status);
-  if (tokens > 0 && t.seqs > 0)
+  if (t.seqs == 0) a.k.heads = a.v.heads = 0;  // q alone: k and v belong to no sequence
+  if (tokens > 0 && a.q.heads + a.k.heads > 0)
     rotary::dispatch<true>(a, type, plan.halves, c10::cuda::getCurrentCUDAStream(q.get_device()).stream(), sm_count(q.get_device()));
   return q_out;
 }

@@ -257,3 +257,18 @@ def test_more_new_tokens_than_the_bound_are_reported(cuda_device, new, bound):
     call(q=q[:-1])  # fewer rows than cu_q names
     with pytest.raises(DeviceStatusError, match="max_q_len"):
         _ext.check_status(cuda_device)
+
+
+def test_append_without_sequences_still_rotates():
+    """Tokens of no sequence are rotated, like those past the last sequence, and written nowhere."""
+    from reelcache_b200.ops import paged
+    from reelcache_b200.ops.rope import AxisRope, rotate
+    g = _gen(62)
+    rope = AxisRope.wan(64)
+    k_pages, v_pages, table, kv_lens, cu_q = paged_batch(g, [2], [10], 2, 64, 8, BF16)
+    before = k_pages.clone(), v_pages.clone()
+    q, k = (torch.randn(3, n, 64, generator=g, device="cuda").bfloat16() for n in (4, 2))
+    positions = torch.randint(0, 900, (3, 3), generator=g, device="cuda", dtype=torch.int32)
+    out = paged.append(q, k, k, positions, rope, k_pages, v_pages, table[:0], kv_lens[:0], cu_q[:1], out=torch.full_like(q, 7.0))
+    assert torch.equal(out, rotate(q, None, positions, rope)[0])
+    assert torch.equal(k_pages, before[0]) and torch.equal(v_pages, before[1])
