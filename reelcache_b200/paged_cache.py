@@ -223,11 +223,13 @@ class PagedKVCache:
         return PagedBatch(tuple(sessions), tuple(counts), tuple(s.length for s in sessions), table, lens, self._ints(starts),
                           self, self._changes, [self._changes])
 
-    def _check_batch(self, batch: PagedBatch, *, write: bool):
-        """Refuse a batch whose pages may hold something else by now, or (``write``) whose new tokens a fork has taken:
+    def _check_batch(self, batch: PagedBatch, q, *, write: bool):
+        """Refuse fewer rows than the batch has new tokens (lengths would no longer say where they are), a batch whose pages may hold something else by now, or (``write``) whose new tokens a fork has taken:
         writing them would change the child's history, or leave what it copied behind."""
         if batch.cache is not self:
             raise StateError("the batch is another cache's")
+        if q.shape[0] < batch.tokens:
+            raise ConfigurationError(f"the batch has {batch.tokens} new tokens, q has {q.shape[0]} rows")
         if batch.checked[0] == self._changes:
             return
         self._check(batch.sessions)
@@ -256,14 +258,14 @@ class PagedKVCache:
 
     def append(self, layer: int, batch: PagedBatch, q, k, v, positions, rope: AxisRope, *, out=None):
         """Write the new tokens of one layer (``k`` rotated at ``positions``, ``v`` as it is); returns ``q`` rotated."""
-        self._check_batch(batch, write=True)
+        self._check_batch(batch, q, write=True)
         return paged.append(q, k, v, positions, rope, self.storage[layer, 0], self.storage[layer, 1], batch.table,
                             batch.kv_lens, batch.cu_q, out=out)
 
     def attend(self, layer: int, batch: PagedBatch, q, *, causal: bool = False, window: int | None = None, sinks: int = 0,
                scale: float | None = None, return_lse: bool = False, out=None):
         """Attention of the new tokens over their sessions (:func:`reelcache_b200.ops.paged.attention`)."""
-        self._check_batch(batch, write=False)
+        self._check_batch(batch, q, write=False)
         return paged.attention(q, self.storage[layer, 0], self.storage[layer, 1], batch.table, batch.kv_lens, batch.cu_q,
                                max_q_len=max(max(batch.counts), 1), causal=causal, window=window, sinks=sinks, scale=scale,
                                return_lse=return_lse, out=out)

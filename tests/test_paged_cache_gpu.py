@@ -279,3 +279,18 @@ def test_a_later_extension_leaves_a_batch_as_it_is():
     cache.extend([(a, cfg.chunk_tokens)])
     assert torch.equal(model.forward_sessions(x, 500.0, cache, batch, text_kv), want)
     assert torch.equal(cache.storage, kept)
+
+
+def test_fewer_rows_than_new_tokens_are_refused():
+    """The lengths count all new tokens, so a shorter call would put the ones it has in the wrong places."""
+    from reelcache_b200.errors import ConfigurationError
+    from reelcache_b200.ops.rope import AxisRope
+    cache = _cache()
+    batch = cache.extend([(cache.open(), 20), (cache.open(), 7)])
+    before = cache.storage.clone()
+    for call in (lambda: cache.append(0, batch, *_rows(26), AxisRope.wan(64)), lambda: cache.attend(0, batch, _rows(20)[0])):
+        with pytest.raises(ConfigurationError):
+            call()
+    assert torch.equal(cache.storage, before)
+    cache.append(0, batch, *_rows(30), AxisRope.wan(64))  # rows past the batch's belong to no session
+    cache.attend(0, batch, _rows(30)[0])
