@@ -70,11 +70,10 @@ def status_word(device) -> torch.Tensor:
 def check_status(device) -> None:
     """Raise DeviceStatusError if any kernel on ``device`` recorded a failure (synchronizes)."""
     word = status_word(device)
-    first, paged = word[:2].tolist()  # the second word is the paged-cache operators'
-    code = first or paged
-    if code:
+    codes = [code for code in word[:2].tolist() if code]  # the second word is the paged-cache operators'
+    if codes:
         word.zero_()
-        raise DeviceStatusError(f"kernel status 0x{code:x}: {STATUS_NAMES.get(code, 'unknown failure')}")
+        raise DeviceStatusError("; ".join(f"kernel status 0x{code:x}: {STATUS_NAMES.get(code, 'unknown failure')}" for code in codes))
 
 
 def require_cuda(tensor: torch.Tensor, what: str) -> None:

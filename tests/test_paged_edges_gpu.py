@@ -272,3 +272,15 @@ def test_append_without_sequences_still_rotates():
     out = paged.append(q, k, k, positions, rope, k_pages, v_pages, table[:0], kv_lens[:0], cu_q[:1], out=torch.full_like(q, 7.0))
     assert torch.equal(out, rotate(q, None, positions, rope)[0])
     assert torch.equal(k_pages, before[0]) and torch.equal(v_pages, before[1])
+
+
+# -- what is reported, and what callers can see --------------------------------------------------------------------------
+
+def test_both_status_words_are_reported(cuda_device):
+    from reelcache_b200.errors import DeviceStatusError
+    from reelcache_b200.ops import _ext
+    word = _ext.status_word(cuda_device)
+    word[0], word[1] = 0x103, 0x402
+    with pytest.raises(DeviceStatusError, match="0x103.*0x402"):
+        _ext.check_status(cuda_device)
+    _ext.check_status(cuda_device)
