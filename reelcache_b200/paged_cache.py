@@ -121,10 +121,11 @@ class PagedKVCache:
             if not s.open:
                 raise StateError(f"session in slot {s.slot} is closed")
 
-    def _take_slots(self, count: int) -> list[int]:
+    def _next_slots(self, count: int) -> list[int]:
+        """The slots that the next sessions get, last in the list of free ones first (they stay in it)."""
         if count > len(self._free_slots):
             raise CapacityError(f"{count} session slots wanted, {len(self._free_slots)} free")
-        return [self._free_slots.pop() for _ in range(count)]
+        return self._free_slots[::-1][:count]
 
     def _admit(self, pages: int):
         if pages > self.free_pages:
@@ -132,7 +133,9 @@ class PagedKVCache:
 
     def open(self) -> PagedSession:
         """A session without history."""
-        return PagedSession(self._take_slots(1)[0])
+        (slot,) = self._next_slots(1)
+        self._free_slots.pop()
+        return PagedSession(slot)
 
     def fork(self, session: PagedSession, lengths: Sequence[int] | None = None, *, count: int | None = None) -> list[PagedSession]:
         """Sessions that begin with the first ``lengths[i]`` tokens of ``session`` (``count`` times all of it): whole pages
@@ -148,7 +151,10 @@ class PagedKVCache:
         if not lengths:
             return []
         self._admit(sum(n % self.page_size > 0 for n in lengths))
-        slots = self._take_slots(len(lengths))
+        slots = self._next_slots(len(lengths))
+        # (the host's books follow the device: what raises until here has changed neither)
+        self.table.fork(self._ints([session.slot] * len(slots)), self._ints(slots), self._ints(lengths), self._planes)
+        del self._free_slots[len(self._free_slots) - len(slots):]
         self._changes += 1
         children = []
         for slot, n in zip(slots, lengths):
@@ -160,7 +166,6 @@ class PagedKVCache:
                 child.blocks.append(_Block())
                 self._held += 1
             children.append(child)
-        self.table.fork(self._ints([session.slot] * len(slots)), self._ints(slots), self._ints(lengths), self._planes)
         return children
 
     def close(self, *sessions: PagedSession):
@@ -192,14 +197,13 @@ class PagedKVCache:
                 raise CapacityError(f"a session of {s.length} tokens cannot take {n} more (at most {self.max_tokens})")
         blocks = [-(-(s.length + n) // self.page_size) - len(s.blocks) for s, n in pairs]
         self._admit(sum(blocks))
+        batch, slots = self._batch(sessions, [n for _, n in pairs], [s.length + n for s, n in pairs])
+        self.table.allocate(slots, batch.kv_lens)
         for (s, n), b in zip(pairs, blocks):
             s.length += n
             s.blocks.extend(_Block() for _ in range(b))
         self._held += sum(blocks)
-        slots = self._ints(s.slot for s in sessions)
-        lens = self._ints(s.length for s in sessions)
-        self.table.allocate(slots, lens)
-        return self._batch(sessions, [n for _, n in pairs], slots, lens)
+        return self._name_pages(batch, slots)
 
     def again(self, pairs: Sequence[tuple[PagedSession, int]]) -> PagedBatch:
         """The last tokens of sessions once more, as :meth:`extend` gave them (a further denoising step over a chunk)."""
@@ -211,17 +215,21 @@ class PagedKVCache:
         shared = [s.slot for s, n in pairs if any(b.holders > 1 for b in s.blocks[(s.length - n) // self.page_size:]) and n]
         if shared:
             raise StateError(f"the last tokens of the sessions in slots {shared} are shared with others: fork before them")
-        return self._batch(sessions, [n for _, n in pairs], self._ints(s.slot for s in sessions),
-                           self._ints(s.length for s in sessions))
+        return self._name_pages(*self._batch(sessions, [n for _, n in pairs], [s.length for s in sessions]))
 
-    def _batch(self, sessions, counts, slots, lens) -> PagedBatch:
-        width = max(max(len(s.blocks) for s in sessions), 1)
+    def _batch(self, sessions, counts, lengths) -> tuple[PagedBatch, torch.Tensor]:
+        """A batch whose rows of the block table are yet to be filled in, and its slots."""
+        width = max(-(-max(lengths) // self.page_size), 1)
         starts = [0]
         for n in counts:
             starts.append(starts[-1] + n)
-        table = self.table.block_table[:, :width].index_select(0, slots)
-        return PagedBatch(tuple(sessions), tuple(counts), tuple(s.length for s in sessions), table, lens, self._ints(starts),
-                          self, self._changes, [self._changes])
+        table = torch.empty(len(sessions), width, dtype=torch.int32, device=self.device)
+        return PagedBatch(tuple(sessions), tuple(counts), tuple(lengths), table, self._ints(lengths), self._ints(starts), self,
+                          self._changes, [self._changes]), self._ints(s.slot for s in sessions)
+
+    def _name_pages(self, batch: PagedBatch, slots: torch.Tensor) -> PagedBatch:
+        torch.index_select(self.table.block_table[:, :batch.table.shape[1]], 0, slots, out=batch.table)
+        return batch
 
     def _check_batch(self, batch: PagedBatch, q, *, write: bool):
         """Refuse fewer rows than the batch has new tokens (lengths would no longer say where they are), a batch whose pages may hold something else by now, or (``write``) whose new tokens a fork has taken:

@@ -294,3 +294,28 @@ def test_fewer_rows_than_new_tokens_are_refused():
     assert torch.equal(cache.storage, before)
     cache.append(0, batch, *_rows(30), AxisRope.wan(64))  # rows past the batch's belong to no session
     cache.attend(0, batch, _rows(30)[0])
+
+
+def test_books_stay_as_they_were_when_a_call_fails(monkeypatch):
+    """An exception on the way to the device leaves the host's counts, slots and lengths alone."""
+    from reelcache_b200.ops import paged
+    cache = _cache()
+    a = cache.open()
+    cache.extend([(a, 20)])
+    books = lambda: (cache.free_pages, list(cache._free_slots), a.length, len(a.blocks), [b.holders for b in a.blocks], a.open)  # noqa: E731
+    before, state = books(), cache.table.state.clone()
+
+    def fails(*args, **kw):
+        raise RuntimeError("no memory")
+
+    for name, call in (("allocate", lambda: cache.extend([(a, 30)])), ("fork", lambda: cache.fork(a, [20, 3])),
+                       ("release", lambda: cache.close(a))):
+        for target, attribute in ((paged.PageTable, name), (type(cache), "_ints")):
+            with monkeypatch.context() as patch:
+                patch.setattr(target, attribute, fails)
+                with pytest.raises(RuntimeError, match="no memory"):
+                    call()
+            assert books() == before and torch.equal(cache.table.state, state)
+    cache.fork(a, [20, 3])
+    cache.extend([(a, 30)])
+    cache.close(a)
