@@ -74,8 +74,9 @@ class PagedBatch:
 
 
 class PagedKVCache:
-    """``pages`` pages of ``page_size`` tokens (a multiple of 8) for ``layers`` layers of ``kv_heads`` heads of
-    ``head_dim`` channels; at most ``max_sessions`` open sessions of at most ``max_tokens`` tokens.
+    """``pages`` pages (below 2^20) of ``page_size`` tokens (a multiple of 8, at most 65536) for ``layers`` layers of
+    ``kv_heads`` heads of ``head_dim`` channels; at most ``max_sessions`` open sessions (below 2^20) of at most ``max_tokens``
+    tokens.
 
     ``storage`` is ``[layers, 2, pages, page_size, kv_heads, head_dim]`` (K, V). A page is ``page_size`` consecutive token
     rows of one layer and target, the layout that the restore kernels write, so a restored chunk can go straight into
@@ -92,8 +93,10 @@ class PagedKVCache:
                 raise ConfigurationError(f"PagedKVCache: {name} must be a positive integer, got {value!r}")
         if head_dim not in (64, 128) or dtype not in (torch.bfloat16, torch.float16):
             raise ConfigurationError(f"PagedKVCache: head_dim is 64 or 128 and the type bf16 or fp16, got {head_dim} {dtype}")
-        if type(page_size) is not int or page_size < 8 or page_size % 8:
-            raise ConfigurationError(f"PagedKVCache: page_size must be a multiple of 8 tokens, got {page_size!r}")
+        if type(page_size) is not int or not 8 <= page_size <= 65536 or page_size % 8:
+            raise ConfigurationError(f"PagedKVCache: page_size must be a multiple of 8 tokens, at most 65536, got {page_size!r}")
+        if max(pages, max_sessions) >= 1 << 20:  # what the page table's prefix sums hold
+            raise ConfigurationError(f"PagedKVCache: pages and max_sessions must be below 2^20, got {pages} and {max_sessions}")
         self.page_size, self.pages, self.max_tokens = page_size, pages, max_tokens
         self.storage = torch.zeros(layers, 2, pages, page_size, kv_heads, head_dim, dtype=dtype, device=device)
         self.table = paged.PageTable.empty(pages, max_sessions, -(-max_tokens // page_size), page_size, device)

@@ -319,3 +319,10 @@ def test_books_stay_as_they_were_when_a_call_fails(monkeypatch):
     cache.fork(a, [20, 3])
     cache.extend([(a, 30)])
     cache.close(a)
+
+
+def test_sizes_that_the_page_table_cannot_hold_are_refused_at_once():
+    from reelcache_b200.errors import ConfigurationError
+    for wrong in (dict(page_size=65536 + 8, max_tokens=65536 + 8, pages=1), dict(pages=1 << 20, page_size=8), dict(max_sessions=1 << 20, max_tokens=8)):
+        with pytest.raises(ConfigurationError):
+            _cache(**wrong)
