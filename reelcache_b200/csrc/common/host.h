@@ -100,6 +100,11 @@ inline void check_cuda_tensor(const at::Tensor& t, const char* name) {
   RC_CHECK(t.is_cuda(), std::string(name) + " must be a CUDA tensor");
 }
 
+// A tensor that a kernel has written in place: autograd must see that what it kept of it is gone.
+inline void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // A dual tensor's tangent would be dropped by a kernel that computes on its values alone.
 inline void refuse_tangents(std::initializer_list<const at::Tensor*> tensors, const char* what) {
   if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;

@@ -99,6 +99,7 @@ std::pair<at::Tensor, c10::optional<at::Tensor>> paged_attention(
   const int most = static_cast<int>(std::min<int64_t>(max_q_len, a.tokens));
   const auto attend = static_cast<int64_t>(most) * a.group <= paged::kShortRows ? paged::attend_short : paged::attend_chunk;
   attend(a, static_cast<int>(q.size(2)), type == at::kHalf, k_pages, v_pages, most, q, stream, device);
+  if (out_given.has_value()) written(out);
   return {out, lse};
 }
 

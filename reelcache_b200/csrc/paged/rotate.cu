@@ -428,6 +428,11 @@ at::Tensor paged_append(const at::Tensor& q, const at::Tensor& k, const at::Tens
   if (t.seqs == 0) a.k.heads = a.v.heads = 0;  // q alone: k and v belong to no sequence
   if (tokens > 0 && a.q.heads + a.k.heads > 0)
     rotary::dispatch<true>(a, type, plan.halves, c10::cuda::getCurrentCUDAStream(q.get_device()).stream(), sm_count(q.get_device()));
+  if (out.has_value()) written(*out);
+  if (t.seqs > 0) {
+    written(k_pages);
+    written(v_pages);
+  }
   return q_out;
 }
 

@@ -450,6 +450,7 @@ void pages_allocate(at::Tensor& state, int64_t pages, int64_t seqs_held, int64_t
   paged::launch(pagetable::allocate_kernel, dim3(1), pagetable::kPlanThreads, 0, 0, stream, s, ids, to, static_cast<int>(n), list,
                                                                        list + s.pages, list + s.pages + n + 1,
                                                                        status_ptr(status));
+  written(state);
 }
 
 void pages_fork(at::Tensor& state, int64_t pages, int64_t seqs_held, int64_t page_size, const at::Tensor& parents,
@@ -472,6 +473,8 @@ void pages_fork(at::Tensor& state, int64_t pages, int64_t seqs_held, int64_t pag
                                                                         list + s.pages, plan, status_ptr(status));
   paged::launch(pagetable::fork_kernel, dim3(pagetable::move_grid(state.get_device())), pagetable::kMoveThreads, 0, 0, stream,
       s, st, from, to, len, static_cast<int>(n), plan, status_ptr(status));
+  written(state);
+  written(storage);
 }
 
 void pages_release(at::Tensor& state, int64_t pages, int64_t seqs_held, int64_t page_size, const at::Tensor& seqs,
@@ -485,6 +488,7 @@ void pages_release(at::Tensor& state, int64_t pages, int64_t seqs_held, int64_t 
   const int64_t blocks = (n * s.width + pagetable::kMoveThreads - 1) / pagetable::kMoveThreads;
   const int grid = static_cast<int>(std::min<int64_t>(blocks, pagetable::move_grid(state.get_device())));
   paged::launch(pagetable::release_kernel, dim3(grid), pagetable::kMoveThreads, 0, 0, stream, s, ids, static_cast<int>(n), status_ptr(status));
+  written(state);
 }
 
 // Returns an int32 tensor of one entry: the pages in use, which after the call are pages 0 .. in_use.
@@ -502,6 +506,8 @@ at::Tensor pages_compact(at::Tensor& state, int64_t pages, int64_t seqs_held, in
   paged::launch(pagetable::compact_plan_kernel, dim3(1), pagetable::kPlanThreads, 0, 0, stream, s, place, plan, in_use.data_ptr<int>());
   paged::launch(pagetable::compact_kernel, dim3(pagetable::move_grid(state.get_device())), pagetable::kMoveThreads, 0, 0, stream,
       s, st, place, in_use.data_ptr<int>(), plan, status_ptr(status));
+  written(state);
+  written(storage);
   return in_use;
 }
 
@@ -520,6 +526,7 @@ void pages_copy(at::Tensor& storage, const at::Tensor& source, const at::Tensor&
   cudaStream_t stream = c10::cuda::getCurrentCUDAStream(storage.get_device()).stream();
   paged::launch(pagetable::copy_kernel, dim3(pagetable::move_grid(storage.get_device())), pagetable::kMoveThreads, 0, 0, stream,
       st, static_cast<int>(storage.size(1)), from, to, part, static_cast<int>(n), status_ptr(status));
+  written(storage);
 }
 
 }  // namespace rc

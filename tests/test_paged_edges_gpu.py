@@ -284,3 +284,35 @@ def test_both_status_words_are_reported(cuda_device):
     with pytest.raises(DeviceStatusError, match="0x103.*0x402"):
         _ext.check_status(cuda_device)
     _ext.check_status(cuda_device)
+
+
+def test_written_tensors_carry_a_new_version():
+    """What autograd has kept of a tensor must be seen to have changed."""
+    from reelcache_b200.ops import paged
+    from reelcache_b200.ops.rope import AxisRope
+    g = _gen(71)
+    rope = AxisRope.wan(64)
+    k_pages, v_pages, table, kv_lens, cu_q = paged_batch(g, [3], [20], 2, 64, 16, BF16)
+    (positions,) = _ints([[1, 2, 3]] * 3)
+    q, k = (torch.randn(3, n, 64, generator=g, device="cuda").bfloat16() for n in (4, 2))
+    weight = torch.ones(64, device="cuda", dtype=BF16, requires_grad=True)
+    loss = (k_pages * weight).sum()
+    out = torch.empty_like(q)
+    versions = [t._version for t in (k_pages, v_pages, out)]
+    paged.append(q, k, k, positions, rope, k_pages, v_pages, table, kv_lens, cu_q, out=out)
+    assert all(t._version > n for t, n in zip((k_pages, v_pages, out), versions))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    version = out._version
+    paged.attention(q, k_pages, v_pages, table, kv_lens, cu_q, max_q_len=3, out=out)
+    assert out._version > version
+    storage = torch.randn(2, 6, 16, 8, device="cuda")
+    held = paged.PageTable.empty(6, 3, 2, 16, "cuda")
+    for call in (lambda: paged.copy_pages(storage, *_ints([1], [2])), lambda: held.allocate(*_ints([0], [20])),
+                 lambda: held.fork(*_ints([0], [1], [20]), storage), lambda: held.release(*_ints([0])), lambda: held.compact(storage)):
+        before = storage._version, held.state._version
+        call()
+        assert (storage._version, held.state._version) != before
+    with torch.inference_mode():
+        kept = k_pages.clone(), v_pages.clone()
+        paged.append(q, k, k, positions, rope, *kept, table, kv_lens, cu_q)
