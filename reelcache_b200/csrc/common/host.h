@@ -4,6 +4,7 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/AutogradState.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -98,6 +99,13 @@ inline int sm_count(int device) {
 
 inline void check_cuda_tensor(const at::Tensor& t, const char* name) {
   RC_CHECK(t.is_cuda(), std::string(name) + " must be a CUDA tensor");
+}
+
+// Tensors that kernels without a gradient read or write must not want one (outside of grad mode they may).
+inline void refuse_gradients(std::initializer_list<const at::Tensor*> tensors, const char* what) {
+  if (!c10::GradMode::is_enabled()) return;
+  for (const at::Tensor* t : tensors)
+    RC_CHECK(!t->defined() || !t->requires_grad(), std::string(what) + " has no gradient: call it without grad");
 }
 
 // A tensor that a kernel has written in place: autograd must see that what it kept of it is gone.

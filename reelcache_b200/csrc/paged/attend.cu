@@ -3,7 +3,6 @@
 // Few query rows (new tokens x heads of a group) cannot fill the 128-row products of tcgen05, and reading K and V bounds
 // them anyway: they take the streaming kernel of attend_short.cu. More rows take attend_chunk.cu.
 #include <ATen/ATen.h>
-#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -34,8 +33,8 @@ std::pair<at::Tensor, c10::optional<at::Tensor>> paged_attention(
     c10::optional<double> scale_given, bool want_lse, const c10::optional<at::Tensor>& out_given,
     const c10::optional<at::Tensor>& status) {
   check_cuda_tensor(q, "q");
-  RC_CHECK(!c10::GradMode::is_enabled() || !(q.requires_grad() || k_pages.requires_grad() || v_pages.requires_grad()),
-           "attention over pages has no gradient: call it without grad");
+  refuse_gradients({&q, &k_pages, &v_pages}, "attention over pages");
+  if (out_given.has_value()) refuse_gradients({&*out_given}, "attention over pages");
   refuse_tangents({&q, &k_pages, &v_pages}, "attention over pages");
   const at::ScalarType type = q.scalar_type();
   RC_CHECK(type == at::kBFloat16 || type == at::kHalf, "paged attention takes bf16 or fp16");

@@ -23,7 +23,6 @@
 // x 36 heads into pages 41.7 us, 6.2 TB/s (51 us with one head group of q, k and v mixed per thread, 81 us with two heads
 // a thread).
 #include <ATen/ATen.h>
-#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda_bf16.h>
@@ -384,8 +383,8 @@ at::Tensor paged_append(const at::Tensor& q, const at::Tensor& k, const at::Tens
                         const at::Tensor& kv_lens, const at::Tensor& cu_q, const c10::optional<at::Tensor>& out,
                         const c10::optional<at::Tensor>& status) {
   check_cuda_tensor(q, "q");
-  RC_CHECK(!c10::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || v.requires_grad() || positions.requires_grad()),
-           "append has no gradient: call it without grad");
+  refuse_gradients({&q, &k, &v, &positions, &k_pages, &v_pages}, "append");
+  if (out.has_value()) refuse_gradients({&*out}, "append");
   refuse_tangents({&q, &k, &v, &positions, &k_pages, &v_pages}, "append");
   const at::ScalarType type = q.scalar_type();
   RC_CHECK(type == at::kBFloat16 || type == at::kHalf, "a paged cache holds bf16 or fp16");

@@ -410,6 +410,7 @@ const int* check_list(const at::Tensor& t, const at::Device& device, int64_t n, 
 
 // storage [planes, pages, page_size, ...]: pages whole and contiguous, planes and pages anywhere.
 Storage check_storage(at::Tensor& t, int64_t pages, int64_t page_size, const at::Device& device) {
+  refuse_gradients({&t}, "moving pages");
   RC_CHECK(t.device() == device && t.dim() >= 3 && t.size(1) == pages && t.size(2) == page_size,
            "storage must be [planes, pages, page_size, ...] on the page table's device");
   const int64_t size = t.element_size();

@@ -316,3 +316,24 @@ def test_written_tensors_carry_a_new_version():
     with torch.inference_mode():
         kept = k_pages.clone(), v_pages.clone()
         paged.append(q, k, k, positions, rope, *kept, table, kv_lens, cu_q)
+
+
+def test_pages_that_want_a_gradient_are_refused():
+    from reelcache_b200.ops import paged
+    from reelcache_b200.ops.rope import AxisRope
+    g = _gen(72)
+    k_pages, v_pages, table, kv_lens, cu_q = paged_batch(g, [3], [20], 2, 64, 16, BF16)
+    (positions,) = _ints([[1, 2, 3]] * 3)
+    q, k = (torch.randn(3, n, 64, generator=g, device="cuda").bfloat16() for n in (4, 2))
+    call = lambda kp=k_pages, vp=v_pages, **kw: paged.append(q, k, k, positions, AxisRope.wan(64), kp, vp, table, kv_lens, cu_q, **kw)  # noqa: E731
+    for wrong in (dict(kp=k_pages.clone().requires_grad_()), dict(vp=v_pages.clone().requires_grad_()),
+                  dict(out=torch.empty_like(q).requires_grad_())):
+        with pytest.raises(RuntimeError, match="gradient"):
+            call(**wrong)
+        with torch.no_grad():
+            call(**wrong)
+    with pytest.raises(RuntimeError, match="gradient"):
+        paged.attention(q, k_pages, v_pages, table, kv_lens, cu_q, max_q_len=3, out=torch.empty_like(q).requires_grad_())
+    storage = torch.randn(2, 6, 16, 8, device="cuda", requires_grad=True)
+    with pytest.raises(RuntimeError, match="gradient"):
+        paged.copy_pages(storage, *_ints([1], [2]))
