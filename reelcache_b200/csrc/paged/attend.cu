@@ -3,6 +3,7 @@
 // Few query rows (new tokens x heads of a group) cannot fill the 128-row products of tcgen05, and reading K and V bounds
 // them anyway: they take the streaming kernel of attend_short.cu. More rows take attend_chunk.cu.
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -44,6 +45,8 @@ std::pair<at::Tensor, c10::optional<at::Tensor>> paged_attention(
   const double scale = scale_given.has_value() ? *scale_given : 1.0 / std::sqrt(static_cast<double>(q.size(2)));
   const at::Tensor out = out_given.has_value() ? *out_given : at::empty(q.sizes(), q.options());
   RC_CHECK(out.sizes() == q.sizes() && out.scalar_type() == type && out.device() == q.device(), "out must match q");
+  at::assert_no_internal_overlap(out);
+  at::assert_no_partial_overlap(out, q);
   const at::Tensor* rows[2] = {&q, &out};
   for (const at::Tensor* t : rows)
     RC_CHECK(t->numel() == 0 || (t->stride(2) == 1 && t->stride(0) % 8 == 0 && t->stride(1) % 8 == 0 &&

@@ -23,6 +23,7 @@
 // x 36 heads into pages 41.7 us, 6.2 TB/s (51 us with one head group of q, k and v mixed per thread, 81 us with two heads
 // a thread).
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda_bf16.h>
@@ -399,6 +400,11 @@ at::Tensor paged_append(const at::Tensor& q, const at::Tensor& k, const at::Tens
     RC_CHECK(t->scalar_type() == type && t->device() == q.device(), "q, k, v and the pages must agree on type and device");
   for (int i = 0; i < 4; ++i)
     RC_CHECK(rotary_rows_ok(*all[i]), "rows must have unit inner stride and 16-byte aligned strides and base");
+  // what threads of one launch write must not lie on top of itself (q may be turned in place)
+  for (const at::Tensor* t : {static_cast<const at::Tensor*>(&q_out), static_cast<const at::Tensor*>(&k_pages), static_cast<const at::Tensor*>(&v_pages)})
+    at::assert_no_internal_overlap(*t);
+  RC_CHECK(k_pages.data_ptr() != v_pages.data_ptr(), "k_pages and v_pages must be different pages");
+  at::assert_no_partial_overlap(q_out, q);
   const paged::Table t = paged::check_table(table, kv_lens, cu_q, q.device());
   const paged::Pages kp = paged::check_pages(k_pages, k.size(1), k.size(2), "k_pages");
   const paged::Pages vp = paged::check_pages(v_pages, k.size(1), k.size(2), "v_pages");

@@ -337,3 +337,26 @@ def test_pages_that_want_a_gradient_are_refused():
     storage = torch.randn(2, 6, 16, 8, device="cuda", requires_grad=True)
     with pytest.raises(RuntimeError, match="gradient"):
         paged.copy_pages(storage, *_ints([1], [2]))
+
+
+def test_outputs_that_overlap_themselves_are_refused():
+    from reelcache_b200.ops import paged
+    from reelcache_b200.ops.rope import AxisRope
+    g = _gen(73)
+    k_pages, v_pages, table, kv_lens, cu_q = paged_batch(g, [3], [20], 2, 64, 16, BF16)
+    (positions,) = _ints([[1, 2, 3]] * 3)
+    q, k = (torch.randn(3, n, 64, generator=g, device="cuda").bfloat16() for n in (4, 2))
+    append = lambda kp=k_pages, vp=v_pages, **kw: paged.append(q, k, k, positions, AxisRope.wan(64), kp, vp, table, kv_lens, cu_q, **kw)  # noqa: E731
+    thin = torch.empty(1, 4, 64, device="cuda", dtype=BF16).expand(3, 4, 64)
+    for call in (lambda: append(kp=k_pages[:1].expand_as(k_pages)), lambda: append(vp=v_pages[:, :, :1].expand_as(v_pages)),
+                 lambda: append(out=thin), lambda: append(vp=k_pages),
+                 lambda: paged.attention(q, k_pages, v_pages, table, kv_lens, cu_q, max_q_len=3, out=thin)):
+        with pytest.raises(RuntimeError):
+            call()
+    # (pages that are only read may be expanded)
+    paged.attention(q, k_pages[:, :, :1].expand_as(k_pages), v_pages, table, kv_lens, cu_q, max_q_len=3)
+    both = torch.randn(5, 4, 64, generator=g, device="cuda").bfloat16()
+    with pytest.raises(RuntimeError):  # rows that are still to be read
+        paged.append(both[:3], k, k, positions, AxisRope.wan(64), k_pages, v_pages, table, kv_lens, cu_q, out=both[1:4])
+    want = paged.attention(both[:3], k_pages, v_pages, table, kv_lens, cu_q, max_q_len=3)
+    assert torch.equal(paged.attention(both[:3], k_pages, v_pages, table, kv_lens, cu_q, max_q_len=3, out=both[:3]), want)
