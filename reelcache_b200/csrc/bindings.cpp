@@ -29,7 +29,8 @@ void ln_modulate(const at::Tensor& x, at::Tensor& y, const c10::optional<at::Ten
                  const c10::optional<at::Tensor>& bias, double eps);
 void qkv_norm_rope(const at::Tensor& qkv, const at::Tensor& wq, const at::Tensor& wk, const at::Tensor& cos_tok,
                    const at::Tensor& sin_tok, at::Tensor& q_out, const c10::optional<at::Tensor>& k_pre,
-                   at::Tensor& k_cache, at::Tensor& v_cache, int64_t head_dim, double eps);
+                   at::Tensor& k_cache, at::Tensor& v_cache, const c10::optional<at::Tensor>& kv_rows, int64_t head_dim,
+                   double eps);
 void rms_norm(const at::Tensor& x, at::Tensor& y, const at::Tensor& w, double eps);
 void head_norm_rope(const at::Tensor& x, at::Tensor& y, const c10::optional<at::Tensor>& w,
                     const c10::optional<at::Tensor>& cos_tok, const c10::optional<at::Tensor>& sin_tok, double eps);
@@ -119,7 +120,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("bias") = py::none(), py::arg("eps") = 1e-6);
   m.def("qkv_norm_rope", &rc::qkv_norm_rope, "q/k RMSNorm + RoPE from fused qkv into q and KV-cache slots",
         py::arg("qkv"), py::arg("wq"), py::arg("wk"), py::arg("cos_tok"), py::arg("sin_tok"), py::arg("q_out"),
-        py::arg("k_pre"), py::arg("k_cache"), py::arg("v_cache"), py::arg("head_dim"), py::arg("eps") = 1e-6);
+        py::arg("k_pre"), py::arg("k_cache"), py::arg("v_cache"), py::arg("kv_rows"), py::arg("head_dim"),
+        py::arg("eps") = 1e-6);
   m.def("head_norm_rope", &rc::head_norm_rope, "per-head RMSNorm and / or interleaved RoPE of [T, H, D]",
         py::arg("x"), py::arg("y"), py::arg("w"), py::arg("cos_tok"), py::arg("sin_tok"), py::arg("eps"));
   m.def("rms_norm", &rc::rms_norm, "y = RMSNorm(x) * w", py::arg("x"), py::arg("y"), py::arg("w"),

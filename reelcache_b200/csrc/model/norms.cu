@@ -3,7 +3,8 @@
 //   ln_modulate      y = LayerNorm(x) * (1 + scale) + shift          (AdaLN; optional affine weight/bias)
 //   qkv_norm_rope    from the fused QKV projection [T, 3C]: q = RoPE(RMSNorm(q) * wq),
 //                    k_pre = RMSNorm(k) * wk (normalized pre-RoPE K, the archival capture),
-//                    k = RoPE(k_pre) and v written straight into the KV-cache slots
+//                    k = RoPE(k_pre) and v written straight into the KV-cache slots (or, given their rows, anywhere in a
+//                    paged cache)
 //   rms_norm         y = RMSNorm(x) * w over the full row (cross-attention q / context k)
 //
 // RMSNorm spans all heads (Wan's qk-norm over the model width). RoPE rotates interleaved pairs with
@@ -176,7 +177,8 @@ __device__ __forceinline__ void rope_row(float* v, int C, int lane, int head_dim
   }
 }
 
-// One warp per token: qkv row [3C] -> q_out [C], k_pre [C], k_cache [C], v_cache [C]
+// One warp per token: qkv row [3C] -> q_out [C], k_pre [C], k_cache [C], v_cache [C]. With kv_rows, k and v of a token go
+// to row kv_rows[token] of cache_rows (nowhere if it is none of them).
 template <int VEC>
 __global__ void qkv_norm_rope_kernel(const __nv_bfloat16* __restrict__ qkv, int64_t ld_qkv, int rows, int C,
                                      int head_dim, const float* __restrict__ wq, const float* __restrict__ wk,
@@ -184,7 +186,8 @@ __global__ void qkv_norm_rope_kernel(const __nv_bfloat16* __restrict__ qkv, int6
                                      __nv_bfloat16* __restrict__ q_out, int64_t ld_q,
                                      __nv_bfloat16* __restrict__ k_pre, int64_t ld_kp,
                                      __nv_bfloat16* __restrict__ k_cache, int64_t ld_k,
-                                     __nv_bfloat16* __restrict__ v_cache, int64_t ld_v, float eps) {
+                                     __nv_bfloat16* __restrict__ v_cache, int64_t ld_v,
+                                     const int64_t* __restrict__ kv_rows, int64_t cache_rows, float eps) {
   const int row = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (row >= rows) return;
@@ -201,11 +204,13 @@ __global__ void qkv_norm_rope_kernel(const __nv_bfloat16* __restrict__ qkv, int6
   load_row<VEC>(src + C, C, lane, v);
   rms_row<VEC>(v, C, lane, wk, eps);
   if (k_pre != nullptr) store_row<VEC>(k_pre + static_cast<int64_t>(row) * ld_kp, C, lane, v);
+  const int64_t at = kv_rows != nullptr ? kv_rows[row] : row;
+  if (at < 0 || at >= cache_rows) return;
   rope_row<VEC>(v, C, lane, head_dim, cs, sn);
-  store_row<VEC>(k_cache + static_cast<int64_t>(row) * ld_k, C, lane, v);
+  store_row<VEC>(k_cache + at * ld_k, C, lane, v);
   // v
   load_row<VEC>(src + 2 * C, C, lane, v);
-  store_row<VEC>(v_cache + static_cast<int64_t>(row) * ld_v, C, lane, v);
+  store_row<VEC>(v_cache + at * ld_v, C, lane, v);
 }
 
 template <int VEC>
@@ -322,7 +327,8 @@ void ln_modulate(const at::Tensor& x, at::Tensor& y, const c10::optional<at::Ten
 
 void qkv_norm_rope(const at::Tensor& qkv, const at::Tensor& wq, const at::Tensor& wk, const at::Tensor& cos_tok,
                    const at::Tensor& sin_tok, at::Tensor& q_out, const c10::optional<at::Tensor>& k_pre,
-                   at::Tensor& k_cache, at::Tensor& v_cache, int64_t head_dim, double eps) {
+                   at::Tensor& k_cache, at::Tensor& v_cache, const c10::optional<at::Tensor>& kv_rows, int64_t head_dim,
+                   double eps) {
   check_rows(qkv, "qkv");
   check_rows(q_out, "q_out");
   check_rows(k_cache, "k_cache");
@@ -330,8 +336,12 @@ void qkv_norm_rope(const at::Tensor& qkv, const at::Tensor& wq, const at::Tensor
   const int rows = static_cast<int>(qkv.size(0));
   const int C = static_cast<int>(qkv.size(1) / 3);
   RC_CHECK(qkv.size(1) == 3 * C && q_out.size(1) == C && k_cache.size(1) == C && v_cache.size(1) == C &&
-               q_out.size(0) == rows && k_cache.size(0) == rows && v_cache.size(0) == rows,
-           "qkv is [T, 3C]; outputs are [T, C]");
+               q_out.size(0) == rows && k_cache.size(0) == v_cache.size(0) && (kv_rows.has_value() || k_cache.size(0) == rows),
+           "qkv is [T, 3C]; outputs are [T, C] (with kv_rows, the cache [rows, C])");
+  if (kv_rows.has_value())
+    RC_CHECK(kv_rows->device() == qkv.device() && kv_rows->scalar_type() == at::kLong && kv_rows->is_contiguous() &&
+                 kv_rows->dim() == 1 && kv_rows->size(0) == rows,
+             "kv_rows must be a contiguous int64 [T] vector on the same device");
   RC_CHECK(cos_tok.is_cuda() && cos_tok.scalar_type() == at::kFloat && cos_tok.is_contiguous() &&
                cos_tok.size(0) == rows && cos_tok.size(1) * 2 == head_dim && sin_tok.sizes() == cos_tok.sizes() &&
                sin_tok.is_contiguous() && reinterpret_cast<uintptr_t>(cos_tok.data_ptr()) % 16 == 0 &&
@@ -352,7 +362,12 @@ void qkv_norm_rope(const at::Tensor& qkv, const at::Tensor& wq, const at::Tensor
                   cos_tok.data_ptr<float>(), sin_tok.data_ptr<float>(),
                   reinterpret_cast<__nv_bfloat16*>(q_out.data_ptr()), q_out.stride(0), kp, ld_kp,
                   reinterpret_cast<__nv_bfloat16*>(k_cache.data_ptr()), k_cache.stride(0),
-                  reinterpret_cast<__nv_bfloat16*>(v_cache.data_ptr()), v_cache.stride(0), static_cast<float>(eps));
+                  reinterpret_cast<__nv_bfloat16*>(v_cache.data_ptr()), v_cache.stride(0),
+                  kv_rows.has_value() ? kv_rows->data_ptr<int64_t>() : nullptr, k_cache.size(0), static_cast<float>(eps));
+  if (kv_rows.has_value()) {
+    written(k_cache);
+    written(v_cache);
+  }
 }
 
 void rms_norm(const at::Tensor& x, at::Tensor& y, const at::Tensor& w, double eps) {

@@ -172,6 +172,7 @@ class CausalWanDiT:
         self.rope = RopeTable.wan(cfg.head_dim, 1024, theta=cfg.rope_theta, device=self.device)
         assert self.rope.pairs == pairs
         self._axis_rope = None
+        self._session_rope = self.rope  # longer where a session is
 
     # -- conditioning ------------------------------------------------------------------------------------------
 
@@ -269,7 +270,8 @@ class CausalWanDiT:
 
     @property
     def axis_rope(self) -> AxisRope:
-        """The rotation of :attr:`rope` from per-token positions (the paged cache's form)."""
+        """The rotation of :attr:`rope` from per-token positions, for rows that are written with the paged cache's
+        ``append``."""
         if self._axis_rope is None:
             self._axis_rope = AxisRope.wan(self.cfg.head_dim, theta=self.cfg.rope_theta)
         return self._axis_rope
@@ -283,11 +285,22 @@ class CausalWanDiT:
         first = torch.tensor([[cfg.frames_per_chunk * c, 0, 0] for c in chunk_indices], dtype=torch.int32)
         return (grid + first.to(self.device)[:, None]).flatten(0, 1)
 
+    def session_rope(self, chunk_indices):
+        """Per-token cos/sin ``[len(chunk_indices) * chunk_tokens, pairs]`` of some chunks, the values of :meth:`token_rope`."""
+        frames = self.cfg.frames_per_chunk * (max(chunk_indices) + 1)
+        if frames > self._session_rope.rows:
+            self._session_rope = RopeTable.wan(self.cfg.head_dim, 2 * frames, theta=self.cfg.rope_theta, device=self.device)
+        positions = self.session_positions(chunk_indices).long()
+        ends = [sum(self._session_rope.sections[:axis + 1]) for axis in range(3)]
+        return tuple(torch.cat([table[positions[:, axis], end - pairs:end] for axis, (end, pairs) in
+                                enumerate(zip(ends, self._session_rope.sections))], dim=1)
+                     for table in self._session_rope.kernel_tables(self.device))
+
     def forward_sessions(self, latents: torch.Tensor, t: float, cache, batch, text_kv, *, capture=None) -> torch.Tensor:
         """One forward of the newest chunk of several sessions of a :class:`~reelcache_b200.paged_cache.PagedKVCache`
         (``batch`` from its ``extend`` or ``again``, a chunk for each): ``latents[sessions, in_dim, F, H, W]`` at timestep
         ``t``, the weights read once for all of them, histories shared page by page between forks. Same block math as
-        :meth:`forward_chunk`. ``capture(layer, k_pre, v)`` receives the rows of all sessions, one after the other.
+        :meth:`forward_chunk`, by the same kernels but for the attention over pages. ``capture(layer, k_pre, v)`` receives the rows of all sessions, one after the other.
         Returns the flow predictions ``[sessions, in_dim, F, H, W]`` (FP32)."""
         cfg = self.cfg
         tokens, sessions = cfg.chunk_tokens, len(batch.sessions)
@@ -299,21 +312,20 @@ class CausalWanDiT:
         x = gemm.linear(torch.cat([self.patchify(one) for one in latents]).to(torch.bfloat16).contiguous(), self.patch_w,
                         self.patch_b)
         e, e0 = self.time_modulation(t)
-        positions = self.session_positions([n // tokens - 1 for n in batch.lengths])
+        cos_tok, sin_tok = self.session_rope([n // tokens - 1 for n in batch.lengths])
+        kv_rows = cache.new_rows(batch)
         heads = (rows, cfg.heads, cfg.head_dim)
+        q = torch.empty((rows, cfg.dim), dtype=torch.bfloat16, device=self.device)
         for layer, blk in enumerate(self.blocks):
             mod = blk["modulation"] + e0
             y = norms.ln_modulate(x, shift=mod[0], scale=mod[1], eps=cfg.eps)
             qkv = gemm.linear(y, blk["qkv_w"], blk["qkv_b"])
-            q = torch.empty((rows, cfg.dim), dtype=torch.bfloat16, device=self.device)
-            k = torch.empty_like(q)
-            norms.rms_norm(qkv[:, :cfg.dim], blk["norm_q"], eps=cfg.eps, out=q)
-            norms.rms_norm(qkv[:, cfg.dim:2 * cfg.dim], blk["norm_k"], eps=cfg.eps, out=k)
-            v = qkv[:, 2 * cfg.dim:]
+            k_pre = torch.empty_like(q) if capture is not None else None
+            norms.qkv_norm_rope(qkv, blk["norm_q"], blk["norm_k"], cos_tok, sin_tok, q, cache.token_rows(layer, "K"),
+                                cache.token_rows(layer, "V"), head_dim=cfg.head_dim, k_pre=k_pre, kv_rows=kv_rows, eps=cfg.eps)
             if capture is not None:
-                capture(layer, k, v)
-            q = cache.append(layer, batch, q.view(heads), k.view(heads), v.unflatten(1, heads[1:]), positions, self.axis_rope)
-            o = cache.attend(layer, batch, q)
+                capture(layer, k_pre, qkv[:, 2 * cfg.dim:])
+            o = cache.attend(layer, batch, q.view(heads))
             gemm.linear_gated_residual(o.view(rows, cfg.dim), blk["o_w"], blk["o_b"], mod[2].contiguous(), x)
             y = norms.ln_modulate(x, weight=blk["norm3_w"], bias=blk["norm3_b"], eps=cfg.eps)
             cq = norms.rms_norm(gemm.linear(y, blk["cq_w"], blk["cq_b"]), blk["cnorm_q"], eps=cfg.eps)

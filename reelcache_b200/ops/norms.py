@@ -16,10 +16,13 @@ def ln_modulate(x, *, shift=None, scale=None, weight=None, bias=None, eps=1e-6, 
     return out.reshape(x.shape)
 
 
-def qkv_norm_rope(qkv, wq, wk, cos_tok, sin_tok, q_out, k_cache, v_cache, *, head_dim, k_pre=None, eps=1e-6):
+def qkv_norm_rope(qkv, wq, wk, cos_tok, sin_tok, q_out, k_cache, v_cache, *, head_dim, k_pre=None, kv_rows=None,
+                  eps=1e-6):
     """From fused ``qkv[T, 3C]``: ``q_out = RoPE(RMSNorm(q) wq)``; ``k_pre = RMSNorm(k) wk`` (optional
-    capture); ``k_cache = RoPE(k_pre)``; ``v_cache = v`` (all ``[T, C]`` row views)."""
-    ext().qkv_norm_rope(qkv, wq, wk, cos_tok, sin_tok, q_out, k_pre, k_cache, v_cache, int(head_dim), float(eps))
+    capture); ``k_cache = RoPE(k_pre)``; ``v_cache = v`` (all ``[T, C]`` row views). With ``kv_rows`` (int64 ``[T]``),
+    ``k_cache`` and ``v_cache`` are all token rows of a cache and token ``i`` writes row ``kv_rows[i]``, or none if that lies
+    outside."""
+    ext().qkv_norm_rope(qkv, wq, wk, cos_tok, sin_tok, q_out, k_pre, k_cache, v_cache, kv_rows, int(head_dim), float(eps))
 
 
 def rms_norm(x, w, *, eps=1e-6, out=None):

@@ -239,7 +239,7 @@ class PagedKVCache:
         writing them would change the child's history, or leave what it copied behind."""
         if batch.cache is not self:
             raise StateError("the batch is another cache's")
-        if q.shape[0] < batch.tokens:
+        if q is not None and q.shape[0] < batch.tokens:
             raise ConfigurationError(f"the batch has {batch.tokens} new tokens, q has {q.shape[0]} rows")
         if batch.checked[0] == self._changes:
             return
@@ -280,6 +280,19 @@ class PagedKVCache:
         return paged.attention(q, self.storage[layer, 0], self.storage[layer, 1], batch.table, batch.kv_lens, batch.cu_q,
                                max_q_len=max(max(batch.counts), 1), causal=causal, window=window, sinks=sinks, scale=scale,
                                return_lse=return_lse, out=out)
+
+    def token_rows(self, layer: int, which: str) -> torch.Tensor:
+        """All token rows ``[pages * page_size, kv_heads * head_dim]`` of one layer's K or V (``which``), page by page."""
+        return self.storage[layer, 0 if which == "K" else 1].flatten(0, 1).flatten(1)
+
+    def new_rows(self, batch: PagedBatch) -> torch.Tensor:
+        """Where the batch's new tokens lie in :meth:`token_rows` (int64, one after the other), for a kernel that writes them
+        itself instead of :meth:`append`."""
+        self._check_batch(batch, None, write=True)
+        token = torch.arange(batch.tokens, dtype=torch.int32, device=self.device)
+        seq = torch.bucketize(token, batch.cu_q[1:], right=True)
+        at = (batch.kv_lens - batch.cu_q[1:])[seq] + token
+        return batch.table[seq, at // self.page_size].long() * self.page_size + at % self.page_size
 
     def rows(self, layer: int, which: str, page: int) -> torch.Tensor:
         """Token rows ``[page_size, kv_heads * head_dim]`` of one page (``which``: ``"K"`` or ``"V"``)."""

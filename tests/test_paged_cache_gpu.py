@@ -326,3 +326,60 @@ def test_sizes_that_the_page_table_cannot_hold_are_refused_at_once():
     for wrong in (dict(page_size=65536 + 8, max_tokens=65536 + 8, pages=1), dict(pages=1 << 20, page_size=8), dict(max_sessions=1 << 20, max_tokens=8)):
         with pytest.raises(ConfigurationError):
             _cache(**wrong)
+
+
+def test_dit_over_pages_writes_the_dense_caches_rows():
+    """Keys and values of the first layer, whose input is the same on both paths, are the dense cache's bit for bit: one
+    rounding after norm and rotation."""
+    from reelcache_b200.models.causal_wan import CAUSVID, CausalWanDiT, KVCache
+    from reelcache_b200.paged_cache import PagedKVCache
+    cfg = CAUSVID.scaled(layers=1, dim=256, heads=2, ffn=512, text_dim=128, text_len=16, latent_height=8, latent_width=16)
+    model = CausalWanDiT(cfg, "cuda", seed=5)
+    text_kv = model.encode_text(torch.randn(cfg.text_len, cfg.text_dim, device="cuda"))
+    chunk = cfg.chunk_tokens
+    cache = PagedKVCache(1, cfg.heads, cfg.head_dim, pages=60, page_size=16, max_sessions=3, max_tokens=4 * chunk)
+    sessions = [cache.open() for _ in range(2)]
+    cache.extend([(sessions[1], 2 * chunk)])  # the second session is at its third chunk
+    batch = cache.extend([(s, chunk) for s in sessions])
+    x = torch.randn(2, cfg.in_dim, cfg.frames_per_chunk, cfg.latent_height, cfg.latent_width, device="cuda")
+    captured = {}
+    model.forward_sessions(x, 500.0, cache, batch, text_kv, capture=lambda l, k, v: captured.__setitem__(l, (k.clone(), v.clone())))
+    for i, (s, index) in enumerate(zip(sessions, (0, 2))):
+        dense, kept = KVCache(cfg, 3, "cuda"), {}
+        model.forward_chunk(x[i], 500.0, index, dense, text_kv, capture=lambda l, k, v: kept.__setitem__(l, (k.clone(), v.clone())))
+        at = torch.arange(index * chunk, (index + 1) * chunk, device="cuda")
+        pages = batch.table[i, at // 16].long()
+        for which, rows in enumerate((dense.rows(0, "K"), dense.rows(0, "V"))):
+            assert torch.equal(cache.storage[0, which, pages, at % 16].flatten(1), rows[at])
+            assert torch.equal(captured[0][which][i * chunk:(i + 1) * chunk], kept[0][which])
+
+
+def test_new_rows_are_where_append_writes():
+    """The rows that a kernel of its own writes are those of append; the model's rotation from positions is its tables'."""
+    from reelcache_b200.models.causal_wan import CAUSVID, CausalWanDiT
+    from reelcache_b200.paged_cache import PagedKVCache
+    cfg = CAUSVID.scaled(layers=1, dim=256, heads=2, ffn=512, text_dim=128, text_len=16, latent_height=8, latent_width=16)
+    model = CausalWanDiT(cfg, "cuda", seed=5)
+    cache = PagedKVCache(1, cfg.heads, cfg.head_dim, pages=60, page_size=24, max_sessions=4, max_tokens=4 * cfg.chunk_tokens)
+    a, b, c = (cache.open() for _ in range(3))
+    cache.extend([(b, cfg.chunk_tokens)])
+    batch = cache.extend([(a, cfg.chunk_tokens), (c, 0), (b, cfg.chunk_tokens)])
+    positions = model.session_positions([0, 1])
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v = (torch.randn(batch.tokens, cfg.heads, cfg.head_dim, generator=g, device="cuda").bfloat16() for _ in range(3))
+    cache.append(0, batch, q, k, v, positions, model.axis_rope)
+    rows = cache.new_rows(batch)
+    assert torch.equal(cache.token_rows(0, "V")[rows], v.flatten(1))
+    cos, sin = (t[:, None].double() for t in model.session_rope([0, 1]))
+    x, y = k.double()[..., 0::2], k.double()[..., 1::2]
+    want = torch.stack([x * cos - y * sin, x * sin + y * cos], dim=-1).flatten(1)
+    size = torch.stack([x.abs() + y.abs()] * 2, dim=-1).flatten(1)  # tables in FP32, the rotation's sines within 2^-20, bf16
+    assert bool(((cache.token_rows(0, "K")[rows].double() - want).abs() <= size * 2.0 ** -19 + want.abs() * 2.0 ** -8).all())
+    for i, index in enumerate((0, 1)):
+        for got, table in zip(model.session_rope([0, 1]), model.token_rope(index)):
+            assert torch.equal(got[i * cfg.chunk_tokens:(i + 1) * cfg.chunk_tokens], table)
+    far = model.session_rope([model.rope.rows])  # beyond the model's own table
+    assert far[0].shape == (cfg.chunk_tokens, cfg.head_dim // 2) and bool((far[0] ** 2 + far[1] ** 2 - 1).abs().max() < 1e-6)
+    cache.fork(b)
+    with pytest.raises(Exception, match="forked"):
+        cache.new_rows(batch)
