@@ -72,6 +72,8 @@ std::pair<at::Tensor, c10::optional<at::Tensor>> paged_attention(
     const at::Tensor& kv_lens, const at::Tensor& cu_q, int64_t max_q_len, bool causal, int64_t window, int64_t sinks,
     c10::optional<double> scale, bool want_lse, const c10::optional<at::Tensor>& out_given,
     const c10::optional<at::Tensor>& status);
+std::string paged_attention_form(int64_t device, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t seqs,
+                                 int64_t width, int64_t page_size, int64_t max_q_len, bool causal, int64_t window, int64_t sinks);
 void pages_allocate(at::Tensor& state, int64_t pages, int64_t seqs_held, int64_t page_size, const at::Tensor& seqs,
                     const at::Tensor& new_lens, const c10::optional<at::Tensor>& status);
 void pages_fork(at::Tensor& state, int64_t pages, int64_t seqs_held, int64_t page_size, const at::Tensor& parents,
@@ -172,6 +174,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("k_pages"), py::arg("v_pages"), py::arg("table"), py::arg("kv_lens"), py::arg("cu_q"),
         py::arg("max_q_len"), py::arg("causal"), py::arg("window"), py::arg("sinks"), py::arg("scale"),
         py::arg("want_lse"), py::arg("out"), py::arg("status"));
+  m.def("paged_attention_form", &rc::paged_attention_form, "the form of the kernels that a call of these sizes takes",
+        py::arg("device"), py::arg("tokens"), py::arg("heads"), py::arg("kv_heads"), py::arg("head_dim"), py::arg("seqs"),
+        py::arg("width"), py::arg("page_size"), py::arg("max_q_len"), py::arg("causal") = false, py::arg("window") = 0,
+        py::arg("sinks") = 0);
   m.def("pages_allocate", &rc::pages_allocate, "grow sequences of a page table", py::arg("state"), py::arg("pages"), py::arg("seqs_held"), py::arg("page_size"), py::arg("seqs"), py::arg("new_lens"), py::arg("status") = py::none());
   m.def("pages_fork", &rc::pages_fork, "share pages with forked sequences, copy partial tails", py::arg("state"),
         py::arg("pages"), py::arg("seqs_held"), py::arg("page_size"), py::arg("parents"), py::arg("children"),

@@ -9,6 +9,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <string>
 #include <utility>
 
 #include "attend.cuh"
@@ -22,8 +23,32 @@ void attend_short(const Args& a, int head_dim, bool half, const at::Tensor& k_pa
                   int max_q_len, const at::Tensor& like, cudaStream_t stream, int device);
 void attend_chunk(const Args& a, int head_dim, bool half, const at::Tensor& k_pages, const at::Tensor& v_pages,
                   int max_q_len, const at::Tensor& like, cudaStream_t stream, int device);
+std::string short_form_name(const Args& a, int head_dim, int device);
+std::string chunk_form_name(const Args& a, int head_dim, int max_q_len, int device);
 
 }  // namespace paged
+
+// The form that a call of these sizes takes on `device`: "few rows, cluster N", "few rows, line", "twin N", "direct N" (N CTAs
+// to a cluster) or "planned".
+std::string paged_attention_form(int64_t device, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t seqs,
+                                 int64_t width, int64_t page_size, int64_t max_q_len, bool causal, int64_t window, int64_t sinks) {
+  RC_CHECK((head_dim == 64 || head_dim == 128) && tokens > 0 && kv_heads > 0 && heads % kv_heads == 0 && seqs > 0 && max_q_len > 0,
+           "no such call of paged attention");
+  c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
+  paged::Args a{};
+  a.tokens = static_cast<int>(tokens);
+  a.heads = static_cast<int>(heads);
+  a.kv_heads = static_cast<int>(kv_heads);
+  a.group = a.heads / a.kv_heads;
+  a.seqs = static_cast<int>(seqs);
+  a.width = static_cast<int>(width);
+  a.tiling.page = static_cast<int>(page_size);
+  a.causal = causal;
+  a.window = static_cast<int>(window);
+  a.sinks = window > 0 ? static_cast<int>(sinks) : 0;
+  const int most = static_cast<int>(std::min(max_q_len, tokens)), d = static_cast<int>(head_dim), at = static_cast<int>(device);
+  return static_cast<int64_t>(most) * a.group <= paged::kShortRows ? paged::short_form_name(a, d, at) : paged::chunk_form_name(a, d, most, at);
+}
 
 // out = softmax over the visible keys of scale * q k^T, times v, for the new tokens of every sequence; lse its natural
 // log-sum-exp. max_q_len bounds every sequence's new tokens (more are reported); rows of q that no sequence names are left

@@ -1095,18 +1095,23 @@ int clusters_at_once(int size, int device) {
 
 // CTAs of an item in the direct form, or 0 for the planned form, by estimated time in tile pairs (about 1.8 us each):
 // direct, every item takes its tiles over its cluster, in as many rounds as its clusters need, and each round has its start
-// and end to pay: about 3.5 tiles alone, 6 in a cluster, which joins. Planned, all SMs share all tiles, but the plan, the join
-// and the cut items cost about 16. Measured with 1, 2, 4 and 8 CTAs and planned (us): 16 items of 63 tiles
-// 117, 65, 40, 52 and 40; 54 of 27: 55, 38, 50, 80 and 52; 32 of 63: 118, 66, 42, 78 and 57; 84 of 49: 97, 108, 105, 150
-// and 87; 16 of 8: 21, 18, 15, 25 and 25.
+// and end to pay: about 3.5 tiles alone, 6 in a cluster, which joins. A block of the grid without an item (its row tile lies
+// past its sequence's rows: one long sequence among short ones) keeps an SM for up to 2.4 us, half of it next to other work:
+// 0.6. Planned, all SMs share all tiles, but the plan, the join and the cut items cost about 16. Measured with 1, 2, 4 and 8
+// CTAs and planned (us): 16 items of 63 tiles 117, 65, 40, 52 and 40; 54 of 27: 55, 38, 50, 80 and 52; 32 of 63: 118, 66, 42,
+// 78 and 57; 84 of 49: 97, 108, 105, 150 and 87; 16 of 8: 21, 18, 15, 25 and 25. 16 sequences with one of 4,000 new tokens
+// (141 items, 1,859 empty blocks) 107 directly and 84 planned. Over 655 shapes, batches of unequal sequences among them, the
+// choice costs 2.6 % on average (3.9 % without the empty blocks).
 template <typename T, int D>
-int direct_cluster(int64_t items, int64_t tiles, bool uneven, int device) {
-  double best = static_cast<double>(items) * tiles / sm_count(device) * (uneven ? 0.75 : 1.0) + 16.0;
+int direct_cluster(int64_t items, int64_t empty, int64_t tiles, bool uneven, int device) {
+  const int sms = sm_count(device);
+  double best = static_cast<double>(items) * tiles / sms * (uneven ? 0.75 : 1.0) + 16.0;
   int cluster = 0;
   for (int c = 1; c <= 16; c *= 2) {
     const int64_t slots = clusters_at_once<T, D>(c, device);
     if (slots <= 0) continue;
-    const double t = static_cast<double>((items + slots - 1) / slots) * (static_cast<double>((tiles + c - 1) / c) + (c > 1 ? 6.0 : 3.5));
+    const double t = static_cast<double>((items + slots - 1) / slots) * (static_cast<double>((tiles + c - 1) / c) + (c > 1 ? 6.0 : 3.5)) +
+                     0.6 * static_cast<double>(empty * c) / sms;
     if (t < best) {
       best = t;
       cluster = c;
@@ -1115,37 +1120,57 @@ int direct_cluster(int64_t items, int64_t tiles, bool uneven, int device) {
   return cluster;
 }
 
+// The form that a call takes, and its size: row tiles of a sequence and KV head (at most), items of the direct grid and of
+// the plan (at most).
+struct ChunkForm {
+  int64_t row_tiles, grid_items, most_items;
+  int cluster;  // 0: planned
+  bool twin;
+};
+
+template <typename T, int D>
+ChunkForm chunk_form(const Args& a, int max_q_len, int device) {
+  ChunkForm form{};
+  form.row_tiles = (static_cast<int64_t>(max_q_len) * a.group + kItemRows - 1) / kItemRows;
+  form.grid_items = static_cast<int64_t>(a.seqs) * form.row_tiles * a.kv_heads;
+  form.most_items =
+      std::min<int64_t>(form.grid_items, (static_cast<int64_t>(a.tokens) * a.group / kItemRows + a.seqs) * a.kv_heads);
+  // tiles of an item, at most: the table's width, or what a window leaves of it
+  int64_t keys = static_cast<int64_t>(a.width) * a.tiling.page;
+  if (a.window > 0) keys = std::min<int64_t>(keys, static_cast<int64_t>(a.window) + a.sinks + kItemRows / a.group + 2 * kTile);
+  const int64_t tiles = (keys + kTile - 1) / kTile;
+  form.twin = static_cast<int64_t>(max_q_len) * a.group <= kTile;
+  chunk_configure<T, D, true, false>(device);
+  form.cluster = direct_cluster<T, D>(form.most_items, form.grid_items - form.most_items, form.twin ? (tiles + 1) / 2 : tiles,
+                                      a.causal && form.row_tiles > 1, device);
+  return form;
+}
+
 template <typename T, int D>
 void chunk_launch(const Args& args, const at::Tensor& k_pages, const at::Tensor& v_pages, int max_q_len,
                   const at::Tensor& like, cudaStream_t stream, int device) {
   using Shape = ChunkShape<D, false>;
+  const ChunkForm form = chunk_form<T, D>(args, max_q_len, device);
+  const int64_t most_items = form.most_items;
+  RC_CHECK(most_items < (1ll << 26), "too many rows for one launch");
   Chunk p{};
   p.a = args;
   p.a.tiling = Tiling::of(args.tiling.page, kTile);
-  const int64_t row_tiles = (static_cast<int64_t>(max_q_len) * args.group + kItemRows - 1) / kItemRows;
-  const int64_t grid_items = static_cast<int64_t>(args.seqs) * row_tiles * args.kv_heads;
-  const int64_t most_items = std::min<int64_t>(grid_items, (static_cast<int64_t>(args.tokens) * args.group / kItemRows + args.seqs) * args.kv_heads);
-  RC_CHECK(most_items < (1ll << 26), "too many rows for one launch");
-  p.row_tiles = static_cast<int>(row_tiles);
+  p.row_tiles = static_cast<int>(form.row_tiles);
   p.most_items = static_cast<int>(most_items);
   p.ctas = sm_count(device);
+  p.cluster = form.cluster;
   const PageMaps maps = page_maps(k_pages, v_pages, p.a.tiling, kTile);
-  // tiles of an item, at most: the table's width, or what a window leaves of it
-  int64_t keys = static_cast<int64_t>(args.width) * args.tiling.page;
-  if (args.window > 0) keys = std::min<int64_t>(keys, static_cast<int64_t>(args.window) + args.sinks + kItemRows / args.group + 2 * kTile);
-  chunk_configure<T, D, true, false>(device);
-  const int64_t tiles = (keys + kTile - 1) / kTile;
-  const bool twin = static_cast<int64_t>(max_q_len) * args.group <= kTile;
-  p.cluster = direct_cluster<T, D>(most_items, twin ? (tiles + 1) / 2 : tiles, args.causal && row_tiles > 1, device);
-  if (p.cluster > 0 && twin) {
-    chunk_configure<T, D, true, true>(device);
-    launch(chunk_kernel<T, D, true, true>, dim3(static_cast<unsigned>(grid_items * p.cluster)), kChunkThreads,
-           ChunkShape<D, true>::bytes, p.cluster, stream, maps, p);
-    return;
-  }
   if (p.cluster > 0) {
-    launch(chunk_kernel<T, D, true, false>, dim3(static_cast<unsigned>(grid_items * p.cluster)), kChunkThreads, Shape::bytes, p.cluster,
-           stream, maps, p);
+    const int64_t blocks = form.grid_items * p.cluster;
+    RC_CHECK(blocks < (1ll << 31), "too many sequences and rows for one launch");
+    const dim3 grid(static_cast<unsigned>(blocks));
+    if (form.twin) {
+      chunk_configure<T, D, true, true>(device);
+      launch(chunk_kernel<T, D, true, true>, grid, kChunkThreads, ChunkShape<D, true>::bytes, p.cluster, stream, maps, p);
+    } else {
+      launch(chunk_kernel<T, D, true, false>, grid, kChunkThreads, Shape::bytes, p.cluster, stream, maps, p);
+    }
     return;
   }
   chunk_configure<T, D, false, false>(device);
@@ -1173,6 +1198,13 @@ void attend_chunk(const Args& a, int head_dim, bool half, const at::Tensor& k_pa
   else
     half ? chunk_launch<__half, 64>(a, k_pages, v_pages, max_q_len, like, stream, device)
          : chunk_launch<__nv_bfloat16, 64>(a, k_pages, v_pages, max_q_len, like, stream, device);
+}
+
+std::string chunk_form_name(const Args& a, int head_dim, int max_q_len, int device) {
+  const ChunkForm form = head_dim == 128 ? chunk_form<__nv_bfloat16, 128>(a, max_q_len, device)
+                                         : chunk_form<__nv_bfloat16, 64>(a, max_q_len, device);
+  if (form.cluster == 0) return "planned";
+  return (form.twin ? "twin " : "direct ") + std::to_string(form.cluster);
 }
 
 }  // namespace paged

@@ -709,8 +709,7 @@ int short_cluster(int64_t items, int64_t tiles, int step, bool several, int devi
 }
 
 template <typename T, int D>
-void short_launch(Args a, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& like, cudaStream_t stream,
-                  int device) {
+void short_configure(int device) {
   using Shape = ShortShape<D>;
   static bool known[64] = {};
   bool& configured = known[device & 63];
@@ -720,20 +719,35 @@ void short_launch(Args a, const at::Tensor& k_pages, const at::Tensor& v_pages, 
     RC_CUDA(cudaFuncSetAttribute(short_kernel<T, D, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     configured = true;
   }
+}
+
+int64_t short_tiles(const Args& a) { return (static_cast<int64_t>(a.width) * a.tiling.page + kShortTile - 1) / kShortTile; }
+
+// CTAs of a cluster, or 0 for the line.
+template <typename T, int D>
+int short_form(const Args& a, int device) {
+  short_configure<T, D>(device);
+  return short_cluster<T, D>(static_cast<int64_t>(a.seqs) * a.kv_heads, short_tiles(a), Tiling::of(a.tiling.page, kShortTile).step,
+                             a.seqs > 1, device);
+}
+
+template <typename T, int D>
+void short_launch(Args a, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& like, cudaStream_t stream,
+                  int device) {
+  using Shape = ShortShape<D>;
   static_assert(kRows * (D + 2) * 4 <= Shape::stages * 2 * Shape::tile_bytes, "a CTA's rows fit its stages");
   Short p{};
   p.a = a;
   p.a.tiling = Tiling::of(a.tiling.page, kShortTile);
   const PageMaps maps = page_maps(k_pages, v_pages, p.a.tiling, kShortTile);
   const int64_t items = static_cast<int64_t>(a.seqs) * a.kv_heads, slots = sm_count(device) * kShortCtasPerSm;
-  const int64_t most_tiles = (static_cast<int64_t>(a.width) * a.tiling.page + kShortTile - 1) / kShortTile;
-  p.cluster = short_cluster<T, D>(items, most_tiles, p.a.tiling.step, a.seqs > 1, device);
+  p.cluster = short_form<T, D>(a, device);
   if (p.cluster > 0) {
     launch(short_kernel<T, D, true>, dim3(static_cast<unsigned>(items * p.cluster)), kShortThreads, Shape::bytes, p.cluster,
            stream, maps, p);
     return;
   }
-  const int ctas = static_cast<int>(std::min<int64_t>(slots, items * (most_tiles + 1)));
+  const int ctas = static_cast<int>(std::min<int64_t>(slots, items * (short_tiles(a) + 1)));
   RC_CHECK(items * (kRows / 4) < (1ll << 31), "too many sequences and rows for one launch");
   const int64_t floats = 2ll * ctas * kRows * (D + 2), ints = 1 + 2ll * a.seqs;
   at::Tensor workspace = at::empty({floats + ints}, like.options().dtype(at::kFloat));
@@ -753,6 +767,11 @@ void attend_short(const Args& a, int head_dim, bool half, const at::Tensor& k_pa
   else
     half ? short_launch<__half, 64>(a, k_pages, v_pages, like, stream, device)
          : short_launch<__nv_bfloat16, 64>(a, k_pages, v_pages, like, stream, device);
+}
+
+std::string short_form_name(const Args& a, int head_dim, int device) {
+  const int cluster = head_dim == 128 ? short_form<__nv_bfloat16, 128>(a, device) : short_form<__nv_bfloat16, 64>(a, device);
+  return cluster > 0 ? "few rows, cluster " + std::to_string(cluster) : "few rows, line";
 }
 
 }  // namespace paged

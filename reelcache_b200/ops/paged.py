@@ -53,6 +53,14 @@ def attention(q, k_pages, v_pages, block_table, kv_lens, cu_q, *, max_q_len: int
     return (out, lse) if return_lse else out
 
 
+def attention_form(tokens, heads, kv_heads, head_dim, seqs, width, page_size, *, max_q_len: int, causal: bool = False,
+                   window: int | None = None, sinks: int = 0, device: int = 0) -> str:
+    """Which form of the kernels a call of :func:`attention` with these sizes takes: ``"few rows, cluster N"``, ``"few rows,
+    line"``, ``"twin N"``, ``"direct N"`` (``N`` CTAs to a cluster) or ``"planned"``. ``width``: columns of the block table."""
+    return ext().paged_attention_form(device, tokens, heads, kv_heads, head_dim, seqs, width, page_size, max_q_len, causal,
+                                      window or 0, sinks)
+
+
 def copy_pages(storage, source, target, rows=None):
     """Copy pages ``source[i]`` to ``target[i]`` (int32 vectors) in every plane of ``storage [planes, pages, page_size,
     ...]``: whole pages, or their first ``rows[i]`` tokens. Pairs of -1 are skipped. Targets must differ from one another

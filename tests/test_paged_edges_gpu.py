@@ -247,10 +247,10 @@ def test_more_new_tokens_than_the_bound_are_reported(cuda_device, new, bound):
     k_pages, v_pages, table, kv_lens, cu_q = paged_batch(g, new, [n + 50 for n in new], 2, 64, 16, BF16)
     q = torch.randn(sum(new), 4, 64, generator=g, device="cuda").bfloat16()
     call = lambda q=q, **kw: paged.attention(q, k_pages, v_pages, table, kv_lens, cu_q, **{"max_q_len": max(new), **kw})  # noqa: E731
-    want = call()
-    _ext.check_status(cuda_device)
-    assert torch.equal(call(max_q_len=10 ** 6), want)
-    _ext.check_status(cuda_device)
+    want, _, error, _ = attend(q, k_pages, v_pages, table, kv_lens, new)
+    for most in (max(new), 10 ** 6):  # (a looser bound may take another form, and round elsewhere)
+        assert within(call(max_q_len=most), want, error)
+        _ext.check_status(cuda_device)
     call(max_q_len=bound)
     with pytest.raises(DeviceStatusError, match="max_q_len"):
         _ext.check_status(cuda_device)
@@ -360,3 +360,24 @@ def test_outputs_that_overlap_themselves_are_refused():
         paged.append(both[:3], k, k, positions, AxisRope.wan(64), k_pages, v_pages, table, kv_lens, cu_q, out=both[1:4])
     want = paged.attention(both[:3], k_pages, v_pages, table, kv_lens, cu_q, max_q_len=3)
     assert torch.equal(paged.attention(both[:3], k_pages, v_pages, table, kv_lens, cu_q, max_q_len=3, out=both[:3]), want)
+
+
+# -- which form a call takes ------------------------------------------------------------------------------------------
+
+def _form(new, totals, heads, kv_heads, d, page, **mask):
+    """The form that the checks of these sizes take (:func:`paged_batch` with two columns more)."""
+    from reelcache_b200.ops import paged
+    width = max(max(-(-t // page) for t in totals), 1) + 2
+    return paged.attention_form(sum(new), heads, kv_heads, d, len(new), width, page, max_q_len=max(max(new), 1), **mask)
+
+
+def test_a_long_sequence_among_short_ones_is_planned():
+    """The direct grid has a block for every row tile that the longest sequence has, in every sequence: 2,000 here, of which
+    1,859 would each take an SM to find that they have nothing to do."""
+    assert _form([4000] + [1] * 15, [4096] * 16, 8, 1, 128, 64, causal=True) == "planned"
+    assert _form([250] * 16, [4096] * 16, 8, 1, 128, 64, causal=True) == "direct 1"  # the same rows, evenly
+
+
+def test_grids_beyond_31_bits_are_not_launched_directly():
+    """One sequence of a million tokens among 10,000: 4 * 10^9 blocks would wrap, and leave rows without a result."""
+    assert _form([1_000_000] + [1] * 9_999, [8] * 10_000, 8, 8, 128, 8) == "planned"
