@@ -381,3 +381,129 @@ def test_a_long_sequence_among_short_ones_is_planned():
 def test_grids_beyond_31_bits_are_not_launched_directly():
     """One sequence of a million tokens among 10,000: 4 * 10^9 blocks would wrap, and leave rows without a result."""
     assert _form([1_000_000] + [1] * 9_999, [8] * 10_000, 8, 8, 128, 8) == "planned"
+
+
+# -- the planned form of chunks ---------------------------------------------------------------------------------------
+
+# items cut into single tiles; odd groups and pages; more items than SMs (whole rounds, then cut ones)
+PLANNED = [([300, 0, 45, 1], [1100, 30, 200, 700], 6, 2, 64, 16, BF16), ([700, 129], [700, 2300], 5, 1, 128, 24, FP16),
+           ([900, 0, 333, 1], [1300, 50, 1333, 800], 40, 40, 64, 200, BF16)]
+
+
+def _planned(g, new, totals, heads, kv_heads, d, page, dtype, *, causal=False, window=None, sinks=0, **kw):
+    """A batch with a table wide enough for 60,000 tokens of each sequence (as one has that is kept for a graph), which takes
+    the planned form whatever the lengths are, and its queries."""
+    from reelcache_b200.ops import paged
+    k_pages, v_pages, table, kv_lens, cu_q = paged_batch(g, new, totals, kv_heads, d, page, dtype, width_extra=60_000 // page, **kw)
+    assert paged.attention_form(sum(new), heads, kv_heads, d, len(new), table.shape[1], page, max_q_len=max(new), causal=causal,
+                                window=window, sinks=sinks) == "planned"
+    q = torch.randn(sum(new), heads, d, generator=g, device="cuda").to(dtype)
+    return q, k_pages, v_pages, table, kv_lens, cu_q
+
+
+def _check(batch, new, **mask):
+    from reelcache_b200.ops import paged
+    out, lse = paged.attention(*batch, max_q_len=max(new), return_lse=True, **mask)
+    q, k_pages, v_pages, table, kv_lens, _ = batch
+    want, want_lse, bound, lse_bound = attend(q, k_pages, v_pages, table, kv_lens, new, **mask)
+    assert within(out, want, bound), float(((out.double() - want).abs() - bound).max())
+    assert within(lse, want_lse, lse_bound)
+    return out
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("fill", [None, math.nan, math.inf, torch.finfo(BF16).min])
+@pytest.mark.parametrize("shape", PLANNED)
+def test_planned_shapes_and_what_no_session_holds(shape, fill, causal):
+    out = _check(_planned(_gen(81), *shape, causal=causal, fill=fill if shape[-1] == BF16 or fill is None else math.nan), shape[0], causal=causal)
+    assert bool(torch.isfinite(out.float()).all())
+
+
+@pytest.mark.parametrize("d,dtype", [(64, BF16), (128, FP16)])
+@pytest.mark.parametrize("mask", [dict(window=1, causal=True), dict(window=333, sinks=5, causal=True), dict(window=333, sinks=5),
+                                  dict(window=500, sinks=130), dict(window=100, sinks=400, causal=True),
+                                  dict(window=700, sinks=130, causal=True)])
+def test_planned_windows_and_sinks(mask, d, dtype):
+    new, totals = [900, 0, 333, 1], [1300, 50, 1333, 800]
+    _check(_planned(_gen(82), new, totals, 40, 40, d, 48, dtype, fill=math.nan, **mask), new, **mask)
+
+
+def test_planned_long_window():
+    new, mask = [1000], dict(window=5000, sinks=200, causal=True)
+    _check(_planned(_gen(83), new, [12_000], 40, 40, 64, 64, BF16, **mask), new, **mask)
+
+
+@pytest.mark.parametrize("new,totals", [([300, 20], [60, 0]), ([900, 40, 1], [890, 700, 0])])
+def test_planned_rows_that_see_nothing(new, totals):
+    batch = _planned(_gen(84), new, totals, 4, 2, 64, 16, BF16, causal=True, fill=math.nan)
+    out = _check(batch, new, causal=True)
+    assert not bool(out[:new[0] - totals[0]].any())
+
+
+@pytest.mark.parametrize("shape", PLANNED[:2])
+def test_planned_layouts_and_strides(shape):
+    """Heads outside of tokens in memory, queries out of a fused projection, outputs on 16 but not on 32 bytes."""
+    from reelcache_b200.ops import paged
+    new, _, heads, _, d = shape[:5]
+    q, *rest = _planned(_gen(85), *shape, causal=True, layout="hnd")
+    _check((q, *rest), new, causal=True)
+    fused = torch.randn(sum(new), heads + 3, d, generator=_gen(86), device="cuda").to(q.dtype)
+    fused[:, 1:heads + 1] = q
+    want = paged.attention(q, *rest, max_q_len=max(new), causal=True)
+    assert torch.equal(paged.attention(fused[:, 1:heads + 1], *rest, max_q_len=max(new), causal=True), want)
+    buffer = torch.zeros(sum(new), heads + 1, d + 8, dtype=q.dtype, device="cuda")
+    paged.attention(q, *rest, max_q_len=max(new), causal=True, out=buffer[:, :heads, 8:])
+    assert torch.equal(buffer[:, :heads, 8:], want)
+    assert not bool(buffer[:, heads].any()) and not bool(buffer[:, :, :8].any())
+
+
+@pytest.mark.parametrize("shape", PLANNED)
+def test_planned_repeats_bits_on_several_streams_and_in_a_graph(shape):
+    """Each call has a workspace of its own; a captured call follows lengths, pages and queries."""
+    from reelcache_b200.ops import paged
+    new = shape[0]
+    q, k_pages, v_pages, table, kv_lens, cu_q = _planned(_gen(87), *shape, causal=True)
+    call = lambda q=q: paged.attention(q, k_pages, v_pages, table, kv_lens, cu_q, max_q_len=max(new), causal=True)  # noqa: E731
+    others = [q * x for x in (0.5, 2.0, -1.0)]
+    want = [call(x) for x in others]
+    streams = [torch.cuda.Stream() for _ in others]
+    got = [[] for _ in others]
+    for stream in streams:
+        stream.wait_stream(torch.cuda.current_stream())
+    for _ in range(4):  # calls of all streams at once
+        for stream, x, outs in zip(streams, others, got):
+            with torch.cuda.stream(stream):
+                outs.append(call(x))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, outs in zip(want, got) for y in outs)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    kv_lens[0] -= 57
+    table[0, :2] = table[0, :2].flip(0)
+    q.mul_(0.5)
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, call())
+
+
+# -- items of many parts ----------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("mask", [dict(causal=True), dict(causal=True, window=60_000, sinks=70), dict()])
+@pytest.mark.parametrize("new,kv_heads,total,form", [
+    (1, 1, 131_072, "few rows, line"), (8, 1, 131_072, "few rows, line"), (1, 8, 65_536, "few rows, line"), (7, 2, 100_001, "few rows, line"),
+    (16, 1, 65_536, "planned"), (40, 1, 131_072, "planned"), (128, 2, 65_537, "planned"), (40, 8, 131_072, "planned"), (300, 1, 70_000, "planned")])
+def test_items_joined_out_of_many_parts(new, kv_heads, total, form, mask):
+    """More parts than a join takes at a time (32): statistics are carried from one pass to the next. Scores grow along the
+    keys and shrink again, so the maximum moves between the passes."""
+    from reelcache_b200.ops import paged
+    d, page, heads = 64, 64, 2 * kv_heads
+    g = _gen(new + total)
+    k_pages, v_pages, table, kv_lens, cu_q = paged_batch(g, [new], [total], kv_heads, d, page, BF16)
+    if kv_heads in (1, 2):
+        assert paged.attention_form(new, heads, kv_heads, d, 1, table.shape[1], page, max_q_len=new, **mask) == form
+    hill = 3.0 - 12.0 * (torch.arange(table.shape[1] * page, device="cuda") / total - 0.7).abs()
+    k_pages[table[0].long()] += hill.view(-1, page, 1, 1).bfloat16()
+    q = (torch.randn(new, heads, d, generator=g, device="cuda") * 0.3 + 0.5).bfloat16()
+    _check((q, k_pages, v_pages, table, kv_lens, cu_q), [new], **mask)
