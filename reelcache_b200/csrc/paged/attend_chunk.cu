@@ -3,10 +3,11 @@
 //
 // What bounds it: the tensor core and the exponentials. A tile of 128 rows x 128 keys (head_dim 128) is 8.4 MFLOP, 1,024
 // cycles of an SM's tcgen05 rate, and 16,384 exponentials, 1,024 cycles of its 16 a cycle, so the two have to run at the
-// same time. Measured: 3,300 cycles for a pair of tiles (2,048 of them on the tensor core); 4,680 tokens over 23,400 keys
-// of 12 heads 556 us in a short run (1,210 TFLOP/s), 645 us in a long one, where the card's power limit binds before
-// either (990 W, 1.3 to 1.7 GHz): what saves energy is what helps then (exponentials by a polynomial on the FMA pipe cost
-// 2 to 5 %; items out of step with each other 15 to 20 %).
+// same time. Measured: 3,700 cycles for a pair of tiles over a whole launch, the tensor pipe busy for 56 % of them
+// (counters, 2,340 tokens over 23,400 keys); 4,680 tokens over 23,400 keys of 12 heads 594 us in runs of three calls (1,130
+// TFLOP/s) and 656 us in one of seconds (1,025), where the card's power limit binds too (993 W, 1.64 GHz): what saves energy
+// is what helps then (exponentials by a polynomial on the FMA pipe cost 2 to 5 %; items out of step with each other 15 to
+// 20 %).
 //
 // A CTA works on 256 rows as two tiles of 128 that share every K and V block. Rows are (query, head of the group),
 // query-major, so grouped heads share the loads of their KV head. 384 threads:
@@ -54,7 +55,8 @@ constexpr int kChunkThreads = 384;
 constexpr int kPlanThreads = 1024;
 constexpr int kKStages = 3;
 // Register split (setmaxnreg): the launch holds kLaunchRegs a thread (checked on the host); the third warpgroup gives up
-// registers for the softmax warpgroups, which hold a row of 128 scores.
+// registers for the softmax warpgroups, which hold a row of 128 scores. Spilled at that cap (bytes stored and read, 128
+// channels): planned form 8 and 56, direct 36 and 184, twin 40 and 240.
 constexpr int kLaunchRegs = 168;
 constexpr int kSoftmaxRegs = 208;
 constexpr int kRoleRegs = 88;

@@ -1,9 +1,10 @@
 // Attention of few query rows (single tokens, drafts) over a paged cache, for sm_100a.
 //
-// What bounds it: reading K and V once. A tile of 64 keys is 32 KB (head_dim 128) and needs 256 m16n8k16 products for
-// 16 query rows, a fifth of the time that the tile's bytes take at an SM's share of HBM, so the products run on
-// mma.sync from registers and the design is about keeping bytes in flight: one producer warp streams K and V tiles with
-// TMA (one box per page and 64 channels, 128-byte swizzle) through a ring of stages, two CTAs per SM.
+// What bounds it: reading K and V once. A tile of 64 keys is 32 KB (head_dim 128) and needs 128 m16n8k16 products for
+// 16 query rows (64 for S, 64 for P V), which keep the tensor pipe busy for a sixth of the time that the bytes take
+// (counters: 17 %), so the products run on mma.sync from registers and the design is about keeping bytes in flight: one
+// producer warp streams K and V tiles with TMA (one box per page and 64 channels, 128-byte swizzle) through a ring of
+// stages, two CTAs per SM (168 registers a thread; the line form with 128 channels spills 12 bytes).
 //
 // Rows: the heads of a group share K and V, so a row is (query, head of the group), query-major, 16 rows at most. The four
 // consumer warps take 16 keys of each tile: every warp runs its own online softmax (maximum, sum and output in FP32
@@ -16,7 +17,7 @@
 // Work, clustered (few sequences): a cluster of up to 16 CTAs per sequence and head, joined through distributed shared
 // memory; no scan of the lengths, no workspace, no second launch.
 //
-// Measured: 48 sessions of up to 16,384 keys (32 / 8 heads, 1.67 GB) 255 to 260 us, 6.5 TB/s; one session over 2,048 keys
+// Measured: 48 sessions of up to 16,384 keys (32 / 8 heads, 1.67 GB) 259 us, 6.45 TB/s; one session over 2,048 keys
 // 8.1 us clustered, 13.4 us as a line (launches back to back).
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>

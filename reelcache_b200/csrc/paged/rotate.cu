@@ -19,8 +19,8 @@
 //
 // 16-bit types take sin and cos from the special function unit (off by at most 2^-21, a thousandth of what rounding to
 // fp16 loses), fp32 takes sincospi.
-// Measured: q and k of 14,400 tokens x 64 heads of 128 (472 MB moved) 76 us, 6.2 TB/s; three chunks of 4,680 tokens
-// x 36 heads into pages 41.7 us, 6.2 TB/s (51 us with one head group of q, k and v mixed per thread, 81 us with two heads
+// Measured: q and k of 14,400 tokens x 64 heads of 128 (472 MB moved) 75 us, 6.3 TB/s; three chunks of 4,680 tokens
+// x 36 heads into pages 42.2 us, 6.1 TB/s (47 us with each store before the loads of the next heads, 51 us with one head group of q, k and v mixed per thread, 81 us with two heads
 // a thread).
 #include <ATen/ATen.h>
 #include <ATen/MemoryOverlap.h>

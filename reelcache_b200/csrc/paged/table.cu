@@ -17,7 +17,7 @@
 // plan writes nothing but the status word (a release skips sequences out of range, and gives back once what is named
 // twice). Tables, counts and data are then moved by one launch over all SMs, which
 // reads the plan from device memory. The plan is latency (4 to 6 us); the move is a copy, bound by HBM (measured: 0.5 GB of
-// pages moved together in 155 us, 6.3 TB/s read and written).
+// pages moved together in 152 us, 6.3 TB/s read and written).
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
