@@ -51,6 +51,7 @@ class PagedSession:
     length: int = 0
     open: bool = True
     blocks: list = field(default_factory=list, repr=False)
+    cache: "PagedKVCache | None" = field(default=None, repr=False, compare=False)
 
 
 @dataclass(frozen=True)
@@ -121,6 +122,8 @@ class PagedKVCache:
 
     def _check(self, sessions: Sequence[PagedSession]):
         for s in sessions:
+            if s.cache is not self:
+                raise StateError(f"the session in slot {s.slot} is another cache's")
             if not s.open:
                 raise StateError(f"session in slot {s.slot} is closed")
 
@@ -138,7 +141,7 @@ class PagedKVCache:
         """A session without history."""
         (slot,) = self._next_slots(1)
         self._free_slots.pop()
-        return PagedSession(slot)
+        return PagedSession(slot, cache=self)
 
     def fork(self, session: PagedSession, lengths: Sequence[int] | None = None, *, count: int | None = None) -> list[PagedSession]:
         """Sessions that begin with the first ``lengths[i]`` tokens of ``session`` (``count`` times all of it): whole pages
@@ -161,7 +164,7 @@ class PagedKVCache:
         self._changes += 1
         children = []
         for slot, n in zip(slots, lengths):
-            child = PagedSession(slot, n, True, session.blocks[:n // self.page_size])
+            child = PagedSession(slot, n, True, session.blocks[:n // self.page_size], self)
             for block in child.blocks:
                 block.holders += 1
             if n % self.page_size:

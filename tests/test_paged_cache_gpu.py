@@ -383,3 +383,19 @@ def test_new_rows_are_where_append_writes():
     cache.fork(b)
     with pytest.raises(Exception, match="forked"):
         cache.new_rows(batch)
+
+
+def test_a_session_of_another_cache_is_refused():
+    """Its slot and pages are other ones here."""
+    from reelcache_b200.errors import StateError
+    cache, other = _cache(), _cache()
+    a, b = cache.open(), other.open()
+    other.extend([(b, 20)])
+    (c,) = other.fork(b)
+    state = cache.table.state.clone()
+    for call in (lambda: cache.extend([(a, 3), (b, 3)]), lambda: cache.extend([(c, 3)]), lambda: cache.fork(b), lambda: cache.close(b),
+                 lambda: cache.again([(b, 3)])):
+        with pytest.raises(StateError):
+            call()
+    assert torch.equal(cache.table.state, state) and a.length == 0 and cache.free_pages == cache.pages
+    other.close(b, c)
