@@ -399,3 +399,19 @@ def test_a_session_of_another_cache_is_refused():
             call()
     assert torch.equal(cache.table.state, state) and a.length == 0 and cache.free_pages == cache.pages
     other.close(b, c)
+
+
+def test_rows_are_the_pages_token_rows():
+    """A restored chunk can be written straight into a session's pages."""
+    cache = _cache()
+    a = cache.open()
+    batch = cache.extend([(a, 40)])
+    k, v = (torch.randn(40, 2, 64, device="cuda").bfloat16() for _ in range(2))
+    for block in range(3):
+        page, n = int(batch.table[0, block]), min(16, 40 - 16 * block)
+        for which, rows in (("K", k), ("V", v)):
+            cache.rows(1, which, page)[:n] = rows[16 * block:16 * block + n].flatten(1)
+    q = torch.randn(40, 4, 64, device="cuda").bfloat16()
+    out = cache.attend(1, batch, q)
+    want = attend(q, k[None], v[None], torch.zeros(1, 1, dtype=torch.int32, device="cuda"), [40], [40])[0]
+    assert float((out.double() - want).norm() / want.norm()) < 1e-2
