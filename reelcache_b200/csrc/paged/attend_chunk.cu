@@ -52,7 +52,6 @@ namespace paged {
 constexpr int kTile = 128;      // keys of a block, rows of a tile
 constexpr int kItemRows = 256;  // rows of an item: two tiles
 constexpr int kChunkThreads = 384;
-constexpr int kPlanThreads = 1024;
 constexpr int kKStages = 3;
 // Register split (setmaxnreg): the launch holds kLaunchRegs a thread (checked on the host); the third warpgroup gives up
 // registers for the softmax warpgroups, which hold a row of 128 scores. Spilled at that cap (bytes stored and read, 128
@@ -106,31 +105,6 @@ struct Chunk {
   int most_items;  // room for items
 };
 
-__device__ __forceinline__ int plan_scan(int value, int* warp_sums, int* total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int x = value;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
-  }
-  __syncthreads();
-  if (lane == 31) warp_sums[warp] = x;
-  __syncthreads();
-  if (warp == 0) {
-    int w = warp_sums[lane];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, w, o);
-      if (lane >= o) w += y;
-    }
-    warp_sums[lane] = w;
-  }
-  __syncthreads();
-  *total = warp_sums[31];
-  return x - value + (warp > 0 ? warp_sums[warp - 1] : 0);
-}
-
 // New tokens of a sequence (returned), where they begin and how many keys it has.
 __device__ __forceinline__ int sequence(const Args& a, int s, int* q_first, int* kv_len) {
   *kv_len = held_keys(a, s);
@@ -168,7 +142,7 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const __grid_c
       report_rows(a, s);
     }
     int total;
-    const int before = plan_scan(n, warp_sums, &total);
+    const int before = block_scan(n, warp_sums, &total);
     if (s < a.seqs) plan.base[s] = items + before;
     items += total;
   }
@@ -195,7 +169,7 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const __grid_c
     sum += item.tiles;
   }
   int all;
-  plan_scan(sum, warp_sums, &all);
+  block_scan(sum, warp_sums, &all);
   const int share = (all + p.ctas - 1) / p.ctas;
   // whole rounds: 3 % above the share is less than cutting the last items costs
   const int limit = share + share / 32;
@@ -215,13 +189,13 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const __grid_c
     const int i = i0 + threadIdx.x;
     const int n = i < items ? plan.items[i].tiles : 0;
     int total;
-    const int before = plan_scan(n, warp_sums, &total);
+    const int before = block_scan(n, warp_sums, &total);
     if (i < items) plan.items[i].start = line + before;
     line += total;
   }
   __syncthreads();
   int wanted_all;
-  const int before = plan_scan(c < p.ctas ? max(0, share - whole) : 0, warp_sums, &wanted_all);
+  const int before = block_scan(c < p.ctas ? max(0, share - whole) : 0, warp_sums, &wanted_all);
   // if whole rounds went over the share, the last CTA takes what is left
   if (c <= p.ctas) {
     const int cut = c == p.ctas ? line : min(line, before);

@@ -18,6 +18,8 @@ constexpr int kPageRows = 0x404;
 
 namespace paged {
 
+constexpr int kPlanThreads = 1024;  // of the one-block kernels that plan
+
 // Every kernel here is launched as a programmatic dependent of what runs before it on the stream: its launch and its setup
 // overlap that kernel's end. after_earlier() comes before its first access to global memory and waits until everything
 // before it on the stream is complete and visible; let_later() allows the next such kernel to be set up.
@@ -27,6 +29,32 @@ namespace paged {
 #ifdef __CUDACC__
 __device__ __forceinline__ void after_earlier() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_later() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// Exclusive prefix sum over the block and its total (kPlanThreads threads, all of them).
+__device__ __forceinline__ int block_scan(int value, int* warp_sums, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = value;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();  // warp_sums of a previous call has been read
+  if (lane == 31) warp_sums[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    int w = warp_sums[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += y;
+    }
+    warp_sums[lane] = w;
+  }
+  __syncthreads();
+  *total = warp_sums[31];
+  return x - value + (warp > 0 ? warp_sums[warp - 1] : 0);
+}
 
 // `cluster` CTAs to a cluster (0: no clusters).
 template <typename... Params, typename... Args>

@@ -31,7 +31,9 @@
 namespace rc {
 namespace pagetable {
 
-constexpr int kPlanThreads = 1024;
+using paged::block_scan;
+using paged::kPlanThreads;
+
 constexpr int kMoveThreads = 256;
 constexpr int kMoveVecs = 8;                                  // 16-byte vectors per thread and work item
 constexpr int kMoveBytes = kMoveThreads * kMoveVecs * 16;     // 32 KB of a page and plane
@@ -54,32 +56,6 @@ struct Plan {
 
 __device__ __forceinline__ void refuse(int* status, int code) {
   if (status != nullptr) atomicCAS(status + kPagedWord, 0, code);
-}
-
-// Exclusive prefix sum over the block and its total (kPlanThreads threads, all of them).
-__device__ __forceinline__ int block_scan(int value, int* warp_sums, int* total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int x = value;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
-  }
-  __syncthreads();  // warp_sums of a previous call has been read
-  if (lane == 31) warp_sums[warp] = x;
-  __syncthreads();
-  if (warp == 0) {
-    int w = warp_sums[lane];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, w, o);
-      if (lane >= o) w += y;
-    }
-    warp_sums[lane] = w;
-  }
-  __syncthreads();
-  *total = warp_sums[31];
-  return x - value + (warp > 0 ? warp_sums[warp - 1] : 0);
 }
 
 // Lists the first `wanted` free pages, lowest first, into `list`; returns how many there are (at most `wanted`).
