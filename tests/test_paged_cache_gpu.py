@@ -415,3 +415,15 @@ def test_rows_are_the_pages_token_rows():
     out = cache.attend(1, batch, q)
     want = attend(q, k[None], v[None], torch.zeros(1, 1, dtype=torch.int32, device="cuda"), [40], [40])[0]
     assert float((out.double() - want).norm() / want.norm()) < 1e-2
+
+
+def test_example_decodes_token_by_token():
+    """Forked sessions that append and attend a token at a time against one pass over each whole sequence; the tails of 100
+    prompt tokens (7 pages of 16) are copied, 12 tokens take a page more at most."""
+    path = Path(__file__).resolve().parents[1] / "examples" / "paged_sessions.py"
+    spec = importlib.util.spec_from_file_location("paged_sessions", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    for heads, kv_heads, branches in ((8, 2, 3), (4, 4, 1)):
+        difference, beyond = module.decode(heads=heads, kv_heads=kv_heads, branches=branches)
+        assert difference < 2e-2 and beyond == branches
