@@ -71,7 +71,23 @@ std::pair<at::Tensor, c10::optional<at::Tensor>> paged_attention(
     const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
     const at::Tensor& kv_lens, const at::Tensor& cu_q, int64_t max_q_len, bool causal, int64_t window, int64_t sinks,
     c10::optional<double> scale, bool want_lse, const c10::optional<at::Tensor>& out_given,
-    const c10::optional<at::Tensor>& status);
+    const c10::optional<at::Tensor>& status, const c10::optional<at::Tensor>& k_scales, const c10::optional<at::Tensor>& v_scales);
+at::Tensor packed_append(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& positions,
+                         const RopePlan& plan, const at::Tensor& k_codes, const at::Tensor& k_scales, const at::Tensor& v_codes,
+                         const at::Tensor& v_scales, const at::Tensor& table, const at::Tensor& kv_lens, const at::Tensor& cu_q,
+                         const c10::optional<at::Tensor>& out, const c10::optional<at::Tensor>& status);
+void packed_store(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_codes, const at::Tensor& k_scales,
+                  const at::Tensor& v_codes, const at::Tensor& v_scales, const at::Tensor& table, const at::Tensor& kv_lens,
+                  const at::Tensor& cu_q, const c10::optional<at::Tensor>& status);
+std::pair<at::Tensor, at::Tensor> packed_read(const at::Tensor& k_codes, const at::Tensor& k_scales, const at::Tensor& v_codes,
+                                              const at::Tensor& v_scales, const at::Tensor& table, const at::Tensor& starts,
+                                              int64_t rows, at::ScalarType type, const c10::optional<at::Tensor>& status);
+void paged_block_means(const at::Tensor& k_pages, const c10::optional<at::Tensor>& k_scales, const at::Tensor& means, const at::Tensor& table,
+                       const at::Tensor& kv_lens, const at::Tensor& cu_q, int64_t max_q_len, const c10::optional<at::Tensor>& status);
+std::tuple<at::Tensor, at::Tensor, at::Tensor> paged_select_blocks(const at::Tensor& q, const at::Tensor& means, const at::Tensor& table,
+                                                                   const at::Tensor& kv_lens, const at::Tensor& cu_q, int64_t block, int64_t keep,
+                                                                   int64_t query_block, int64_t max_q_len, bool causal, int64_t sinks,
+                                                                   int64_t recent, const c10::optional<at::Tensor>& status);
 std::string paged_attention_form(int64_t device, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t seqs,
                                  int64_t width, int64_t page_size, int64_t max_q_len, bool causal, int64_t window, int64_t sinks);
 void pages_allocate(at::Tensor& state, int64_t pages, int64_t seqs_held, int64_t page_size, const at::Tensor& seqs,
@@ -173,7 +189,20 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("paged_attention", &rc::paged_attention, "attention of new tokens over a paged KV cache", py::arg("q"),
         py::arg("k_pages"), py::arg("v_pages"), py::arg("table"), py::arg("kv_lens"), py::arg("cu_q"),
         py::arg("max_q_len"), py::arg("causal"), py::arg("window"), py::arg("sinks"), py::arg("scale"),
-        py::arg("want_lse"), py::arg("out"), py::arg("status"));
+        py::arg("want_lse"), py::arg("out"), py::arg("status"), py::arg("k_scales") = py::none(), py::arg("v_scales") = py::none());
+  m.def("packed_append", &rc::packed_append, "rotate q, write rotated k and v into their pages in 8 bits", py::arg("q"), py::arg("k"),
+        py::arg("v"), py::arg("positions"), py::arg("plan"), py::arg("k_codes"), py::arg("k_scales"), py::arg("v_codes"),
+        py::arg("v_scales"), py::arg("table"), py::arg("kv_lens"), py::arg("cu_q"), py::arg("out"), py::arg("status"));
+  m.def("packed_store", &rc::packed_store, "write k and v into their pages in 8 bits", py::arg("k"), py::arg("v"), py::arg("k_codes"),
+        py::arg("k_scales"), py::arg("v_codes"), py::arg("v_scales"), py::arg("table"), py::arg("kv_lens"), py::arg("cu_q"),
+        py::arg("status"));
+  m.def("packed_read", &rc::packed_read, "rows of sequences out of pages in 8 bits", py::arg("k_codes"), py::arg("k_scales"),
+        py::arg("v_codes"), py::arg("v_scales"), py::arg("table"), py::arg("starts"), py::arg("rows"), py::arg("type"), py::arg("status"));
+  m.def("paged_block_means", &rc::paged_block_means, "means of the keys of the blocks that hold new tokens", py::arg("k_pages"),
+        py::arg("k_scales"), py::arg("means"), py::arg("table"), py::arg("kv_lens"), py::arg("cu_q"), py::arg("max_q_len"), py::arg("status"));
+  m.def("paged_select_blocks", &rc::paged_select_blocks, "the blocks that each block of queries attends to", py::arg("q"), py::arg("means"),
+        py::arg("table"), py::arg("kv_lens"), py::arg("cu_q"), py::arg("block"), py::arg("keep"), py::arg("query_block"),
+        py::arg("max_q_len"), py::arg("causal"), py::arg("sinks"), py::arg("recent"), py::arg("status"));
   m.def("paged_attention_form", &rc::paged_attention_form, "the form of the kernels that a call of these sizes takes",
         py::arg("device"), py::arg("tokens"), py::arg("heads"), py::arg("kv_heads"), py::arg("head_dim"), py::arg("seqs"),
         py::arg("width"), py::arg("page_size"), py::arg("max_q_len"), py::arg("causal") = false, py::arg("window") = 0,

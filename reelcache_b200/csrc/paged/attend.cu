@@ -13,6 +13,7 @@
 #include <utility>
 
 #include "attend.cuh"
+#include "packed.h"
 
 namespace rc {
 namespace paged {
@@ -23,6 +24,10 @@ void attend_short(const Args& a, int head_dim, bool half, const at::Tensor& k_pa
                   int max_q_len, const at::Tensor& like, cudaStream_t stream, int device);
 void attend_chunk(const Args& a, int head_dim, bool half, const at::Tensor& k_pages, const at::Tensor& v_pages,
                   int max_q_len, const at::Tensor& like, cudaStream_t stream, int device);
+void attend_packed_short(const Args& a, int head_dim, bool half, const at::Tensor& k_codes, const at::Tensor& v_codes, const Packed& k,
+                         const Packed& v, const at::Tensor& like, cudaStream_t stream, int device);
+void expand_pages(Args& a, const at::Tensor& k_codes, const at::Tensor& v_codes, const Packed& k, const Packed& v, at::Tensor& k_pages,
+                  at::Tensor& v_pages, at::Tensor& workspace, const at::Tensor& like, cudaStream_t stream);
 std::string short_form_name(const Args& a, int head_dim, int device);
 std::string chunk_form_name(const Args& a, int head_dim, int max_q_len, int device);
 
@@ -51,13 +56,13 @@ std::string paged_attention_form(int64_t device, int64_t tokens, int64_t heads, 
 }
 
 // out = softmax over the visible keys of scale * q k^T, times v, for the new tokens of every sequence; lse its natural
-// log-sum-exp. max_q_len bounds every sequence's new tokens (more are reported); rows of q that no sequence names are left
+// log-sum-exp. The pages are of q's type, or e4m3 codes with scales. max_q_len bounds every sequence's new tokens (more are reported); rows of q that no sequence names are left
 // alone.
 std::pair<at::Tensor, c10::optional<at::Tensor>> paged_attention(
     const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
     const at::Tensor& kv_lens, const at::Tensor& cu_q, int64_t max_q_len, bool causal, int64_t window, int64_t sinks,
     c10::optional<double> scale_given, bool want_lse, const c10::optional<at::Tensor>& out_given,
-    const c10::optional<at::Tensor>& status) {
+    const c10::optional<at::Tensor>& status, const c10::optional<at::Tensor>& k_scales, const c10::optional<at::Tensor>& v_scales) {
   check_cuda_tensor(q, "q");
   refuse_gradients({&q, &k_pages, &v_pages}, "attention over pages");
   if (out_given.has_value()) refuse_gradients({&*out_given}, "attention over pages");
@@ -77,15 +82,29 @@ std::pair<at::Tensor, c10::optional<at::Tensor>> paged_attention(
     RC_CHECK(t->numel() == 0 || (t->stride(2) == 1 && t->stride(0) % 8 == 0 && t->stride(1) % 8 == 0 &&
                                  reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0),
              "rows must have unit inner stride and 16-byte aligned strides and base");
-  RC_CHECK(k_pages.device() == q.device() && v_pages.device() == q.device() && k_pages.scalar_type() == type &&
-               v_pages.scalar_type() == type && k_pages.dim() == 4,
+  const bool packed = k_scales.has_value();
+  RC_CHECK(packed == v_scales.has_value(), "both or neither of k_pages and v_pages must be packed");
+  RC_CHECK(k_pages.dim() == 4 && (packed || (k_pages.device() == q.device() && v_pages.device() == q.device() &&
+                                            k_pages.scalar_type() == type && v_pages.scalar_type() == type)),
            "the pages must have the type and device of q");
   const int64_t kv_heads = k_pages.size(2);
   RC_CHECK(kv_heads >= 1 && q.size(1) % kv_heads == 0 && q.size(1) >= kv_heads, "heads must be a multiple of the KV heads");
-  const paged::Pages kp = paged::check_pages(k_pages, kv_heads, q.size(2), "k_pages");
-  const paged::Pages vp = paged::check_pages(v_pages, kv_heads, q.size(2), "v_pages");
-  RC_CHECK(kp.count == vp.count && kp.size == vp.size, "k_pages and v_pages must have the same pages");
-  const paged::Table t = paged::check_table(table, kv_lens, cu_q, q.device());
+  paged::Packed k8{}, v8{};
+  int pages, page_size;
+  if (packed) {
+    k8 = paged::check_packed(k_pages, *k_scales, kv_heads, q.size(2), q.device(), "k_pages");
+    v8 = paged::check_packed(v_pages, *v_scales, kv_heads, q.size(2), q.device(), "v_pages");
+    RC_CHECK(k8.count == v8.count && k8.size == v8.size, "k_pages and v_pages must have the same pages");
+    pages = k8.count;
+    page_size = k8.size;
+  } else {
+    const paged::Pages kp = paged::check_pages(k_pages, kv_heads, q.size(2), "k_pages");
+    const paged::Pages vp = paged::check_pages(v_pages, kv_heads, q.size(2), "v_pages");
+    RC_CHECK(kp.count == vp.count && kp.size == vp.size, "k_pages and v_pages must have the same pages");
+    pages = kp.count;
+    page_size = kp.size;
+  }
+  const paged::Table t = paged::check_table(table, kv_lens, cu_q, q.device(), kv_heads);
   RC_CHECK(window >= 0 && sinks >= 0 && window < (1ll << 31) && sinks < (1ll << 31), "window and sinks must not be negative");
   RC_CHECK(scale > 0.0, "scale must be positive");
   RC_CHECK(max_q_len >= 1 && max_q_len < (1ll << 24), "max_q_len must be positive");
@@ -108,7 +127,8 @@ std::pair<at::Tensor, c10::optional<at::Tensor>> paged_attention(
   a.seqs = t.seqs;
   a.width = t.width;
   a.table_row = t.row;
-  a.pages = kp.count;
+  a.table_head = t.head;
+  a.pages = pages;
   a.heads = static_cast<int>(q.size(1));
   a.kv_heads = static_cast<int>(kv_heads);
   a.group = a.heads / a.kv_heads;
@@ -118,14 +138,23 @@ std::pair<at::Tensor, c10::optional<at::Tensor>> paged_attention(
   a.tokens = static_cast<int>(q.size(0));
   a.max_q_len = static_cast<int>(max_q_len);
   a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
-  a.tiling.page = kp.size;
+  a.tiling.page = page_size;
   a.status = status_ptr(status);
   if (a.tokens == 0 || a.seqs == 0) return {out, lse};
   const int device = q.get_device();
   cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device).stream();
   const int most = static_cast<int>(std::min<int64_t>(max_q_len, a.tokens));
-  const auto attend = static_cast<int64_t>(most) * a.group <= paged::kShortRows ? paged::attend_short : paged::attend_chunk;
-  attend(a, static_cast<int>(q.size(2)), type == at::kHalf, k_pages, v_pages, most, q, stream, device);
+  const bool few = static_cast<int64_t>(most) * a.group <= paged::kShortRows;
+  const int d = static_cast<int>(q.size(2));
+  if (packed && few) {
+    paged::attend_packed_short(a, d, type == at::kHalf, k_pages, v_pages, k8, v8, q, stream, device);
+  } else if (packed) {
+    at::Tensor k16, v16, workspace;
+    paged::expand_pages(a, k_pages, v_pages, k8, v8, k16, v16, workspace, q, stream);
+    paged::attend_chunk(a, d, type == at::kHalf, k16, v16, most, q, stream, device);
+  } else {
+    (few ? paged::attend_short : paged::attend_chunk)(a, d, type == at::kHalf, k_pages, v_pages, most, q, stream, device);
+  }
   if (out_given.has_value()) written(out);
   return {out, lse};
 }

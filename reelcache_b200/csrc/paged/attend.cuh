@@ -38,6 +38,7 @@ struct Args {
   const int* cu_q;
   int seqs, width, pages;
   int64_t table_row;  // elements from one sequence's row of the table to the next
+  int64_t table_head;  // and from one KV head's to the next (0: the heads share it)
   int heads, kv_heads, group;
   int causal, window, sinks;  // window 0: no window
   int tokens, max_q_len;
@@ -209,17 +210,18 @@ struct PageMaps {
   CUtensorMap k_wide, v_wide, k_step, v_step;
 };
 
-inline PageMaps page_maps(const at::Tensor& k, const at::Tensor& v, const Tiling& t, int rows) {
+inline PageMaps page_maps(const at::Tensor& k, const at::Tensor& v, const Tiling& t, int rows,
+                          CUtensorMap (*map_of)(const at::Tensor&, int) = page_map) {
   PageMaps maps;
   // a box may not be larger than the page it is cut from: without whole tiles in a page the wide maps are not used
   const bool wide = t.page >= rows, step = t.step < rows;
   if (wide) {
-    maps.k_wide = page_map(k, rows);
-    maps.v_wide = page_map(v, rows);
+    maps.k_wide = map_of(k, rows);
+    maps.v_wide = map_of(v, rows);
   }
   if (step) {
-    maps.k_step = page_map(k, t.step);
-    maps.v_step = page_map(v, t.step);
+    maps.k_step = map_of(k, t.step);
+    maps.v_step = map_of(v, t.step);
   }
   if (!wide) {
     maps.k_wide = maps.k_step;

@@ -534,7 +534,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         const Sight sight(a, seg.item.kv_len, seg.item.q_len);
         const TileRange<kTile> range(sight, rows.first, rows.end);
         const int low = sight.low(sight.last(rows.first)), top = min(sight.last(rows.end - 1), seg.item.kv_len - 1);
-        const int* table = a.table + seg.item.seq * a.table_row;
+        const int* table = a.table + seg.item.seq * a.table_row + seg.item.head * a.table_head;
         for (int t = seg.t0; t < seg.t1; ++t) {
           const int first = range.tile(t) * kTile;
           const Boxes<kTile> boxes(a.tiling, first, seg.item.kv_len);

@@ -83,11 +83,12 @@ struct Pages {  // [pages, page_size, kv_heads, head_dim], strides in elements
 };
 
 struct Table {
-  const int* table;    // [seqs, width], `row` elements apart
+  const int* table;    // [seqs, width], `row` elements apart, or [seqs, kv_heads, width]
   const int* kv_lens;  // [seqs]
   const int* cu_q;     // [seqs + 1]
   int seqs, width;
   int64_t row;         // elements from one sequence's row to the next
+  int64_t head;        // and from one KV head's to the next (0: the heads share it)
 };
 
 inline Pages check_pages(const at::Tensor& t, int64_t heads, int64_t head_dim, const char* name) {
@@ -102,19 +103,23 @@ inline Pages check_pages(const at::Tensor& t, int64_t heads, int64_t head_dim, c
   return {static_cast<int>(t.size(0)), static_cast<int>(t.size(1)), t.stride(0), t.stride(1), t.stride(2)};
 }
 
+// kv_heads: of a call that takes a table for each KV head too (0: of one that does not).
 inline Table check_table(const at::Tensor& table, const at::Tensor& kv_lens, const at::Tensor& cu_q,
-                         const at::Device& device) {
+                         const at::Device& device, int64_t kv_heads = 0) {
   const at::Tensor* all[3] = {&table, &kv_lens, &cu_q};
   for (const at::Tensor* t : all)
     RC_CHECK(t->device() == device && t->scalar_type() == at::kInt && (t == &table || t->is_contiguous()),
              "block_table, kv_lens and cu_q must be contiguous int32 tensors on the device of q (rows of the table may be "
              "strided)");
-  RC_CHECK(table.dim() == 2 && (table.stride(1) == 1 || table.size(1) <= 1) && table.stride(0) >= 0 && kv_lens.dim() == 1 && cu_q.dim() == 1 && kv_lens.size(0) == table.size(0) &&
-               cu_q.size(0) == table.size(0) + 1,
-           "block_table is [seqs, width], kv_lens [seqs], cu_q [seqs + 1]");
-  RC_CHECK(table.size(0) < (1 << 20) && table.size(1) < (1ll << 31), "too many sequences or pages per sequence");
+  const bool each = kv_heads > 0 && table.dim() == 3 && table.size(1) == kv_heads && table.stride(1) >= 0;
+  const int64_t last = table.dim() - 1;
+  RC_CHECK((table.dim() == 2 || each) && (table.stride(last) == 1 || table.size(last) <= 1) && table.stride(0) >= 0 && kv_lens.dim() == 1 &&
+               cu_q.dim() == 1 && kv_lens.size(0) == table.size(0) && cu_q.size(0) == table.size(0) + 1,
+           kv_heads > 0 ? "block_table is [seqs, width] or [seqs, kv_heads, width], kv_lens [seqs], cu_q [seqs + 1]"
+                        : "block_table is [seqs, width], kv_lens [seqs], cu_q [seqs + 1]");
+  RC_CHECK(table.size(0) < (1 << 20) && table.size(last) < (1ll << 31), "too many sequences or pages per sequence");
   return {table.data_ptr<int>(), kv_lens.data_ptr<int>(), cu_q.data_ptr<int>(), static_cast<int>(table.size(0)),
-          static_cast<int>(table.size(1)), table.stride(0)};
+          static_cast<int>(table.size(last)), table.stride(0), each ? table.stride(1) : 0};
 }
 
 }  // namespace paged

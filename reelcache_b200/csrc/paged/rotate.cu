@@ -26,122 +26,11 @@
 #include <ATen/MemoryOverlap.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 
-#include <algorithm>
-
-#include "../common/host.h"
-#include "paged.h"
-#include "rope_plan.h"
+#include "rotary.cuh"
 
 namespace rc {
 namespace rotary {
-
-constexpr int kThreads = 256;
-
-template <typename T>
-struct Vec;  // one 16-byte vector of T as floats
-
-template <>
-struct Vec<__nv_bfloat16> {
-  static constexpr int n = 8;
-  static __device__ __forceinline__ void unpack(const uint4& u, float* f) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[2 * i] = __uint_as_float(w[i] << 16);
-      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-  }
-  static __device__ __forceinline__ uint4 pack(const float* f) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      __nv_bfloat162 v = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-      w[i] = *reinterpret_cast<uint32_t*>(&v);
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
-  }
-};
-
-template <>
-struct Vec<__half> {
-  static constexpr int n = 8;
-  static __device__ __forceinline__ void unpack(const uint4& u, float* f) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      f[2 * i] = v.x;
-      f[2 * i + 1] = v.y;
-    }
-  }
-  static __device__ __forceinline__ uint4 pack(const float* f) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      __half2 v = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
-      w[i] = *reinterpret_cast<uint32_t*>(&v);
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
-  }
-};
-
-template <>
-struct Vec<float> {
-  static constexpr int n = 4;
-  static __device__ __forceinline__ void unpack(const uint4& u, float* f) {
-    f[0] = __uint_as_float(u.x);
-    f[1] = __uint_as_float(u.y);
-    f[2] = __uint_as_float(u.z);
-    f[3] = __uint_as_float(u.w);
-  }
-  static __device__ __forceinline__ uint4 pack(const float* f) {
-    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
-  }
-};
-
-struct Rows {  // one tensor [tokens, heads, head_dim]: byte strides
-  const char* src;
-  char* dst;
-  int64_t src_token, src_head, dst_token, dst_head;
-  int heads;
-  int per;     // heads of a thread
-  int groups;  // threads that share a token and vector
-};
-
-struct Args {
-  Rows q, k, v;            // v only where pages are written (heads == 0 otherwise)
-  const void* positions;   // [tokens, axes], int32 or float32
-  int position_float;
-  int axes;
-  int ends[4];             // first pair after each axis's section
-  const float* turns;      // [2, pairs]: hi, lo
-  const double* exact;     // [pairs]: the same in FP64
-  float sign;              // -1 turns back
-  int tokens, pairs;
-  // the paged form: k and v rows go to page table[seq][at / page], row at % page
-  const int* table;
-  const int* kv_lens;
-  const int* cu_q;
-  int seqs, table_width, page, pages;
-  int64_t table_row;
-  int64_t page_k, page_v;  // page strides in bytes (dst_token / dst_head are strides inside a page)
-  int* status;
-};
-
-constexpr float kFar = 16777216.0f;  // 2^24: from here on FP32 does not hold every whole number
-
-// The fraction of a turn of pair j at a far position.
-__device__ __forceinline__ float far_part(const Args& a, int token, int j) {
-  const int axis = j < a.ends[0] ? 0 : j < a.ends[1] ? 1 : j < a.ends[2] ? 2 : 3;
-  const int64_t at = static_cast<int64_t>(token) * a.axes + axis;
-  const double p = a.position_float ? static_cast<double>(static_cast<const float*>(a.positions)[at])
-                                    : static_cast<double>(static_cast<const int*>(a.positions)[at]);
-  const double t = __ldg(a.exact + j), n = p * t;
-  return static_cast<float>((n - rint(n)) + fma(p, t, -n));
-}
 
 // kHalves: pairs (j, j + pairs), a thread holds one vector of each half; else neighbours in one vector.
 template <typename T, bool kHalves, bool kPaged, int kHeads>
@@ -178,60 +67,13 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant_
   if (!kPaged || is_q) {
     dst += token * r.dst_token;
   } else {
-    int lo = 0, hi = a.seqs - 1;  // the last sequence that starts at or before the token
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (a.cu_q[mid] <= token) lo = mid;
-      else hi = mid - 1;
-    }
-    const int begin = a.cu_q[lo], end = a.cu_q[lo + 1];
-    if (token < begin || token >= end) return;  // tokens past the last sequence belong to none
-    const int at = a.kv_lens[lo] - end + token;
-    const int slot = at >= 0 ? at / a.page : -1;
-    const int page = slot >= 0 && slot < a.table_width ? a.table[lo * a.table_row + slot] : -1;
-    if (page < 0 || page >= a.pages) {
-      if (vec == 0 && a.status != nullptr) atomicCAS(a.status + kPagedWord, 0, kPageRange);
-      return;
-    }
-    dst += page * (is_k ? a.page_k : a.page_v) + (at - slot * a.page) * r.dst_token;
+    int page, row;
+    if (!place(a, token, vec == 0, &page, &row)) return;
+    dst += page * (is_k ? a.page_k : a.page_v) + row * r.dst_token;
   }
 
   float cs[kPairs], sn[kPairs];
-  if (!kPaged || is_q || is_k) {
-    float p[4];
-    bool far = false;
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      p[x] = 0.0f;
-      if (x < a.axes) {
-        const int64_t at = static_cast<int64_t>(token) * a.axes + x;
-        p[x] = a.position_float ? static_cast<const float*>(a.positions)[at]
-                                : static_cast<float>(static_cast<const int*>(a.positions)[at]);
-        far = far || fabsf(p[x]) >= kFar;
-      }
-    }
-#pragma unroll
-    for (int e0 = 0; e0 < kPairs; e0 += 2) {
-      const int j0 = vec * kPairs + e0;
-      // (the table is written once, long before: the one input that no kernel writes)
-      const float2 hi2 = __ldg(reinterpret_cast<const float2*>(a.turns + j0));
-      const float2 lo2 = __ldg(reinterpret_cast<const float2*>(a.turns + a.pairs + j0));
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int j = j0 + e;
-        const float pos = j < a.ends[0] ? p[0] : j < a.ends[1] ? p[1] : j < a.ends[2] ? p[2] : p[3];
-        const float hi = e ? hi2.y : hi2.x, lo = e ? lo2.y : lo2.x;
-        float part = fmaf(pos, lo, fmaf(pos, hi, -rintf(pos * hi)));
-        if (far) part = far_part(a, token, j);
-        if (sizeof(T) == 4) {
-          sincospif(2.0f * part, &sn[e0 + e], &cs[e0 + e]);
-        } else {
-          __sincosf(6.283185307179586f * part, &sn[e0 + e], &cs[e0 + e]);
-        }
-        sn[e0 + e] *= a.sign;
-      }
-    }
-  }
+  if (!kPaged || is_q || is_k) sines<T>(a, token, vec, cs, sn);
 
   for (int done = 0; done < count; done += kHeads) {
 #pragma unroll
@@ -241,29 +83,12 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant_
 #pragma unroll
       for (int s = 0; s < kParts; ++s) out[s] = raw[i][s];
       if (!kPaged || is_q || is_k) {
-        if (kHalves) {
-          float x[kVec], y2[kVec];
-          Vec<T>::unpack(out[0], x);
-          Vec<T>::unpack(out[kParts - 1], y2);
-#pragma unroll
-          for (int e = 0; e < kVec; ++e) {
-            const float u = x[e] * cs[e % kPairs] - y2[e] * sn[e % kPairs];
-            y2[e] = x[e] * sn[e % kPairs] + y2[e] * cs[e % kPairs];
-            x[e] = u;
-          }
-          out[0] = Vec<T>::pack(x);
-          out[kParts - 1] = Vec<T>::pack(y2);
-        } else {
-          float x[kVec];
-          Vec<T>::unpack(out[0], x);
-#pragma unroll
-          for (int e = 0; e < kVec / 2; ++e) {
-            const float u = x[2 * e] * cs[e] - x[2 * e + 1] * sn[e];
-            x[2 * e + 1] = x[2 * e] * sn[e] + x[2 * e + 1] * cs[e];
-            x[2 * e] = u;
-          }
-          out[0] = Vec<T>::pack(x);
-        }
+        float x[kVec], y2[kVec];
+        Vec<T>::unpack(out[0], x);
+        if (kHalves) Vec<T>::unpack(out[kParts - 1], y2);
+        turn<kHalves>(x, y2, cs, sn);
+        out[0] = Vec<T>::pack(x);
+        if (kHalves) out[kParts - 1] = Vec<T>::pack(y2);
       }
       load(i, done + kHeads + i);  // before the store, which the compiler must take for one to the same memory
 #pragma unroll
@@ -276,15 +101,7 @@ template <typename T, bool kHalves, bool kPaged>
 void launch(Args a, cudaStream_t stream, int sms) {
   const int per_row = a.pairs / (kHalves ? Vec<T>::n : Vec<T>::n / 2);
   const int64_t rows = static_cast<int64_t>(a.tokens) * per_row;
-  const int heads = a.q.heads + a.k.heads + a.v.heads;
-  // Heads of a thread: as many as leave every SM a full set of threads, and then evenly spread over a tensor's threads.
-  const int most = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(64, rows * heads / (static_cast<int64_t>(sms) * 2048))));
-  int widest = 1;
-  for (Rows* r : {&a.q, &a.k, &a.v}) {
-    r->groups = (r->heads + most - 1) / most;
-    r->per = r->groups > 0 ? (r->heads + r->groups - 1) / r->groups : 1;
-    widest = std::max(widest, r->per);
-  }
+  const int widest = spread_heads(a, rows, sms);
   const int64_t blocks = (rows + kThreads - 1) / kThreads;
   const int groups = a.q.groups + a.k.groups + a.v.groups;
   RC_CHECK(blocks < (1ll << 31) && groups < 65536, "too many tokens or heads for one launch");
@@ -304,36 +121,6 @@ void dispatch(const Args& a, at::ScalarType type, bool halves, cudaStream_t stre
   } else if constexpr (!kPaged) {
     halves ? launch<float, true, false>(a, stream, sms) : launch<float, false, false>(a, stream, sms);
   }
-}
-
-// The rotation's part of the arguments, checked: positions [tokens, axes].
-void set_rotation(Args& a, const at::Tensor& positions, const RopePlan& plan, int64_t tokens, int64_t head_dim,
-                  const at::Device& device) {
-  const int axes = static_cast<int>(plan.sections.size());
-  RC_CHECK(head_dim == 2 * plan.pairs, "the rotation is for another head_dim");
-  RC_CHECK(plan.turns.device() == device, "the rotation's table is on another device");
-  a.pairs = static_cast<int>(plan.pairs);
-  int end = 0;
-  for (int i = 0; i < 4; ++i) {
-    if (i < axes) end += static_cast<int>(plan.sections[i]);
-    a.ends[i] = end;
-  }
-  RC_CHECK(positions.device() == device && positions.dim() == 2 && positions.size(0) == tokens &&
-               positions.size(1) == axes && positions.is_contiguous() &&
-               (positions.scalar_type() == at::kInt || positions.scalar_type() == at::kFloat),
-           "positions must be a contiguous int32 or float32 [tokens, axes] tensor on the same device");
-  a.positions = positions.data_ptr();
-  a.position_float = positions.scalar_type() == at::kFloat;
-  a.axes = axes;
-  a.turns = plan.turns.data_ptr<float>();
-  a.exact = plan.exact.data_ptr<double>();
-  a.tokens = static_cast<int>(tokens);
-}
-
-bool vector_rows(const at::Tensor& t) {
-  const int64_t size = t.element_size();
-  return t.dim() == 3 && t.stride(2) == 1 && (t.stride(0) * size) % 16 == 0 && (t.stride(1) * size) % 16 == 0 &&
-         reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
 }
 
 }  // namespace rotary

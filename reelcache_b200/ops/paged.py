@@ -1,5 +1,6 @@
-"""A paged KV cache's operators on sm_100a: writing new tokens (csrc/paged/rotate.cu), attending over the pages
-(attend_short.cu, attend_chunk.cu) and the page table (table.cu).
+"""A paged KV cache's operators on sm_100a: writing new tokens (csrc/paged/rotate.cu, in 8 bits pack.cu), attending over the
+pages (attend_short.cu, attend_chunk.cu, in 8 bits attend_packed.cu and expand.cu), choosing the blocks of sparse attention
+(select.cu) and the page table (table.cu).
 
 Pages: ``k_pages, v_pages [pages, page_size, kv_heads, head_dim]`` of one layer (any 16-byte aligned strides; the page
 size is a multiple of 8 tokens). A batch of sequences is described by ``block_table [seqs, width]`` (page of each block
@@ -8,11 +9,17 @@ of ``page_size`` tokens, -1 for none), ``kv_lens [seqs]`` (tokens held, the new 
 ``table[:, :n]`` will do): nothing is read back, every call can be captured in a graph. Sequence ``s``'s new tokens are
 its last ``cu_q[s + 1] - cu_q[s]`` positions.
 
+Pages may hold their rows in 8 bits (:class:`PackedPages`): :func:`append`, :func:`attention` and :func:`block_means` take
+either kind. Sparse attention is a choice of blocks for every few queries (:func:`select_blocks`) and attention over the
+blocks as pages (:func:`blocks`), with a block table for each KV head.
+
 Calls with page numbers outside the pool, lengths that do not fit their tensors or bounds, or page-table calls that cannot
 be served, do nothing out of bounds and are reported by :func:`reelcache_b200.ops._ext.check_status`.
 """
 
 from __future__ import annotations
+
+from typing import NamedTuple
 
 import torch
 
@@ -21,16 +28,73 @@ from ._ext import ext, status_word
 from .rope import AxisRope
 
 
+class PackedPages(NamedTuple):
+    """K or V pages of one layer in 8 bits: ``codes`` float8_e4m3fn ``[pages, page_size, kv_heads, head_dim]`` and ``scales``
+    float8_e8m0fnu ``[kv_heads, pages, page_size]``; head_dim 64 or 128.
+
+    A row (one token's channels of one KV head) holds ``code * scale``, the scale the smallest power of two that brings the row's
+    largest magnitude to 448 and below, within 2^-124 .. 2^119 (bf16) or 2^-15 .. 2^7 (fp16, whose numbers above 57,344 are
+    held as that): so what a row holds is a number of the 16-bit type that it came in, off by half a step of e4m3 (2^-4 of its size, or
+    2^-10 of the scale where that is more), and reading rounds nothing. A row with a NaN or infinity has a scale of NaN and reads as NaN."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    @classmethod
+    def empty(cls, pages: int, page_size: int, kv_heads: int, head_dim: int, device) -> "PackedPages":
+        """Pages that hold zeros."""
+        codes = torch.zeros(pages, page_size, kv_heads, head_dim, dtype=torch.uint8, device=device)
+        scales = torch.full((kv_heads, pages, page_size), 127, dtype=torch.uint8, device=device)
+        return cls(codes.view(torch.float8_e4m3fn), scales.view(torch.float8_e8m0fnu))
+
+
+def _parts(pages):
+    """Tensor of pages, and its scales where they are packed."""
+    return (pages.codes, pages.scales) if isinstance(pages, PackedPages) else (pages, None)
+
+
+def _both(k_pages, v_pages) -> bool:
+    """Whether the pages are packed (both or neither)."""
+    packed = isinstance(k_pages, PackedPages)
+    if packed != isinstance(v_pages, PackedPages):
+        raise ConfigurationError("both or neither of k_pages and v_pages must be packed")
+    return packed
+
+
 def append(q, k, v, positions, rope: AxisRope, k_pages, v_pages, block_table, kv_lens, cu_q, *, out=None):
     """Rotate ``q[T, heads, D]`` and ``k[T, kv_heads, D]`` at ``positions[T, axes]`` and write ``k`` and ``v`` into
-    their sequences' pages, in one launch. Returns the rotated ``q`` (``out`` if given). bf16 or fp16."""
+    their sequences' pages, in one launch. Returns the rotated ``q`` (``out`` if given). bf16 or fp16; into packed pages ``k``
+    and ``v`` are quantised from the rotated rows in FP32, in one rounding."""
     if not q.is_cuda:
         raise UnsupportedError("append needs CUDA tensors")
     if q.shape[-1] != rope.head_dim:
         raise ConfigurationError(f"the rotation is for head_dim {rope.head_dim}, q has {q.shape[-1]}")
     device = q.device
+    if _both(k_pages, v_pages):
+        return ext().packed_append(q, k, v, positions, rope.plan(device), *k_pages, *v_pages, block_table, kv_lens, cu_q, out,
+                                   status_word(device))
     return ext().paged_append(q, k, v, positions, rope.plan(device), k_pages, v_pages, block_table, kv_lens, cu_q, out,
                               status_word(device))
+
+
+def store(k, v, k_pages: PackedPages, v_pages: PackedPages, block_table, kv_lens, cu_q):
+    """Write ``k`` and ``v[T, kv_heads, D]`` (bf16 or fp16) as they are into their sequences' packed pages, in one launch."""
+    if not k.is_cuda:
+        raise UnsupportedError("store needs CUDA tensors")
+    if not _both(k_pages, v_pages):
+        raise ConfigurationError("store writes packed pages")
+    ext().packed_store(k, v, *k_pages, *v_pages, block_table, kv_lens, cu_q, status_word(k.device))
+
+
+def read(k_pages: PackedPages, v_pages: PackedPages, block_table, starts, rows: int, *, dtype=torch.bfloat16):
+    """K and V of sequences out of packed pages, dense ``[rows, kv_heads, D]`` in the 16-bit type that they were written from: the first
+    ``starts[s + 1] - starts[s]`` tokens of sequence ``s`` are rows ``starts[s]`` and on (``starts [seqs + 1]`` int32 on the device).
+    Rows of no sequence hold anything."""
+    if not _both(k_pages, v_pages):
+        raise ConfigurationError("read takes packed pages")
+    if not k_pages.codes.is_cuda:
+        raise UnsupportedError("read needs CUDA tensors")
+    return ext().packed_read(*k_pages, *v_pages, block_table, starts, rows, dtype, status_word(k_pages.codes.device))
 
 
 def attention(q, k_pages, v_pages, block_table, kv_lens, cu_q, *, max_q_len: int, causal: bool = False,
@@ -47,13 +111,20 @@ def attention(q, k_pages, v_pages, block_table, kv_lens, cu_q, *, max_q_len: int
     Rows of ``v`` that no new token of the sequence sees may hold anything; one with a NaN or infinity that some see may make
     the outputs of tokens beside them NaN too (a weight of zero times NaN).
     ``max_q_len`` bounds the new tokens of every sequence (more are reported, see the module). Rows of ``q`` outside of
-    ``cu_q`` belong to no sequence: they have no result (a new output holds anything there). ``return_lse`` adds the natural log-sum-exp ``[T, heads]``."""
+    ``cu_q`` belong to no sequence: they have no result (a new output holds anything there). ``return_lse`` adds the natural log-sum-exp ``[T, heads]``.
+
+    ``block_table`` may be ``[seqs, kv_heads, width]``, a table for each KV head. Packed pages give what their rows read as
+    :func:`read` gives, in ``q``'s type; with up to 16 rows (new tokens x heads of a group) the codes are taken as they are and
+    the probabilities are rounded to fp16, with more the pages that are seen are expanded first (16-bit copies of them, for
+    the time of the call)."""
     if not q.is_cuda:
         raise UnsupportedError("paged attention needs CUDA tensors")
     if window is not None and window < 1:
         raise ConfigurationError(f"window {window} must be positive")
+    _both(k_pages, v_pages)
+    (k_pages, k_scales), (v_pages, v_scales) = _parts(k_pages), _parts(v_pages)
     out, lse = ext().paged_attention(q, k_pages, v_pages, block_table, kv_lens, cu_q, max_q_len, causal, window or 0, sinks,
-                                     scale, return_lse, out, status_word(q.device))
+                                     scale, return_lse, out, status_word(q.device), k_scales, v_scales)
     return (out, lse) if return_lse else out
 
 
@@ -63,6 +134,68 @@ def attention_form(tokens, heads, kv_heads, head_dim, seqs, width, page_size, *,
     line"``, ``"twin N"``, ``"direct N"`` (``N`` CTAs to a cluster) or ``"planned"``. ``width``: columns of the block table."""
     return ext().paged_attention_form(device, tokens, heads, kv_heads, head_dim, seqs, width, page_size, max_q_len, causal,
                                       window or 0, sinks)
+
+
+def blocks(pages, block: int):
+    """Pages ``[pages, page_size, kv_heads, D]`` (or packed ones) cut into pages of ``block`` tokens, a view: page ``p`` becomes pages
+    ``p * page_size / block`` and on. ``block`` divides the page size and is a multiple of 8; the pages must lie one after the
+    other."""
+    tensor, scales = _parts(pages)
+    count, size = tensor.shape[:2]
+    if block < 8 or block % 8 or size % block:
+        raise ConfigurationError(f"blocks of {block} tokens must be multiples of 8 and divide the page size, {size}")
+    if count > 1 and tensor.stride(0) != size * tensor.stride(1):
+        raise ConfigurationError("pages that are cut into blocks must lie one after the other")
+    tensor = tensor.as_strided((count * (size // block), block, *tensor.shape[2:]), (block * tensor.stride(1), *tensor.stride()[1:]))
+    if scales is None:
+        return tensor
+    if count > 1 and scales.stride(1) != size:
+        raise ConfigurationError("pages that are cut into blocks must lie one after the other")
+    return PackedPages(tensor, scales.as_strided((scales.shape[0], count * (size // block), block), (scales.stride(0), block, 1)))
+
+
+def block_means(k_pages, means, block_table, kv_lens, cu_q, *, max_q_len: int):
+    """Bring the means of the keys of blocks up to date after new tokens were written: those of the blocks that hold the last
+    ``cu_q[s + 1] - cu_q[s]`` tokens of every sequence, over the tokens that they hold. ``means [pages, page_size / block,
+    kv_heads, D]`` of the pages' type (of packed pages bf16 or fp16) lie beside the pages. Sums are in FP64."""
+    tensor, scales = _parts(k_pages)
+    if not tensor.is_cuda:
+        raise UnsupportedError("block_means needs CUDA tensors")
+    ext().paged_block_means(tensor, scales, means, block_table, kv_lens, cu_q, max_q_len, status_word(tensor.device))
+    return means
+
+
+class ChosenBlocks(NamedTuple):
+    """A batch for :func:`attention` over :func:`blocks`: every query block is a sequence of its own. ``table [items, kv_heads,
+    width]`` (-1 behind the chosen blocks), ``kv_lens [items]``, ``cu_q [items + 1]``; ``max_q_len`` new tokens at most."""
+
+    table: torch.Tensor
+    kv_lens: torch.Tensor
+    cu_q: torch.Tensor
+    max_q_len: int
+
+
+def select_blocks(q, means, block_table, kv_lens, cu_q, *, block: int, keep: int, max_q_len: int, query_block: int = 1,
+                  causal: bool = False, sinks: int = 0, recent: int = 0) -> ChosenBlocks:
+    """Choose the blocks of ``block`` positions that the new tokens ``q[T, heads, D]`` attend to, for every ``query_block`` of them
+    (consecutive tokens of a sequence; 1: each its own) and KV head: the ``keep`` blocks of the past that score highest, and always those that
+    hold the first ``sinks`` positions, the ``recent`` positions before the new tokens, and the new tokens (``causal``: before and up
+    to those of the query block).
+
+    A block's score is the largest over the heads of the group of the sum of the query block's ``q`` times the mean of the
+    block's keys (``means`` from :func:`block_means`), in FP64: the choice does not depend on the order of sums. Equal scores go to the lower block; a
+    score of NaN comes last. Attention over the choice (its tables name the past in order, the query block's own tokens
+    last, so that ``causal`` holds there)::
+
+        chosen = select_blocks(q, means, block_table, kv_lens, cu_q, block=64, keep=16, max_q_len=n, causal=True)
+        out = attention(q, blocks(k_pages, 64), blocks(v_pages, 64), chosen.table, chosen.kv_lens, chosen.cu_q,
+                        max_q_len=chosen.max_q_len, causal=True)
+    """
+    if not q.is_cuda:
+        raise UnsupportedError("the choice of blocks needs CUDA tensors")
+    table, lens, cu = ext().paged_select_blocks(q, means, block_table, kv_lens, cu_q, block, keep, query_block, max_q_len, causal,
+                                                sinks, recent, status_word(q.device))
+    return ChosenBlocks(table, lens, cu, min(query_block, max_q_len))
 
 
 def copy_pages(storage, source, target, rows=None):
