@@ -25,7 +25,7 @@ void attend_short(const Args& a, int head_dim, bool half, const at::Tensor& k_pa
 void attend_chunk(const Args& a, int head_dim, bool half, const at::Tensor& k_pages, const at::Tensor& v_pages,
                   int max_q_len, const at::Tensor& like, cudaStream_t stream, int device);
 void attend_packed_short(const Args& a, int head_dim, bool half, const at::Tensor& k_codes, const at::Tensor& v_codes, const Packed& k,
-                         const Packed& v, const at::Tensor& like, cudaStream_t stream, int device);
+                         const Packed& v, int max_q_len, const at::Tensor& like, cudaStream_t stream, int device);
 void expand_pages(Args& a, const at::Tensor& k_codes, const at::Tensor& v_codes, const Packed& k, const Packed& v, at::Tensor& k_pages,
                   at::Tensor& v_pages, at::Tensor& workspace, const at::Tensor& like, cudaStream_t stream);
 std::string short_form_name(const Args& a, int head_dim, int device);
@@ -147,7 +147,7 @@ std::pair<at::Tensor, c10::optional<at::Tensor>> paged_attention(
   const bool few = static_cast<int64_t>(most) * a.group <= paged::kShortRows;
   const int d = static_cast<int>(q.size(2));
   if (packed && few) {
-    paged::attend_packed_short(a, d, type == at::kHalf, k_pages, v_pages, k8, v8, q, stream, device);
+    paged::attend_packed_short(a, d, type == at::kHalf, k_pages, v_pages, k8, v8, most, q, stream, device);
   } else if (packed) {
     at::Tensor k16, v16, workspace;
     paged::expand_pages(a, k_pages, v_pages, k8, v8, k16, v16, workspace, q, stream);

@@ -1,21 +1,24 @@
 // Attention of few query rows (single tokens, drafts) over pages in 8 bits (packed.h), for sm_100a.
 //
-// What bounds it: reading the codes once, half the bytes of a 16-bit cache in the same time per product, so the design of
+// What bounds it: reading the codes once, half the bytes of a 16-bit cache in the same time per product, so the frame of
 // attend_short.cu is kept (a producer warp streams tiles of 64 keys with TMA, four consumer warps with 16 keys each on
-// mma.sync, work in a line or in clusters) and what comes between the bytes and the products is kept short:
+// mma.sync, work in a line or in clusters) and what comes between the bytes and the products is kept short.
+//
+// Products are transposed: S^T = K Q^T and O^T = V^T P^T have keys and channels in the 16 rows of the instruction and the queries in its 8
+// columns, so that up to 8 rows (a single token's group of heads) take one instruction where Q K^T would take two, half empty.
+// P^T comes out of S^T's layout by a transposition of 8 x 8 numbers (movmatrix).
 //
 // Codes become fp16 in registers, exactly, two by one conversion; the products are fp16 whatever the rows' type. Q is brought
 // to fp16 by a power of two for each row that puts its largest magnitude between 2^6 and 2^7: exact for what is at least 2^-20
-// of that, off by at most 2^-31 of it below. Scales multiply neither codes nor channels: K's multiply the scores (FP32),
-// V's multiply the probabilities, which are rounded to fp16 for the product (half a step of 2^-11; their sum is not): a warp
-// keeps the largest exponent of V's scales that it has seen as the unit of its output, so that no product overflows, and
-// rescales the output when it grows, as with the maximum of the scores.
+// of that, off by at most 2^-31 of it below. Scales multiply neither codes nor channels: K's multiply the scores (FP32), V's
+// multiply the probabilities, which are rounded to fp16 for the product (half a step of 2^-10; their sum is not): a warp keeps the
+// largest scale of V that it has seen as the unit of its output, so that no product overflows. Maximum and unit move
+// rarely, each after a vote: the maximum when a score is more than 2^8 above it, the unit when a scale is.
 //
-// Fragments without shuffles: a row of K lies as 16 bytes a chunk; ldmatrix hands a lane four consecutive channels of a key,
-// taken as its pairs (2 t, 2 t + 1) and (2 t + 8, 2 t + 9) of the product's inner index: any order of channels gives the same sum,
-// and Q is read in that order. Of V, transposed, a lane gets two neighbouring channels of two keys, which two byte
-// permutations (over two registers) part into the even and the odd channel's product; a lane's outputs are then four
-// consecutive channels.
+// Fragments without shuffles: ldmatrix hands a lane four consecutive channels of a key, taken as the pairs (2 t, 2 t + 1) and (2 t +
+// 8, 2 t + 9) of the product's inner index: any order of channels gives the same sum, and Q is read in that order. Of V,
+// transposed, a lane gets two neighbouring channels of two keys, which two byte permutations (over two registers) part into
+// the rows r and r + 8 of the product: a lane's outputs are two consecutive channels.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -55,11 +58,16 @@ __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
   return D == 128 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
 }
 
-// 2^(e - base) of a scale byte as the factor of a probability; e above base never comes.
-__device__ __forceinline__ float relative_scale(int e, int base) {
-  const int d = 127 + e - base;
-  return e == kNanScale ? __uint_as_float(0x7fffffffu) : d <= 0 ? 0.0f : __uint_as_float(static_cast<uint32_t>(d) << 23);
+// 2^(e - base) of a scale byte not above base. (A scale of NaN is above all others: what then is in its units is NaN.)
+__device__ __forceinline__ float relative_scale(int e, int base) { return __uint_as_float(static_cast<uint32_t>(max(127 + e - base, 0)) << 23); }
+
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
+  uint32_t out;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(out) : "r"(v));
+  return out;
 }
+
+constexpr float kFewRescale = 8.0f;  // log2
 
 template <typename T>
 __device__ __forceinline__ float2 two_of(uint32_t v);
@@ -70,7 +78,8 @@ __device__ __forceinline__ float2 two_of<__nv_bfloat16>(uint32_t v) {
 template <>
 __device__ __forceinline__ float2 two_of<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
 
-template <typename T, int D, bool kCluster>
+// kN: groups of eight rows, 1 or 2.
+template <typename T, int D, bool kCluster, int kN>
 __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
     packed_short_kernel(const __grid_constant__ PageMaps maps, const __grid_constant__ PackedShort ps) {
   using Shape = PackedShape<D>;
@@ -196,7 +205,9 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
 
   // ---------------- consumers ----------------
   const int kg = warp;  // its keys
-  const int r0 = lane >> 2, quad = lane & 3, c0 = quad * 2;
+  const int r0 = lane >> 2, quad = lane & 3;
+  // this lane's operand rows for ldmatrix: keys 0-7 and 8-15 of the warp's, of two chunks
+  const int key_row = kg * kKeys + (lane & 15), chunk = lane >> 4;
   bool ok = true;
   for (int at = begin; kCluster || at < end;) {  // a cluster's CTA goes round once, also without tiles
     const SeqWork w(a, s);
@@ -212,32 +223,27 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
     const Sight sight(a, w.kv_len, w.q_len);
     const TileRange<kShortTile> range(sight, 0, w.q_len);
 
-    // this thread's two rows, channels 16 j + 4 quad + 0 .. 3
-    int row_q[2], row_h[2], last[2], low[2];
-    bool valid[2];
-    float row_scale[2];  // of a raw score, with log2(e)
-    uint32_t q[D / 16][4];
+    // Q as the right operand: row r0 of each group of eight, channels 16 c + 4 quad + 0 .. 3
+    uint32_t q[kN][D / 16][2];
+    float row_scale[kN][2];  // of the raw scores of rows 2 quad, 2 quad + 1, with log2(e)
+    int last[kN][2], low[kN][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int row = r0 + i * 8;
-      row_q[i] = row / a.group;
-      row_h[i] = head * a.group + row - row_q[i] * a.group;
-      valid[i] = row_q[i] < w.q_len;
-      last[i] = sight.last(min(row_q[i], w.q_len - 1));
-      low[i] = sight.low(last[i]);
-      const T* src = static_cast<const T*>(a.q) + static_cast<int64_t>(w.q_first + row_q[i]) * a.q_token + row_h[i] * a.q_head + quad * 4;
-#pragma unroll
-      for (int j = 0; j < D / 16; ++j) {
-        const uint2 x = valid[i] ? *reinterpret_cast<const uint2*>(src + j * 16) : make_uint2(0u, 0u);
-        q[j][i] = x.x;
-        q[j][i + 2] = x.y;
-      }
+    for (int g = 0; g < kN; ++g) {
+      const int row = g * 8 + r0, query = row / a.group, h = head * a.group + row - query * a.group;
+      const bool valid = query < w.q_len;
+      const T* src = static_cast<const T*>(a.q) + static_cast<int64_t>(w.q_first + query) * a.q_token + h * a.q_head + quad * 4;
       float top = 0.0f;
 #pragma unroll
-      for (int j = 0; j < D / 16; ++j)
+      for (int c = 0; c < D / 16; ++c) {
+        const uint2 x = valid ? *reinterpret_cast<const uint2*>(src + c * 16) : make_uint2(0u, 0u);
+        q[g][c][0] = x.x;
+        q[g][c][1] = x.y;
+      }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float2 f = two_of<T>(q[j][i + 2 * h]);
+      for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float2 f = two_of<T>(q[g][c][i]);
           top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
         }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -245,136 +251,147 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
       // 2^(6 - e) for a largest magnitude of 2^e and above (e within what leaves both factors numbers)
       const int e = max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -120);
       const float up = __uint_as_float(static_cast<uint32_t>(127 + 6 - e) << 23);
-      row_scale[i] = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - 6 + e) << 23);
+      const float scale = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - 6 + e) << 23);
 #pragma unroll
-      for (int j = 0; j < D / 16; ++j)
+      for (int c = 0; c < D / 16; ++c)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float2 f = two_of<T>(q[j][i + 2 * h]);
-          q[j][i + 2 * h] = pack_f16x2(f.x * up, f.y * up);
+        for (int i = 0; i < 2; ++i) {
+          const float2 f = two_of<T>(q[g][c][i]);
+          q[g][c][i] = pack_f16x2(f.x * up, f.y * up);
         }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        row_scale[g][i] = __shfl_sync(0xffffffffu, scale, (2 * quad + i) * 4);
+        last[g][i] = sight.last(min((g * 8 + 2 * quad + i) / a.group, w.q_len - 1));
+        low[g][i] = sight.low(last[g][i]);
+      }
     }
     const int rows_here = w.q_len * a.group;  // or fewer: kRows
     // bounds over the queries, for tiles that need no mask
     const int all_last = sight.last(0), all_low = sight.low(sight.last(w.q_len - 1));
     const int any_low = sight.low(all_last);
 
-    float o[D / 8][4];  // products: 2 j the even channels of chunk j, 2 j + 1 the odd ones
+    float o[kN][D / 16][4];  // channels 16 c + 2 r0 of rows 2 quad, 2 quad + 1, and the channels after them
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i)
+    for (int g = 0; g < kN; ++g)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-    int unit = 1;  // o is in units of 2^(unit - 127): the largest scale of V so far
+      for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[g][c][e] = 0.0f;
+    float m[kN][2], l[kN][2];  // a maximum that no score is more than 2^8 above; this lane's part of the sum
+#pragma unroll
+    for (int g = 0; g < kN; ++g) {
+      m[g][0] = m[g][1] = -INFINITY;
+      l[g][0] = l[g][1] = 0.0f;
+    }
+    int unit = 0;  // o is in units of 2^(unit - 127): the largest scale of V so far
 
     for (int t = t0; t < t1; ++t) {
       const int first = range.tile(t) * kShortTile;
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, a.status, kTimeoutEpilogue));
       if (ok) {
-        const uint32_t kb = smem_u32(smem + stage * 2 * Shape::tile_bytes);
-        const uint32_t vb = kb + Shape::tile_bytes;
-        // scales of this lane's keys: c0, c0 + 1, c0 + 8, c0 + 9 of the warp's
-        const uint8_t* ks = scales + stage * 2 * kShortTile + kg * kKeys + c0;
-        const uint32_t k2[2] = {*reinterpret_cast<const uint16_t*>(ks), *reinterpret_cast<const uint16_t*>(ks + 8)};
-        const uint32_t v2[2] = {*reinterpret_cast<const uint16_t*>(ks + kShortTile), *reinterpret_cast<const uint16_t*>(ks + kShortTile + 8)};
-        float sc[2][4];
+        const uint32_t kb = smem_u32(smem + stage * 2 * Shape::tile_bytes), vb = kb + Shape::tile_bytes;
+        // scales of this lane's keys r0, r0 + 8 of the warp's
+        const uint8_t* ks = scales + stage * 2 * kShortTile + kg * kKeys + r0;
+        const int k_scale[2] = {ks[0], ks[8]};
+        int v_scale[2] = {ks[kShortTile], ks[kShortTile + 8]};
+        float sc[kN][4];  // keys r0, r0 + 8 (pairs) of rows 2 quad, 2 quad + 1
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int g = 0; g < kN; ++g)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sc[j][e] = 0.0f;
-        // S = Q K^T: matrices (keys 0-7, chunk 2 c), (keys 0-7, 2 c + 1), (keys 8-15, 2 c), (keys 8-15, 2 c + 1)
+          for (int e = 0; e < 4; ++e) sc[g][e] = 0.0f;
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t b[4];
-          ldmatrix_x4(b, kb + chunk_at<D>(kg * kKeys + (lane & 7) + ((lane >> 4) << 3), c * 2 + ((lane >> 3) & 1)));
+        for (int c = 0; c < D / 16; c += 2) {
+          uint32_t b[4];  // keys 0-7 and 8-15 of chunk c, and of chunk c + 1
+          ldmatrix_x4(b, kb + chunk_at<D>(key_row, c + chunk));
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            mma_16816(sc[e >> 1], q[2 * c + (e & 1)], codes_to_half2(b[e]), upper_codes_to_half2(b[e]), __half());
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t k4[4] = {codes_to_half2(b[2 * i]), codes_to_half2(b[2 * i + 1]), upper_codes_to_half2(b[2 * i]),
+                                    upper_codes_to_half2(b[2 * i + 1])};
+#pragma unroll
+            for (int g = 0; g < kN; ++g) mma_16816(sc[g], k4, q[g][c + i][0], q[g][c + i][1], __half());
+          }
         }
+        const float factor[2] = {scale_value(k_scale[0]), scale_value(k_scale[1])};
+#pragma unroll
+        for (int g = 0; g < kN; ++g)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[g][e] *= factor[e >> 1] * row_scale[g][e & 1];
         const bool whole = first + kShortTile - 1 <= all_last && (first >= all_low || first + kShortTile <= a.sinks);
-        // a key that no query sees counts for nothing: neither its scales (never read, perhaps) nor its codes
-        bool seen[2][2] = {{true, true}, {true, true}};
+        uint32_t keep[2] = {0xffffffffu, 0xffffffffu};  // (of V's operand: keys 2 quad, 2 quad + 1 and those 8 on)
+        if (!whole) {
+          // a key that no query sees counts for nothing: neither its scales (never read, perhaps) nor its codes
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+          for (int i = 0; i < 2; ++i) {
+            const int key = first + kg * kKeys + r0 + 8 * i;
+            if (!(key < w.kv_len && (key >= any_low || key < a.sinks))) v_scale[i] = 0;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int key = first + kg * kKeys + j * 8 + c0 + e;
-            if (!whole) seen[j][e] = key < w.kv_len && (key >= any_low || key < a.sinks);
-            const float factor = scale_value((k2[j] >> (8 * e)) & 0xff);
+            for (int g = 0; g < kN; ++g)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              float& x = sc[j][2 * i + e];
-              x *= factor;
-              if (!whole && !(key <= last[i] && key < w.kv_len && (key >= low[i] || key < a.sinks))) x = -INFINITY;
-            }
-          }
-        int above = 0;
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int byte = (v2[j] >> (8 * e)) & 0xff;
-            if (seen[j][e] && byte != kNanScale) above = max(above, byte);
-          }
-        const int before = unit;
-        unit = max(unit, __reduce_max_sync(0xffffffffu, above));
-        const float grown = relative_scale(before, unit);
-        float alpha[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float mx = fmaxf(fmaxf(sc[0][2 * i], sc[0][2 * i + 1]), fmaxf(sc[1][2 * i], sc[1][2 * i + 1]));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          const float top = fmaxf(m[i], mx * row_scale[i]);
-          const float use = base_of(top);
-          const float faded = fade(m[i], top);
-          m[i] = top;
-          float sum = 0.0f;
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
+              for (int e = 0; e < 2; ++e)
+                if (!(key <= last[g][e] && key < w.kv_len && (key >= low[g][e] || key < a.sinks))) sc[g][2 * i + e] = -INFINITY;
+            keep[i] = 0;
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const float x = exp2_approx(fmaf(sc[j][2 * i + e], row_scale[i], -use));
-              sc[j][2 * i + e] = x;
-              sum += x;
+              const int of = first + kg * kKeys + 2 * quad + e + 8 * i;
+              if (of < w.kv_len && (of >= any_low || of < a.sinks)) keep[i] |= 0xffffu << (16 * e);
             }
-          l[i] = l[i] * faded + sum;
-          alpha[i] = faded * grown;
-        }
-        if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
-#pragma unroll
-          for (int i = 0; i < D / 8; ++i) {
-            o[i][0] *= alpha[0];
-            o[i][1] *= alpha[0];
-            o[i][2] *= alpha[1];
-            o[i][3] *= alpha[1];
           }
         }
-        uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+        bool grows = max(v_scale[0], v_scale[1]) > unit;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int g = 0; g < kN; ++g)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float factor = seen[j][e] ? relative_scale((v2[j] >> (8 * e)) & 0xff, unit) : 0.0f;
-            sc[j][e] *= factor;
-            sc[j][2 + e] *= factor;
-          }
-          if (!whole) keep[j] = (seen[j][0] ? 0xffffu : 0u) | (seen[j][1] ? 0xffff0000u : 0u);
+          for (int e = 0; e < 2; ++e) grows = grows || fmaxf(sc[g][e], sc[g][2 + e]) > m[g][e] + kFewRescale;
+        if (__any_sync(0xffffffffu, grows)) {
+          const int before = unit;
+          unit = max(unit, __reduce_max_sync(0xffffffffu, max(v_scale[0], v_scale[1])));
+          const float grown = relative_scale(before, unit);
+#pragma unroll
+          for (int g = 0; g < kN; ++g)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float top = fmaxf(sc[g][e], sc[g][2 + e]);
+#pragma unroll
+              for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+              top = fmaxf(top, m[g][e]);
+              const float faded = fade(m[g][e], top);
+              m[g][e] = top;
+              l[g][e] *= faded;
+#pragma unroll
+              for (int c = 0; c < D / 16; ++c) {
+                o[g][c][e] *= faded * grown;
+                o[g][c][2 + e] *= faded * grown;
+              }
+            }
         }
-        const uint32_t pa[4] = {pack_f16x2(sc[0][0], sc[0][1]), pack_f16x2(sc[0][2], sc[0][3]), pack_f16x2(sc[1][0], sc[1][1]),
-                                pack_f16x2(sc[1][2], sc[1][3])};
-        // O += P V: matrices (keys 0-7, chunk 2 c), (keys 8-15, 2 c), (keys 0-7, 2 c + 1), (keys 8-15, 2 c + 1); codes of keys
-        // that no query sees are taken as zeros whatever they are: 0 * NaN is NaN
+        // P^T, and with V's scales in fp16 as the right operand
+        const float v_factor[2] = {relative_scale(v_scale[0], unit), relative_scale(v_scale[1], unit)};
+        uint32_t pb[kN][2];
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
+        for (int g = 0; g < kN; ++g) {
+          const float use[2] = {base_of(m[g][0]), base_of(m[g][1])};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            sc[g][e] = exp2_approx(sc[g][e] - use[e & 1]);
+            l[g][e & 1] += sc[g][e];
+            sc[g][e] *= v_factor[e >> 1];
+          }
+          pb[g][0] = transpose_8x8(pack_f16x2(sc[g][0], sc[g][1]));
+          pb[g][1] = transpose_8x8(pack_f16x2(sc[g][2], sc[g][3]));
+        }
+        // codes of keys that no query sees are taken as zeros whatever they are: 0 * NaN is NaN
+#pragma unroll
+        for (int c = 0; c < D / 16; c += 2) {
           uint32_t b[4];
-          ldmatrix_x4_trans(b, vb + chunk_at<D>(kg * kKeys + (lane & 7) + (((lane >> 3) & 1) << 3), c * 2 + (lane >> 4)));
+          ldmatrix_x4_trans(b, vb + chunk_at<D>(key_row, c + chunk));
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t lower = b[2 * h] & keep[0], upper = b[2 * h + 1] & keep[1];
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t lower = b[2 * i] & keep[0], upper = b[2 * i + 1] & keep[1];
             const uint32_t even = __byte_perm(lower, upper, 0x6420), odd = __byte_perm(lower, upper, 0x7531);
-            mma_16816(o[4 * c + 2 * h], pa, codes_to_half2(even), upper_codes_to_half2(even), __half());
-            mma_16816(o[4 * c + 2 * h + 1], pa, codes_to_half2(odd), upper_codes_to_half2(odd), __half());
+            const uint32_t v4[4] = {codes_to_half2(even), codes_to_half2(odd), upper_codes_to_half2(even), upper_codes_to_half2(odd)};
+#pragma unroll
+            for (int g = 0; g < kN; ++g) mma_16816(o[g][c + i], v4, pb[g][0], pb[g][1], __half());
           }
         }
         __syncwarp();
@@ -385,26 +402,77 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
         phase ^= 1;
       }
     }
+
+    // Warps that split the keys join theirs into key group 0 through shared memory. The same lane of every warp holds the same
+    // rows and channels, so the buffer is laid out by lane.
     const float in_units = scale_value(unit);
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i)
+    for (int g = 0; g < kN; ++g)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[i][e] *= in_units;
-    join_warps<D>(o, m, l, join_ml, smem + Shape::join_off, rows_here);
-    // four consecutive channels of row i of chunk j
-    auto four = [&](int i, int j) { return make_float4(o[2 * j][2 * i], o[2 * j + 1][2 * i], o[2 * j][2 * i + 1], o[2 * j + 1][2 * i + 1]); };
-    if (kCluster) {
-      float* res = reinterpret_cast<float*>(smem);  // [kRows][D]: every tile has been consumed
-      float* res_ml = res + kRows * D;              // [kRows][2]
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l[g][e] += __shfl_xor_sync(0xffffffffu, l[g][e], x);
+        if (r0 == 0) *reinterpret_cast<float2*>(join_ml + (kg * kRows + g * 8 + 2 * quad + e) * 2) = make_float2(m[g][e], l[g][e]);
+      }
+    consumers_sync();
+#pragma unroll
+    for (int g = 0; g < kN; ++g)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float2 ml[kGroups];
+        float top = -INFINITY, total = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kGroups; ++k) {
+          ml[k] = *reinterpret_cast<const float2*>(join_ml + (k * kRows + g * 8 + 2 * quad + e) * 2);
+          top = fmaxf(top, ml[k].x);
+        }
+        const float use = base_of(top);
+#pragma unroll
+        for (int k = 0; k < kGroups; ++k) total = fmaf(ml[k].y, exp2_approx(ml[k].x - use), total);
+        const float weight = exp2_approx(m[g][e] - use) * in_units;
+        m[g][e] = top;
+        l[g][e] = total;
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) {
+          o[g][c][e] *= weight;
+          o[g][c][2 + e] *= weight;
+        }
+      }
+#pragma unroll
+    for (int g = 0; g < kN; ++g) {
+      float4* buf = reinterpret_cast<float4*>(smem + Shape::join_off) + lane;
+      if (kg > 0) {
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) buf[((kg - 1) * (D / 16) + c) * 32] = make_float4(o[g][c][0], o[g][c][1], o[g][c][2], o[g][c][3]);
+      }
       consumers_sync();
       if (kg == 0) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int row = r0 + 8 * i;
+        for (int k = 0; k < kGroups - 1; ++k)
 #pragma unroll
-          for (int j = 0; j < D / 16; ++j) *reinterpret_cast<float4*>(res + row * D + j * 16 + quad * 4) = four(i, j);
-          if (quad == 0) *reinterpret_cast<float2*>(res_ml + row * 2) = make_float2(m[i], l[i]);
-        }
+          for (int c = 0; c < D / 16; ++c) {
+            const float4 x = buf[(k * (D / 16) + c) * 32];
+            o[g][c][0] += x.x;
+            o[g][c][1] += x.y;
+            o[g][c][2] += x.z;
+            o[g][c][3] += x.w;
+          }
+      }
+      consumers_sync();
+    }
+    if (kCluster) {
+      float* res = reinterpret_cast<float*>(smem);  // [kRows][D]: every tile has been consumed
+      float* res_ml = res + kRows * D;              // [kRows][2]
+      if (kg == 0) {
+#pragma unroll
+        for (int g = 0; g < kN; ++g)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int row = g * 8 + 2 * quad + e;
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) *reinterpret_cast<float2*>(res + row * D + c * 16 + 2 * r0) = make_float2(o[g][c][e], o[g][c][2 + e]);
+            if (r0 == 0) *reinterpret_cast<float2*>(res_ml + row * 2) = make_float2(m[g][e], l[g][e]);
+          }
       }
       cluster_sync_all();
       join_few_cluster<T, D>(p, w, head, rows_here, res, res_ml, ok);
@@ -415,44 +483,44 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
       const int item_first = base + head * w.tiles;
       const bool starts = item_first >= begin, ends = item_first + w.tiles <= end;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (!valid[i]) continue;
-        const int64_t token = w.q_first + row_q[i];
-        if (starts && ends) {
-          const float inv = inverse(l[i]);
-          T* dst = static_cast<T*>(a.out) + token * a.out_token + row_h[i] * a.out_head + quad * 4;
+      for (int g = 0; g < kN; ++g)
 #pragma unroll
-          for (int j = 0; j < D / 16; ++j) {
-            const float4 x = four(i, j);
-            *reinterpret_cast<uint2*>(dst + j * 16) = make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
+        for (int e = 0; e < 2; ++e) {
+          const int row = g * 8 + 2 * quad + e, query = row / a.group, h = head * a.group + row - query * a.group;
+          if (query >= w.q_len) continue;
+          const int64_t token = w.q_first + query;
+          if (starts && ends) {
+            const float inv = inverse(l[g][e]);
+            T* dst = static_cast<T*>(a.out) + token * a.out_token + h * a.out_head + 2 * r0;
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) *reinterpret_cast<uint32_t*>(dst + c * 16) = pack2<T>(o[g][c][e] * inv, o[g][c][2 + e] * inv);
+            if (a.lse != nullptr && r0 == 0) a.lse[token * a.heads + h] = log_sum(m[g][e], l[g][e]);
+          } else {
+            const int64_t slot = (2 * static_cast<int64_t>(blockIdx.x) + (starts ? 1 : 0)) * kRows + row;
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) *reinterpret_cast<float2*>(p.part_o + slot * D + c * 16 + 2 * r0) = make_float2(o[g][c][e], o[g][c][2 + e]);
+            if (r0 == 0) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(m[g][e], l[g][e]);
           }
-          if (a.lse != nullptr && quad == 0) a.lse[token * a.heads + row_h[i]] = log_sum(m[i], l[i]);
-        } else {
-          const int64_t slot = (2 * static_cast<int64_t>(blockIdx.x) + (starts ? 1 : 0)) * kRows + r0 + 8 * i;
-#pragma unroll
-          for (int j = 0; j < D / 16; ++j) *reinterpret_cast<float4*>(p.part_o + slot * D + j * 16 + quad * 4) = four(i, j);
-          if (quad == 0) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(m[i], l[i]);
         }
-      }
     }
     at += t1 - t0;
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, int kN>
 struct PackedForm {
   static constexpr int bytes = PackedShape<D>::bytes, tile_bytes = PackedShape<D>::tile_bytes, boxes = 1;
-  static constexpr auto clustered() { return packed_short_kernel<T, D, true>; }
+  static constexpr auto clustered() { return packed_short_kernel<T, D, true, kN>; }
 };
 
-template <typename T, int D>
+template <typename T, int D, int kN>
 void packed_configure(int device) {
   static bool known[64] = {};
   bool& configured = known[device & 63];
   if (configured) return;
-  RC_CUDA(cudaFuncSetAttribute(packed_short_kernel<T, D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, PackedShape<D>::bytes));
-  RC_CUDA(cudaFuncSetAttribute(packed_short_kernel<T, D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, PackedShape<D>::bytes));
-  RC_CUDA(cudaFuncSetAttribute(packed_short_kernel<T, D, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  RC_CUDA(cudaFuncSetAttribute(packed_short_kernel<T, D, false, kN>, cudaFuncAttributeMaxDynamicSharedMemorySize, PackedShape<D>::bytes));
+  RC_CUDA(cudaFuncSetAttribute(packed_short_kernel<T, D, true, kN>, cudaFuncAttributeMaxDynamicSharedMemorySize, PackedShape<D>::bytes));
+  RC_CUDA(cudaFuncSetAttribute(packed_short_kernel<T, D, true, kN>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   configured = true;
 }
 
@@ -461,7 +529,8 @@ CUtensorMap code_map(const at::Tensor& t, int box) {
   CUtensorMap map;
   const cuuint64_t d = static_cast<cuuint64_t>(t.size(3));
   const cuuint64_t dims[4] = {d, static_cast<cuuint64_t>(t.size(1)), static_cast<cuuint64_t>(t.size(2)), static_cast<cuuint64_t>(t.size(0))};
-  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(t.stride(1)), static_cast<cuuint64_t>(t.stride(2)), static_cast<cuuint64_t>(t.stride(0))};
+  const auto stride = [&](int64_t i) { return static_cast<cuuint64_t>(t.size(i) == 1 ? 16 : t.stride(i)); };  // (of one place: any)
+  const cuuint64_t strides[3] = {stride(1), stride(2), stride(0)};
   const cuuint32_t boxes[4] = {static_cast<cuuint32_t>(d), static_cast<cuuint32_t>(box), 1, 1};
   const cuuint32_t ones[4] = {1, 1, 1, 1};
   const CUresult res = encode_tiled_fn()(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, t.data_ptr(), dims, strides, boxes, ones,
@@ -471,7 +540,7 @@ CUtensorMap code_map(const at::Tensor& t, int box) {
   return map;
 }
 
-template <typename T, int D>
+template <typename T, int D, int kN>
 void packed_launch(const Args& a, const at::Tensor& k_codes, const at::Tensor& v_codes, const Packed& k, const Packed& v,
                    const at::Tensor& like, cudaStream_t stream, int device) {
   using Shape = PackedShape<D>;
@@ -486,11 +555,11 @@ void packed_launch(const Args& a, const at::Tensor& k_codes, const at::Tensor& v
   ps.v_scale_page = v.scale_page;
   ps.v_scale_head = v.scale_head;
   const PageMaps maps = page_maps(k_codes, v_codes, p.a.tiling, kShortTile, code_map);
-  packed_configure<T, D>(device);
+  packed_configure<T, D, kN>(device);
   const int64_t items = static_cast<int64_t>(a.seqs) * a.kv_heads, slots = sm_count(device) * kShortCtasPerSm;
-  p.cluster = short_cluster<PackedForm<T, D>>(items, short_tiles(a), p.a.tiling.step, a.seqs > 1, device);
+  p.cluster = short_cluster<PackedForm<T, D, kN>>(items, short_tiles(a), p.a.tiling.step, a.seqs > 1, device);
   if (p.cluster > 0) {
-    launch(packed_short_kernel<T, D, true>, dim3(static_cast<unsigned>(items * p.cluster)), kShortThreads, Shape::bytes, p.cluster,
+    launch(packed_short_kernel<T, D, true, kN>, dim3(static_cast<unsigned>(items * p.cluster)), kShortThreads, Shape::bytes, p.cluster,
            stream, maps, ps);
     return;
   }
@@ -502,18 +571,25 @@ void packed_launch(const Args& a, const at::Tensor& k_codes, const at::Tensor& v
   p.part_ml = p.part_o + 2ll * ctas * kRows * D;
   int* line = reinterpret_cast<int*>(p.part_o + floats);
   p.line = {line, line + 1, line + 1 + a.seqs};
-  launch(packed_short_kernel<T, D, false>, dim3(ctas), kShortThreads, Shape::bytes, 0, stream, maps, ps);
+  launch(packed_short_kernel<T, D, false, kN>, dim3(ctas), kShortThreads, Shape::bytes, 0, stream, maps, ps);
   launch(short_join_kernel<T, D>, dim3(static_cast<unsigned>(items * (kRows / 4))), 128, 0, 0, stream, p);
 }
 
+template <typename T, int D>
+void packed_rows(const Args& a, int max_q_len, const at::Tensor& k_codes, const at::Tensor& v_codes, const Packed& k, const Packed& v,
+                 const at::Tensor& like, cudaStream_t stream, int device) {
+  max_q_len * a.group <= 8 ? packed_launch<T, D, 1>(a, k_codes, v_codes, k, v, like, stream, device)
+                           : packed_launch<T, D, 2>(a, k_codes, v_codes, k, v, like, stream, device);
+}
+
 void attend_packed_short(const Args& a, int head_dim, bool half, const at::Tensor& k_codes, const at::Tensor& v_codes, const Packed& k,
-                         const Packed& v, const at::Tensor& like, cudaStream_t stream, int device) {
+                         const Packed& v, int max_q_len, const at::Tensor& like, cudaStream_t stream, int device) {
   if (head_dim == 128)
-    half ? packed_launch<__half, 128>(a, k_codes, v_codes, k, v, like, stream, device)
-         : packed_launch<__nv_bfloat16, 128>(a, k_codes, v_codes, k, v, like, stream, device);
+    half ? packed_rows<__half, 128>(a, max_q_len, k_codes, v_codes, k, v, like, stream, device)
+         : packed_rows<__nv_bfloat16, 128>(a, max_q_len, k_codes, v_codes, k, v, like, stream, device);
   else
-    half ? packed_launch<__half, 64>(a, k_codes, v_codes, k, v, like, stream, device)
-         : packed_launch<__nv_bfloat16, 64>(a, k_codes, v_codes, k, v, like, stream, device);
+    half ? packed_rows<__half, 64>(a, max_q_len, k_codes, v_codes, k, v, like, stream, device)
+         : packed_rows<__nv_bfloat16, 64>(a, max_q_len, k_codes, v_codes, k, v, like, stream, device);
 }
 
 }  // namespace paged

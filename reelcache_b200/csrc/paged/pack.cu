@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(const __grid_constant__ 
 
   float cs[kPairs], sn[kPairs];
   const bool turned = kTurn != 0 && (is_q || is_k);
-  if (turned) rotary::sines<T>(a, token, vec, cs, sn);
+  if (turned) rotary::sines<true>(a, token, vec, cs, sn);  // (a code that falls to its neighbour is 2^-3 off)
 
   for (int done = 0; done < count; done += kHeads) {
 #pragma unroll

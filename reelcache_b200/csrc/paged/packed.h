@@ -36,15 +36,20 @@ inline Packed check_packed(const at::Tensor& codes, const at::Tensor& scales, in
            who + ": codes must be [pages, page_size, kv_heads, head_dim] with unit inner stride");
   RC_CHECK(codes.size(0) >= 1 && codes.size(0) < (1ll << 31) && codes.size(1) >= 8 && codes.size(1) % 8 == 0 && codes.size(1) <= 65536,
            who + ": the page size must be a multiple of 8 tokens, at most 65536");
-  RC_CHECK(codes.stride(0) % 16 == 0 && codes.stride(1) % 16 == 0 && codes.stride(2) % 16 == 0 &&
-               reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0,
-           who + ": codes must have 16-byte aligned strides and base");
   RC_CHECK(scales.dim() == 3 && scales.size(0) == heads && scales.size(1) == codes.size(0) && scales.size(2) == codes.size(1) &&
-               scales.stride(2) == 1 && scales.stride(0) >= 0 && scales.stride(1) >= 0 && scales.stride(0) % 8 == 0 &&
-               scales.stride(1) % 8 == 0 && reinterpret_cast<uintptr_t>(scales.data_ptr()) % 8 == 0,
-           who + ": scales must be [kv_heads, pages, page_size] with unit inner stride and 8-byte aligned strides and base");
-  return {static_cast<int>(codes.size(0)), static_cast<int>(codes.size(1)), codes.stride(0), codes.stride(1), codes.stride(2),
-          static_cast<const uint8_t*>(scales.data_ptr()), scales.stride(1), scales.stride(0)};
+               scales.stride(2) == 1,
+           who + ": scales must be [kv_heads, pages, page_size] with unit inner stride");
+  // (a dimension of one has any stride: nothing is at its other places)
+  const auto stride = [](const at::Tensor& t, int64_t d, int64_t own) { return t.size(d) == 1 ? own : t.stride(d); };
+  const Packed p{static_cast<int>(codes.size(0)), static_cast<int>(codes.size(1)), stride(codes, 0, 16), stride(codes, 1, 16),
+                 stride(codes, 2, 16), static_cast<const uint8_t*>(scales.data_ptr()), stride(scales, 1, 8), stride(scales, 0, 8)};
+  RC_CHECK(p.page_stride >= 0 && p.page_stride % 16 == 0 && p.token_stride >= 0 && p.token_stride % 16 == 0 && p.head_stride >= 0 &&
+               p.head_stride % 16 == 0 && reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0,
+           who + ": codes must have 16-byte aligned strides and base");
+  RC_CHECK(p.scale_page >= 0 && p.scale_page % 8 == 0 && p.scale_head >= 0 && p.scale_head % 8 == 0 &&
+               reinterpret_cast<uintptr_t>(p.scales) % 8 == 0,
+           who + ": scales must have 8-byte aligned strides and base");
+  return p;
 }
 
 constexpr int kNanScale = 255;

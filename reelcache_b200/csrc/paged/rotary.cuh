@@ -120,8 +120,9 @@ __device__ __forceinline__ float far_part(const Args& a, int token, int j) {
   return static_cast<float>((n - rint(n)) + fma(p, t, -n));
 }
 
-// Sines of the kPairs pairs of a token that begin at vec * kPairs (sn times a.sign).
-template <typename T, int kPairs>
+// Sines of the kPairs pairs of a token that begin at vec * kPairs (sn times a.sign): within a few ULP (kFine), or from the special
+// function unit (within 2^-21).
+template <bool kFine, int kPairs>
 __device__ __forceinline__ void sines(const Args& a, int token, int vec, float (&cs)[kPairs], float (&sn)[kPairs]) {
   float p[4];
   bool far = false;
@@ -148,7 +149,7 @@ __device__ __forceinline__ void sines(const Args& a, int token, int vec, float (
       const float hi = e ? hi2.y : hi2.x, lo = e ? lo2.y : lo2.x;
       float part = fmaf(pos, lo, fmaf(pos, hi, -rintf(pos * hi)));
       if (far) part = far_part(a, token, j);
-      if (sizeof(T) == 4) {
+      if (kFine) {
         sincospif(2.0f * part, &sn[e0 + e], &cs[e0 + e]);
       } else {
         __sincosf(6.283185307179586f * part, &sn[e0 + e], &cs[e0 + e]);

@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant_
   }
 
   float cs[kPairs], sn[kPairs];
-  if (!kPaged || is_q || is_k) sines<T>(a, token, vec, cs, sn);
+  if (!kPaged || is_q || is_k) sines<sizeof(T) == 4>(a, token, vec, cs, sn);
 
   for (int done = 0; done < count; done += kHeads) {
 #pragma unroll

@@ -6,13 +6,16 @@
 // not show, whichever tokens came in which call.
 //
 // The score of a block for the queries of a KV head's group is max over the heads h of (sum over the tokens of the query block
-// of q_h) . mean. Blocks at the border of the choice differ by little, so it is computed in FP64, where the order of a sum
-// moves it by 2^-50 of its size: the choice is that of the exact scores, the same for every batch and form of the kernel.
-// Equal scores go to the lower block.
+// of q_h) . mean. Blocks at the border of the choice differ by little, so the choice is that of scores in FP64, where the order
+// of a sum moves them by 2^-50 of their size: the same for every batch and form of the kernel. Equal scores go to the lower
+// block. Few blocks need FP64: scores come from the tensor core first (the pooled query as the sum of three 16-bit numbers, one for
+// single tokens), together with the sum of their products' magnitudes, which bounds their error (2^-15 of it: 24 steps at most, each a sum
+// of 17 terms cut at 2^-24 of the largest). With T the keep-th largest and E the largest bound, blocks above T + 2 E are chosen and blocks below T - 2 E are not;
+// only the blocks between, where there is more than one way to choose from them, are computed again.
 //
-// One CTA, or a cluster of them that splits the blocks, for every (query block, KV head): pooled queries in shared memory,
-// scores as 64-bit keys that sort like them in the shared memory of the cluster's first CTA, which finds the keep-th largest
-// by digits of eight bits (a histogram each, until a digit's candidates are all taken) and writes the chosen blocks in order.
+// One CTA, or a cluster of them that splits the blocks, for every (query block, KV head): scores as 32-bit keys that sort
+// like them in the shared memory of the cluster's first CTA, which finds the keep-th largest by digits of eight bits (a
+// histogram each, until a digit's candidates are all taken) and writes the chosen blocks in order.
 //
 // What bounds it: the latency of a chain of small steps for few sequences, reading the means for many.
 #include <ATen/ATen.h>
@@ -133,7 +136,8 @@ __global__ void __launch_bounds__(kMeanThreads) means_kernel(const __grid_consta
 
 constexpr int kSelectThreads = 256;
 constexpr int kSelectWarps = kSelectThreads / 32;
-constexpr int kMostBlocks = 24576;  // whose keys fit one CTA's shared memory
+constexpr int kMostBlocks = 12288;  // whose keys fit one CTA's shared memory
+constexpr int kPieces = 3;          // 16-bit numbers that add up to a pooled query
 
 struct Select {
   Args a;              // q, table, lengths, heads; causal; tokens, max_q_len
@@ -147,14 +151,39 @@ struct Select {
   int cluster;
 };
 
-// A number that sorts like the score (both zeros alike).
+// Shared memory of a CTA: pooled queries in FP64 [group][D], their pieces as the products' operand, scales of those, then the
+// keys [blocks] (64 bits), of whose room the first half holds the 32-bit scores and the second half the list of blocks that
+// are computed again... in that order: scores, list, exact keys.
+template <int D>
+struct SelectShape {
+  static constexpr int piece_row = D * 2 + 64;  // bytes: rows 64 bytes apart in the banks
+  int tiles;                                    // groups of eight heads
+  int pieces_off, scale_off, score_off, list_off, exact_off, bytes;
+  __host__ __device__ SelectShape(int group, int blocks) {
+    tiles = (group + 7) / 8;
+    pieces_off = group * D * 8;
+    scale_off = pieces_off + tiles * 8 * kPieces * piece_row;
+    score_off = (scale_off + tiles * 8 * 4 + 15) / 16 * 16;
+    list_off = score_off + (blocks + 3) / 4 * 16;
+    exact_off = list_off + (blocks + 3) / 4 * 16;
+    const int room = kSelectThreads * 64;  // where the parts of the pooled queries meet first
+    const int most = exact_off + blocks * 8;
+    bytes = most > score_off + room ? most : score_off + room;
+  }
+};
+
+// Numbers that sort like scores (both zeros alike).
 __device__ __forceinline__ uint64_t key_of(double score) {
   const uint64_t bits = static_cast<uint64_t>(__double_as_longlong(score + 0.0));
   return (bits >> 63) != 0 ? ~bits : bits | 0x8000000000000000ull;
 }
+__device__ __forceinline__ uint32_t key_of(float score) {
+  const uint32_t bits = __float_as_uint(score + 0.0f);
+  return (bits >> 31) != 0 ? ~bits : bits | 0x80000000u;
+}
 
-__device__ __forceinline__ void store_cluster_u64(uint32_t addr, uint64_t v) {
-  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+__device__ __forceinline__ void store_cluster(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 
 // Exclusive prefix sum over the block's threads and its total.
@@ -179,22 +208,85 @@ __device__ __forceinline__ int select_scan(int value, int* sums, int* total) {
   return before;
 }
 
+// The `rest`-th largest of n keys, digit by digit from the top: its upper bits `prefix` above `shift` (0: all of it), and how many of
+// the keys with that prefix are among the `rest` largest (`rest` comes out as that number).
+template <typename Key, typename Get>
+__device__ __forceinline__ void nth_largest(Get get, int n, Key& prefix, int& shift, int& rest, int* histogram, int* digit, int* sums) {
+  constexpr int kBits = sizeof(Key) * 8;
+  prefix = 0;
+  shift = kBits;
+  while (shift > 0) {
+    for (int i = threadIdx.x; i < 256; i += kSelectThreads) histogram[i] = 0;
+    __syncthreads();
+    for (int c = threadIdx.x; c < n; c += kSelectThreads) {
+      const Key key = get(c);
+      if (shift == kBits || (key >> shift) == prefix) atomicAdd(&histogram[static_cast<int>((key >> (shift - 8)) & 255)], 1);
+    }
+    __syncthreads();
+    // thread i looks at digit 255 - i
+    const int mine = histogram[255 - threadIdx.x];
+    int total;
+    const int above = select_scan(mine, sums, &total);
+    if (above < rest && above + mine >= rest) {
+      digit[0] = 255 - static_cast<int>(threadIdx.x);
+      digit[1] = above;
+    }
+    __syncthreads();
+    const int d = digit[0];
+    rest -= digit[1];
+    prefix = (prefix << 8) | static_cast<Key>(d);
+    shift -= 8;
+    if (histogram[d] == rest) break;  // all of them
+    __syncthreads();
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ void mma_means(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_means(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The 16-bit number nearest to x (bits), and what it stands for.
+__device__ __forceinline__ uint32_t nearest(double x, double* stands, __nv_bfloat16) {
+  const __nv_bfloat16 v = __float2bfloat16_rn(static_cast<float>(x));
+  *stands = static_cast<double>(__bfloat162float(v));
+  return *reinterpret_cast<const uint16_t*>(&v);
+}
+__device__ __forceinline__ uint32_t nearest(double x, double* stands, __half) {
+  const __half v = __float2half_rn(static_cast<float>(x));
+  *stands = static_cast<double>(__half2float(v));
+  return *reinterpret_cast<const uint16_t*>(&v);
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const __grid_constant__ Select p) {
-  constexpr int kLanes = D / 8;          // lanes of a block's mean
-  constexpr int kAtOnce = 32 / kLanes;   // blocks of a warp
-  constexpr int kDepth = 4;              // of those in flight
+  constexpr int kLanes = D / 8;  // vectors of eight channels
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int found[4];               // sequence, its first item, item's new tokens, items in all
+  __shared__ int found[4];  // sequence, its first item, its new tokens
   __shared__ int sums[kSelectWarps];
   __shared__ int histogram[256];
-  __shared__ int digit[2];               // the digit of the keep-th largest key, how many of it are still to be taken
+  __shared__ int digit[2];
+  __shared__ float bounds[8 * kSelectWarps];  // of every warp of the cluster
   const Args& a = p.a;
   const int index = static_cast<int>(blockIdx.x) / p.cluster, rank = static_cast<int>(blockIdx.x) - index * p.cluster;
   const int item = index / a.kv_heads, head = index - item * a.kv_heads;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  double* pooled = reinterpret_cast<double*>(smem);                             // [group][D]
-  uint64_t* keys = reinterpret_cast<uint64_t*>(smem + static_cast<size_t>(a.group) * D * 8);  // [blocks]
+  const SelectShape<D> shape(a.group, a.width * p.per_page);
+  double* pooled = reinterpret_cast<double*>(smem);
+  uint8_t* pieces = smem + shape.pieces_off;
+  float* scales = reinterpret_cast<float*>(smem + shape.scale_off);  // [heads of the group, up to eights]
+  float* scores = reinterpret_cast<float*>(smem + shape.score_off);
+  int* list = reinterpret_cast<int*>(smem + shape.list_off);
+  uint64_t* exact = reinterpret_cast<uint64_t*>(smem + shape.exact_off);
   let_later();
   after_earlier();
 
@@ -227,18 +319,19 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const __grid_
     if (rank == 0)
       for (int i = threadIdx.x; i < p.width; i += kSelectThreads) out[i] = -1;
     if (writes) {
+      const int end = min(max(a.cu_q[a.seqs], 0), a.tokens);
       p.kv_lens[item] = 0;
-      p.cu_q[item] = min(max(a.cu_q[a.seqs], 0), a.tokens);
-      if (item == p.items - 1) p.cu_q[p.items] = min(max(a.cu_q[a.seqs], 0), a.tokens);
+      p.cu_q[item] = end;
+      if (item == p.items - 1) p.cu_q[p.items] = end;
     }
     return;
   }
   const int start = (item - found[1]) * p.query_block, q_len = found[2], count = min(p.query_block, q_len - start);
   const int kv_len = held_keys(a, s), q_first = a.cu_q[s];
-  const int end = a.causal ? max(0, min(kv_len, kv_len - q_len + start + count)) : kv_len;
+  const int end = a.causal ? max(0, kv_len - q_len + start + count) : kv_len;
   const int blocks = (end + p.block - 1) / p.block;
   const int64_t near = max(static_cast<int64_t>(0), static_cast<int64_t>(kv_len) - q_len + (a.causal ? start : 0) - p.recent);
-  const int high = min(blocks, static_cast<int>(near / p.block)), low = min(high, (p.sinks - 1) / p.block + (p.sinks > 0));
+  const int high = min(blocks, static_cast<int>(near / p.block)), low = min(high, p.sinks / p.block + (p.sinks % p.block > 0));
   const int candidates = high - low, keep = min(p.keep, candidates);
   const int chosen = low + keep + blocks - high;
   if (writes) {
@@ -248,10 +341,14 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const __grid_
   }
   const int* table = a.table + s * a.table_row;
   const bool scored = keep > 0 && keep < candidates;  // else there is nothing to choose
+  const int used = count == 1 ? 1 : kPieces;          // (a single token is its own first piece)
+  const auto mean_at = [&](int b, int page) {
+    return p.means + page * p.mean_page + (b % p.per_page) * p.mean_block + head * p.mean_head;
+  };
 
   if (scored) {
-    // pooled queries: a thread sums eight channels of a head over a part of the tokens; the parts meet where the keys will be
-    double* parts = reinterpret_cast<double*>(keys);
+    // pooled queries: a thread sums eight channels of a head over a part of the tokens; the parts meet where the scores will be
+    double* parts = reinterpret_cast<double*>(scores);
     const int vecs = a.group * kLanes, splits = max(1, min(kSelectThreads / vecs, count));
     for (int i = threadIdx.x; i < vecs * splits; i += kSelectThreads) {
       const int split = i / vecs, v = i - split * vecs, h = v / kLanes, vec = v - h * kLanes;
@@ -270,84 +367,112 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const __grid_
         for (int k = 0; k < splits; ++k) sum += parts[k * vecs * 8 + i];
         pooled[i] = sum;
       }
+      __syncthreads();
     }
-    if (p.cluster > 1) cluster_sync_all();  // (the first CTA's parts have been read: others may write their keys there)
+    // their pieces, a warp a head; fp16's are of a multiple by a power of two whose largest magnitude lies between 2^13 and 2^14: what
+    // the last piece cannot hold is below 2^-25, with 128 means of 2^16 at most 0.25
+    for (int h = warp; h < shape.tiles * 8; h += kSelectWarps) {
+      constexpr int kPer = D / 32;
+      double x[kPer];
+      float top = 0.0f;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        x[e] = h < a.group ? pooled[h * D + lane * kPer + e] : 0.0;
+        top = fmaxf(top, fabsf(static_cast<float>(x[e])));
+      }
+      float down = 1.0f;
+      if (std::is_same<T, __half>::value && used > 1) {
+        const int power = max(static_cast<int>(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23) - 127, -100);
+        const double up = __longlong_as_double(static_cast<long long>(1023 + 13 - power) << 52);
+        down = __uint_as_float(static_cast<uint32_t>(min(127 - 13 + power, 254)) << 23);
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) x[e] *= up;
+      }
+      if (lane == 0) scales[h] = down;
+#pragma unroll
+      for (int k = 0; k < kPieces; ++k)
+#pragma unroll
+        for (int e = 0; e < kPer; e += 2) {
+          double stands[2];
+          const uint32_t lower = nearest(x[e], &stands[0], T()), upper = nearest(x[e + 1], &stands[1], T());
+          *reinterpret_cast<uint32_t*>(pieces + (h * kPieces + k) * SelectShape<D>::piece_row + (lane * kPer + e) * 2) = lower | upper << 16;
+          x[e] -= stands[0];
+          x[e + 1] -= stands[1];
+        }
+    }
+    if (p.cluster > 1) cluster_sync_all();  // (the first CTA's parts have been read: others may write their scores there)
     else __syncthreads();
 
-    // scores of this CTA's part of the candidates
-    const int vec = lane % kLanes, sub = lane / kLanes;
-    const uint32_t keys_at = cluster_addr(keys, 0);
-    const int from = static_cast<int>(static_cast<int64_t>(candidates) * rank / p.cluster);
-    const int to = static_cast<int>(static_cast<int64_t>(candidates) * (rank + 1) / p.cluster);
-    for (int c0 = from + warp * kAtOnce * kDepth; c0 < to; c0 += kSelectWarps * kAtOnce * kDepth) {
-      uint4 mean[kDepth];
-      int page[kDepth];
+    // scores of this CTA's part of the candidates, sixteen to a warp: rows r0 and r0 + 8 of the operand, channels 32 j + 8 quad
+    // and on (any order of channels gives the same sum), heads 2 quad and 2 quad + 1 of the result
+    const int r0 = lane >> 2, quad = lane & 3;
+    const uint32_t scores_at = cluster_addr(scores, 0);
+    const int sixteens = (candidates + 15) / 16;
+    const int from = static_cast<int>(static_cast<int64_t>(sixteens) * rank / p.cluster) * 16;
+    const int to = min(candidates, static_cast<int>(static_cast<int64_t>(sixteens) * (rank + 1) / p.cluster) * 16);
+    float most = 0.0f;
+    const auto page_of = [&](int c) { return c < to ? table[(low + c) / p.per_page] : -1; };
+    int page[2] = {page_of(from + warp * 16 + r0), page_of(from + warp * 16 + r0 + 8)};
+    for (int c0 = from + warp * 16; c0 < to; c0 += kSelectWarps * 16) {
+      uint4 mean[2][D / 32];
 #pragma unroll
-      for (int d = 0; d < kDepth; ++d) {
-        const int b = low + c0 + d * kAtOnce + sub;
-        page[d] = c0 + d * kAtOnce + sub < to ? table[b / p.per_page] : -1;
+      for (int i = 0; i < 2; ++i) {
+        const bool there = page[i] >= 0 && page[i] < a.pages;
+        const char* src = there ? mean_at(low + c0 + r0 + 8 * i, page[i]) + quad * 16 : nullptr;
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) mean[i][j] = there ? *reinterpret_cast<const uint4*>(src + j * 64) : make_uint4(0, 0, 0, 0);
+        page[i] = page_of(c0 + kSelectWarps * 16 + r0 + 8 * i);
       }
+      float best[2] = {-INFINITY, -INFINITY};
+      for (int tile = 0; tile < shape.tiles; ++tile) {
+        const uint8_t* piece = pieces + ((tile * 8 + r0) * kPieces) * SelectShape<D>::piece_row + quad * 16;
+        float sc[4] = {}, size[4] = {};
 #pragma unroll
-      for (int d = 0; d < kDepth; ++d) {
-        const int b = low + c0 + d * kAtOnce + sub;
-        mean[d] = make_uint4(0, 0, 0, 0);
-        if (page[d] >= 0 && page[d] < a.pages)
-          mean[d] = *reinterpret_cast<const uint4*>(p.means + page[d] * p.mean_page + (b % p.per_page) * p.mean_block + head * p.mean_head + vec * 16);
-      }
+        for (int j = 0; j < D / 32; ++j) {
+          const uint32_t m0[4] = {mean[0][j].x, mean[0][j].y, mean[0][j].z, mean[0][j].w};
+          const uint32_t m1[4] = {mean[1][j].x, mean[1][j].y, mean[1][j].z, mean[1][j].w};
+          for (int k = 0; k < used; ++k) {
+            const uint4 b = *reinterpret_cast<const uint4*>(piece + k * SelectShape<D>::piece_row + j * 64);
+            const uint32_t q[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-      for (int d = 0; d < kDepth; ++d) {
-        double x[8] = {};
-        add_eight(x, mean[d], T());
-        double best = -INFINITY;
-        for (int h = 0; h < a.group; ++h) {
-          const double* q = pooled + h * D + vec * 8;
-          double dot = 0.0;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) dot = fma(q[e], x[e], dot);
-#pragma unroll
-          for (int o = kLanes / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-          best = fmax(best, dot);  // (NaN counts for nothing)
+            for (int h = 0; h < 4; h += 2) {
+              const uint32_t x[4] = {m0[h], m1[h], m0[h + 1], m1[h + 1]};
+              mma_means(sc, x, q[h], q[h + 1], T());
+              if (k > 0) continue;
+              const uint32_t y[4] = {x[0] & 0x7fff7fffu, x[1] & 0x7fff7fffu, x[2] & 0x7fff7fffu, x[3] & 0x7fff7fffu};
+              mma_means(size, y, q[h] & 0x7fff7fffu, q[h + 1] & 0x7fff7fffu, T());
+            }
+          }
         }
-        const int c = c0 + d * kAtOnce + sub;
-        if (vec == 0 && c < to) store_cluster_u64(keys_at + c * 8, key_of(best));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int h = tile * 8 + 2 * quad + (e & 1);
+          if (h >= a.group) continue;
+          const float x = sc[e] * scales[h];
+          best[e >> 1] = fmaxf(best[e >> 1], x);
+          // (a bound or score that is no number makes every block one that is computed again)
+          const float bound = fmaf(size[e], 0x1p-15f, std::is_same<T, __half>::value && used > 1 ? 0.25f : 0.0f) * scales[h];
+          most = bound < INFINITY && fabsf(x) < INFINITY ? fmaxf(most, bound) : INFINITY;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        best[i] = fmaxf(best[i], __shfl_xor_sync(0xffffffffu, best[i], 1));
+        best[i] = fmaxf(best[i], __shfl_xor_sync(0xffffffffu, best[i], 2));
+        const int c = c0 + r0 + 8 * i;
+        if (quad == 0 && c < to) store_cluster(scores_at + c * 4, best[i]);
       }
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (lane == 0) store_cluster(cluster_addr(&bounds[rank * kSelectWarps + warp], 0), most);
   }
   if (p.cluster > 1) cluster_sync_all();
   else __syncthreads();
   if (rank != 0) return;
 
-  // the keep-th largest key, digit by digit from the top: `prefix` so far, `rest` of it still to be taken
-  uint64_t prefix = 0;
-  int shift = 64, rest = keep;
-  if (scored) {
-    while (shift > 0) {
-      for (int i = threadIdx.x; i < 256; i += kSelectThreads) histogram[i] = 0;
-      __syncthreads();
-      for (int c = threadIdx.x; c < candidates; c += kSelectThreads) {
-        const uint64_t key = keys[c];
-        if (shift == 64 || (key >> shift) == prefix) atomicAdd(&histogram[(key >> (shift - 8)) & 255], 1);
-      }
-      __syncthreads();
-      // thread i looks at digit 255 - i
-      const int mine = histogram[255 - threadIdx.x];
-      int total;
-      const int above = select_scan(mine, sums, &total);
-      if (above < rest && above + mine >= rest) {
-        digit[0] = 255 - static_cast<int>(threadIdx.x);
-        digit[1] = above;
-      }
-      __syncthreads();
-      const int d = digit[0];
-      rest -= digit[1];
-      prefix = (prefix << 8) | static_cast<uint64_t>(d);
-      shift -= 8;
-      if (histogram[d] == rest) break;  // all of them
-      __syncthreads();
-    }
-  }
   // blocks in order: the first ones, the chosen, the last ones
-  auto write = [&](int at, int b) {
+  const auto write = [&](int at, int b) {
     const int page = table[b / p.per_page];
     out[at] = page >= 0 && page < a.pages ? page * p.per_page + b % p.per_page : -1;
   };
@@ -355,21 +480,89 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const __grid_
   for (int i = threadIdx.x; i < blocks - high; i += kSelectThreads) write(low + keep + i, high + i);
   for (int i = chosen + static_cast<int>(threadIdx.x); i < p.width; i += kSelectThreads) out[i] = -1;
   if (!scored) {
-    if (keep > 0)
-      for (int i = threadIdx.x; i < candidates; i += kSelectThreads) write(low + i, low + i);
+    for (int i = threadIdx.x; i < keep; i += kSelectThreads) write(low + i, low + i);
     return;
   }
-  int before = 0, equal = 0;  // taken and equal ones so far
+  float spread = 0.0f;  // 2 E
+  for (int i = 0; i < p.cluster * kSelectWarps; ++i) spread = fmaxf(spread, 2.0f * bounds[i]);
+
+  // T: the smallest score that has the keep-th largest's digits
+  uint32_t prefix;
+  int shift, rest = keep;
+  nth_largest<uint32_t>([&](int c) { return key_of(scores[c]); }, candidates, prefix, shift, rest, histogram, digit, sums);
+  const uint32_t border_key = shift == 0 ? prefix : prefix << shift;
+  // (its digits end where all that share them are taken: the smallest of those is T)
+  float least = INFINITY;
+  for (int c = threadIdx.x; c < candidates; c += kSelectThreads)
+    if (key_of(scores[c]) >= border_key) least = fminf(least, scores[c]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
+  if (lane == 0) bounds[warp] = least;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kSelectWarps; ++w) least = fminf(least, bounds[w]);
+  const float sure = least + spread, out_of = least - spread;
+
+  // the blocks between, in order
+  int doubtful = 0, above = 0;
+  for (int c0 = 0; c0 < candidates; c0 += kSelectThreads) {
+    const int c = c0 + static_cast<int>(threadIdx.x);
+    const bool in = c < candidates && scores[c] > sure, between = c < candidates && !in && !(scores[c] < out_of);
+    int total;
+    const int packed = select_scan((in ? 1 << 16 : 0) | (between ? 1 : 0), sums, &total);
+    if (between) list[doubtful + (packed & 0xffff)] = c;
+    doubtful += total & 0xffff;
+    above += total >> 16;
+  }
+  __syncthreads();
+  rest = keep - above;
+  uint64_t prefix64 = 0;
+  int shift64 = 64;
+  if (doubtful > rest) {
+    for (int i = warp; i < doubtful; i += kSelectWarps) {
+      const int b = low + list[i], at = table[b / p.per_page];
+      constexpr int kPer = D / 32;
+      double x[kPer] = {};
+      if (at >= 0 && at < a.pages) {
+        const char* src = mean_at(b, at) + lane * kPer * 2;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+          if (std::is_same<T, __half>::value) x[e] = static_cast<double>(__half2float(*reinterpret_cast<const __half*>(src + 2 * e)));
+          else x[e] = static_cast<double>(__bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(src + 2 * e)));
+        }
+      }
+      double best = -INFINITY;
+      for (int h = 0; h < a.group; ++h) {
+        double dot = 0.0;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) dot = fma(pooled[h * D + lane * kPer + e], x[e], dot);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+        best = fmax(best, dot);  // (NaN counts for nothing)
+      }
+      if (lane == 0) exact[i] = key_of(best);
+    }
+    __syncthreads();
+    nth_largest<uint64_t>([&](int i) { return exact[i]; }, doubtful, prefix64, shift64, rest, histogram, digit, sums);
+  }
+  // in the order of the blocks: those above, and of the ones between those that have been found, of equal ones the first `rest`
+  int before = 0, equal = 0, seen = 0;
   for (int c0 = 0; c0 < candidates && before < keep; c0 += kSelectThreads) {
     const int c = c0 + static_cast<int>(threadIdx.x);
-    const uint64_t top = c < candidates ? (shift == 64 ? 0 : keys[c] >> shift) : 0;
-    const bool is_above = c < candidates && top > prefix, is_equal = c < candidates && top == prefix;
-    int total_equal, total;
-    const int rank_equal = equal + select_scan(is_equal, sums, &total_equal);
-    const bool take = is_above || (is_equal && rank_equal < rest);
+    const bool in = c < candidates && scores[c] > sure, between = c < candidates && !in && !(scores[c] < out_of);
+    bool take = in || between;
+    int total;
+    if (doubtful > keep - above) {
+      const int at = seen + select_scan(between, sums, &total);
+      seen += total;
+      const uint64_t top = between ? exact[at] >> shift64 : 0;
+      const bool same = between && top == prefix64;
+      const int place = equal + select_scan(same, sums, &total);
+      equal += total;
+      take = in || (between && top > prefix64) || (same && place < rest);
+    }
     const int at = before + select_scan(take, sums, &total);
     if (take) write(low + at, low + c);
-    equal += total_equal;
     before += total;
   }
 }
@@ -546,13 +739,13 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> paged_select_blocks(const at::Ten
   const int device = q.get_device();
   // CTAs of an item and KV head: as many as leave every SM one, and each enough blocks to be worth the cluster's meeting
   p.cluster = 1;
-  while (p.cluster < 8 && items * kv_heads * p.cluster * 2 <= sm_count(device) && held >= 128 * p.cluster) p.cluster *= 2;
-  const int64_t smem = static_cast<int64_t>(a.group) * q.size(2) * 8 + std::max<int64_t>(held, paged::kSelectThreads * 8) * 8;
-  RC_CHECK(smem <= 220 * 1024, "too many heads in a group, or blocks in the table, for the choice of blocks");
+  while (p.cluster < 8 && items * kv_heads * p.cluster * 2 <= sm_count(device) && held >= 256 * p.cluster) p.cluster *= 2;
+  RC_CHECK(a.group <= 128, "too many heads in a group for the choice of blocks");
+  const int smem = q.size(2) == 128 ? paged::SelectShape<128>(a.group, static_cast<int>(held)).bytes : paged::SelectShape<64>(a.group, static_cast<int>(held)).bytes;
+  RC_CHECK(smem <= 224 * 1024, "too many heads in a group, or blocks in the table, for the choice of blocks: take larger blocks");
   cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device).stream();
-  const int bytes = static_cast<int>(smem);
-  if (type == at::kHalf) q.size(2) == 128 ? paged::select_launch<__half, 128>(p, bytes, stream, device) : paged::select_launch<__half, 64>(p, bytes, stream, device);
-  else q.size(2) == 128 ? paged::select_launch<__nv_bfloat16, 128>(p, bytes, stream, device) : paged::select_launch<__nv_bfloat16, 64>(p, bytes, stream, device);
+  if (type == at::kHalf) q.size(2) == 128 ? paged::select_launch<__half, 128>(p, smem, stream, device) : paged::select_launch<__half, 64>(p, smem, stream, device);
+  else q.size(2) == 128 ? paged::select_launch<__nv_bfloat16, 128>(p, smem, stream, device) : paged::select_launch<__nv_bfloat16, 64>(p, smem, stream, device);
   return {out, lens, cu};
 }
 
