@@ -1078,10 +1078,11 @@ int clusters_at_once(int size, int device) {
 // 78 and 57; 84 of 49: 97, 108, 105, 150 and 87; 16 of 8: 21, 18, 15, 25 and 25. 16 sequences with one of 4,000 new tokens
 // (141 items, 1,859 empty blocks) 107 directly and 84 planned. Over 655 shapes, batches of unequal sequences among them, the
 // choice costs 2.6 % on average (3.9 % without the empty blocks).
+// planned_tiles: tile pairs of an item in the planned form.
 template <typename T, int D>
-int direct_cluster(int64_t items, int64_t empty, int64_t tiles, bool uneven, int device) {
+int direct_cluster(int64_t items, int64_t empty, int64_t tiles, int64_t planned_tiles, bool uneven, int device) {
   const int sms = sm_count(device);
-  double best = static_cast<double>(items) * tiles / sms * (uneven ? 0.75 : 1.0) + 16.0;
+  double best = static_cast<double>(items) * planned_tiles / sms * (uneven ? 0.75 : 1.0) + 16.0;
   int cluster = 0;
   for (int c = 1; c <= 16; c *= 2) {
     const int64_t slots = clusters_at_once<T, D>(c, device);
@@ -1117,7 +1118,10 @@ ChunkForm chunk_form(const Args& a, int max_q_len, int device) {
   const int64_t tiles = (keys + kTile - 1) / kTile;
   form.twin = static_cast<int64_t>(max_q_len) * a.group <= kTile;
   chunk_configure<T, D, true, false>(device);
-  form.cluster = direct_cluster<T, D>(form.most_items, form.grid_items - form.most_items, form.twin ? (tiles + 1) / 2 : tiles,
+  // Up to 128 rows the planned form leaves its second tile idle. Where every KV head has a table of its own, that counts (370
+  // items of 128 rows and 99 tiles: 678 us planned, 330 directly); where heads share one, the choice stays as it was measured.
+  const int64_t each = form.twin ? (tiles + 1) / 2 : tiles;
+  form.cluster = direct_cluster<T, D>(form.most_items, form.grid_items - form.most_items, each, a.table_head != 0 ? tiles : each,
                                       a.causal && form.row_tiles > 1, device);
   return form;
 }

@@ -32,16 +32,18 @@
 namespace rc {
 namespace paged {
 
-template <int D>
+// kN: groups of eight rows. One group leaves registers for three CTAs on an SM.
+template <int D, int kN>
 struct PackedShape {
+  static constexpr int ctas = kN == 1 ? 3 : 2;       // of an SM
   static constexpr int tile_bytes = kShortTile * D;  // one of K, V: 64 keys
-  static constexpr int stages = D == 128 ? 6 : 10;
+  static constexpr int stages = (D == 128 ? 1 : 2) * (kN == 1 ? 3 : 6);
   static constexpr int scale_off = stages * 2 * tile_bytes;  // [stages][K, V][64]
   static constexpr int join_off = scale_off + stages * 2 * kShortTile;
   static constexpr int join_bytes = 24 * D * 4;
   static constexpr int bar_off = join_off + join_bytes;
   static constexpr int bytes = bar_off + 1024 + 1024;  // + alignment slack
-  static_assert((bytes + 1024) * kShortCtasPerSm <= 228 * 1024, "two CTAs per SM");
+  static_assert((bytes + 1024) * ctas <= 228 * 1024, "the CTAs of an SM");
   static_assert(kRows * (D + 2) * 4 <= stages * 2 * tile_bytes, "a CTA's rows fit its stages");
 };
 
@@ -61,6 +63,12 @@ __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
 // 2^(e - base) of a scale byte not above base. (A scale of NaN is above all others: what then is in its units is NaN.)
 __device__ __forceinline__ float relative_scale(int e, int base) { return __uint_as_float(static_cast<uint32_t>(max(127 + e - base, 0)) << 23); }
 
+__device__ __forceinline__ int load_byte(uint32_t shared) {
+  uint32_t v;
+  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(shared) : "memory");
+  return static_cast<int>(v);
+}
+
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
   uint32_t out;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(out) : "r"(v));
@@ -78,11 +86,10 @@ __device__ __forceinline__ float2 two_of<__nv_bfloat16>(uint32_t v) {
 template <>
 __device__ __forceinline__ float2 two_of<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
 
-// kN: groups of eight rows, 1 or 2.
 template <typename T, int D, bool kCluster, int kN>
-__global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
+__global__ void __launch_bounds__(kShortThreads, PackedShape<D, kN>::ctas)
     packed_short_kernel(const __grid_constant__ PageMaps maps, const __grid_constant__ PackedShort ps) {
-  using Shape = PackedShape<D>;
+  using Shape = PackedShape<D, kN>;
   constexpr int kKeys = kShortTile / kGroups;  // keys of a warp
   static_assert(kKeys == 16, "a warp's keys are one inner step of P V");
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -114,6 +121,7 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
   } else if (warp < 4) {
     place_share(p, work);
   }
+  const int side = kCluster ? 0 : static_cast<int>(blockIdx.x) % p.par;  // which of the heads that are taken side by side
   int s, base, begin, end;
   if (kCluster) {
     const int item = static_cast<int>(blockIdx.x) / p.cluster, rank = static_cast<int>(blockIdx.x) - item * p.cluster;
@@ -142,13 +150,13 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
     bool ok = true;
     for (int at = begin; ok && at < end;) {
       const SeqWork w(a, s);
-      const int n = w.tiles * a.kv_heads;
+      const int n = w.tiles * (a.kv_heads / p.par);
       if (at >= base + n) {
         base += n;
         ++s;
         continue;
       }
-      const int head = (at - base) / w.tiles, t0 = (at - base) - head * w.tiles;
+      const int place = (at - base) / w.tiles, t0 = (at - base) - place * w.tiles, head = place * p.par + side;
       const int t1 = min(w.tiles, t0 + end - at);
       const TileRange<kShortTile> range(Sight(a, w.kv_len, w.q_len), 0, w.q_len);
       const int* table = a.table + s * a.table_row + head * a.table_head;
@@ -166,7 +174,7 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
           const int key = first + part * 8, block = key / a.tiling.page, held = table[block];
           if (held >= 0 && held < a.pages) from = scale_base + held * scale_page + (key - block * a.tiling.page);
         }
-        ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1, a.status, kTimeoutProducer));
+        ok = __all_sync(0xffffffffu, mbar_wait_park(&empty[stage], phase ^ 1, a.status, kTimeoutProducer));
         if (!ok) break;
         if (lane == 0) {
           if (boxes.count > 0) mbar_arrive_expect_tx(&full[stage], boxes.count * boxes.rows * D * 2);
@@ -206,19 +214,20 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
   // ---------------- consumers ----------------
   const int kg = warp;  // its keys
   const int r0 = lane >> 2, quad = lane & 3;
-  // this lane's operand rows for ldmatrix: keys 0-7 and 8-15 of the warp's, of two chunks
-  const int key_row = kg * kKeys + (lane & 15), chunk = lane >> 4;
+  // place of this lane's operand rows for ldmatrix: keys 0-7 and 8-15 of the warp's, of chunks 0 and 1; chunks c and c + 1 lie at
+  // that ^ 16 c (tiles begin on 1,024 bytes, and the swizzle turns the same bits)
+  const uint32_t operand = smem_u32(smem) + chunk_at<D>(kg * kKeys + (lane & 15), lane >> 4);
   bool ok = true;
   for (int at = begin; kCluster || at < end;) {  // a cluster's CTA goes round once, also without tiles
     const SeqWork w(a, s);
-    const int n = w.tiles * a.kv_heads;
+    const int n = w.tiles * (a.kv_heads / p.par);
     if (!kCluster && at >= base + n) {
       base += n;
       ++s;
       continue;
     }
-    const int head = kCluster ? static_cast<int>(blockIdx.x) / p.cluster - s * a.kv_heads : (at - base) / w.tiles;
-    const int t0 = kCluster ? begin : (at - base) - head * w.tiles;
+    const int place = kCluster ? static_cast<int>(blockIdx.x) / p.cluster - s * a.kv_heads : (at - base) / w.tiles;
+    const int t0 = kCluster ? begin : (at - base) - place * w.tiles, head = place * p.par + side;
     const int t1 = kCluster ? end : min(w.tiles, t0 + end - at);
     const Sight sight(a, w.kv_len, w.q_len);
     const TileRange<kShortTile> range(sight, 0, w.q_len);
@@ -288,13 +297,13 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
 
     for (int t = t0; t < t1; ++t) {
       const int first = range.tile(t) * kShortTile;
-      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, a.status, kTimeoutEpilogue));
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait_park(&full[stage], phase, a.status, kTimeoutEpilogue));
       if (ok) {
-        const uint32_t kb = smem_u32(smem + stage * 2 * Shape::tile_bytes), vb = kb + Shape::tile_bytes;
+        const uint32_t k_at = operand + stage * 2 * Shape::tile_bytes, v_at = k_at + Shape::tile_bytes;
         // scales of this lane's keys r0, r0 + 8 of the warp's
-        const uint8_t* ks = scales + stage * 2 * kShortTile + kg * kKeys + r0;
-        const int k_scale[2] = {ks[0], ks[8]};
-        int v_scale[2] = {ks[kShortTile], ks[kShortTile + 8]};
+        const uint32_t scale_at = smem_u32(scales) + stage * 2 * kShortTile + kg * kKeys + r0;
+        const int k_scale[2] = {load_byte(scale_at), load_byte(scale_at + 8)};
+        int v_scale[2] = {load_byte(scale_at + kShortTile), load_byte(scale_at + kShortTile + 8)};
         float sc[kN][4];  // keys r0, r0 + 8 (pairs) of rows 2 quad, 2 quad + 1
 #pragma unroll
         for (int g = 0; g < kN; ++g)
@@ -303,7 +312,7 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
 #pragma unroll
         for (int c = 0; c < D / 16; c += 2) {
           uint32_t b[4];  // keys 0-7 and 8-15 of chunk c, and of chunk c + 1
-          ldmatrix_x4(b, kb + chunk_at<D>(key_row, c + chunk));
+          ldmatrix_x4(b, k_at ^ (c << 4));
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const uint32_t k4[4] = {codes_to_half2(b[2 * i]), codes_to_half2(b[2 * i + 1]), upper_codes_to_half2(b[2 * i]),
@@ -384,7 +393,7 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
 #pragma unroll
         for (int c = 0; c < D / 16; c += 2) {
           uint32_t b[4];
-          ldmatrix_x4_trans(b, vb + chunk_at<D>(key_row, c + chunk));
+          ldmatrix_x4_trans(b, v_at ^ (c << 4));
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const uint32_t lower = b[2 * i] & keep[0], upper = b[2 * i + 1] & keep[1];
@@ -480,7 +489,7 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
       return;
     }
     if (kg == 0 && ok) {
-      const int item_first = base + head * w.tiles;
+      const int item_first = base + place * w.tiles;
       const bool starts = item_first >= begin, ends = item_first + w.tiles <= end;
 #pragma unroll
       for (int g = 0; g < kN; ++g)
@@ -509,7 +518,7 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
 
 template <typename T, int D, int kN>
 struct PackedForm {
-  static constexpr int bytes = PackedShape<D>::bytes, tile_bytes = PackedShape<D>::tile_bytes, boxes = 1;
+  static constexpr int ctas = PackedShape<D, kN>::ctas, bytes = PackedShape<D, kN>::bytes, tile_bytes = PackedShape<D, kN>::tile_bytes, boxes = 1;
   static constexpr auto clustered() { return packed_short_kernel<T, D, true, kN>; }
 };
 
@@ -518,8 +527,8 @@ void packed_configure(int device) {
   static bool known[64] = {};
   bool& configured = known[device & 63];
   if (configured) return;
-  RC_CUDA(cudaFuncSetAttribute(packed_short_kernel<T, D, false, kN>, cudaFuncAttributeMaxDynamicSharedMemorySize, PackedShape<D>::bytes));
-  RC_CUDA(cudaFuncSetAttribute(packed_short_kernel<T, D, true, kN>, cudaFuncAttributeMaxDynamicSharedMemorySize, PackedShape<D>::bytes));
+  RC_CUDA(cudaFuncSetAttribute(packed_short_kernel<T, D, false, kN>, cudaFuncAttributeMaxDynamicSharedMemorySize, PackedShape<D, kN>::bytes));
+  RC_CUDA(cudaFuncSetAttribute(packed_short_kernel<T, D, true, kN>, cudaFuncAttributeMaxDynamicSharedMemorySize, PackedShape<D, kN>::bytes));
   RC_CUDA(cudaFuncSetAttribute(packed_short_kernel<T, D, true, kN>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   configured = true;
 }
@@ -535,7 +544,7 @@ CUtensorMap code_map(const at::Tensor& t, int box) {
   const cuuint32_t ones[4] = {1, 1, 1, 1};
   const CUresult res = encode_tiled_fn()(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, t.data_ptr(), dims, strides, boxes, ones,
                                          CU_TENSOR_MAP_INTERLEAVE_NONE, d == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-                                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                                         CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   RC_CHECK(res == CUDA_SUCCESS, "cuTensorMapEncodeTiled (codes) failed (code " + std::to_string(static_cast<int>(res)) + ")");
   return map;
 }
@@ -543,7 +552,7 @@ CUtensorMap code_map(const at::Tensor& t, int box) {
 template <typename T, int D, int kN>
 void packed_launch(const Args& a, const at::Tensor& k_codes, const at::Tensor& v_codes, const Packed& k, const Packed& v,
                    const at::Tensor& like, cudaStream_t stream, int device) {
-  using Shape = PackedShape<D>;
+  using Shape = PackedShape<D, kN>;
   PackedShort ps{};
   Short& p = ps.s;
   p.a = a;
@@ -556,14 +565,18 @@ void packed_launch(const Args& a, const at::Tensor& k_codes, const at::Tensor& v
   ps.v_scale_head = v.scale_head;
   const PageMaps maps = page_maps(k_codes, v_codes, p.a.tiling, kShortTile, code_map);
   packed_configure<T, D, kN>(device);
-  const int64_t items = static_cast<int64_t>(a.seqs) * a.kv_heads, slots = sm_count(device) * kShortCtasPerSm;
+  const int64_t items = static_cast<int64_t>(a.seqs) * a.kv_heads, slots = sm_count(device) * Shape::ctas;
+  p.par = 1;
   p.cluster = short_cluster<PackedForm<T, D, kN>>(items, short_tiles(a), p.a.tiling.step, a.seqs > 1, device);
   if (p.cluster > 0) {
     launch(packed_short_kernel<T, D, true, kN>, dim3(static_cast<unsigned>(items * p.cluster)), kShortThreads, Shape::bytes, p.cluster,
            stream, maps, ps);
     return;
   }
-  const int ctas = static_cast<int>(std::min<int64_t>(slots, items * (short_tiles(a) + 1)));
+  // The line's CTAs take the KV heads side by side: the rows of neighbouring heads lie next to each other, and 128 bytes here
+  // and there are too little for HBM (48 sessions of up to 16,384 keys: 163 us head after head).
+  for (p.par = std::min(a.kv_heads, 32); a.kv_heads % p.par != 0;) --p.par;
+  const int ctas = static_cast<int>(std::min<int64_t>(slots / p.par, items / p.par * (short_tiles(a) + 1))) * p.par;
   RC_CHECK(items * (kRows / 4) < (1ll << 31), "too many sequences and rows for one launch");
   const int64_t floats = 2ll * ctas * kRows * (D + 2), ints = 1 + 2ll * a.seqs;
   at::Tensor workspace = at::empty({floats + ints}, like.options().dtype(at::kFloat));

@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
 
 template <typename T, int D>
 struct ShortForm {
-  static constexpr int bytes = ShortShape<D>::bytes, tile_bytes = ShortShape<D>::tile_bytes, boxes = ShortShape<D>::boxes;
+  static constexpr int ctas = kShortCtasPerSm, bytes = ShortShape<D>::bytes, tile_bytes = ShortShape<D>::tile_bytes, boxes = ShortShape<D>::boxes;
   static constexpr auto clustered() { return short_kernel<T, D, true>; }
 };
 
@@ -395,6 +395,7 @@ void short_launch(Args a, const at::Tensor& k_pages, const at::Tensor& v_pages, 
   p.a.tiling = Tiling::of(a.tiling.page, kShortTile);
   const PageMaps maps = page_maps(k_pages, v_pages, p.a.tiling, kShortTile);
   const int64_t items = static_cast<int64_t>(a.seqs) * a.kv_heads, slots = sm_count(device) * kShortCtasPerSm;
+  p.par = 1;
   p.cluster = short_form<T, D>(a, device);
   if (p.cluster > 0) {
     launch(short_kernel<T, D, true>, dim3(static_cast<unsigned>(items * p.cluster)), kShortThreads, Shape::bytes, p.cluster,

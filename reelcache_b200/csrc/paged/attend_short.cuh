@@ -29,6 +29,7 @@ struct Short {
   float* part_o;   // [2 * CTAs, 16, D]
   float* part_ml;  // [2 * CTAs, 16, 2]
   int cluster;     // CTAs of a cluster (the clustered form)
+  int par;         // KV heads that the line's CTAs take side by side (a divisor of their number): CTA par i + j the share i of the j-th
 };
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
@@ -73,7 +74,7 @@ struct SeqWork {
 // it begins. For the four consumer warps; work[4 ..] takes their sums.
 __device__ __forceinline__ void place_share(const Short& p, int* work) {
   const Args& a = p.a;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, heads = a.kv_heads / p.par;
   // Thread i counts the tiles of sequences [i per, i per + per); their prefix sums place the share.
   const int per = (a.seqs + 127) / 128, s0 = static_cast<int>(threadIdx.x) * per;
   int mine = 0;
@@ -81,7 +82,7 @@ __device__ __forceinline__ void place_share(const Short& p, int* work) {
   for (int i = 0; i < per; ++i) {
     if (s0 + i < a.seqs) {
       const SeqWork w(a, s0 + i);
-      mine += w.tiles * a.kv_heads;
+      mine += w.tiles * heads;
     }
   }
   int x = mine;
@@ -99,9 +100,9 @@ __device__ __forceinline__ void place_share(const Short& p, int* work) {
     if (i < warp) before += n;
     total += n;
   }
-  const int ctas = static_cast<int>(gridDim.x);
+  const int ctas = static_cast<int>(gridDim.x) / p.par, index = static_cast<int>(blockIdx.x) / p.par;
   const int share = max(min(kShortLeast, total), (total + ctas - 1) / ctas);
-  const int begin = min(total, static_cast<int>(blockIdx.x) * share), end = min(total, begin + share);
+  const int begin = min(total, index * share), end = min(total, begin + share);
   if (threadIdx.x == 0) {
     work[0] = begin;
     work[1] = end;
@@ -111,7 +112,7 @@ __device__ __forceinline__ void place_share(const Short& p, int* work) {
   if (here || blockIdx.x == 0) {
     for (int i = 0; i < per && s0 + i < a.seqs; ++i) {
       const SeqWork w(a, s0 + i);
-      const int n = w.tiles * a.kv_heads;
+      const int n = w.tiles * heads;
       if (here && begin >= before && begin < before + n) {
         work[2] = s0 + i;
         work[3] = before;
@@ -284,19 +285,19 @@ __global__ void __launch_bounds__(128) short_join_kernel(const __grid_constant__
   const int query = row / a.group;
   if (query >= w.q_len) return;
   const int share = *p.line.share;
-  const int begin = p.line.first[s] + head * w.tiles, end = begin + w.tiles;
+  const int place = head / p.par, side = head - place * p.par;
+  const int begin = p.line.first[s] + place * w.tiles, end = begin + w.tiles;
   const int c0 = begin / share, c1 = (end - 1) / share;
   if (c0 == c1) return;
+  const auto slot_of = [&](int c) { return (2 * (static_cast<int64_t>(c) * p.par + side) + (c == c0)) * kRows + row; };
   // 32 parts at a time, a lane to each one's maximum and sum
   float top = -INFINITY, acc[kPer], sum = 0.0f;
 #pragma unroll
   for (int e = 0; e < kPer; ++e) acc[e] = 0.0f;
   for (int cb = c0; cb <= c1; cb += 32) {
     const int n = min(32, c1 - cb + 1);
-    const int64_t first_slot = (2 * static_cast<int64_t>(cb) + (cb == c0)) * kRows + row;
-    const int64_t slot = (2 * static_cast<int64_t>(cb + lane) + (cb + lane == c0)) * kRows + row;
     float2 ml = make_float2(-INFINITY, 0.0f);
-    if (lane < n) ml = *reinterpret_cast<const float2*>(p.part_ml + slot * 2);
+    if (lane < n) ml = *reinterpret_cast<const float2*>(p.part_ml + slot_of(cb + lane) * 2);
     float mx = ml.x;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -312,7 +313,7 @@ __global__ void __launch_bounds__(128) short_join_kernel(const __grid_constant__
 #pragma unroll 8
     for (int i = 0; i < n; ++i) {
       const float weight = __shfl_sync(0xffffffffu, wt, i);
-      const int64_t at = i == 0 ? first_slot : 2 * static_cast<int64_t>(cb + i) * kRows + row;
+      const int64_t at = slot_of(cb + i);
 #pragma unroll
       for (int e = 0; e < kPer; e += 2) {
         const float2 x = *reinterpret_cast<const float2*>(p.part_o + at * D + lane * kPer + e);
@@ -371,7 +372,7 @@ template <typename Form>
 int short_cluster(int64_t items, int64_t tiles, int step, bool several, int device) {
   const double hbm = 2.0 * Form::tile_bytes / 6.5e6;  // us of a tile, for one CTA alone
   const double box = 0.6 + 0.045 * (2 * Form::boxes * kShortTile / step);
-  const double slots = kShortCtasPerSm * sm_count(device), share = std::max<double>(kShortLeast, items * tiles / slots);
+  const double slots = Form::ctas * sm_count(device), share = std::max<double>(kShortLeast, items * tiles / slots);
   double best = 10.0 + 0.2 * std::min<double>(tiles / kShortLeast, slots / items) + hbm * slots * (several ? 0.75 : 1.0) * share;
   int cluster = 0;
   for (int c = 2; c <= 16; c *= 2) {

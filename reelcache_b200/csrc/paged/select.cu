@@ -8,14 +8,17 @@
 // The score of a block for the queries of a KV head's group is max over the heads h of (sum over the tokens of the query block
 // of q_h) . mean. Blocks at the border of the choice differ by little, so the choice is that of scores in FP64, where the order
 // of a sum moves them by 2^-50 of their size: the same for every batch and form of the kernel. Equal scores go to the lower
-// block. Few blocks need FP64: scores come from the tensor core first (the pooled query as the sum of three 16-bit numbers, one for
-// single tokens), together with the sum of their products' magnitudes, which bounds their error (2^-15 of it: 24 steps at most, each a sum
-// of 17 terms cut at 2^-24 of the largest). With T the keep-th largest and E the largest bound, blocks above T + 2 E are chosen and blocks below T - 2 E are not;
-// only the blocks between, where there is more than one way to choose from them, are computed again.
+// block. Few blocks need FP64. Scores come from the tensor core first, the pooled query (summed in FP32) as three 16-bit
+// numbers that add up to it, a single token as itself. What they may be off by is summed next to them, as one more product:
+// with x the pooled query, y the sum of the tokens' magnitudes and m the mean, 2^-15.8 sum |x| |m| for the products (8 steps, each a
+// sum of 17 terms cut at 2^-23 of the largest; those of the small numbers come first and count for little) and n 2^-24 sum y |m| for
+// the FP32 sums of n terms one after the other. With T the keep-th largest score and E the largest bound, blocks above T + 2 E
+// are chosen and blocks below T - 2 E are not; only where there is more than one way to choose from those between are they
+// computed again, in FP64 (in a call of 128 query blocks and heads for a few of them).
 //
-// One CTA, or a cluster of them that splits the blocks, for every (query block, KV head): scores as 32-bit keys that sort
-// like them in the shared memory of the cluster's first CTA, which finds the keep-th largest by digits of eight bits (a
-// histogram each, until a digit's candidates are all taken) and writes the chosen blocks in order.
+// One CTA, or a cluster of them that splits the blocks, for every (query block, KV head): scores go to the shared memory of the
+// cluster's first CTA, which finds the keep-th largest (a histogram between the smallest and the largest, then the bucket
+// that holds it; digit by digit where that bucket holds many) and writes the chosen blocks in order.
 //
 // What bounds it: the latency of a chain of small steps for few sequences, reading the means for many.
 #include <ATen/ATen.h>
@@ -34,9 +37,23 @@
 namespace rc {
 namespace paged {
 
+// Division by a number below 2^24 of numbers below 2^31 as a product (an integer division takes some hundred cycles, of which a
+// chain of small steps has few to spare).
+struct Divider {
+  uint32_t magic, shift;
+  int by;
+  static Divider of(int by) {
+    uint32_t bits = 0;
+    while ((int64_t{1} << bits) < by) ++bits;
+    return {static_cast<uint32_t>(((uint64_t{1} << (31 + bits)) + by - 1) / by), 31 + bits, by};
+  }
+  __device__ __forceinline__ int over(int n) const { return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * magic) >> shift); }
+  __device__ __forceinline__ int up(int n) const { return over(n) + (n > over(n) * by); }  // rounded up
+};
+
 // -- means ------------------------------------------------------------------------------------------------------------
 
-constexpr int kMeanThreads = 128;
+constexpr int kMeanThreads = 256;
 
 struct Means {
   Args a;                // table, lengths, pages; tokens, max_q_len
@@ -46,7 +63,7 @@ struct Means {
   int64_t scale_page, scale_head;
   char* means;           // [pages, page_size / block, kv_heads, D]: strides in bytes
   int64_t mean_page, mean_block, mean_head;
-  int block;
+  Divider block, per_page;
 };
 
 __device__ __forceinline__ void add_eight(double (&sum)[8], const uint4& u, __nv_bfloat16) {
@@ -67,19 +84,14 @@ __device__ __forceinline__ void add_eight(double (&sum)[8], const uint4& u, __ha
   }
 }
 
-template <typename T>
-__device__ __forceinline__ uint4 eight_of(const double (&x)[8]) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = pack2<T>(static_cast<float>(x[2 * i]), static_cast<float>(x[2 * i + 1]));
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
+__device__ __forceinline__ __nv_bfloat16 rounded(float x, __nv_bfloat16) { return __float2bfloat16_rn(x); }
+__device__ __forceinline__ __half rounded(float x, __half) { return __float2half_rn(x); }
 
-// Block (touched block, sequence, KV head): a thread sums eight channels of every (128 / lanes of a row)-th token.
+// Block (touched block, sequence, KV head): a thread sums eight channels of every (256 / lanes of a row)-th token.
 template <typename T, int D, bool kPacked>
 __global__ void __launch_bounds__(kMeanThreads) means_kernel(const __grid_constant__ Means p) {
   constexpr int kLanes = D / 8, kRowsAtOnce = kMeanThreads / kLanes;
-  __shared__ double part[kRowsAtOnce][kLanes][8];
+  __shared__ double part[kMeanThreads / 32][D];
   let_later();
   after_earlier();
   const Args& a = p.a;
@@ -88,12 +100,10 @@ __global__ void __launch_bounds__(kMeanThreads) means_kernel(const __grid_consta
   int q_first;
   const int q_len = min(new_tokens(a, s, &q_first), a.max_q_len), kv_len = held_keys(a, s);
   if (q_len <= 0 || kv_len == 0) return;
-  const int b = max(kv_len - q_len, 0) / p.block + blockIdx.x;
-  const int64_t from = static_cast<int64_t>(b) * p.block;
-  if (from >= kv_len) return;
-  const int rows = static_cast<int>(min(static_cast<int64_t>(p.block), kv_len - from));
-  const int slot = static_cast<int>(from / a.tiling.page), row0 = static_cast<int>(from - static_cast<int64_t>(slot) * a.tiling.page);
-  const int page = a.table[s * a.table_row + slot];
+  const int b = p.block.over(max(kv_len - q_len, 0)) + blockIdx.x;
+  if (b >= p.block.up(kv_len)) return;
+  const int rows = min(p.block.by, kv_len - b * p.block.by), slot = p.per_page.over(b), part_of = b - slot * p.per_page.by;
+  const int row0 = part_of * p.block.by, page = a.table[s * a.table_row + slot];
   if (page < 0 || page >= a.pages) {
     if (threadIdx.x == 0 && head == 0 && a.status != nullptr) atomicCAS(a.status + kPagedWord, 0, kPageRange);
     return;
@@ -119,17 +129,23 @@ __global__ void __launch_bounds__(kMeanThreads) means_kernel(const __grid_consta
       add_eight(sum, *reinterpret_cast<const uint4*>(at), T());
     }
   }
+  // the rows that a warp holds meet by shuffles, then the warps, a thread to each channel
 #pragma unroll
-  for (int e = 0; e < 8; ++e) part[group][vec][e] = sum[e];
+  for (int o = kLanes; o < 32; o <<= 1)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], o);
+  if ((threadIdx.x & 31) < kLanes) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) part[threadIdx.x >> 5][vec * 8 + e] = sum[e];
+  }
   __syncthreads();
-  if (group != 0) return;
-  for (int g = 1; g < kRowsAtOnce; ++g)
+  const int c = threadIdx.x;
+  if (c >= D) return;
+  double all = 0.0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum[e] += part[g][vec][e];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) sum[e] /= static_cast<double>(rows);
-  char* dst = p.means + page * p.mean_page + (row0 / p.block) * p.mean_block + head * p.mean_head + vec * 16;
-  *reinterpret_cast<uint4*>(dst) = eight_of<T>(sum);
+  for (int w = 0; w < kMeanThreads / 32; ++w) all += part[w][c];
+  char* dst = p.means + page * p.mean_page + part_of * p.mean_block + head * p.mean_head;
+  reinterpret_cast<T*>(dst)[c] = rounded(static_cast<float>(all / static_cast<double>(rows)), T());
 }
 
 // -- the choice -------------------------------------------------------------------------------------------------------
@@ -137,23 +153,24 @@ __global__ void __launch_bounds__(kMeanThreads) means_kernel(const __grid_consta
 constexpr int kSelectThreads = 256;
 constexpr int kSelectWarps = kSelectThreads / 32;
 constexpr int kMostBlocks = 12288;  // whose keys fit one CTA's shared memory
-constexpr int kPieces = 3;          // 16-bit numbers that add up to a pooled query
+constexpr int kBuckets = 256;       // one for each thread
+constexpr int kPieces = 3;          // 16-bit numbers that add up to a pooled query; a fourth row holds what bounds its errors
 
 struct Select {
   Args a;              // q, table, lengths, heads; causal; tokens, max_q_len
   const char* means;
   int64_t mean_page, mean_block, mean_head;
-  int block, per_page, keep, query_block, sinks, recent;
+  Divider block, per_page, query_block, kv_heads;
+  int keep, sinks, recent;
   int items, width;
   int* table;          // [items, kv_heads, width]
   int* kv_lens;        // [items]
   int* cu_q;           // [items + 1]
-  int cluster;
+  int cluster, log_cluster;
 };
 
-// Shared memory of a CTA: pooled queries in FP64 [group][D], their pieces as the products' operand, scales of those, then the
-// keys [blocks] (64 bits), of whose room the first half holds the 32-bit scores and the second half the list of blocks that
-// are computed again... in that order: scores, list, exact keys.
+// Shared memory of a CTA: pooled queries in FP64 [group][D] (for the border; at first the sums of a lone part), their pieces as
+// the products' operand, scales of those, scores [blocks], the list of the blocks that are computed again, their keys in 64 bits.
 template <int D>
 struct SelectShape {
   static constexpr int piece_row = D * 2 + 64;  // bytes: rows 64 bytes apart in the banks
@@ -162,7 +179,7 @@ struct SelectShape {
   __host__ __device__ SelectShape(int group, int blocks) {
     tiles = (group + 7) / 8;
     pieces_off = group * D * 8;
-    scale_off = pieces_off + tiles * 8 * kPieces * piece_row;
+    scale_off = pieces_off + tiles * 8 * (kPieces + 1) * piece_row;
     score_off = (scale_off + tiles * 8 * 4 + 15) / 16 * 16;
     list_off = score_off + (blocks + 3) / 4 * 16;
     exact_off = list_off + (blocks + 3) / 4 * 16;
@@ -216,7 +233,7 @@ __device__ __forceinline__ void nth_largest(Get get, int n, Key& prefix, int& sh
   prefix = 0;
   shift = kBits;
   while (shift > 0) {
-    for (int i = threadIdx.x; i < 256; i += kSelectThreads) histogram[i] = 0;
+    histogram[threadIdx.x] = 0;
     __syncthreads();
     for (int c = threadIdx.x; c < n; c += kSelectThreads) {
       const Key key = get(c);
@@ -242,46 +259,162 @@ __device__ __forceinline__ void nth_largest(Get get, int n, Key& prefix, int& sh
   __syncthreads();
 }
 
-__device__ __forceinline__ void mma_means(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
+// The keep-th largest of n scores between bottom and top (histogram: zeros). `list` takes a few of their places.
+__device__ __forceinline__ float keep_th(const float* scores, int n, int keep, float top, float bottom, int* histogram, int* sums, int* digit,
+                                         int* list) {
+  if (top == bottom) return top;
+  const int lane = threadIdx.x & 31;
+  const float step = static_cast<float>(kBuckets) / (top - bottom);
+  if (step > 0.0f && step < INFINITY && fabsf(bottom) < INFINITY) {  // (else: bounds that are no numbers, or a range that FP32 cannot cut)
+    const auto bucket_of = [&](float x) { return min(kBuckets - 1, static_cast<int>((x - bottom) * step)); };  // grows with x
+    if (threadIdx.x == 0) digit[2] = 0;
+    for (int c = threadIdx.x; c < n; c += kSelectThreads) atomicAdd(&histogram[bucket_of(scores[c])], 1);
+    __syncthreads();
+    // every warp by itself: a lane sums eight buckets from the top
+    constexpr int kPer = kBuckets / 32;
+    int counts[kPer], sum = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) sum += counts[i] = histogram[kBuckets - 1 - (lane * kPer + i)];
+    int above = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, above, o);
+      if (lane >= o) above += y;
+    }
+    above -= sum;
+    int bucket = -1, members = 0, rest = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (above < keep && above + counts[i] >= keep) {
+        bucket = kBuckets - 1 - (lane * kPer + i);
+        members = counts[i];
+        rest = keep - above;
+      }
+      above += counts[i];
+    }
+    const int holder = __ffs(__ballot_sync(0xffffffffu, bucket >= 0)) - 1;
+    bucket = __shfl_sync(0xffffffffu, bucket, holder);
+    members = __shfl_sync(0xffffffffu, members, holder);
+    rest = __shfl_sync(0xffffffffu, rest, holder);
+    if (members <= 32) {
+      for (int c = threadIdx.x; c < n; c += kSelectThreads)
+        if (bucket_of(scores[c]) == bucket) list[atomicAdd(&digit[2], 1)] = c;
+      __syncthreads();
+      // every warp by itself: a member's place among them (of equal ones each counts the others that come before it in the list)
+      const float x = lane < members ? scores[list[lane]] : -INFINITY;
+      int place = 0;
+      for (int i = 0; i < members; ++i) {
+        const float other = __shfl_sync(0xffffffffu, x, i);
+        place += other > x || (other == x && i < lane);
+      }
+      const uint32_t who = __ballot_sync(0xffffffffu, lane < members && place == rest - 1);
+      return __shfl_sync(0xffffffffu, x, __ffs(who) - 1);  // (the list is written again only after further barriers)
+    }
+  }
+  uint32_t prefix;
+  int shift, rest = keep;
+  __syncthreads();
+  nth_largest<uint32_t>([&](int c) { return key_of(scores[c]); }, n, prefix, shift, rest, histogram, digit, sums);
+  // its digits end where all that share them are among the keep largest: the smallest of those
+  const uint32_t border = shift == 0 ? prefix : prefix << shift;
+  float least = INFINITY;
+  for (int c = threadIdx.x; c < n; c += kSelectThreads)
+    if (key_of(scores[c]) >= border) least = fminf(least, scores[c]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
+  if (lane == 0) histogram[threadIdx.x >> 5] = __float_as_int(least);
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kSelectWarps; ++w) least = fminf(least, __int_as_float(histogram[w]));
+  __syncthreads();
+  return least;
+}
+
+struct Operand {
+  uint32_t x[4];
+};
+__device__ __forceinline__ void mma_means(float (&d)[4], const Operand& a, uint32_t b0, uint32_t b1, __nv_bfloat16) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+      : "r"(a.x[0]), "r"(a.x[1]), "r"(a.x[2]), "r"(a.x[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_means(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
+__device__ __forceinline__ void mma_means(float (&d)[4], const Operand& a, uint32_t b0, uint32_t b1, __half) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+      : "r"(a.x[0]), "r"(a.x[1]), "r"(a.x[2]), "r"(a.x[3]), "r"(b0), "r"(b1));
 }
 
-// The 16-bit number nearest to x (bits), and what it stands for.
-__device__ __forceinline__ uint32_t nearest(double x, double* stands, __nv_bfloat16) {
-  const __nv_bfloat16 v = __float2bfloat16_rn(static_cast<float>(x));
-  *stands = static_cast<double>(__bfloat162float(v));
+__device__ __forceinline__ float value_of(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float value_of(__half x) { return __half2float(x); }
+
+// The 16-bit number nearest to x (bits), and x without it.
+__device__ __forceinline__ uint32_t nearest(float& x, __nv_bfloat16) {
+  const __nv_bfloat16 v = __float2bfloat16_rn(x);
+  x -= __bfloat162float(v);
   return *reinterpret_cast<const uint16_t*>(&v);
 }
-__device__ __forceinline__ uint32_t nearest(double x, double* stands, __half) {
-  const __half v = __float2half_rn(static_cast<float>(x));
-  *stands = static_cast<double>(__half2float(v));
+__device__ __forceinline__ uint32_t nearest(float& x, __half) {
+  const __half v = __float2half_rn(x);
+  x -= __half2float(v);
   return *reinterpret_cast<const uint16_t*>(&v);
+}
+
+__device__ __forceinline__ void add_eight(float (&sum)[8], float (&size)[8], const uint4& u, __nv_bfloat16) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float lo = __uint_as_float(w[i] << 16), hi = __uint_as_float(w[i] & 0xffff0000u);
+    sum[2 * i] += lo;
+    sum[2 * i + 1] += hi;
+    size[2 * i] += fabsf(lo);
+    size[2 * i + 1] += fabsf(hi);
+  }
+}
+__device__ __forceinline__ void add_eight(float (&sum)[8], float (&size)[8], const uint4& u, __half) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    sum[2 * i] += f.x;
+    sum[2 * i + 1] += f.y;
+    size[2 * i] += fabsf(f.x);
+    size[2 * i + 1] += fabsf(f.y);
+  }
+}
+
+// Bits of a thread's candidates (words by constant index, so that they stay in registers).
+template <int kWords>
+__device__ __forceinline__ void mark(uint32_t (&words)[kWords], int i, bool set) {
+#pragma unroll
+  for (int w = 0; w < kWords; ++w)
+    if (set && i >> 5 == w) words[w] |= 1u << (i & 31);
+}
+template <int kWords>
+__device__ __forceinline__ bool marked(const uint32_t (&words)[kWords], int i) {
+  uint32_t word = 0;
+#pragma unroll
+  for (int w = 0; w < kWords; ++w)
+    if (i >> 5 == w) word = words[w];
+  return (word >> (i & 31)) & 1;
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const __grid_constant__ Select p) {
+__global__ void __launch_bounds__(kSelectThreads, 3) select_kernel(const __grid_constant__ Select p) {
   constexpr int kLanes = D / 8;  // vectors of eight channels
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int found[4];  // sequence, its first item, its new tokens
+  __shared__ int found[5];  // sequence, its first item, its new tokens, the first of them, its keys
   __shared__ int sums[kSelectWarps];
-  __shared__ int histogram[256];
-  __shared__ int digit[2];
-  __shared__ float bounds[8 * kSelectWarps];  // of every warp of the cluster
+  __shared__ int histogram[kBuckets];
+  __shared__ int digit[3];
+  __shared__ float bounds[3 * 8 * kSelectWarps];  // of every warp of the cluster: largest error, largest and smallest score
   const Args& a = p.a;
-  const int index = static_cast<int>(blockIdx.x) / p.cluster, rank = static_cast<int>(blockIdx.x) - index * p.cluster;
-  const int item = index / a.kv_heads, head = index - item * a.kv_heads;
+  const int index = static_cast<int>(blockIdx.x) >> p.log_cluster, rank = static_cast<int>(blockIdx.x) & (p.cluster - 1);
+  const int item = p.kv_heads.over(index), head = index - item * a.kv_heads;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const SelectShape<D> shape(a.group, a.width * p.per_page);
-  double* pooled = reinterpret_cast<double*>(smem);
+  const SelectShape<D> shape(a.group, a.width * p.per_page.by);
+  double* pooled = reinterpret_cast<double*>(smem);  // (for the border)
   uint8_t* pieces = smem + shape.pieces_off;
   float* scales = reinterpret_cast<float*>(smem + shape.scale_off);  // [heads of the group, up to eights]
   float* scores = reinterpret_cast<float*>(smem + shape.score_off);
@@ -295,10 +428,11 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const __grid_
   if (threadIdx.x == 0) found[0] = -1;
   for (int base = 0; base < a.seqs; base += kSelectThreads) {
     const int s = base + static_cast<int>(threadIdx.x);
-    int n = 0, q_first = 0, q_len = 0;
+    int n = 0, q_first = 0, q_len = 0, kv_len = 0;
     if (s < a.seqs) {
       q_len = min(new_tokens(a, s, &q_first), a.max_q_len);
-      n = (q_len + p.query_block - 1) / p.query_block;
+      kv_len = held_keys(a, s);
+      n = q_len > 0 ? p.query_block.up(q_len) : 0;
       if (index == 0 && rank == 0) report_rows(a, s);
     }
     int total;
@@ -307,6 +441,8 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const __grid_
       found[0] = s;
       found[1] = before;
       found[2] = q_len;
+      found[3] = q_first;
+      found[4] = kv_len;
     }
     items += total;
     if (item < items && index > 0) break;  // (the same for all threads; the first CTA looks at every sequence)
@@ -326,16 +462,16 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const __grid_
     }
     return;
   }
-  const int start = (item - found[1]) * p.query_block, q_len = found[2], count = min(p.query_block, q_len - start);
-  const int kv_len = held_keys(a, s), q_first = a.cu_q[s];
+  const int start = (item - found[1]) * p.query_block.by, q_len = found[2], count = min(p.query_block.by, q_len - start);
+  const int q_first = found[3], kv_len = found[4];
   const int end = a.causal ? max(0, kv_len - q_len + start + count) : kv_len;
-  const int blocks = (end + p.block - 1) / p.block;
-  const int64_t near = max(static_cast<int64_t>(0), static_cast<int64_t>(kv_len) - q_len + (a.causal ? start : 0) - p.recent);
-  const int high = min(blocks, static_cast<int>(near / p.block)), low = min(high, p.sinks / p.block + (p.sinks % p.block > 0));
+  const int blocks = p.block.up(end);
+  const int near = static_cast<int>(max(static_cast<int64_t>(0), static_cast<int64_t>(kv_len) - q_len + (a.causal ? start : 0) - p.recent));
+  const int high = min(blocks, p.block.over(near)), low = min(high, p.block.up(p.sinks));
   const int candidates = high - low, keep = min(p.keep, candidates);
   const int chosen = low + keep + blocks - high;
   if (writes) {
-    p.kv_lens[item] = chosen > 0 ? (chosen - 1) * p.block + end - (blocks - 1) * p.block : 0;
+    p.kv_lens[item] = chosen > 0 ? (chosen - blocks) * p.block.by + end : 0;
     p.cu_q[item] = q_first + start;
     if (item == p.items - 1) p.cu_q[p.items] = q_first + start + count;
   }
@@ -343,106 +479,122 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const __grid_
   const bool scored = keep > 0 && keep < candidates;  // else there is nothing to choose
   const int used = count == 1 ? 1 : kPieces;          // (a single token is its own first piece)
   const auto mean_at = [&](int b, int page) {
-    return p.means + page * p.mean_page + (b % p.per_page) * p.mean_block + head * p.mean_head;
+    return p.means + page * p.mean_page + (b - p.per_page.over(b) * p.per_page.by) * p.mean_block + head * p.mean_head;
   };
 
   if (scored) {
-    // pooled queries: a thread sums eight channels of a head over a part of the tokens; the parts meet where the scores will be
-    double* parts = reinterpret_cast<double*>(scores);
-    const int vecs = a.group * kLanes, splits = max(1, min(kSelectThreads / vecs, count));
-    for (int i = threadIdx.x; i < vecs * splits; i += kSelectThreads) {
-      const int split = i / vecs, v = i - split * vecs, h = v / kLanes, vec = v - h * kLanes;
-      double sum[8] = {};
-      const T* src = static_cast<const T*>(a.q) + static_cast<int64_t>(q_first + start) * a.q_token + (head * a.group + h) * a.q_head + vec * 8;
-#pragma unroll 4
-      for (int t = split; t < count; t += splits) add_eight(sum, *reinterpret_cast<const uint4*>(src + t * a.q_token), T());
-      double* to = splits == 1 ? pooled + v * 8 : parts + i * 8;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) to[e] = sum[e];
-    }
-    __syncthreads();
-    if (splits > 1) {
-      for (int i = threadIdx.x; i < vecs * 8; i += kSelectThreads) {
-        double sum = 0.0;
-        for (int k = 0; k < splits; ++k) sum += parts[k * vecs * 8 + i];
-        pooled[i] = sum;
-      }
-      __syncthreads();
-    }
-    // their pieces, a warp a head; fp16's are of a multiple by a power of two whose largest magnitude lies between 2^13 and 2^14: what
-    // the last piece cannot hold is below 2^-25, with 128 means of 2^16 at most 0.25
-    for (int h = warp; h < shape.tiles * 8; h += kSelectWarps) {
-      constexpr int kPer = D / 32;
-      double x[kPer];
-      float top = 0.0f;
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) {
-        x[e] = h < a.group ? pooled[h * D + lane * kPer + e] : 0.0;
-        top = fmaxf(top, fabsf(static_cast<float>(x[e])));
-      }
-      float down = 1.0f;
-      if (std::is_same<T, __half>::value && used > 1) {
-        const int power = max(static_cast<int>(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23) - 127, -100);
-        const double up = __longlong_as_double(static_cast<long long>(1023 + 13 - power) << 52);
-        down = __uint_as_float(static_cast<uint32_t>(min(127 - 13 + power, 254)) << 23);
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) x[e] *= up;
-      }
-      if (lane == 0) scales[h] = down;
-#pragma unroll
-      for (int k = 0; k < kPieces; ++k)
-#pragma unroll
-        for (int e = 0; e < kPer; e += 2) {
-          double stands[2];
-          const uint32_t lower = nearest(x[e], &stands[0], T()), upper = nearest(x[e + 1], &stands[1], T());
-          *reinterpret_cast<uint32_t*>(pieces + (h * kPieces + k) * SelectShape<D>::piece_row + (lane * kPer + e) * 2) = lower | upper << 16;
-          x[e] -= stands[0];
-          x[e + 1] -= stands[1];
-        }
-    }
-    if (p.cluster > 1) cluster_sync_all();  // (the first CTA's parts have been read: others may write their scores there)
-    else __syncthreads();
-
-    // scores of this CTA's part of the candidates, sixteen to a warp: rows r0 and r0 + 8 of the operand, channels 32 j + 8 quad
-    // and on (any order of channels gives the same sum), heads 2 quad and 2 quad + 1 of the result
+    // This CTA's part of the candidates, sixteen to a warp: rows r0 and r0 + 8 of the operand, channels 32 j + 8 quad and on (any
+    // order of channels gives the same sum), heads 2 quad and 2 quad + 1 of the result. The first ones are asked for before the queries.
     const int r0 = lane >> 2, quad = lane & 3;
-    const uint32_t scores_at = cluster_addr(scores, 0);
     const int sixteens = (candidates + 15) / 16;
-    const int from = static_cast<int>(static_cast<int64_t>(sixteens) * rank / p.cluster) * 16;
-    const int to = min(candidates, static_cast<int>(static_cast<int64_t>(sixteens) * (rank + 1) / p.cluster) * 16);
-    float most = 0.0f;
-    const auto page_of = [&](int c) { return c < to ? table[(low + c) / p.per_page] : -1; };
-    int page[2] = {page_of(from + warp * 16 + r0), page_of(from + warp * 16 + r0 + 8)};
-    for (int c0 = from + warp * 16; c0 < to; c0 += kSelectWarps * 16) {
-      uint4 mean[2][D / 32];
+    const int from = ((sixteens * rank) >> p.log_cluster) * 16, to = min(candidates, ((sixteens * (rank + 1)) >> p.log_cluster) * 16);
+    int page[2];
+    uint4 mean[2][D / 32];
+    const auto look_up = [&](int c0) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) page[i] = c0 + r0 + 8 * i < to ? table[p.per_page.over(low + c0 + r0 + 8 * i)] : -1;
+    };
+    const auto load = [&](int c0) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const bool there = page[i] >= 0 && page[i] < a.pages;
         const char* src = there ? mean_at(low + c0 + r0 + 8 * i, page[i]) + quad * 16 : nullptr;
 #pragma unroll
         for (int j = 0; j < D / 32; ++j) mean[i][j] = there ? *reinterpret_cast<const uint4*>(src + j * 64) : make_uint4(0, 0, 0, 0);
-        page[i] = page_of(c0 + kSelectWarps * 16 + r0 + 8 * i);
       }
+    };
+    look_up(from + warp * 16);
+
+    // pooled queries: a thread sums eight channels of a head over a part of the tokens
+    const int vecs = a.group * kLanes, splits = max(1, min(kSelectThreads / vecs, count));
+    float2* parts = reinterpret_cast<float2*>(splits == 1 ? smem : smem + shape.score_off);  // [splits][head][channel]: sum, magnitudes
+    for (int i = threadIdx.x; i < vecs * splits; i += kSelectThreads) {
+      const int split = i / vecs, v = i - split * vecs, h = v / kLanes, vec = v - h * kLanes;
+      const T* src = static_cast<const T*>(a.q) + static_cast<int64_t>(q_first + start) * a.q_token + (head * a.group + h) * a.q_head + vec * 8;
+      if (used == 1) {
+        const uint4 x = *reinterpret_cast<const uint4*>(src);
+        uint8_t* to_piece = pieces + h * (kPieces + 1) * SelectShape<D>::piece_row + vec * 16;
+        *reinterpret_cast<uint4*>(to_piece) = x;
+        *reinterpret_cast<uint4*>(to_piece + kPieces * SelectShape<D>::piece_row) =
+            make_uint4(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu, x.z & 0x7fff7fffu, x.w & 0x7fff7fffu);
+        if (vec == 0) scales[h] = 1.0f;
+      } else {
+        float sum[8] = {}, size[8] = {};
+#pragma unroll 4
+        for (int t = split; t < count; t += splits) add_eight(sum, size, *reinterpret_cast<const uint4*>(src + t * a.q_token), T());
+#pragma unroll
+        for (int e = 0; e < 8; e += 2)
+          *reinterpret_cast<float4*>(parts + i * 8 + e) = make_float4(sum[e], size[e], sum[e + 1], size[e + 1]);
+      }
+    }
+    load(from + warp * 16);
+    if (used > 1) {
+      __syncthreads();
+      // their pieces, a warp a head; fp16's are of a multiple by a power of two that brings the bounds' largest between 2^13 and
+      // 2^14: what the last piece cannot hold is below 2^-25, with 128 means of 2^16 at most 0.25
+      const float steps = static_cast<float>(count / splits + 1 + splits) * (0x1p-24f / 0x1.2p-16f);  // of the sums in FP32, over that of the products
+      for (int h = warp; h < a.group; h += kSelectWarps) {
+        constexpr int kPer = D / 32;
+        float x[kPer], y[kPer], top = 0.0f;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+          float2 f = make_float2(0.0f, 0.0f);
+          for (int k = 0; k < splits; ++k) {
+            const float2 add = parts[k * vecs * 8 + h * D + lane * kPer + e];
+            f.x += add.x;
+            f.y += add.y;
+          }
+          x[e] = f.x;
+          y[e] = fmaf(f.y, steps, fabsf(f.x)) * 1.01f;  // (and its own rounding to 16 bits)
+          top = fmaxf(top, y[e]);
+        }
+        float down = 1.0f;
+        if (std::is_same<T, __half>::value) {
+          const int power = max(static_cast<int>(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23) - 127, -100);
+          const float up = __uint_as_float(static_cast<uint32_t>(127 + 13 - power) << 23);
+          down = __uint_as_float(static_cast<uint32_t>(min(127 - 13 + power, 254)) << 23);
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) {
+            x[e] *= up;
+            y[e] *= up;
+          }
+        }
+        if (lane == 0) scales[h] = down;
+#pragma unroll
+        for (int k = 0; k <= kPieces; ++k)
+#pragma unroll
+          for (int e = 0; e < kPer; e += 2) {
+            const uint32_t lower = nearest(k < kPieces ? x[e] : y[e], T()), upper = nearest(k < kPieces ? x[e + 1] : y[e + 1], T());
+            *reinterpret_cast<uint32_t*>(pieces + (h * (kPieces + 1) + k) * SelectShape<D>::piece_row + (lane * kPer + e) * 2) = lower | upper << 16;
+          }
+      }
+    }
+    for (int i = threadIdx.x; i < kBuckets; i += kSelectThreads) histogram[i] = 0;
+    if (p.cluster > 1) cluster_sync_all();  // (the first CTA's parts have been read: others may write their scores there)
+    else __syncthreads();
+
+    const uint32_t scores_at = cluster_addr(scores, 0);
+    float most = 0.0f, top = -INFINITY, bottom = INFINITY;
+    for (int c0 = from + warp * 16; c0 < to; c0 += kSelectWarps * 16) {
+      look_up(c0 + kSelectWarps * 16);
       float best[2] = {-INFINITY, -INFINITY};
       for (int tile = 0; tile < shape.tiles; ++tile) {
-        const uint8_t* piece = pieces + ((tile * 8 + r0) * kPieces) * SelectShape<D>::piece_row + quad * 16;
+        const uint8_t* piece = pieces + ((tile * 8 + r0) * (kPieces + 1)) * SelectShape<D>::piece_row + quad * 16;
         float sc[4] = {}, size[4] = {};
+        for (int k = used - 1; k >= 0; --k) {
+#pragma unroll
+          for (int j = 0; j < D / 32; ++j) {
+            const uint4 b = *reinterpret_cast<const uint4*>(piece + k * SelectShape<D>::piece_row + j * 64);
+            mma_means(sc, Operand{mean[0][j].x, mean[1][j].x, mean[0][j].y, mean[1][j].y}, b.x, b.y, T());
+            mma_means(sc, Operand{mean[0][j].z, mean[1][j].z, mean[0][j].w, mean[1][j].w}, b.z, b.w, T());
+          }
+        }
 #pragma unroll
         for (int j = 0; j < D / 32; ++j) {
-          const uint32_t m0[4] = {mean[0][j].x, mean[0][j].y, mean[0][j].z, mean[0][j].w};
-          const uint32_t m1[4] = {mean[1][j].x, mean[1][j].y, mean[1][j].z, mean[1][j].w};
-          for (int k = 0; k < used; ++k) {
-            const uint4 b = *reinterpret_cast<const uint4*>(piece + k * SelectShape<D>::piece_row + j * 64);
-            const uint32_t q[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-            for (int h = 0; h < 4; h += 2) {
-              const uint32_t x[4] = {m0[h], m1[h], m0[h + 1], m1[h + 1]};
-              mma_means(sc, x, q[h], q[h + 1], T());
-              if (k > 0) continue;
-              const uint32_t y[4] = {x[0] & 0x7fff7fffu, x[1] & 0x7fff7fffu, x[2] & 0x7fff7fffu, x[3] & 0x7fff7fffu};
-              mma_means(size, y, q[h] & 0x7fff7fffu, q[h + 1] & 0x7fff7fffu, T());
-            }
-          }
+          constexpr uint32_t kSize = 0x7fff7fffu;
+          const uint4 b = *reinterpret_cast<const uint4*>(piece + kPieces * SelectShape<D>::piece_row + j * 64);
+          mma_means(size, Operand{mean[0][j].x & kSize, mean[1][j].x & kSize, mean[0][j].y & kSize, mean[1][j].y & kSize}, b.x, b.y, T());
+          mma_means(size, Operand{mean[0][j].z & kSize, mean[1][j].z & kSize, mean[0][j].w & kSize, mean[1][j].w & kSize}, b.z, b.w, T());
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -451,21 +603,35 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const __grid_
           const float x = sc[e] * scales[h];
           best[e >> 1] = fmaxf(best[e >> 1], x);
           // (a bound or score that is no number makes every block one that is computed again)
-          const float bound = fmaf(size[e], 0x1p-15f, std::is_same<T, __half>::value && used > 1 ? 0.25f : 0.0f) * scales[h];
+          const float bound = fmaf(size[e], 0x1.24p-16f, std::is_same<T, __half>::value && used > 1 ? 0.25f : 0.0f) * scales[h];
           most = bound < INFINITY && fabsf(x) < INFINITY ? fmaxf(most, bound) : INFINITY;
         }
       }
+      load(c0 + kSelectWarps * 16);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         best[i] = fmaxf(best[i], __shfl_xor_sync(0xffffffffu, best[i], 1));
         best[i] = fmaxf(best[i], __shfl_xor_sync(0xffffffffu, best[i], 2));
         const int c = c0 + r0 + 8 * i;
-        if (quad == 0 && c < to) store_cluster(scores_at + c * 4, best[i]);
+        if (c < to) {
+          top = fmaxf(top, best[i]);
+          bottom = fminf(bottom, best[i]);
+          if (quad == 0) store_cluster(scores_at + c * 4, best[i]);
+        }
       }
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-    if (lane == 0) store_cluster(cluster_addr(&bounds[rank * kSelectWarps + warp], 0), most);
+    for (int o = 16; o > 0; o >>= 1) {
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      bottom = fminf(bottom, __shfl_xor_sync(0xffffffffu, bottom, o));
+    }
+    if (lane == 0) {
+      const uint32_t at = cluster_addr(&bounds[3 * (rank * kSelectWarps + warp)], 0);
+      store_cluster(at, most);
+      store_cluster(at + 4, top);
+      store_cluster(at + 8, bottom);
+    }
   }
   if (p.cluster > 1) cluster_sync_all();
   else __syncthreads();
@@ -473,8 +639,8 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const __grid_
 
   // blocks in order: the first ones, the chosen, the last ones
   const auto write = [&](int at, int b) {
-    const int page = table[b / p.per_page];
-    out[at] = page >= 0 && page < a.pages ? page * p.per_page + b % p.per_page : -1;
+    const int slot = p.per_page.over(b), page = table[slot];
+    out[at] = page >= 0 && page < a.pages ? (page - slot) * p.per_page.by + b : -1;
   };
   for (int i = threadIdx.x; i < low; i += kSelectThreads) write(i, i);
   for (int i = threadIdx.x; i < blocks - high; i += kSelectThreads) write(low + keep + i, high + i);
@@ -483,88 +649,128 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const __grid_
     for (int i = threadIdx.x; i < keep; i += kSelectThreads) write(low + i, low + i);
     return;
   }
-  float spread = 0.0f;  // 2 E
-  for (int i = 0; i < p.cluster * kSelectWarps; ++i) spread = fmaxf(spread, 2.0f * bounds[i]);
-
-  // T: the smallest score that has the keep-th largest's digits
-  uint32_t prefix;
-  int shift, rest = keep;
-  nth_largest<uint32_t>([&](int c) { return key_of(scores[c]); }, candidates, prefix, shift, rest, histogram, digit, sums);
-  const uint32_t border_key = shift == 0 ? prefix : prefix << shift;
-  // (its digits end where all that share them are taken: the smallest of those is T)
-  float least = INFINITY;
-  for (int c = threadIdx.x; c < candidates; c += kSelectThreads)
-    if (key_of(scores[c]) >= border_key) least = fminf(least, scores[c]);
+  float spread = 0.0f, top = -INFINITY, bottom = INFINITY;  // 2 E, and the scores' range
+  for (int i = lane; i < p.cluster * kSelectWarps; i += 32) {
+    spread = fmaxf(spread, 2.0f * bounds[3 * i]);
+    top = fmaxf(top, bounds[3 * i + 1]);
+    bottom = fminf(bottom, bounds[3 * i + 2]);
+  }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
-  if (lane == 0) bounds[warp] = least;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kSelectWarps; ++w) least = fminf(least, bounds[w]);
+  for (int o = 16; o > 0; o >>= 1) {
+    spread = fmaxf(spread, __shfl_xor_sync(0xffffffffu, spread, o));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    bottom = fminf(bottom, __shfl_xor_sync(0xffffffffu, bottom, o));
+  }
+  const float least = keep_th(scores, candidates, keep, top, bottom, histogram, sums, digit, list);
   const float sure = least + spread, out_of = least - spread;
 
-  // the blocks between, in order
-  int doubtful = 0, above = 0;
-  for (int c0 = 0; c0 < candidates; c0 += kSelectThreads) {
-    const int c = c0 + static_cast<int>(threadIdx.x);
-    const bool in = c < candidates && scores[c] > sure, between = c < candidates && !in && !(scores[c] < out_of);
-    int total;
-    const int packed = select_scan((in ? 1 << 16 : 0) | (between ? 1 : 0), sums, &total);
-    if (between) list[doubtful + (packed & 0xffff)] = c;
-    doubtful += total & 0xffff;
-    above += total >> 16;
+  // a thread looks at `per` neighbouring candidates, so that one prefix sum puts what it finds in order
+  const int per = (candidates + kSelectThreads - 1) / kSelectThreads;
+  const int mine = min(candidates, static_cast<int>(threadIdx.x) * per), past = min(candidates, mine + per);
+  int counts = 0;  // those above, and times 2^16 those between
+  for (int c = mine; c < past; ++c) counts += scores[c] > sure ? 1 : scores[c] < out_of ? 0 : 1 << 16;
+  int total;
+  const int before = select_scan(counts, sums, &total);
+  const int above = total & 0xffff, doubtful = total >> 16;
+  int at = (before & 0xffff) + (before >> 16);
+  if (doubtful <= keep - above) {
+    for (int c = mine; c < past; ++c)
+      if (!(scores[c] < out_of)) write(low + at++, low + c);
+    return;
+  }
+
+  // ---------------- the border in FP64 ----------------
+  {
+    int place = before >> 16;
+    for (int c = mine; c < past; ++c)
+      if (!(scores[c] > sure) && !(scores[c] < out_of)) list[place++] = c;
+  }
+  // pooled queries in FP64: a warp takes every eighth group of tokens, a lane eight channels; the warps meet where the pieces were
+  double* meet = reinterpret_cast<double*>(pieces);  // [warps][D]
+  for (int h = 0; h < a.group; ++h) {
+    double sum[8] = {};
+    const int vec = lane % kLanes;
+    const T* src = static_cast<const T*>(a.q) + static_cast<int64_t>(q_first + start) * a.q_token + (head * a.group + h) * a.q_head + vec * 8;
+#pragma unroll 4
+    for (int t = warp * (32 / kLanes) + lane / kLanes; t < count; t += kSelectWarps * (32 / kLanes))
+      add_eight(sum, *reinterpret_cast<const uint4*>(src + t * a.q_token), T());
+#pragma unroll
+    for (int o = kLanes; o < 32; o <<= 1)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], o);
+    __syncthreads();  // the last head's have been read
+    if (lane < kLanes)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) meet[warp * D + vec * 8 + e] = sum[e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < D; i += kSelectThreads) {
+      double all = 0.0;
+      for (int w = 0; w < min(kSelectWarps, count); ++w) all += meet[w * D + i];
+      pooled[h * D + i] = all;
+    }
   }
   __syncthreads();
-  rest = keep - above;
-  uint64_t prefix64 = 0;
-  int shift64 = 64;
-  if (doubtful > rest) {
-    for (int i = warp; i < doubtful; i += kSelectWarps) {
-      const int b = low + list[i], at = table[b / p.per_page];
-      constexpr int kPer = D / 32;
-      double x[kPer] = {};
-      if (at >= 0 && at < a.pages) {
-        const char* src = mean_at(b, at) + lane * kPer * 2;
+  for (int i = warp; i < doubtful; i += kSelectWarps) {
+    const int b = low + list[i], page = table[p.per_page.over(b)];
+    constexpr int kPer = D / 32;
+    double x[kPer] = {};
+    if (page >= 0 && page < a.pages) {
+      const T* src = reinterpret_cast<const T*>(mean_at(b, page)) + lane * kPer;
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-          if (std::is_same<T, __half>::value) x[e] = static_cast<double>(__half2float(*reinterpret_cast<const __half*>(src + 2 * e)));
-          else x[e] = static_cast<double>(__bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(src + 2 * e)));
-        }
-      }
-      double best = -INFINITY;
-      for (int h = 0; h < a.group; ++h) {
-        double dot = 0.0;
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) dot = fma(pooled[h * D + lane * kPer + e], x[e], dot);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-        best = fmax(best, dot);  // (NaN counts for nothing)
-      }
-      if (lane == 0) exact[i] = key_of(best);
+      for (int e = 0; e < kPer; ++e) x[e] = static_cast<double>(value_of(src[e]));
     }
-    __syncthreads();
-    nth_largest<uint64_t>([&](int i) { return exact[i]; }, doubtful, prefix64, shift64, rest, histogram, digit, sums);
-  }
-  // in the order of the blocks: those above, and of the ones between those that have been found, of equal ones the first `rest`
-  int before = 0, equal = 0, seen = 0;
-  for (int c0 = 0; c0 < candidates && before < keep; c0 += kSelectThreads) {
-    const int c = c0 + static_cast<int>(threadIdx.x);
-    const bool in = c < candidates && scores[c] > sure, between = c < candidates && !in && !(scores[c] < out_of);
-    bool take = in || between;
-    int total;
-    if (doubtful > keep - above) {
-      const int at = seen + select_scan(between, sums, &total);
-      seen += total;
-      const uint64_t top = between ? exact[at] >> shift64 : 0;
-      const bool same = between && top == prefix64;
-      const int place = equal + select_scan(same, sums, &total);
-      equal += total;
-      take = in || (between && top > prefix64) || (same && place < rest);
+    double best = -INFINITY;
+    for (int h = 0; h < a.group; ++h) {
+      double dot = 0.0;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) dot = fma(pooled[h * D + lane * kPer + e], x[e], dot);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+      best = fmax(best, dot);  // (NaN counts for nothing)
     }
-    const int at = before + select_scan(take, sums, &total);
-    if (take) write(low + at, low + c);
-    before += total;
+    if (lane == 0) exact[i] = key_of(best);
   }
+  __syncthreads();
+  int rest = keep - above, number = 0;
+  uint32_t taken[(kMostBlocks / kSelectThreads + 31) / 32] = {};  // of this thread's candidates
+  int place = before >> 16;
+  if (doubtful <= 32) {
+    // every warp by itself: a member's place among them, equal ones in their order
+    const uint64_t key = lane < doubtful ? exact[lane] : 0;
+    int rank_of = 0;
+    for (int i = 0; i < doubtful; ++i) {
+      const uint64_t other = __shfl_sync(0xffffffffu, key, i);
+      rank_of += other > key || (other == key && i < lane);
+    }
+    const uint32_t best = __ballot_sync(0xffffffffu, lane < doubtful && rank_of < rest);
+    for (int c = mine; c < past; ++c) {
+      bool take = scores[c] > sure;
+      if (!take && !(scores[c] < out_of)) take = (best >> place++) & 1;
+      mark(taken, c - mine, take);
+      number += take;
+    }
+  } else {
+    uint64_t prefix;
+    int shift, equals = 0;
+    nth_largest<uint64_t>([&](int i) { return exact[i]; }, doubtful, prefix, shift, rest, histogram, digit, sums);
+    // those above the rest-th largest, and of its equals the first `rest`
+    for (int c = mine; c < past; ++c)
+      if (!(scores[c] > sure) && !(scores[c] < out_of)) equals += (exact[place++] >> shift) == prefix;
+    int equal = select_scan(equals, sums, &total);
+    place = before >> 16;
+    for (int c = mine; c < past; ++c) {
+      bool take = scores[c] > sure;
+      if (!take && !(scores[c] < out_of)) {
+        const uint64_t digits = exact[place++] >> shift;
+        take = digits > prefix || (digits == prefix && equal++ < rest);
+      }
+      mark(taken, c - mine, take);
+      number += take;
+    }
+  }
+  at = select_scan(number, sums, &total);
+  for (int c = mine; c < past; ++c)
+    if (marked(taken, c - mine)) write(low + at++, low + c);
 }
 
 template <typename T, int D>
@@ -639,7 +845,8 @@ void paged_block_means(const at::Tensor& k_pages, const c10::optional<at::Tensor
   p.mean_page = means.stride(0) * 2;
   p.mean_block = means.stride(1) * 2;
   p.mean_head = means.stride(2) * 2;
-  p.block = static_cast<int>(k_pages.size(1) / per_page);
+  p.block = paged::Divider::of(static_cast<int>(k_pages.size(1) / per_page));
+  p.per_page = paged::Divider::of(static_cast<int>(per_page));
   paged::Args& a = p.a;
   a.table = t.table;
   a.kv_lens = t.kv_lens;
@@ -654,8 +861,8 @@ void paged_block_means(const at::Tensor& k_pages, const c10::optional<at::Tensor
   a.tiling.page = static_cast<int>(k_pages.size(1));
   a.status = status_ptr(status);
   if (a.seqs == 0) return;
-  const int64_t held = (static_cast<int64_t>(a.width) * a.tiling.page + p.block - 1) / p.block;
-  const int touched = static_cast<int>(std::min<int64_t>(held, (max_q_len + p.block - 2) / p.block + 1));
+  const int64_t held = static_cast<int64_t>(a.width) * per_page;
+  const int touched = static_cast<int>(std::min<int64_t>(held, (max_q_len + p.block.by - 2) / p.block.by + 1));
   if (touched == 0) return;
   cudaStream_t stream = c10::cuda::getCurrentCUDAStream(k_pages.get_device()).stream();
   if (type == at::kHalf) d == 128 ? paged::means_launch<__half, 128>(p, touched, stream) : paged::means_launch<__half, 64>(p, touched, stream);
@@ -725,10 +932,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> paged_select_blocks(const at::Ten
   p.mean_page = means.stride(0) * 2;
   p.mean_block = means.stride(1) * 2;
   p.mean_head = means.stride(2) * 2;
-  p.block = static_cast<int>(block);
-  p.per_page = static_cast<int>(per_page);
+  p.block = paged::Divider::of(static_cast<int>(block));
+  p.per_page = paged::Divider::of(static_cast<int>(per_page));
+  p.query_block = paged::Divider::of(static_cast<int>(query_block));
+  p.kv_heads = paged::Divider::of(static_cast<int>(kv_heads));
   p.keep = static_cast<int>(keep);
-  p.query_block = static_cast<int>(query_block);
   p.sinks = static_cast<int>(sinks);
   p.recent = static_cast<int>(recent);
   p.items = static_cast<int>(items);
@@ -737,9 +945,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> paged_select_blocks(const at::Ten
   p.kv_lens = lens.data_ptr<int>();
   p.cu_q = cu.data_ptr<int>();
   const int device = q.get_device();
-  // CTAs of an item and KV head: as many as leave every SM one, and each enough blocks to be worth the cluster's meeting
+  // CTAs of an item and KV head: as many as find room at once (three on an SM), with 128 blocks each
   p.cluster = 1;
-  while (p.cluster < 8 && items * kv_heads * p.cluster * 2 <= sm_count(device) && held >= 256 * p.cluster) p.cluster *= 2;
+  while (p.cluster < 8 && items * kv_heads * p.cluster * 2 <= 3 * sm_count(device) && held > 128 * p.cluster) {
+    p.cluster *= 2;
+    ++p.log_cluster;
+  }
   RC_CHECK(a.group <= 128, "too many heads in a group for the choice of blocks");
   const int smem = q.size(2) == 128 ? paged::SelectShape<128>(a.group, static_cast<int>(held)).bytes : paged::SelectShape<64>(a.group, static_cast<int>(held)).bytes;
   RC_CHECK(smem <= 224 * 1024, "too many heads in a group, or blocks in the table, for the choice of blocks: take larger blocks");
