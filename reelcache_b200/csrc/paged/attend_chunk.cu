@@ -101,6 +101,7 @@ struct Chunk {
   float* part_ml;  // [2 * ctas, 256, 2]
   int ctas;
   int cluster;     // CTAs of an item (the direct form)
+  int first_item;  // of the grid (the direct form)
   int row_tiles;   // of a sequence and KV head, at most
   int most_items;  // room for items
 };
@@ -246,7 +247,8 @@ struct Segment {
   }
 
   __device__ __forceinline__ bool direct(const Chunk& p, int block, int item_rows) {
-    const int index = block / p.cluster, rank = block - index * p.cluster, each = p.a.kv_heads * p.row_tiles;
+    const int local = block / p.cluster, rank = block - local * p.cluster, each = p.a.kv_heads * p.row_tiles;
+    const int index = p.first_item + local;
     item.seq = index / each;
     item.head = (index - item.seq * each) / p.row_tiles;
     item.row_tile = p.row_tiles - 1 - index % p.row_tiles;  // the rows that see most come first
@@ -1103,6 +1105,7 @@ struct ChunkForm {
   int64_t row_tiles, grid_items, most_items;
   int cluster;  // 0: planned
   bool twin;
+  int64_t whole_items;  // direct: the first ones that take a CTA each, in a launch of their own
 };
 
 template <typename T, int D>
@@ -1123,6 +1126,23 @@ ChunkForm chunk_form(const Args& a, int max_q_len, int device) {
   const int64_t each = form.twin ? (tiles + 1) / 2 : tiles;
   form.cluster = direct_cluster<T, D>(form.most_items, form.grid_items - form.most_items, each, a.table_head != 0 ? tiles : each,
                                       a.causal && form.row_tiles > 1, device);
+  // Such calls are one long line of equal items: whole rounds of them with a CTA each, and the rest, which would leave SMs idle, in
+  // clusters (370 items of 128 rows and 99 tiles: 2 rounds and 74 items in pairs).
+  if (a.table_head != 0 && form.cluster > 0) {
+    const int64_t sms = sm_count(device), rest = form.grid_items % sms;
+    if (form.grid_items > sms && rest > 0) {
+      int cluster = 1;
+      while (cluster < 16 && rest * cluster * 2 <= sms) cluster *= 2;
+      const double split = static_cast<double>(form.grid_items / sms) * (each + 3.5) + (each + cluster - 1) / cluster + (cluster > 1 ? 6.0 : 3.5);
+      const int64_t slots = form.cluster > 1 ? clusters_at_once<T, D>(form.cluster, device) : sms;
+      const double one = static_cast<double>((form.grid_items + slots - 1) / slots) *
+                         (static_cast<double>((each + form.cluster - 1) / form.cluster) + (form.cluster > 1 ? 6.0 : 3.5));
+      if (split < one) {
+        form.whole_items = form.grid_items - rest;
+        form.cluster = cluster;
+      }
+    }
+  }
   return form;
 }
 
@@ -1142,15 +1162,22 @@ void chunk_launch(const Args& args, const at::Tensor& k_pages, const at::Tensor&
   p.cluster = form.cluster;
   const PageMaps maps = page_maps(k_pages, v_pages, p.a.tiling, kTile);
   if (p.cluster > 0) {
-    const int64_t blocks = form.grid_items * p.cluster;
-    RC_CHECK(blocks < (1ll << 31), "too many sequences and rows for one launch");
-    const dim3 grid(static_cast<unsigned>(blocks));
-    if (form.twin) {
-      chunk_configure<T, D, true, true>(device);
-      launch(chunk_kernel<T, D, true, true>, grid, kChunkThreads, ChunkShape<D, true>::bytes, p.cluster, stream, maps, p);
-    } else {
-      launch(chunk_kernel<T, D, true, false>, grid, kChunkThreads, Shape::bytes, p.cluster, stream, maps, p);
-    }
+    const auto run = [&](int64_t first, int64_t items, int cluster) {
+      const int64_t blocks = items * cluster;
+      RC_CHECK(blocks < (1ll << 31), "too many sequences and rows for one launch");
+      const dim3 grid(static_cast<unsigned>(blocks));
+      p.first_item = static_cast<int>(first);
+      p.cluster = cluster;
+      if (form.twin) {
+        chunk_configure<T, D, true, true>(device);
+        launch(chunk_kernel<T, D, true, true>, grid, kChunkThreads, ChunkShape<D, true>::bytes, cluster, stream, maps, p);
+      } else {
+        launch(chunk_kernel<T, D, true, false>, grid, kChunkThreads, Shape::bytes, cluster, stream, maps, p);
+      }
+    };
+    RC_CHECK(form.grid_items < (1ll << 31), "too many sequences and rows for one launch");
+    if (form.whole_items > 0) run(0, form.whole_items, 1);
+    if (form.whole_items < form.grid_items) run(form.whole_items, form.grid_items - form.whole_items, form.cluster);
     return;
   }
   chunk_configure<T, D, false, false>(device);

@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(128) short_join_kernel(const __grid_constant__
 }
 
 // Clusters of `size` CTAs of a form that run at the same time, or -1 where none does. A form names its clustered kernel, its
-// shared memory, the bytes of a tile of K (or V) and the boxes of 128 bytes or less that a row of it takes.
+// CTAs on an SM and shared memory, the bytes of a tile of K (or V) and the boxes of 128 bytes or less that a row of it takes.
 template <typename Form>
 int short_clusters_at_once(int size, int device) {
   static int known[64][5] = {};

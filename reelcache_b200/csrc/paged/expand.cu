@@ -98,11 +98,7 @@ __global__ void __launch_bounds__(kExpandThreads) expand_kernel(const __grid_con
     for (int i = 0; i < kExpandItems; ++i) {
       const int v = first + i * kExpandThreads;
       if (v >= per_page) continue;
-      uint4 lo, hi;
-      values_of<T>(codes[i], scale_value(scale[i]), &lo, &hi);
-      uint4* dst = reinterpret_cast<uint4*>(to + static_cast<int64_t>(v) * 32);
-      dst[0] = lo;
-      dst[1] = hi;
+      store_values<T>(to + static_cast<int64_t>(v) * 32, codes[i], scale_value(scale[i]));
     }
   }
 }

@@ -7,7 +7,8 @@
 // Layout of threads as in the rotation: a thread owns a vector of eight channels (two, half a head apart) of a token for as
 // many heads as leave every SM full, so that its sines are computed once.
 //
-// What bounds it: memory; 1.5 bytes a number of k and v, 4 of q.
+// What bounds it: memory at first sight (3 bytes a number of k and v, 4 of q), in fact the chain of a row: load, turn, maximum over the
+// row's lanes, codes (4.4 TB/s for three chunks of 4,680 tokens and 12 heads).
 #include <ATen/ATen.h>
 #include <ATen/MemoryOverlap.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -37,12 +38,17 @@ struct Args {
   Exponents range;
 };
 
-// Largest magnitude's bits over the `width` lanes of a row (a power of two; the lanes of a row are active together).
+// Largest magnitude's bits over the `width` lanes of a row (a power of two; all lanes of the warp take part).
 __device__ __forceinline__ uint32_t row_top(uint32_t top, int width) {
-  const int lane = threadIdx.x & 31;
-  const uint32_t lanes = (width == 32 ? 0xffffffffu : (1u << width) - 1u) << (lane & ~(width - 1));
-  for (int o = width >> 1; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(lanes, top, o));
+  for (int o = width >> 1; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
   return top;
+}
+
+// max(top, |a|, |b|), NaN if one of them is.
+__device__ __forceinline__ float top_of(float top, float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(top), "f"(fabsf(a)), "f"(fabsf(b)));
+  return r;
 }
 
 __device__ __forceinline__ uint2 codes_of_vec(const float (&x)[8], float inverse, bool finite) {
@@ -52,32 +58,37 @@ __device__ __forceinline__ uint2 codes_of_vec(const float (&x)[8], float inverse
 }
 
 // kTurn: 0 rows as they are, 1 pairs are neighbours, 2 half a head apart.
+// (Five blocks on an SM: 48.8 us for three chunks of 4,680 tokens, 52.0 with four. Scales gathered over a block's tokens and
+// written together at its end: no faster than a byte each as they come.)
 template <typename T, int kTurn, int kHeads>
-__global__ void __launch_bounds__(kThreads) pack_kernel(const __grid_constant__ Args p) {
+__global__ void __launch_bounds__(kThreads, kTurn == 2 ? 2 : 5) pack_kernel(const __grid_constant__ Args p) {
   paged::let_later();
   paged::after_earlier();
   constexpr bool kHalves = kTurn == 2;
   constexpr int kPairs = kHalves ? 8 : 4, kParts = kHalves ? 2 : 1;
   const rotary::Args& a = p.a;
   const int per_row = a.pairs / kPairs;  // lanes of a row: 4, 8 or 16
-  const int64_t index = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  const int token = static_cast<int>(index / per_row);
-  const int vec = static_cast<int>(index - static_cast<int64_t>(token) * per_row);
-  if (token >= a.tokens) return;
+  const int log_row = 31 - __clz(per_row);
+  const int local = threadIdx.x >> log_row, vec = threadIdx.x & (per_row - 1), tokens = kThreads >> log_row;
+  const int64_t token64 = static_cast<int64_t>(blockIdx.x) * tokens + local;
+  const int token = static_cast<int>(min(token64, static_cast<int64_t>(a.tokens)));
   const int y = blockIdx.y;
   const bool is_q = y < a.q.groups, is_k = !is_q && y < a.q.groups + a.k.groups;
   const Rows& r = is_q ? a.q : is_k ? a.k : a.v;
   const int first = (is_q ? y : is_k ? y - a.q.groups : y - a.q.groups - a.k.groups) * r.per;
-  const int count = min(r.heads - first, r.per);
+  const int heads = min(r.heads - first, r.per);
+  bool active = token < a.tokens;
   const int part_bytes = a.pairs * 2;  // from the first half of a head to the second
   const char* src = r.src + token * r.src_token + first * r.src_head + vec * 16;
 
   uint4 raw[kHeads][kParts];
-  auto load = [&](int i, int head) {
-    if (head < count) {
+  auto load = [&](int i, int head) {  // the next head's vectors
 #pragma unroll
-      for (int s = 0; s < kParts; ++s) raw[i][s] = *reinterpret_cast<const uint4*>(src + head * r.src_head + s * part_bytes);
+    for (int s = 0; s < kParts; ++s) {
+      raw[i][s] = make_uint4(0, 0, 0, 0);
+      if (active && head < heads) raw[i][s] = *reinterpret_cast<const uint4*>(src + s * part_bytes);
     }
+    src += r.src_head;
   };
 #pragma unroll
   for (int i = 0; i < kHeads; ++i) load(i, i);
@@ -89,44 +100,49 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(const __grid_constant__ 
     dst += token * r.dst_token + vec * 16;
   } else {
     int page, row;
-    if (!rotary::place(a, token, vec == 0, &page, &row)) return;
-    dst += page * (is_k ? a.page_k : a.page_v) + row * r.dst_token + vec * 8;
-    scale_head = is_k ? p.k_scale_head : p.v_scale_head;
-    scale = (is_k ? p.k_scales : p.v_scales) + page * (is_k ? p.k_scale_page : p.v_scale_page) + row + first * scale_head;
+    if (active && rotary::place(a, token, vec == 0, &page, &row)) {
+      dst += page * (is_k ? a.page_k : a.page_v) + row * r.dst_token + vec * 8;
+      scale_head = is_k ? p.k_scale_head : p.v_scale_head;
+      scale = (is_k ? p.k_scales : p.v_scales) + page * (is_k ? p.k_scale_page : p.v_scale_page) + row + first * scale_head;
+    } else {
+      active = false;
+    }
   }
 
-  float cs[kPairs], sn[kPairs];
+  float cs[kPairs] = {}, sn[kPairs] = {};
   const bool turned = kTurn != 0 && (is_q || is_k);
-  if (turned) rotary::sines<true>(a, token, vec, cs, sn);  // (a code that falls to its neighbour is 2^-3 off)
+  if (turned && active) rotary::sines<true>(a, token, vec, cs, sn);  // (a code that falls to its neighbour is 2^-3 off)
 
-  for (int done = 0; done < count; done += kHeads) {
+  for (int done = 0; done < heads; done += kHeads) {
 #pragma unroll
     for (int i = 0; i < kHeads; ++i) {
-      if (done + i >= count) continue;
+      if (done + i >= heads) continue;
       float x[8], y2[8];
       Vec<T>::unpack(raw[i][0], x);
       if (kHalves) Vec<T>::unpack(raw[i][kParts - 1], y2);
       if (turned) rotary::turn<kHalves>(x, y2, cs, sn);
       load(i, done + kHeads + i);  // before the stores, which the compiler must take for ones to the same memory
-      char* to = dst + (done + i) * r.dst_head;
+      char* to = dst;
+      dst += r.dst_head;
       if (is_q) {
-        *reinterpret_cast<uint4*>(to) = Vec<T>::pack(x);
-        if (kHalves) *reinterpret_cast<uint4*>(to + part_bytes) = Vec<T>::pack(y2);
+        if (active) *reinterpret_cast<uint4*>(to) = Vec<T>::pack(x);
+        if (active && kHalves) *reinterpret_cast<uint4*>(to + part_bytes) = Vec<T>::pack(y2);
         continue;
       }
-      uint32_t top = 0;
+      float most = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-        if (kHalves) top = max(top, __float_as_uint(y2[e]) & 0x7fffffffu);
+      for (int e = 0; e < 8; e += 2) {
+        most = top_of(most, x[e], x[e + 1]);
+        if (kHalves) most = top_of(most, y2[e], y2[e + 1]);
       }
-      top = row_top(top, per_row);
+      const uint32_t top = row_top(__float_as_uint(most), per_row);
       const bool finite = top < 0x7f800000u;
       const int power = min(max(static_cast<int>(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u), p.range.low), p.range.high);
       const float inverse = __uint_as_float(static_cast<uint32_t>(127 - power) << 23);
-      *reinterpret_cast<uint2*>(to) = codes_of_vec(x, inverse, finite);
-      if (kHalves) *reinterpret_cast<uint2*>(to + a.pairs) = codes_of_vec(y2, inverse, finite);
-      if (vec == 0) scale[(done + i) * scale_head] = static_cast<uint8_t>(finite ? power + 127 : paged::kNanScale);
+      if (active) *reinterpret_cast<uint2*>(to) = codes_of_vec(x, inverse, finite);
+      if (active && kHalves) *reinterpret_cast<uint2*>(to + a.pairs) = codes_of_vec(y2, inverse, finite);
+      if (active && vec == 0) *scale = static_cast<uint8_t>(finite ? power + 127 : paged::kNanScale);
+      scale += scale_head;
     }
   }
 }
@@ -210,64 +226,78 @@ struct Read {
   const int* table;
   int64_t table_row;
   const int* starts;       // [seqs + 1]
-  int seqs, width, heads, vecs, rows;
+  int seqs, width, heads, rows;
+  int tokens;              // of a block
+  int log_vecs;            // vectors of sixteen channels of a head
+  paged::Divider heads_by;
   int* status;
 };
 
-constexpr int kReadItems = 4;  // vectors of sixteen channels of a thread
+constexpr int kReadVectors = 512;  // of a block, about
+constexpr int kReadTokens = 256;    // of a block, at most
 
-// Vectors of sixteen channels, a block kReadItems * 256 consecutive ones of K or V.
+// A block reads K or V of some consecutive rows: first a thread for each finds its place, then all fetch vectors of sixteen
+// channels (many small blocks: deeper loops at fewer blocks were slower).
 template <typename T>
 __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ Read p) {
+  __shared__ int64_t code_at[kReadTokens], scale_at[kReadTokens];  // (-1: reads as zeros, -2: a row of no sequence)
   paged::let_later();
   paged::after_earlier();
   const int which = blockIdx.y;
   const paged::Packed& pages = which ? p.pages[1] : p.pages[0];
   const uint8_t* base = which ? p.codes[1] : p.codes[0];
-  char* out = which ? p.out[1] : p.out[0];
-  const int per_token = p.heads * p.vecs;
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * kThreads * kReadItems + threadIdx.x;
-  uint4 codes[kReadItems];
-  int scale[kReadItems];
-  int seq = -1;
-#pragma unroll
-  for (int i = 0; i < kReadItems; ++i) {
-    const int64_t at = first + i * kThreads;
-    const int64_t token = at / per_token;
-    scale[i] = -1;
-    if (token >= p.rows) continue;
-    const int part = static_cast<int>(at - token * per_token), head = part / p.vecs, vec = part - head * p.vecs;
-    if (seq < 0) {
-      int hi = p.seqs - 1;  // the last sequence that starts at or before the token
-      seq = 0;
-      while (seq < hi) {
-        const int mid = (seq + hi + 1) >> 1;
-        if (p.starts[mid] <= token) seq = mid;
-        else hi = mid - 1;
+  const int token0 = static_cast<int>(blockIdx.x) * p.tokens, tokens = min(p.tokens, p.rows - token0);
+  if (static_cast<int>(threadIdx.x) < tokens) {
+    const int token = token0 + static_cast<int>(threadIdx.x);
+    int seq = 0, hi = p.seqs - 1;  // the last sequence that starts at or before the token
+    while (seq < hi) {
+      const int mid = (seq + hi + 1) >> 1;
+      if (p.starts[mid] <= token) seq = mid;
+      else hi = mid - 1;
+    }
+    const int begin = p.starts[seq], end = p.starts[seq + 1];
+    int64_t code = -2, scale = 0;
+    if (token >= begin && token < end) {
+      const int pos = token - begin, slot = pos / pages.size, row = pos - slot * pages.size;
+      const int page = slot < p.width ? p.table[seq * p.table_row + slot] : -1;
+      if (page >= 0 && page < pages.count) {
+        code = page * pages.page_stride + row * pages.token_stride;
+        scale = page * pages.scale_page + row;
+      } else {
+        code = -1;
+        if (p.status != nullptr) atomicCAS(p.status + kPagedWord, 0, kPageRange);
       }
     }
-    while (seq + 1 < p.seqs && p.starts[seq + 1] <= token) ++seq;
-    const int begin = p.starts[seq], end = p.starts[seq + 1];
-    if (token < begin || token >= end) continue;  // rows of no sequence
-    const int pos = static_cast<int>(token) - begin, slot = pos / pages.size, row = pos - slot * pages.size;
-    const int page = slot < p.width ? p.table[seq * p.table_row + slot] : -1;
-    if (page < 0 || page >= pages.count) {  // reads as zeros
-      if (vec == 0 && p.status != nullptr) atomicCAS(p.status + kPagedWord, 0, kPageRange);
-      codes[i] = make_uint4(0, 0, 0, 0);
-      scale[i] = 127;
-      continue;
-    }
-    codes[i] = *reinterpret_cast<const uint4*>(base + page * pages.page_stride + row * pages.token_stride + head * pages.head_stride + vec * 16);
-    scale[i] = pages.scales[page * pages.scale_page + head * pages.scale_head + row];
+    code_at[threadIdx.x] = code;
+    scale_at[threadIdx.x] = scale;
   }
+  __syncthreads();
+  uint4* out = reinterpret_cast<uint4*>(which ? p.out[1] : p.out[0]) + static_cast<int64_t>(token0) * p.heads * 2 * (1 << p.log_vecs);
+  const int vectors = (tokens * p.heads) << p.log_vecs;
+  constexpr int kDepth = 2;
+  for (int v0 = threadIdx.x; v0 < vectors; v0 += kThreads * kDepth) {
+    uint4 codes[kDepth];
+    int scale[kDepth];
 #pragma unroll
-  for (int i = 0; i < kReadItems; ++i) {
-    if (scale[i] < 0) continue;
-    uint4 lo, hi;
-    paged::values_of<T>(codes[i], paged::scale_value(scale[i]), &lo, &hi);
-    uint4* to = reinterpret_cast<uint4*>(out + (first + i * kThreads) * 32);
-    to[0] = lo;
-    to[1] = hi;
+    for (int i = 0; i < kDepth; ++i) {
+      const int v = v0 + i * kThreads, row = v >> p.log_vecs, vec = v - (row << p.log_vecs);
+      scale[i] = -1;
+      if (v >= vectors) continue;
+      const int token = p.heads_by.over(row), head = row - token * p.heads;
+      const int64_t at = code_at[token];
+      codes[i] = make_uint4(0, 0, 0, 0);
+      if (at >= 0) {
+        codes[i] = *reinterpret_cast<const uint4*>(base + at + head * pages.head_stride + vec * 16);
+        scale[i] = pages.scales[scale_at[token] + head * pages.scale_head];
+      } else if (at == -1) {
+        scale[i] = 127;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kDepth; ++i) {
+      if (scale[i] < 0) continue;
+      paged::store_values<T>(out + 2 * (v0 + i * kThreads), codes[i], paged::scale_value(scale[i]));
+    }
   }
 }
 
@@ -355,11 +385,13 @@ std::pair<at::Tensor, at::Tensor> packed_read(const at::Tensor& k_codes, const a
   p.seqs = static_cast<int>(table.size(0));
   p.width = static_cast<int>(table.size(1));
   p.heads = static_cast<int>(heads);
-  p.vecs = static_cast<int>(d / 16);
+  p.log_vecs = d == 128 ? 3 : 2;
   p.rows = static_cast<int>(rows);
+  RC_CHECK(heads < (1 << 20), "too many KV heads");
+  p.heads_by = paged::Divider::of(static_cast<int>(heads));
+  p.tokens = static_cast<int>(std::min<int64_t>(pack::kReadTokens, std::max<int64_t>(1, pack::kReadVectors / (heads * (d / 16)))));
   p.status = status_ptr(status);
-  const int64_t each = static_cast<int64_t>(pack::kThreads) * pack::kReadItems, blocks = (rows * heads * p.vecs + each - 1) / each;
-  RC_CHECK(blocks < (1ll << 31), "too many rows for one launch");
+  const int64_t blocks = (rows + p.tokens - 1) / p.tokens;
   paged::launch(type == at::kHalf ? pack::read_kernel<__half> : pack::read_kernel<__nv_bfloat16>, dim3(static_cast<unsigned>(blocks), 2),
                 pack::kThreads, 0, 0, c10::cuda::getCurrentCUDAStream(k_codes.get_device()).stream(), p);
   return {out[0], out[1]};

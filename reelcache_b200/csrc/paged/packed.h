@@ -79,9 +79,9 @@ __device__ __forceinline__ uint32_t codes_of(float lo, float hi) {
   return out;
 }
 
-// Sixteen codes times a scale as 16-bit numbers, exactly.
+// Sixteen codes times a scale as 16-bit numbers, exactly, to 32 aligned bytes (a whole sector in one store).
 template <typename T>
-__device__ __forceinline__ void values_of(const uint4& codes, float scale, uint4* lo, uint4* hi) {
+__device__ __forceinline__ void store_values(void* dst, const uint4& codes, float scale) {
   const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
   uint32_t out[8];
 #pragma unroll
@@ -89,20 +89,19 @@ __device__ __forceinline__ void values_of(const uint4& codes, float scale, uint4
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const uint32_t two = h ? upper_codes_to_half2(w[i]) : codes_to_half2(w[i]);
-      float2 f = __half22float2(*reinterpret_cast<const __half2*>(&two));
-      f.x *= scale;
-      f.y *= scale;
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&two));
       if (std::is_same<T, __half>::value) {
-        const __half2 v = __floats2half2_rn(f.x, f.y);
+        const __half2 v = __floats2half2_rn(f.x * scale, f.y * scale);
         out[2 * i + h] = *reinterpret_cast<const uint32_t*>(&v);
       } else {
-        const __nv_bfloat162 v = __floats2bfloat162_rn(f.x, f.y);
+        const __nv_bfloat162 v = __floats2bfloat162_rn(f.x * scale, f.y * scale);
         out[2 * i + h] = *reinterpret_cast<const uint32_t*>(&v);
       }
     }
   }
-  *lo = make_uint4(out[0], out[1], out[2], out[3]);
-  *hi = make_uint4(out[4], out[5], out[6], out[7]);
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(out[0]), "r"(out[1]), "r"(out[2]), "r"(out[3]),
+               "r"(out[4]), "r"(out[5]), "r"(out[6]), "r"(out[7])
+               : "memory");
 }
 #endif
 

@@ -77,6 +77,22 @@ void launch(void (*kernel)(Params...), dim3 grid, int threads, int smem, int clu
 }
 #endif
 
+// Division by a number below 2^24 of numbers below 2^31 as a product (an integer division takes some hundred cycles, of which a
+// chain of small steps has few to spare).
+struct Divider {
+  uint32_t magic, shift;
+  int by;
+  static Divider of(int by) {
+    uint32_t bits = 0;
+    while ((int64_t{1} << bits) < by) ++bits;
+    return {static_cast<uint32_t>(((uint64_t{1} << (31 + bits)) + by - 1) / by), 31 + bits, by};
+  }
+#ifdef __CUDACC__
+  __device__ __forceinline__ int over(int n) const { return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * magic) >> shift); }
+  __device__ __forceinline__ int up(int n) const { return over(n) + (n > over(n) * by); }  // rounded up
+#endif
+};
+
 struct Pages {  // [pages, page_size, kv_heads, head_dim], strides in elements
   int count, size;
   int64_t page_stride, token_stride, head_stride;

@@ -10,9 +10,9 @@
 // of a sum moves them by 2^-50 of their size: the same for every batch and form of the kernel. Equal scores go to the lower
 // block. Few blocks need FP64. Scores come from the tensor core first, the pooled query (summed in FP32) as three 16-bit
 // numbers that add up to it, a single token as itself. What they may be off by is summed next to them, as one more product:
-// with x the pooled query, y the sum of the tokens' magnitudes and m the mean, 2^-15.8 sum |x| |m| for the products (8 steps, each a
-// sum of 17 terms cut at 2^-23 of the largest; those of the small numbers come first and count for little) and n 2^-24 sum y |m| for
-// the FP32 sums of n terms one after the other. With T the keep-th largest score and E the largest bound, blocks above T + 2 E
+// with x the pooled query, y the sum of the tokens' magnitudes and m the mean, 2^-18.5 sum |x| |m| for the products (16 channels at a
+// time, a sum of 16 terms cut at 2^-23 of the largest: 2^-19; those added in FP32: 2^-21; the small numbers' with them 2^-22) and n
+// 2^-24 sum y |m| for the FP32 sums of n terms one after the other. With T the keep-th largest score and E the largest bound, blocks above T + 2 E
 // are chosen and blocks below T - 2 E are not; only where there is more than one way to choose from those between are they
 // computed again, in FP64 (in a call of 128 query blocks and heads for a few of them).
 //
@@ -36,20 +36,6 @@
 
 namespace rc {
 namespace paged {
-
-// Division by a number below 2^24 of numbers below 2^31 as a product (an integer division takes some hundred cycles, of which a
-// chain of small steps has few to spare).
-struct Divider {
-  uint32_t magic, shift;
-  int by;
-  static Divider of(int by) {
-    uint32_t bits = 0;
-    while ((int64_t{1} << bits) < by) ++bits;
-    return {static_cast<uint32_t>(((uint64_t{1} << (31 + bits)) + by - 1) / by), 31 + bits, by};
-  }
-  __device__ __forceinline__ int over(int n) const { return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * magic) >> shift); }
-  __device__ __forceinline__ int up(int n) const { return over(n) + (n > over(n) * by); }  // rounded up
-};
 
 // -- means ------------------------------------------------------------------------------------------------------------
 
@@ -153,6 +139,7 @@ __global__ void __launch_bounds__(kMeanThreads) means_kernel(const __grid_consta
 constexpr int kSelectThreads = 256;
 constexpr int kSelectWarps = kSelectThreads / 32;
 constexpr int kMostBlocks = 12288;  // whose keys fit one CTA's shared memory
+constexpr float kProductError = 0x1.6p-19f;
 constexpr int kBuckets = 256;       // one for each thread
 constexpr int kPieces = 3;          // 16-bit numbers that add up to a pooled query; a fourth row holds what bounds its errors
 
@@ -482,6 +469,18 @@ __global__ void __launch_bounds__(kSelectThreads, 3) select_kernel(const __grid_
     return p.means + page * p.mean_page + (b - p.per_page.over(b) * p.per_page.by) * p.mean_block + head * p.mean_head;
   };
 
+  // blocks in order: the first ones, the chosen, the last ones; what is not chosen is written while the rest waits for its loads
+  const auto write = [&](int at, int b) {
+    const int slot = p.per_page.over(b), page = table[slot];
+    out[at] = page >= 0 && page < a.pages ? (page - slot) * p.per_page.by + b : -1;
+  };
+  if (rank == p.cluster - 1) {
+    const int last = blocks - high;
+    for (int i = kSelectThreads - 1 - static_cast<int>(threadIdx.x); i < p.width - keep; i += kSelectThreads) {
+      if (i < low + last) write(i < low ? i : i + keep, i < low ? i : high + i - low);
+      else out[i + keep] = -1;
+    }
+  }
   if (scored) {
     // This CTA's part of the candidates, sixteen to a warp: rows r0 and r0 + 8 of the operand, channels 32 j + 8 quad and on (any
     // order of channels gives the same sum), heads 2 quad and 2 quad + 1 of the result. The first ones are asked for before the queries.
@@ -532,7 +531,7 @@ __global__ void __launch_bounds__(kSelectThreads, 3) select_kernel(const __grid_
       __syncthreads();
       // their pieces, a warp a head; fp16's are of a multiple by a power of two that brings the bounds' largest between 2^13 and
       // 2^14: what the last piece cannot hold is below 2^-25, with 128 means of 2^16 at most 0.25
-      const float steps = static_cast<float>(count / splits + 1 + splits) * (0x1p-24f / 0x1.2p-16f);  // of the sums in FP32, over that of the products
+      const float steps = static_cast<float>(count / splits + 1 + splits) * (0x1p-24f / kProductError);  // of the sums in FP32, over that of the products
       for (int h = warp; h < a.group; h += kSelectWarps) {
         constexpr int kPer = D / 32;
         float x[kPer], y[kPer], top = 0.0f;
@@ -580,8 +579,9 @@ __global__ void __launch_bounds__(kSelectThreads, 3) select_kernel(const __grid_
       float best[2] = {-INFINITY, -INFINITY};
       for (int tile = 0; tile < shape.tiles; ++tile) {
         const uint8_t* piece = pieces + ((tile * 8 + r0) * (kPieces + 1)) * SelectShape<D>::piece_row + quad * 16;
+        // the products of 16 channels by themselves, added in FP32: a sum over all of them would be cut at each step
         float sc[4] = {}, size[4] = {};
-        for (int k = used - 1; k >= 0; --k) {
+        for (int k = used - 1; k > 0; --k) {
 #pragma unroll
           for (int j = 0; j < D / 32; ++j) {
             const uint4 b = *reinterpret_cast<const uint4*>(piece + k * SelectShape<D>::piece_row + j * 64);
@@ -592,9 +592,14 @@ __global__ void __launch_bounds__(kSelectThreads, 3) select_kernel(const __grid_
 #pragma unroll
         for (int j = 0; j < D / 32; ++j) {
           constexpr uint32_t kSize = 0x7fff7fffu;
-          const uint4 b = *reinterpret_cast<const uint4*>(piece + kPieces * SelectShape<D>::piece_row + j * 64);
-          mma_means(size, Operand{mean[0][j].x & kSize, mean[1][j].x & kSize, mean[0][j].y & kSize, mean[1][j].y & kSize}, b.x, b.y, T());
-          mma_means(size, Operand{mean[0][j].z & kSize, mean[1][j].z & kSize, mean[0][j].w & kSize, mean[1][j].w & kSize}, b.z, b.w, T());
+          const uint4 b = *reinterpret_cast<const uint4*>(piece + j * 64), y = *reinterpret_cast<const uint4*>(piece + kPieces * SelectShape<D>::piece_row + j * 64);
+          float one[4] = {}, two[4] = {};
+          mma_means(one, Operand{mean[0][j].x, mean[1][j].x, mean[0][j].y, mean[1][j].y}, b.x, b.y, T());
+          mma_means(two, Operand{mean[0][j].z, mean[1][j].z, mean[0][j].w, mean[1][j].w}, b.z, b.w, T());
+          mma_means(size, Operand{mean[0][j].x & kSize, mean[1][j].x & kSize, mean[0][j].y & kSize, mean[1][j].y & kSize}, y.x, y.y, T());
+          mma_means(size, Operand{mean[0][j].z & kSize, mean[1][j].z & kSize, mean[0][j].w & kSize, mean[1][j].w & kSize}, y.z, y.w, T());
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[e] += one[e] + two[e];
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -603,7 +608,7 @@ __global__ void __launch_bounds__(kSelectThreads, 3) select_kernel(const __grid_
           const float x = sc[e] * scales[h];
           best[e >> 1] = fmaxf(best[e >> 1], x);
           // (a bound or score that is no number makes every block one that is computed again)
-          const float bound = fmaf(size[e], 0x1.24p-16f, std::is_same<T, __half>::value && used > 1 ? 0.25f : 0.0f) * scales[h];
+          const float bound = fmaf(size[e], kProductError * 1.02f, std::is_same<T, __half>::value && used > 1 ? 0.25f : 0.0f) * scales[h];
           most = bound < INFINITY && fabsf(x) < INFINITY ? fmaxf(most, bound) : INFINITY;
         }
       }
@@ -637,14 +642,6 @@ __global__ void __launch_bounds__(kSelectThreads, 3) select_kernel(const __grid_
   else __syncthreads();
   if (rank != 0) return;
 
-  // blocks in order: the first ones, the chosen, the last ones
-  const auto write = [&](int at, int b) {
-    const int slot = p.per_page.over(b), page = table[slot];
-    out[at] = page >= 0 && page < a.pages ? (page - slot) * p.per_page.by + b : -1;
-  };
-  for (int i = threadIdx.x; i < low; i += kSelectThreads) write(i, i);
-  for (int i = threadIdx.x; i < blocks - high; i += kSelectThreads) write(low + keep + i, high + i);
-  for (int i = chosen + static_cast<int>(threadIdx.x); i < p.width; i += kSelectThreads) out[i] = -1;
   if (!scored) {
     for (int i = threadIdx.x; i < keep; i += kSelectThreads) write(low + i, low + i);
     return;
