@@ -94,11 +94,11 @@ void pages_allocate(at::Tensor& state, int64_t pages, int64_t seqs_held, int64_t
                     const at::Tensor& new_lens, const c10::optional<at::Tensor>& status);
 void pages_fork(at::Tensor& state, int64_t pages, int64_t seqs_held, int64_t page_size, const at::Tensor& parents,
                 const at::Tensor& children, const at::Tensor& at_lens, at::Tensor& storage,
-                const c10::optional<at::Tensor>& status);
+                const c10::optional<at::Tensor>& status, const std::vector<at::Tensor>& sides);
 void pages_release(at::Tensor& state, int64_t pages, int64_t seqs_held, int64_t page_size, const at::Tensor& seqs,
                    const c10::optional<at::Tensor>& status);
 at::Tensor pages_compact(at::Tensor& state, int64_t pages, int64_t seqs_held, int64_t page_size, at::Tensor& storage,
-                         const c10::optional<at::Tensor>& status);
+                         const c10::optional<at::Tensor>& status, const std::vector<at::Tensor>& sides);
 void pages_copy(at::Tensor& storage, const at::Tensor& source, const at::Tensor& target,
                 const c10::optional<at::Tensor>& rows, const c10::optional<at::Tensor>& status);
 }  // namespace rc
@@ -210,11 +210,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("pages_allocate", &rc::pages_allocate, "grow sequences of a page table", py::arg("state"), py::arg("pages"), py::arg("seqs_held"), py::arg("page_size"), py::arg("seqs"), py::arg("new_lens"), py::arg("status") = py::none());
   m.def("pages_fork", &rc::pages_fork, "share pages with forked sequences, copy partial tails", py::arg("state"),
         py::arg("pages"), py::arg("seqs_held"), py::arg("page_size"), py::arg("parents"), py::arg("children"),
-        py::arg("at_lens"), py::arg("storage"), py::arg("status") = py::none());
+        py::arg("at_lens"), py::arg("storage"), py::arg("status") = py::none(), py::arg("sides") = std::vector<at::Tensor>());
   m.def("pages_release", &rc::pages_release, "give the pages of sequences back", py::arg("state"), py::arg("pages"), py::arg("seqs_held"), py::arg("page_size"), py::arg("seqs"), py::arg("status") = py::none());
   m.def("pages_compact", &rc::pages_compact, "move the pages in use to the front; returns their number (on the device)",
         py::arg("state"), py::arg("pages"), py::arg("seqs_held"), py::arg("page_size"), py::arg("storage"),
-        py::arg("status") = py::none());
+        py::arg("status") = py::none(), py::arg("sides") = std::vector<at::Tensor>());
   m.def("pages_copy", &rc::pages_copy, "copy pages (or their first rows) in every plane", py::arg("storage"),
         py::arg("source"), py::arg("target"), py::arg("rows") = py::none(), py::arg("status") = py::none());
 }

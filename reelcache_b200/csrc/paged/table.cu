@@ -10,6 +10,7 @@
 //   release   a sequence gives its pages back
 //   compact   with n pages in use, those at n and above move to the free ones below n (i-th to i-th); tables follow
 //   copy      given pages (or their first rows) to given others
+// What lies beside the pages (scales of packed ones, means of blocks) moves with them, whole pages of it.
 //
 // allocate, fork and compact start with a plan by one block of 1,024 threads: prefix sums over the call's sequences and
 // over refcount, which it reads only as far as it finds what it needs. A call that cannot be served (too few free pages,
@@ -24,6 +25,7 @@
 
 #include <algorithm>
 #include <string>
+#include <vector>
 
 #include "../common/host.h"
 #include "paged.h"
@@ -292,6 +294,34 @@ __device__ __forceinline__ void move_pages(const Storage& st, int moves, int pag
   }
 }
 
+// Tensors beside the storage, [planes, pages, ...], of which whole pages move: in words of 8 bytes, small next to the pages.
+struct Side {
+  char* base;
+  int64_t plane_stride, page_stride;
+  int planes, words;
+};
+constexpr int kMostSides = 2;
+struct Sides {
+  Side at[kMostSides];
+  int count;
+};
+
+__device__ __forceinline__ void move_sides(const Sides& sides, int moves, int pages, const int* source, const int* target, const int* rows) {
+  for (int i = 0; i < sides.count; ++i) {
+    const Side& side = sides.at[i];
+    const int64_t each = static_cast<int64_t>(side.planes) * side.words, items = moves * each;
+    for (int64_t item = static_cast<int64_t>(blockIdx.x) * kMoveThreads + threadIdx.x; item < items; item += static_cast<int64_t>(gridDim.x) * kMoveThreads) {
+      const int move = static_cast<int>(item / each);
+      const int64_t rest = item - move * each, plane = rest / side.words, word = rest - plane * side.words;
+      if (rows != nullptr && rows[move] == 0) continue;
+      const int src = source[move], dst = target[move];
+      if (src < 0 || src >= pages || dst < 0 || dst >= pages) continue;  // (reported with the pages)
+      char* base = side.base + plane * side.plane_stride + word * 8;
+      *reinterpret_cast<uint2*>(base + dst * side.page_stride) = *reinterpret_cast<const uint2*>(base + src * side.page_stride);
+    }
+  }
+}
+
 __global__ void __launch_bounds__(kMoveThreads) copy_kernel(Storage st, int pages, const int* source, const int* target,
                                                             const int* rows, int moves, int* status) {
   paged::let_later();
@@ -299,7 +329,7 @@ __global__ void __launch_bounds__(kMoveThreads) copy_kernel(Storage st, int page
   move_pages(st, moves, pages, source, target, rows, status);
 }
 
-__global__ void __launch_bounds__(kMoveThreads) fork_kernel(State s, Storage st, const int* parents, const int* children,
+__global__ void __launch_bounds__(kMoveThreads) fork_kernel(State s, Storage st, Sides sides, const int* parents, const int* children,
                                                             const int* at, int n, Plan plan, int* status) {
   paged::let_later();
   paged::after_earlier();
@@ -321,9 +351,10 @@ __global__ void __launch_bounds__(kMoveThreads) fork_kernel(State s, Storage st,
     if (block == 0) s.lens[child] = len;
   }
   move_pages(st, n, s.pages, plan.source, plan.target, plan.rows, status);
+  move_sides(sides, n, s.pages, plan.source, plan.target, plan.rows);
 }
 
-__global__ void __launch_bounds__(kMoveThreads) compact_kernel(State s, Storage st, const int* place, const int* in_use, Plan plan,
+__global__ void __launch_bounds__(kMoveThreads) compact_kernel(State s, Storage st, Sides sides, const int* place, const int* in_use, Plan plan,
                                                                int* status) {
   paged::let_later();
   paged::after_earlier();
@@ -340,6 +371,7 @@ __global__ void __launch_bounds__(kMoveThreads) compact_kernel(State s, Storage 
     s.refcount[plan.source[m]] = 0;
   }
   move_pages(st, moves, s.pages, plan.source, plan.target, nullptr, status);
+  move_sides(sides, moves, s.pages, plan.source, plan.target, nullptr);
 }
 
 __global__ void __launch_bounds__(kMoveThreads) release_kernel(State s, const int* seqs, int n, int* status) {
@@ -407,6 +439,31 @@ Storage check_storage(at::Tensor& t, int64_t pages, int64_t page_size, const at:
           inner * size, static_cast<int>(row)};
 }
 
+// sides: [planes, pages, ...], pages whole, contiguous and of 8-byte words, planes anywhere.
+Sides check_sides(const std::vector<at::Tensor>& tensors, int64_t pages, const at::Device& device) {
+  RC_CHECK(tensors.size() <= kMostSides, "at most " + std::to_string(kMostSides) + " tensors beside the storage");
+  Sides sides{};
+  for (const at::Tensor& t : tensors) {
+    refuse_gradients({&t}, "moving pages");
+    RC_CHECK(t.device() == device && t.dim() >= 2 && t.size(1) == pages && t.numel() > 0,
+             "a tensor beside the storage must be [planes, pages, ...] on the page table's device");
+    const int64_t size = t.element_size();
+    int64_t inner = 1;
+    bool dense = true;
+    for (int64_t d = t.dim() - 1; d >= 2; --d) {
+      dense = dense && (t.stride(d) == inner || t.size(d) == 1);
+      inner *= t.size(d);
+    }
+    RC_CHECK(dense && (inner * size) % 8 == 0 && inner * size < (1ll << 31) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 8 == 0 &&
+                 (t.stride(0) * size) % 8 == 0 && (t.stride(1) * size) % 8 == 0 && (pages == 1 || t.stride(1) >= inner) &&
+                 (t.size(0) == 1 || t.stride(0) >= inner) && t.size(0) < (1 << 24),
+             "pages of a tensor beside the storage must be contiguous, apart and multiples of 8 bytes");
+    sides.at[sides.count++] = {static_cast<char*>(t.data_ptr()), t.stride(0) * size, t.stride(1) * size, static_cast<int>(t.size(0)),
+                               static_cast<int>(inner * size / 8)};
+  }
+  return sides;
+}
+
 int move_grid(int device) { return sm_count(device) * 8; }
 
 }  // namespace pagetable
@@ -432,13 +489,14 @@ void pages_allocate(at::Tensor& state, int64_t pages, int64_t seqs_held, int64_t
 
 void pages_fork(at::Tensor& state, int64_t pages, int64_t seqs_held, int64_t page_size, const at::Tensor& parents,
                 const at::Tensor& children, const at::Tensor& at_lens, at::Tensor& storage,
-                const c10::optional<at::Tensor>& status) {
+                const c10::optional<at::Tensor>& status, const std::vector<at::Tensor>& sides) {
   const State s = pagetable::check_state(state, pages, seqs_held, page_size);
   const int64_t n = parents.numel();
   const int* from = pagetable::check_list(parents, state.device(), n, "parents");
   const int* to = pagetable::check_list(children, state.device(), n, "children");
   const int* len = pagetable::check_list(at_lens, state.device(), n, "lens");
   const pagetable::Storage st = pagetable::check_storage(storage, s.pages, page_size, state.device());
+  const pagetable::Sides beside = pagetable::check_sides(sides, s.pages, state.device());
   if (n == 0) return;
   c10::cuda::CUDAGuard guard(state.device());
   cudaStream_t stream = c10::cuda::getCurrentCUDAStream(state.get_device()).stream();
@@ -449,9 +507,10 @@ void pages_fork(at::Tensor& state, int64_t pages, int64_t seqs_held, int64_t pag
   paged::launch(pagetable::fork_plan_kernel, dim3(1), pagetable::kPlanThreads, 0, 0, stream, s, from, to, len, static_cast<int>(n), list,
                                                                         list + s.pages, plan, status_ptr(status));
   paged::launch(pagetable::fork_kernel, dim3(pagetable::move_grid(state.get_device())), pagetable::kMoveThreads, 0, 0, stream,
-      s, st, from, to, len, static_cast<int>(n), plan, status_ptr(status));
+      s, st, beside, from, to, len, static_cast<int>(n), plan, status_ptr(status));
   written(state);
   written(storage);
+  for (const at::Tensor& t : sides) written(t);
 }
 
 void pages_release(at::Tensor& state, int64_t pages, int64_t seqs_held, int64_t page_size, const at::Tensor& seqs,
@@ -470,9 +529,10 @@ void pages_release(at::Tensor& state, int64_t pages, int64_t seqs_held, int64_t 
 
 // Returns an int32 tensor of one entry: the pages in use, which after the call are pages 0 .. in_use.
 at::Tensor pages_compact(at::Tensor& state, int64_t pages, int64_t seqs_held, int64_t page_size, at::Tensor& storage,
-                         const c10::optional<at::Tensor>& status) {
+                         const c10::optional<at::Tensor>& status, const std::vector<at::Tensor>& sides) {
   const State s = pagetable::check_state(state, pages, seqs_held, page_size);
   const pagetable::Storage st = pagetable::check_storage(storage, s.pages, page_size, state.device());
+  const pagetable::Sides beside = pagetable::check_sides(sides, s.pages, state.device());
   c10::cuda::CUDAGuard guard(state.device());
   cudaStream_t stream = c10::cuda::getCurrentCUDAStream(state.get_device()).stream();
   at::Tensor scratch = at::empty({1 + 3 * s.pages}, state.options());
@@ -482,9 +542,10 @@ at::Tensor pages_compact(at::Tensor& state, int64_t pages, int64_t seqs_held, in
   int* place = p + 1 + 2 * static_cast<int64_t>(s.pages);
   paged::launch(pagetable::compact_plan_kernel, dim3(1), pagetable::kPlanThreads, 0, 0, stream, s, place, plan, in_use.data_ptr<int>());
   paged::launch(pagetable::compact_kernel, dim3(pagetable::move_grid(state.get_device())), pagetable::kMoveThreads, 0, 0, stream,
-      s, st, place, in_use.data_ptr<int>(), plan, status_ptr(status));
+      s, st, beside, place, in_use.data_ptr<int>(), plan, status_ptr(status));
   written(state);
   written(storage);
+  for (const at::Tensor& t : sides) written(t);
   return in_use;
 }
 

@@ -296,11 +296,13 @@ class CausalWanDiT:
                                 enumerate(zip(ends, self._session_rope.sections))], dim=1)
                      for table in self._session_rope.kernel_tables(self.device))
 
-    def forward_sessions(self, latents: torch.Tensor, t: float, cache, batch, text_kv, *, capture=None) -> torch.Tensor:
+    def forward_sessions(self, latents: torch.Tensor, t: float, cache, batch, text_kv, *, capture=None, sparse=None) -> torch.Tensor:
         """One forward of the newest chunk of several sessions of a :class:`~reelcache_b200.paged_cache.PagedKVCache`
         (``batch`` from its ``extend`` or ``again``, a chunk for each): ``latents[sessions, in_dim, F, H, W]`` at timestep
         ``t``, the weights read once for all of them, histories shared page by page between forks. Same block math as
         :meth:`forward_chunk`, by the same kernels but for the attention over pages. ``capture(layer, k_pre, v)`` receives the rows of all sessions, one after the other.
+        A packed cache holds the rotated rows in 8 bits. ``sparse`` (``keep``, ``query_block``, ``sinks`` and ``recent`` of the cache's
+        ``attend``) keeps self-attention to the chunk itself and chosen blocks of its past.
         Returns the flow predictions ``[sessions, in_dim, F, H, W]`` (FP32)."""
         cfg = self.cfg
         tokens, sessions = cfg.chunk_tokens, len(batch.sessions)
@@ -313,19 +315,25 @@ class CausalWanDiT:
                         self.patch_b)
         e, e0 = self.time_modulation(t)
         cos_tok, sin_tok = self.session_rope([n // tokens - 1 for n in batch.lengths])
-        kv_rows = cache.new_rows(batch)
+        kv_rows = None if cache.packed else cache.new_rows(batch)
         heads = (rows, cfg.heads, cfg.head_dim)
         q = torch.empty((rows, cfg.dim), dtype=torch.bfloat16, device=self.device)
+        k_new, v_new = (torch.empty_like(q), torch.empty_like(q)) if cache.packed else (None, None)
         for layer, blk in enumerate(self.blocks):
             mod = blk["modulation"] + e0
             y = norms.ln_modulate(x, shift=mod[0], scale=mod[1], eps=cfg.eps)
             qkv = gemm.linear(y, blk["qkv_w"], blk["qkv_b"])
             k_pre = torch.empty_like(q) if capture is not None else None
-            norms.qkv_norm_rope(qkv, blk["norm_q"], blk["norm_k"], cos_tok, sin_tok, q, cache.token_rows(layer, "K"),
-                                cache.token_rows(layer, "V"), head_dim=cfg.head_dim, k_pre=k_pre, kv_rows=kv_rows, eps=cfg.eps)
+            k_rows, v_rows = (k_new, v_new) if cache.packed else (cache.token_rows(layer, "K"), cache.token_rows(layer, "V"))
+            norms.qkv_norm_rope(qkv, blk["norm_q"], blk["norm_k"], cos_tok, sin_tok, q, k_rows, v_rows, head_dim=cfg.head_dim,
+                                k_pre=k_pre, kv_rows=kv_rows, eps=cfg.eps)
+            if cache.packed:
+                cache.store(layer, batch, k_new.view(heads), v_new.view(heads))
+            else:
+                cache.rows_written(layer, batch)
             if capture is not None:
                 capture(layer, k_pre, qkv[:, 2 * cfg.dim:])
-            o = cache.attend(layer, batch, q.view(heads))
+            o = cache.attend(layer, batch, q.view(heads), **(sparse or {}))
             gemm.linear_gated_residual(o.view(rows, cfg.dim), blk["o_w"], blk["o_b"], mod[2].contiguous(), x)
             y = norms.ln_modulate(x, weight=blk["norm3_w"], bias=blk["norm3_b"], eps=cfg.eps)
             cq = norms.rms_norm(gemm.linear(y, blk["cq_w"], blk["cq_b"]), blk["cnorm_q"], eps=cfg.eps)

@@ -251,17 +251,18 @@ class PageTable:
         """Sequences ``seqs[i]`` grow to ``lens[i]`` tokens (at least what they hold)."""
         ext().pages_allocate(*self._parts(), seqs, lens, status_word(self.state.device))
 
-    def fork(self, parents, children, lens, storage):
+    def fork(self, parents, children, lens, storage, sides=()):
         """Sequences ``children[i]`` (holding nothing) take the first ``lens[i]`` tokens of ``parents[i]``: whole pages
         are shared, the rows of a partly filled last page are copied in every plane of ``storage [planes, pages,
-        page_size, ...]`` to a page of the child's own."""
-        ext().pages_fork(*self._parts(), parents, children, lens, storage, status_word(self.state.device))
+        page_size, ...]`` to a page of the child's own, and with them its page in ``sides`` (up to two tensors ``[planes, pages,
+        ...]``: scales of packed pages, means of blocks)."""
+        ext().pages_fork(*self._parts(), parents, children, lens, storage, status_word(self.state.device), list(sides))
 
     def release(self, seqs):
         """Sequences ``seqs[i]`` give all their pages back; a page is free when no sequence holds it."""
         ext().pages_release(*self._parts(), seqs, status_word(self.state.device))
 
-    def compact(self, storage) -> torch.Tensor:
-        """Move the pages in use to the front of ``storage`` and follow them in the tables. Returns their number, an
-        int32 tensor of one entry on the device."""
-        return ext().pages_compact(*self._parts(), storage, status_word(self.state.device))
+    def compact(self, storage, sides=()) -> torch.Tensor:
+        """Move the pages in use to the front of ``storage`` (and of ``sides``) and follow them in the tables. Returns their
+        number, an int32 tensor of one entry on the device."""
+        return ext().pages_compact(*self._parts(), storage, status_word(self.state.device), list(sides))

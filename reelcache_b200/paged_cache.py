@@ -10,6 +10,9 @@ A step over a batch of sessions::
     q = cache.append(layer, batch, q, k, v, positions, rope)
     o = cache.attend(layer, batch, q)
 
+Rows can be held in 8 bits (``packed``), and attention kept to blocks of the history that a cheap score chooses (``block``, and
+``keep`` in :meth:`PagedKVCache.attend`).
+
 A session is rewound by forking it at the earlier length and closing it. A batch is good as long as its sessions are open
 and their pages where they were; it can be written as long as no fork has taken its new tokens. :meth:`PagedKVCache.again`
 gives a new one.
@@ -81,10 +84,15 @@ class PagedKVCache:
 
     ``storage`` is ``[layers, 2, pages, page_size, kv_heads, head_dim]`` (K, V). A page is ``page_size`` consecutive token
     rows of one layer and target, the layout that the restore kernels write, so a restored chunk can go straight into
-    a session's pages (:meth:`rows`)."""
+    a session's pages (:meth:`rows`).
+
+    ``packed``: rows of ``dtype`` are held in 8 bits (:class:`~reelcache_b200.ops.paged.PackedPages`); ``storage`` has the codes, ``scales
+    [layers, 2, kv_heads, pages, page_size]`` their scales. ``block`` (a divisor of the page size, a multiple of 8): ``means
+    [layers, pages, page_size / block, kv_heads, head_dim]`` has the mean key of every ``block`` positions, kept up to date by
+    :meth:`append` and :meth:`store`, for attention over chosen blocks."""
 
     def __init__(self, layers: int, kv_heads: int, head_dim: int, *, pages: int, page_size: int, max_sessions: int,
-                 max_tokens: int, device="cuda", dtype=torch.bfloat16):
+                 max_tokens: int, device="cuda", dtype=torch.bfloat16, packed: bool = False, block: int | None = None):
         device = torch.device(device)
         if device.type != "cuda":
             raise UnsupportedError("PagedKVCache needs a CUDA device")
@@ -98,8 +106,23 @@ class PagedKVCache:
             raise ConfigurationError(f"PagedKVCache: page_size must be a multiple of 8 tokens, at most 65536, got {page_size!r}")
         if max(pages, max_sessions) >= 1 << 20:  # what the page table's prefix sums hold
             raise ConfigurationError(f"PagedKVCache: pages and max_sessions must be below 2^20, got {pages} and {max_sessions}")
+        if block is not None and (type(block) is not int or block < 8 or block % 8 or page_size % block):
+            raise ConfigurationError(f"PagedKVCache: block must be a multiple of 8 tokens that divides the page size, got {block!r}")
         self.page_size, self.pages, self.max_tokens = page_size, pages, max_tokens
-        self.storage = torch.zeros(layers, 2, pages, page_size, kv_heads, head_dim, dtype=dtype, device=device)
+        self.dtype, self.packed, self.block = dtype, bool(packed), block
+        shape = (layers, 2, pages, page_size, kv_heads, head_dim)
+        self.scales = self.means = None
+        self._sides = []
+        if packed:
+            self.storage = torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+            scales = torch.full((layers, 2, kv_heads, pages, page_size), 127, dtype=torch.uint8, device=device)
+            self.scales = scales.view(torch.float8_e8m0fnu)
+            self._sides.append(self.scales.flatten(0, 2))
+        else:
+            self.storage = torch.zeros(shape, dtype=dtype, device=device)
+        if block is not None:
+            self.means = torch.zeros(layers, pages, page_size // block, kv_heads, head_dim, dtype=dtype, device=device)
+            self._sides.append(self.means)
         self.table = paged.PageTable.empty(pages, max_sessions, -(-max_tokens // page_size), page_size, device)
         self.device = self.storage.device
         self._planes = self.storage.flatten(0, 1)
@@ -115,7 +138,7 @@ class PagedKVCache:
 
     @property
     def nbytes(self) -> int:
-        return self.storage.numel() * self.storage.element_size()
+        return sum(t.numel() * t.element_size() for t in (self.storage, *self._sides))
 
     def _ints(self, values) -> torch.Tensor:
         return torch.tensor(list(values), dtype=torch.int32).pin_memory().to(self.device, non_blocking=True)
@@ -159,7 +182,7 @@ class PagedKVCache:
         self._admit(sum(n % self.page_size > 0 for n in lengths))
         slots = self._next_slots(len(lengths))
         # (the host's books follow the device: what raises until here has changed neither)
-        self.table.fork(self._ints([session.slot] * len(slots)), self._ints(slots), self._ints(lengths), self._planes)
+        self.table.fork(self._ints([session.slot] * len(slots)), self._ints(slots), self._ints(lengths), self._planes, self._sides)
         del self._free_slots[len(self._free_slots) - len(slots):]
         self._changes += 1
         children = []
@@ -263,34 +286,100 @@ class PagedKVCache:
     def compact(self) -> int:
         """Move the pages in use to the front of the pool (the rest of the storage is then free in one piece). Returns how
         many there are. Batches made before are refused from here on."""
-        self.table.compact(self._planes)
+        self.table.compact(self._planes, self._sides)
         self._changes += 1
         self._compacted = self._changes
         return self._held
 
     # -- layers ----------------------------------------------------------------------------------------------------------
 
+    def layer_pages(self, layer: int):
+        """K and V pages of one layer, as the operators of :mod:`reelcache_b200.ops.paged` take them."""
+        k, v = self.storage[layer, 0], self.storage[layer, 1]
+        if not self.packed:
+            return k, v
+        return paged.PackedPages(k, self.scales[layer, 0]), paged.PackedPages(v, self.scales[layer, 1])
+
     def append(self, layer: int, batch: PagedBatch, q, k, v, positions, rope: AxisRope, *, out=None):
         """Write the new tokens of one layer (``k`` rotated at ``positions``, ``v`` as it is); returns ``q`` rotated."""
         self._check_batch(batch, q, write=True)
-        return paged.append(q, k, v, positions, rope, self.storage[layer, 0], self.storage[layer, 1], batch.table,
-                            batch.kv_lens, batch.cu_q, out=out)
+        self._check_type(q)
+        out = paged.append(q, k, v, positions, rope, *self.layer_pages(layer), batch.table, batch.kv_lens, batch.cu_q, out=out)
+        self._update_means(layer, batch)
+        return out
+
+    def store(self, layer: int, batch: PagedBatch, k, v):
+        """Write the new tokens' rows of one layer as they are into a packed cache."""
+        if not self.packed:
+            raise UnsupportedError("store writes a packed cache (rows of a 16-bit one are written in place: token_rows)")
+        self._check_batch(batch, k, write=True)
+        self._check_type(k)
+        paged.store(k, v, *self.layer_pages(layer), batch.table, batch.kv_lens, batch.cu_q)
+        self._update_means(layer, batch)
+
+    def rows_written(self, layer: int, batch: PagedBatch):
+        """Tell the cache that a kernel has written the new tokens' keys of one layer itself (:meth:`new_rows`)."""
+        self._check_batch(batch, None, write=True)
+        self._update_means(layer, batch)
+
+    def _check_type(self, rows):
+        if self.packed and rows.dtype != self.dtype:
+            raise ConfigurationError(f"the cache holds rows of {self.dtype}, got {rows.dtype}")
+
+    def _update_means(self, layer: int, batch: PagedBatch):
+        if self.block is not None and batch.tokens:
+            paged.block_means(self.layer_pages(layer)[0], self.means[layer], batch.table, batch.kv_lens, batch.cu_q,
+                              max_q_len=max(batch.counts))
 
     def attend(self, layer: int, batch: PagedBatch, q, *, causal: bool = False, window: int | None = None, sinks: int = 0,
-               scale: float | None = None, return_lse: bool = False, out=None):
-        """Attention of the new tokens over their sessions (:func:`reelcache_b200.ops.paged.attention`)."""
+               scale: float | None = None, return_lse: bool = False, out=None, keep: int | None = None, query_block: int = 1,
+               recent: int = 0):
+        """Attention of the new tokens over their sessions (:func:`reelcache_b200.ops.paged.attention`), or with ``keep`` over
+        the ``keep`` blocks of their past that score highest for every ``query_block`` of them, besides the first ``sinks`` and the
+        last ``recent`` positions and the new tokens (:func:`reelcache_b200.ops.paged.select_blocks`)."""
         self._check_batch(batch, q, write=False)
-        return paged.attention(q, self.storage[layer, 0], self.storage[layer, 1], batch.table, batch.kv_lens, batch.cu_q,
-                               max_q_len=max(max(batch.counts), 1), causal=causal, window=window, sinks=sinks, scale=scale,
-                               return_lse=return_lse, out=out)
+        self._check_type(q)
+        k, v = self.layer_pages(layer)
+        longest = max(max(batch.counts), 1)
+        if keep is None:
+            if query_block != 1 or recent:
+                raise ConfigurationError("query_block and recent belong to a choice of blocks (keep)")
+            return paged.attention(q, k, v, batch.table, batch.kv_lens, batch.cu_q, max_q_len=longest, causal=causal, window=window,
+                                   sinks=sinks, scale=scale, return_lse=return_lse, out=out)
+        if self.block is None:
+            raise UnsupportedError("the cache has no means of blocks: make it with block=")
+        if window is not None:
+            raise ConfigurationError("attention over chosen blocks takes recent positions, no window")
+        chosen = paged.select_blocks(q, self.means[layer], batch.table, batch.kv_lens, batch.cu_q, block=self.block, keep=keep,
+                                     max_q_len=longest, query_block=query_block, causal=causal, sinks=sinks, recent=recent)
+        return paged.attention(q, paged.blocks(k, self.block), paged.blocks(v, self.block), chosen.table, chosen.kv_lens, chosen.cu_q,
+                               max_q_len=chosen.max_q_len, causal=causal, scale=scale, return_lse=return_lse, out=out)
+
+    def read(self, layer: int, sessions: Sequence[PagedSession]):
+        """K and V of whole sessions of a packed cache, one after the other: ``[sum of lengths, kv_heads, head_dim]`` each."""
+        if not self.packed:
+            raise UnsupportedError("read takes a packed cache")
+        sessions = list(sessions)
+        self._check(sessions)
+        if not sessions:
+            raise StateError("read takes at least one session")
+        lengths = [s.length for s in sessions]
+        batch, slots = self._batch(sessions, lengths, lengths)
+        self._name_pages(batch, slots)
+        return paged.read(*self.layer_pages(layer), batch.table, batch.cu_q, sum(lengths), dtype=self.dtype)
 
     def token_rows(self, layer: int, which: str) -> torch.Tensor:
         """All token rows ``[pages * page_size, kv_heads * head_dim]`` of one layer's K or V (``which``), page by page."""
+        self._in_16_bits()
         return self.storage[layer, 0 if which == "K" else 1].flatten(0, 1).flatten(1)
+
+    def _in_16_bits(self):
+        if self.packed:
+            raise UnsupportedError("a packed cache has no rows in 16 bits: read and store them")
 
     def new_rows(self, batch: PagedBatch) -> torch.Tensor:
         """Where the batch's new tokens lie in :meth:`token_rows` (int64, one after the other), for a kernel that writes them
-        itself instead of :meth:`append`."""
+        itself instead of :meth:`append` (and then :meth:`rows_written`, where the cache keeps means)."""
         self._check_batch(batch, None, write=True)
         token = torch.arange(batch.tokens, dtype=torch.int32, device=self.device)
         seq = torch.bucketize(token, batch.cu_q[1:], right=True)
@@ -299,4 +388,5 @@ class PagedKVCache:
 
     def rows(self, layer: int, which: str, page: int) -> torch.Tensor:
         """Token rows ``[page_size, kv_heads * head_dim]`` of one page (``which``: ``"K"`` or ``"V"``)."""
+        self._in_16_bits()
         return self.storage[layer, 0 if which == "K" else 1, page].flatten(1)
