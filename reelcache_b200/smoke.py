@@ -1,7 +1,7 @@
 """One tiny end-to-end pass of the flagship path on a CUDA device (used by the driver's smoke check):
 restore a compressed chunk history into a KV cache with the fused sm_100a kernel, run one tcgen05 GEMM, and take a step of
-two forked sessions of a paged cache (rotation with gradient, append, attention, page table), checking all against fp64 / fp32
-references."""
+two forked sessions of a paged cache (rotation with gradient, append, attention, page table) and of one in 8 bits (attention over
+all of it and over chosen blocks), checking all against fp64 / fp32 references."""
 
 from __future__ import annotations
 
@@ -48,6 +48,24 @@ def _paged_step(device):
     return worst
 
 
+def _packed_step(device):
+    """A prompt and a token in a cache in 8 bits: the error of attention over all of it against FP32, and over all of its blocks."""
+    cache = PagedKVCache(1, 2, 64, pages=16, page_size=16, max_sessions=2, max_tokens=96, device=device, packed=True, block=8)
+    session = cache.open()
+    for n in (70, 1):
+        batch = cache.extend([(session, n)])
+        q, k, v = (torch.randn(n, h, 64, device=device).bfloat16() for h in (4, 2, 2))
+        cache.store(0, batch, k, v)
+    k, v = (x.float().repeat_interleave(2, dim=1) for x in cache.read(0, [session]))
+    p = torch.softmax(torch.einsum("hd,khd->hk", q[0].float(), k) / 8.0, dim=1)
+    want = torch.einsum("hk,khd->hd", p, v)
+    outs = [cache.attend(0, batch, q, causal=True, **how)[0].float() for how in ({}, dict(keep=20))]
+    worst = max(float((out - want).abs().max()) for out in outs)
+    few = cache.attend(0, batch, q, causal=True, keep=2)
+    assert bool(few.isfinite().all()) and worst < 5e-2, "packed attention mismatch"
+    return worst
+
+
 def run(device):
     torch.manual_seed(0)
     rng = np.random.default_rng(0)
@@ -77,7 +95,7 @@ def run(device):
     _ext.check_status(device)
     ref = a.float() @ b.float().t()
     assert torch.allclose(out, ref, atol=1e-2, rtol=1e-3), "tcgen05 GEMM mismatch"
-    paged_err = _paged_step(device)
+    paged_err, packed_err = _paged_step(device), _packed_step(device)
     _ext.check_status(device)
     return {"restore_max_err": float((got - expect).abs().max()), "gemm_max_err": float((out - ref).abs().max()),
-            "paged_max_err": paged_err}
+            "paged_max_err": paged_err, "packed_max_err": packed_err}
