@@ -73,7 +73,7 @@ std::pair<at::Tensor, c10::optional<at::Tensor>> paged_attention(
   RC_CHECK(q.size(0) < (1ll << 31), "too many tokens for one launch");
   c10::cuda::CUDAGuard guard(q.device());
   const double scale = scale_given.has_value() ? *scale_given : 1.0 / std::sqrt(static_cast<double>(q.size(2)));
-  const at::Tensor out = out_given.has_value() ? *out_given : at::empty(q.sizes(), q.options());
+  const at::Tensor out = out_given.has_value() ? *out_given : paged::new_tensor(q.sizes(), q, type);
   RC_CHECK(out.sizes() == q.sizes() && out.scalar_type() == type && out.device() == q.device(), "out must match q");
   at::assert_no_internal_overlap(out);
   at::assert_no_partial_overlap(out, q);
@@ -118,7 +118,7 @@ std::pair<at::Tensor, c10::optional<at::Tensor>> paged_attention(
   a.out_sectors = out.stride(0) % 16 == 0 && out.stride(1) % 16 == 0 && reinterpret_cast<uintptr_t>(out.data_ptr()) % 32 == 0;
   c10::optional<at::Tensor> lse;
   if (want_lse) {
-    lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
+    lse = paged::new_tensor({q.size(0), q.size(1)}, q, at::kFloat);
     a.lse = lse->data_ptr<float>();
   }
   a.table = t.table;

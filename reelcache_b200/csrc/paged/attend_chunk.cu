@@ -1184,7 +1184,7 @@ void chunk_launch(const Args& args, const at::Tensor& k_pages, const at::Tensor&
   RC_CHECK(p.ctas < kPlanThreads, "more SMs than the plan's threads");
   const int64_t o_floats = 2ll * p.ctas * kItemRows * D, ml_floats = 2ll * p.ctas * kItemRows * 2;
   const int64_t ints = most_items * 8 + 4 + 2ll * (p.ctas + 1) + args.seqs;
-  at::Tensor workspace = at::empty({o_floats + ml_floats + ints}, like.options().dtype(at::kFloat));
+  at::Tensor workspace = new_tensor({o_floats + ml_floats + ints}, like, at::kFloat);
   p.part_o = workspace.data_ptr<float>();
   p.part_ml = p.part_o + o_floats;
   p.plan.items = reinterpret_cast<Item*>(p.part_ml + ml_floats);

@@ -405,7 +405,7 @@ void short_launch(Args a, const at::Tensor& k_pages, const at::Tensor& v_pages, 
   const int ctas = static_cast<int>(std::min<int64_t>(slots, items * (short_tiles(a) + 1)));
   RC_CHECK(items * (kRows / 4) < (1ll << 31), "too many sequences and rows for one launch");
   const int64_t floats = 2ll * ctas * kRows * (D + 2), ints = 1 + 2ll * a.seqs;
-  at::Tensor workspace = at::empty({floats + ints}, like.options().dtype(at::kFloat));
+  at::Tensor workspace = new_tensor({floats + ints}, like, at::kFloat);
   p.part_o = workspace.data_ptr<float>();
   p.part_ml = p.part_o + 2ll * ctas * kRows * D;
   int* line = reinterpret_cast<int*>(p.part_o + floats);

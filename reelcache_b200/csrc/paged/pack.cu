@@ -317,7 +317,7 @@ at::Tensor packed_append(const at::Tensor& q, const at::Tensor& k, const at::Ten
   pack::set_rows(p, k, v, k_codes, k_scales, v_codes, v_scales, table, kv_lens, cu_q, status);
   RC_CHECK(q.dim() == 3 && q.size(0) == k.size(0) && q.size(2) == k.size(2) && q.scalar_type() == k.scalar_type() && q.device() == k.device(),
            "q is [tokens, heads, head_dim], k and v [tokens, kv_heads, head_dim], of one type and device");
-  at::Tensor q_out = out.has_value() ? *out : at::empty(q.sizes(), q.options());
+  at::Tensor q_out = out.has_value() ? *out : paged::new_tensor(q.sizes(), q, q.scalar_type());
   RC_CHECK(q_out.sizes() == q.sizes() && q_out.scalar_type() == q.scalar_type() && q_out.device() == q.device(), "out must match q");
   RC_CHECK((q.numel() == 0 || rotary::vector_rows(q)) && (q.numel() == 0 || rotary::vector_rows(q_out)),
            "rows must have unit inner stride and 16-byte aligned strides and base");
@@ -373,7 +373,7 @@ std::pair<at::Tensor, at::Tensor> packed_read(const at::Tensor& k_codes, const a
            "starts must be a contiguous int32 [seqs + 1] tensor on the device of the pages");
   RC_CHECK(rows >= 0 && rows < (1ll << 31), "too many rows");
   at::Tensor out[2];
-  for (int i = 0; i < 2; ++i) out[i] = at::empty({rows, heads, d}, k_codes.options().dtype(type));
+  for (int i = 0; i < 2; ++i) out[i] = paged::new_tensor({rows, heads, d}, k_codes, type);
   if (rows == 0 || heads == 0 || table.size(0) == 0) return {out[0], out[1]};
   p.codes[0] = static_cast<const uint8_t*>(k_codes.data_ptr());
   p.codes[1] = static_cast<const uint8_t*>(v_codes.data_ptr());

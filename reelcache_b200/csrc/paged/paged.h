@@ -2,6 +2,7 @@
 #pragma once
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 
 #include "../common/host.h"
 
@@ -92,6 +93,11 @@ struct Divider {
   __device__ __forceinline__ int up(int n) const { return over(n) + (n > over(n) * by); }  // rounded up
 #endif
 };
+
+// A new tensor on `like`'s device, without the dispatcher (half a microsecond of a call's five).
+inline at::Tensor new_tensor(at::IntArrayRef sizes, const at::Tensor& like, at::ScalarType type) {
+  return at::detail::empty_cuda(sizes, like.options().dtype(type));
+}
 
 struct Pages {  // [pages, page_size, kv_heads, head_dim], strides in elements
   int count, size;

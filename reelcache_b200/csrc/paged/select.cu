@@ -898,8 +898,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> paged_select_blocks(const at::Ten
   items = std::min(items, seqs * ((longest + query_block - 1) / query_block));
   const int64_t span = (causal ? std::min(query_block, longest) : longest) + recent;
   const int64_t width = std::min(held, (sinks + block - 1) / block + keep + (span + block - 2) / block + 1);
-  const at::TensorOptions ints = q.options().dtype(at::kInt);
-  at::Tensor out = at::empty({items, kv_heads, width}, ints), lens = at::empty({items}, ints), cu = at::empty({items + 1}, ints);
+  at::Tensor out = paged::new_tensor({items, kv_heads, width}, q, at::kInt), lens = paged::new_tensor({items}, q, at::kInt),
+             cu = paged::new_tensor({items + 1}, q, at::kInt);
   if (items == 0) {
     cu.zero_();
     return {out, lens, cu};

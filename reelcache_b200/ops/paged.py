@@ -138,20 +138,21 @@ def attention_form(tokens, heads, kv_heads, head_dim, seqs, width, page_size, *,
 
 def blocks(pages, block: int):
     """Pages ``[pages, page_size, kv_heads, D]`` (or packed ones) cut into pages of ``block`` tokens, a view: page ``p`` becomes pages
-    ``p * page_size / block`` and on. ``block`` divides the page size and is a multiple of 8; the pages must lie one after the
-    other."""
+    ``p * page_size / block`` and on. ``block`` divides the page size and is a multiple of 8; where it is less, the pages must lie one
+    after the other."""
     tensor, scales = _parts(pages)
-    count, size = tensor.shape[:2]
+    (count, size, heads, dim), (page, token, *rest) = tensor.shape, tensor.stride()
     if block < 8 or block % 8 or size % block:
         raise ConfigurationError(f"blocks of {block} tokens must be multiples of 8 and divide the page size, {size}")
-    if count > 1 and tensor.stride(0) != size * tensor.stride(1):
+    if block == size:
+        return pages
+    if count > 1 and page != size * token or scales is not None and count > 1 and scales.stride(1) != size:
         raise ConfigurationError("pages that are cut into blocks must lie one after the other")
-    tensor = tensor.as_strided((count * (size // block), block, *tensor.shape[2:]), (block * tensor.stride(1), *tensor.stride()[1:]))
+    number = count * (size // block)
+    tensor = tensor.as_strided((number, block, heads, dim), (block * token, token, *rest))
     if scales is None:
         return tensor
-    if count > 1 and scales.stride(1) != size:
-        raise ConfigurationError("pages that are cut into blocks must lie one after the other")
-    return PackedPages(tensor, scales.as_strided((scales.shape[0], count * (size // block), block), (scales.stride(0), block, 1)))
+    return PackedPages(tensor, scales.as_strided((heads, number, block), (scales.stride(0), block, 1)))
 
 
 def block_means(k_pages, means, block_table, kv_lens, cu_q, *, max_q_len: int):
