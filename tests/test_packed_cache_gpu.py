@@ -230,3 +230,16 @@ def test_example_runs(options, capsys):
     example.main(["--small", "--chunks", "2", "--branches", "2", *options])
     got = json.loads(capsys.readouterr().out)
     assert got["packed"] == ("--packed" in options) and got["page_bytes"] > 0
+
+
+def test_batches_without_new_tokens():
+    cache = _cache(packed=True, block=8)
+    a = cache.open()
+    rows = torch.randn(30, 2, 64, device="cuda").to(BF16)
+    cache.store(0, cache.extend([(a, 30)]), rows, rows)
+    batch = cache.extend([(a, 0)])
+    none = torch.zeros(0, 4, 64, dtype=BF16, device="cuda")
+    cache.store(0, batch, none[:, :2], none[:, :2])
+    assert cache.attend(0, batch, none).shape == none.shape
+    assert cache.attend(0, batch, none, keep=2).shape == none.shape
+    assert torch.equal(cache.read(0, [a])[0], _values(rows))

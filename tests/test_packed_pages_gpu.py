@@ -387,3 +387,30 @@ def test_stores_of_nothing_and_without_sequences():
     version = pages[0].codes._version
     paged.store(rows[:1], rows[:1], *pages, table, torch.ones_like(zeros[:1]), torch.tensor([0, 1], dtype=torch.int32, device="cuda"))
     assert pages[0].codes._version > version and float(held(pages[1])[0, 0].min()) == 1.0
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_attention_over_pages_outside_the_pool(new, cuda_device):
+    """Such pages read as zeros and are reported."""
+    from reelcache_b200.errors import DeviceStatusError
+    from reelcache_b200.ops import _ext, paged
+    g = _gen(4)
+    k, v, table, kv_lens, cu_q = paged_batch(g, [new], [200], 2, 128, 16, torch.float32)
+    packed = [pack_pages(x, BF16) for x in (k, v)]
+    values = [held(p, BF16) for p in packed]
+    q = torch.randn(new, 4, 128, generator=g, device="cuda").to(BF16)
+    bad = table.clone()
+    bad[0, 2], bad[0, 5] = -1, 10 ** 6
+    out = paged.attention(q, *packed, bad, kv_lens, cu_q, max_q_len=new, causal=True)
+    with pytest.raises(DeviceStatusError, match="0x403"):
+        _ext.check_status(cuda_device)
+    for x in values:
+        x[table[0, [2, 5]].long()] = 0.0
+    want, _, bound, _ = attend(q, *values, table, kv_lens, [new], causal=True)
+    assert within(out, want, bound + 200 * 2.0 ** -24 * float(values[1].abs().max()))
+
+
+def test_many_kv_heads_side_by_side():
+    """The line of few rows with head numbers that have no divisor up to 32, and with more heads than that."""
+    _check([1] * 30, [600 + 30 * i for i in range(30)], 37, 37, 64, 64, BF16, causal=True)
+    _check([1] * 20, [600 + 30 * i for i in range(20)], 80, 40, 64, 64, BF16, causal=True)

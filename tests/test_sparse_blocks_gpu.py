@@ -271,3 +271,51 @@ def test_calls_without_tokens_or_sequences():
     paged.block_means(k, means, table[:0], kv_lens[:0], cu_q[:1], max_q_len=1)
     paged.block_means(k, means, table, kv_lens, torch.zeros_like(cu_q), max_q_len=1)
     assert torch.equal(means, before)
+
+
+@pytest.mark.parametrize("query_block", [1, 3])
+def test_many_sequences_and_rows_of_none(query_block):
+    """More sequences than a CTA has threads, rows of q before the first and behind the last of them."""
+    from reelcache_b200.ops import paged
+    g = _gen(8)
+    new = [(i * 7) % 4 for i in range(700)]
+    totals = [n + (i * 37) % 300 for i, n in enumerate(new)]
+    k, v, table, kv_lens, cu_q = paged_batch(g, new, totals, 1, 64, 16, BF16)
+    q = torch.randn(sum(new) + 9, 2, 64, generator=g, device="cuda").to(BF16)
+    means = _means(k, 16)
+    chosen, _ = _select(q, means, table, kv_lens, cu_q + 4, new, block=16, keep=2, query_block=query_block, causal=True)
+    out = torch.full_like(q, 7.0)
+    paged.attention(q, k, v, chosen.table, chosen.kv_lens, chosen.cu_q, max_q_len=chosen.max_q_len, causal=True, out=out)
+    assert bool((out[:4] == 7.0).all()) and bool((out[sum(new) + 4:] == 7.0).all()) and not bool((out[4:sum(new) + 4] == 7.0).any())
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("new,totals", [([5], [2]), ([40, 1], [30, 0]), ([3, 2], [0, 700])])
+def test_tokens_before_the_first_position(new, totals, causal):
+    from reelcache_b200.ops import paged
+    g = _gen(9)
+    k, v, table, kv_lens, cu_q = paged_batch(g, new, totals, 2, 64, 8, BF16)
+    q = torch.randn(sum(new), 4, 64, generator=g, device="cuda").to(BF16)
+    means = _means(k, 8)
+    paged.block_means(k, means, table, kv_lens, cu_q, max_q_len=max(new))
+    chosen, _ = _select(q, means, table, kv_lens, cu_q, new, block=8, keep=200, query_block=4, causal=causal)
+    out, lse = paged.attention(q, k, v, chosen.table, chosen.kv_lens, chosen.cu_q, max_q_len=chosen.max_q_len, causal=causal, return_lse=True)
+    want, want_lse, bound, lse_bound = attend(q, k, v, table, kv_lens, new, causal=causal)
+    assert within(out, want, bound) and within(lse, want_lse, lse_bound)
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_more_rounds_than_sms(packed):
+    """Items of up to 128 rows in more than one round, the last ones in clusters."""
+    from reelcache_b200.ops import paged
+    g = _gen(10)
+    k, v, table, kv_lens, cu_q = paged_batch(g, [2700], [9000], 4, 64, 64, BF16)
+    pages = [pack_pages(x, BF16) for x in (k, v)] if packed else [k, v]
+    if packed:
+        k, v = (held(p, BF16) for p in pages)
+    q = torch.randn(2700, 4, 64, generator=g, device="cuda").to(BF16)
+    chosen = paged.select_blocks(q, _means(k, 64), table, kv_lens, cu_q, block=64, keep=10000, query_block=60, max_q_len=2700, causal=True)
+    assert chosen.table.shape[0] * 4 % 148 != 0 and chosen.table.shape[0] * 4 > 148
+    out, lse = paged.attention(q, *pages, chosen.table, chosen.kv_lens, chosen.cu_q, max_q_len=60, causal=True, return_lse=True)
+    want, want_lse, bound, lse_bound = attend(q, k, v, table, kv_lens, [2700], causal=True)
+    assert within(out, want, bound) and within(lse, want_lse, lse_bound)
