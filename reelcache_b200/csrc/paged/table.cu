@@ -329,6 +329,8 @@ __global__ void __launch_bounds__(kMoveThreads) copy_kernel(Storage st, int page
   move_pages(st, moves, pages, source, target, rows, status);
 }
 
+// kSides: whether anything lies beside the pages (the copies of the pages alone keep their registers).
+template <bool kSides>
 __global__ void __launch_bounds__(kMoveThreads) fork_kernel(State s, Storage st, Sides sides, const int* parents, const int* children,
                                                             const int* at, int n, Plan plan, int* status) {
   paged::let_later();
@@ -351,9 +353,10 @@ __global__ void __launch_bounds__(kMoveThreads) fork_kernel(State s, Storage st,
     if (block == 0) s.lens[child] = len;
   }
   move_pages(st, n, s.pages, plan.source, plan.target, plan.rows, status);
-  move_sides(sides, n, s.pages, plan.source, plan.target, plan.rows);
+  if (kSides) move_sides(sides, n, s.pages, plan.source, plan.target, plan.rows);
 }
 
+template <bool kSides>
 __global__ void __launch_bounds__(kMoveThreads) compact_kernel(State s, Storage st, Sides sides, const int* place, const int* in_use, Plan plan,
                                                                int* status) {
   paged::let_later();
@@ -371,7 +374,7 @@ __global__ void __launch_bounds__(kMoveThreads) compact_kernel(State s, Storage 
     s.refcount[plan.source[m]] = 0;
   }
   move_pages(st, moves, s.pages, plan.source, plan.target, nullptr, status);
-  move_sides(sides, moves, s.pages, plan.source, plan.target, nullptr);
+  if (kSides) move_sides(sides, moves, s.pages, plan.source, plan.target, nullptr);
 }
 
 __global__ void __launch_bounds__(kMoveThreads) release_kernel(State s, const int* seqs, int n, int* status) {
@@ -506,7 +509,7 @@ void pages_fork(at::Tensor& state, int64_t pages, int64_t seqs_held, int64_t pag
   int* list = p + 1 + 3 * n;
   paged::launch(pagetable::fork_plan_kernel, dim3(1), pagetable::kPlanThreads, 0, 0, stream, s, from, to, len, static_cast<int>(n), list,
                                                                         list + s.pages, plan, status_ptr(status));
-  paged::launch(pagetable::fork_kernel, dim3(pagetable::move_grid(state.get_device())), pagetable::kMoveThreads, 0, 0, stream,
+  paged::launch(beside.count > 0 ? pagetable::fork_kernel<true> : pagetable::fork_kernel<false>, dim3(pagetable::move_grid(state.get_device())), pagetable::kMoveThreads, 0, 0, stream,
       s, st, beside, from, to, len, static_cast<int>(n), plan, status_ptr(status));
   written(state);
   written(storage);
@@ -541,7 +544,7 @@ at::Tensor pages_compact(at::Tensor& state, int64_t pages, int64_t seqs_held, in
   const pagetable::Plan plan{p, p + 1, p + 1 + s.pages, nullptr};
   int* place = p + 1 + 2 * static_cast<int64_t>(s.pages);
   paged::launch(pagetable::compact_plan_kernel, dim3(1), pagetable::kPlanThreads, 0, 0, stream, s, place, plan, in_use.data_ptr<int>());
-  paged::launch(pagetable::compact_kernel, dim3(pagetable::move_grid(state.get_device())), pagetable::kMoveThreads, 0, 0, stream,
+  paged::launch(beside.count > 0 ? pagetable::compact_kernel<true> : pagetable::compact_kernel<false>, dim3(pagetable::move_grid(state.get_device())), pagetable::kMoveThreads, 0, 0, stream,
       s, st, beside, place, in_use.data_ptr<int>(), plan, status_ptr(status));
   written(state);
   written(storage);
