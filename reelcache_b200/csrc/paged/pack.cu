@@ -7,8 +7,11 @@
 // Layout of threads as in the rotation: a thread owns a vector of eight channels (two, half a head apart) of a token for as
 // many heads as leave every SM full, so that its sines are computed once.
 //
-// What bounds it: memory at first sight (3 bytes a number of k and v, 4 of q), in fact the chain of a row: load, turn, maximum over the
-// row's lanes, codes (4.4 TB/s for three chunks of 4,680 tokens and 12 heads).
+// What bounds it: memory (3 bytes a number of k and v, 4 of q), and the chain of a row: load, turn, maximum over the row's lanes,
+// codes. Three chunks of 4,680 tokens and 12 heads 41 us, 5.2 TB/s; 25.8 us without q and the rotation (129 MB).
+//
+// Out of pages: a block looks up where its rows lie, then every thread turns vectors of sixteen codes into 32 bytes, a whole
+// sector in one store (16-byte stores: 42 us where these take 36.4, five chunks of 12 heads, 216 MB).
 #include <ATen/ATen.h>
 #include <ATen/MemoryOverlap.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -38,12 +41,6 @@ struct Args {
   Exponents range;
 };
 
-// Largest magnitude's bits over the `width` lanes of a row (a power of two; all lanes of the warp take part).
-__device__ __forceinline__ uint32_t row_top(uint32_t top, int width) {
-  for (int o = width >> 1; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  return top;
-}
-
 // max(top, |a|, |b|), NaN if one of them is.
 __device__ __forceinline__ float top_of(float top, float a, float b) {
   float r;
@@ -58,10 +55,10 @@ __device__ __forceinline__ uint2 codes_of_vec(const float (&x)[8], float inverse
 }
 
 // kTurn: 0 rows as they are, 1 pairs are neighbours, 2 half a head apart.
-// (Five blocks on an SM: 48.8 us for three chunks of 4,680 tokens, 52.0 with four. Scales gathered over a block's tokens and
-// written together at its end: no faster than a byte each as they come.)
+// (Blocks on an SM and heads of a round, three chunks of 4,680 tokens and 36 heads: neighbours 41.2 us with five and two, 43.7 with
+// four, 46.4 with three and four heads, 48.8 one head after the other; half a head apart 40.6 with three, 47.0 with two.)
 template <typename T, int kTurn, int kHeads>
-__global__ void __launch_bounds__(kThreads, kTurn == 2 ? 2 : 5) pack_kernel(const __grid_constant__ Args p) {
+__global__ void __launch_bounds__(kThreads, kTurn == 2 ? 3 : 5) pack_kernel(const __grid_constant__ Args p) {
   paged::let_later();
   paged::after_earlier();
   constexpr bool kHalves = kTurn == 2;
@@ -113,35 +110,45 @@ __global__ void __launch_bounds__(kThreads, kTurn == 2 ? 2 : 5) pack_kernel(cons
   const bool turned = kTurn != 0 && (is_q || is_k);
   if (turned && active) rotary::sines<true>(a, token, vec, cs, sn);  // (a code that falls to its neighbour is 2^-3 off)
 
+  // a round of heads at a time, step by step, so that their chains run next to each other
   for (int done = 0; done < heads; done += kHeads) {
+    float x[kHeads][8], y2[kHeads][8];
+    uint32_t top[kHeads];
 #pragma unroll
     for (int i = 0; i < kHeads; ++i) {
-      if (done + i >= heads) continue;
-      float x[8], y2[8];
-      Vec<T>::unpack(raw[i][0], x);
-      if (kHalves) Vec<T>::unpack(raw[i][kParts - 1], y2);
-      if (turned) rotary::turn<kHalves>(x, y2, cs, sn);
-      load(i, done + kHeads + i);  // before the stores, which the compiler must take for ones to the same memory
-      char* to = dst;
-      dst += r.dst_head;
-      if (is_q) {
-        if (active) *reinterpret_cast<uint4*>(to) = Vec<T>::pack(x);
-        if (active && kHalves) *reinterpret_cast<uint4*>(to + part_bytes) = Vec<T>::pack(y2);
-        continue;
-      }
+      Vec<T>::unpack(raw[i][0], x[i]);
+      if (kHalves) Vec<T>::unpack(raw[i][kParts - 1], y2[i]);
+      if (turned) rotary::turn<kHalves>(x[i], y2[i], cs, sn);
       float most = 0.0f;
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
-        most = top_of(most, x[e], x[e + 1]);
-        if (kHalves) most = top_of(most, y2[e], y2[e + 1]);
+        most = top_of(most, x[i][e], x[i][e + 1]);
+        if (kHalves) most = top_of(most, y2[i][e], y2[i][e + 1]);
       }
-      const uint32_t top = row_top(__float_as_uint(most), per_row);
-      const bool finite = top < 0x7f800000u;
-      const int power = min(max(static_cast<int>(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u), p.range.low), p.range.high);
+      top[i] = __float_as_uint(most);
+      load(i, done + kHeads + i);  // before the stores, which the compiler must take for ones to the same memory
+    }
+    if (!is_q) {
+      for (int o = per_row >> 1; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i) top[i] = max(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+    }
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+      const bool here = active && done + i < heads;
+      char* to = dst;
+      dst += r.dst_head;
+      if (is_q) {
+        if (here) *reinterpret_cast<uint4*>(to) = Vec<T>::pack(x[i]);
+        if (here && kHalves) *reinterpret_cast<uint4*>(to + part_bytes) = Vec<T>::pack(y2[i]);
+        continue;
+      }
+      const bool finite = top[i] < 0x7f800000u;
+      const int power = min(max(static_cast<int>(top[i] >> 23) - 127 - 8 + ((top[i] & 0x7fffffu) > 0x600000u), p.range.low), p.range.high);
       const float inverse = __uint_as_float(static_cast<uint32_t>(127 - power) << 23);
-      if (active) *reinterpret_cast<uint2*>(to) = codes_of_vec(x, inverse, finite);
-      if (active && kHalves) *reinterpret_cast<uint2*>(to + a.pairs) = codes_of_vec(y2, inverse, finite);
-      if (active && vec == 0) *scale = static_cast<uint8_t>(finite ? power + 127 : paged::kNanScale);
+      if (here) *reinterpret_cast<uint2*>(to) = codes_of_vec(x[i], inverse, finite);
+      if (here && kHalves) *reinterpret_cast<uint2*>(to + a.pairs) = codes_of_vec(y2[i], inverse, finite);
+      if (here && vec == 0) *scale = static_cast<uint8_t>(finite ? power + 127 : paged::kNanScale);
       scale += scale_head;
     }
   }
@@ -158,7 +165,7 @@ void pack_launch(Args p, cudaStream_t stream, int sms) {
   const dim3 grid(static_cast<unsigned>(blocks), groups);
   if (widest == 1) paged::launch(pack_kernel<T, kTurn, 1>, grid, kThreads, 0, 0, stream, p);
   else if (widest == 2) paged::launch(pack_kernel<T, kTurn, 2>, grid, kThreads, 0, 0, stream, p);
-  else paged::launch(pack_kernel<T, kTurn, 4>, grid, kThreads, 0, 0, stream, p);
+  else paged::launch(pack_kernel<T, kTurn, 2>, grid, kThreads, 0, 0, stream, p);
 }
 
 template <int kTurn>

@@ -898,8 +898,16 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> paged_select_blocks(const at::Ten
   items = std::min(items, seqs * ((longest + query_block - 1) / query_block));
   const int64_t span = (causal ? std::min(query_block, longest) : longest) + recent;
   const int64_t width = std::min(held, (sinks + block - 1) / block + keep + (span + block - 2) / block + 1);
-  at::Tensor out = paged::new_tensor({items, kv_heads, width}, q, at::kInt), lens = paged::new_tensor({items}, q, at::kInt),
-             cu = paged::new_tensor({items + 1}, q, at::kInt);
+  // one allocation for the three of them
+  at::Tensor room = paged::new_tensor({items * (kv_heads * width + 2) + 1}, q, at::kInt);
+  const auto part = [&](int64_t offset, at::IntArrayRef sizes) {
+    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(room.storage()), room.key_set(), room.dtype());
+    t.unsafeGetTensorImpl()->set_storage_offset(offset);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+    return t;
+  };
+  at::Tensor out = part(0, {items, kv_heads, width}), lens = part(items * kv_heads * width, {items}),
+             cu = part(items * (kv_heads * width + 1), {items + 1});
   if (items == 0) {
     cu.zero_();
     return {out, lens, cu};

@@ -38,6 +38,8 @@ STATUS_NAMES = {
 
 def ext():
     """The loaded extension module; raises UnsupportedError naming the missing library."""
+    if _native_build._module is not None:
+        return _native_build._module
     try:
         return _native_build.load()
     except ImportError as error:
@@ -53,7 +55,8 @@ def available() -> bool:
 
 
 def status_word(device) -> torch.Tensor:
-    device = torch.device(device)
+    if not isinstance(device, torch.device):
+        device = torch.device(device)
     word = _status.get(device.index)
     if word is not None:
         return word

@@ -50,13 +50,13 @@ class PackedPages(NamedTuple):
 
 def _parts(pages):
     """Tensor of pages, and its scales where they are packed."""
-    return (pages.codes, pages.scales) if isinstance(pages, PackedPages) else (pages, None)
+    return pages if type(pages) is PackedPages else (pages, None)
 
 
 def _both(k_pages, v_pages) -> bool:
     """Whether the pages are packed (both or neither)."""
-    packed = isinstance(k_pages, PackedPages)
-    if packed != isinstance(v_pages, PackedPages):
+    packed = type(k_pages) is PackedPages
+    if packed is not (type(v_pages) is PackedPages):
         raise ConfigurationError("both or neither of k_pages and v_pages must be packed")
     return packed
 
@@ -67,8 +67,8 @@ def append(q, k, v, positions, rope: AxisRope, k_pages, v_pages, block_table, kv
     and ``v`` are quantised from the rotated rows in FP32, in one rounding."""
     if not q.is_cuda:
         raise UnsupportedError("append needs CUDA tensors")
-    if q.shape[-1] != rope.head_dim:
-        raise ConfigurationError(f"the rotation is for head_dim {rope.head_dim}, q has {q.shape[-1]}")
+    if q.size(-1) != rope.head_dim:
+        raise ConfigurationError(f"the rotation is for head_dim {rope.head_dim}, q has {q.size(-1)}")
     device = q.device
     if _both(k_pages, v_pages):
         return ext().packed_append(q, k, v, positions, rope.plan(device), *k_pages, *v_pages, block_table, kv_lens, cu_q, out,
@@ -121,8 +121,9 @@ def attention(q, k_pages, v_pages, block_table, kv_lens, cu_q, *, max_q_len: int
         raise UnsupportedError("paged attention needs CUDA tensors")
     if window is not None and window < 1:
         raise ConfigurationError(f"window {window} must be positive")
-    _both(k_pages, v_pages)
-    (k_pages, k_scales), (v_pages, v_scales) = _parts(k_pages), _parts(v_pages)
+    k_scales = v_scales = None
+    if _both(k_pages, v_pages):
+        (k_pages, k_scales), (v_pages, v_scales) = k_pages, v_pages
     out, lse = ext().paged_attention(q, k_pages, v_pages, block_table, kv_lens, cu_q, max_q_len, causal, window or 0, sinks,
                                      scale, return_lse, out, status_word(q.device), k_scales, v_scales)
     return (out, lse) if return_lse else out
