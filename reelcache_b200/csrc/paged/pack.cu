@@ -8,7 +8,8 @@
 // many heads as leave every SM full, so that its sines are computed once.
 //
 // What bounds it: memory (3 bytes a number of k and v, 4 of q), and the chain of a row: load, turn, maximum over the row's lanes,
-// codes. Three chunks of 4,680 tokens and 12 heads 41 us, 5.2 TB/s; 25.8 us without q and the rotation (129 MB).
+// codes. Three chunks of 4,680 tokens and 12 heads 46.3 us, 4.7 TB/s (41.2 with sines of FP32 alone); 25.8 us without q and the
+// rotation (129 MB, 5.0 TB/s).
 //
 // Out of pages: a block looks up where its rows lie, then every thread turns vectors of sixteen codes into 32 bytes, a whole
 // sector in one store (16-byte stores: 42 us where these take 36.4, five chunks of 12 heads, 216 MB).
@@ -55,10 +56,10 @@ __device__ __forceinline__ uint2 codes_of_vec(const float (&x)[8], float inverse
 }
 
 // kTurn: 0 rows as they are, 1 pairs are neighbours, 2 half a head apart.
-// (Blocks on an SM and heads of a round, three chunks of 4,680 tokens and 36 heads: neighbours 41.2 us with five and two, 43.7 with
-// four, 46.4 with three and four heads, 48.8 one head after the other; half a head apart 40.6 with three, 47.0 with two.)
+// (Blocks on an SM, two heads a round, three chunks of 4,680 tokens and 36 heads: neighbours 46.3 us with four, 48.5 with five; half
+// a head apart 49.2 with two, 58.8 with three; one head after the other 10 us more.)
 template <typename T, int kTurn, int kHeads>
-__global__ void __launch_bounds__(kThreads, kTurn == 2 ? 3 : 5) pack_kernel(const __grid_constant__ Args p) {
+__global__ void __launch_bounds__(kThreads, kTurn == 2 ? 2 : kTurn == 1 ? 4 : 5) pack_kernel(const __grid_constant__ Args p) {
   paged::let_later();
   paged::after_earlier();
   constexpr bool kHalves = kTurn == 2;
@@ -106,9 +107,26 @@ __global__ void __launch_bounds__(kThreads, kTurn == 2 ? 3 : 5) pack_kernel(cons
     }
   }
 
-  float cs[kPairs] = {}, sn[kPairs] = {};
+  // A code that falls to its neighbour is 2^-3 off, so k is turned nearer than FP32's sines allow: by sines of FP64 as the sums of
+  // two numbers, computed once for all of the thread's heads. What is left are two roundings, 2^-24 each.
+  float cs[kPairs] = {}, sn[kPairs] = {}, cs_low[kPairs] = {}, sn_low[kPairs] = {};
   const bool turned = kTurn != 0 && (is_q || is_k);
-  if (turned && active) rotary::sines<true>(a, token, vec, cs, sn);  // (a code that falls to its neighbour is 2^-3 off)
+  if (turned && active && is_q) rotary::sines<false>(a, token, vec, cs, sn);
+  if (turned && active && is_k) {
+#pragma unroll 1
+    for (int e = 0; e < kPairs; ++e) {
+      double s, c;
+      sincospi(2.0 * rotary::turn_part(a, token, vec * kPairs + e), &s, &c);
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i)
+        if (i == e) {
+          cs[i] = static_cast<float>(c);
+          sn[i] = static_cast<float>(s);
+          cs_low[i] = static_cast<float>(c - static_cast<double>(cs[i]));
+          sn_low[i] = static_cast<float>(s - static_cast<double>(sn[i]));
+        }
+    }
+  }
 
   // a round of heads at a time, step by step, so that their chains run next to each other
   for (int done = 0; done < heads; done += kHeads) {
@@ -118,7 +136,16 @@ __global__ void __launch_bounds__(kThreads, kTurn == 2 ? 3 : 5) pack_kernel(cons
     for (int i = 0; i < kHeads; ++i) {
       Vec<T>::unpack(raw[i][0], x[i]);
       if (kHalves) Vec<T>::unpack(raw[i][kParts - 1], y2[i]);
-      if (turned) rotary::turn<kHalves>(x[i], y2[i], cs, sn);
+      if (turned) {
+#pragma unroll
+        for (int e = 0; e < kPairs; ++e) {
+          float& p = x[i][kHalves ? e : 2 * e];
+          float& q = kHalves ? y2[i][e] : x[i][2 * e + 1];
+          const float u = fmaf(p, cs[e], fmaf(-q, sn[e], fmaf(p, cs_low[e], -q * sn_low[e])));
+          q = fmaf(p, sn[e], fmaf(q, cs[e], fmaf(p, sn_low[e], q * cs_low[e])));
+          p = u;
+        }
+      }
       float most = 0.0f;
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {

@@ -110,15 +110,16 @@ struct Args {
 
 constexpr float kFar = 16777216.0f;  // 2^24: from here on FP32 does not hold every whole number
 
-// The fraction of a turn of pair j at a far position.
-__device__ __forceinline__ float far_part(const Args& a, int token, int j) {
+// The fraction of a turn of pair j at a token's position, in FP64.
+__device__ __forceinline__ double turn_part(const Args& a, int token, int j) {
   const int axis = j < a.ends[0] ? 0 : j < a.ends[1] ? 1 : j < a.ends[2] ? 2 : 3;
   const int64_t at = static_cast<int64_t>(token) * a.axes + axis;
   const double p = a.position_float ? static_cast<double>(static_cast<const float*>(a.positions)[at])
                                     : static_cast<double>(static_cast<const int*>(a.positions)[at]);
   const double t = __ldg(a.exact + j), n = p * t;
-  return static_cast<float>((n - rint(n)) + fma(p, t, -n));
+  return (n - rint(n)) + fma(p, t, -n);
 }
+__device__ __forceinline__ float far_part(const Args& a, int token, int j) { return static_cast<float>(turn_part(a, token, j)); }
 
 // Sines of the kPairs pairs of a token that begin at vec * kPairs (sn times a.sign): within a few ULP (kFine), or from the special
 // function unit (within 2^-21).

@@ -20,7 +20,10 @@
 // cluster's first CTA, which finds the keep-th largest (a histogram between the smallest and the largest, then the bucket
 // that holds it; digit by digit where that bucket holds many) and writes the chosen blocks in order.
 //
-// What bounds it: the latency of a chain of small steps for few sequences, reading the means for many.
+// What bounds it: the latency of a chain of small steps for few sequences (a CTA with 64 candidates takes 10,000 cycles: looking up the
+// sequence 1,100, the queries and means 1,400, products 1,900, the keep-th largest 2,200 are the longest), reading the means
+// for many (an SM's share through L2 at 64 bytes a cycle). Measured (us): one token over 1,024 blocks and 8 KV heads 8.5; 40
+// tokens over up to 512 blocks 15; 77 query blocks of 32 tokens over up to 500 blocks 30. In FP64 throughout: 27, 100 and 159.
 #include <ATen/ATen.h>
 #include <ATen/MemoryOverlap.h>
 #include <c10/cuda/CUDAGuard.h>
