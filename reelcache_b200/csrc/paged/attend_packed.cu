@@ -571,6 +571,7 @@ void packed_launch(const Args& a, const at::Tensor& k_codes, const at::Tensor& v
   packed_configure<T, D, kN>(device);
   const int64_t items = static_cast<int64_t>(a.seqs) * a.kv_heads, slots = sm_count(device) * Shape::ctas;
   p.par = 1;
+  p.rows = 8 * kN;
   p.cluster = short_cluster<PackedForm<T, D, kN>>(items, short_tiles(a), p.a.tiling.step, a.seqs > 1 && a.table_head == 0, device);
   if (p.cluster > 0) {
     launch(packed_short_kernel<T, D, true, kN>, dim3(static_cast<unsigned>(items * p.cluster)), kShortThreads, Shape::bytes, p.cluster,

@@ -396,6 +396,7 @@ void short_launch(Args a, const at::Tensor& k_pages, const at::Tensor& v_pages, 
   const PageMaps maps = page_maps(k_pages, v_pages, p.a.tiling, kShortTile);
   const int64_t items = static_cast<int64_t>(a.seqs) * a.kv_heads, slots = sm_count(device) * kShortCtasPerSm;
   p.par = 1;
+  p.rows = kRows;
   p.cluster = short_form<T, D>(a, device);
   if (p.cluster > 0) {
     launch(short_kernel<T, D, true>, dim3(static_cast<unsigned>(items * p.cluster)), kShortThreads, Shape::bytes, p.cluster,

@@ -29,6 +29,7 @@ struct Short {
   float* part_o;   // [2 * CTAs, 16, D]
   float* part_ml;  // [2 * CTAs, 16, 2]
   int cluster;     // CTAs of a cluster (the clustered form)
+  int rows;        // that the kernel takes: of a sequence with more new tokens than it was told, the others have no result
   int par;         // KV heads that the line's CTAs take side by side (a divisor of their number): CTA par i + j the share i of the j-th
 };
 
@@ -224,7 +225,7 @@ __device__ __forceinline__ void join_few_cluster(const Short& p, const SeqWork& 
   const Args& a = p.a;
   const int rank = static_cast<int>(blockIdx.x) % p.cluster;
   const int vecs = D / 4 / p.cluster;  // float4 of a row that this CTA joins
-  const int rows = min(kRows, rows_here);
+  const int rows = min(p.rows, rows_here);
   for (int v = static_cast<int>(threadIdx.x); v < rows * vecs; v += 128) {
     const int row = v / vecs, col = (rank * vecs + v - row * vecs) * 4;
     float top = -INFINITY, sum = 0.0f;
@@ -283,7 +284,7 @@ __global__ void __launch_bounds__(128) short_join_kernel(const __grid_constant__
   if (row == 0 && head == 0 && lane == 0) report_rows(a, s);
   const SeqWork w(a, s);
   const int query = row / a.group;
-  if (query >= w.q_len) return;
+  if (query >= w.q_len || row >= p.rows) return;
   const int share = *p.line.share;
   const int place = head / p.par, side = head - place * p.par;
   const int begin = p.line.first[s] + place * w.tiles, end = begin + w.tiles;

@@ -414,3 +414,26 @@ def test_many_kv_heads_side_by_side():
     """The line of few rows with head numbers that have no divisor up to 32, and with more heads than that."""
     _check([1] * 30, [600 + 30 * i for i in range(30)], 37, 37, 64, 64, BF16, causal=True)
     _check([1] * 20, [600 + 30 * i for i in range(20)], 80, 40, 64, 64, BF16, causal=True)
+
+
+@pytest.mark.parametrize("seqs", [1, 60])
+@pytest.mark.parametrize("new,bound", [(5, 1), (9, 3)])
+def test_more_new_tokens_than_the_bound_are_reported(new, bound, seqs, cuda_device):
+    """The tokens up to the bound have their results; rows that the kernel does not take are left as they were."""
+    from reelcache_b200.errors import DeviceStatusError
+    from reelcache_b200.ops import _ext, paged
+    g = _gen(new)
+    k, v, table, kv_lens, cu_q = paged_batch(g, [new] * seqs, [700 + i for i in range(seqs)], 2, 64, 16, torch.float32)
+    packed = [pack_pages(x, BF16) for x in (k, v)]
+    values = [held(p, BF16) for p in packed]
+    q = torch.randn(new * seqs, 8, 64, generator=g, device="cuda").to(BF16)
+    out = torch.full_like(q, 7.0)
+    paged.attention(q, *packed, table, kv_lens, cu_q, max_q_len=bound, causal=True, out=out)
+    with pytest.raises(DeviceStatusError, match="0x404"):
+        _ext.check_status(cuda_device)
+    want, _, error, _ = attend(q, *values, table, kv_lens, [new] * seqs, causal=True)
+    took = -(-bound * 4 // 8) * 2  # tokens of the rows that the kernel takes, eight at a time, four to a token
+    for s in range(seqs):
+        rows = slice(s * new, s * new + bound)
+        assert within(out[rows], want[rows], error[rows] + 800 * 2.0 ** -24 * float(values[1].abs().max()))
+        assert bool((out[s * new + took:(s + 1) * new] == 7.0).all())
