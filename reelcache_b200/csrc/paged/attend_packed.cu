@@ -20,6 +20,8 @@
 // transposed, a lane gets two neighbouring channels of two keys, which two byte permutations (over two registers) part into
 // the rows r and r + 8 of the product: a lane's outputs are two consecutive channels.
 //
+// More than 16 rows are slices of 16, each an item of its own next to the others of its head.
+//
 // Measured: 48 sessions of up to 16,384 keys (32 / 8 heads, 0.84 GB) 151 to 164 us, 5.1 to 5.6 TB/s (282 with the queries in the
 // rows of the product; 232 with spinning waits and copies that prefetch 256 bytes, of which a head's rows have 128; 163 head after
 // head instead of side by side); three CTAs on an SM and four are alike. One session over 2,048 keys 8 us clustered, a call 9.
@@ -125,14 +127,17 @@ __global__ void __launch_bounds__(kShortThreads, PackedShape<D, kN>::ctas)
   } else if (warp < 4) {
     place_share(p, work);
   }
-  const int side = kCluster ? 0 : static_cast<int>(blockIdx.x) % p.par;  // which of the heads that are taken side by side
+  // which of the heads, and slice of rows, that are taken side by side
+  const int sides = p.par * p.slices, beside = static_cast<int>(blockIdx.x) % sides;
+  const int slice = kCluster ? static_cast<int>(blockIdx.x) / p.cluster % p.slices : beside / p.par, side = kCluster ? 0 : beside - slice * p.par;
+  const int row0 = slice * 8 * kN;
   int s, base, begin, end;
   if (kCluster) {
-    const int item = static_cast<int>(blockIdx.x) / p.cluster, rank = static_cast<int>(blockIdx.x) - item * p.cluster;
+    const int index = static_cast<int>(blockIdx.x) / p.cluster, rank = static_cast<int>(blockIdx.x) - index * p.cluster, item = index / p.slices;
     s = item / a.kv_heads;
     const SeqWork w(a, s);
-    if (w.tiles == 0) {  // no new tokens: the whole cluster
-      if (threadIdx.x == 0) report_rows(a, s);
+    if (row0 >= w.q_len * a.group) {  // no rows: the whole cluster
+      if (threadIdx.x == 0 && slice == 0) report_rows(a, s);
       return;
     }
     base = (s * a.kv_heads - item) * w.tiles;  // the item's tiles are places 0 ..
@@ -162,6 +167,10 @@ __global__ void __launch_bounds__(kShortThreads, PackedShape<D, kN>::ctas)
       }
       const int place = (at - base) / w.tiles, t0 = (at - base) - place * w.tiles, head = place * p.par + side;
       const int t1 = min(w.tiles, t0 + end - at);
+      if (row0 >= w.q_len * a.group) {  // a slice without rows
+        at += t1 - t0;
+        continue;
+      }
       const TileRange<kShortTile> range(Sight(a, w.kv_len, w.q_len), 0, w.q_len);
       const int* table = a.table + s * a.table_row + head * a.table_head;
       // lanes 0-7 bring the scales of K, 8-15 those of V, eight keys each (eight never cross a page's end)
@@ -208,7 +217,7 @@ __global__ void __launch_bounds__(kShortThreads, PackedShape<D, kN>::ctas)
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     if (kCluster) {
-      if (lane == 0) report_rows(a, s);
+      if (lane == 0 && slice == 0) report_rows(a, s);
       cluster_sync_all();
       cluster_sync_all();
     }
@@ -230,9 +239,13 @@ __global__ void __launch_bounds__(kShortThreads, PackedShape<D, kN>::ctas)
       ++s;
       continue;
     }
-    const int place = kCluster ? static_cast<int>(blockIdx.x) / p.cluster - s * a.kv_heads : (at - base) / w.tiles;
+    const int place = kCluster ? static_cast<int>(blockIdx.x) / p.cluster / p.slices - s * a.kv_heads : (at - base) / w.tiles;
     const int t0 = kCluster ? begin : (at - base) - place * w.tiles, head = place * p.par + side;
     const int t1 = kCluster ? end : min(w.tiles, t0 + end - at);
+    if (row0 >= w.q_len * a.group) {  // a slice without rows
+      at += t1 - t0;
+      continue;
+    }
     const Sight sight(a, w.kv_len, w.q_len);
     const TileRange<kShortTile> range(sight, 0, w.q_len);
 
@@ -242,7 +255,7 @@ __global__ void __launch_bounds__(kShortThreads, PackedShape<D, kN>::ctas)
     int last[kN][2], low[kN][2];
 #pragma unroll
     for (int g = 0; g < kN; ++g) {
-      const int row = g * 8 + r0, query = row / a.group, h = head * a.group + row - query * a.group;
+      const int row = row0 + g * 8 + r0, query = row / a.group, h = head * a.group + row - query * a.group;
       const bool valid = query < w.q_len;
       const T* src = static_cast<const T*>(a.q) + static_cast<int64_t>(w.q_first + query) * a.q_token + h * a.q_head + quad * 4;
       float top = 0.0f;
@@ -275,11 +288,11 @@ __global__ void __launch_bounds__(kShortThreads, PackedShape<D, kN>::ctas)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         row_scale[g][i] = __shfl_sync(0xffffffffu, scale, (2 * quad + i) * 4);
-        last[g][i] = sight.last(min((g * 8 + 2 * quad + i) / a.group, w.q_len - 1));
+        last[g][i] = sight.last(min((row0 + g * 8 + 2 * quad + i) / a.group, w.q_len - 1));
         low[g][i] = sight.low(last[g][i]);
       }
     }
-    const int rows_here = w.q_len * a.group;  // or fewer: kRows
+    const int rows_here = w.q_len * a.group - row0;  // or fewer: 8 kN
     // bounds over the queries, for tiles that need no mask
     const int all_last = sight.last(0), all_low = sight.low(sight.last(w.q_len - 1));
     const int any_low = sight.low(all_last);
@@ -488,7 +501,7 @@ __global__ void __launch_bounds__(kShortThreads, PackedShape<D, kN>::ctas)
           }
       }
       cluster_sync_all();
-      join_few_cluster<T, D>(p, w, head, rows_here, res, res_ml, ok);
+      join_few_cluster<T, D>(p, w, head, row0, rows_here, res, res_ml, ok);
       cluster_sync_all();  // the others have read this CTA's rows
       return;
     }
@@ -499,7 +512,7 @@ __global__ void __launch_bounds__(kShortThreads, PackedShape<D, kN>::ctas)
       for (int g = 0; g < kN; ++g)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int row = g * 8 + 2 * quad + e, query = row / a.group, h = head * a.group + row - query * a.group;
+          const int row = g * 8 + 2 * quad + e, packed = row0 + row, query = packed / a.group, h = head * a.group + packed - query * a.group;
           if (query >= w.q_len) continue;
           const int64_t token = w.q_first + query;
           if (starts && ends) {
@@ -554,7 +567,7 @@ CUtensorMap code_map(const at::Tensor& t, int box) {
 }
 
 template <typename T, int D, int kN>
-void packed_launch(const Args& a, const at::Tensor& k_codes, const at::Tensor& v_codes, const Packed& k, const Packed& v,
+void packed_launch(const Args& a, int slices, const at::Tensor& k_codes, const at::Tensor& v_codes, const Packed& k, const Packed& v,
                    const at::Tensor& like, cudaStream_t stream, int device) {
   using Shape = PackedShape<D, kN>;
   PackedShort ps{};
@@ -569,9 +582,10 @@ void packed_launch(const Args& a, const at::Tensor& k_codes, const at::Tensor& v
   ps.v_scale_head = v.scale_head;
   const PageMaps maps = page_maps(k_codes, v_codes, p.a.tiling, kShortTile, code_map);
   packed_configure<T, D, kN>(device);
-  const int64_t items = static_cast<int64_t>(a.seqs) * a.kv_heads, slots = sm_count(device) * Shape::ctas;
+  const int64_t items = static_cast<int64_t>(a.seqs) * a.kv_heads * slices, slots = sm_count(device) * Shape::ctas;
   p.par = 1;
   p.rows = 8 * kN;
+  p.slices = slices;
   p.cluster = short_cluster<PackedForm<T, D, kN>>(items, short_tiles(a), p.a.tiling.step, a.seqs > 1 && a.table_head == 0, device);
   if (p.cluster > 0) {
     launch(packed_short_kernel<T, D, true, kN>, dim3(static_cast<unsigned>(items * p.cluster)), kShortThreads, Shape::bytes, p.cluster,
@@ -581,7 +595,9 @@ void packed_launch(const Args& a, const at::Tensor& k_codes, const at::Tensor& v
   // The line's CTAs take the KV heads side by side: the rows of neighbouring heads lie next to each other, and 128 bytes here
   // and there are too little for HBM (48 sessions of up to 16,384 keys: 163 us head after head).
   for (p.par = std::min(a.kv_heads, 32); a.kv_heads % p.par != 0;) --p.par;
-  const int ctas = static_cast<int>(std::min<int64_t>(slots / p.par, items / p.par * (short_tiles(a) + 1))) * p.par;
+  while (p.par > 1 && p.par * slices > slots)  // (few SMs)
+    for (--p.par; a.kv_heads % p.par != 0;) --p.par;
+  const int sides = p.par * slices, ctas = static_cast<int>(std::min<int64_t>(slots / sides, items / sides * (short_tiles(a) + 1))) * sides;
   RC_CHECK(items * (kRows / 4) < (1ll << 31), "too many sequences and rows for one launch");
   const int64_t floats = 2ll * ctas * kRows * (D + 2), ints = 1 + 2ll * a.seqs;
   at::Tensor workspace = new_tensor({floats + ints}, like, at::kFloat);
@@ -596,8 +612,9 @@ void packed_launch(const Args& a, const at::Tensor& k_codes, const at::Tensor& v
 template <typename T, int D>
 void packed_rows(const Args& a, int max_q_len, const at::Tensor& k_codes, const at::Tensor& v_codes, const Packed& k, const Packed& v,
                  const at::Tensor& like, cudaStream_t stream, int device) {
-  max_q_len * a.group <= 8 ? packed_launch<T, D, 1>(a, k_codes, v_codes, k, v, like, stream, device)
-                           : packed_launch<T, D, 2>(a, k_codes, v_codes, k, v, like, stream, device);
+  const int rows = max_q_len * a.group;
+  rows <= 8 ? packed_launch<T, D, 1>(a, 1, k_codes, v_codes, k, v, like, stream, device)
+            : packed_launch<T, D, 2>(a, (rows + 15) / 16, k_codes, v_codes, k, v, like, stream, device);
 }
 
 void attend_packed_short(const Args& a, int head_dim, bool half, const at::Tensor& k_codes, const at::Tensor& v_codes, const Packed& k,

@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(kShortThreads, kShortCtasPerSm)
         }
       }
       cluster_sync_all();
-      join_few_cluster<T, D>(p, w, head, rows_here, res, res_ml, ok);
+      join_few_cluster<T, D>(p, w, head, 0, rows_here, res, res_ml, ok);
       cluster_sync_all();  // the others have read this CTA's rows
       return;
     }
@@ -397,6 +397,7 @@ void short_launch(Args a, const at::Tensor& k_pages, const at::Tensor& v_pages, 
   const int64_t items = static_cast<int64_t>(a.seqs) * a.kv_heads, slots = sm_count(device) * kShortCtasPerSm;
   p.par = 1;
   p.rows = kRows;
+  p.slices = 1;
   p.cluster = short_form<T, D>(a, device);
   if (p.cluster > 0) {
     launch(short_kernel<T, D, true>, dim3(static_cast<unsigned>(items * p.cluster)), kShortThreads, Shape::bytes, p.cluster,

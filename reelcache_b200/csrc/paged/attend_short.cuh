@@ -29,8 +29,10 @@ struct Short {
   float* part_o;   // [2 * CTAs, 16, D]
   float* part_ml;  // [2 * CTAs, 16, 2]
   int cluster;     // CTAs of a cluster (the clustered form)
-  int rows;        // that the kernel takes: of a sequence with more new tokens than it was told, the others have no result
-  int par;         // KV heads that the line's CTAs take side by side (a divisor of their number): CTA par i + j the share i of the j-th
+  int rows;        // of an item: those of a sequence and KV head, or a slice of them
+  int slices;      // slices of a sequence's rows (others than they hold have no result)
+  int par;         // KV heads that the line's CTAs take side by side (a divisor of their number): of them and their
+                   // slices: CTA (par slices) i + j takes share i of the j-th, j = slice par + head
 };
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
@@ -101,7 +103,7 @@ __device__ __forceinline__ void place_share(const Short& p, int* work) {
     if (i < warp) before += n;
     total += n;
   }
-  const int ctas = static_cast<int>(gridDim.x) / p.par, index = static_cast<int>(blockIdx.x) / p.par;
+  const int sides = p.par * p.slices, ctas = static_cast<int>(gridDim.x) / sides, index = static_cast<int>(blockIdx.x) / sides;
   const int share = max(min(kShortLeast, total), (total + ctas - 1) / ctas);
   const int begin = min(total, index * share), end = min(total, begin + share);
   if (threadIdx.x == 0) {
@@ -220,7 +222,7 @@ __device__ __forceinline__ void join_warps(float (&o)[D / 8][4], float (&m)[2], 
 // [kRows][D] FP32, `res_ml` [kRows][maximum, sum] of each CTA. For 128 threads; the cluster has to meet once more before `res`
 // may be written again.
 template <typename T, int D>
-__device__ __forceinline__ void join_few_cluster(const Short& p, const SeqWork& w, int head, int rows_here, const float* res,
+__device__ __forceinline__ void join_few_cluster(const Short& p, const SeqWork& w, int head, int row0, int rows_here, const float* res,
                                                  const float* res_ml, bool ok) {
   const Args& a = p.a;
   const int rank = static_cast<int>(blockIdx.x) % p.cluster;
@@ -261,7 +263,7 @@ __device__ __forceinline__ void join_few_cluster(const Short& p, const SeqWork& 
       }
     }
     const float inv = inverse(sum);
-    const int query = row / a.group, h = head * a.group + row - query * a.group;
+    const int query = (row0 + row) / a.group, h = head * a.group + row0 + row - query * a.group;
     const int64_t token = w.q_first + query;
     T* dst = static_cast<T*>(a.out) + token * a.out_token + h * a.out_head + col;
     if (ok) *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
@@ -278,19 +280,19 @@ __global__ void __launch_bounds__(128) short_join_kernel(const __grid_constant__
   const int lane = threadIdx.x & 31;
   const int quads = kRows / 4;
   const int row = (blockIdx.x % quads) * 4 + (threadIdx.x >> 5);
-  const int item = blockIdx.x / quads, s = item / a.kv_heads, head = item - s * a.kv_heads;
+  const int index = blockIdx.x / quads, item = index / p.slices, slice = index - item * p.slices, s = item / a.kv_heads, head = item - s * a.kv_heads;
   let_later();
   after_earlier();
-  if (row == 0 && head == 0 && lane == 0) report_rows(a, s);
+  if (row == 0 && head == 0 && slice == 0 && lane == 0) report_rows(a, s);
   const SeqWork w(a, s);
-  const int query = row / a.group;
+  const int packed = slice * p.rows + row, query = packed / a.group;
   if (query >= w.q_len || row >= p.rows) return;
   const int share = *p.line.share;
-  const int place = head / p.par, side = head - place * p.par;
+  const int place = head / p.par, side = slice * p.par + head - place * p.par;
   const int begin = p.line.first[s] + place * w.tiles, end = begin + w.tiles;
   const int c0 = begin / share, c1 = (end - 1) / share;
   if (c0 == c1) return;
-  const auto slot_of = [&](int c) { return (2 * (static_cast<int64_t>(c) * p.par + side) + (c == c0)) * kRows + row; };
+  const auto slot_of = [&](int c) { return (2 * (static_cast<int64_t>(c) * p.par * p.slices + side) + (c == c0)) * kRows + row; };
   // 32 parts at a time, a lane to each one's maximum and sum
   float top = -INFINITY, acc[kPer], sum = 0.0f;
 #pragma unroll
@@ -325,7 +327,7 @@ __global__ void __launch_bounds__(128) short_join_kernel(const __grid_constant__
   }
   const float inv = inverse(sum);
   const int64_t token = w.q_first + query;
-  const int h = head * a.group + row - query * a.group;
+  const int h = head * a.group + packed - query * a.group;
   T* dst = static_cast<T*>(a.out) + token * a.out_token + h * a.out_head + lane * kPer;
 #pragma unroll
   for (int e = 0; e < kPer; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack2<T>(acc[e] * inv, acc[e + 1] * inv);

@@ -114,7 +114,7 @@ def attention(q, k_pages, v_pages, block_table, kv_lens, cu_q, *, max_q_len: int
     ``cu_q`` belong to no sequence: they have no result (a new output holds anything there). ``return_lse`` adds the natural log-sum-exp ``[T, heads]``.
 
     ``block_table`` may be ``[seqs, kv_heads, width]``, a table for each KV head. Packed pages give what their rows read as
-    :func:`read` gives, in ``q``'s type; with up to 16 rows (new tokens x heads of a group) the codes are taken as they are and
+    :func:`read` gives, in ``q``'s type; with up to 48 rows (new tokens x heads of a group) the codes are taken as they are and
     the probabilities are rounded to fp16, with more the pages that are seen are expanded first (16-bit copies of them, for
     the time of the call)."""
     if not q.is_cuda:

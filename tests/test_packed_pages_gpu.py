@@ -199,6 +199,15 @@ def test_drafts_and_chunks(new, totals, heads, kv_heads, d, page, dtype, causal)
     _check(new, totals, heads, kv_heads, d, page, dtype, causal=causal, scales=4)
 
 
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("new,totals,heads,kv_heads,d", [
+    ([12, 1, 0, 7], [700, 300, 40, 7], 8, 2, 128), ([12] * 40, [300 + 17 * i for i in range(40)], 8, 2, 64), ([3, 2, 1], [90, 4000, 65], 48, 3, 64),
+    ([1] * 9, [50 + 333 * i for i in range(9)], 37, 1, 128), ([17], [2000], 2, 1, 128), ([24] * 20, [24 + 90 * i for i in range(20)], 2, 1, 64)])
+def test_slices_of_rows(new, totals, heads, kv_heads, d, causal):
+    """17 to 48 rows: slices of 16, of which some sequences have fewer, in a line and in clusters."""
+    _check(new, totals, heads, kv_heads, d, 16, BF16, causal=causal, scales=4, noise=True)
+
+
 @pytest.mark.parametrize("new,totals,heads,page", [([1, 1], [70, 333], 4, 16), ([3], [41], 4, 24), ([20], [141], 4, 24), ([200, 3], [333, 3], 2, 64)])
 def test_what_no_session_holds_may_hold_anything(new, totals, heads, page):
     _check(new, totals, heads, 2, 128, page, BF16, noise=True, causal=True, scales=3)
@@ -417,7 +426,7 @@ def test_many_kv_heads_side_by_side():
 
 
 @pytest.mark.parametrize("seqs", [1, 60])
-@pytest.mark.parametrize("new,bound", [(5, 1), (9, 3)])
+@pytest.mark.parametrize("new,bound", [(5, 1), (9, 3), (16, 9)])
 def test_more_new_tokens_than_the_bound_are_reported(new, bound, seqs, cuda_device):
     """The tokens up to the bound have their results; rows that the kernel does not take are left as they were."""
     from reelcache_b200.errors import DeviceStatusError
@@ -432,7 +441,8 @@ def test_more_new_tokens_than_the_bound_are_reported(new, bound, seqs, cuda_devi
     with pytest.raises(DeviceStatusError, match="0x404"):
         _ext.check_status(cuda_device)
     want, _, error, _ = attend(q, *values, table, kv_lens, [new] * seqs, causal=True)
-    took = -(-bound * 4 // 8) * 2  # tokens of the rows that the kernel takes, eight at a time, four to a token
+    # tokens of the rows that the kernel takes: eight, or slices of 16 (9 tokens of four rows: 36, three slices, 12 tokens)
+    took = 2 if bound * 4 <= 8 else -(-bound * 4 // 16) * 4
     for s in range(seqs):
         rows = slice(s * new, s * new + bound)
         assert within(out[rows], want[rows], error[rows] + 800 * 2.0 ** -24 * float(values[1].abs().max()))
