@@ -387,6 +387,7 @@ class PagedKVCache:
         return batch.table[seq, at // self.page_size].long() * self.page_size + at % self.page_size
 
     def rows(self, layer: int, which: str, page: int) -> torch.Tensor:
-        """Token rows ``[page_size, kv_heads * head_dim]`` of one page (``which``: ``"K"`` or ``"V"``)."""
+        """Token rows ``[page_size, kv_heads * head_dim]`` of one page (``which``: ``"K"`` or ``"V"``). Keys written there are unknown to
+        the means of a cache that keeps some until :meth:`rows_written`."""
         self._in_16_bits()
         return self.storage[layer, 0 if which == "K" else 1, page].flatten(1)
