@@ -108,7 +108,8 @@ __global__ void __launch_bounds__(kThreads, kTurn == 2 ? 2 : kTurn == 1 ? 4 : 5)
   }
 
   // A code that falls to its neighbour is 2^-3 off, so k is turned nearer than FP32's sines allow: by sines of FP64 as the sums of
-  // two numbers, computed once for all of the thread's heads. What is left are two roundings, 2^-24 each.
+  // two numbers, computed once for all of the thread's heads. What is left are two roundings, 2^-24 each (18 of 21.6 million
+  // codes are not the exact rotation's; over 100 with FP32 throughout).
   float cs[kPairs] = {}, sn[kPairs] = {}, cs_low[kPairs] = {}, sn_low[kPairs] = {};
   const bool turned = kTurn != 0 && (is_q || is_k);
   if (turned && active && is_q) rotary::sines<false>(a, token, vec, cs, sn);
