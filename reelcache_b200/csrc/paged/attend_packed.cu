@@ -11,9 +11,11 @@
 // Codes become fp16 in registers, exactly, two by one conversion; the products are fp16 whatever the rows' type. Q is brought
 // to fp16 by a power of two for each row that puts its largest magnitude between 2^6 and 2^7: exact for what is at least 2^-20
 // of that, off by at most 2^-31 of it below. Scales multiply neither codes nor channels: K's multiply the scores (FP32), V's
-// multiply the probabilities, which are rounded to fp16 for the product (half a step of 2^-10; their sum is not): a warp keeps the
-// largest scale of V that it has seen as the unit of its output, so that no product overflows. Maximum and unit move
-// rarely, each after a vote: the maximum when a score is more than 2^8 above it, the unit when a scale is.
+// the probabilities, as addends of their exponents: weight = 2^(score + log2 scale - unit). A row's unit follows the largest
+// score + log2 scale that the row sees (not the largest scale, which may belong to a key of no weight), so that this key's weight
+// lies between 2^7 and 2^15 of fp16's range. Weights are rounded to fp16 for the product: by half a step of 2^-10 of their size, or,
+// below 2^-14, by 2^-25, which is 2^-32 of the largest weight; their sum, of the probabilities alone, is FP32. Maximum and unit move
+// rarely, after one vote: the maximum when a score is more than 2^8 above it, the unit when a weight is above 2^15.
 //
 // Fragments without shuffles: ldmatrix hands a lane four consecutive channels of a key, taken as the pairs (2 t, 2 t + 1) and (2 t +
 // 8, 2 t + 9) of the product's inner index: any order of channels gives the same sum, and Q is read in that order. Of V,
@@ -66,8 +68,8 @@ __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
   return D == 128 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
 }
 
-// 2^(e - base) of a scale byte not above base. (A scale of NaN is above all others: what then is in its units is NaN.)
-__device__ __forceinline__ float relative_scale(int e, int base) { return __uint_as_float(static_cast<uint32_t>(max(127 + e - base, 0)) << 23); }
+// log2 of a scale byte.
+__device__ __forceinline__ float scale_log2(int byte) { return byte == kNanScale ? __uint_as_float(0x7fffffffu) : static_cast<float>(byte - 127); }
 
 __device__ __forceinline__ int load_byte(uint32_t shared) {
   uint32_t v;
@@ -81,7 +83,9 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
   return out;
 }
 
-constexpr float kFewRescale = 8.0f;  // log2
+constexpr float kFewRescale = 8.0f;  // log2 of how far a score may be above the maximum
+constexpr float kUnitTop = 7.0f;     // log2 of the largest weight when the unit moves,
+constexpr float kUnitRoom = 15.0f;   // and of what it may grow to before the unit moves again
 
 template <typename T>
 __device__ __forceinline__ float2 two_of(uint32_t v);
@@ -310,7 +314,9 @@ __global__ void __launch_bounds__(kShortThreads, PackedShape<D, kN>::ctas)
       m[g][0] = m[g][1] = -INFINITY;
       l[g][0] = l[g][1] = 0.0f;
     }
-    int unit = 0;  // o is in units of 2^(unit - 127): the largest scale of V so far
+    float unit[kN][2];  // o is in units of 2^unit
+#pragma unroll
+    for (int g = 0; g < kN; ++g) unit[g][0] = unit[g][1] = -INFINITY;
 
     for (int t = t0; t < t1; ++t) {
       const int first = range.tile(t) * kShortTile;
@@ -364,44 +370,47 @@ __global__ void __launch_bounds__(kShortThreads, PackedShape<D, kN>::ctas)
             }
           }
         }
-        bool grows = max(v_scale[0], v_scale[1]) > unit;
+        const float v_log[2] = {scale_log2(v_scale[0]), scale_log2(v_scale[1])};
+        bool grows = false;
 #pragma unroll
         for (int g = 0; g < kN; ++g)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) grows = grows || fmaxf(sc[g][e], sc[g][2 + e]) > m[g][e] + kFewRescale;
+          for (int e = 0; e < 2; ++e)
+            grows = grows || fmaxf(sc[g][e], sc[g][2 + e]) > m[g][e] + kFewRescale ||
+                    fmaxf(sc[g][e] + v_log[0], sc[g][2 + e] + v_log[1]) > unit[g][e] + kUnitRoom;
         if (__any_sync(0xffffffffu, grows)) {
-          const int before = unit;
-          unit = max(unit, __reduce_max_sync(0xffffffffu, max(v_scale[0], v_scale[1])));
-          const float grown = relative_scale(before, unit);
 #pragma unroll
           for (int g = 0; g < kN; ++g)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              float top = fmaxf(sc[g][e], sc[g][2 + e]);
+              float top = fmaxf(sc[g][e], sc[g][2 + e]), high = fmaxf(sc[g][e] + v_log[0], sc[g][2 + e] + v_log[1]);
 #pragma unroll
-              for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+              for (int x = 4; x < 32; x <<= 1) {
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, x));
+              }
               top = fmaxf(top, m[g][e]);
-              const float faded = fade(m[g][e], top);
+              high = fmaxf(high - kUnitTop, unit[g][e]);
+              l[g][e] *= fade(m[g][e], top);
               m[g][e] = top;
-              l[g][e] *= faded;
+              const float faded = fade(unit[g][e], high);
+              unit[g][e] = high;
 #pragma unroll
               for (int c = 0; c < D / 16; ++c) {
-                o[g][c][e] *= faded * grown;
-                o[g][c][2 + e] *= faded * grown;
+                o[g][c][e] *= faded;
+                o[g][c][2 + e] *= faded;
               }
             }
         }
-        // P^T, and with V's scales in fp16 as the right operand
-        const float v_factor[2] = {relative_scale(v_scale[0], unit), relative_scale(v_scale[1], unit)};
+        // the probabilities for their sum, and the weights in fp16 as the right operand
         uint32_t pb[kN][2];
 #pragma unroll
         for (int g = 0; g < kN; ++g) {
-          const float use[2] = {base_of(m[g][0]), base_of(m[g][1])};
+          const float use[2] = {base_of(m[g][0]), base_of(m[g][1])}, in[2] = {base_of(unit[g][0]), base_of(unit[g][1])};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            sc[g][e] = exp2_approx(sc[g][e] - use[e & 1]);
-            l[g][e & 1] += sc[g][e];
-            sc[g][e] *= v_factor[e >> 1];
+            l[g][e & 1] += exp2_approx(sc[g][e] - use[e & 1]);
+            sc[g][e] = exp2_approx(sc[g][e] + (v_log[e >> 1] - in[e & 1]));
           }
           pb[g][0] = transpose_8x8(pack_f16x2(sc[g][0], sc[g][1]));
           pb[g][1] = transpose_8x8(pack_f16x2(sc[g][2], sc[g][3]));
@@ -430,12 +439,13 @@ __global__ void __launch_bounds__(kShortThreads, PackedShape<D, kN>::ctas)
     }
 
     // Warps that split the keys join theirs into key group 0 through shared memory. The same lane of every warp holds the same
-    // rows and channels, so the buffer is laid out by lane.
-    const float in_units = scale_value(unit);
+    // rows and channels, so the buffer is laid out by lane. Maxima become ones that no score is above.
 #pragma unroll
     for (int g = 0; g < kN; ++g)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
+        m[g][e] += kFewRescale;
+        l[g][e] *= exp2f(-kFewRescale);
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) l[g][e] += __shfl_xor_sync(0xffffffffu, l[g][e], x);
         if (r0 == 0) *reinterpret_cast<float2*>(join_ml + (kg * kRows + g * 8 + 2 * quad + e) * 2) = make_float2(m[g][e], l[g][e]);
@@ -455,13 +465,13 @@ __global__ void __launch_bounds__(kShortThreads, PackedShape<D, kN>::ctas)
         const float use = base_of(top);
 #pragma unroll
         for (int k = 0; k < kGroups; ++k) total = fmaf(ml[k].y, exp2_approx(ml[k].x - use), total);
-        const float weight = exp2_approx(m[g][e] - use) * in_units;
+        const float root = exp2_approx(0.5f * (unit[g][e] - use));  // (its square may be below FP32's range where o times it is not)
         m[g][e] = top;
         l[g][e] = total;
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) {
-          o[g][c][e] *= weight;
-          o[g][c][2 + e] *= weight;
+          o[g][c][e] = o[g][c][e] * root * root;
+          o[g][c][2 + e] = o[g][c][2 + e] * root * root;
         }
       }
 #pragma unroll

@@ -115,7 +115,7 @@ def attention(q, k_pages, v_pages, block_table, kv_lens, cu_q, *, max_q_len: int
 
     ``block_table`` may be ``[seqs, kv_heads, width]``, a table for each KV head. Packed pages give what their rows read as
     :func:`read` gives, in ``q``'s type; with up to 48 rows (new tokens x heads of a group) the codes are taken as they are and
-    the probabilities are rounded to fp16, with more the pages that are seen are expanded first (16-bit copies of them, for
+    the probabilities times V's scales are rounded to fp16 (a key's by half a step, or by 2^-32 of the largest where that is more), with more the pages that are seen are expanded first (16-bit copies of them, for
     the time of the call)."""
     if not q.is_cuda:
         raise UnsupportedError("paged attention needs CUDA tensors")
