@@ -137,7 +137,9 @@ __global__ void __launch_bounds__(kThreads, kTurn == 2 ? 2 : kTurn == 1 ? 4 : 5)
     for (int i = 0; i < kHeads; ++i) {
       Vec<T>::unpack(raw[i][0], x[i]);
       if (kHalves) Vec<T>::unpack(raw[i][kParts - 1], y2[i]);
-      if (turned) {
+      if (turned && is_q) {  // (as beside 16-bit pages: products with low parts of 0 would turn infinities into NaN)
+        rotary::turn<kHalves>(x[i], y2[i], cs, sn);
+      } else if (turned) {
 #pragma unroll
         for (int e = 0; e < kPairs; ++e) {
           float& p = x[i][kHalves ? e : 2 * e];
