@@ -21,6 +21,7 @@ gives a new one.
 from __future__ import annotations
 
 from dataclasses import dataclass, field
+from itertools import accumulate
 from typing import Sequence
 
 import torch
@@ -89,7 +90,8 @@ class PagedKVCache:
     ``packed``: rows of ``dtype`` are held in 8 bits (:class:`~reelcache_b200.ops.paged.PackedPages`); ``storage`` has the codes, ``scales
     [layers, 2, kv_heads, pages, page_size]`` their scales. ``block`` (a divisor of the page size, a multiple of 8): ``means
     [layers, pages, page_size / block, kv_heads, head_dim]`` has the mean key of every ``block`` positions, kept up to date by
-    :meth:`append` and :meth:`store`, for attention over chosen blocks."""
+    :meth:`append` and :meth:`store`, for attention over chosen blocks (a captured call brings them to what the sessions held when it
+    was captured)."""
 
     def __init__(self, layers: int, kv_heads: int, head_dim: int, *, pages: int, page_size: int, max_sessions: int,
                  max_tokens: int, device="cuda", dtype=torch.bfloat16, packed: bool = False, block: int | None = None):
@@ -327,9 +329,18 @@ class PagedKVCache:
             raise ConfigurationError(f"the cache holds rows of {self.dtype}, got {rows.dtype}")
 
     def _update_means(self, layer: int, batch: PagedBatch):
-        if self.block is not None and batch.tokens:
-            paged.block_means(self.layer_pages(layer)[0], self.means[layer], batch.table, batch.kv_lens, batch.cu_q,
-                              max_q_len=max(batch.counts))
+        if self.block is None or not batch.tokens:
+            return
+        table, kv_lens, cu_q, longest = batch.table, batch.kv_lens, batch.cu_q, max(batch.counts)
+        if any(s.length != n for s, n in zip(batch.sessions, batch.lengths)):
+            # a block's mean is that of what its session holds by now: the batch's new tokens and all that came after
+            # them (by kernels that take the numbers as arguments: a capture must not keep copies from host memory)
+            width = -(-max(s.length for s in batch.sessions) // self.page_size)
+            counts = [s.length - (length - n) if n else 0 for s, n, length in zip(batch.sessions, batch.counts, batch.lengths)]
+            ints = lambda values: torch.cat([torch.full((1,), n, dtype=torch.int32, device=self.device) for n in values])  # noqa: E731
+            table = torch.cat([self.table.block_table[s.slot:s.slot + 1, :width] for s in batch.sessions])
+            kv_lens, cu_q, longest = ints(s.length for s in batch.sessions), ints(accumulate(counts, initial=0)), max(counts)
+        paged.block_means(self.layer_pages(layer)[0], self.means[layer], table, kv_lens, cu_q, max_q_len=longest)
 
     def attend(self, layer: int, batch: PagedBatch, q, *, causal: bool = False, window: int | None = None, sinks: int = 0,
                scale: float | None = None, return_lse: bool = False, out=None, keep: int | None = None, query_block: int = 1,
