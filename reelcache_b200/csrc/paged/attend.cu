@@ -33,13 +33,16 @@ void expand_pages(Args& a, const at::Tensor& k_codes, const at::Tensor& v_codes,
                   at::Tensor& v_pages, at::Tensor& workspace, const at::Tensor& like, cudaStream_t stream);
 std::string short_form_name(const Args& a, int head_dim, int device);
 std::string chunk_form_name(const Args& a, int head_dim, int max_q_len, int device);
+std::string packed_form_name(const Args& a, int head_dim, int max_q_len, int device);
 
 }  // namespace paged
 
 // The form that a call of these sizes takes on `device`: "few rows, cluster N", "few rows, line", "twin N", "direct N" (N CTAs
-// to a cluster) or "planned".
+// to a cluster), "planned"; with a table for each KV head (`tables`) also "twin 1, then M items in N"; over packed pages few rows may be
+// in "S slices, ...", and more rows are "expanded, " and a form of theirs.
 std::string paged_attention_form(int64_t device, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t seqs,
-                                 int64_t width, int64_t page_size, int64_t max_q_len, bool causal, int64_t window, int64_t sinks) {
+                                 int64_t width, int64_t page_size, int64_t max_q_len, bool causal, int64_t window, int64_t sinks, bool packed,
+                                 bool tables) {
   RC_CHECK((head_dim == 64 || head_dim == 128) && tokens > 0 && kv_heads > 0 && heads % kv_heads == 0 && seqs > 0 && max_q_len > 0,
            "no such call of paged attention");
   c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
@@ -54,8 +57,11 @@ std::string paged_attention_form(int64_t device, int64_t tokens, int64_t heads, 
   a.causal = causal;
   a.window = static_cast<int>(window);
   a.sinks = window > 0 ? static_cast<int>(sinks) : 0;
+  a.table_head = tables ? std::max(a.width, 1) : 0;
   const int most = static_cast<int>(std::min(max_q_len, tokens)), d = static_cast<int>(head_dim), at = static_cast<int>(device);
-  return static_cast<int64_t>(most) * a.group <= paged::kShortRows ? paged::short_form_name(a, d, at) : paged::chunk_form_name(a, d, most, at);
+  const bool few = static_cast<int64_t>(most) * a.group <= (packed ? paged::kPackedRows : paged::kShortRows);
+  if (few) return packed ? paged::packed_form_name(a, d, most, at) : paged::short_form_name(a, d, at);
+  return (packed ? "expanded, " : "") + paged::chunk_form_name(a, d, most, at);
 }
 
 // out = softmax over the visible keys of scale * q k^T, times v, for the new tokens of every sequence; lse its natural

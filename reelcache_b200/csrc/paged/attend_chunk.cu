@@ -1211,7 +1211,9 @@ std::string chunk_form_name(const Args& a, int head_dim, int max_q_len, int devi
   const ChunkForm form = head_dim == 128 ? chunk_form<__nv_bfloat16, 128>(a, max_q_len, device)
                                          : chunk_form<__nv_bfloat16, 64>(a, max_q_len, device);
   if (form.cluster == 0) return "planned";
-  return (form.twin ? "twin " : "direct ") + std::to_string(form.cluster);
+  const std::string name = form.twin ? "twin " : "direct ";
+  if (form.whole_items == 0) return name + std::to_string(form.cluster);
+  return name + "1, then " + std::to_string(form.grid_items - form.whole_items) + " items in " + std::to_string(form.cluster);
 }
 
 }  // namespace paged

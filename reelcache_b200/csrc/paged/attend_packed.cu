@@ -576,6 +576,13 @@ CUtensorMap code_map(const at::Tensor& t, int box) {
   return map;
 }
 
+// CTAs of an item's cluster, or 0 for the line.
+template <typename T, int D, int kN>
+int packed_cluster(const Args& a, int slices, int device) {
+  return short_cluster<PackedForm<T, D, kN>>(static_cast<int64_t>(a.seqs) * a.kv_heads * slices, short_tiles(a),
+                                             Tiling::of(a.tiling.page, kShortTile).step, a.seqs > 1 && a.table_head == 0, device);
+}
+
 template <typename T, int D, int kN>
 void packed_launch(const Args& a, int slices, const at::Tensor& k_codes, const at::Tensor& v_codes, const Packed& k, const Packed& v,
                    const at::Tensor& like, cudaStream_t stream, int device) {
@@ -596,7 +603,7 @@ void packed_launch(const Args& a, int slices, const at::Tensor& k_codes, const a
   p.par = 1;
   p.rows = 8 * kN;
   p.slices = slices;
-  p.cluster = short_cluster<PackedForm<T, D, kN>>(items, short_tiles(a), p.a.tiling.step, a.seqs > 1 && a.table_head == 0, device);
+  p.cluster = packed_cluster<T, D, kN>(a, slices, device);
   if (p.cluster > 0) {
     launch(packed_short_kernel<T, D, true, kN>, dim3(static_cast<unsigned>(items * p.cluster)), kShortThreads, Shape::bytes, p.cluster,
            stream, maps, ps);
@@ -619,12 +626,14 @@ void packed_launch(const Args& a, int slices, const at::Tensor& k_codes, const a
   launch(short_join_kernel<T, D>, dim3(static_cast<unsigned>(items * (kRows / 4))), 128, 0, 0, stream, p);
 }
 
+int packed_slices(int rows) { return (rows + 15) / 16; }
+
 template <typename T, int D>
 void packed_rows(const Args& a, int max_q_len, const at::Tensor& k_codes, const at::Tensor& v_codes, const Packed& k, const Packed& v,
                  const at::Tensor& like, cudaStream_t stream, int device) {
   const int rows = max_q_len * a.group;
   rows <= 8 ? packed_launch<T, D, 1>(a, 1, k_codes, v_codes, k, v, like, stream, device)
-            : packed_launch<T, D, 2>(a, (rows + 15) / 16, k_codes, v_codes, k, v, like, stream, device);
+            : packed_launch<T, D, 2>(a, packed_slices(rows), k_codes, v_codes, k, v, like, stream, device);
 }
 
 void attend_packed_short(const Args& a, int head_dim, bool half, const at::Tensor& k_codes, const at::Tensor& v_codes, const Packed& k,
@@ -635,6 +644,20 @@ void attend_packed_short(const Args& a, int head_dim, bool half, const at::Tenso
   else
     half ? packed_rows<__half, 64>(a, max_q_len, k_codes, v_codes, k, v, like, stream, device)
          : packed_rows<__nv_bfloat16, 64>(a, max_q_len, k_codes, v_codes, k, v, like, stream, device);
+}
+
+template <int D, int kN>
+int packed_form(const Args& a, int slices, int device) {
+  packed_configure<__nv_bfloat16, D, kN>(device);
+  return packed_cluster<__nv_bfloat16, D, kN>(a, slices, device);
+}
+
+std::string packed_form_name(const Args& a, int head_dim, int max_q_len, int device) {
+  const int rows = max_q_len * a.group, slices = packed_slices(rows);
+  const int cluster = head_dim == 128 ? (rows <= 8 ? packed_form<128, 1>(a, 1, device) : packed_form<128, 2>(a, slices, device))
+                                      : (rows <= 8 ? packed_form<64, 1>(a, 1, device) : packed_form<64, 2>(a, slices, device));
+  return (slices > 1 ? std::to_string(slices) + " slices, " : std::string("few rows, ")) +
+         (cluster > 0 ? "cluster " + std::to_string(cluster) : "line");
 }
 
 }  // namespace paged

@@ -130,11 +130,13 @@ def attention(q, k_pages, v_pages, block_table, kv_lens, cu_q, *, max_q_len: int
 
 
 def attention_form(tokens, heads, kv_heads, head_dim, seqs, width, page_size, *, max_q_len: int, causal: bool = False,
-                   window: int | None = None, sinks: int = 0, device: int = 0) -> str:
+                   window: int | None = None, sinks: int = 0, packed: bool = False, tables: bool = False, device: int = 0) -> str:
     """Which form of the kernels a call of :func:`attention` with these sizes takes: ``"few rows, cluster N"``, ``"few rows,
-    line"``, ``"twin N"``, ``"direct N"`` (``N`` CTAs to a cluster) or ``"planned"``. ``width``: columns of the block table."""
+    line"``, ``"twin N"``, ``"direct N"`` (``N`` CTAs to a cluster) or ``"planned"``. ``width``: columns of the block table.
+    ``packed``: over packed pages, ``"few rows, ..."``, ``"S slices, ..."`` (of 16 rows) or ``"expanded, "`` and a form of more rows.
+    ``tables``: with a table for each KV head, also ``"twin 1, then M items in N"`` (the last ``M`` in clusters of ``N``)."""
     return ext().paged_attention_form(device, tokens, heads, kv_heads, head_dim, seqs, width, page_size, max_q_len, causal,
-                                      window or 0, sinks)
+                                      window or 0, sinks, packed, tables)
 
 
 def blocks(pages, block: int):
