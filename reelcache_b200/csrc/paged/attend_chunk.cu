@@ -41,6 +41,7 @@
 #include <c10/cuda/CUDAStream.h>
 
 #include <algorithm>
+#include <cmath>
 #include <string>
 #include <type_traits>
 
@@ -1131,13 +1132,15 @@ ChunkForm chunk_form(const Args& a, int max_q_len, int device) {
   if (a.table_head != 0 && form.cluster > 0) {
     const int64_t sms = sm_count(device), rest = form.grid_items % sms;
     if (form.grid_items > sms && rest > 0) {
+      // (rounds of clusters: what the device holds of a size at a time, none of some sizes perhaps)
+      const auto rounds = [&](int64_t items, int c) {
+        const int64_t slots = c > 1 ? clusters_at_once<T, D>(c, device) : sms;
+        return slots <= 0 ? HUGE_VAL : static_cast<double>((items + slots - 1) / slots) * (static_cast<double>((each + c - 1) / c) + (c > 1 ? 6.0 : 3.5));
+      };
       int cluster = 1;
-      while (cluster < 16 && rest * cluster * 2 <= sms) cluster *= 2;
-      const double split = static_cast<double>(form.grid_items / sms) * (each + 3.5) + (each + cluster - 1) / cluster + (cluster > 1 ? 6.0 : 3.5);
-      const int64_t slots = form.cluster > 1 ? clusters_at_once<T, D>(form.cluster, device) : sms;
-      const double one = static_cast<double>((form.grid_items + slots - 1) / slots) *
-                         (static_cast<double>((each + form.cluster - 1) / form.cluster) + (form.cluster > 1 ? 6.0 : 3.5));
-      if (split < one) {
+      for (int c = 2; c <= 16; c *= 2)
+        if (rounds(rest, c) < rounds(rest, cluster)) cluster = c;
+      if (rounds(form.grid_items - rest, 1) + rounds(rest, cluster) < rounds(form.grid_items, form.cluster)) {
         form.whole_items = form.grid_items - rest;
         form.cluster = cluster;
       }
