@@ -2,7 +2,9 @@
 #pragma once
 
 #include <ATen/ATen.h>
+#include <ATen/Context.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 
 #include "../common/host.h"
 
@@ -94,9 +96,15 @@ struct Divider {
 #endif
 };
 
-// A new tensor on `like`'s device, without the dispatcher (half a microsecond of a call's five).
+// A new tensor on `like`'s device, without the dispatcher (half a microsecond of a call's five) where nobody asks for it: a
+// dispatch mode sees allocations, and deterministic algorithms fill new memory.
 inline at::Tensor new_tensor(at::IntArrayRef sizes, const at::Tensor& like, at::ScalarType type) {
-  return at::detail::empty_cuda(sizes, like.options().dtype(type));
+  const at::TensorOptions options = like.options().dtype(type);
+  const at::Context& context = at::globalContext();
+  if (c10::impl::TorchDispatchModeTLS::any_modes_set() ||
+      (context.deterministicAlgorithms() && context.deterministicFillUninitializedMemory()))
+    return at::empty(sizes, options);
+  return at::detail::empty_cuda(sizes, options);
 }
 
 struct Pages {  // [pages, page_size, kv_heads, head_dim], strides in elements
