@@ -76,6 +76,11 @@ std::pair<at::Tensor, c10::optional<at::Tensor>> paged_attention(
   refuse_gradients({&q, &k_pages, &v_pages}, "attention over pages");
   if (out_given.has_value()) refuse_gradients({&*out_given}, "attention over pages");
   refuse_tangents({&q, &k_pages, &v_pages}, "attention over pages");
+  for (const c10::optional<at::Tensor>* scales : {&k_scales, &v_scales}) {
+    if (!scales->has_value()) continue;
+    refuse_gradients({&**scales}, "attention over pages");
+    refuse_tangents({&**scales}, "attention over pages");
+  }
   const at::ScalarType type = q.scalar_type();
   RC_CHECK(type == at::kBFloat16 || type == at::kHalf, "paged attention takes bf16 or fp16");
   RC_CHECK(q.dim() == 3 && (q.size(2) == 64 || q.size(2) == 128), "q must be [tokens, heads, head_dim] with head_dim 64 or 128");

@@ -346,9 +346,9 @@ at::Tensor packed_append(const at::Tensor& q, const at::Tensor& k, const at::Ten
                          const at::Tensor& v_scales, const at::Tensor& table, const at::Tensor& kv_lens, const at::Tensor& cu_q,
                          const c10::optional<at::Tensor>& out, const c10::optional<at::Tensor>& status) {
   check_cuda_tensor(q, "q");
-  refuse_gradients({&q, &k, &v, &positions, &k_codes, &v_codes}, "append");
+  refuse_gradients({&q, &k, &v, &positions, &k_codes, &k_scales, &v_codes, &v_scales}, "append");
   if (out.has_value()) refuse_gradients({&*out}, "append");
-  refuse_tangents({&q, &k, &v, &positions}, "append");
+  refuse_tangents({&q, &k, &v, &positions, &k_codes, &k_scales, &v_codes, &v_scales}, "append");
   c10::cuda::CUDAGuard guard(q.device());
   pack::Args p{};
   pack::set_rows(p, k, v, k_codes, k_scales, v_codes, v_scales, table, kv_lens, cu_q, status);
@@ -378,8 +378,8 @@ void packed_store(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_
                   const at::Tensor& v_codes, const at::Tensor& v_scales, const at::Tensor& table, const at::Tensor& kv_lens,
                   const at::Tensor& cu_q, const c10::optional<at::Tensor>& status) {
   check_cuda_tensor(k, "k");
-  refuse_gradients({&k, &v, &k_codes, &v_codes}, "store");
-  refuse_tangents({&k, &v}, "store");
+  refuse_gradients({&k, &v, &k_codes, &k_scales, &v_codes, &v_scales}, "store");
+  refuse_tangents({&k, &v, &k_codes, &k_scales, &v_codes, &v_scales}, "store");
   c10::cuda::CUDAGuard guard(k.device());
   pack::Args p{};
   pack::set_rows(p, k, v, k_codes, k_scales, v_codes, v_scales, table, kv_lens, cu_q, status);
@@ -394,6 +394,8 @@ std::pair<at::Tensor, at::Tensor> packed_read(const at::Tensor& k_codes, const a
                                               const at::Tensor& v_scales, const at::Tensor& table, const at::Tensor& starts,
                                               int64_t rows, at::ScalarType type, const c10::optional<at::Tensor>& status) {
   check_cuda_tensor(k_codes, "k_pages");
+  refuse_gradients({&k_codes, &k_scales, &v_codes, &v_scales}, "read");
+  refuse_tangents({&k_codes, &k_scales, &v_codes, &v_scales}, "read");
   RC_CHECK(type == at::kBFloat16 || type == at::kHalf, "packed pages are read as bf16 or fp16");
   RC_CHECK(k_codes.dim() == 4 && (k_codes.size(3) == 64 || k_codes.size(3) == 128), "packed pages have a head_dim of 64 or 128");
   c10::cuda::CUDAGuard guard(k_codes.device());

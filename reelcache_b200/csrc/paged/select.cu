@@ -811,6 +811,10 @@ void paged_block_means(const at::Tensor& k_pages, const c10::optional<at::Tensor
   check_cuda_tensor(k_pages, "k_pages");
   refuse_gradients({&k_pages, &means}, "block_means");
   refuse_tangents({&k_pages, &means}, "block_means");
+  if (k_scales.has_value()) {
+    refuse_gradients({&*k_scales}, "block_means");
+    refuse_tangents({&*k_scales}, "block_means");
+  }
   const at::ScalarType type = means.scalar_type();
   RC_CHECK(type == at::kBFloat16 || type == at::kHalf, "means are bf16 or fp16");
   RC_CHECK(k_pages.dim() == 4 && (k_pages.size(3) == 64 || k_pages.size(3) == 128), "pages must have a head_dim of 64 or 128");
