@@ -141,7 +141,8 @@ __global__ void __launch_bounds__(kMeanThreads) means_kernel(const __grid_consta
 
 constexpr int kSelectThreads = 256;
 constexpr int kSelectWarps = kSelectThreads / 32;
-constexpr int kMostBlocks = 12288;  // whose keys fit one CTA's shared memory
+constexpr int kMostBlocks = 12288;  // of a table: what a thread marks of its candidates is two words
+constexpr int kSelectBytes = 224 * 1024;  // of shared memory: 16 a block of the table, and 16 D + 260 a head of the group, about
 constexpr float kProductError = 0x1.6p-19f;
 constexpr int kBuckets = 256;       // one for each thread
 constexpr int kPieces = 3;          // 16-bit numbers that add up to a pooled query; a fourth row holds what bounds its errors
@@ -957,15 +958,18 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> paged_select_blocks(const at::Ten
   p.kv_lens = lens.data_ptr<int>();
   p.cu_q = cu.data_ptr<int>();
   const int device = q.get_device();
-  // CTAs of an item and KV head: as many as find room at once (three on an SM), with 128 blocks each
+  RC_CHECK(a.group <= 256, "too many heads in a group for the choice of blocks");  // (more never fit, and their bytes could wrap)
+  const int smem = q.size(2) == 128 ? paged::SelectShape<128>(a.group, static_cast<int>(held)).bytes : paged::SelectShape<64>(a.group, static_cast<int>(held)).bytes;
+  RC_CHECK(smem <= paged::kSelectBytes, "a group of " + std::to_string(a.group) + " heads with a block table of " + std::to_string(held) + " blocks needs " +
+                                            std::to_string(smem) + " bytes of shared memory for the choice of blocks, of which there are " +
+                                            std::to_string(paged::kSelectBytes) + ": take larger blocks, or fewer heads at a time");
+  // CTAs of an item and KV head: as many as find room at once (up to three on an SM), with 128 blocks each
+  const int resident = std::max(1, std::min(3, paged::kSelectBytes / smem));
   p.cluster = 1;
-  while (p.cluster < 8 && items * kv_heads * p.cluster * 2 <= 3 * sm_count(device) && held > 128 * p.cluster) {
+  while (p.cluster < 8 && items * kv_heads * p.cluster * 2 <= static_cast<int64_t>(resident) * sm_count(device) && held > 128 * p.cluster) {
     p.cluster *= 2;
     ++p.log_cluster;
   }
-  RC_CHECK(a.group <= 128, "too many heads in a group for the choice of blocks");
-  const int smem = q.size(2) == 128 ? paged::SelectShape<128>(a.group, static_cast<int>(held)).bytes : paged::SelectShape<64>(a.group, static_cast<int>(held)).bytes;
-  RC_CHECK(smem <= 224 * 1024, "too many heads in a group, or blocks in the table, for the choice of blocks: take larger blocks");
   cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device).stream();
   if (type == at::kHalf) q.size(2) == 128 ? paged::select_launch<__half, 128>(p, smem, stream, device) : paged::select_launch<__half, 64>(p, smem, stream, device);
   else q.size(2) == 128 ? paged::select_launch<__nv_bfloat16, 128>(p, smem, stream, device) : paged::select_launch<__nv_bfloat16, 64>(p, smem, stream, device);

@@ -188,7 +188,9 @@ def select_blocks(q, means, block_table, kv_lens, cu_q, *, block: int, keep: int
 
     A block's score is the largest over the heads of the group of the sum of the query block's ``q`` times the mean of the
     block's keys (``means`` from :func:`block_means`), in FP64: the choice does not depend on the order of sums. Equal scores go to the lower block; a
-    score of NaN comes last. Attention over the choice (its tables name the past in order, the query block's own tokens
+    score of NaN comes last. A table has at most 12,288 blocks (its width times the blocks of a page), fewer where groups are large:
+    16 bytes a block and about ``16 D + 260`` a head of a group must fit 224 KB (11 heads of 128 with 12,288 blocks, 88 with
+    1,024); other calls are refused. Attention over the choice (its tables name the past in order, the query block's own tokens
     last, so that ``causal`` holds there)::
 
         chosen = select_blocks(q, means, block_table, kv_lens, cu_q, block=64, keep=16, max_q_len=n, causal=True)

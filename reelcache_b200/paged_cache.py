@@ -90,7 +90,7 @@ class PagedKVCache:
     ``packed``: rows of ``dtype`` are held in 8 bits (:class:`~reelcache_b200.ops.paged.PackedPages`); ``storage`` has the codes, ``scales
     [layers, 2, kv_heads, pages, page_size]`` their scales. ``block`` (a divisor of the page size, a multiple of 8): ``means
     [layers, pages, page_size / block, kv_heads, head_dim]`` has the mean key of every ``block`` positions, kept up to date by
-    :meth:`append` and :meth:`store`, for attention over chosen blocks (a captured call brings them to what the sessions held when it
+    :meth:`append` and :meth:`store`, for attention over chosen blocks (of sessions of up to 12,288 blocks; a captured call brings them to what the sessions held when it
     was captured)."""
 
     def __init__(self, layers: int, kv_heads: int, head_dim: int, *, pages: int, page_size: int, max_sessions: int,
