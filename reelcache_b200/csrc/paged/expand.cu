@@ -4,8 +4,9 @@
 // codes into numbers once for every 256 rows; doing it once for each page of the call costs 5 bytes of traffic a number (1 read, 2 written, 2
 // read) next to hundreds of operations. Only pages that the call's queries see are expanded, each once however many sequences
 // and heads name it: a first kernel gives them places in the order in which it meets them (the place of a page depends on
-// timing, what is in it does not), a second one expands them and writes the table of places. Room is taken for as many pages as
-// the table has entries (or the pool pages). Measured: 4,680 tokens over 23,400 keys of 12 heads 667 us, 661 over 16-bit pages.
+// timing, what is in it does not), a second one expands them and writes the table of places. Room is taken before it is known which
+// those are: for as many pages as the table has entries, of which a window and its sinks leave a part, or as the pool has pages.
+// Measured: 4,680 tokens over 23,400 keys of 12 heads 667 us, 661 over 16-bit pages.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -21,7 +22,8 @@ namespace paged {
 
 constexpr int kExpandThreads = 256;
 constexpr int kExpandItems = 4;   // vectors of sixteen channels of a thread
-constexpr int kTileKeys = 128;    // of the attention that reads the places: what it touches of a window's edge
+constexpr int kTileKeys = 128;    // of the attention that reads the places: what it touches of a window's edge,
+constexpr int kTileRows = 256;    // and rows of an item of it: some may be of tokens beyond max_q_len
 
 struct Expand {
   Args a;
@@ -31,6 +33,7 @@ struct Expand {
   int* list;        // [places]: page of each place
   int* table;       // [seqs, table_heads, width]: places
   int places;
+  int reach;        // new tokens of a sequence that the attention takes, at most
   Packed pages[2];
   const uint8_t* codes[2];
   char* out[2];     // [places, page_size, kv_heads, head_dim]
@@ -50,12 +53,15 @@ __global__ void __launch_bounds__(kExpandThreads) place_kernel(const __grid_cons
     const int64_t from = static_cast<int64_t>(block) * a.tiling.page;
     if (q_len == 0 || from >= kv_len) continue;
     const Sight sight(a, kv_len, q_len);
-    const int low = sight.low(sight.last(0)) / kTileKeys * kTileKeys;
+    const int low = sight.low(sight.last(0)) / kTileKeys * kTileKeys, top = sight.last(min(q_len, p.reach) - 1);
+    if (top < 0) continue;
     const int64_t sinks = (static_cast<int64_t>(a.sinks) + kTileKeys - 1) / kTileKeys * kTileKeys;
-    if (from + a.tiling.page <= low && from >= sinks) continue;
+    const int64_t end = (static_cast<int64_t>(top) / kTileKeys + 1) * kTileKeys;
+    if ((from + a.tiling.page <= low || from >= end) && from >= sinks) continue;
     const int page = a.table[s * a.table_row + head * a.table_head + block];
     if (page < 0 || page >= a.pages || atomicCAS(p.place + page, -1, -2) != -1) continue;
     const int at = atomicAdd(p.count, 1) + 1;
+    if (at >= p.places) continue;  // (more than the room was reckoned for: never)
     p.list[at] = page;
     p.place[page] = at;
   }
@@ -71,7 +77,8 @@ __global__ void __launch_bounds__(kExpandThreads) expand_kernel(const __grid_con
     const int64_t row = c / a.width;
     const int64_t s = row / p.table_heads, head = row - s * p.table_heads;
     const int page = a.table[s * a.table_row + head * a.table_head + c - row * a.width];
-    p.table[c] = page >= 0 && page < a.pages ? p.place[page] : -1;
+    // (a page that nothing taken sees has no place: any does, since what reads it has no result)
+    p.table[c] = page >= 0 && page < a.pages ? max(p.place[page], 0) : -1;
   }
   const int places = min(p.places, *p.count + 1);
   const int per_token = a.kv_heads * p.vecs, per_page = a.tiling.page * per_token;
@@ -112,7 +119,15 @@ void expand_pages(Args& a, const at::Tensor& k_codes, const at::Tensor& v_codes,
   p.table_heads = a.table_head != 0 ? a.kv_heads : 1;
   const int64_t cells = static_cast<int64_t>(a.seqs) * p.table_heads * a.width;
   RC_CHECK(cells < (1ll << 31), "too many sequences and blocks for packed pages");
-  p.places = static_cast<int>(std::min<int64_t>(a.pages, std::max<int64_t>(cells, 1)));
+  const int64_t rows = static_cast<int64_t>(std::min(a.max_q_len, a.tokens)) * a.group;
+  p.reach = static_cast<int>(((rows + kTileRows - 1) / kTileRows * kTileRows + a.group - 1) / a.group);
+  int64_t seen = a.width;  // pages of a table's row that the queries see, at most: those of the sinks' tiles, and of the window's
+  if (a.window > 0) {
+    const auto pages_of = [&](int64_t keys) { return (keys + a.tiling.page - 2) / a.tiling.page + 1; };
+    seen = std::min(seen, (a.sinks > 0 ? pages_of(static_cast<int64_t>(a.sinks) + kTileKeys) : 0) +
+                              pages_of(static_cast<int64_t>(a.window) + p.reach + 2 * kTileKeys));
+  }
+  p.places = static_cast<int>(std::min<int64_t>(a.pages, std::max<int64_t>(seen * a.seqs * p.table_heads, 1)));
   const int64_t d = like.size(2), per_page = static_cast<int64_t>(a.tiling.page) * a.kv_heads * (d / 16);
   RC_CHECK(per_page < (1ll << 30), "a packed page is too large");
   k_pages = at::empty({p.places, a.tiling.page, a.kv_heads, d}, like.options());
