@@ -193,9 +193,7 @@ void pack_launch(Args p, cudaStream_t stream, int sms) {
   const int groups = p.a.q.groups + p.a.k.groups + p.a.v.groups;
   RC_CHECK(blocks < (1ll << 31) && groups < 65536, "too many tokens or heads for one launch");
   const dim3 grid(static_cast<unsigned>(blocks), groups);
-  if (widest == 1) paged::launch(pack_kernel<T, kTurn, 1>, grid, kThreads, 0, 0, stream, p);
-  else if (widest == 2) paged::launch(pack_kernel<T, kTurn, 2>, grid, kThreads, 0, 0, stream, p);
-  else paged::launch(pack_kernel<T, kTurn, 2>, grid, kThreads, 0, 0, stream, p);
+  paged::launch(widest == 1 ? pack_kernel<T, kTurn, 1> : pack_kernel<T, kTurn, 2>, grid, kThreads, 0, 0, stream, p);
 }
 
 template <int kTurn>

@@ -324,18 +324,6 @@ __device__ __forceinline__ float keep_th(const float* scores, int n, int keep, f
 struct Operand {
   uint32_t x[4];
 };
-__device__ __forceinline__ void mma_means(float (&d)[4], const Operand& a, uint32_t b0, uint32_t b1, __nv_bfloat16) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a.x[0]), "r"(a.x[1]), "r"(a.x[2]), "r"(a.x[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma_means(float (&d)[4], const Operand& a, uint32_t b0, uint32_t b1, __half) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a.x[0]), "r"(a.x[1]), "r"(a.x[2]), "r"(a.x[3]), "r"(b0), "r"(b1));
-}
 
 __device__ __forceinline__ float value_of(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float value_of(__half x) { return __half2float(x); }
@@ -589,8 +577,8 @@ __global__ void __launch_bounds__(kSelectThreads, 3) select_kernel(const __grid_
 #pragma unroll
           for (int j = 0; j < D / 32; ++j) {
             const uint4 b = *reinterpret_cast<const uint4*>(piece + k * SelectShape<D>::piece_row + j * 64);
-            mma_means(sc, Operand{mean[0][j].x, mean[1][j].x, mean[0][j].y, mean[1][j].y}, b.x, b.y, T());
-            mma_means(sc, Operand{mean[0][j].z, mean[1][j].z, mean[0][j].w, mean[1][j].w}, b.z, b.w, T());
+            mma_16816(sc, Operand{mean[0][j].x, mean[1][j].x, mean[0][j].y, mean[1][j].y}.x, b.x, b.y, T());
+            mma_16816(sc, Operand{mean[0][j].z, mean[1][j].z, mean[0][j].w, mean[1][j].w}.x, b.z, b.w, T());
           }
         }
 #pragma unroll
@@ -598,10 +586,10 @@ __global__ void __launch_bounds__(kSelectThreads, 3) select_kernel(const __grid_
           constexpr uint32_t kSize = 0x7fff7fffu;
           const uint4 b = *reinterpret_cast<const uint4*>(piece + j * 64), y = *reinterpret_cast<const uint4*>(piece + kPieces * SelectShape<D>::piece_row + j * 64);
           float one[4] = {}, two[4] = {};
-          mma_means(one, Operand{mean[0][j].x, mean[1][j].x, mean[0][j].y, mean[1][j].y}, b.x, b.y, T());
-          mma_means(two, Operand{mean[0][j].z, mean[1][j].z, mean[0][j].w, mean[1][j].w}, b.z, b.w, T());
-          mma_means(size, Operand{mean[0][j].x & kSize, mean[1][j].x & kSize, mean[0][j].y & kSize, mean[1][j].y & kSize}, y.x, y.y, T());
-          mma_means(size, Operand{mean[0][j].z & kSize, mean[1][j].z & kSize, mean[0][j].w & kSize, mean[1][j].w & kSize}, y.z, y.w, T());
+          mma_16816(one, Operand{mean[0][j].x, mean[1][j].x, mean[0][j].y, mean[1][j].y}.x, b.x, b.y, T());
+          mma_16816(two, Operand{mean[0][j].z, mean[1][j].z, mean[0][j].w, mean[1][j].w}.x, b.z, b.w, T());
+          mma_16816(size, Operand{mean[0][j].x & kSize, mean[1][j].x & kSize, mean[0][j].y & kSize, mean[1][j].y & kSize}.x, y.x, y.y, T());
+          mma_16816(size, Operand{mean[0][j].z & kSize, mean[1][j].z & kSize, mean[0][j].w & kSize, mean[1][j].w & kSize}.x, y.z, y.w, T());
 #pragma unroll
           for (int e = 0; e < 4; ++e) sc[e] += one[e] + two[e];
         }
