@@ -186,8 +186,10 @@ def select_blocks(q, means, block_table, kv_lens, cu_q, *, block: int, keep: int
                   causal: bool = False, sinks: int = 0, recent: int = 0) -> ChosenBlocks:
     """Choose the blocks of ``block`` positions that the new tokens ``q[T, heads, D]`` attend to, for every ``query_block`` of them
     (consecutive tokens of a sequence; 1: each its own) and KV head: the ``keep`` blocks of the past that score highest, and always those that
-    hold the first ``sinks`` positions, the ``recent`` positions before the new tokens, and the new tokens (``causal``: before and up
-    to those of the query block).
+    hold the first ``sinks`` positions, the ``recent`` positions before the new tokens, and the new tokens; with ``causal`` the
+    ``recent`` positions before the query block, and the query block (new tokens before those are past like any). The tokens of a query block share a choice that all of their queries make: ``causal`` keeps each
+    from seeing later positions, but which blocks of the past it sees depends on the queries of the tokens after it in its query block.
+    A prompt read in query blocks is thus not the same as its tokens one by one (``query_block=1`` is).
 
     A block's score is the largest over the heads of the group of the sum of the query block's ``q`` times the mean of the
     block's keys (``means`` from :func:`block_means`), in FP64: the choice does not depend on the order of sums. Equal scores go to the lower block; a

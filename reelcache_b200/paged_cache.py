@@ -347,7 +347,8 @@ class PagedKVCache:
                recent: int = 0):
         """Attention of the new tokens over their sessions (:func:`reelcache_b200.ops.paged.attention`), or with ``keep`` over
         the ``keep`` blocks of their past that score highest for every ``query_block`` of them, besides the first ``sinks`` and the
-        last ``recent`` positions and the new tokens (:func:`reelcache_b200.ops.paged.select_blocks`)."""
+        last ``recent`` positions and the new tokens (:func:`reelcache_b200.ops.paged.select_blocks`). The tokens of a query block
+        share a choice that all of them make, ``causal`` or not."""
         self._check_batch(batch, q, write=False)
         self._check_type(q)
         k, v = self.layer_pages(layer)

@@ -43,3 +43,19 @@ def test_larger_ones_are_refused(heads, d, blocks, what):
     from reelcache_b200.ops import paged
     with pytest.raises(RuntimeError, match=what):
         paged.select_blocks(**_call(heads, d, blocks))
+
+
+def test_a_query_block_chooses_as_one():
+    """Causal or not, all tokens of a query block make its choice: the first one's blocks follow the last one's query; with a query
+    block for each token they do not."""
+    from reelcache_b200.ops import paged
+    call = {**_call(2, 64, 64, 4), "keep": 1}
+    q = call.pop("q")
+    other = q.clone()
+    best = call["means"][int(call["block_table"][0, 5]), 3, 0]  # block 43
+    other[3] = 1000.0 * best  # the last of the first sequence's tokens
+    first, changed = (paged.select_blocks(x, **call).table for x in (q, other))
+    assert first.shape[0] == changed.shape[0] == 2 and int(changed[0, 0, 0]) == int(call["block_table"][0, 5]) * 8 + 3
+    assert not torch.equal(first[0], changed[0]) and torch.equal(first[1], changed[1])
+    alone, after = (paged.select_blocks(x, **{**call, "query_block": 1}).table for x in (q, other))
+    assert torch.equal(alone[:3], after[:3]) and not torch.equal(alone[3], after[3])
