@@ -20,7 +20,9 @@ namespace paged {
 
 constexpr int kShortRows = 16;
 // Packed pages: slices of 16 rows side by side, which read the same codes through L2, while that is less than expanding them first
-// (16 sessions over 4,096 keys, 32 / 8 heads: 20 to 32 rows 75 us, 48 rows 107, 64 rows 136; expanded 124).
+// (16 sessions over 4,096 keys, 32 / 8 heads, pages of 64: 32 rows 81 us, 48 rows 116, expanded 127). One number for all
+// calls: slices cost conversions for every session and key, expansion for every page that differs; for 64 sessions over 1,024
+// keys of pages of 16 48 rows take 158 and 64, expanded, 167, for one over 32,768 keys 81 and 101.
 constexpr int kPackedRows = 48;
 
 void attend_short(const Args& a, int head_dim, bool half, const at::Tensor& k_pages, const at::Tensor& v_pages,

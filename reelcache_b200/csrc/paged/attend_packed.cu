@@ -24,7 +24,7 @@
 //
 // More than 16 rows are slices of 16, each an item of its own next to the others of its head.
 //
-// Measured: 48 sessions of up to 16,384 keys (32 / 8 heads, 0.84 GB) 151 to 164 us, 5.1 to 5.6 TB/s (282 with the queries in the
+// Measured: 48 sessions of up to 16,384 keys (32 / 8 heads, 0.84 GB) 161 to 168 us, 5.0 to 5.2 TB/s (282 with the queries in the
 // rows of the product; 232 with spinning waits and copies that prefetch 256 bytes, of which a head's rows have 128; 163 head after
 // head instead of side by side); three CTAs on an SM and four are alike. One session over 2,048 keys 8 us clustered, a call 9.
 #include <ATen/ATen.h>

@@ -8,7 +8,7 @@
 // many heads as leave every SM full, so that its sines are computed once.
 //
 // What bounds it: memory (3 bytes a number of k and v, 4 of q), and the chain of a row: load, turn, maximum over the row's lanes,
-// codes. Three chunks of 4,680 tokens and 12 heads 46.3 us, 4.7 TB/s (41.2 with sines of FP32 alone); 25.8 us without q and the
+// codes. Three chunks of 4,680 tokens and 12 heads 46.1 us, 4.7 TB/s (41.2 with sines of FP32 alone); 25.8 us without q and the
 // rotation (129 MB, 5.0 TB/s).
 //
 // Out of pages: a block looks up where its rows lie, then every thread turns vectors of sixteen codes into 32 bytes, a whole
@@ -108,8 +108,8 @@ __global__ void __launch_bounds__(kThreads, kTurn == 2 ? 2 : kTurn == 1 ? 4 : 5)
   }
 
   // A code that falls to its neighbour is 2^-3 off, so k is turned nearer than FP32's sines allow: by sines of FP64 as the sums of
-  // two numbers, computed once for all of the thread's heads. What is left are two roundings, 2^-24 each (18 of 21.6 million
-  // codes are not the exact rotation's; over 100 with FP32 throughout).
+  // two numbers, computed once for all of the thread's heads. What is left are two roundings, 2^-24 each (14 to
+  // 22 of 21.6 million codes are not the exact rotation's).
   float cs[kPairs] = {}, sn[kPairs] = {}, cs_low[kPairs] = {}, sn_low[kPairs] = {};
   const bool turned = kTurn != 0 && (is_q || is_k);
   if (turned && active && is_q) rotary::sines<false>(a, token, vec, cs, sn);

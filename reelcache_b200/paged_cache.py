@@ -91,7 +91,7 @@ class PagedKVCache:
     [layers, 2, kv_heads, pages, page_size]`` their scales. ``block`` (a divisor of the page size, a multiple of 8): ``means
     [layers, pages, page_size / block, kv_heads, head_dim]`` has the mean key of every ``block`` positions, kept up to date by
     :meth:`append` and :meth:`store`, for attention over chosen blocks (of sessions of up to 12,288 blocks; a captured call brings them to what the sessions held when it
-    was captured)."""
+    was captured; a fork's partly filled last block has its own once it is written)."""
 
     def __init__(self, layers: int, kv_heads: int, head_dim: int, *, pages: int, page_size: int, max_sessions: int,
                  max_tokens: int, device="cuda", dtype=torch.bfloat16, packed: bool = False, block: int | None = None):
