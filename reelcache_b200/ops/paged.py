@@ -116,7 +116,8 @@ def attention(q, k_pages, v_pages, block_table, kv_lens, cu_q, *, max_q_len: int
     ``block_table`` may be ``[seqs, kv_heads, width]``, a table for each KV head. Packed pages give what their rows read as
     :func:`read` gives, in ``q``'s type, which must be the one that the rows were written from (fp16 does not hold what bf16's
     range of scales does). With up to 48 rows (new tokens x heads of a group) the codes are taken as they are and the
-    probabilities times V's scales are rounded to fp16 (a key's by half a step, or by 2^-32 of the largest where that is more).
+    probabilities times V's scales are rounded to fp16 (a key's by half a step, or by 2^-32 of the largest where that is more);
+    channels of ``q`` below 2^-20 of their row's largest are off by up to 2^-31 of that.
     With more, the pages that are seen are expanded first: 16-bit copies of them for the time of the call, in room for as many
     pages as the table has entries, or a window leaves of them, or the pool has; in a batch with one long prompt among single
     tokens, of all its sequences."""

@@ -72,6 +72,7 @@ class PagedBatch:
     cache: "PagedKVCache" = field(repr=False, compare=False)
     made: int = field(repr=False, compare=False)  # the cache's change before it
     checked: list = field(repr=False, compare=False)  # [the change after which it was last found good to write]
+    grown: int = field(default=0, repr=False, compare=False)  # the cache's extensions, with its own
 
     @property
     def tokens(self) -> int:
@@ -131,6 +132,7 @@ class PagedKVCache:
         self._free_slots = list(range(max_sessions))[::-1]
         self._held = 0
         self._changes = self._compacted = 0  # forks, ends and compactions so far; which of them was the last compaction
+        self._grown = 0  # extensions so far
 
     # -- sessions --------------------------------------------------------------------------------------------------------
 
@@ -228,6 +230,7 @@ class PagedKVCache:
                 raise CapacityError(f"a session of {s.length} tokens cannot take {n} more (at most {self.max_tokens})")
         blocks = [-(-(s.length + n) // self.page_size) - len(s.blocks) for s, n in pairs]
         self._admit(sum(blocks))
+        self._grown += 1
         batch, slots = self._batch(sessions, [n for _, n in pairs], [s.length + n for s, n in pairs])
         self.table.allocate(slots, batch.kv_lens)
         for (s, n), b in zip(pairs, blocks):
@@ -256,7 +259,7 @@ class PagedKVCache:
             starts.append(starts[-1] + n)
         table = torch.empty(len(sessions), width, dtype=torch.int32, device=self.device)
         return PagedBatch(tuple(sessions), tuple(counts), tuple(lengths), table, self._ints(lengths), self._ints(starts), self,
-                          self._changes, [self._changes]), self._ints(s.slot for s in sessions)
+                          self._changes, [self._changes], self._grown), self._ints(s.slot for s in sessions)
 
     def _name_pages(self, batch: PagedBatch, slots: torch.Tensor) -> PagedBatch:
         torch.index_select(self.table.block_table[:, :batch.table.shape[1]], 0, slots, out=batch.table)
@@ -332,7 +335,7 @@ class PagedKVCache:
         if self.block is None or not batch.tokens:
             return
         table, kv_lens, cu_q, longest = batch.table, batch.kv_lens, batch.cu_q, max(batch.counts)
-        if any(s.length != n for s, n in zip(batch.sessions, batch.lengths)):
+        if batch.grown != self._grown and any(s.length != n for s, n in zip(batch.sessions, batch.lengths)):
             # a block's mean is that of what its session holds by now: the batch's new tokens and all that came after
             # them (by kernels that take the numbers as arguments: a capture must not keep copies from host memory)
             width = -(-max(s.length for s in batch.sessions) // self.page_size)

@@ -145,3 +145,38 @@ def test_scores_that_rise_while_sizes_fall(new, totals, heads, kv_heads, rise):
             k[at, :, :, 0] = ((step - step.amax()) * rise).clamp(min=-200.0)
             v[at] *= torch.exp2(-step / 40.0)[..., None]
     _check(new, totals, heads, kv_heads, 64, BF16, change)
+
+
+@pytest.mark.parametrize("new,totals,heads,kv_heads", FORMS)
+def test_infinite_scores(new, totals, heads, kv_heads):
+    """A score of plus infinity makes the log-sum-exp plus infinity and the output NaN; of minus infinity a key that counts for nothing."""
+    from reelcache_b200.ops import paged
+    g = torch.Generator(device="cuda").manual_seed(len(new))
+    k, v, table, kv_lens, cu_q = paged_batch(g, new, totals, kv_heads, 64, 16, torch.float32)
+    k[..., 0] = 0.0
+    at = table[:, 0].long()
+    k[at, 3, :, 0] = -4.0e4 * 64
+    q = torch.zeros(sum(new), heads, 64, device="cuda", dtype=BF16)
+    packed = [pack_pages(x, BF16) for x in (k, v)]
+    below = q.clone()
+    below[..., 0] = 2.0 ** 120
+    above = q.clone()
+    above[..., 0] = -(2.0 ** 120)
+    call = lambda x: paged.attention(x, *packed, table, kv_lens, cu_q, max_q_len=max(new), causal=True, return_lse=True)  # noqa: E731
+    out, lse = call(above)
+    assert bool(out.isnan().all()) and bool((lse == math.inf).all())
+    # every key but the one of minus infinity scores zero
+    out, lse = call(below)
+    values = held(packed[1], BF16).double()
+    first = 0
+    for s, n in enumerate(new):
+        total = totals[s]
+        rows = values[table[s][:-(-total // 16)].long()].flatten(0, 1)[:total]
+        for i in range(n):
+            seen = [p for p in range(total - n + i + 1) if p != 3]
+            want = rows[seen].mean(dim=0).repeat_interleave(heads // kv_heads, dim=0)
+            size = rows[seen].abs().mean(dim=0).repeat_interleave(heads // kv_heads, dim=0)
+            # equal weights, a power of two times V's scales: exact in fp16; sums in FP32 and one rounding
+            assert within(out[first + i], want, want.abs() * 2.0 ** -8 + size * (len(seen) + 8) * 2.0 ** -22)
+            assert within(lse[first + i], torch.full_like(lse[first + i], math.log(len(seen))).double(), torch.full_like(lse[first + i], 2.0 ** -18).double())
+        first += n
